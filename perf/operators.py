@@ -381,7 +381,9 @@ def prepare(case, seed):
                               slopes_ptr=ptr(s["slopes"]), positions_ptr=s["pos"].data_ptr())
     if c["kind"] == "step":
         s["qrot"] = torch.empty_like(s["q"])
-        s["qt"] = fa.rotary_tensor(c["heads"], _strides(s["q"]), _strides(s["qrot"]))
+        s["append"] = fa.append_config(c["n"], rotary=s["rot"], k_strides=_strides(s["knew"]),
+                                       v_strides=_strides(s["vnew"]),
+                                       q_layout=fa.rotary_tensor(c["heads"], _strides(s["q"]), _strides(s["qrot"])))
     return s
 
 
@@ -421,10 +423,8 @@ def _run_own(s):
         fa.tree_attention_device(s["cfg"], s["cache"], s["q"].data_ptr(), s["out"].data_ptr(), stream=stream)
         return {"out": s["out"]}
     pos = s["pos"].data_ptr()
-    fa.rotary_device(s["rot"], c["batch"], c["n"], pos, s["qt"], s["q"].data_ptr(), s["qrot"].data_ptr(),
-                     stream=stream)
-    fa.cache_append_device(s["cache"], c["n"], s["knew"].data_ptr(), s["vnew"].data_ptr(), rotary=s["rot"],
-                           positions_ptr=pos, stream=stream)
+    fa.cache_append_device(s["cache"], s["append"], s["knew"].data_ptr(), s["vnew"].data_ptr(), pos,
+                           s["q"].data_ptr(), s["qrot"].data_ptr(), stream=stream)
     fa.tree_attention_device(s["cfg"], s["cache"], s["qrot"].data_ptr(), s["out"].data_ptr(), stream=stream)
     return {"out": s["out"], "k": s["kcache"], "v": s["vcache"]}
 
