@@ -1,7 +1,10 @@
 """Build the MI355X library in-tree.
 
 Outputs, next to this file (git-ignored, used in place):
-  fa_kernels.hsaco  gfx950 code object with every kernel (hipcc --genco)
+  fa_kernels.hsaco  gfx950 code object with the attention kernels (hipcc --genco)
+  fa_score.hsaco, fa_cache.hsaco, fa_rotary.hsaco
+                    code objects of attention with modified scores, of the
+                    key / value cache and of rotary positions
   libfa_hip.so      C ABI of include/fa_hip.h over the HIP runtime
 
 Run as ``python flash-attention-cpu_amd/build.py`` or via
@@ -13,6 +16,7 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -20,6 +24,7 @@ CSRC = os.path.join(HERE, "csrc")
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 
 HSACO = os.path.join(HERE, "fa_kernels.hsaco")
+OPS = ("fa_score", "fa_cache", "fa_rotary")   # code objects of the operators, one a source file
 LIB = os.path.join(HERE, "libfa_hip.so")
 BUILD = os.path.join(HERE, "_build")   # intermediate objects (git-ignored)
 
@@ -35,9 +40,17 @@ def _run(cmd: list[str]) -> None:
     subprocess.run(cmd, check=True)
 
 
-def build_kernels() -> str:
+def _genco(name: str) -> str:
+    out = os.path.join(HERE, name + ".hsaco")
     _run([os.path.join(ROCM, "bin", "hipcc"), *HIP_FLAGS, "--genco",
-          os.path.join(CSRC, "fa_kernels.hip"), "-o", HSACO])
+          os.path.join(CSRC, name + ".hip"), "-o", out])
+    return out
+
+
+def build_kernels() -> str:
+    """Every code object, compiled at the same time."""
+    with ThreadPoolExecutor(max_workers=1 + len(OPS)) as pool:
+        list(pool.map(_genco, ("fa_kernels", *OPS)))
     return HSACO
 
 

@@ -89,6 +89,9 @@ struct DeviceState {
         void* ptr = nullptr;
         size_t bytes = 0;
         std::vector<void*> retired;   // outgrown buffers: kept, a captured graph may name them
+        void* cap_ptr = nullptr;      // the buffer that the capture cap_id took over (one of the retired)
+        size_t cap_bytes = 0;
+        unsigned long long cap_id = 0;
     };
     std::mutex ws_mu;
     std::unordered_map<std::string, Workspace> ws;   // freed by fa_release_stream_workspace
@@ -183,6 +186,8 @@ CopyPool& copy_pool() {
 }
 
 DeviceState g_dev[kMaxDevices];
+
+void ops_init(int dev);   // fa_ops_host.h
 
 std::string module_path() {
     const char* env = std::getenv("FA_HIP_MODULE");
@@ -1018,7 +1023,8 @@ size_t free_device_bytes() {
 
 //
 // A call captured into a graph takes the buffer over: it moves to the
-// stream's retired list (kept until fa_release_stream_workspace), and the
+// stream's retired list (kept until fa_release_stream_workspace), later calls
+// of the same capture, which run after it, use it too, and the
 // next eager call on the stream gets a new one.  So replays of the graph --
 // on any stream -- never share partials with later eager calls on the
 // capture stream, nor with another graph captured there.
@@ -1026,7 +1032,8 @@ int stream_workspace(int dev, hipStream_t stream, size_t bytes, void** out) {
     DeviceState& s = g_dev[dev];
     const std::string key = workspace_key(stream);
     hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
-    if (hipStreamIsCapturing(stream, &cap) != hipSuccess) {
+    unsigned long long id = 0;
+    if (hipStreamGetCaptureInfo(stream, &cap, &id) != hipSuccess) {
         (void)hipGetLastError();
         cap = hipStreamCaptureStatusNone;
     }
@@ -1034,16 +1041,31 @@ int stream_workspace(int dev, hipStream_t stream, size_t bytes, void** out) {
     std::lock_guard<std::mutex> lock(s.ws_mu);
     DeviceState::Workspace& w = s.ws[key];
     if (capturing) {
+        if (w.cap_ptr && w.cap_id == id && w.cap_bytes >= bytes) {   // a later call of the same capture
+            *out = w.cap_ptr;
+            return FA_OK;
+        }
         void* ptr = nullptr;
         if (w.ptr && w.bytes >= bytes) {
             ptr = w.ptr;
+            w.cap_bytes = w.bytes;
             w.ptr = nullptr;
             w.bytes = 0;
-        } else if (hipMalloc(&ptr, bytes) != hipSuccess) {
-            (void)hipGetLastError();
-            return FA_ERR_ALLOC;
+        } else {
+            // not a stream operation: allowed here whatever the capture's mode
+            hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+            const bool relaxed = hipThreadExchangeStreamCaptureMode(&mode) == hipSuccess;
+            const hipError_t err = hipMalloc(&ptr, bytes);
+            if (relaxed) (void)hipThreadExchangeStreamCaptureMode(&mode);
+            if (err != hipSuccess) {
+                (void)hipGetLastError();
+                return FA_ERR_ALLOC;
+            }
+            w.cap_bytes = bytes;
         }
         w.retired.push_back(ptr);
+        w.cap_ptr = ptr;
+        w.cap_id = id;
         *out = ptr;
         return FA_OK;
     }
@@ -1456,9 +1478,11 @@ fa_config fa_config_default(void) {
 
 int fa_init(void) {
     int dev;
-    const int rc = current_device(&dev);
+    int rc = current_device(&dev);
     if (rc != FA_OK) return rc;
-    return ensure_loaded(dev);
+    rc = ensure_loaded(dev);
+    if (rc == FA_OK) ops_init(dev);   // a missing operator module concerns only its entry points
+    return rc;
 }
 
 int fa_v1(const float* q, size_t q_len, const float* k, size_t k_len, const float* v, size_t v_len, size_t sq,
@@ -1714,3 +1738,5 @@ int fa_probe_launch(int kind, void* stream, void* buf, size_t bytes, unsigned it
 }
 
 }  // extern "C"
+
+#include "fa_ops_host.h"

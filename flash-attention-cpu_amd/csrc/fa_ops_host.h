@@ -1,0 +1,656 @@
+// fa_ops_host.h -- host side of attention with modified scores, rotary
+// positions and the key / value cache (included by fa_host.cpp, whose device
+// state and stream workspaces it uses).
+//
+// Their kernels are code objects of their own next to fa_kernels.hsaco, loaded
+// on first use (or by fa_init).  Every argument is checked before anything is queued.
+
+#include "fa_ops_params.h"
+
+namespace {
+
+enum OpsModule { kScoreModule, kCacheModule, kRotaryModule, kOpsModules };
+
+struct OpsState {
+    std::once_flag once[kOpsModules];
+    int status[kOpsModules] = {};
+    hipModule_t module[kOpsModules] = {};
+    std::mutex mu;
+    std::unordered_map<std::string, hipFunction_t> fns;
+};
+
+OpsState g_ops[kMaxDevices];
+
+constexpr size_t kOpsMaxSeq = size_t(1) << 30;      // tokens: positions and their sums stay in 32 bits
+constexpr size_t kOpsMaxD = 256;
+constexpr int64_t kOpsMaxRowStride = int64_t(1) << 23;   // elements: a tile's byte offsets stay in 32 bits
+constexpr int64_t kOpsMaxStride = int64_t(1) << 44;
+constexpr size_t kTreeMaxTokens = 256;
+
+int ops_module(int dev, OpsModule which) {
+    static const char* const files[] = {"fa_score.hsaco", "fa_cache.hsaco", "fa_rotary.hsaco"};
+    OpsState& s = g_ops[dev];
+    std::call_once(s.once[which], [&] {
+        std::string path = module_path();
+        const size_t pos = path.rfind('/');
+        path = (pos == std::string::npos ? std::string() : path.substr(0, pos + 1)) + files[which];
+        FILE* f = std::fopen(path.c_str(), "rb");
+        if (f) std::fclose(f);
+        if (!f || hipModuleLoad(&s.module[which], path.c_str()) != hipSuccess) {
+            (void)hipGetLastError();
+            s.status[which] = FA_ERR_MODULE;
+        }
+    });
+    return s.status[which];
+}
+
+void ops_init(int dev) {
+    for (int m = 0; m < kOpsModules; ++m) (void)ops_module(dev, static_cast<OpsModule>(m));
+}
+
+template <typename P>
+int ops_launch(int dev, OpsModule which, const char* name, size_t grid, unsigned block, P* p, hipStream_t stream) {
+    if (grid == 0) return FA_OK;
+    OpsState& s = g_ops[dev];
+    hipFunction_t fn = nullptr;
+    {
+        std::lock_guard<std::mutex> lock(s.mu);
+        auto it = s.fns.find(name);
+        if (it != s.fns.end()) {
+            fn = it->second;
+        } else {
+            if (hipModuleGetFunction(&fn, s.module[which], name) != hipSuccess) {
+                (void)hipGetLastError();
+                return FA_ERR_MODULE;
+            }
+            s.fns.emplace(name, fn);
+        }
+    }
+    void* args[] = {p};
+    if (hipModuleLaunchKernel(fn, static_cast<unsigned>(grid), 1, 1, block, 1, 1, 0, stream, args, nullptr) !=
+        hipSuccess) {
+        (void)hipGetLastError();
+        return FA_ERR_LAUNCH;
+    }
+    return FA_OK;
+}
+
+// Device and module of a call; *dev is the current device.
+int ops_begin(int* dev, OpsModule which) {
+    int rc = current_device(dev);
+    if (rc == FA_OK) rc = ensure_loaded(*dev);
+    if (rc == FA_OK) rc = ops_module(*dev, which);
+    return rc;
+}
+
+// A call's scratch memory: the stream's workspace, or an allocation around the call above its limit.
+struct OpsWorkspace {
+    void* ptr = nullptr;
+    bool own = false;
+    int get(int dev, hipStream_t stream, size_t bytes) {
+        if (bytes <= kWorkspaceCacheMax) return stream_workspace(dev, stream, bytes, &ptr);
+        if (bytes > free_device_bytes() || hipMallocAsync(&ptr, bytes, stream) != hipSuccess) {
+            (void)hipGetLastError();
+            return FA_ERR_ALLOC;
+        }
+        own = true;
+        return FA_OK;
+    }
+    int done(hipStream_t stream, int rc) {
+        if (own && hipFreeAsync(ptr, stream) != hipSuccess) {
+            (void)hipGetLastError();
+            if (rc == FA_OK) rc = FA_ERR_ALLOC;
+        }
+        return rc;
+    }
+};
+
+size_t elem_size(int dtype) { return dtype == FA_DTYPE_F32 ? 4 : 2; }
+const char* dtype_name(int dtype) { return dtype == FA_DTYPE_F32 ? "f32" : dtype == FA_DTYPE_BF16 ? "bf16" : "f16"; }
+bool valid_dtype(int dtype) { return dtype == FA_DTYPE_F32 || dtype == FA_DTYPE_BF16 || dtype == FA_DTYPE_F16; }
+int ops_pad_d(size_t d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
+
+// A tensor's layout: strides resolved, and what they allow.
+struct OpsLayout {
+    OpsStrides st{};
+    bool aligned16 = true;   // rows start 16-byte aligned (given the pointer)
+    bool aligned4 = true;    // rows start at multiples of 4 elements
+};
+
+int resolve_layout(const fa_strides& in, size_t batch, size_t seq, size_t heads, size_t d, size_t esize, bool writable,
+                   OpsLayout* out) {
+    int64_t b = in.batch, s = in.seq, h = in.head;
+    if (b < 0 || s < 0 || h < 0) return FA_ERR_INVALID_ARG;
+    if (b > kOpsMaxStride || h > kOpsMaxStride || s >= kOpsMaxRowStride) return FA_ERR_UNSUPPORTED;
+    const int64_t row = static_cast<int64_t>(d);
+    if (b == 0 && s == 0 && h == 0) {
+        s = row;
+        h = static_cast<int64_t>(seq) * row;
+        b = static_cast<int64_t>(heads) * h;
+    }
+    // strides of single entries are never used
+    if (seq <= 1) s = row;
+    if (heads <= 1) h = 0;
+    if (batch <= 1) b = 0;
+    if (s < row) return FA_ERR_INVALID_ARG;
+    if (writable) {
+        // no two rows overlap: each dimension steps over all of the smaller ones
+        struct Dim {
+            int64_t stride;
+            size_t n;
+        } dims[3] = {{b, batch}, {s, seq}, {h, heads}};
+        std::sort(dims, dims + 3, [](const Dim& x, const Dim& y) { return x.stride < y.stride; });
+        int64_t extent = row;
+        for (const Dim& x : dims) {
+            if (x.n <= 1) continue;
+            if (x.stride < extent) return FA_ERR_INVALID_ARG;
+            extent = x.stride * static_cast<int64_t>(x.n);
+        }
+    }
+    out->st = {b, s, h};
+    const int64_t unit = static_cast<int64_t>(16 / esize);
+    out->aligned16 = b % unit == 0 && s % unit == 0 && h % unit == 0 && row % unit == 0;
+    out->aligned4 = b % 4 == 0 && s % 4 == 0 && h % 4 == 0;
+    return FA_OK;
+}
+
+// 16-byte loads of 8-column chunks / stores of 4 columns.
+bool vec_ok(const void* ptr, const OpsLayout& l, size_t d) { return l.aligned16 && d % 8 == 0 && aligned16(ptr); }
+bool ovec_ok(const void* ptr, const OpsLayout& l, size_t esize) {
+    return l.aligned4 && (reinterpret_cast<uintptr_t>(ptr) & (4 * esize - 1)) == 0;
+}
+
+struct ScoreScale {
+    float scale, scale_log2e, cap_in, cap_log2e;
+};
+int resolve_scale(float scale, float softcap, size_t d, ScoreScale* out) {
+    if (!(softcap >= 0.0f) || !std::isfinite(softcap)) return FA_ERR_INVALID_ARG;
+    if (!(scale > 0.0f) || !std::isfinite(scale)) scale = 1.0f / std::sqrt(static_cast<float>(d));
+    constexpr float log2e = 1.44269504088896341f;
+    out->scale = scale;
+    out->scale_log2e = scale * log2e;
+    out->cap_in = softcap > 0.0f ? 2.0f * log2e * scale / softcap : 0.0f;
+    out->cap_log2e = softcap * log2e;
+    return FA_OK;
+}
+
+// Query rows of a workgroup of the forward and dQ kernels, threads of theirs.
+struct ScoreGeo {
+    int rows, threads;
+};
+ScoreGeo score_geo(int dtype, int D) {
+    const bool wide = dtype == FA_DTYPE_F32 || D > 128;
+    return wide ? ScoreGeo{128, 512} : ScoreGeo{128, 256};
+}
+constexpr int kDkvRows = 128, kDkvThreads = 512;
+constexpr size_t kOpsMaxGrid = size_t(1) << 22;   // workgroups: threads of a launch stay in 32 bits
+
+size_t doc_tiles(size_t n) { return (n + kDocTile - 1) / kDocTile; }
+
+// Fewest-row plan: key splits of the rows kernel.
+struct RowsPlan {
+    int mt, nw, nrb, splits;
+    size_t floats;
+};
+RowsPlan plan_rows(int dtype, int D, size_t nkv, size_t rows, size_t keys, int num_cus) {
+    RowsPlan r{};
+    const bool f32 = dtype == FA_DTYPE_F32;
+    const int most = f32 ? (D > 128 ? 1 : 2) : (D > 128 ? 2 : 4);
+    r.mt = rows <= 16 ? 1 : rows <= 32 ? std::min(2, most) : most;
+    r.nw = f32 && D > 128 ? 2 : 4;
+    r.nrb = static_cast<int>((rows + 16 * r.mt - 1) / (16 * r.mt));
+    const size_t units = nkv * r.nrb;
+    size_t splits = std::max<size_t>(1, 2 * static_cast<size_t>(num_cus) / std::max<size_t>(units, 1));
+    splits = std::min(splits, std::max<size_t>(1, keys / (32 * r.nw)));
+    r.splits = static_cast<int>(std::min<size_t>(splits, 256));
+    r.floats = r.splits > 1 ? units * r.splits * 16 * r.mt * (D + 2) : 0;
+    return r;
+}
+
+int run_rows(int dev, hipStream_t stream, int dtype, int D, RowsParams* p, size_t keys) {
+    const size_t nkv = static_cast<size_t>(p->batch) * p->kv_heads;
+    const size_t rows = static_cast<size_t>(p->n) * p->group;
+    const RowsPlan plan = plan_rows(dtype, D, nkv, rows, keys, g_dev[dev].num_cus);
+    p->nrb = plan.nrb;
+    p->num_splits = plan.splits;
+    const size_t grid = nkv * plan.nrb * plan.splits, mgrid = (nkv * rows + 3) / 4;
+    if (grid > kOpsMaxGrid || mgrid > kOpsMaxGrid) return FA_ERR_UNSUPPORTED;
+    OpsWorkspace ws;
+    if (plan.floats) {
+        const int rc = ws.get(dev, stream, plan.floats * sizeof(float));
+        if (rc != FA_OK) return rc;
+        p->part_o = static_cast<float*>(ws.ptr);
+        p->part_ml = p->part_o + nkv * plan.nrb * plan.splits * 16 * plan.mt * D;
+    }
+    char name[64];
+    std::snprintf(name, sizeof(name), "fa_rows_%s_d%d_t%d", dtype_name(dtype), D, plan.mt);
+    int rc = ops_launch(dev, kCacheModule, name, grid, 64 * plan.nw, p, stream);
+    if (rc == FA_OK && plan.splits > 1) {
+        std::snprintf(name, sizeof(name), "fa_rows_merge_%s_d%d_t%d", dtype_name(dtype), D, plan.mt);
+        rc = ops_launch(dev, kCacheModule, name, mgrid, 256, p, stream);
+    }
+    return ws.done(stream, rc);
+}
+
+// Short query blocks, and few workgroups over many keys, run on the rows kernel, which splits the keys.
+bool score_takes_rows(const fa_score_config& c, int num_cus) {
+    const size_t group = c.heads / c.kv_heads;
+    if (c.seq_len_q * group <= 64) return true;
+    const size_t blocks = c.batch * c.heads * ((c.seq_len_q + 127) / 128);
+    return c.seq_len_k >= 512 && blocks * 4 <= static_cast<size_t>(num_cus);
+}
+
+int check_score(const fa_score_config* c) {
+    if (!c || !valid_dtype(c->dtype)) return FA_ERR_INVALID_ARG;
+    if (c->batch == 0 || c->heads == 0 || c->d_head == 0) return FA_OK;
+    if (c->kv_heads == 0 || c->heads % c->kv_heads != 0) return FA_ERR_INVALID_ARG;
+    if ((c->q_doc == nullptr) != (c->k_doc == nullptr)) return FA_ERR_INVALID_ARG;
+    if (c->d_head > kOpsMaxD || c->seq_len_q > kOpsMaxSeq || c->seq_len_k > kOpsMaxSeq || c->batch > kOpsMaxSeq ||
+        c->heads > kOpsMaxSeq || c->q_start > (int64_t)kOpsMaxSeq || c->q_start < -(int64_t)kOpsMaxSeq)
+        return FA_ERR_UNSUPPORTED;
+    return FA_OK;
+}
+
+void fill_score(const fa_score_config& c, const ScoreScale& sc, ScoreParams* p) {
+    p->batch = static_cast<int>(c.batch);
+    p->heads = static_cast<int>(c.heads);
+    p->kv_heads = static_cast<int>(c.kv_heads);
+    p->group = static_cast<int>(c.heads / c.kv_heads);
+    p->sq = static_cast<int>(c.seq_len_q);
+    p->sk = static_cast<int>(c.seq_len_k);
+    p->d = static_cast<int>(c.d_head);
+    p->causal = c.causal ? 1 : 0;
+    p->q_start = static_cast<int>(c.q_start);
+    p->slopes = c.slopes;
+    p->q_doc = c.q_doc;
+    p->k_doc = c.k_doc;
+    p->prefix = c.causal ? c.prefix : nullptr;
+    p->scale = sc.scale;
+    p->scale_log2e = sc.scale_log2e;
+    p->cap_in = sc.cap_in;
+    p->cap_log2e = sc.cap_log2e;
+}
+
+int launch_doc_ranges(int dev, hipStream_t stream, ScoreParams* p, int32_t* ws) {
+    const size_t tiles = static_cast<size_t>(p->batch) * (doc_tiles(p->sq) + doc_tiles(p->sk));
+    p->q_rng = ws;
+    p->k_rng = ws + 2 * static_cast<size_t>(p->batch) * doc_tiles(p->sq);
+    return ops_launch(dev, kScoreModule, "fa_score_doc_ranges", (tiles + 3) / 4, 256, p, stream);
+}
+size_t doc_range_bytes(const fa_score_config& c) {
+    return c.q_doc ? 2 * sizeof(int32_t) * c.batch * (doc_tiles(c.seq_len_q) + doc_tiles(c.seq_len_k)) : 0;
+}
+
+int check_cache(const fa_kv_cache* c, OpsLayout* k, OpsLayout* v, size_t* capacity) {
+    if (!c || !valid_dtype(c->dtype)) return FA_ERR_INVALID_ARG;
+    if (c->batch == 0 || c->kv_heads == 0 || c->d_head == 0) return FA_OK;
+    if (c->d_head > kOpsMaxD || c->batch > kOpsMaxSeq || c->kv_heads > kOpsMaxSeq) return FA_ERR_UNSUPPORTED;
+    if (!c->lens) return FA_ERR_INVALID_ARG;
+    size_t rows = c->capacity, blocks = c->batch;
+    if (c->block_table) {
+        if (c->page_size == 0 || (c->page_size & (c->page_size - 1)) != 0) return FA_ERR_INVALID_ARG;
+        if (c->page_size > kOpsMaxSeq || c->pages_per_seq > kOpsMaxSeq || c->n_pages > kOpsMaxSeq)
+            return FA_ERR_UNSUPPORTED;
+        *capacity = c->page_size * c->pages_per_seq;
+        rows = c->page_size;
+        blocks = c->n_pages;
+    } else {
+        *capacity = rows;
+    }
+    if (*capacity > kOpsMaxSeq) return FA_ERR_UNSUPPORTED;
+    int rc = resolve_layout(c->k_strides, blocks, rows, c->kv_heads, c->d_head, elem_size(c->dtype), true, k);
+    if (rc == FA_OK) rc = resolve_layout(c->v_strides, blocks, rows, c->kv_heads, c->d_head, elem_size(c->dtype), true, v);
+    if (rc == FA_OK && *capacity > 0 && (!c->k || !c->v)) rc = FA_ERR_INVALID_ARG;
+    return rc;
+}
+
+int page_shift(const fa_kv_cache& c) {
+    int s = 0;
+    while (c.block_table && (size_t(1) << s) < c.page_size) ++s;
+    return s;
+}
+
+int check_rotary(const fa_rotary_config* c) {
+    if (!c || !valid_dtype(c->dtype)) return FA_ERR_INVALID_ARG;
+    if (c->d_head > kOpsMaxD) return FA_ERR_UNSUPPORTED;
+    if (c->rot_dim < 2 || c->rot_dim % 2 != 0 || c->rot_dim > c->d_head) return FA_ERR_INVALID_ARG;
+    return FA_OK;
+}
+
+int add_rotary_tensor(RotParams* p, const void* src, void* dst, const OpsLayout& in, const OpsLayout& out, size_t heads,
+                      bool rotate, bool cache, bool* wide) {
+    RotTensor& t = p->t[p->nt++];
+    t.src = src;
+    t.dst = dst;
+    t.in = in.st;
+    t.out = out.st;
+    t.heads = static_cast<int>(heads);
+    t.rotate = rotate ? 1 : 0;
+    t.cache = cache ? 1 : 0;
+    *wide = *wide && in.aligned16 && out.aligned16 && aligned16(src) && aligned16(dst);
+    return FA_OK;
+}
+
+int launch_rotary(int dev, hipStream_t stream, int dtype, RotParams* p, bool wide) {
+    const int w = static_cast<int>(16 / elem_size(dtype));
+    const int run = p->interleaved ? p->rot : p->rot / 2;   // columns that a unit's runs divide
+    wide = wide && run % w == 0 && (p->d - p->rot) % w == 0;
+    p->cols = wide ? run / w + (p->d - p->rot) / w : p->rot / 2 + p->d - p->rot;
+    const size_t tokens = static_cast<size_t>(p->batch) * p->seq;
+    int heads = 1;
+    for (int i = 0; i < p->nt; ++i) heads = std::max(heads, p->t[i].heads);
+    // threads that share a token's heads: eight heads each where there are tokens enough to fill the GPU
+    size_t ht = std::max(1, heads / 8);
+    const size_t fill = static_cast<size_t>(g_dev[dev].num_cus) * 2048;
+    while (ht < static_cast<size_t>(heads) && tokens * p->cols * ht < fill) ht *= 2;
+    p->hthreads = static_cast<int>(std::min<size_t>(ht, heads));
+    const size_t grid = (tokens * p->cols * p->hthreads + 255) / 256;
+    if (grid > 2 * kOpsMaxGrid) return FA_ERR_UNSUPPORTED;
+    char name[64];
+    std::snprintf(name, sizeof(name), "fa_rotary_%s_%d", dtype_name(dtype), wide ? 1 : 0);
+    return ops_launch(dev, kRotaryModule, name, grid, 256, p, stream);
+}
+
+}  // namespace
+
+extern "C" {
+
+int fa_score_forward(void* stream_, const fa_score_config* c, const void* q, const void* k, const void* v, void* out,
+                     float* lse) {
+    int rc = check_score(c);
+    if (rc != FA_OK) return rc;
+    if (c->batch == 0 || c->heads == 0 || c->seq_len_q == 0 || c->d_head == 0) return FA_OK;
+    const size_t es = elem_size(c->dtype), d = c->d_head;
+    ScoreScale sc;
+    OpsLayout lq, lk, lv, lo;
+    if ((rc = resolve_scale(c->softmax_scale, c->softcap, d, &sc)) != FA_OK ||
+        (rc = resolve_layout(c->q, c->batch, c->seq_len_q, c->heads, d, es, false, &lq)) != FA_OK ||
+        (rc = resolve_layout(c->k, c->batch, c->seq_len_k, c->kv_heads, d, es, false, &lk)) != FA_OK ||
+        (rc = resolve_layout(c->v, c->batch, c->seq_len_k, c->kv_heads, d, es, false, &lv)) != FA_OK ||
+        (rc = resolve_layout(c->out, c->batch, c->seq_len_q, c->heads, d, es, true, &lo)) != FA_OK)
+        return rc;
+    if (!q || !out || (c->seq_len_k > 0 && (!k || !v))) return FA_ERR_INVALID_ARG;
+    const int D = ops_pad_d(d);
+    const ScoreGeo geo = score_geo(c->dtype, D);
+    const size_t nqb = (c->seq_len_q + geo.rows - 1) / geo.rows, grid = nqb * c->batch * c->heads;
+    if (c->batch * c->heads > kOpsMaxGrid || grid > kOpsMaxGrid) return FA_ERR_UNSUPPORTED;
+    int dev;
+    if ((rc = ops_begin(&dev, kScoreModule)) != FA_OK) return rc;
+    const hipStream_t stream = static_cast<hipStream_t>(stream_);
+    const bool vec = vec_ok(q, lq, d) && vec_ok(k, lk, d) && vec_ok(v, lv, d);
+    const bool ovec = ovec_ok(out, lo, es);
+
+    if (score_takes_rows(*c, g_dev[dev].num_cus)) {
+        if ((rc = ops_module(dev, kCacheModule)) != FA_OK) return rc;
+        RowsParams p{};
+        p.q = q, p.k = k, p.v = v, p.out = out, p.lse = lse;
+        p.slopes = c->slopes, p.q_doc = c->q_doc, p.k_doc = c->k_doc, p.prefix = c->causal ? c->prefix : nullptr;
+        p.qs = lq.st, p.ks = lk.st, p.vs = lv.st, p.os = lo.st;
+        p.batch = static_cast<int>(c->batch), p.heads = static_cast<int>(c->heads);
+        p.kv_heads = static_cast<int>(c->kv_heads), p.group = static_cast<int>(c->heads / c->kv_heads);
+        p.n = static_cast<int>(c->seq_len_q), p.sk = static_cast<int>(c->seq_len_k), p.d = static_cast<int>(d);
+        p.causal = c->causal ? 1 : 0, p.q_start = static_cast<int>(c->q_start);
+        p.vec = vec, p.ovec = ovec;
+        p.scale = sc.scale, p.scale_log2e = sc.scale_log2e, p.cap_in = sc.cap_in, p.cap_log2e = sc.cap_log2e;
+        return run_rows(dev, stream, c->dtype, D, &p, c->seq_len_k);
+    }
+    ScoreParams p{};
+    fill_score(*c, sc, &p);
+    p.q = q, p.k = k, p.v = v, p.out = out, p.lse = lse;
+    p.qs = lq.st, p.ks = lk.st, p.vs = lv.st, p.os = lo.st;
+    p.vec = vec, p.ovec = ovec;
+    p.nqb = static_cast<int>(nqb);
+    OpsWorkspace ws;
+    if (c->q_doc) {
+        if ((rc = ws.get(dev, stream, doc_range_bytes(*c))) != FA_OK) return rc;
+        rc = launch_doc_ranges(dev, stream, &p, static_cast<int32_t*>(ws.ptr));
+    }
+    if (rc == FA_OK) {
+        char name[64];
+        std::snprintf(name, sizeof(name), "fa_score_forward_%s_d%d", dtype_name(c->dtype), D);
+        rc = ops_launch(dev, kScoreModule, name, grid, geo.threads, &p, stream);
+    }
+    return ws.done(stream, rc);
+}
+
+int fa_score_backward(void* stream_, const fa_score_config* c, const void* q, const void* k, const void* v,
+                      const void* out, const float* lse, const void* dout, void* dq, void* dk, void* dv) {
+    int rc = check_score(c);
+    if (rc != FA_OK) return rc;
+    if (c->batch == 0 || c->heads == 0 || c->d_head == 0) return FA_OK;
+    if (c->seq_len_q == 0 && c->seq_len_k == 0) return FA_OK;
+    const size_t es = elem_size(c->dtype), d = c->d_head, sq = c->seq_len_q, sk = c->seq_len_k;
+    ScoreScale sc;
+    OpsLayout lq, lk, lv, lo, ldo, ldq, ldk, ldv;
+    if ((rc = resolve_scale(c->softmax_scale, c->softcap, d, &sc)) != FA_OK ||
+        (rc = resolve_layout(c->q, c->batch, sq, c->heads, d, es, false, &lq)) != FA_OK ||
+        (rc = resolve_layout(c->k, c->batch, sk, c->kv_heads, d, es, false, &lk)) != FA_OK ||
+        (rc = resolve_layout(c->v, c->batch, sk, c->kv_heads, d, es, false, &lv)) != FA_OK ||
+        (rc = resolve_layout(c->out, c->batch, sq, c->heads, d, es, true, &lo)) != FA_OK ||
+        (rc = resolve_layout(c->dout, c->batch, sq, c->heads, d, es, false, &ldo)) != FA_OK ||
+        (rc = resolve_layout(c->dq, c->batch, sq, c->heads, d, es, true, &ldq)) != FA_OK ||
+        (rc = resolve_layout(c->dk, c->batch, sk, c->kv_heads, d, es, true, &ldk)) != FA_OK ||
+        (rc = resolve_layout(c->dv, c->batch, sk, c->kv_heads, d, es, true, &ldv)) != FA_OK)
+        return rc;
+    if (sq > 0 && (!q || !out || !lse || !dout)) return FA_ERR_INVALID_ARG;
+    if (sk > 0 && (!k || !v)) return FA_ERR_INVALID_ARG;
+    const int D = ops_pad_d(d);
+    const ScoreGeo geo = score_geo(c->dtype, D);
+    const size_t nqb = (sq + geo.rows - 1) / geo.rows, nkb = (sk + kDkvRows - 1) / kDkvRows;
+    const size_t rows = c->batch * c->heads * sq, dgrid = (rows + 15) / 16;
+    if (c->batch * c->heads > kOpsMaxGrid || nqb * c->batch * c->heads > kOpsMaxGrid ||
+        nkb * c->batch * c->kv_heads > kOpsMaxGrid || dgrid > 4 * kOpsMaxGrid)
+        return FA_ERR_UNSUPPORTED;
+    int dev;
+    if ((rc = ops_begin(&dev, kScoreModule)) != FA_OK) return rc;
+    const hipStream_t stream = static_cast<hipStream_t>(stream_);
+    ScoreParams p{};
+    fill_score(*c, sc, &p);
+    p.q = q, p.k = k, p.v = v, p.out_in = out, p.dout = dout, p.lse_in = lse;
+    p.dq = dq, p.dk = dk, p.dv = dv;
+    p.qs = lq.st, p.ks = lk.st, p.vs = lv.st, p.os = lo.st, p.dos = ldo.st;
+    p.dqs = ldq.st, p.dks = ldk.st, p.dvs = ldv.st;
+    p.vec = vec_ok(q, lq, d) && vec_ok(k, lk, d) && vec_ok(v, lv, d) && vec_ok(out, lo, d) && vec_ok(dout, ldo, d);
+    p.ovec = ovec_ok(dq, ldq, es) && ovec_ok(dk, ldk, es) && ovec_ok(dv, ldv, es);
+    OpsWorkspace ws;
+    const size_t rng = doc_range_bytes(*c);
+    if ((rc = ws.get(dev, stream, 2 * rows * sizeof(float) + rng + 16)) != FA_OK) return rc;
+    p.lse2 = static_cast<float*>(ws.ptr);
+    p.delta = p.lse2 + rows;
+    char name[64];
+    if (c->q_doc) rc = launch_doc_ranges(dev, stream, &p, reinterpret_cast<int32_t*>(p.delta + rows));
+    if (rc == FA_OK) {
+        std::snprintf(name, sizeof(name), "fa_score_delta_%s", dtype_name(c->dtype));
+        rc = ops_launch(dev, kScoreModule, name, dgrid, 256, &p, stream);
+    }
+    if (rc == FA_OK && (dk || dv)) {
+        p.nqb = static_cast<int>(nkb);
+        std::snprintf(name, sizeof(name), "fa_score_dkv_%s_d%d", dtype_name(c->dtype), D);
+        rc = ops_launch(dev, kScoreModule, name, nkb * c->batch * c->kv_heads, kDkvThreads, &p, stream);
+    }
+    if (rc == FA_OK && dq) {
+        p.nqb = static_cast<int>(nqb);
+        std::snprintf(name, sizeof(name), "fa_score_dq_%s_d%d", dtype_name(c->dtype), D);
+        rc = ops_launch(dev, kScoreModule, name, nqb * c->batch * c->heads, geo.threads, &p, stream);
+    }
+    return ws.done(stream, rc);
+}
+
+int fa_rotary_init(fa_rotary_config* cfg, int dtype, size_t d_head, size_t rot_dim, int interleaved, double base,
+                   int scaling, double factor, double original_len) {
+    if (!cfg) return FA_ERR_INVALID_ARG;
+    std::memset(cfg, 0, sizeof(*cfg));
+    cfg->dtype = dtype;
+    cfg->interleaved = interleaved ? 1 : 0;
+    cfg->d_head = d_head;
+    cfg->rot_dim = rot_dim;
+    cfg->gain = 1.0f;
+    const int rc = check_rotary(cfg);
+    if (rc != FA_OK) return rc;
+    if (!(base > 1.0) || !std::isfinite(base)) return FA_ERR_INVALID_ARG;
+    if (scaling < FA_ROTARY_NONE || scaling > FA_ROTARY_YARN) return FA_ERR_INVALID_ARG;
+    if (scaling != FA_ROTARY_NONE && (!(factor >= 1.0) || !std::isfinite(factor))) return FA_ERR_INVALID_ARG;
+    if (scaling == FA_ROTARY_NTK && rot_dim == 2) return FA_ERR_INVALID_ARG;   // its exponent has no value
+    if (scaling == FA_ROTARY_YARN && (!(original_len > 0.0) || !std::isfinite(original_len))) return FA_ERR_INVALID_ARG;
+    const double two_pi = 6.283185307179586476925, rot = static_cast<double>(rot_dim);
+    if (scaling == FA_ROTARY_NTK) base *= std::pow(factor, rot / (rot - 2.0));
+    double lo = 0.0, hi = 0.0;
+    if (scaling == FA_ROTARY_YARN) {
+        // pair index at which a pair makes that many turns over the trained length
+        auto index = [&](double turns) { return rot * std::log(original_len / (turns * two_pi)) / (2.0 * std::log(base)); };
+        lo = std::max(std::floor(index(32.0)), 0.0);
+        hi = std::min(std::ceil(index(1.0)), rot - 1.0);
+        cfg->gain = static_cast<float>(0.1 * std::log(factor) + 1.0);
+    }
+    for (size_t c = 0; c < rot_dim / 2; ++c) {
+        double f = std::pow(base, -2.0 * static_cast<double>(c) / rot) / two_pi;
+        if (scaling == FA_ROTARY_LINEAR) f /= factor;
+        if (scaling == FA_ROTARY_YARN) {
+            const double ramp =
+                std::min(1.0, std::max(0.0, (static_cast<double>(c) - lo) / std::max(hi - lo, 0.001)));
+            f = f / factor * ramp + f * (1.0 - ramp);
+        }
+        cfg->turns[c] = f;
+    }
+    return FA_OK;
+}
+
+int fa_rotary(void* stream, const fa_rotary_config* cfg, size_t batch, size_t seq_len, const int32_t* positions,
+              int inverse, const fa_rotary_tensor* ql, const void* q, void* q_out, const fa_rotary_tensor* kl,
+              const void* k, void* k_out) {
+    int rc = check_rotary(cfg);
+    if (rc != FA_OK) return rc;
+    if (!ql) return FA_ERR_INVALID_ARG;
+    if (batch == 0 || seq_len == 0) return FA_OK;
+    if (batch > kOpsMaxSeq || seq_len > kOpsMaxSeq) return FA_ERR_UNSUPPORTED;
+    if (!positions) return FA_ERR_INVALID_ARG;
+    RotParams p{};
+    bool wide = true;
+    for (int n = 0; n < (kl ? 2 : 1); ++n) {
+        const fa_rotary_tensor* t = n ? kl : ql;
+        const void* src = n ? k : q;
+        void* dst = n ? k_out : q_out;
+        if (t->heads == 0) continue;
+        if (t->heads > kOpsMaxSeq) return FA_ERR_UNSUPPORTED;
+        OpsLayout in, out;
+        if ((rc = resolve_layout(t->in, batch, seq_len, t->heads, cfg->d_head, elem_size(cfg->dtype), false, &in)) !=
+                FA_OK ||
+            (rc = resolve_layout(t->out, batch, seq_len, t->heads, cfg->d_head, elem_size(cfg->dtype), true, &out)) !=
+                FA_OK)
+            return rc;
+        if (!src || !dst) return FA_ERR_INVALID_ARG;
+        // in place the layouts have to agree: a thread reads what it writes
+        if (src == dst && (in.st.b != out.st.b || in.st.s != out.st.s || in.st.h != out.st.h)) return FA_ERR_INVALID_ARG;
+        add_rotary_tensor(&p, src, dst, in, out, t->heads, true, false, &wide);
+    }
+    if (p.nt == 0) return FA_OK;
+    p.batch = static_cast<int>(batch);
+    p.seq = static_cast<int>(seq_len);
+    p.d = static_cast<int>(cfg->d_head);
+    p.rot = static_cast<int>(cfg->rot_dim);
+    p.interleaved = cfg->interleaved ? 1 : 0;
+    p.pos = positions;
+    p.gain = cfg->gain;
+    p.sign = inverse ? -1.0f : 1.0f;
+    std::memcpy(p.turns, cfg->turns, sizeof(p.turns));
+    int dev;
+    if ((rc = ops_begin(&dev, kRotaryModule)) != FA_OK) return rc;
+    return launch_rotary(dev, static_cast<hipStream_t>(stream), cfg->dtype, &p, wide);
+}
+
+int fa_cache_append(void* stream, const fa_kv_cache* cache, const fa_append_config* cfg, const void* k, const void* v,
+                    const int32_t* positions, const void* q, void* q_out) {
+    OpsLayout ck, cv, lk, lv;
+    size_t capacity = 0;
+    int rc = check_cache(cache, &ck, &cv, &capacity);
+    if (rc != FA_OK) return rc;
+    if (!cfg) return FA_ERR_INVALID_ARG;
+    const fa_rotary_config* rot = cfg->rotary;
+    if (rot && (rc = check_rotary(rot)) != FA_OK) return rc;
+    if (rot && (rot->dtype != cache->dtype || rot->d_head != cache->d_head)) return FA_ERR_INVALID_ARG;
+    if (cfg->q_layout && !rot) return FA_ERR_INVALID_ARG;
+    if (cache->batch == 0 || cache->kv_heads == 0 || cache->d_head == 0 || cfg->n_tokens == 0) return FA_OK;
+    const size_t es = elem_size(cache->dtype), d = cache->d_head, n = cfg->n_tokens;
+    if (n > kOpsMaxSeq) return FA_ERR_UNSUPPORTED;
+    if ((rc = resolve_layout(cfg->k, cache->batch, n, cache->kv_heads, d, es, false, &lk)) != FA_OK ||
+        (rc = resolve_layout(cfg->v, cache->batch, n, cache->kv_heads, d, es, false, &lv)) != FA_OK)
+        return rc;
+    if (!k || !v || (rot && !positions)) return FA_ERR_INVALID_ARG;
+    RotParams p{};
+    bool wide = true;
+    if (capacity > 0) {
+        add_rotary_tensor(&p, k, cache->k, lk, ck, cache->kv_heads, rot != nullptr, true, &wide);
+        add_rotary_tensor(&p, v, cache->v, lv, cv, cache->kv_heads, false, true, &wide);
+    }
+    if (cfg->q_layout && cfg->q_layout->heads > 0) {
+        const fa_rotary_tensor* t = cfg->q_layout;
+        OpsLayout in, out;
+        if (t->heads > kOpsMaxSeq) return FA_ERR_UNSUPPORTED;
+        if ((rc = resolve_layout(t->in, cache->batch, n, t->heads, d, es, false, &in)) != FA_OK ||
+            (rc = resolve_layout(t->out, cache->batch, n, t->heads, d, es, true, &out)) != FA_OK)
+            return rc;
+        if (!q || !q_out) return FA_ERR_INVALID_ARG;
+        if (q == q_out && (in.st.b != out.st.b || in.st.s != out.st.s || in.st.h != out.st.h)) return FA_ERR_INVALID_ARG;
+        add_rotary_tensor(&p, q, q_out, in, out, t->heads, true, false, &wide);
+    }
+    if (p.nt == 0) return FA_OK;
+    p.batch = static_cast<int>(cache->batch);
+    p.seq = static_cast<int>(n);
+    p.d = static_cast<int>(d);
+    p.pos = positions;
+    p.lens = cache->lens;
+    p.table = cache->block_table;
+    p.capacity = static_cast<int>(capacity);
+    p.page_shift = page_shift(*cache);
+    p.n_pages = static_cast<int>(cache->n_pages);
+    p.pages_per_seq = static_cast<int>(cache->pages_per_seq);
+    p.sign = 1.0f;
+    if (rot) {
+        p.rot = static_cast<int>(rot->rot_dim);
+        p.interleaved = rot->interleaved ? 1 : 0;
+        p.gain = rot->gain;
+        std::memcpy(p.turns, rot->turns, sizeof(p.turns));
+    }
+    int dev;
+    if ((rc = ops_begin(&dev, kRotaryModule)) != FA_OK) return rc;
+    return launch_rotary(dev, static_cast<hipStream_t>(stream), cache->dtype, &p, wide);
+}
+
+int fa_tree_attention(void* stream, const fa_tree_config* c, const fa_kv_cache* cache, const void* q, void* out,
+                      float* lse) {
+    OpsLayout ck, cv, lq, lo;
+    size_t capacity = 0;
+    int rc = check_cache(cache, &ck, &cv, &capacity);
+    if (rc != FA_OK) return rc;
+    if (!c) return FA_ERR_INVALID_ARG;
+    if (cache->batch == 0 || c->heads == 0 || c->n_tokens == 0 || cache->d_head == 0) return FA_OK;
+    if (cache->kv_heads == 0 || c->heads % cache->kv_heads != 0) return FA_ERR_INVALID_ARG;
+    if (c->heads > kOpsMaxSeq || c->n_tokens > kTreeMaxTokens) return FA_ERR_UNSUPPORTED;
+    const size_t es = elem_size(cache->dtype), d = cache->d_head, n = c->n_tokens;
+    ScoreScale sc;
+    if ((rc = resolve_scale(c->softmax_scale, c->softcap, d, &sc)) != FA_OK ||
+        (rc = resolve_layout(c->q, cache->batch, n, c->heads, d, es, false, &lq)) != FA_OK ||
+        (rc = resolve_layout(c->out, cache->batch, n, c->heads, d, es, true, &lo)) != FA_OK)
+        return rc;
+    if (!q || !out) return FA_ERR_INVALID_ARG;
+    if (cache->batch * c->heads > kOpsMaxGrid) return FA_ERR_UNSUPPORTED;
+    RowsParams p{};
+    p.q = q, p.k = cache->k, p.v = cache->v, p.out = out, p.lse = lse;
+    p.slopes = c->slopes, p.lens = cache->lens, p.table = cache->block_table;
+    p.pos = c->positions, p.mask = c->mask;
+    p.qs = lq.st, p.ks = ck.st, p.vs = cv.st, p.os = lo.st;
+    p.batch = static_cast<int>(cache->batch), p.heads = static_cast<int>(c->heads);
+    p.kv_heads = static_cast<int>(cache->kv_heads), p.group = static_cast<int>(c->heads / cache->kv_heads);
+    p.n = static_cast<int>(n), p.sk = static_cast<int>(capacity), p.d = static_cast<int>(d);
+    p.page_shift = page_shift(*cache);
+    p.n_pages = static_cast<int>(cache->n_pages), p.pages_per_seq = static_cast<int>(cache->pages_per_seq);
+    p.mask_words = static_cast<int>((n + 63) / 64), p.mask_shared = c->mask_shared ? 1 : 0;
+    p.vec = vec_ok(q, lq, d) && vec_ok(cache->k, ck, d) && vec_ok(cache->v, cv, d);
+    p.ovec = ovec_ok(out, lo, es);
+    p.scale = sc.scale, p.scale_log2e = sc.scale_log2e, p.cap_in = sc.cap_in, p.cap_log2e = sc.cap_log2e;
+    int dev;
+    if ((rc = ops_begin(&dev, kCacheModule)) != FA_OK) return rc;
+    return run_rows(dev, static_cast<hipStream_t>(stream), cache->dtype, ops_pad_d(d), &p, capacity);
+}
+
+}  // extern "C"

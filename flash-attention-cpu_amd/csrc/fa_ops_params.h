@@ -1,0 +1,80 @@
+// fa_ops_params.h -- parameter blocks and geometry shared by the host code
+// (fa_ops_host.h) and the kernels of fa_score.hip, fa_cache.hip and
+// fa_rotary.hip.
+#ifndef FA_OPS_PARAMS_H
+#define FA_OPS_PARAMS_H
+
+#include <stdint.h>
+
+// Element strides between batches, tokens and heads.
+struct OpsStrides {
+    int64_t b, s, h;
+};
+
+// Tokens per entry of the document range tables.
+constexpr int kDocTile = 64;
+
+struct ScoreParams {
+    const void *q, *k, *v, *out_in, *dout;
+    void *out, *dq, *dk, *dv;
+    float* lse;               // forward: written where not NULL
+    const float* lse_in;      // backward
+    float *lse2, *delta;      // [batch, heads, sq]: lse * log2(e) (+inf: empty row) and dO . O
+    const float* slopes;
+    const int32_t *q_doc, *k_doc, *prefix;
+    int32_t *q_rng, *k_rng;   // (min, max) id of each kDocTile tokens
+    OpsStrides qs, ks, vs, os, dos, dqs, dks, dvs;
+    int batch, heads, kv_heads, group, sq, sk, d;
+    int causal, q_start;
+    int nqb;                  // query (dK/dV: key) blocks a slice
+    int vec;                  // 16-byte loads of Q, K, V, dO
+    int ovec;                 // wide stores of the outputs
+    float scale;              // of the scores
+    float scale_log2e;
+    float cap_in;             // 2 log2(e) scale / softcap: exponent of the cap's tanh
+    float cap_log2e;          // softcap * log2(e); 0: no cap
+};
+
+// Attention of few rows over a long key range, keys split over workgroups.
+struct RowsParams {
+    const void *q, *k, *v;
+    void* out;
+    float* lse;               // [batch, heads, n] or NULL
+    float *part_o, *part_ml;  // [slot][16 MT rows][D], [slot][2][16 MT]
+    const float* slopes;
+    const int32_t *q_doc, *k_doc, *prefix;   // score attention
+    const int32_t *lens, *table, *pos;       // tree attention (lens != NULL)
+    const uint64_t* mask;
+    OpsStrides qs, ks, vs, os;
+    int batch, heads, kv_heads, group, n, sk, d;   // n: tokens; sk: keys (tree: capacity)
+    int causal, q_start;
+    int page_shift, n_pages, pages_per_seq;
+    int mask_words, mask_shared;
+    int nrb, num_splits;      // row blocks of a (batch, kv head), splits of its keys
+    int vec, ovec;
+    float scale, scale_log2e, cap_in, cap_log2e;
+};
+
+// One tensor of a rotary or append launch.
+struct RotTensor {
+    const void* src;
+    void* dst;
+    OpsStrides in, out;
+    int heads;
+    int rotate;               // 0: copied
+    int cache;                // dst is a cache: rows lens[b] + token
+};
+
+struct RotParams {
+    RotTensor t[3];
+    int nt;
+    int batch, seq, d, rot, interleaved;
+    int cols;                 // units of a token and head (columns or column pairs, or chunks of them)
+    int hthreads;             // threads that share a token's heads
+    const int32_t *pos, *lens, *table;
+    int capacity, page_shift, n_pages, pages_per_seq;
+    float gain, sign;
+    double turns[128];
+};
+
+#endif  // FA_OPS_PARAMS_H

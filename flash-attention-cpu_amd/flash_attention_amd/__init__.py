@@ -27,6 +27,8 @@ from dataclasses import dataclass
 
 import numpy as np
 
+from . import operators
+
 _PKG_DIR = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 # FA_HIP_LIBRARY overrides the library (e.g. a build with other tuning macros);
 # the code object is found next to it unless FA_HIP_MODULE names one.
@@ -70,6 +72,7 @@ EXPORTED_SYMBOLS = (
     "fa_device_lp", "fa_multihead_lp",
     "fa_naive_attention", "fa_naive_device",
     "fa_init", "fa_describe_launch", "fa_probe_launch",
+    "fa_score_forward", "fa_score_backward", "fa_rotary_init", "fa_rotary", "fa_cache_append", "fa_tree_attention",
 )
 
 
@@ -177,6 +180,7 @@ def lib() -> ctypes.CDLL:
     L.fa_probe_launch.argtypes = [ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, _SZ, ctypes.c_uint,
                                   ctypes.POINTER(ctypes.c_double)]
     L.fa_probe_launch.restype = ctypes.c_int
+    operators.declare(L)
     _lib = L
     return L
 
@@ -410,3 +414,11 @@ def probe_launch(kind: int, stream: int, buf: int, nbytes: int, iters: int = 0) 
 def init() -> None:
     """Load the gfx950 code object on the current device; raises without one."""
     _check(lib().fa_init())
+
+
+# Attention with modified scores, rotary positions, key / value cache (operators.py)
+ROTARY_NONE, ROTARY_LINEAR, ROTARY_NTK, ROTARY_YARN = 0, 1, 2, 3
+from .operators import (  # noqa: E402
+    AppendConfig, KvCache, RotaryConfig, RotaryTensor, ScoreConfig, Strides, TreeConfig, append_config,
+    cache_append_device, kv_cache, rotary_config, rotary_device, rotary_tensor, score_attention_backward_device,
+    score_attention_device, score_config, tree_attention_device, tree_config)

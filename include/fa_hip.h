@@ -247,6 +247,161 @@ int fa_multihead_lp(int dtype, const void* q, size_t q_len, const void* k, size_
                     size_t seq_len_k, size_t d_head, const fa_config* config, float* out,
                     size_t out_len);
 
+/* ---- attention with modified scores ---------------------------------------
+ * No counterpart in the reference.  Softmax attention, forward and backward,
+ * on device pointers, stream-ordered.  Query i of head h stands at position
+ * i' = q_start + i, key j at position j:
+ *     x = softmax_scale * (q_i . k_j)
+ *     y = softcap > 0 ? softcap * tanh(x / softcap) : x
+ *     z = slopes ? y - slopes[h] * |i' - j| : y
+ *     key j is visible to query i iff
+ *         (!causal || j <= i' || (prefix && j < prefix[b]))  and
+ *         (!q_doc  || (q_doc[b][i] == k_doc[b][j] && q_doc[b][i] >= 0))
+ *     lse_i = log sum over visible j of e^z,   o_i = sum e^(z - lse_i) v_j
+ * A query that sees no key gets o = 0 and lse = -inf.  Document ids may come
+ * in any order; tokens with a negative id (padding) see nothing and are seen
+ * by none.  Keys and values that a query does not see do not reach it, also
+ * where they are infinite or NaN.
+ *
+ * heads is a multiple of kv_heads: query head h reads key / value head
+ * h / (heads / kv_heads).  Q, K, V, O and all gradients have the type `dtype`
+ * (products accumulate in f32; 16-bit inputs: probabilities and score
+ * gradients are rounded to the type for the products they enter).  slopes, prefix
+ * and lse are f32 / int32 / f32 whatever the type.  d_head <= 256.
+ *
+ * Layouts: element strides between batches, tokens and heads, columns next to
+ * each other; all three 0 means contiguous [batch, heads, seq, d_head].  The
+ * token stride is at least d_head.  Inputs may share memory between batches or heads
+ * (stride 0); outputs may not overlap.  Any alignment works; 16-byte aligned
+ * rows (pointers, strides and d_head) are faster. */
+typedef struct fa_strides {
+    int64_t batch, seq, head;
+} fa_strides;
+
+typedef struct fa_score_config {
+    int dtype;                 /* FA_DTYPE_* */
+    int causal;
+    size_t batch, heads, kv_heads, seq_len_q, seq_len_k, d_head;
+    int64_t q_start;           /* position of query 0 (a decode step: the cache length) */
+    float softmax_scale;       /* <= 0 or NaN: 1/sqrt(d_head) */
+    float softcap;             /* 0: none */
+    const float* slopes;       /* [heads], device memory; NULL: no bias */
+    const int32_t* q_doc;      /* [batch, seq_len_q], device memory; both or neither */
+    const int32_t* k_doc;      /* [batch, seq_len_k] */
+    const int32_t* prefix;     /* [batch], device memory; NULL: none; read if causal */
+    fa_strides q, k, v, out, dout, dq, dk, dv;
+} fa_score_config;
+
+/* O and, if lse != NULL, lse [batch, heads, seq_len_q].  With no keys
+ * (seq_len_k = 0) O is zero and lse -inf; any other zero dimension queues
+ * nothing. */
+int fa_score_forward(void* stream, const fa_score_config* cfg, const void* q, const void* k, const void* v,
+                     void* out, float* lse);
+/* dQ, dK, dV of fa_score_forward from its inputs, its O and lse and the
+ * gradient of O (lse itself gets none; slopes are constants).  Each of dq, dk and dv may be NULL
+ * where it is not wanted.  Results do not depend on the order in which
+ * workgroups run. */
+int fa_score_backward(void* stream, const fa_score_config* cfg, const void* q, const void* k, const void* v,
+                      const void* out, const float* lse, const void* dout, void* dq, void* dk, void* dv);
+
+/* ---- rotary positions -------------------------------------------------------
+ * No counterpart in the reference.  Column pairs of the first rot_dim columns
+ * of each head row are rotated by position * 2 pi * turns[c]:
+ *     (a, b) -> gain * (a cos - b sin, a sin + b cos)
+ * pairs (c, c + rot_dim / 2), or (2c, 2c + 1) where interleaved; the other
+ * columns are copied.  inverse rotates back with the same gain, which is the
+ * gradient.  Angles are reduced in 64 bits, so far positions keep their
+ * accuracy.  fa_rotary_init (host only) fills a config:
+ *     turns[c] = base^(-2c / rot_dim) / (2 pi), and
+ *     FA_ROTARY_LINEAR  turns / factor
+ *     FA_ROTARY_NTK     base * factor^(rot_dim / (rot_dim - 2)) as base
+ *     FA_ROTARY_YARN    turns of pairs that make more than 32 turns over
+ *                       original_len, turns / factor below one turn, a linear
+ *                       ramp between them; gain = 0.1 ln(factor) + 1
+ * or the caller writes turns and gain (of other schemes) into it. */
+#define FA_ROTARY_NONE 0
+#define FA_ROTARY_LINEAR 1
+#define FA_ROTARY_NTK 2
+#define FA_ROTARY_YARN 3
+#define FA_ROTARY_MAX_DIM 256
+typedef struct fa_rotary_config {
+    int dtype;                 /* FA_DTYPE_* */
+    int interleaved;
+    size_t d_head, rot_dim;    /* rot_dim even, 2 .. d_head; d_head <= 256 */
+    float gain;
+    double turns[FA_ROTARY_MAX_DIM / 2];
+} fa_rotary_config;
+int fa_rotary_init(fa_rotary_config* cfg, int dtype, size_t d_head, size_t rot_dim, int interleaved, double base,
+                   int scaling, double factor, double original_len);
+
+/* A tensor of `heads` head rows a token and the layouts of its input and
+ * output (as in fa_score_config; in place where pointers and strides are the same). */
+typedef struct fa_rotary_tensor {
+    size_t heads;
+    fa_strides in, out;
+} fa_rotary_tensor;
+/* positions: int32 [batch, seq_len], device memory.  k_layout may be NULL
+ * (one tensor). */
+int fa_rotary(void* stream, const fa_rotary_config* cfg, size_t batch, size_t seq_len, const int32_t* positions,
+              int inverse, const fa_rotary_tensor* q_layout, const void* q, void* q_out,
+              const fa_rotary_tensor* k_layout, const void* k, void* k_out);
+
+/* ---- key / value cache and attention of drafted trees -----------------------
+ * No counterpart in the reference.  A cache holds capacity rows a sequence,
+ * either one after another (block_table NULL: row r of sequence b at
+ * b * batch + r * seq + head * head elements) or in pages of a pool: row r
+ * lies in page block_table[b][r / page_size] at row r % page_size of it, and
+ * the batch stride is the stride between pages (page_size: a power of two;
+ * capacity is pages_per_seq * page_size).  Page numbers outside [0, n_pages)
+ * hold no rows: their keys are not seen, and writes to them are dropped.
+ * lens[b] rows of sequence b are filled (device memory); the drafted tokens'
+ * rows come right after them.  lens[b] < 0 marks an idle sequence: its
+ * queries get zeros, and nothing is written to it.  Rows at or past the capacity are not seen. */
+typedef struct fa_kv_cache {
+    int dtype;
+    size_t batch, kv_heads, d_head;
+    void *k, *v;
+    fa_strides k_strides, v_strides;   /* all 0: [batch or pages, kv_heads, rows, d_head] */
+    const int32_t* lens;               /* [batch] */
+    size_t capacity;                   /* rows a sequence, without pages */
+    const int32_t* block_table;        /* [batch, pages_per_seq] or NULL */
+    size_t page_size, n_pages, pages_per_seq;
+} fa_kv_cache;
+
+/* Writes the n tokens' keys and values (layouts as in fa_score_config,
+ * [batch, kv_heads, n, d_head]) to rows lens[b] .. lens[b] + n - 1; lens stays
+ * as it is.  With rotary and positions (int32 [batch, n]) the keys are
+ * rotated on the way, and so are, in the same launch, the queries q -> q_out
+ * where q_layout is given (rotary then has to be too). */
+typedef struct fa_append_config {
+    size_t n_tokens;
+    fa_strides k, v;
+    const fa_rotary_config* rotary;    /* NULL: keys are copied, positions not read */
+    const fa_rotary_tensor* q_layout;  /* NULL: no queries */
+} fa_append_config;
+int fa_cache_append(void* stream, const fa_kv_cache* cache, const fa_append_config* cfg, const void* k, const void* v,
+                    const int32_t* positions, const void* q, void* q_out);
+
+/* Attention of n drafted tokens a sequence: token i sees the rows before
+ * lens[b] and the drafted row lens[b] + t iff bit t % 64 of
+ * mask[b][i][t / 64] is set (mask: [batch, n, ceil(n / 64)] 64-bit words, device memory;
+ * mask_shared: one for all sequences; NULL: t <= i, so one token is a decode
+ * step).  softmax_scale, softcap and slopes as in fa_score_config, where
+ * filled rows stand at their row number and drafted ones at positions[b][t]
+ * (int32 [batch, n]; NULL: lens[b] + t).  q, out: [batch, heads, n, d_head]
+ * by default; lse: f32 [batch, heads, n] or NULL.  n <= 256, d_head <= 256. */
+typedef struct fa_tree_config {
+    size_t heads, n_tokens;
+    float softmax_scale, softcap;
+    const float* slopes;
+    const int32_t* positions;
+    const uint64_t* mask;
+    int mask_shared;
+    fa_strides q, out;
+} fa_tree_config;
+int fa_tree_attention(void* stream, const fa_tree_config* cfg, const fa_kv_cache* cache, const void* q, void* out,
+                      float* lse);
+
 /* ---- naive attention (materialised scores) -------------------------------
  * naive_attention -- src/naive.rs:14-75: the textbook O(seq_q * seq_k)
  * memory form (scores, row softmax, PV) that the crate keeps as its
