@@ -89,7 +89,7 @@ __device__ __forceinline__ void rows_body(const RowsParams& p) {
     v8 qreg[MT][NDC];
     f32x4 o[MT][NDB];
     float m[MT], l[MT], slope[MT];
-    int token[MT], pos[MT], qd[MT];
+    int token[MT], pos[MT];
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
         const int r = rfirst + 16 * t + li;
@@ -101,13 +101,29 @@ __device__ __forceinline__ void rows_body(const RowsParams& p) {
         for (int dc = 0; dc < NDC; ++dc)
             qreg[t][dc] = global_row<T>(q, p.qs.s, token[t], real ? p.n : 0, 32 * dc + 8 * g, p.d, p.vec);
         pos[t] = !tree ? p.q_start + token[t] : p.pos ? p.pos[b * p.n + token[t]] : len + token[t];
-        qd[t] = docs ? p.q_doc[(int64_t)b * p.n + token[t]] : 0;
         slope[t] = p.slopes ? p.slopes[h] * kLog2e : 0.0f;
 #pragma unroll
         for (int j = 0; j < NDB; ++j) o[t][j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
         m[t] = OPS_NEG_INF;
         l[t] = 0.0f;
     }
+
+    // whether token `tok` sees a key
+    auto sees = [&](int tok, int key) -> bool {
+        if (krows.at(key) < 0) return false;
+        if (!tree) {
+            if (p.causal && !(key <= p.q_start + tok || key < prefix)) return false;
+            if (!docs) return true;
+            const int id = p.q_doc[(int64_t)b * p.n + tok];
+            return id >= 0 && p.k_doc[(int64_t)b * p.sk + key] == id;
+        }
+        if (key < len) return true;
+        const int bit = key - len;
+        if (!p.mask) return bit <= tok;
+        const int64_t row = (p.mask_shared ? 0 : (int64_t)b * p.n) + tok;
+        return (p.mask[row * p.mask_words + (bit >> 6)] >> (bit & 63)) & 1;
+    };
+    bool special = false;   // V held infinities or NaN in a masked block
 
     for (int k0 = kbeg + SK * wave; k0 < kend; k0 += SK * NW) {
         bool hidden = k0 + SK > min(open, kend);
@@ -139,22 +155,8 @@ __device__ __forceinline__ void rows_body(const RowsParams& p) {
                     int kpos = key;
                     bool see = true;
                     if (masked) {
-                        see = krows.at(key) >= 0;
-                        if (tree) {
-                            if (key >= len && see) {
-                                const int bit = key - len;
-                                if (p.pos) kpos = p.pos[b * p.n + bit];
-                                if (p.mask) {
-                                    const int64_t row = (p.mask_shared ? 0 : (int64_t)b * p.n) + token[t];
-                                    see = (p.mask[row * p.mask_words + (bit >> 6)] >> (bit & 63)) & 1;
-                                } else {
-                                    see = bit <= token[t];
-                                }
-                            }
-                        } else {
-                            if (p.causal) see = see && (key <= pos[t] || key < prefix);
-                            if (docs) see = see && qd[t] >= 0 && p.k_doc[(int64_t)b * p.sk + min(key, p.sk - 1)] == qd[t];
-                        }
+                        see = sees(token[t], key);
+                        if (tree && p.pos && key >= len && see) kpos = p.pos[b * p.n + key - len];
                     }
                     z -= slope[t] * fabsf((float)(pos[t] - kpos));
                     s[kb][r] = see ? z : OPS_NEG_INF;
@@ -184,10 +186,11 @@ __device__ __forceinline__ void rows_body(const RowsParams& p) {
             for (int j = 0; j < NDB; ++j) o[t][j] *= corr;
         }
         if (masked) {
-#pragma unroll
-            for (int t = 0; t < MT; ++t)
-                mma_seen<T>(o[t], pb[t], [&](int, int j) { return col_op<T, LD>(Vs, 0, 16 * j, g, li); });
-        } else {
+            reread();
+            special = tile_clean<T, LD, D, SK, 64>(Vs, lane) || special;
+            reread();
+        }
+        {
 #pragma unroll
             for (int j = 0; j < NDB; ++j) {
                 const v8 a = col_op<T, LD>(Vs, 0, 16 * j, g, li);
@@ -197,6 +200,10 @@ __device__ __forceinline__ void rows_body(const RowsParams& p) {
         }
         reread();
     }
+
+    __shared__ int any_special[NW];
+    if (lane == 0) any_special[wave] = 0;
+    if (__builtin_amdgcn_ballot_w64(special) != 0 && lane == 0) any_special[wave] = 1;
 
     // join the waves' sums: the upper half leaves its own, the lower half adds them
     f32x4* const sums = reinterpret_cast<f32x4*>(smem);
@@ -231,6 +238,15 @@ __device__ __forceinline__ void rows_body(const RowsParams& p) {
         }
     }
     if (wave != 0) return;
+    int specials = 0;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) specials |= any_special[i];
+    auto row_at = [&](int key) -> const T* {
+        const int64_t at = vrows.at(key);
+        return at < 0 ? nullptr : V + at;
+    };
+    auto row_sees = [&](int key, int r) { return sees((rfirst + r) / p.group, key); };
+    const int mine = min(16 * MT, nrows - rfirst);
 
     if (p.num_splits > 1) {
         const int64_t part = ((int64_t)kv * p.nrb + rb) * p.num_splits + split;
@@ -243,6 +259,11 @@ __device__ __forceinline__ void rows_body(const RowsParams& p) {
                 p.part_ml[part * 32 * MT + 16 * t + li] = m[t];
                 p.part_ml[part * 32 * MT + 16 * MT + 16 * t + li] = l[t];
             }
+        }
+        if (specials) {
+            __threadfence();
+            add_specials<T, float, true>(kbeg, kend, mine, p.d, lane, row_at, row_sees,
+                                         [&](int r) { return p.part_o + (part * 16 * MT + r) * D; });
         }
         return;
     }
@@ -258,6 +279,13 @@ __device__ __forceinline__ void rows_body(const RowsParams& p) {
         if (p.lse && g == 0)
             p.lse[((int64_t)b * p.heads + h) * p.n + token[t]] =
                 l[t] == 0.0f ? OPS_NEG_INF : (m[t] + __builtin_log2f(l[t]) - kProbLog2<T>) * kLn2;
+    }
+    if (specials) {
+        __threadfence();
+        add_specials<T, T, true>(kbeg, kend, mine, p.d, lane, row_at, row_sees, [&](int r) {
+            const int h = hk * p.group + (rfirst + r) % p.group;
+            return reinterpret_cast<T*>(p.out) + b * p.os.b + h * p.os.h + (rfirst + r) / p.group * p.os.s;
+        });
     }
 }
 

@@ -169,74 +169,125 @@ __device__ __forceinline__ bool any_not_finite(typename Mma<T>::v8 v) {
 }
 
 // LDS reads do not move over this, nor are their values kept in registers for a second use.
-__device__ __forceinline__ void reread() { asm volatile("" ::: "memory"); }
+__device__ __forceinline__ void reread() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
 
-// acc[j] += op(i, j) * w[i] over the 32-row chunks i, where a weight of exactly 0
-// means "not seen": operand values of rows that are not seen must not reach the
-// sum, not even as 0 * inf.  Used on tiles with hidden pairs.  Values are
-// nearly always finite: that is checked first, and the plain product taken.  Otherwise the
-// finite values are summed, and infinities and NaN looked for among the seen ones,
-// one kind after another.
-template <typename T, int NB, int NCH, typename Op>
-__device__ __forceinline__ void mma_seen(f32x4 (&acc)[NB], const typename Mma<T>::v8 (&w)[NCH], Op op) {
+// Tiles that hold hidden pairs: a hidden pair has the weight 0, and values of rows that a
+// query does not see must not reach its sum, not even as 0 * inf.  So before
+// such a tile is multiplied, its infinities and NaN are replaced by zeros in LDS, each
+// thread looking at its share; where there were any, the kernel adds them once its
+// sums are written, to the rows that see them.  Returns whether the thread found one.
+template <typename T, int LD, int D, int ROWS, int NT>
+__device__ __forceinline__ bool tile_clean(T* tile, int tid) {
     using v8 = typename Mma<T>::v8;
-    bool bad = false;
+    constexpr int CPR = D / 8;
+    bool found = false;
+#pragma unroll 1
+    for (int pos = tid; pos < ROWS * CPR; pos += NT) {
+        T* at = tile + pos / CPR * LD + 8 * (pos % CPR);
+        v8 x = *reinterpret_cast<v8*>(at);
+        bool bad = false;
+        if constexpr (sizeof(T) == 2) {
+            // half words: magnitude + (2^15 - infinity) reaches 2^15 where not finite
+            constexpr unsigned kAdd = (0x8000u - (std::is_same<T, __bf16>::value ? 0x7f80u : 0x7c00u)) * 0x10001u;
+            typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+            const u32x4 u = __builtin_bit_cast(u32x4, x);
+            unsigned any = 0;
 #pragma unroll
-    for (int i = 0; i < NCH; ++i)
-#pragma unroll
-        for (int j = 0; j < NB; ++j) {
-            bad = bad || any_not_finite<T>(op(i, j));
-            reread();
+            for (int e = 0; e < 4; ++e) any |= (u[e] & 0x7fff7fffu) + kAdd;
+            bad = (any & 0x80008000u) != 0;
+        } else {
+            bad = any_not_finite<T>(x);
         }
-    if (__builtin_amdgcn_ballot_w64(bad) == 0) {
+        if (bad) {
+            found = true;
 #pragma unroll
-        for (int i = 0; i < NCH; ++i)
-#pragma unroll
-            for (int j = 0; j < NB; ++j) {
-                acc[j] = Mma<T>::mma(op(i, j), w[i], acc[j]);
-                reread();
-            }
-        return;
+            for (int e = 0; e < 8; ++e)
+                if (not_finite(float(x[e]))) x[e] = T(0.0f);
+            *reinterpret_cast<v8*>(at) = x;
+        }
     }
-    for (int kind = 0; kind < 4; ++kind) {   // finite, +inf, -inf, NaN
-#pragma unroll
-        for (int j = 0; j < NB; ++j) {
-            f32x4 sum = kind == 0 ? acc[j] : (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-            f32x4 neg = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int i = 0; i < NCH; ++i) {
-                reread();
-                v8 a = op(i, j), b = w[i], c = w[i];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float x = float(a[e]), y = float(w[i][e]);
-                    if (kind == 0) {
-                        if (not_finite(x)) a[e] = T(0.0f);
-                    } else {
-                        const bool hit = kind == 3 ? x != x : x == (kind == 1 ? 1.0f : -1.0f) * __builtin_huge_valf();
-                        a[e] = T(hit ? 1.0f : 0.0f);
-                        b[e] = T(y > 0.0f ? 1.0f : 0.0f);   // infinities keep the weight's sign
-                        c[e] = T(y < 0.0f ? 1.0f : 0.0f);
-                    }
-                }
-                sum = Mma<T>::mma(a, b, sum);
-                if (kind != 0) neg = Mma<T>::mma(a, c, neg);
-            }
-            if (kind == 0) {
-                acc[j] = sum;
-            } else {
-                const float special = kind == 1   ? __builtin_huge_valf()
-                                      : kind == 2 ? -__builtin_huge_valf()
-                                                  : __builtin_nanf("");
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    if (sum[r] > 0.0f) acc[j][r] += special;
-                    if (neg[r] > 0.0f) acc[j][r] -= special;
-                }
+    return found;
+}
+
+// Adds what tile_clean took out: rows [from, to) of src (a row's address: at(row), nullptr: none) that hold infinities or NaN, to
+// the rows r < n of the wave that see them.  POSITIVE weights: as they are, else as NaN.
+template <typename T, typename O, bool POSITIVE, typename At, typename See, typename Out>
+__device__ __forceinline__ void add_specials(int from, int to, int n, int d, int lane, At at, See see, Out out) {
+#pragma unroll 1
+    for (int row = from; row < to; ++row) {
+        const T* x = at(row);
+        if (!x) continue;
+#pragma unroll 1
+        for (int c = lane; c - lane < d; c += 64) {
+            const float y = c < d ? float(x[c]) : 0.0f;
+            if (__builtin_amdgcn_ballot_w64(not_finite(y)) == 0) continue;
+#pragma unroll 1
+            for (int r = 0; r < n; ++r) {
+                if (!see(row, r)) continue;
+                O* to_ = out(r);
+                if (not_finite(y)) to_[c] = O(POSITIVE ? float(to_[c]) + y : __builtin_nanf(""));
             }
         }
     }
 }
+
+// N elements of LDS, one array per (N, ID) in a kernel: distinct arrays, so that the
+// compiler sees that a DMA into one does not change what is read from another.
+template <typename T, int N, int ID>
+__device__ __forceinline__ T* lds_array() {
+    __shared__ __attribute__((aligned(16))) T buf[N];
+    return buf;
+}
+
+// The calling wave's outstanding loads and DMA have arrived.
+__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }
+
+// Fills ROWS x D tiles (rows of LD elements) from a matrix in global memory, zero
+// outside [0, rows) x [0, d): by DMA, lane L of run R = i NW + wave at 16-byte chunk 64 R + L of the
+// tile's image (pad chunks included) with offsets fixed for the whole kernel -- the buffer's range ends at the
+// last row, and lanes past it, past column d or in the pad read zeros --
+// or, where rows are not 16-byte aligned, element by element.
+template <typename T, int D, int ROWS, int NW>
+struct TileFill {
+    static constexpr int LD = D + kPad<T>, E = 16 / (int)sizeof(T), RCH = LD / E;
+    static constexpr int TOTAL = ROWS * RCH, RUNS = (TOTAL + 63) / 64, NI = (RUNS + NW - 1) / NW;
+    static constexpr int SIZE = RUNS * 64 * E;   // elements of a tile's buffer: whole runs
+    int voff[NI];
+    int wave, lane, d;
+    int64_t stride;
+    bool vec;
+    __device__ __forceinline__ TileFill(int64_t stride_, int d_, bool vec_, int wave_, int lane_)
+        : wave(wave_), lane(lane_), d(d_), stride(stride_), vec(vec_) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            const int pos = (i * NW + wave) * 64 + lane, r = pos / RCH, col = pos % RCH * E;
+            voff[i] = pos < TOTAL && col < d ? (int)(r * stride + col) * (int)sizeof(T) : 0x7ffffff0;
+        }
+    }
+    __device__ __forceinline__ void operator()(T* dst, const T* base, int row0, int rows) const {
+        const T* src = base + row0 * stride;
+        if (vec) {
+            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+                const_cast<T*>(src), (short)0, (int)(min(ROWS, rows - row0) * stride) * (int)sizeof(T), 0x00020000);
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                const int run = i * NW + wave;
+                if ((i + 1) * NW <= RUNS || run < RUNS)
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                        rs, (__attribute__((address_space(3))) void*)(dst + run * 64 * E), 16, voff[i], 0, 0, 0);
+            }
+        } else {
+            for (int pos = wave * 64 + lane; pos < ROWS * (D / 8); pos += 64 * NW) {
+                const int r = pos / (D / 8), col = 8 * (pos % (D / 8));
+                *reinterpret_cast<typename Mma<T>::v8*>(dst + r * LD + col) =
+                    global_row<T>(src, stride, r, rows - row0, col, d, false);
+            }
+        }
+    }
+};
 
 // Visibility of key j to the query at position pos (score attention).
 struct ScoreMask {

@@ -23,7 +23,7 @@ OpsState g_ops[kMaxDevices];
 
 constexpr size_t kOpsMaxSeq = size_t(1) << 30;      // tokens: positions and their sums stay in 32 bits
 constexpr size_t kOpsMaxD = 256;
-constexpr int64_t kOpsMaxRowStride = int64_t(1) << 23;   // elements: a tile's byte offsets stay in 32 bits
+constexpr int64_t kOpsMaxRowStride = int64_t(1) << 22;   // elements: a tile's byte offsets stay in 32 bits
 constexpr int64_t kOpsMaxStride = int64_t(1) << 44;
 constexpr size_t kTreeMaxTokens = 256;
 
@@ -174,15 +174,12 @@ int resolve_scale(float scale, float softcap, size_t d, ScoreScale* out) {
     return FA_OK;
 }
 
-// Query rows of a workgroup of the forward and dQ kernels, threads of theirs.
-struct ScoreGeo {
-    int rows, threads;
-};
-ScoreGeo score_geo(int dtype, int D) {
-    const bool wide = dtype == FA_DTYPE_F32 || D > 128;
-    return wide ? ScoreGeo{128, 512} : ScoreGeo{128, 256};
+// 16-row tiles a wave of the score kernels, which have four waves: two where that makes at
+// least `least` workgroups for every CU (what a wave reads from LDS serves both tiles).
+int score_tiles(int dtype, int D, size_t rows, size_t slices, size_t least, int num_cus) {
+    if (dtype == FA_DTYPE_F32 || D > 128) return 1;
+    return (rows + 127) / 128 * slices >= least * static_cast<size_t>(num_cus) ? 2 : 1;
 }
-constexpr int kDkvRows = 128, kDkvThreads = 512;
 constexpr size_t kOpsMaxGrid = size_t(1) << 22;   // workgroups: threads of a launch stay in 32 bits
 
 size_t doc_tiles(size_t n) { return (n + kDocTile - 1) / kDocTile; }
@@ -371,9 +368,8 @@ int fa_score_forward(void* stream_, const fa_score_config* c, const void* q, con
         return rc;
     if (!q || !out || (c->seq_len_k > 0 && (!k || !v))) return FA_ERR_INVALID_ARG;
     const int D = ops_pad_d(d);
-    const ScoreGeo geo = score_geo(c->dtype, D);
-    const size_t nqb = (c->seq_len_q + geo.rows - 1) / geo.rows, grid = nqb * c->batch * c->heads;
-    if (c->batch * c->heads > kOpsMaxGrid || grid > kOpsMaxGrid) return FA_ERR_UNSUPPORTED;
+    if (c->batch * c->heads > kOpsMaxGrid || (c->seq_len_q + 63) / 64 * c->batch * c->heads > kOpsMaxGrid)
+        return FA_ERR_UNSUPPORTED;
     int dev;
     if ((rc = ops_begin(&dev, kScoreModule)) != FA_OK) return rc;
     const hipStream_t stream = static_cast<hipStream_t>(stream_);
@@ -399,7 +395,8 @@ int fa_score_forward(void* stream_, const fa_score_config* c, const void* q, con
     p.q = q, p.k = k, p.v = v, p.out = out, p.lse = lse;
     p.qs = lq.st, p.ks = lk.st, p.vs = lv.st, p.os = lo.st;
     p.vec = vec, p.ovec = ovec;
-    p.nqb = static_cast<int>(nqb);
+    const int mt = score_tiles(c->dtype, D, c->seq_len_q, c->batch * c->heads, 2, g_dev[dev].num_cus);
+    p.nqb = static_cast<int>((c->seq_len_q + 64 * mt - 1) / (64 * mt));
     OpsWorkspace ws;
     if (c->q_doc) {
         if ((rc = ws.get(dev, stream, doc_range_bytes(*c))) != FA_OK) return rc;
@@ -407,8 +404,9 @@ int fa_score_forward(void* stream_, const fa_score_config* c, const void* q, con
     }
     if (rc == FA_OK) {
         char name[64];
-        std::snprintf(name, sizeof(name), "fa_score_forward_%s_d%d", dtype_name(c->dtype), D);
-        rc = ops_launch(dev, kScoreModule, name, grid, geo.threads, &p, stream);
+        std::snprintf(name, sizeof(name), "fa_score_forward_%s_d%d_t%d%s", dtype_name(c->dtype), D, mt,
+                      c->slopes || c->softcap > 0.0f ? "m" : "");
+        rc = ops_launch(dev, kScoreModule, name, c->batch * c->heads * p.nqb, 256, &p, stream);
     }
     return ws.done(stream, rc);
 }
@@ -435,11 +433,9 @@ int fa_score_backward(void* stream_, const fa_score_config* c, const void* q, co
     if (sq > 0 && (!q || !out || !lse || !dout)) return FA_ERR_INVALID_ARG;
     if (sk > 0 && (!k || !v)) return FA_ERR_INVALID_ARG;
     const int D = ops_pad_d(d);
-    const ScoreGeo geo = score_geo(c->dtype, D);
-    const size_t nqb = (sq + geo.rows - 1) / geo.rows, nkb = (sk + kDkvRows - 1) / kDkvRows;
     const size_t rows = c->batch * c->heads * sq, dgrid = (rows + 15) / 16;
-    if (c->batch * c->heads > kOpsMaxGrid || nqb * c->batch * c->heads > kOpsMaxGrid ||
-        nkb * c->batch * c->kv_heads > kOpsMaxGrid || dgrid > 4 * kOpsMaxGrid)
+    if (c->batch * c->heads > kOpsMaxGrid || (sq + 63) / 64 * c->batch * c->heads > kOpsMaxGrid ||
+        (sk + 63) / 64 * c->batch * c->kv_heads > kOpsMaxGrid || dgrid > 4 * kOpsMaxGrid)
         return FA_ERR_UNSUPPORTED;
     int dev;
     if ((rc = ops_begin(&dev, kScoreModule)) != FA_OK) return rc;
@@ -463,15 +459,18 @@ int fa_score_backward(void* stream_, const fa_score_config* c, const void* q, co
         std::snprintf(name, sizeof(name), "fa_score_delta_%s", dtype_name(c->dtype));
         rc = ops_launch(dev, kScoreModule, name, dgrid, 256, &p, stream);
     }
+    const char* mod = c->slopes || c->softcap > 0.0f ? "m" : "";
     if (rc == FA_OK && (dk || dv)) {
-        p.nqb = static_cast<int>(nkb);
-        std::snprintf(name, sizeof(name), "fa_score_dkv_%s_d%d", dtype_name(c->dtype), D);
-        rc = ops_launch(dev, kScoreModule, name, nkb * c->batch * c->kv_heads, kDkvThreads, &p, stream);
+        const int mt = score_tiles(c->dtype, D, sk, c->batch * c->kv_heads, 1, g_dev[dev].num_cus);
+        p.nqb = static_cast<int>((sk + 64 * mt - 1) / (64 * mt));
+        std::snprintf(name, sizeof(name), "fa_score_dkv_%s_d%d_t%d%s", dtype_name(c->dtype), D, mt, mod);
+        rc = ops_launch(dev, kScoreModule, name, c->batch * c->kv_heads * p.nqb, 256, &p, stream);
     }
     if (rc == FA_OK && dq) {
-        p.nqb = static_cast<int>(nqb);
-        std::snprintf(name, sizeof(name), "fa_score_dq_%s_d%d", dtype_name(c->dtype), D);
-        rc = ops_launch(dev, kScoreModule, name, nqb * c->batch * c->heads, geo.threads, &p, stream);
+        const int mt = score_tiles(c->dtype, D, sq, c->batch * c->heads, 2, g_dev[dev].num_cus);
+        p.nqb = static_cast<int>((sq + 64 * mt - 1) / (64 * mt));
+        std::snprintf(name, sizeof(name), "fa_score_dq_%s_d%d_t%d%s", dtype_name(c->dtype), D, mt, mod);
+        rc = ops_launch(dev, kScoreModule, name, c->batch * c->heads * p.nqb, 256, &p, stream);
     }
     return ws.done(stream, rc);
 }

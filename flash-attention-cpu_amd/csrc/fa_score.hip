@@ -14,15 +14,6 @@
 
 #include "fa_ops_common.h"
 
-// Tile shapes: MT 16-row tiles a wave, NW waves a workgroup, SK walked rows a stage.
-template <typename T, int D>
-struct Geo {
-    static constexpr bool wide = sizeof(T) == 4 || D > 128;
-    static constexpr int MT = wide ? 1 : 2;
-    static constexpr int NW = wide ? 8 : 4;
-    static constexpr int SK = sizeof(T) == 4 || D > 128 ? 32 : 64;
-};
-
 template <typename T>
 __device__ __forceinline__ const T* slice(const void* base, OpsStrides st, int b, int h) {
     return reinterpret_cast<const T*>(base) + b * st.b + h * st.h;
@@ -85,6 +76,23 @@ struct Stages {
     }
 };
 
+// f(stage) for every stage that holds a visible and a hidden pair.
+template <typename Test, typename F>
+__device__ __forceinline__ void each_masked(Test test, int count, int lane, F f) {
+    Stages<Test> stages(count, lane, test);
+    bool masked;
+    for (int st = stages.next(&masked); st >= 0; st = stages.next(&masked))
+        if (masked) f(st);
+}
+
+// Whether query `row` sees key `key`.
+__device__ __forceinline__ bool pair_seen(const ScoreParams& p, const ScoreMask& mask, int b, int row, int key) {
+    if (!mask.seen(key, p.q_start + row)) return false;
+    if (!p.q_doc) return true;
+    const int d = p.q_doc[(int64_t)b * p.sq + row];
+    return d >= 0 && d == p.k_doc[(int64_t)b * p.sk + key];
+}
+
 // (min, max) document of rows [r0, r1) from the range table (the tiles they touch).
 __device__ __forceinline__ void doc_range(const int32_t* rng, int r0, int r1, int* lo, int* hi) {
     *lo = 0x7fffffff;
@@ -101,55 +109,54 @@ __device__ __forceinline__ bool docs_meet(int alo, int ahi, int blo, int bhi, bo
     return alo <= bhi && blo <= ahi && ahi >= 0 && bhi >= 0;
 }
 
-// ROWS rows of a matrix into LDS, zero outside [0, rows) x [0, d).
-template <typename T, int D, int ROWS, int NT>
-__device__ __forceinline__ void fill_tile(T* dst, const T* src, int64_t stride, int row0, int rows, int d, bool vec,
-                                          int tid) {
-    constexpr int CPR = D / 8, LD = D + kPad<T>;
-    const T* p = src + row0 * stride;
-#pragma unroll
-    for (int i = 0; i < (ROWS * CPR + NT - 1) / NT; ++i) {
-        const int pos = tid + i * NT;
-        if (ROWS * CPR % NT == 0 || pos < ROWS * CPR) {
-            const int r = pos / CPR, col = 8 * (pos % CPR);
-            *reinterpret_cast<typename Mma<T>::v8*>(dst + r * LD + col) =
-                global_row<T>(p, stride, r, rows - row0, col, d, vec);
-        }
-    }
+// One value a lane from global memory into LDS, zero past n.
+__device__ __forceinline__ void fill_words(void* dst, const void* src, int n, int lane) {
+    const __amdgpu_buffer_rsrc_t rs =
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(src), (short)0, 4 * max(n, 0), 0x00020000);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)dst, 4, 4 * lane, 0, 0, 0);
 }
 
-// Scores in log2 units of the C registers of one 16-row block: cap and bias.
-// dist: position of the lane's row minus that of register 0 of the block.
-// t: the cap's tanh (backward).
-template <typename T>
-__device__ __forceinline__ f32x4 modify(const ScoreParams& p, f32x4 s, float slope, float dist, f32x4* t) {
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        float z;
-        if (p.cap_log2e != 0.0f) {
-            float th;
-            z = capped<T>(s[r], p.cap_in, p.cap_log2e, &th);
-            (*t)[r] = th;
-        } else {
-            z = s[r] * p.scale_log2e;
-        }
-        s[r] = z - slope * fabsf(dist - (float)r);
+// Keys of a stage.
+template <typename T, int D>
+constexpr int kStageKeys = sizeof(T) == 4 || D > 128 ? 32 : 64;
+
+// Whether queries [q0, q1), of documents qlo .. qhi, see a key of stage st, and whether
+// some pair is hidden.
+template <int SK>
+__device__ __forceinline__ bool key_stage(const ScoreParams& p, const ScoreMask& mask, int st, int q0, int q1, bool docs,
+                                          int qlo, int qhi, const int32_t* krng, bool* part) {
+    const int k0 = st * SK, k1 = k0 + SK;
+    bool v = true;
+    if (k1 > p.sk) *part = true;
+    if (p.causal) {
+        v = k0 <= p.q_start + q1 - 1 || k0 < mask.prefix;
+        if (!(k1 - 1 <= p.q_start + q0 || k1 <= mask.prefix)) *part = true;
     }
-    return s;
+    if (docs && v) v = docs_meet(qlo, qhi, krng[k0 / kDocTile * 2], krng[k0 / kDocTile * 2 + 1], part);
+    return v;
 }
 
 // ---------------------------------------------------------------------------
 // Forward
 // ---------------------------------------------------------------------------
-template <typename T, int D>
+// Four waves of MT 16-row tiles.  K and V tiles are double-buffered and filled by DMA: while
+// a stage's softmax and PV product run, K of the stage after the next and V of
+// the next arrive; one barrier a stage.  The loop is unrolled by two so that each buffer is
+// an array of its own.
+template <typename T, int D, int MT, bool MOD>
 __device__ __forceinline__ void score_forward(const ScoreParams& p) {
     using M = Mma<T>;
     using v8 = typename M::v8;
-    using G = Geo<T, D>;
-    constexpr int MT = G::MT, NW = G::NW, SK = G::SK, NT = 64 * NW, BQ = 16 * MT * NW;
+    constexpr int NW = 4, SK = kStageKeys<T, D>, BQ = 16 * MT * NW;
     constexpr int KB = SK / 16, NCH = SK / 32, NDC = D / 32, NDB = D / 16, LD = D + kPad<T>;
-    __shared__ __attribute__((aligned(16))) T Ks[SK * LD];
-    __shared__ __attribute__((aligned(16))) T Vs[SK * LD];
+    using Fill = TileFill<T, D, SK, NW>;
+    T* const Kb0 = lds_array<T, Fill::SIZE, 0>();
+    T* const Vb0 = lds_array<T, Fill::SIZE, 1>();
+    T* const Kb1 = lds_array<T, Fill::SIZE, 2>();
+    T* const Vb1 = lds_array<T, Fill::SIZE, 3>();
+    int* const Db0 = lds_array<int, 64, 4>();   // documents of the stage's keys
+    int* const Db1 = lds_array<int, 64, 5>();
+    int* const Special = lds_array<int, 1, 6>();   // V held infinities or NaN in a masked stage
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, li = lane & 15;
@@ -162,12 +169,15 @@ __device__ __forceinline__ void score_forward(const ScoreParams& p) {
     const bool docs = p.q_doc != nullptr;
     const int32_t* kdoc = docs ? p.k_doc + (int64_t)w.b * p.sk : nullptr;
     const ScoreMask mask = {p.causal, p.prefix ? p.prefix[w.b] : 0, p.sk};
-    const float slope = p.slopes ? p.slopes[h] * kLog2e : 0.0f;
+    const float slope = MOD && p.slopes ? p.slopes[h] * kLog2e : 0.0f;
+    const bool cap = MOD && p.cap_log2e != 0.0f;
+    // scores leave the QK^T chains raw, and the scale goes into the exponent; modified ones are in log2 units
+    const float c = MOD ? 1.0f : p.scale_log2e;
 
     v8 qreg[MT][NDC];
     int qd[MT];
     f32x4 o[MT][NDB];
-    float m[MT], l[MT];
+    float m[MT], l[MT], ref[MT];   // l: the lane's share of the row's sum; ref: m, or 0 while m = -inf
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
         const int row = row0 + 16 * t + li;
@@ -177,7 +187,7 @@ __device__ __forceinline__ void score_forward(const ScoreParams& p) {
 #pragma unroll
         for (int j = 0; j < NDB; ++j) o[t][j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
         m[t] = OPS_NEG_INF;
-        l[t] = 0.0f;
+        l[t] = ref[t] = 0.0f;
     }
 
     const int q1 = min(q0 + BQ, p.sq);
@@ -187,101 +197,220 @@ __device__ __forceinline__ void score_forward(const ScoreParams& p) {
         doc_range(p.q_rng + (int64_t)w.b * 2 * ((p.sq + kDocTile - 1) / kDocTile), q0, q1, &qlo, &qhi);
         krng = p.k_rng + (int64_t)w.b * 2 * ((p.sk + kDocTile - 1) / kDocTile);
     }
-    auto test = [&](int st, bool* part) -> bool {
-        const int k0 = st * SK, k1 = k0 + SK;
-        bool v = true;
-        if (k1 > p.sk) *part = true;
-        if (p.causal) {
-            v = k0 <= p.q_start + q1 - 1 || k0 < mask.prefix;
-            if (!(k1 - 1 <= p.q_start + q0 || k1 <= mask.prefix)) *part = true;
-        }
-        if (docs && v) v = docs_meet(qlo, qhi, krng[k0 / kDocTile * 2], krng[k0 / kDocTile * 2 + 1], part);
-        return v;
-    };
+    auto test = [&](int st, bool* part) -> bool { return key_stage<SK>(p, mask, st, q0, q1, docs, qlo, qhi, krng, part); };
     Stages<decltype(test)> stages((p.sk + SK - 1) / SK, lane, test);
+    const Fill kfill(p.ks.s, p.d, p.vec, wave, lane), vfill(p.vs.s, p.d, p.vec, wave, lane);
+    auto fill_k = [&](int st, T* dst, int* ids) {
+        kfill(dst, K, st * SK, p.sk);
+        if (docs && wave == 0 && lane < SK) fill_words(ids, kdoc + st * SK, p.sk - st * SK, lane);
+    };
 
-    bool masked;
-    for (int st = stages.next(&masked); st >= 0; st = stages.next(&masked)) {
-        const int k0 = st * SK;
-        __syncthreads();
-        fill_tile<T, D, SK, NT>(Ks, K, p.ks.s, k0, p.sk, p.d, p.vec, tid);
-        fill_tile<T, D, SK, NT>(Vs, V, p.vs.s, k0, p.sk, p.d, p.vec, tid);
-        __syncthreads();
-        v8 pb[MT][NCH];
+    // S^T of a stage, relative to the rows' references (log2 units where modified)
+    constexpr int PRE_K = NDC > 1 ? 2 : 1;
+    f32x4 s[MT][KB];
+    auto qk = [&](const T* Ks, int k0) {
+        constexpr int KR = PRE_K + 1;
+        v8 kk[KR][KB];
 #pragma unroll
-        for (int t = 0; t < MT; ++t) {
-            f32x4 s[KB];
-            const int pos = p.q_start + row0 + 16 * t + li;
+        for (int dc = 0; dc < PRE_K && dc < NDC; ++dc)
+#pragma unroll
+            for (int b = 0; b < KB; ++b) kk[dc][b] = row_op<T, LD>(Ks, 16 * b, dc, g, li);
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
 #pragma unroll
             for (int b = 0; b < KB; ++b) {
-                s[b] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int dc = 0; dc < NDC; ++dc) s[b] = M::mma(row_op<T, LD>(Ks, 16 * b, dc, g, li), qreg[t][dc], s[b]);
-                f32x4 th;
-                s[b] = modify<T>(p, s[b], slope, (float)(pos - (k0 + 16 * b + 4 * g)), &th);
+                const float x = MOD ? 0.0f : -ref[t];
+                s[t][b] = (f32x4){x, x, x, x};
             }
-            if (masked) {
 #pragma unroll
-                for (int b = 0; b < KB; ++b)
+        for (int dc = 0; dc < NDC; ++dc) {
+            if (dc + PRE_K < NDC) {
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int key = k0 + 16 * b + 4 * g + r;
-                        bool see = mask.seen(key, pos);
-                        if (docs) see = see && qd[t] >= 0 && kdoc[min(key, p.sk - 1)] == qd[t];
-                        if (!see) s[b][r] = OPS_NEG_INF;
-                    }
+                for (int b = 0; b < KB; ++b) kk[(dc + PRE_K) % KR][b] = row_op<T, LD>(Ks, 16 * b, dc + PRE_K, g, li);
             }
-            float mt = s[0][0];
 #pragma unroll
             for (int b = 0; b < KB; ++b)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) mt = fmaxf(mt, s[b][r]);
-            mt = row4_max(mt);
-            const float mn = fmaxf(m[t], mt);
-            const float ref = mn == OPS_NEG_INF ? 0.0f : mn;
-            const float corr = ops_exp2(m[t] - ref);
-            m[t] = mn;
+                for (int t = 0; t < MT; ++t) s[t][b] = M::mma(kk[dc % KR][b], qreg[t][dc], s[t][b]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if constexpr (MOD) {
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                const float dist = (float)(p.q_start + row0 + 16 * t + li - k0 - 4 * g);
+#pragma unroll
+                for (int b = 0; b < KB; ++b) {
+                    if (cap) {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            float th;
+                            s[t][b][r] = capped<T>(s[t][b][r], p.cap_in, p.cap_log2e, &th) - ref[t];
+                        }
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) s[t][b][r] = __builtin_fmaf(s[t][b][r], p.scale_log2e, -ref[t]);
+                    }
+                    if (p.slopes) {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            s[t][b][r] = __builtin_fmaf(-slope, fabsf(dist - (float)(16 * b + r)), s[t][b][r]);
+                    }
+                }
+            }
+        }
+    };
+    auto hide = [&](int k0, const int* ids) {
+#pragma unroll
+        for (int b = 0; b < KB; ++b) {
+            i32x4 kd = {0, 0, 0, 0};
+            if (docs) kd = *reinterpret_cast<const i32x4*>(ids + 16 * b + 4 * g);
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                const int pos = p.q_start + row0 + 16 * t + li;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    bool see = mask.seen(k0 + 16 * b + 4 * g + r, pos);
+                    if (docs) see = see && qd[t] >= 0 && kd[r] == qd[t];
+                    if (!see) s[t][b][r] = OPS_NEG_INF;
+                }
+            }
+        }
+    };
+    v8 pb[MT][NCH];
+    auto softmax = [&] {
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            float mt = s[t][0][0];
+#pragma unroll
+            for (int b = 0; b < KB; ++b)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) mt = fmaxf(mt, s[t][b][r]);
+            // the reference moves only when a score passes it by more than kLazy, or at a row's first key
+            const bool seen = m[t] != OPS_NEG_INF;
+            const float limit = seen ? kLazy : OPS_NEG_INF;
+            if (__builtin_amdgcn_ballot_w64(mt * c > limit) != 0) {
+                mt = row4_max(mt);
+                const bool grow = mt * c > limit;
+                const float delta = grow ? mt : 0.0f;
+#pragma unroll
+                for (int b = 0; b < KB; ++b) s[t][b] -= delta;
+                if (grow) m[t] = ref[t] = ref[t] + delta;
+                if (__builtin_amdgcn_ballot_w64(grow && seen) != 0) {
+                    const float corr = grow && seen ? ops_exp2(-delta * c) : 1.0f;
+                    l[t] *= corr;
+#pragma unroll
+                    for (int j = 0; j < NDB; ++j) o[t][j] *= corr;
+                }
+            }
             float sum = 0.0f;
 #pragma unroll
             for (int b = 0; b < KB; ++b)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const float x = ops_exp2(s[b][r] - ref + kProbLog2<T>);
+                    const float x = ops_exp2(__builtin_fmaf(s[t][b][r], c, kProbLog2<T>));
                     pb[t][b / 2][4 * (b & 1) + r] = T(x);
                     sum += x;
                 }
-            l[t] = l[t] * corr + row4_sum(sum);
-#pragma unroll
-            for (int j = 0; j < NDB; ++j) o[t][j] *= corr;
+            l[t] += sum;
         }
-        if (masked) {
+    };
+    constexpr int PRE_V = NCH * NDB >= 4 ? 3 : 1, VR = PRE_V + 1;
+    v8 va[VR];
+    auto v_op = [&](const T* Vs, int i) { return col_op<T, LD>(Vs, 32 * (i / NDB), 16 * (i % NDB), g, li); };
+    auto pv_preload = [&](const T* Vs) {
 #pragma unroll
-            for (int t = 0; t < MT; ++t)
-                mma_seen<T>(o[t], pb[t], [&](int i, int j) { return col_op<T, LD>(Vs, 32 * i, 16 * j, g, li); });
-        } else {
+        for (int i = 0; i < PRE_V; ++i) va[i] = v_op(Vs, i);
+    };
+    auto pv = [&](const T* Vs) {
 #pragma unroll
-            for (int i = 0; i < NCH; ++i)
+        for (int i = 0; i < NCH * NDB; ++i) {
+            if (i + PRE_V < NCH * NDB) va[(i + PRE_V) % VR] = v_op(Vs, i + PRE_V);
 #pragma unroll
-                for (int j = 0; j < NDB; ++j) {
-                    const v8 a = col_op<T, LD>(Vs, 32 * i, 16 * j, g, li);
-#pragma unroll
-                    for (int t = 0; t < MT; ++t) o[t][j] = M::mma(a, pb[t][i], o[t][j]);
-                }
+            for (int t = 0; t < MT; ++t) o[t][i % NDB] = M::mma(va[i % VR], pb[t][i / NDB], o[t][i % NDB]);
+            __builtin_amdgcn_sched_barrier(0);
         }
+    };
+    // whether some row of the wave sees some key of the stage (as far as causal and prefix tell)
+    auto active = [&](int st) -> bool {
+        if (st < 0 || row0 >= p.sq) return false;
+        return !p.causal || st * SK <= p.q_start + row0 + 16 * MT - 1 || st * SK < mask.prefix;
+    };
+
+    bool masked, masked_next = false;
+    int st = stages.next(&masked), nx = st < 0 ? -1 : stages.next(&masked_next);
+    if (st >= 0) {
+        fill_k(st, Kb0, Db0);
+        vfill(Vb0, V, st * SK, p.sk);
+    }
+    if (nx >= 0) fill_k(nx, Kb1, Db1);
+    if (tid == 0) *Special = 0;
+    wait_loads();
+    __syncthreads();
+    bool act = active(st);
+    if (act) {
+        qk(Kb0, st * SK);
+        if (masked) hide(st * SK, Db0);
+    }
+    __syncthreads();
+    auto step = [&](auto parity) {
+        constexpr int P = decltype(parity)::value;
+        T* const k_cur = P ? Kb1 : Kb0;
+        T* const k_next = P ? Kb0 : Kb1;
+        T* const v_cur = P ? Vb1 : Vb0;
+        T* const v_next = P ? Vb0 : Vb1;
+        bool masked_after = false;
+        const int after = nx < 0 ? -1 : stages.next(&masked_after);
+        if (after >= 0) fill_k(after, k_cur, P ? Db1 : Db0);
+        if (nx >= 0) vfill(v_next, V, nx * SK, p.sk);
+        if (masked && tile_clean<T, LD, D, SK, 64 * NW>(v_cur, tid)) *Special = 1;
+        if (act) {
+            if (!masked) pv_preload(v_cur);
+            softmax();
+        }
+        if (masked) __syncthreads();
+        if (act) {
+            if (masked) pv_preload(v_cur);
+            pv(v_cur);
+        }
+        act = active(nx);
+        if (act) {
+            qk(k_next, nx * SK);
+            if (masked_next) hide(nx * SK, P ? Db0 : Db1);
+        }
+        wait_loads();
+        __syncthreads();
+        st = nx, masked = masked_next;
+        nx = after, masked_next = masked_after;
+    };
+    while (st >= 0) {
+        step(std::integral_constant<int, 0>{});
+        if (st < 0) break;
+        step(std::integral_constant<int, 1>{});
     }
 
     T* O = slice<T>(p.out, p.os, w.b, h);
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
         const int row = row0 + 16 * t + li;
+        const float lt = row4_sum(l[t]);
         if (row >= p.sq) continue;
-        const float inv = l[t] == 0.0f ? 0.0f : 1.0f / l[t];
+        const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;
 #pragma unroll
         for (int j = 0; j < NDB; ++j) store4<T>(O + row * p.os.s, 16 * j + 4 * g, p.d, p.ovec, o[t][j] * inv);
         if (p.lse && g == 0) {
-            const float lse = (m[t] + __builtin_log2f(l[t]) - kProbLog2<T>) * kLn2;
-            p.lse[((int64_t)w.b * p.heads + h) * p.sq + row] = l[t] == 0.0f ? OPS_NEG_INF : lse;
+            const float lse = (m[t] * c + __builtin_log2f(lt) - kProbLog2<T>) * kLn2;
+            p.lse[((int64_t)w.b * p.heads + h) * p.sq + row] = lt == 0.0f ? OPS_NEG_INF : lse;
         }
+    }
+    if (*Special) {
+        __threadfence();
+        each_masked(test, stages.count, lane, [&](int stage) {
+            add_specials<T, T, true>(
+                stage * SK, min(stage * SK + SK, p.sk), min(16 * MT, p.sq - row0), p.d, lane,
+                [&](int key) { return V + key * p.vs.s; },
+                [&](int key, int r) { return pair_seen(p, mask, w.b, row0 + r, key); },
+                [&](int r) { return O + (row0 + r) * p.os.s; });
+        });
     }
 }
 
@@ -312,20 +441,46 @@ __device__ __forceinline__ void score_delta(const ScoreParams& p) {
     if (li == 0) {
         const float lse = p.lse_in[row];
         p.delta[row] = sum;
-        p.lse2[row] = lse == OPS_NEG_INF ? -OPS_NEG_INF : lse * kLog2e;
+        p.lse2[row] = lse == OPS_NEG_INF ? -OPS_NEG_INF : lse == -OPS_NEG_INF ? __builtin_nanf("") : lse * kLog2e;
     }
 }
 
-// dQ: query rows kept, keys walked.
-template <typename T, int D>
+// The weight p = e^(z - lse) and the gradient of the raw score (without the scale) of four scores.
+template <typename T, bool MOD>
+__device__ __forceinline__ void weigh(const ScoreParams& p, bool cap, f32x4 s, f32x4 dp, f32x4 lse2, f32x4 delta,
+                                      float slope, float dist, f32x4* w, f32x4* ds) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        float z, th = 0.0f;
+        if (MOD && cap) {
+            z = capped<T>(s[r], p.cap_in, p.cap_log2e, &th) - lse2[r];
+        } else {
+            z = __builtin_fmaf(s[r], p.scale_log2e, -lse2[r]);
+        }
+        if (MOD && p.slopes) z = __builtin_fmaf(-slope, fabsf(dist - (float)r), z);
+        const float x = ops_exp2(z);
+        float y = x * (dp[r] - delta[r]);
+        if (MOD && cap) y = __builtin_fmaf(-th * th, y, y);
+        (*w)[r] = x;
+        (*ds)[r] = y;
+    }
+}
+
+// dQ: query rows kept, keys walked.  Four waves of MT 16-row tiles; K and V tiles double-buffered, one barrier a stage.
+template <typename T, int D, int MT, bool MOD>
 __device__ __forceinline__ void score_dq(const ScoreParams& p) {
     using M = Mma<T>;
     using v8 = typename M::v8;
-    using G = Geo<T, D>;
-    constexpr int MT = G::MT, NW = G::NW, SK = G::SK, NT = 64 * NW, BQ = 16 * MT * NW;
-    constexpr int KB = SK / 16, NCH = SK / 32, NDC = D / 32, NDB = D / 16, LD = D + kPad<T>;
-    __shared__ __attribute__((aligned(16))) T Ks[SK * LD];
-    __shared__ __attribute__((aligned(16))) T Vs[SK * LD];
+    constexpr int NW = 4, SK = kStageKeys<T, D>, BQ = 16 * MT * NW;
+    constexpr int NCH = SK / 32, NDC = D / 32, NDB = D / 16, LD = D + kPad<T>;
+    using Fill = TileFill<T, D, SK, NW>;
+    T* const Kb0 = lds_array<T, Fill::SIZE, 0>();
+    T* const Vb0 = lds_array<T, Fill::SIZE, 1>();
+    T* const Kb1 = lds_array<T, Fill::SIZE, 2>();
+    T* const Vb1 = lds_array<T, Fill::SIZE, 3>();
+    int* const Db0 = lds_array<int, 64, 4>();
+    int* const Db1 = lds_array<int, 64, 5>();
+    int* const Special = lds_array<int, 1, 6>();
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, li = lane & 15;
@@ -339,8 +494,8 @@ __device__ __forceinline__ void score_dq(const ScoreParams& p) {
     const bool docs = p.q_doc != nullptr;
     const int32_t* kdoc = docs ? p.k_doc + (int64_t)w.b * p.sk : nullptr;
     const ScoreMask mask = {p.causal, p.prefix ? p.prefix[w.b] : 0, p.sk};
-    const float slope = p.slopes ? p.slopes[h] * kLog2e : 0.0f;
-    const bool cap = p.cap_log2e != 0.0f;
+    const float slope = MOD && p.slopes ? p.slopes[h] * kLog2e : 0.0f;
+    const bool cap = MOD && p.cap_log2e != 0.0f;
 
     v8 qreg[MT][NDC], doreg[MT][NDC];
     int qd[MT];
@@ -368,67 +523,104 @@ __device__ __forceinline__ void score_dq(const ScoreParams& p) {
         doc_range(p.q_rng + (int64_t)w.b * 2 * ((p.sq + kDocTile - 1) / kDocTile), q0, q1, &qlo, &qhi);
         krng = p.k_rng + (int64_t)w.b * 2 * ((p.sk + kDocTile - 1) / kDocTile);
     }
-    auto test = [&](int st, bool* part) -> bool {
-        const int k0 = st * SK, k1 = k0 + SK;
-        bool v = true;
-        if (k1 > p.sk) *part = true;
-        if (p.causal) {
-            v = k0 <= p.q_start + q1 - 1 || k0 < mask.prefix;
-            if (!(k1 - 1 <= p.q_start + q0 || k1 <= mask.prefix)) *part = true;
-        }
-        if (docs && v) v = docs_meet(qlo, qhi, krng[k0 / kDocTile * 2], krng[k0 / kDocTile * 2 + 1], part);
-        return v;
-    };
+    auto test = [&](int st, bool* part) -> bool { return key_stage<SK>(p, mask, st, q0, q1, docs, qlo, qhi, krng, part); };
     Stages<decltype(test)> stages((p.sk + SK - 1) / SK, lane, test);
+    const Fill kfill(p.ks.s, p.d, p.vec, wave, lane), vfill(p.vs.s, p.d, p.vec, wave, lane);
+    auto fill = [&](int st, T* k, T* v, int* ids) {
+        kfill(k, K, st * SK, p.sk);
+        vfill(v, V, st * SK, p.sk);
+        if (docs && wave == 0 && lane < SK) fill_words(ids, kdoc + st * SK, p.sk - st * SK, lane);
+    };
+    auto active = [&](int st) -> bool {
+        if (row0 >= p.sq) return false;
+        return !p.causal || st * SK <= p.q_start + row0 + 16 * MT - 1 || st * SK < mask.prefix;
+    };
 
-    bool masked;
-    for (int st = stages.next(&masked); st >= 0; st = stages.next(&masked)) {
+    bool masked = false, masked_next = false;
+    int st = stages.next(&masked);
+    if (tid == 0) *Special = 0;
+    if (st >= 0) fill(st, Kb0, Vb0, Db0);
+    wait_loads();
+    __syncthreads();
+    auto step = [&](auto parity) {
+        constexpr int P = decltype(parity)::value;
+        T* const Ks = P ? Kb1 : Kb0;
+        T* const Vs = P ? Vb1 : Vb0;
+        const int* const ids = P ? Db1 : Db0;
+        const int nx = stages.next(&masked_next);
+        if (nx >= 0) fill(nx, P ? Kb0 : Kb1, P ? Vb0 : Vb1, P ? Db0 : Db1);
         const int k0 = st * SK;
-        __syncthreads();
-        fill_tile<T, D, SK, NT>(Ks, K, p.ks.s, k0, p.sk, p.d, p.vec, tid);
-        fill_tile<T, D, SK, NT>(Vs, V, p.vs.s, k0, p.sk, p.d, p.vec, tid);
-        __syncthreads();
-        v8 db[MT][NCH];
+        const bool act = active(st);
 #pragma unroll
-        for (int t = 0; t < MT; ++t) {
-            const int pos = p.q_start + row0 + 16 * t + li;
+        for (int i = 0; i < NCH; ++i) {
+            v8 db[MT][1];
+            if (act) {
+                f32x4 s[MT][2], dp[MT][2];
 #pragma unroll
-            for (int b = 0; b < KB; ++b) {
-                f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f}, dp = {0.0f, 0.0f, 0.0f, 0.0f}, th;
+                for (int t = 0; t < MT; ++t)
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) s[t][b] = dp[t][b] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int dc = 0; dc < NDC; ++dc) {
-                    s = M::mma(row_op<T, LD>(Ks, 16 * b, dc, g, li), qreg[t][dc], s);
-                    dp = M::mma(row_op<T, LD>(Vs, 16 * b, dc, g, li), doreg[t][dc], dp);
-                }
-                s = modify<T>(p, s, slope, (float)(pos - (k0 + 16 * b + 4 * g)), &th);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    float ds = ops_exp2(s[r] - lse2[t]) * (dp[r] - delta[t]);
-                    if (cap) ds *= 1.0f - th[r] * th[r];
-                    if (masked) {
-                        const int key = k0 + 16 * b + 4 * g + r;
-                        bool see = mask.seen(key, pos) && lse2[t] != -OPS_NEG_INF;
-                        if (docs) see = see && qd[t] >= 0 && kdoc[min(key, p.sk - 1)] == qd[t];
-                        if (!see) ds = 0.0f;
+                    for (int b = 0; b < 2; ++b) {
+                        const v8 ka = row_op<T, LD>(Ks, 32 * i + 16 * b, dc, g, li);
+                        const v8 va = row_op<T, LD>(Vs, 32 * i + 16 * b, dc, g, li);
+#pragma unroll
+                        for (int t = 0; t < MT; ++t) {
+                            s[t][b] = M::mma(ka, qreg[t][dc], s[t][b]);
+                            dp[t][b] = M::mma(va, doreg[t][dc], dp[t][b]);
+                        }
                     }
-                    db[t][b / 2][4 * (b & 1) + r] = T(ds);
+                    if (NDC > 4 || MT > 1) __builtin_amdgcn_sched_barrier(0);
+                }
+#pragma unroll
+                for (int t = 0; t < MT; ++t) {
+                    const int pos = p.q_start + row0 + 16 * t + li;
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) {
+                        f32x4 x, ds;
+                        const int key = k0 + 32 * i + 16 * b + 4 * g;
+                        weigh<T, MOD>(p, cap, s[t][b], dp[t][b], (f32x4){lse2[t], lse2[t], lse2[t], lse2[t]},
+                                      (f32x4){delta[t], delta[t], delta[t], delta[t]}, slope, (float)(pos - key), &x, &ds);
+                        if (masked) {
+                            i32x4 kd = {0, 0, 0, 0};
+                            if (docs) kd = *reinterpret_cast<const i32x4*>(ids + 32 * i + 16 * b + 4 * g);
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                bool see = mask.seen(key + r, pos) && lse2[t] != -OPS_NEG_INF;
+                                if (docs) see = see && qd[t] >= 0 && kd[r] == qd[t];
+                                if (!see) ds[r] = 0.0f;
+                            }
+                        }
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) db[t][0][4 * b + r] = T(ds[r]);
+                    }
                 }
             }
-        }
-        if (masked) {
-#pragma unroll
-            for (int t = 0; t < MT; ++t)
-                mma_seen<T>(dq[t], db[t], [&](int i, int j) { return col_op<T, LD>(Ks, 32 * i, 16 * j, g, li); });
-        } else {
-#pragma unroll
-            for (int i = 0; i < NCH; ++i)
+            if (masked) {
+                __syncthreads();
+                if (tile_clean<T, LD, D, 32, 64 * NW>(Ks + 32 * i * LD, tid)) *Special = 1;
+                __syncthreads();
+            }
+            if (act) {
 #pragma unroll
                 for (int j = 0; j < NDB; ++j) {
                     const v8 a = col_op<T, LD>(Ks, 32 * i, 16 * j, g, li);
 #pragma unroll
-                    for (int t = 0; t < MT; ++t) dq[t][j] = M::mma(a, db[t][i], dq[t][j]);
+                    for (int t = 0; t < MT; ++t) dq[t][j] = M::mma(a, db[t][0], dq[t][j]);
+                    if (j % 4 == 3) __builtin_amdgcn_sched_barrier(0);
                 }
+            }
         }
+        wait_loads();
+        __syncthreads();
+        st = nx, masked = masked_next;
+    };
+    while (st >= 0) {
+        step(std::integral_constant<int, 0>{});
+        if (st < 0) break;
+        step(std::integral_constant<int, 1>{});
     }
     T* out = slice<T>(p.dq, p.dqs, w.b, h);
 #pragma unroll
@@ -438,42 +630,62 @@ __device__ __forceinline__ void score_dq(const ScoreParams& p) {
 #pragma unroll
         for (int j = 0; j < NDB; ++j) store4<T>(out + row * p.dqs.s, 16 * j + 4 * g, p.d, p.ovec, dq[t][j] * p.scale);
     }
+    if (*Special) {
+        __threadfence();
+        each_masked(test, stages.count, lane, [&](int stage) {
+            add_specials<T, T, false>(
+                stage * SK, min(stage * SK + SK, p.sk), min(16 * MT, p.sq - row0), p.d, lane,
+                [&](int key) { return K + key * p.ks.s; },
+                [&](int key, int r) { return pair_seen(p, mask, w.b, row0 + r, key); },
+                [&](int r) { return out + (row0 + r) * p.dqs.s; });
+        });
+    }
 }
 
-// dK and dV: key rows kept, the queries of every head of the group walked.
-template <typename T, int D>
+// dK and dV: key rows kept, the queries of every head of the group walked.  Four waves
+// of MT 16-row tiles; Q and dO tiles double-buffered, one barrier a stage.  A kv head's sums over its
+// query heads are formed here, in head order.
+template <typename T, int D, int MT, bool MOD>
 __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
     using M = Mma<T>;
     using v8 = typename M::v8;
-    constexpr int MT = 1, NW = 8, SQ = 32, NT = 64 * NW, BK = 16 * MT * NW;
-    constexpr int QB = SQ / 16, NCH = SQ / 32, NDC = D / 32, NDB = D / 16, LD = D + kPad<T>;
-    __shared__ __attribute__((aligned(16))) T Qs[SQ * LD];
-    __shared__ __attribute__((aligned(16))) T Os[SQ * LD];
-    __shared__ float Ls[2][SQ];
-    __shared__ int Ds[SQ];
+    constexpr int NW = 4, SQ = kStageKeys<T, D>, BK = 16 * MT * NW;
+    constexpr int NCH = SQ / 32, NDC = D / 32, NDB = D / 16, LD = D + kPad<T>;
+    using Fill = TileFill<T, D, SQ, NW>;
+    T* const Qb0 = lds_array<T, Fill::SIZE, 0>();
+    T* const Ob0 = lds_array<T, Fill::SIZE, 1>();
+    T* const Qb1 = lds_array<T, Fill::SIZE, 2>();
+    T* const Ob1 = lds_array<T, Fill::SIZE, 3>();
+    int* const Wb0 = lds_array<int, 192, 4>();   // of the stage's queries: lse2, delta, document
+    int* const Wb1 = lds_array<int, 192, 5>();
+    int* const Special = lds_array<int, 1, 6>();
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, li = lane & 15;
-    // a workgroup owns whole (batch, kv head) columns: no group in the map
-    const Work w = find_work(blockIdx.x, p.nqb, p.batch * p.kv_heads, 1, p.kv_heads);
-    const int kbeg = w.blk * BK, key = kbeg + 16 * wave + li;
+    // a workgroup owns whole (batch, kv head) columns: no group in the map; the first key blocks have most queries where causal
+    const Work w = find_work(gridDim.x - 1 - blockIdx.x, p.nqb, p.batch * p.kv_heads, 1, p.kv_heads);
+    const int kbeg = w.blk * BK, key0 = kbeg + 16 * MT * wave;
     const T* K = slice<T>(p.k, p.ks, w.b, w.hk);
     const T* V = slice<T>(p.v, p.vs, w.b, w.hk);
     const bool docs = p.q_doc != nullptr;
     const ScoreMask mask = {p.causal, p.prefix ? p.prefix[w.b] : 0, p.sk};
-    const bool cap = p.cap_log2e != 0.0f;
+    const bool cap = MOD && p.cap_log2e != 0.0f;
 
-    v8 kreg[NDC], vreg[NDC];
-    f32x4 dk[NDB], dv[NDB];
+    v8 kreg[MT][NDC], vreg[MT][NDC];
+    f32x4 dk[MT][NDB], dv[MT][NDB];
+    int kd[MT];
 #pragma unroll
-    for (int dc = 0; dc < NDC; ++dc) {
-        kreg[dc] = global_row<T>(K, p.ks.s, key, p.sk, 32 * dc + 8 * g, p.d, p.vec);
-        vreg[dc] = global_row<T>(V, p.vs.s, key, p.sk, 32 * dc + 8 * g, p.d, p.vec);
+    for (int t = 0; t < MT; ++t) {
+        const int key = key0 + 16 * t + li;
+#pragma unroll
+        for (int dc = 0; dc < NDC; ++dc) {
+            kreg[t][dc] = global_row<T>(K, p.ks.s, key, p.sk, 32 * dc + 8 * g, p.d, p.vec);
+            vreg[t][dc] = global_row<T>(V, p.vs.s, key, p.sk, 32 * dc + 8 * g, p.d, p.vec);
+        }
+        kd[t] = docs && key < p.sk ? p.k_doc[(int64_t)w.b * p.sk + key] : -1;
+#pragma unroll
+        for (int j = 0; j < NDB; ++j) dk[t][j] = dv[t][j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
     }
-    const int kd = docs && key < p.sk ? p.k_doc[(int64_t)w.b * p.sk + key] : -1;
-#pragma unroll
-    for (int j = 0; j < NDB; ++j) dk[j] = dv[j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-
     const int kend = min(kbeg + BK, p.sk);
     int klo = 0, khi = 0;
     const int32_t* qrng = nullptr;
@@ -491,74 +703,163 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
         if (docs && v) v = docs_meet(klo, khi, qrng[q0 / kDocTile * 2], qrng[q0 / kDocTile * 2 + 1], part);
         return v;
     };
+    const int nst = (p.sq + SQ - 1) / SQ;
+    Stages<decltype(test)> stages(nst, lane, test);
+    const Fill qfill(p.qs.s, p.d, p.vec, wave, lane), ofill(p.dos.s, p.d, p.vec, wave, lane);
+    // the next (head, stage): the stages of one head of the group after the other
+    int head = 0;
+    auto next = [&](bool* m) -> int {
+        int s = stages.next(m);
+        while (s < 0 && head + 1 < p.group && stages.count > 0) {
+            ++head;
+            stages.base = -64;
+            s = stages.next(m);
+            if (s < 0) head = p.group;   // no stage for one head is none for any
+        }
+        return s;
+    };
+    auto fill = [&](int hq, int st, T* q, T* o, int* words) {
+        const int h = w.hk * p.group + hq, q0 = st * SQ;
+        qfill(q, slice<T>(p.q, p.qs, w.b, h), q0, p.sq);
+        ofill(o, slice<T>(p.dout, p.dos, w.b, h), q0, p.sq);
+        const int64_t at = ((int64_t)w.b * p.heads + h) * p.sq + q0;
+        if (lane < SQ) {
+            if (wave == 0) fill_words(words, p.lse2 + at, p.sq - q0, lane);
+            if (wave == 1) fill_words(words + 64, p.delta + at, p.sq - q0, lane);
+            if (wave == 2 && docs) fill_words(words + 128, p.q_doc + (int64_t)w.b * p.sq + q0, p.sq - q0, lane);
+        }
+    };
+    auto active = [&](int st) -> bool {
+        if (key0 >= p.sk) return false;
+        return !p.causal || p.q_start + st * SQ + SQ - 1 >= key0 || key0 < mask.prefix;
+    };
 
-    for (int hq = 0; hq < p.group; ++hq) {
-        const int h = w.hk * p.group + hq;
-        const T* Q = slice<T>(p.q, p.qs, w.b, h);
-        const T* dO = slice<T>(p.dout, p.dos, w.b, h);
-        const int64_t rows = ((int64_t)w.b * p.heads + h) * p.sq;
-        const float slope = p.slopes ? p.slopes[h] * kLog2e : 0.0f;
-        Stages<decltype(test)> stages((p.sq + SQ - 1) / SQ, lane, test);
-        bool masked;
-        for (int st = stages.next(&masked); st >= 0; st = stages.next(&masked)) {
-            const int q0 = st * SQ;
-            __syncthreads();
-            fill_tile<T, D, SQ, NT>(Qs, Q, p.qs.s, q0, p.sq, p.d, p.vec, tid);
-            fill_tile<T, D, SQ, NT>(Os, dO, p.dos.s, q0, p.sq, p.d, p.vec, tid);
-            if (tid < SQ) {
-                const int i = q0 + tid;
-                Ls[0][tid] = i < p.sq ? p.lse2[rows + i] : -OPS_NEG_INF;
-                Ls[1][tid] = i < p.sq ? p.delta[rows + i] : 0.0f;
-                Ds[tid] = docs && i < p.sq ? p.q_doc[(int64_t)w.b * p.sq + i] : -1;
-            }
-            __syncthreads();
-            v8 pb[NCH], db[NCH];
+    bool masked = false, masked_next = false;
+    int st = next(&masked), hq = head;
+    if (tid == 0) *Special = 0;
+    if (st >= 0) fill(hq, st, Qb0, Ob0, Wb0);
+    wait_loads();
+    __syncthreads();
+    auto step = [&](auto parity) {
+        constexpr int P = decltype(parity)::value;
+        T* const Qs = P ? Qb1 : Qb0;
+        T* const Os = P ? Ob1 : Ob0;
+        const int* const words = P ? Wb1 : Wb0;
+        const float* const Ls = reinterpret_cast<const float*>(words);
+        const int nx = next(&masked_next), hnx = head;
+        if (nx >= 0) fill(hnx, nx, P ? Qb0 : Qb1, P ? Ob0 : Ob1, P ? Wb0 : Wb1);
+        const int q0 = st * SQ;
+        const bool act = active(st);
+        const float slope = MOD && p.slopes ? p.slopes[w.hk * p.group + hq] * kLog2e : 0.0f;
 #pragma unroll
-            for (int b = 0; b < QB; ++b) {
-                f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f}, dp = {0.0f, 0.0f, 0.0f, 0.0f}, th;
+        for (int i = 0; i < NCH; ++i) {
+            v8 pb[MT][1], db[MT][1];
+            if (act) {
+                f32x4 s[MT][2], dp[MT][2];
+#pragma unroll
+                for (int t = 0; t < MT; ++t)
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) s[t][b] = dp[t][b] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int dc = 0; dc < NDC; ++dc) {
-                    s = M::mma(row_op<T, LD>(Qs, 16 * b, dc, g, li), kreg[dc], s);
-                    dp = M::mma(row_op<T, LD>(Os, 16 * b, dc, g, li), vreg[dc], dp);
-                }
-                // |key - query|: the lane's row is the key here
-                s = modify<T>(p, s, slope, (float)(key - (p.q_start + q0 + 16 * b + 4 * g)), &th);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int i = 16 * b + 4 * g + r;
-                    float x = ops_exp2(s[r] - Ls[0][i]);
-                    float ds = x * (dp[r] - Ls[1][i]);
-                    if (cap) ds *= 1.0f - th[r] * th[r];
-                    if (masked) {
-                        bool see = mask.seen(key, p.q_start + q0 + i) && Ls[0][i] != -OPS_NEG_INF;
-                        if (docs) see = see && kd >= 0 && Ds[i] == kd;
-                        if (!see) x = ds = 0.0f;
+                    for (int b = 0; b < 2; ++b) {
+                        const v8 qa = row_op<T, LD>(Qs, 32 * i + 16 * b, dc, g, li);
+                        const v8 oa = row_op<T, LD>(Os, 32 * i + 16 * b, dc, g, li);
+#pragma unroll
+                        for (int t = 0; t < MT; ++t) {
+                            s[t][b] = M::mma(qa, kreg[t][dc], s[t][b]);
+                            dp[t][b] = M::mma(oa, vreg[t][dc], dp[t][b]);
+                        }
                     }
-                    pb[b / 2][4 * (b & 1) + r] = T(x);
-                    db[b / 2][4 * (b & 1) + r] = T(ds);
+                    if (NDC > 4 || MT > 1) __builtin_amdgcn_sched_barrier(0);
+                }
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    const int at = 32 * i + 16 * b + 4 * g, pos = p.q_start + q0 + at;
+                    const f32x4 lse2 = *reinterpret_cast<const f32x4*>(Ls + at);
+                    const f32x4 delta = *reinterpret_cast<const f32x4*>(Ls + 64 + at);
+#pragma unroll
+                    for (int t = 0; t < MT; ++t) {
+                        const int key = key0 + 16 * t + li;
+                        f32x4 x, ds;
+                        weigh<T, MOD>(p, cap, s[t][b], dp[t][b], lse2, delta, slope, (float)(key - pos), &x, &ds);
+                        if (masked) {
+                            i32x4 qd = {0, 0, 0, 0};
+                            if (docs) qd = *reinterpret_cast<const i32x4*>(words + 128 + at);
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                bool see = mask.seen(key, pos + r) && lse2[r] != -OPS_NEG_INF;
+                                if (docs) see = see && kd[t] >= 0 && qd[r] == kd[t];
+                                if (!see) x[r] = ds[r] = 0.0f;
+                            }
+                        }
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            pb[t][0][4 * b + r] = T(x[r]);
+                            db[t][0][4 * b + r] = T(ds[r]);
+                        }
+                    }
                 }
             }
             if (masked) {
-                mma_seen<T>(dv, pb, [&](int i, int j) { return col_op<T, LD>(Os, 32 * i, 16 * j, g, li); });
-                mma_seen<T>(dk, db, [&](int i, int j) { return col_op<T, LD>(Qs, 32 * i, 16 * j, g, li); });
-            } else {
+                __syncthreads();
+                const bool bad = tile_clean<T, LD, D, 32, 64 * NW>(Qs + 32 * i * LD, tid);
+                if (tile_clean<T, LD, D, 32, 64 * NW>(Os + 32 * i * LD, tid) || bad) *Special = 1;
+                __syncthreads();
+            }
+            if (act) {
 #pragma unroll
-                for (int i = 0; i < NCH; ++i)
+                for (int j = 0; j < NDB; ++j) {
+                    const v8 a = col_op<T, LD>(Os, 32 * i, 16 * j, g, li);
+                    const v8 c = col_op<T, LD>(Qs, 32 * i, 16 * j, g, li);
 #pragma unroll
-                    for (int j = 0; j < NDB; ++j) {
-                        dv[j] = M::mma(col_op<T, LD>(Os, 32 * i, 16 * j, g, li), pb[i], dv[j]);
-                        dk[j] = M::mma(col_op<T, LD>(Qs, 32 * i, 16 * j, g, li), db[i], dk[j]);
+                    for (int t = 0; t < MT; ++t) {
+                        dv[t][j] = M::mma(a, pb[t][0], dv[t][j]);
+                        dk[t][j] = M::mma(c, db[t][0], dk[t][j]);
                     }
+                    if (j % 2 == 1) __builtin_amdgcn_sched_barrier(0);
+                }
             }
         }
+        wait_loads();
+        __syncthreads();
+        st = nx, hq = hnx, masked = masked_next;
+    };
+    while (st >= 0) {
+        step(std::integral_constant<int, 0>{});
+        if (st < 0) break;
+        step(std::integral_constant<int, 1>{});
     }
-    if (key >= p.sk) return;
     T* outk = p.dk ? slice<T>(p.dk, p.dks, w.b, w.hk) : nullptr;
     T* outv = p.dv ? slice<T>(p.dv, p.dvs, w.b, w.hk) : nullptr;
 #pragma unroll
-    for (int j = 0; j < NDB; ++j) {
-        if (outk) store4<T>(outk + key * p.dks.s, 16 * j + 4 * g, p.d, p.ovec, dk[j] * p.scale);
-        if (outv) store4<T>(outv + key * p.dvs.s, 16 * j + 4 * g, p.d, p.ovec, dv[j]);
+    for (int t = 0; t < MT; ++t) {
+        const int key = key0 + 16 * t + li;
+        if (key >= p.sk) continue;
+#pragma unroll
+        for (int j = 0; j < NDB; ++j) {
+            if (outk) store4<T>(outk + key * p.dks.s, 16 * j + 4 * g, p.d, p.ovec, dk[t][j] * p.scale);
+            if (outv) store4<T>(outv + key * p.dvs.s, 16 * j + 4 * g, p.d, p.ovec, dv[t][j]);
+        }
+    }
+    if (*Special) {
+        __threadfence();
+        for (int x = 0; x < p.group; ++x) {
+            const int h = w.hk * p.group + x;
+            const T* Q = slice<T>(p.q, p.qs, w.b, h);
+            const T* dO = slice<T>(p.dout, p.dos, w.b, h);
+            each_masked(test, nst, lane, [&](int stage) {
+                const int from = stage * SQ, to = min(from + SQ, p.sq), n = min(16 * MT, p.sk - key0);
+                auto see = [&](int row, int r) { return pair_seen(p, mask, w.b, row, key0 + r); };
+                if (outk)
+                    add_specials<T, T, false>(from, to, n, p.d, lane, [&](int row) { return Q + row * p.qs.s; }, see,
+                                              [&](int r) { return outk + (key0 + r) * p.dks.s; });
+                if (outv)
+                    add_specials<T, T, true>(from, to, n, p.d, lane, [&](int row) { return dO + row * p.dos.s; }, see,
+                                             [&](int r) { return outv + (key0 + r) * p.dvs.s; });
+            });
+        }
     }
 }
 
@@ -587,23 +888,40 @@ extern "C" __global__ __launch_bounds__(256) void fa_score_doc_ranges(ScoreParam
 
 #define SCORE_TYPE(N, T)                                                                                    \
     extern "C" __global__ __launch_bounds__(256) void fa_score_delta_##N(ScoreParams p) { score_delta<T>(p); }
-#define SCORE_KERNELS(N, T, D)                                                                              \
-    extern "C" __global__ __launch_bounds__((64 * Geo<T, D>::NW)) void fa_score_forward_##N##_d##D(ScoreParams p) { \
-        score_forward<T, D>(p);                                                                             \
+#define SCORE_KERNEL(F, N, T, D, MT, WAVES)                                                                 \
+    extern "C" __global__ __launch_bounds__(256, WAVES) void fa_score_##F##_##N##_d##D##_t##MT(ScoreParams p) { \
+        score_##F<T, D, MT, false>(p);                                                                      \
     }                                                                                                       \
-    extern "C" __global__ __launch_bounds__((64 * Geo<T, D>::NW)) void fa_score_dq_##N##_d##D(ScoreParams p) {   \
-        score_dq<T, D>(p);                                                                                  \
-    }                                                                                                       \
-    extern "C" __global__ __launch_bounds__(512) void fa_score_dkv_##N##_d##D(ScoreParams p) { score_dkv<T, D>(p); }
+    extern "C" __global__ __launch_bounds__(256, WAVES) void fa_score_##F##_##N##_d##D##_t##MT##m(ScoreParams p) { \
+        score_##F<T, D, MT, true>(p);                                                                       \
+    }
+#define SCORE_KERNELS_16(N, T)             \
+    SCORE_KERNEL(forward, N, T, 64, 1, 2)  \
+    SCORE_KERNEL(forward, N, T, 64, 2, 2)  \
+    SCORE_KERNEL(forward, N, T, 128, 1, 2) \
+    SCORE_KERNEL(forward, N, T, 128, 2, 2) \
+    SCORE_KERNEL(forward, N, T, 256, 1, 2) \
+    SCORE_KERNEL(dq, N, T, 64, 1, 2)       \
+    SCORE_KERNEL(dq, N, T, 64, 2, 2)       \
+    SCORE_KERNEL(dq, N, T, 128, 1, 2)      \
+    SCORE_KERNEL(dq, N, T, 128, 2, 2)      \
+    SCORE_KERNEL(dq, N, T, 256, 1, 2)      \
+    SCORE_KERNEL(dkv, N, T, 64, 1, 2)      \
+    SCORE_KERNEL(dkv, N, T, 64, 2, 2)      \
+    SCORE_KERNEL(dkv, N, T, 128, 1, 2)     \
+    SCORE_KERNEL(dkv, N, T, 128, 2, 1)     \
+    SCORE_KERNEL(dkv, N, T, 256, 1, 1)
 SCORE_TYPE(bf16, __bf16)
 SCORE_TYPE(f16, _Float16)
 SCORE_TYPE(f32, float)
-SCORE_KERNELS(bf16, __bf16, 64)
-SCORE_KERNELS(bf16, __bf16, 128)
-SCORE_KERNELS(bf16, __bf16, 256)
-SCORE_KERNELS(f16, _Float16, 64)
-SCORE_KERNELS(f16, _Float16, 128)
-SCORE_KERNELS(f16, _Float16, 256)
-SCORE_KERNELS(f32, float, 64)
-SCORE_KERNELS(f32, float, 128)
-SCORE_KERNELS(f32, float, 256)
+SCORE_KERNELS_16(bf16, __bf16)
+SCORE_KERNELS_16(f16, _Float16)
+SCORE_KERNEL(forward, f32, float, 64, 1, 2)
+SCORE_KERNEL(forward, f32, float, 128, 1, 2)
+SCORE_KERNEL(forward, f32, float, 256, 1, 1)
+SCORE_KERNEL(dq, f32, float, 64, 1, 2)
+SCORE_KERNEL(dq, f32, float, 128, 1, 2)
+SCORE_KERNEL(dq, f32, float, 256, 1, 1)
+SCORE_KERNEL(dkv, f32, float, 64, 1, 2)
+SCORE_KERNEL(dkv, f32, float, 128, 1, 2)
+SCORE_KERNEL(dkv, f32, float, 256, 1, 1)
