@@ -2,7 +2,7 @@
 
 Outputs, next to this file (git-ignored, used in place):
   fa_kernels.hsaco  gfx950 code object with the attention kernels (hipcc --genco)
-  fa_score.hsaco, fa_cache.hsaco, fa_rotary.hsaco
+  fa_score_*.hsaco, fa_cache_*.hsaco (f32, bf16, f16), fa_rotary.hsaco
                     code objects of attention with modified scores, of the
                     key / value cache and of rotary positions
   libfa_hip.so      C ABI of include/fa_hip.h over the HIP runtime
@@ -24,7 +24,11 @@ CSRC = os.path.join(HERE, "csrc")
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 
 HSACO = os.path.join(HERE, "fa_kernels.hsaco")
-OPS = ("fa_score", "fa_cache", "fa_rotary")   # code objects of the operators, one a source file
+# code objects of the operators: name -> (source, defines)
+TYPES = {"f32": ("-DOPS_T=float", "-DOPS_NAME=f32"), "bf16": ("-DOPS_T=__bf16", "-DOPS_NAME=bf16", "-DOPS_16BIT"),
+         "f16": ("-DOPS_T=_Float16", "-DOPS_NAME=f16", "-DOPS_16BIT")}
+OBJECTS = {"fa_kernels": ("fa_kernels", ()), "fa_rotary": ("fa_rotary", ()),
+           **{f"{src}_{t}": (src, flags) for src in ("fa_score", "fa_cache") for t, flags in TYPES.items()}}
 LIB = os.path.join(HERE, "libfa_hip.so")
 BUILD = os.path.join(HERE, "_build")   # intermediate objects (git-ignored)
 
@@ -40,17 +44,18 @@ def _run(cmd: list[str]) -> None:
     subprocess.run(cmd, check=True)
 
 
-def _genco(name: str) -> str:
+def build_object(name: str) -> str:
+    src, flags = OBJECTS[name]
     out = os.path.join(HERE, name + ".hsaco")
-    _run([os.path.join(ROCM, "bin", "hipcc"), *HIP_FLAGS, "--genco",
-          os.path.join(CSRC, name + ".hip"), "-o", out])
+    _run([os.path.join(ROCM, "bin", "hipcc"), *HIP_FLAGS, *flags, "--genco", os.path.join(CSRC, src + ".hip"),
+          "-o", out])
     return out
 
 
 def build_kernels() -> str:
     """Every code object, compiled at the same time."""
-    with ThreadPoolExecutor(max_workers=1 + len(OPS)) as pool:
-        list(pool.map(_genco, ("fa_kernels", *OPS)))
+    with ThreadPoolExecutor(max_workers=len(OBJECTS)) as pool:
+        list(pool.map(build_object, OBJECTS))
     return HSACO
 
 

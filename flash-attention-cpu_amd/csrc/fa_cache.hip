@@ -1,239 +1,568 @@
-// fa_cache.hip -- gfx950 kernels for few query rows over many keys: drafted trees
+// fa_cache.hip -- gfx950 kernels for query rows over a cache: drafted trees
 // over a key / value cache (fa_tree_attention) and short query blocks of score
 // attention (fa_score_forward).
 //
 // The rows of a (sequence, kv head) are its tokens times the query heads of the
-// group, so K and V are read once for all of them.  A workgroup takes a run of keys and up
-// to 16 MT rows; each of its waves walks 32-key blocks of its own through LDS that only it
-// uses, with no barrier until the waves' sums are joined at the end.  Runs
-// of one sequence leave partial sums that fa_rows_merge joins.
+// group, so K and V are read once for all of them.  The keys of a sequence are cut into runs, one a
+// workgroup; more than one run leave partial sums that fa_rows_merge joins.
+//   stream: up to 64 rows.  Bound by memory: every wave walks 32-key blocks of its own
+//           through LDS that only it uses, two slots of K and V, one filled by DMA while the
+//           other is used; no barrier until the waves' sums are joined at the end.
+//   shared: more rows.  Four waves of two 16-row tiles share 64-key stages,
+//           double-buffered, so that K and V cross the L2 once for 128 rows.
+// Tiles in LDS have no padding, so that DMA instructions move 1 KiB of whole rows; row r keeps
+// 16-byte chunk x at position x ^ (r % 16), which spreads row reads and transposed
+// reads over the banks.
+//
+// Built once a type: OPS_T the element type, OPS_NAME its name in the kernels'.
 
 #include "fa_ops_common.h"
 
+// Operands and geometry of an unpadded, swizzled tile.
 template <typename T, int D>
-struct RowsGeo {
-    static constexpr int NW = sizeof(T) == 4 && D > 128 ? 2 : 4;   // LDS: 2 x 32 rows a wave
-    static constexpr int SK = 32;
-};
-
-// Where row `key` of sequence b lies (element offset), or -1: no such row.
-struct CacheRows {
-    const int32_t* table;
-    int64_t seq, batch;
-    int shift, n_pages, limit;
-    __device__ __forceinline__ int64_t at(int key) const {
-        if (key >= limit) return -1;
-        if (!table) return key * seq;
-        const int page = table[key >> shift];
-        if ((unsigned)page >= (unsigned)n_pages) return -1;
-        return page * batch + (key & ((1 << shift) - 1)) * seq;
+struct Swizzled {
+    using v8 = typename Mma<T>::v8;
+    static constexpr int E = 16 / (int)sizeof(T);   // elements of a chunk
+    static constexpr int CPR = D / E;               // chunks of a row
+    static constexpr int CM = CPR < 16 ? CPR : 16;
+    static constexpr int RPR = 64 / CPR > 0 ? 64 / CPR : 1;   // rows of a 1 KiB run
+    static_assert(CPR <= 64, "a run holds whole rows");
+    static __device__ __forceinline__ int at(int row, int col) {   // col: a multiple of E or inside its chunk
+        return row * D + (((col / E) ^ (row % CM)) * E) + col % E;
+    }
+    static __device__ __forceinline__ v8 row_op(const T* tile, int row0, int dc, int g, int li) {
+        const int r = row0 + li;
+        if constexpr (sizeof(T) == 2) {
+            return *reinterpret_cast<const v8*>(tile + at(r, 32 * dc + 8 * g));
+        } else {
+            const f32x4 a = *reinterpret_cast<const f32x4*>(tile + at(r, 32 * dc + 8 * g));
+            const f32x4 b = *reinterpret_cast<const f32x4*>(tile + at(r, 32 * dc + 8 * g + 4));
+            return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+    }
+    static __device__ __forceinline__ v8 col_op(const T* tile, int row0, int col0, int g, int li) {
+        if constexpr (sizeof(T) == 2) {
+            typedef __attribute__((address_space(3))) s16x4* lds4;
+            const int r = row0 + 4 * g + (li >> 2);
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4) const_cast<T*>(tile + at(r, col0 + 4 * (li & 3))));
+            const s16x4 hi =
+                __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4) const_cast<T*>(tile + at(r + 16, col0 + 4 * (li & 3))));
+            return __builtin_bit_cast(v8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        } else {
+            v8 v;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = tile[at(row0 + (e < 4 ? 0 : 12) + 4 * g + e, col0 + li)];
+            return v;
+        }
+    }
+    // tile_clean for this layout: chunks may be visited in any order
+    template <int ROWS, int NT>
+    static __device__ __forceinline__ bool clean(T* tile, int tid) {
+        return tile_clean<T, D, D, ROWS, NT>(tile, tid);
     }
 };
 
-template <typename T, int D, int MT>
-__device__ __forceinline__ void rows_body(const RowsParams& p) {
-    using M = Mma<T>;
-    using v8 = typename M::v8;
-    constexpr int NW = RowsGeo<T, D>::NW, SK = RowsGeo<T, D>::SK;
-    constexpr int KB = SK / 16, NDC = D / 32, NDB = D / 16, LD = D + kPad<T>, CPR = D / 8;
-    constexpr int TILE = SK * LD;
-    constexpr int SLOT = MT * NDB * 64;   // f32x4 of a wave's sums
-    constexpr int BYTES = 2 * NW * TILE * (int)sizeof(T);
-    static_assert(NW / 2 * SLOT * 16 <= BYTES, "the sums fit the tiles");
-    __shared__ __attribute__((aligned(16))) char smem[BYTES];
-    __shared__ float Ml[NW / 2][MT][2][16];
+__device__ __forceinline__ int load_uniform(const int32_t* p) {
+    // a scalar load: a vector load would wait for all of the wave's DMA
+    return *(const __attribute__((address_space(4))) int32_t*)p;
+}
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int g = lane >> 4, li = lane & 15;
-    T* const Ks = reinterpret_cast<T*>(smem) + wave * 2 * TILE;
-    T* const Vs = Ks + TILE;
+// Rows of one sequence's K or V and their way into LDS.
+template <typename T, int D, int ROWS, int NW>
+struct RowSource {
+    using S = Swizzled<T, D>;
+    static constexpr int RUNS = ROWS / S::RPR, NI = (RUNS + NW - 1) / NW;
+    static_assert(RUNS % NW == 0 && 16 % S::RPR == 0 && NW * S::RPR <= 32, "runs of a wave lie in 16-row groups");
+    const T* base;
+    int64_t seq, batch;
+    int voff[NI];
+    __device__ __forceinline__ RowSource(const T* b, int64_t seq_, int64_t batch_, int d, int wave, int lane)
+        : base(b), seq(seq_), batch(batch_) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            const int run = i * NW + wave, q = lane / S::CPR;
+            const int col = ((lane % S::CPR) ^ ((run * S::RPR + q) % S::CM)) * S::E;
+            voff[i] = col < d ? (int)(q * seq + col) * (int)sizeof(T) : 0x7ffffff0;
+        }
+    }
+    // DMA of rows [k0, k0 + ROWS), zeros at and past `end` and where a page is bad; pages of 16 rows or more
+    template <typename Cache>
+    __device__ __forceinline__ void fill(T* dst, int k0, int end, const int (&page)[ROWS / 16], const Cache& c,
+                                         int wave) const {
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            const int run = i * NW + wave, r0 = run * S::RPR, row = k0 + r0;
+            constexpr int kStep = NW * S::RPR;   // rows of the waves' i-th runs: in one 16-row group, or in two
+            int pg = page[i * kStep / 16];
+            if constexpr (kStep > 16) pg = wave * S::RPR >= 16 ? page[i * kStep / 16 + 1] : pg;
+            const int in = c.table ? row & c.page_mask : row;
+            const int n = pg < 0 ? 0 : max(0, min(S::RPR, end - row));
+            const T* src = base + (c.table && n > 0 ? pg * batch : 0) + (n > 0 ? in * seq : 0);
+            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+                const_cast<T*>(src), (short)0, (int)(n * seq) * (int)sizeof(T), 0x00020000);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                rs, (__attribute__((address_space(3))) void*)(dst + run * 64 * S::E), 16, voff[i], 0, 0, 0);
+        }
+    }
+    // the same element by element: any alignment, any page size.  Returns whether the thread met a bad page.
+    template <typename Cache>
+    __device__ __forceinline__ bool fill_slow(T* dst, int k0, int end, const Cache& c, int d, bool vec, int tid) const {
+        bool bad = false;
+        for (int pos = tid; pos < ROWS * (D / 8); pos += 64 * NW) {
+            const int r = pos / (D / 8), col = 8 * (pos % (D / 8));
+            const int64_t at = c.at(k0 + r, end, seq, batch);
+            bad = bad || (at < 0 && k0 + r < end);
+            const typename Mma<T>::v8 x = global_row<T>(base + (at < 0 ? 0 : at), 0, 0, at >= 0, col, d, vec);
+            if constexpr (sizeof(T) == 2) {
+                *reinterpret_cast<typename Mma<T>::v8*>(dst + S::at(r, col)) = x;
+            } else {
+                *reinterpret_cast<f32x4*>(dst + S::at(r, col)) = __builtin_shufflevector(x, x, 0, 1, 2, 3);
+                *reinterpret_cast<f32x4*>(dst + S::at(r, col + 4)) = __builtin_shufflevector(x, x, 4, 5, 6, 7);
+            }
+        }
+        return bad;
+    }
+};
 
-    // split, row block and (sequence, kv head) of the workgroup: the row blocks of one run
-    // of keys side by side on one XCD where the counts allow
+// The pages of a sequence.
+struct CachePages {
+    const int32_t* table;   // nullptr: rows one after another
+    int shift, page_mask, n_pages;
+    // page of a row, -1: bad (0 without pages)
+    __device__ __forceinline__ int page(int row) const {
+        if (!table) return 0;
+        const int pg = load_uniform(table + (row >> shift));
+        return (unsigned)pg < (unsigned)n_pages ? pg : -1;
+    }
+    // element offset of a row, or -1
+    __device__ __forceinline__ int64_t at(int row, int end, int64_t seq, int64_t batch) const {
+        if (row >= end) return -1;
+        if (!table) return row * seq;
+        const int pg = table[row >> shift];
+        return (unsigned)pg < (unsigned)n_pages ? pg * batch + (row & page_mask) * seq : -1;
+    }
+};
+
+// What a workgroup of either kernel works on.
+struct RowsWork {
+    int kv, split, rb, b, hk;
+    int len, prefix, open, kbeg, kend, nrows, rfirst;
+    bool tree, docs;
+};
+template <int STEP>
+__device__ __forceinline__ RowsWork rows_work(const RowsParams& p, int rows) {
+    RowsWork w;
+    // the row blocks of one run of keys side by side on one XCD where the counts allow
     const int nkv = p.batch * p.kv_heads, runs = nkv * p.num_splits;
-    int run, rb;
+    int run;
     if ((runs & 7) == 0) {
         const int t = blockIdx.x >> 3;
-        rb = t % p.nrb;
+        w.rb = t % p.nrb;
         run = t / p.nrb * 8 + (blockIdx.x & 7);
     } else {
-        rb = blockIdx.x % p.nrb;
+        w.rb = blockIdx.x % p.nrb;
         run = blockIdx.x / p.nrb;
     }
-    const int kv = run / p.num_splits, split = run % p.num_splits;
-    const int b = kv / p.kv_heads, hk = kv % p.kv_heads;
-    const bool tree = p.lens != nullptr, docs = p.q_doc != nullptr;
-
-    // keys of the sequence: all of the filled rows, then the drafted ones
-    const int len = tree ? p.lens[b] : 0;
-    const int prefix = p.prefix ? p.prefix[b] : 0;
+    w.kv = run / p.num_splits;
+    w.split = run % p.num_splits;
+    w.b = w.kv / p.kv_heads;
+    w.hk = w.kv % p.kv_heads;
+    w.tree = p.lens != nullptr;
+    w.docs = p.q_doc != nullptr;
+    // keys of the sequence: all of the filled rows, then the drafted ones; every row sees
+    // those before `open`
+    w.len = w.tree ? p.lens[w.b] : 0;
+    w.prefix = p.prefix ? p.prefix[w.b] : 0;
     int total;
-    if (tree) {
-        total = len < 0 ? 0 : (int)min((int64_t)len + p.n, (int64_t)p.sk);
+    if (w.tree) {
+        total = w.len < 0 ? 0 : (int)min((int64_t)w.len + p.n, (int64_t)p.sk);
+        w.open = min(max(w.len, 0), p.sk);
     } else {
-        total = p.causal ? max(min(max(p.q_start + p.n, prefix), p.sk), 0) : p.sk;
+        total = p.causal ? max(min(max(p.q_start + p.n, w.prefix), p.sk), 0) : p.sk;
+        w.open = w.docs ? 0 : p.causal ? max(p.q_start + 1, w.prefix) : p.sk;
     }
-    // keys that every row sees: those before `open`
-    const int open = tree ? min(max(len, 0), p.sk) : docs ? 0 : p.causal ? max(p.q_start + 1, prefix) : p.sk;
-    const int per = ((total + p.num_splits - 1) / p.num_splits + SK - 1) / SK * SK;
-    const int kbeg = min(split * per, total), kend = min(kbeg + per, total);
+    const int per = ((total + p.num_splits - 1) / p.num_splits + STEP - 1) / STEP * STEP;
+    w.kbeg = min((int64_t)w.split * per, (int64_t)total);
+    w.kend = min(w.kbeg + per, total);
+    w.nrows = p.n * p.group;
+    w.rfirst = w.rb * rows;
+    return w;
+}
 
-    const T* K = reinterpret_cast<const T*>(p.k) + hk * p.ks.h + (p.table ? 0 : b * p.ks.b);
-    const T* V = reinterpret_cast<const T*>(p.v) + hk * p.vs.h + (p.table ? 0 : b * p.vs.b);
-    const int32_t* table = p.table ? p.table + (int64_t)b * p.pages_per_seq : nullptr;
-    const CacheRows krows = {table, p.ks.s, p.ks.b, p.page_shift, p.n_pages, kend};
-    const CacheRows vrows = {table, p.vs.s, p.vs.b, p.page_shift, p.n_pages, kend};
+// Whether token `tok` sees key `key` < kend, as far as masks tell.
+__device__ __forceinline__ bool rows_see(const RowsParams& p, const RowsWork& w, int tok, int key) {
+    if (!w.tree) {
+        if (p.causal && !(key <= p.q_start + tok || key < w.prefix)) return false;
+        if (!w.docs) return true;
+        const int id = p.q_doc[(int64_t)w.b * p.n + tok];
+        return id >= 0 && p.k_doc[(int64_t)w.b * p.sk + key] == id;
+    }
+    if (key < w.len) return true;
+    const int bit = key - w.len;
+    if (!p.mask) return bit <= tok;
+    const int64_t row = (p.mask_shared ? 0 : (int64_t)w.b * p.n) + tok;
+    return (p.mask[row * p.mask_words + (bit >> 6)] >> (bit & 63)) & 1;
+}
 
-    // the wave's rows: token r / group, head r % group
-    const int nrows = p.n * p.group, rfirst = rb * 16 * MT;
-    v8 qreg[MT][NDC];
-    f32x4 o[MT][NDB];
-    float m[MT], l[MT], slope[MT];
+// MT 16-row tiles of a wave: their queries, and the running softmax over KB 16-key blocks at a time.
+template <typename T, int D, int MT, int KB, bool MOD>
+struct RowTiles {
+    using M = Mma<T>;
+    using S = Swizzled<T, D>;
+    using v8 = typename M::v8;
+    static constexpr int NDC = D / 32, NDB = D / 16, NCH = KB / 2;
+    v8 q[MT][NDC], pb[MT][NCH];
+    f32x4 o[MT][NDB], s[MT][KB];
+    float m[MT], ref[MT], l[MT];   // l: the lane's share of the row's sum
+    float slope[MT];
     int token[MT], pos[MT];
-#pragma unroll
-    for (int t = 0; t < MT; ++t) {
-        const int r = rfirst + 16 * t + li;
-        const bool real = r < nrows;
-        token[t] = real ? r / p.group : 0;
-        const int h = hk * p.group + (real ? r % p.group : 0);
-        const T* q = reinterpret_cast<const T*>(p.q) + b * p.qs.b + h * p.qs.h;
-#pragma unroll
-        for (int dc = 0; dc < NDC; ++dc)
-            qreg[t][dc] = global_row<T>(q, p.qs.s, token[t], real ? p.n : 0, 32 * dc + 8 * g, p.d, p.vec);
-        pos[t] = !tree ? p.q_start + token[t] : p.pos ? p.pos[b * p.n + token[t]] : len + token[t];
-        slope[t] = p.slopes ? p.slopes[h] * kLog2e : 0.0f;
-#pragma unroll
-        for (int j = 0; j < NDB; ++j) o[t][j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-        m[t] = OPS_NEG_INF;
-        l[t] = 0.0f;
-    }
+    uint64_t word[MT];             // the token's first mask word
+    int g, li;
+    float c;
 
-    // whether token `tok` sees a key
-    auto sees = [&](int tok, int key) -> bool {
-        if (krows.at(key) < 0) return false;
-        if (!tree) {
-            if (p.causal && !(key <= p.q_start + tok || key < prefix)) return false;
-            if (!docs) return true;
-            const int id = p.q_doc[(int64_t)b * p.n + tok];
-            return id >= 0 && p.k_doc[(int64_t)b * p.sk + key] == id;
-        }
-        if (key < len) return true;
-        const int bit = key - len;
-        if (!p.mask) return bit <= tok;
-        const int64_t row = (p.mask_shared ? 0 : (int64_t)b * p.n) + tok;
-        return (p.mask[row * p.mask_words + (bit >> 6)] >> (bit & 63)) & 1;
-    };
-    bool special = false;   // V held infinities or NaN in a masked block
-
-    for (int k0 = kbeg + SK * wave; k0 < kend; k0 += SK * NW) {
-        bool hidden = k0 + SK > min(open, kend);
-#pragma unroll
-        for (int i = 0; i < SK * CPR / 64; ++i) {
-            const int r = (i * 64 + lane) / CPR, col = 8 * ((i * 64 + lane) % CPR);
-            const int64_t ka = krows.at(k0 + r), va = vrows.at(k0 + r);
-            hidden = hidden || ka < 0;
-            *reinterpret_cast<v8*>(Ks + r * LD + col) = global_row<T>(K + ka, 0, 0, ka >= 0, col, p.d, p.vec);
-            *reinterpret_cast<v8*>(Vs + r * LD + col) = global_row<T>(V + va, 0, 0, va >= 0, col, p.d, p.vec);
-        }
-        const bool masked = __builtin_amdgcn_ballot_w64(hidden) != 0;
-        reread();
-        v8 pb[MT][1];
+    __device__ __forceinline__ void init(const RowsParams& p, const RowsWork& w, int rfirst, int lane) {
+        g = lane >> 4, li = lane & 15;
+        c = MOD ? 1.0f : p.scale_log2e;
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
-            f32x4 s[KB];
+            const int r = rfirst + 16 * t + li;
+            const bool real = r < w.nrows;
+            token[t] = real ? r / p.group : 0;
+            const int h = w.hk * p.group + (real ? r % p.group : 0);
+            const T* from = reinterpret_cast<const T*>(p.q) + w.b * p.qs.b + h * p.qs.h;
 #pragma unroll
-            for (int kb = 0; kb < KB; ++kb) {
-                s[kb] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+            for (int dc = 0; dc < NDC; ++dc)
+                q[t][dc] = global_row<T>(from, p.qs.s, token[t], real ? p.n : 0, 32 * dc + 8 * g, p.d, p.vec);
+            pos[t] = !w.tree ? p.q_start + token[t] : p.pos ? p.pos[w.b * p.n + token[t]] : w.len + token[t];
+            slope[t] = MOD && p.slopes ? p.slopes[h] * kLog2e : 0.0f;
+            word[t] = 0;
+            if (w.tree)
+                word[t] = p.mask ? p.mask[((p.mask_shared ? 0 : (int64_t)w.b * p.n) + token[t]) * p.mask_words]
+                                 : token[t] < 63 ? (2ull << token[t]) - 1 : ~0ull;
 #pragma unroll
-                for (int dc = 0; dc < NDC; ++dc)
-                    s[kb] = M::mma(row_op<T, LD>(Ks, 16 * kb, dc, g, li), qreg[t][dc], s[kb]);
+            for (int j = 0; j < NDB; ++j) o[t][j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+            m[t] = OPS_NEG_INF;
+            l[t] = ref[t] = 0.0f;
+        }
+    }
+    // Scores of KB blocks of keys from k0, relative to the references; hidden ones -inf.
+    __device__ __forceinline__ void scores(const RowsParams& p, const RowsWork& w, const CachePages& pages, const T* Ks,
+                                           int k0, bool masked, bool badpage) {
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int key = k0 + 16 * kb + 4 * g + r;
-                    float z = s[kb][r] * p.scale_log2e, th;
-                    if (p.cap_log2e != 0.0f) z = capped<T>(s[kb][r], p.cap_in, p.cap_log2e, &th);
-                    int kpos = key;
-                    bool see = true;
-                    if (masked) {
-                        see = sees(token[t], key);
-                        if (tree && p.pos && key >= len && see) kpos = p.pos[b * p.n + key - len];
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int b = 0; b < KB; ++b) {
+                const float x = MOD ? 0.0f : -ref[t];
+                s[t][b] = (f32x4){x, x, x, x};
+            }
+#pragma unroll
+        for (int dc = 0; dc < NDC; ++dc) {
+#pragma unroll
+            for (int b = 0; b < KB; ++b) {
+                const v8 k = S::row_op(Ks, 16 * b, dc, g, li);
+#pragma unroll
+                for (int t = 0; t < MT; ++t) s[t][b] = M::mma(k, q[t][dc], s[t][b]);
+            }
+            if (dc % 2 == 1) __builtin_amdgcn_sched_barrier(0);
+        }
+        if constexpr (MOD) {
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                const float dist = (float)(pos[t] - k0 - 4 * g);
+#pragma unroll
+                for (int b = 0; b < KB; ++b) {
+                    if (p.cap_log2e != 0.0f) {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            float th;
+                            s[t][b][r] = capped<T>(s[t][b][r], p.cap_in, p.cap_log2e, &th) - ref[t];
+                        }
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) s[t][b][r] = __builtin_fmaf(s[t][b][r], p.scale_log2e, -ref[t]);
                     }
-                    z -= slope[t] * fabsf((float)(pos[t] - kpos));
-                    s[kb][r] = see ? z : OPS_NEG_INF;
+                    if (p.slopes) {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            float x = dist - (float)(16 * b + r);
+                            const int key = k0 + 16 * b + 4 * g + r;
+                            if (masked && w.tree && p.pos && key >= w.len && key < w.kend)
+                                x = (float)(pos[t] - p.pos[w.b * p.n + key - w.len]);
+                            s[t][b][r] = __builtin_fmaf(-slope[t], fabsf(x), s[t][b][r]);
+                        }
+                    }
                 }
             }
-            float mt = OPS_NEG_INF;
-#pragma unroll
-            for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) mt = fmaxf(mt, s[kb][r]);
-            mt = row4_max(mt);
-            const float mn = fmaxf(m[t], mt);
-            const float ref = mn == OPS_NEG_INF ? 0.0f : mn;
-            const float corr = ops_exp2(m[t] - ref);
-            m[t] = mn;
-            float sum = 0.0f;
-#pragma unroll
-            for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float x = ops_exp2(s[kb][r] - ref + kProbLog2<T>);
-                    pb[t][0][4 * kb + r] = T(x);
-                    sum += x;
-                }
-            l[t] = l[t] * corr + row4_sum(sum);
-#pragma unroll
-            for (int j = 0; j < NDB; ++j) o[t][j] *= corr;
         }
         if (masked) {
-            reread();
-            special = tile_clean<T, LD, D, SK, 64>(Vs, lane) || special;
-            reread();
-        }
-        {
 #pragma unroll
-            for (int j = 0; j < NDB; ++j) {
-                const v8 a = col_op<T, LD>(Vs, 0, 16 * j, g, li);
+            for (int b = 0; b < KB; ++b)
 #pragma unroll
-                for (int t = 0; t < MT; ++t) o[t][j] = M::mma(a, pb[t][0], o[t][j]);
-            }
+                for (int r = 0; r < 4; ++r) {
+                    const int key = k0 + 16 * b + 4 * g + r;
+                    const bool there = key < w.kend && (!badpage || pages.at(key, w.kend, 0, 0) >= 0);
+#pragma unroll
+                    for (int t = 0; t < MT; ++t) {
+                        bool see = there;
+                        if (w.tree && key - w.len < 64) {
+                            see = see && (key < w.len || (word[t] >> (max(key - w.len, 0) & 63)) & 1);
+                        } else if (see) {
+                            see = rows_see(p, w, token[t], key);
+                        }
+                        if (!see) s[t][b][r] = OPS_NEG_INF;
+                    }
+                }
         }
-        reread();
     }
-
-    __shared__ int any_special[NW];
-    if (lane == 0) any_special[wave] = 0;
-    if (__builtin_amdgcn_ballot_w64(special) != 0 && lane == 0) any_special[wave] = 1;
-
-    // join the waves' sums: the upper half leaves its own, the lower half adds them
-    f32x4* const sums = reinterpret_cast<f32x4*>(smem);
+    // the reference of a row moves only when a score passes it by more than kLazy, or at its first key
+    __device__ __forceinline__ void softmax() {
 #pragma unroll
-    for (int half = NW / 2; half >= 1; half /= 2) {
-        __syncthreads();
-        if (wave >= half && wave < 2 * half) {
-            f32x4* to = sums + (wave - half) * SLOT;
+        for (int t = 0; t < MT; ++t) {
+            float mt = s[t][0][0];
 #pragma unroll
-            for (int t = 0; t < MT; ++t) {
+            for (int b = 0; b < KB; ++b)
 #pragma unroll
-                for (int j = 0; j < NDB; ++j) to[(t * NDB + j) * 64 + lane] = o[t][j];
-                if (g == 0) {
-                    Ml[wave - half][t][0][li] = m[t];
-                    Ml[wave - half][t][1][li] = l[t];
+                for (int r = 0; r < 4; ++r) mt = fmaxf(mt, s[t][b][r]);
+            const bool seen = m[t] != OPS_NEG_INF;
+            const float limit = seen ? kLazy : OPS_NEG_INF;
+            if (__builtin_amdgcn_ballot_w64(mt * c > limit) != 0) {
+                mt = row4_max(mt);
+                const bool grow = mt * c > limit;
+                const float delta = grow ? mt : 0.0f;
+#pragma unroll
+                for (int b = 0; b < KB; ++b) s[t][b] -= delta;
+                if (grow) m[t] = ref[t] = ref[t] + delta;
+                if (__builtin_amdgcn_ballot_w64(grow && seen) != 0) {
+                    const float corr = grow && seen ? ops_exp2(-delta * c) : 1.0f;
+                    l[t] *= corr;
+#pragma unroll
+                    for (int j = 0; j < NDB; ++j) o[t][j] *= corr;
                 }
             }
+            float sum = 0.0f;
+#pragma unroll
+            for (int b = 0; b < KB; ++b)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float x = ops_exp2(__builtin_fmaf(s[t][b][r], c, kProbLog2<T>));
+                    pb[t][b / 2][4 * (b & 1) + r] = T(x);
+                    sum += x;
+                }
+            l[t] += sum;
         }
-        __syncthreads();
-        if (wave < half) {
-            const f32x4* from = sums + wave * SLOT;
+    }
+    __device__ __forceinline__ void values(const T* Vs) {
+#pragma unroll
+        for (int i = 0; i < NCH; ++i)
+#pragma unroll
+            for (int j = 0; j < NDB; ++j) {
+                const v8 a = S::col_op(Vs, 32 * i, 16 * j, g, li);
+#pragma unroll
+                for (int t = 0; t < MT; ++t) o[t][j] = M::mma(a, pb[t][i], o[t][j]);
+                if (j % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+            }
+    }
+    // maxima in log2 units and whole row sums, before partial sums meet
+    __device__ __forceinline__ void close() {
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            m[t] *= c;
+            l[t] = row4_sum(l[t]);
+        }
+    }
+    // Partial sums, or the rows themselves where the sequence is one run.  specials: V held
+    // infinities or NaN in a masked block.
+    __device__ __forceinline__ void store(const RowsParams& p, const RowsWork& w, const CachePages& pages, const T* V,
+                                          int rfirst, int tile0, int lane, bool specials) {
+        const int mine = min(16 * MT, w.nrows - rfirst);
+        auto row_at = [&](int key) -> const T* {
+            const int64_t at = pages.at(key, w.kend, p.vs.s, p.vs.b);
+            return at < 0 ? nullptr : V + at;
+        };
+        auto row_sees = [&](int key, int r) { return rows_see(p, w, (rfirst + r) / p.group, key); };
+        if (p.num_splits > 1) {
+            const int64_t part = ((int64_t)w.kv * p.nrb + w.rb) * p.num_splits + w.split;
+            const int rows = p.block_rows;
+            float* const po = p.part_o + (part * rows + 16 * tile0) * D;
+            float* const pm = p.part_ml + part * 2 * rows + 16 * tile0;
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
-                const float m2 = Ml[wave][t][0][li], l2 = Ml[wave][t][1][li];
-                const float mn = fmaxf(m[t], m2), ref = mn == OPS_NEG_INF ? 0.0f : mn;
-                const float c1 = ops_exp2(m[t] - ref), c2 = ops_exp2(m2 - ref);
-                m[t] = mn;
-                l[t] = l[t] * c1 + l2 * c2;
 #pragma unroll
-                for (int j = 0; j < NDB; ++j) o[t][j] = o[t][j] * c1 + from[(t * NDB + j) * 64 + lane] * c2;
+                for (int j = 0; j < NDB; ++j)
+                    *reinterpret_cast<f32x4*>(po + (16 * t + li) * D + 16 * j + 4 * g) = o[t][j];
+                if (g == 0) {
+                    pm[16 * t + li] = m[t];
+                    pm[rows + 16 * t + li] = l[t];
+                }
+            }
+            if (specials) {
+                __threadfence();
+                add_specials<T, float, true>(w.kbeg, w.kend, mine, p.d, lane, row_at, row_sees,
+                                             [&](int r) { return po + r * D; });
+            }
+            return;
+        }
+        auto out_row = [&](int r) {
+            const int h = w.hk * p.group + (rfirst + r) % p.group;
+            return reinterpret_cast<T*>(p.out) + w.b * p.os.b + h * p.os.h + (rfirst + r) / p.group * p.os.s;
+        };
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            const int r = rfirst + 16 * t + li;
+            if (r >= w.nrows) continue;
+            T* const out = out_row(16 * t + li);
+            const float inv = l[t] == 0.0f ? 0.0f : 1.0f / l[t];
+#pragma unroll
+            for (int j = 0; j < NDB; ++j) store4<T>(out, 16 * j + 4 * g, p.d, p.ovec, o[t][j] * inv);
+            if (p.lse && g == 0)
+                p.lse[((int64_t)w.b * p.heads + w.hk * p.group + r % p.group) * p.n + token[t]] =
+                    l[t] == 0.0f ? OPS_NEG_INF : (m[t] + __builtin_log2f(l[t]) - kProbLog2<T>) * kLn2;
+        }
+        if (specials) {
+            __threadfence();
+            add_specials<T, T, true>(w.kbeg, w.kend, mine, p.d, lane, row_at, row_sees, out_row);
+        }
+    }
+};
+
+__device__ __forceinline__ CachePages rows_pages(const RowsParams& p, int b) {
+    return {p.table ? p.table + (int64_t)b * p.pages_per_seq : nullptr, p.page_shift, (1 << p.page_shift) - 1, p.n_pages};
+}
+
+template <int N>
+__device__ __forceinline__ void wait_vmcnt() {
+    constexpr int n = N > 63 ? 63 : N;
+    __builtin_amdgcn_s_waitcnt(0x0f70 | (n & 15) | (n >> 4 << 14));
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+}
+
+// ---------------------------------------------------------------------------
+// Up to 16 MT rows, a wave 32-key blocks of its own.
+// ---------------------------------------------------------------------------
+template <typename T, int D, int MT, bool MOD>
+__device__ __forceinline__ void rows_stream(const RowsParams& p) {
+    constexpr int NW = kStreamWaves<D * (int)sizeof(T)>, SK = 32, TILE = SK * D;
+    using R = RowTiles<T, D, MT, 2, MOD>;
+    using Src = RowSource<T, D, SK, 1>;
+    constexpr int RUNS = Src::RUNS, NDB = R::NDB;
+    T* const K0 = lds_array<T, NW * TILE, 0>();
+    T* const V0 = lds_array<T, NW * TILE, 1>();
+    T* const K1 = lds_array<T, NW * TILE, 2>();
+    T* const V1 = lds_array<T, NW * TILE, 3>();
+    __shared__ float Ml[NW][MT][2][16];
+    __shared__ int any_special[NW];
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const RowsWork w = rows_work<SK>(p, 16 * MT);
+    const CachePages pages = rows_pages(p, w.b);
+    const T* const K = reinterpret_cast<const T*>(p.k) + w.hk * p.ks.h + (p.table ? 0 : w.b * p.ks.b);
+    const T* const V = reinterpret_cast<const T*>(p.v) + w.hk * p.vs.h + (p.table ? 0 : w.b * p.vs.b);
+    const Src ksrc(K, p.ks.s, p.ks.b, p.d, 0, lane), vsrc(V, p.vs.s, p.vs.b, p.d, 0, lane);
+    const int k_first = w.kbeg + SK * wave;
+    const int nblk = k_first < w.kend ? (w.kend - k_first + SK * NW - 1) / (SK * NW) : 0;
+    const bool dma = p.dma;
+
+    bool special = false;
+    R x;
+    auto pages_of = [&](int blk, int (&pg)[2]) {
+        const int k = k_first + blk * SK * NW;
+        const bool in = dma && blk < nblk;
+        pg[0] = in ? pages.page(k) : -1;
+        pg[1] = in && k + 16 < w.kend ? pages.page(k + 16) : -1;
+    };
+    auto fill = [&](const Src& src, T* dst, int blk, const int (&pg)[2]) {
+        src.fill(dst + wave * TILE, k_first + blk * SK * NW, w.kend, pg, pages, 0);
+    };
+    int pg0[2], pg1[2], pg2[2];
+    pages_of(0, pg0);
+    pages_of(1, pg1);
+    if (dma && nblk > 0) {
+        fill(ksrc, K0, 0, pg0);
+        fill(vsrc, V0, 0, pg0);
+    }
+    x.init(p, w, w.rfirst, lane);
+    if (dma && nblk > 0) {
+        // Q's loads are through before more DMA starts: only DMA is counted from here
+        wait_vmcnt<0>();
+        fill(ksrc, K1, 1, pg1);
+        fill(vsrc, V1, 1, pg1);
+    }
+    auto block = [&](int i, T* kb, T* vb) {
+        T* const Ks = kb + wave * TILE;
+        T* const Vs = vb + wave * TILE;
+        const int k0 = k_first + i * SK * NW;
+        bool bad = false;
+        if (dma) {
+            bad = pg0[0] < 0 || (pg0[1] < 0 && k0 + 16 < w.kend);
+            pages_of(i + 2, pg2);
+            wait_vmcnt<3 * RUNS>();
+        } else {
+            bool b = ksrc.fill_slow(Ks, k0, w.kend, pages, p.d, p.vec, lane);
+            b = vsrc.fill_slow(Vs, k0, w.kend, pages, p.d, p.vec, lane) || b;
+            bad = __builtin_amdgcn_ballot_w64(b) != 0;
+            reread();
+        }
+        const bool masked = bad || k0 + SK > min(w.open, w.kend);
+        x.scores(p, w, pages, Ks, k0, masked, bad);
+        if (dma) {
+            reread();
+            fill(ksrc, kb, i + 2, pg2);
+        }
+        x.softmax();
+        if (dma) wait_vmcnt<3 * RUNS>();
+        if (masked) {
+            special = Swizzled<T, D>::template clean<SK, 64>(Vs, lane) || special;
+            reread();
+        }
+        x.values(Vs);
+        reread();
+        if (dma) fill(vsrc, vb, i + 2, pg2);
+        pg0[0] = pg1[0], pg0[1] = pg1[1];
+        pg1[0] = pg2[0], pg1[1] = pg2[1];
+    };
+    for (int i = 0; i < nblk; i += 2) {
+        block(i, K0, V0);
+        if (i + 1 < nblk) block(i + 1, K1, V1);
+    }
+    x.close();
+    const bool any = __builtin_amdgcn_ballot_w64(special) != 0;
+    if (lane == 0) any_special[wave] = any;
+    if constexpr (NW > 1) {
+        // Join the waves' sums: the upper half leaves its own in LDS, the lower half adds them, and again.
+        // Each slot array is one wave's or more; the DMA into it has landed.
+        constexpr int SLOT = MT * NDB * 64;
+        static_assert(SLOT * 16 <= NW * TILE * (int)sizeof(T), "a wave's sums fit an array");
+        wait_vmcnt<0>();
+#pragma unroll
+        for (int half = NW / 2; half >= 1; half /= 2) {
+            __syncthreads();
+            auto slot = [&](int i) { return reinterpret_cast<f32x4*>(i == 0 ? K0 : V0); };
+            if (wave >= half && wave < 2 * half) {
+                f32x4* const to = slot(wave - half);
+#pragma unroll
+                for (int t = 0; t < MT; ++t) {
+#pragma unroll
+                    for (int j = 0; j < NDB; ++j) to[(t * NDB + j) * 64 + lane] = x.o[t][j];
+                    if (x.g == 0) {
+                        Ml[wave - half][t][0][x.li] = x.m[t];
+                        Ml[wave - half][t][1][x.li] = x.l[t];
+                    }
+                }
+            }
+            __syncthreads();
+            if (wave < half) {
+                const f32x4* const from = slot(wave);
+#pragma unroll
+                for (int t = 0; t < MT; ++t) {
+                    const float m2 = Ml[wave][t][0][x.li], l2 = Ml[wave][t][1][x.li];
+                    const float mn = fmaxf(x.m[t], m2), ref = mn == OPS_NEG_INF ? 0.0f : mn;
+                    const float c1 = ops_exp2(x.m[t] - ref), c2 = ops_exp2(m2 - ref);
+                    x.m[t] = mn;
+                    x.l[t] = x.l[t] * c1 + l2 * c2;
+#pragma unroll
+                    for (int j = 0; j < NDB; ++j) x.o[t][j] = x.o[t][j] * c1 + from[(t * NDB + j) * 64 + lane] * c2;
+                }
             }
         }
     }
@@ -241,77 +570,130 @@ __device__ __forceinline__ void rows_body(const RowsParams& p) {
     int specials = 0;
 #pragma unroll
     for (int i = 0; i < NW; ++i) specials |= any_special[i];
-    auto row_at = [&](int key) -> const T* {
-        const int64_t at = vrows.at(key);
-        return at < 0 ? nullptr : V + at;
-    };
-    auto row_sees = [&](int key, int r) { return sees((rfirst + r) / p.group, key); };
-    const int mine = min(16 * MT, nrows - rfirst);
+    x.store(p, w, pages, V, w.rfirst, 0, lane, specials != 0);
+}
 
-    if (p.num_splits > 1) {
-        const int64_t part = ((int64_t)kv * p.nrb + rb) * p.num_splits + split;
+// ---------------------------------------------------------------------------
+// Many rows: the waves share the keys.
+// ---------------------------------------------------------------------------
+template <typename T, int D, int MT, bool MOD>
+__device__ __forceinline__ void rows_shared(const RowsParams& p) {
+    constexpr int NW = 4, SK = sizeof(T) == 4 || D > 128 ? 32 : 64, TILE = SK * D, KB = SK / 16;
+    using R = RowTiles<T, D, MT, KB, MOD>;
+    using Src = RowSource<T, D, SK, NW>;
+    T* const Kb0 = lds_array<T, TILE, 0>();
+    T* const Vb0 = lds_array<T, TILE, 1>();
+    T* const Kb1 = lds_array<T, TILE, 2>();
+    T* const Vb1 = lds_array<T, TILE, 3>();
+    __shared__ int bad_any[2], Special;
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const RowsWork w = rows_work<SK>(p, 16 * MT * NW);
+    const CachePages pages = rows_pages(p, w.b);
+    const T* const K = reinterpret_cast<const T*>(p.k) + w.hk * p.ks.h + (p.table ? 0 : w.b * p.ks.b);
+    const T* const V = reinterpret_cast<const T*>(p.v) + w.hk * p.vs.h + (p.table ? 0 : w.b * p.vs.b);
+    const Src ksrc(K, p.ks.s, p.ks.b, p.d, wave, lane), vsrc(V, p.vs.s, p.vs.b, p.d, wave, lane);
+    const int nst = (w.kend - w.kbeg + SK - 1) / SK;
+    const int rfirst = w.rfirst + 16 * MT * wave;
+    const bool dma = p.dma, act = rfirst < w.nrows;
+
+    int pgk[SK / 16], pgv[SK / 16], pgn[SK / 16];   // pages of the current, next and after-next stage
+    auto pages_of = [&](int st, int (&pg)[SK / 16]) {
 #pragma unroll
-        for (int t = 0; t < MT; ++t) {
-            float* po = p.part_o + (part * 16 * MT + 16 * t + li) * D;
-#pragma unroll
-            for (int j = 0; j < NDB; ++j) *reinterpret_cast<f32x4*>(po + 16 * j + 4 * g) = o[t][j];
-            if (g == 0) {
-                p.part_ml[part * 32 * MT + 16 * t + li] = m[t];
-                p.part_ml[part * 32 * MT + 16 * MT + 16 * t + li] = l[t];
-            }
+        for (int i = 0; i < SK / 16; ++i) {
+            const int k = w.kbeg + st * SK + 16 * i;
+            pg[i] = dma && k < w.kend ? pages.page(k) : -1;
         }
-        if (specials) {
-            __threadfence();
-            add_specials<T, float, true>(kbeg, kend, mine, p.d, lane, row_at, row_sees,
-                                         [&](int r) { return p.part_o + (part * 16 * MT + r) * D; });
+    };
+    auto fill = [&](const Src& src, T* dst, int st, const int (&pg)[SK / 16], int parity) {
+        const int k0 = w.kbeg + st * SK;
+        if (dma) {
+            src.fill(dst, k0, w.kend, pg, pages, wave);
+        } else if (src.fill_slow(dst, k0, w.kend, pages, p.d, p.vec, tid)) {
+            bad_any[parity] = 1;
         }
-        return;
-    }
+    };
+    auto bad_stage = [&](int st, const int (&pg)[SK / 16], int parity) {
+        if (!dma) return bad_any[parity] != 0;
+        bool bad = false;
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
-        const int r = rfirst + 16 * t + li;
-        if (r >= nrows) continue;
-        const int h = hk * p.group + r % p.group;
-        T* out = reinterpret_cast<T*>(p.out) + b * p.os.b + h * p.os.h + token[t] * p.os.s;
-        const float inv = l[t] == 0.0f ? 0.0f : 1.0f / l[t];
+        for (int i = 0; i < SK / 16; ++i) bad = bad || (pg[i] < 0 && w.kbeg + st * SK + 16 * i < w.kend);
+        return bad;
+    };
+    if (tid == 0) bad_any[0] = bad_any[1] = Special = 0;
+    R x;
+    x.init(p, w, rfirst, lane);
+    if (!dma) __syncthreads();
+    pages_of(0, pgk);
+    pages_of(1, pgv);
+    if (nst > 0) {
+        fill(ksrc, Kb0, 0, pgk, 0);
+        fill(vsrc, Vb0, 0, pgk, 0);
+    }
+    if (nst > 1) fill(ksrc, Kb1, 1, pgv, 1);
+    wait_loads();
+    __syncthreads();
+    bool bad = false, masked = false;
+    auto score = [&](int st, const T* Ks, const int (&pg)[SK / 16], int parity) {
+        const int k0 = w.kbeg + st * SK;
+        bad = bad_stage(st, pg, parity);
+        masked = bad || k0 + SK > min(w.open, w.kend);
+        if (act) x.scores(p, w, pages, Ks, k0, masked, bad);
+    };
+    if (nst > 0) score(0, Kb0, pgk, 0);
+    __syncthreads();
+    auto step = [&](auto parity, int st) {
+        constexpr int P = decltype(parity)::value;
+        T* const k_cur = P ? Kb1 : Kb0;
+        T* const k_next = P ? Kb0 : Kb1;
+        T* const v_cur = P ? Vb1 : Vb0;
+        T* const v_next = P ? Vb0 : Vb1;
+        // pgv: the next stage's pages
+        if (st + 1 < nst) fill(vsrc, v_next, st + 1, pgv, 1 - P);
+        pages_of(st + 2, pgn);
+        if (st + 2 < nst) fill(ksrc, k_cur, st + 2, pgn, P);
+        if (masked && Swizzled<T, D>::template clean<SK, 64 * NW>(v_cur, tid)) Special = 1;
+        if (act) x.softmax();
+        if (masked) __syncthreads();
+        if (act) x.values(v_cur);
+        if (st + 1 < nst) score(st + 1, k_next, pgv, 1 - P);
+        wait_loads();
+        __syncthreads();
 #pragma unroll
-        for (int j = 0; j < NDB; ++j) store4<T>(out, 16 * j + 4 * g, p.d, p.ovec, o[t][j] * inv);
-        if (p.lse && g == 0)
-            p.lse[((int64_t)b * p.heads + h) * p.n + token[t]] =
-                l[t] == 0.0f ? OPS_NEG_INF : (m[t] + __builtin_log2f(l[t]) - kProbLog2<T>) * kLn2;
+        for (int i = 0; i < SK / 16; ++i) pgv[i] = pgn[i];
+    };
+    for (int st = 0; st < nst; st += 2) {
+        step(std::integral_constant<int, 0>{}, st);
+        if (st + 1 < nst) step(std::integral_constant<int, 1>{}, st + 1);
     }
-    if (specials) {
-        __threadfence();
-        add_specials<T, T, true>(kbeg, kend, mine, p.d, lane, row_at, row_sees, [&](int r) {
-            const int h = hk * p.group + (rfirst + r) % p.group;
-            return reinterpret_cast<T*>(p.out) + b * p.os.b + h * p.os.h + (rfirst + r) / p.group * p.os.s;
-        });
-    }
+    x.close();
+    if (act) x.store(p, w, pages, V, rfirst, MT * wave, lane, Special != 0);
 }
 
 // Joins the partial sums of a row, a wave a row, four columns a lane.
-template <typename T, int D, int ROWS>
+template <typename T, int D>
 __device__ __forceinline__ void rows_merge(const RowsParams& p) {
     const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
-    const int nrows = p.n * p.group;
+    const int nrows = p.n * p.group, rows = p.block_rows;
     if (row >= (int64_t)p.batch * p.kv_heads * nrows) return;
     const int kv = row / nrows, r = row % nrows;
     const int b = kv / p.kv_heads, h = kv % p.kv_heads * p.group + r % p.group, token = r / p.group;
-    const int64_t part = ((int64_t)kv * p.nrb + r / ROWS) * p.num_splits;
-    const float* ml = p.part_ml + part * 2 * ROWS + r % ROWS;
-    const float* po = p.part_o + (part * ROWS + r % ROWS) * D + 4 * lane;
+    const int64_t part = ((int64_t)kv * p.nrb + r / rows) * p.num_splits;
+    const float* const ml = p.part_ml + part * 2 * rows + r % rows;
+    const float* const po = p.part_o + (part * rows + r % rows) * D + 4 * lane;
     float mx = OPS_NEG_INF;
-    for (int s = lane; s < p.num_splits; s += 64) mx = fmaxf(mx, ml[(int64_t)s * 2 * ROWS]);
+    for (int s = lane; s < p.num_splits; s += 64) mx = fmaxf(mx, ml[(int64_t)s * 2 * rows]);
 #pragma unroll
     for (int s = 1; s < 64; s *= 2) mx = fmaxf(mx, __shfl_xor(mx, s));
     const float ref = mx == OPS_NEG_INF ? 0.0f : mx;
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
     float l = 0.0f;
+#pragma unroll 4
     for (int s = 0; s < p.num_splits; ++s) {
-        const float c = ops_exp2(ml[(int64_t)s * 2 * ROWS] - ref);
-        l += c * ml[(int64_t)s * 2 * ROWS + ROWS];
-        if (4 * lane < D) o += c * *reinterpret_cast<const f32x4*>(po + (int64_t)s * ROWS * D);
+        const float c = ops_exp2(ml[(int64_t)s * 2 * rows] - ref);
+        l += c * ml[(int64_t)s * 2 * rows + rows];
+        if (4 * lane < D) o += c * *reinterpret_cast<const f32x4*>(po + (int64_t)s * rows * D);
     }
     if (4 * lane < D)
         store4<T>(reinterpret_cast<T*>(p.out) + b * p.os.b + h * p.os.h + token * p.os.s, 4 * lane, p.d, p.ovec,
@@ -321,31 +703,41 @@ __device__ __forceinline__ void rows_merge(const RowsParams& p) {
             l == 0.0f ? OPS_NEG_INF : (mx + __builtin_log2f(l) - kProbLog2<T>) * kLn2;
 }
 
-#define ROWS_KERNELS(N, T, D, MT)                                                                               \
-    extern "C" __global__ __launch_bounds__((64 * RowsGeo<T, D>::NW)) void fa_rows_##N##_d##D##_t##MT(RowsParams p) { \
-        rows_body<T, D, MT>(p);                                                                                 \
-    }                                                                                                           \
-    extern "C" __global__ __launch_bounds__(256) void fa_rows_merge_##N##_d##D##_t##MT(RowsParams p) {          \
-        rows_merge<T, D, 16 * MT>(p);                                                                           \
+#define PASTE_(a, b, c, d) a##b##c##d
+#define PASTE(a, b, c, d) PASTE_(a, b, c, d)
+#define KERNEL(F, BODY, D, MT, MOD, TAG, THREADS, WAVES)                                                       \
+    extern "C" __global__ __launch_bounds__(THREADS, WAVES) void PASTE(F, OPS_NAME, _d##D##_t##MT, TAG)(RowsParams p) { \
+        BODY<OPS_T, D, MT, MOD>(p);                                                                            \
     }
-ROWS_KERNELS(bf16, __bf16, 64, 1)
-ROWS_KERNELS(bf16, __bf16, 64, 2)
-ROWS_KERNELS(bf16, __bf16, 64, 4)
-ROWS_KERNELS(bf16, __bf16, 128, 1)
-ROWS_KERNELS(bf16, __bf16, 128, 2)
-ROWS_KERNELS(bf16, __bf16, 128, 4)
-ROWS_KERNELS(bf16, __bf16, 256, 1)
-ROWS_KERNELS(bf16, __bf16, 256, 2)
-ROWS_KERNELS(f16, _Float16, 64, 1)
-ROWS_KERNELS(f16, _Float16, 64, 2)
-ROWS_KERNELS(f16, _Float16, 64, 4)
-ROWS_KERNELS(f16, _Float16, 128, 1)
-ROWS_KERNELS(f16, _Float16, 128, 2)
-ROWS_KERNELS(f16, _Float16, 128, 4)
-ROWS_KERNELS(f16, _Float16, 256, 1)
-ROWS_KERNELS(f16, _Float16, 256, 2)
-ROWS_KERNELS(f32, float, 64, 1)
-ROWS_KERNELS(f32, float, 64, 2)
-ROWS_KERNELS(f32, float, 128, 1)
-ROWS_KERNELS(f32, float, 128, 2)
-ROWS_KERNELS(f32, float, 256, 1)
+#define STREAM(D, MT)                                                                                    \
+    KERNEL(fa_rows_stream_, rows_stream, D, MT, false, , (64 * kStreamWaves<D * (int)sizeof(OPS_T)>), 1) \
+    KERNEL(fa_rows_stream_, rows_stream, D, MT, true, m, (64 * kStreamWaves<D * (int)sizeof(OPS_T)>), 1)
+#define SHARED(D, MT, WAVES)                                             \
+    KERNEL(fa_rows_shared_, rows_shared, D, MT, false, , 256, WAVES)     \
+    KERNEL(fa_rows_shared_, rows_shared, D, MT, true, m, 256, WAVES)
+#define MERGE(D)                                                                                          \
+    extern "C" __global__ __launch_bounds__(256) void PASTE(fa_rows_merge_, OPS_NAME, _d##D, )(RowsParams p) { \
+        rows_merge<OPS_T, D>(p);                                                                          \
+    }
+MERGE(64)
+MERGE(128)
+MERGE(256)
+STREAM(64, 1)
+STREAM(128, 1)
+STREAM(256, 1)
+#ifdef OPS_16BIT
+STREAM(64, 2)
+STREAM(64, 4)
+STREAM(128, 2)
+STREAM(128, 4)
+STREAM(256, 2)
+SHARED(64, 2, 2)
+SHARED(128, 2, 2)
+SHARED(256, 1, 2)
+#else
+STREAM(64, 2)
+STREAM(128, 2)
+SHARED(64, 1, 2)
+SHARED(128, 1, 2)
+SHARED(256, 1, 1)
+#endif

@@ -9,14 +9,16 @@
 
 namespace {
 
-enum OpsModule { kScoreModule, kCacheModule, kRotaryModule, kOpsModules };
+// Code objects: those of score attention and of the cache one a type (FA_DTYPE_*).
+enum OpsModule { kRotaryModule, kScoreModule, kCacheModule = kScoreModule + 3, kOpsModules = kCacheModule + 3 };
+OpsModule of_type(OpsModule m, int dtype) { return static_cast<OpsModule>(m + dtype); }
 
 struct OpsState {
     std::once_flag once[kOpsModules];
     int status[kOpsModules] = {};
     hipModule_t module[kOpsModules] = {};
     std::mutex mu;
-    std::unordered_map<std::string, hipFunction_t> fns;
+    std::unordered_map<std::string, hipFunction_t> fns[kOpsModules];
 };
 
 OpsState g_ops[kMaxDevices];
@@ -28,7 +30,9 @@ constexpr int64_t kOpsMaxStride = int64_t(1) << 44;
 constexpr size_t kTreeMaxTokens = 256;
 
 int ops_module(int dev, OpsModule which) {
-    static const char* const files[] = {"fa_score.hsaco", "fa_cache.hsaco", "fa_rotary.hsaco"};
+    static const char* const files[] = {"fa_rotary.hsaco",     "fa_score_f32.hsaco",  "fa_score_bf16.hsaco",
+                                        "fa_score_f16.hsaco",  "fa_cache_f32.hsaco",  "fa_cache_bf16.hsaco",
+                                        "fa_cache_f16.hsaco"};
     OpsState& s = g_ops[dev];
     std::call_once(s.once[which], [&] {
         std::string path = module_path();
@@ -55,15 +59,15 @@ int ops_launch(int dev, OpsModule which, const char* name, size_t grid, unsigned
     hipFunction_t fn = nullptr;
     {
         std::lock_guard<std::mutex> lock(s.mu);
-        auto it = s.fns.find(name);
-        if (it != s.fns.end()) {
+        auto it = s.fns[which].find(name);
+        if (it != s.fns[which].end()) {
             fn = it->second;
         } else {
             if (hipModuleGetFunction(&fn, s.module[which], name) != hipSuccess) {
                 (void)hipGetLastError();
                 return FA_ERR_MODULE;
             }
-            s.fns.emplace(name, fn);
+            s.fns[which].emplace(name, fn);
         }
     }
     void* args[] = {p};
@@ -184,47 +188,67 @@ constexpr size_t kOpsMaxGrid = size_t(1) << 22;   // workgroups: threads of a la
 
 size_t doc_tiles(size_t n) { return (n + kDocTile - 1) / kDocTile; }
 
-// Fewest-row plan: key splits of the rows kernel.
+// Plan of the rows kernels: streaming waves up to 64 rows (as far as registers go), else
+// workgroups that share their keys; the keys in as many runs as fill the GPU.
 struct RowsPlan {
-    int mt, nw, nrb, splits;
+    bool stream;
+    int mt, threads, rows, nrb, splits;
     size_t floats;
 };
 RowsPlan plan_rows(int dtype, int D, size_t nkv, size_t rows, size_t keys, int num_cus) {
     RowsPlan r{};
     const bool f32 = dtype == FA_DTYPE_F32;
-    const int most = f32 ? (D > 128 ? 1 : 2) : (D > 128 ? 2 : 4);
-    r.mt = rows <= 16 ? 1 : rows <= 32 ? std::min(2, most) : most;
-    r.nw = f32 && D > 128 ? 2 : 4;
-    r.nrb = static_cast<int>((rows + 16 * r.mt - 1) / (16 * r.mt));
-    const size_t units = nkv * r.nrb;
-    size_t splits = std::max<size_t>(1, 2 * static_cast<size_t>(num_cus) / std::max<size_t>(units, 1));
-    splits = std::min(splits, std::max<size_t>(1, keys / (32 * r.nw)));
+    const int row_bytes = D * static_cast<int>(elem_size(dtype));
+    const int most = f32 ? (D > 128 ? 1 : 2) : (D > 128 ? 2 : 4);   // tiles a streaming wave
+    r.stream = rows <= static_cast<size_t>(16 * most);
+    size_t step;
+    if (r.stream) {
+        r.mt = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+        const int waves = row_bytes <= 256 ? kStreamWaves<256> : row_bytes <= 512 ? kStreamWaves<512> : kStreamWaves<1024>;
+        r.threads = 64 * waves;
+        r.rows = 16 * r.mt;
+        step = 32 * waves;
+    } else {
+        r.mt = f32 || D > 128 ? 1 : 2;
+        r.threads = 256;
+        r.rows = 64 * r.mt;
+        step = f32 || D > 128 ? 32 : 64;
+    }
+    r.nrb = static_cast<int>((rows + r.rows - 1) / r.rows);
+    const size_t units = std::max<size_t>(nkv * r.nrb, 1);
+    size_t splits = std::max<size_t>(1, 2 * static_cast<size_t>(num_cus) / units);
+    splits = std::min(splits, std::max<size_t>(1, keys / step));
     r.splits = static_cast<int>(std::min<size_t>(splits, 256));
-    r.floats = r.splits > 1 ? units * r.splits * 16 * r.mt * (D + 2) : 0;
+    r.floats = r.splits > 1 ? units * r.splits * r.rows * (D + 2) : 0;
     return r;
 }
 
 int run_rows(int dev, hipStream_t stream, int dtype, int D, RowsParams* p, size_t keys) {
+    const OpsModule module = of_type(kCacheModule, dtype);
+    int rc = ops_module(dev, module);
+    if (rc != FA_OK) return rc;
     const size_t nkv = static_cast<size_t>(p->batch) * p->kv_heads;
     const size_t rows = static_cast<size_t>(p->n) * p->group;
     const RowsPlan plan = plan_rows(dtype, D, nkv, rows, keys, g_dev[dev].num_cus);
     p->nrb = plan.nrb;
     p->num_splits = plan.splits;
+    p->block_rows = plan.rows;
+    p->dma = p->vec && (!p->table || p->page_shift >= 4);
     const size_t grid = nkv * plan.nrb * plan.splits, mgrid = (nkv * rows + 3) / 4;
     if (grid > kOpsMaxGrid || mgrid > kOpsMaxGrid) return FA_ERR_UNSUPPORTED;
     OpsWorkspace ws;
     if (plan.floats) {
-        const int rc = ws.get(dev, stream, plan.floats * sizeof(float));
-        if (rc != FA_OK) return rc;
+        if ((rc = ws.get(dev, stream, plan.floats * sizeof(float))) != FA_OK) return rc;
         p->part_o = static_cast<float*>(ws.ptr);
-        p->part_ml = p->part_o + nkv * plan.nrb * plan.splits * 16 * plan.mt * D;
+        p->part_ml = p->part_o + nkv * plan.nrb * plan.splits * plan.rows * D;
     }
     char name[64];
-    std::snprintf(name, sizeof(name), "fa_rows_%s_d%d_t%d", dtype_name(dtype), D, plan.mt);
-    int rc = ops_launch(dev, kCacheModule, name, grid, 64 * plan.nw, p, stream);
+    std::snprintf(name, sizeof(name), "fa_rows_%s_%s_d%d_t%d%s", plan.stream ? "stream" : "shared", dtype_name(dtype), D,
+                  plan.mt, p->slopes || p->cap_log2e != 0.0f ? "m" : "");
+    rc = ops_launch(dev, module, name, grid, plan.threads, p, stream);
     if (rc == FA_OK && plan.splits > 1) {
-        std::snprintf(name, sizeof(name), "fa_rows_merge_%s_d%d_t%d", dtype_name(dtype), D, plan.mt);
-        rc = ops_launch(dev, kCacheModule, name, mgrid, 256, p, stream);
+        std::snprintf(name, sizeof(name), "fa_rows_merge_%s_d%d", dtype_name(dtype), D);
+        rc = ops_launch(dev, module, name, mgrid, 256, p, stream);
     }
     return ws.done(stream, rc);
 }
@@ -268,11 +292,11 @@ void fill_score(const fa_score_config& c, const ScoreScale& sc, ScoreParams* p) 
     p->cap_log2e = sc.cap_log2e;
 }
 
-int launch_doc_ranges(int dev, hipStream_t stream, ScoreParams* p, int32_t* ws) {
+int launch_doc_ranges(int dev, OpsModule module, hipStream_t stream, ScoreParams* p, int32_t* ws) {
     const size_t tiles = static_cast<size_t>(p->batch) * (doc_tiles(p->sq) + doc_tiles(p->sk));
     p->q_rng = ws;
     p->k_rng = ws + 2 * static_cast<size_t>(p->batch) * doc_tiles(p->sq);
-    return ops_launch(dev, kScoreModule, "fa_score_doc_ranges", (tiles + 3) / 4, 256, p, stream);
+    return ops_launch(dev, module, "fa_score_doc_ranges", (tiles + 3) / 4, 256, p, stream);
 }
 size_t doc_range_bytes(const fa_score_config& c) {
     return c.q_doc ? 2 * sizeof(int32_t) * c.batch * (doc_tiles(c.seq_len_q) + doc_tiles(c.seq_len_k)) : 0;
@@ -371,13 +395,12 @@ int fa_score_forward(void* stream_, const fa_score_config* c, const void* q, con
     if (c->batch * c->heads > kOpsMaxGrid || (c->seq_len_q + 63) / 64 * c->batch * c->heads > kOpsMaxGrid)
         return FA_ERR_UNSUPPORTED;
     int dev;
-    if ((rc = ops_begin(&dev, kScoreModule)) != FA_OK) return rc;
+    if ((rc = ops_begin(&dev, of_type(kScoreModule, c->dtype))) != FA_OK) return rc;
     const hipStream_t stream = static_cast<hipStream_t>(stream_);
     const bool vec = vec_ok(q, lq, d) && vec_ok(k, lk, d) && vec_ok(v, lv, d);
     const bool ovec = ovec_ok(out, lo, es);
 
     if (score_takes_rows(*c, g_dev[dev].num_cus)) {
-        if ((rc = ops_module(dev, kCacheModule)) != FA_OK) return rc;
         RowsParams p{};
         p.q = q, p.k = k, p.v = v, p.out = out, p.lse = lse;
         p.slopes = c->slopes, p.q_doc = c->q_doc, p.k_doc = c->k_doc, p.prefix = c->causal ? c->prefix : nullptr;
@@ -400,13 +423,13 @@ int fa_score_forward(void* stream_, const fa_score_config* c, const void* q, con
     OpsWorkspace ws;
     if (c->q_doc) {
         if ((rc = ws.get(dev, stream, doc_range_bytes(*c))) != FA_OK) return rc;
-        rc = launch_doc_ranges(dev, stream, &p, static_cast<int32_t*>(ws.ptr));
+        rc = launch_doc_ranges(dev, of_type(kScoreModule, c->dtype), stream, &p, static_cast<int32_t*>(ws.ptr));
     }
     if (rc == FA_OK) {
         char name[64];
         std::snprintf(name, sizeof(name), "fa_score_forward_%s_d%d_t%d%s", dtype_name(c->dtype), D, mt,
                       c->slopes || c->softcap > 0.0f ? "m" : "");
-        rc = ops_launch(dev, kScoreModule, name, c->batch * c->heads * p.nqb, 256, &p, stream);
+        rc = ops_launch(dev, of_type(kScoreModule, c->dtype), name, c->batch * c->heads * p.nqb, 256, &p, stream);
     }
     return ws.done(stream, rc);
 }
@@ -438,7 +461,7 @@ int fa_score_backward(void* stream_, const fa_score_config* c, const void* q, co
         (sk + 63) / 64 * c->batch * c->kv_heads > kOpsMaxGrid || dgrid > 4 * kOpsMaxGrid)
         return FA_ERR_UNSUPPORTED;
     int dev;
-    if ((rc = ops_begin(&dev, kScoreModule)) != FA_OK) return rc;
+    if ((rc = ops_begin(&dev, of_type(kScoreModule, c->dtype))) != FA_OK) return rc;
     const hipStream_t stream = static_cast<hipStream_t>(stream_);
     ScoreParams p{};
     fill_score(*c, sc, &p);
@@ -454,23 +477,23 @@ int fa_score_backward(void* stream_, const fa_score_config* c, const void* q, co
     p.lse2 = static_cast<float*>(ws.ptr);
     p.delta = p.lse2 + rows;
     char name[64];
-    if (c->q_doc) rc = launch_doc_ranges(dev, stream, &p, reinterpret_cast<int32_t*>(p.delta + rows));
+    if (c->q_doc) rc = launch_doc_ranges(dev, of_type(kScoreModule, c->dtype), stream, &p, reinterpret_cast<int32_t*>(p.delta + rows));
     if (rc == FA_OK) {
         std::snprintf(name, sizeof(name), "fa_score_delta_%s", dtype_name(c->dtype));
-        rc = ops_launch(dev, kScoreModule, name, dgrid, 256, &p, stream);
+        rc = ops_launch(dev, of_type(kScoreModule, c->dtype), name, dgrid, 256, &p, stream);
     }
     const char* mod = c->slopes || c->softcap > 0.0f ? "m" : "";
     if (rc == FA_OK && (dk || dv)) {
         const int mt = score_tiles(c->dtype, D, sk, c->batch * c->kv_heads, 1, g_dev[dev].num_cus);
         p.nqb = static_cast<int>((sk + 64 * mt - 1) / (64 * mt));
         std::snprintf(name, sizeof(name), "fa_score_dkv_%s_d%d_t%d%s", dtype_name(c->dtype), D, mt, mod);
-        rc = ops_launch(dev, kScoreModule, name, c->batch * c->kv_heads * p.nqb, 256, &p, stream);
+        rc = ops_launch(dev, of_type(kScoreModule, c->dtype), name, c->batch * c->kv_heads * p.nqb, 256, &p, stream);
     }
     if (rc == FA_OK && dq) {
         const int mt = score_tiles(c->dtype, D, sq, c->batch * c->heads, 2, g_dev[dev].num_cus);
         p.nqb = static_cast<int>((sq + 64 * mt - 1) / (64 * mt));
         std::snprintf(name, sizeof(name), "fa_score_dq_%s_d%d_t%d%s", dtype_name(c->dtype), D, mt, mod);
-        rc = ops_launch(dev, kScoreModule, name, c->batch * c->heads * p.nqb, 256, &p, stream);
+        rc = ops_launch(dev, of_type(kScoreModule, c->dtype), name, c->batch * c->heads * p.nqb, 256, &p, stream);
     }
     return ws.done(stream, rc);
 }
@@ -648,7 +671,7 @@ int fa_tree_attention(void* stream, const fa_tree_config* c, const fa_kv_cache* 
     p.ovec = ovec_ok(out, lo, es);
     p.scale = sc.scale, p.scale_log2e = sc.scale_log2e, p.cap_in = sc.cap_in, p.cap_log2e = sc.cap_log2e;
     int dev;
-    if ((rc = ops_begin(&dev, kCacheModule)) != FA_OK) return rc;
+    if ((rc = ops_begin(&dev, of_type(kCacheModule, cache->dtype))) != FA_OK) return rc;
     return run_rows(dev, static_cast<hipStream_t>(stream), cache->dtype, ops_pad_d(d), &p, capacity);
 }
 

@@ -35,12 +35,17 @@ struct ScoreParams {
     float cap_log2e;          // softcap * log2(e); 0: no cap
 };
 
+// Waves of a workgroup of the streaming rows kernel, by the bytes of a padded row: each has
+// two slots of 32 rows of K and V in LDS.
+template <int ROW>
+constexpr int kStreamWaves = ROW <= 256 ? 4 : ROW <= 512 ? 2 : 1;
+
 // Attention of few rows over a long key range, keys split over workgroups.
 struct RowsParams {
     const void *q, *k, *v;
     void* out;
     float* lse;               // [batch, heads, n] or NULL
-    float *part_o, *part_ml;  // [slot][16 MT rows][D], [slot][2][16 MT]
+    float *part_o, *part_ml;  // [slot][block_rows][D], [slot][2][block_rows]
     const float* slopes;
     const int32_t *q_doc, *k_doc, *prefix;   // score attention
     const int32_t *lens, *table, *pos;       // tree attention (lens != NULL)
@@ -51,7 +56,9 @@ struct RowsParams {
     int page_shift, n_pages, pages_per_seq;
     int mask_words, mask_shared;
     int nrb, num_splits;      // row blocks of a (batch, kv head), splits of its keys
+    int block_rows;
     int vec, ovec;
+    int dma;                  // K and V by DMA: 16-byte aligned rows, pages of 16 rows or more
     float scale, scale_log2e, cap_in, cap_log2e;
 };
 

@@ -12,6 +12,9 @@
 // lane tests one (causal and prefix bounds, document ranges), and two ballots give the
 // tiles to visit and those of them that need the mask element by element.
 
+//
+// Built once a type: OPS_T the element type, OPS_NAME its name in the kernels'.
+
 #include "fa_ops_common.h"
 
 template <typename T>
@@ -93,20 +96,31 @@ __device__ __forceinline__ bool pair_seen(const ScoreParams& p, const ScoreMask&
     return d >= 0 && d == p.k_doc[(int64_t)b * p.sk + key];
 }
 
-// (min, max) document of rows [r0, r1) from the range table (the tiles they touch).
-__device__ __forceinline__ void doc_range(const int32_t* rng, int r0, int r1, int* lo, int* hi) {
-    *lo = 0x7fffffff;
-    *hi = -0x7fffffff - 1;
+// Documents of a run of rows: the range of their ids, and whether there is padding among them.
+struct DocRange {
+    int lo, hi;
+    bool padding;
+};
+__device__ __forceinline__ DocRange doc_range(const int32_t* rng, int tile) {
+    const int lo = rng[2 * tile];
+    return {lo < 0 ? ~lo : lo, rng[2 * tile + 1], lo < 0};
+}
+// Of rows [r0, r1): of the tiles they touch.
+__device__ __forceinline__ DocRange doc_range(const int32_t* rng, int r0, int r1) {
+    DocRange x = {0x7fffffff, -1, false};
     for (int t = r0 / kDocTile; t <= (r1 - 1) / kDocTile; ++t) {
-        *lo = min(*lo, rng[2 * t]);
-        *hi = max(*hi, rng[2 * t + 1]);
+        const DocRange y = doc_range(rng, t);
+        x.lo = min(x.lo, y.lo);
+        x.hi = max(x.hi, y.hi);
+        x.padding = x.padding || y.padding;
     }
+    return x;
 }
 
-// Pairs of two row ranges whose documents lie in [alo, ahi] and [blo, bhi].
-__device__ __forceinline__ bool docs_meet(int alo, int ahi, int blo, int bhi, bool* part) {
-    if (!(alo == ahi && blo == bhi && alo == blo && alo >= 0)) *part = true;
-    return alo <= bhi && blo <= ahi && ahi >= 0 && bhi >= 0;
+// Whether rows of two runs may share a document; *part: whether some pair may not.
+__device__ __forceinline__ bool docs_meet(const DocRange& a, const DocRange& b, bool* part) {
+    if (a.padding || b.padding || !(a.lo == a.hi && b.lo == b.hi && a.lo == b.lo)) *part = true;
+    return a.lo <= b.hi && b.lo <= a.hi;
 }
 
 // One value a lane from global memory into LDS, zero past n.
@@ -120,11 +134,11 @@ __device__ __forceinline__ void fill_words(void* dst, const void* src, int n, in
 template <typename T, int D>
 constexpr int kStageKeys = sizeof(T) == 4 || D > 128 ? 32 : 64;
 
-// Whether queries [q0, q1), of documents qlo .. qhi, see a key of stage st, and whether
+// Whether queries [q0, q1), of the documents qr, see a key of stage st, and whether
 // some pair is hidden.
 template <int SK>
 __device__ __forceinline__ bool key_stage(const ScoreParams& p, const ScoreMask& mask, int st, int q0, int q1, bool docs,
-                                          int qlo, int qhi, const int32_t* krng, bool* part) {
+                                          const DocRange& qr, const int32_t* krng, bool* part) {
     const int k0 = st * SK, k1 = k0 + SK;
     bool v = true;
     if (k1 > p.sk) *part = true;
@@ -132,7 +146,7 @@ __device__ __forceinline__ bool key_stage(const ScoreParams& p, const ScoreMask&
         v = k0 <= p.q_start + q1 - 1 || k0 < mask.prefix;
         if (!(k1 - 1 <= p.q_start + q0 || k1 <= mask.prefix)) *part = true;
     }
-    if (docs && v) v = docs_meet(qlo, qhi, krng[k0 / kDocTile * 2], krng[k0 / kDocTile * 2 + 1], part);
+    if (docs && v) v = docs_meet(qr, doc_range(krng, k0 / kDocTile), part);
     return v;
 }
 
@@ -191,13 +205,13 @@ __device__ __forceinline__ void score_forward(const ScoreParams& p) {
     }
 
     const int q1 = min(q0 + BQ, p.sq);
-    int qlo = 0, qhi = 0;
+    DocRange qr = {};
     const int32_t* krng = nullptr;
     if (docs) {
-        doc_range(p.q_rng + (int64_t)w.b * 2 * ((p.sq + kDocTile - 1) / kDocTile), q0, q1, &qlo, &qhi);
+        qr = doc_range(p.q_rng + (int64_t)w.b * 2 * ((p.sq + kDocTile - 1) / kDocTile), q0, q1);
         krng = p.k_rng + (int64_t)w.b * 2 * ((p.sk + kDocTile - 1) / kDocTile);
     }
-    auto test = [&](int st, bool* part) -> bool { return key_stage<SK>(p, mask, st, q0, q1, docs, qlo, qhi, krng, part); };
+    auto test = [&](int st, bool* part) -> bool { return key_stage<SK>(p, mask, st, q0, q1, docs, qr, krng, part); };
     Stages<decltype(test)> stages((p.sk + SK - 1) / SK, lane, test);
     const Fill kfill(p.ks.s, p.d, p.vec, wave, lane), vfill(p.vs.s, p.d, p.vec, wave, lane);
     auto fill_k = [&](int st, T* dst, int* ids) {
@@ -517,13 +531,13 @@ __device__ __forceinline__ void score_dq(const ScoreParams& p) {
         for (int j = 0; j < NDB; ++j) dq[t][j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
     }
     const int q1 = min(q0 + BQ, p.sq);
-    int qlo = 0, qhi = 0;
+    DocRange qr = {};
     const int32_t* krng = nullptr;
     if (docs) {
-        doc_range(p.q_rng + (int64_t)w.b * 2 * ((p.sq + kDocTile - 1) / kDocTile), q0, q1, &qlo, &qhi);
+        qr = doc_range(p.q_rng + (int64_t)w.b * 2 * ((p.sq + kDocTile - 1) / kDocTile), q0, q1);
         krng = p.k_rng + (int64_t)w.b * 2 * ((p.sk + kDocTile - 1) / kDocTile);
     }
-    auto test = [&](int st, bool* part) -> bool { return key_stage<SK>(p, mask, st, q0, q1, docs, qlo, qhi, krng, part); };
+    auto test = [&](int st, bool* part) -> bool { return key_stage<SK>(p, mask, st, q0, q1, docs, qr, krng, part); };
     Stages<decltype(test)> stages((p.sk + SK - 1) / SK, lane, test);
     const Fill kfill(p.ks.s, p.d, p.vec, wave, lane), vfill(p.vs.s, p.d, p.vec, wave, lane);
     auto fill = [&](int st, T* k, T* v, int* ids) {
@@ -687,10 +701,10 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
         for (int j = 0; j < NDB; ++j) dk[t][j] = dv[t][j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
     }
     const int kend = min(kbeg + BK, p.sk);
-    int klo = 0, khi = 0;
+    DocRange kr = {};
     const int32_t* qrng = nullptr;
     if (docs) {
-        doc_range(p.k_rng + (int64_t)w.b * 2 * ((p.sk + kDocTile - 1) / kDocTile), kbeg, kend, &klo, &khi);
+        kr = doc_range(p.k_rng + (int64_t)w.b * 2 * ((p.sk + kDocTile - 1) / kDocTile), kbeg, kend);
         qrng = p.q_rng + (int64_t)w.b * 2 * ((p.sq + kDocTile - 1) / kDocTile);
     }
     auto test = [&](int st, bool* part) -> bool {
@@ -700,7 +714,7 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
             v = p.q_start + q1 - 1 >= kbeg || kbeg < mask.prefix;
             if (!(p.q_start + q0 >= kend - 1 || kend <= mask.prefix)) *part = true;
         }
-        if (docs && v) v = docs_meet(klo, khi, qrng[q0 / kDocTile * 2], qrng[q0 / kDocTile * 2 + 1], part);
+        if (docs && v) v = docs_meet(kr, doc_range(qrng, q0 / kDocTile), part);
         return v;
     };
     const int nst = (p.sq + SQ - 1) / SQ;
@@ -864,7 +878,8 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
 }
 
 // ---------------------------------------------------------------------------
-// (min, max) document of every kDocTile tokens, a wave a tile.
+// Range of the ids of every kDocTile tokens, a wave a tile: (min, max) of those that are not padding,
+// the min with all bits flipped where there is padding (none but padding: min 2^31 - 1, max -1).
 extern "C" __global__ __launch_bounds__(256) void fa_score_doc_ranges(ScoreParams p) {
     const int qt = (p.sq + kDocTile - 1) / kDocTile, kt = (p.sk + kDocTile - 1) / kDocTile;
     const int tile = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -873,7 +888,9 @@ extern "C" __global__ __launch_bounds__(256) void fa_score_doc_ranges(ScoreParam
     const bool isq = t < qt;
     const int at = (isq ? t : t - qt) * kDocTile + lane, n = isq ? p.sq : p.sk;
     const int32_t* ids = (isq ? p.q_doc : p.k_doc) + (int64_t)b * n;
-    int lo = at < n ? ids[at] : 0x7fffffff, hi = at < n ? lo : -0x7fffffff - 1;
+    const int id = at < n ? ids[at] : 0;
+    const bool padding = __builtin_amdgcn_ballot_w64(id < 0) != 0;
+    int lo = at < n && id >= 0 ? id : 0x7fffffff, hi = at < n ? max(id, -1) : -1;
 #pragma unroll
     for (int s = 1; s < 64; s *= 2) {
         lo = min(lo, __shfl_xor(lo, s));
@@ -881,47 +898,41 @@ extern "C" __global__ __launch_bounds__(256) void fa_score_doc_ranges(ScoreParam
     }
     if (lane == 0) {
         int32_t* rng = isq ? p.q_rng + 2 * ((int64_t)b * qt + t) : p.k_rng + 2 * ((int64_t)b * kt + t - qt);
-        rng[0] = lo;
+        rng[0] = padding ? ~lo : lo;
         rng[1] = hi;
     }
 }
 
-#define SCORE_TYPE(N, T)                                                                                    \
-    extern "C" __global__ __launch_bounds__(256) void fa_score_delta_##N(ScoreParams p) { score_delta<T>(p); }
-#define SCORE_KERNEL(F, N, T, D, MT, WAVES)                                                                 \
-    extern "C" __global__ __launch_bounds__(256, WAVES) void fa_score_##F##_##N##_d##D##_t##MT(ScoreParams p) { \
-        score_##F<T, D, MT, false>(p);                                                                      \
-    }                                                                                                       \
-    extern "C" __global__ __launch_bounds__(256, WAVES) void fa_score_##F##_##N##_d##D##_t##MT##m(ScoreParams p) { \
-        score_##F<T, D, MT, true>(p);                                                                       \
+#define PASTE_(a, b, c, d) a##b##c##d
+#define PASTE(a, b, c, d) PASTE_(a, b, c, d)
+extern "C" __global__ __launch_bounds__(256) void PASTE(fa_score_delta_, OPS_NAME, , )(ScoreParams p) {
+    score_delta<OPS_T>(p);
+}
+#define KERNEL(F, D, MT, MOD, TAG, WAVES)                                                             \
+    extern "C" __global__ __launch_bounds__(256, WAVES) void PASTE(fa_score_##F##_, OPS_NAME, _d##D##_t##MT, TAG)( \
+        ScoreParams p) {                                                                              \
+        score_##F<OPS_T, D, MT, MOD>(p);                                                              \
     }
-#define SCORE_KERNELS_16(N, T)             \
-    SCORE_KERNEL(forward, N, T, 64, 1, 2)  \
-    SCORE_KERNEL(forward, N, T, 64, 2, 2)  \
-    SCORE_KERNEL(forward, N, T, 128, 1, 2) \
-    SCORE_KERNEL(forward, N, T, 128, 2, 2) \
-    SCORE_KERNEL(forward, N, T, 256, 1, 2) \
-    SCORE_KERNEL(dq, N, T, 64, 1, 2)       \
-    SCORE_KERNEL(dq, N, T, 64, 2, 2)       \
-    SCORE_KERNEL(dq, N, T, 128, 1, 2)      \
-    SCORE_KERNEL(dq, N, T, 128, 2, 2)      \
-    SCORE_KERNEL(dq, N, T, 256, 1, 2)      \
-    SCORE_KERNEL(dkv, N, T, 64, 1, 2)      \
-    SCORE_KERNEL(dkv, N, T, 64, 2, 2)      \
-    SCORE_KERNEL(dkv, N, T, 128, 1, 2)     \
-    SCORE_KERNEL(dkv, N, T, 128, 2, 1)     \
-    SCORE_KERNEL(dkv, N, T, 256, 1, 1)
-SCORE_TYPE(bf16, __bf16)
-SCORE_TYPE(f16, _Float16)
-SCORE_TYPE(f32, float)
-SCORE_KERNELS_16(bf16, __bf16)
-SCORE_KERNELS_16(f16, _Float16)
-SCORE_KERNEL(forward, f32, float, 64, 1, 2)
-SCORE_KERNEL(forward, f32, float, 128, 1, 2)
-SCORE_KERNEL(forward, f32, float, 256, 1, 1)
-SCORE_KERNEL(dq, f32, float, 64, 1, 2)
-SCORE_KERNEL(dq, f32, float, 128, 1, 2)
-SCORE_KERNEL(dq, f32, float, 256, 1, 1)
-SCORE_KERNEL(dkv, f32, float, 64, 1, 2)
-SCORE_KERNEL(dkv, f32, float, 128, 1, 2)
-SCORE_KERNEL(dkv, f32, float, 256, 1, 1)
+#define KERNELS(F, D, MT, WAVES)       \
+    KERNEL(F, D, MT, false, , WAVES)   \
+    KERNEL(F, D, MT, true, m, WAVES)
+KERNELS(forward, 64, 1, 2)
+KERNELS(forward, 128, 1, 2)
+KERNELS(dq, 64, 1, 2)
+KERNELS(dq, 128, 1, 2)
+KERNELS(dkv, 64, 1, 2)
+KERNELS(dkv, 128, 1, 2)
+KERNELS(dkv, 256, 1, 1)
+#ifdef OPS_16BIT
+KERNELS(forward, 64, 2, 2)
+KERNELS(forward, 128, 2, 2)
+KERNELS(forward, 256, 1, 2)
+KERNELS(dq, 64, 2, 2)
+KERNELS(dq, 128, 2, 2)
+KERNELS(dq, 256, 1, 2)
+KERNELS(dkv, 64, 2, 2)
+KERNELS(dkv, 128, 2, 1)
+#else
+KERNELS(forward, 256, 1, 1)
+KERNELS(dq, 256, 1, 1)
+#endif

@@ -459,3 +459,11 @@ def test_tree_graph_replays_and_two_streams():
         torch.cuda.synchronize()
         for c in cases + [extra]:
             c.check()
+
+
+@pytest.mark.parametrize("n", (63, 64, 65, 128, 256))
+def test_chains_longer_than_a_mask_word(n):
+    """No mask: token i sees tokens up to i, also past the first 64."""
+    c = Tree("bf16", [40, 7], 2, 2, n, 64, mask="chain", seed=n)
+    c.run()
+    c.check()
