@@ -80,39 +80,46 @@ struct RowSource {
         : base(b), seq(seq_), batch(batch_) {
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
-            const int run = i * NW + wave, q = lane / S::CPR;
-            const int col = ((lane % S::CPR) ^ ((run * S::RPR + q) % S::CM)) * S::E;
-            voff[i] = col < d ? (int)(q * seq + col) * (int)sizeof(T) : 0x7ffffff0;
+            const int row = (i * NW + wave) * S::RPR + lane / S::CPR;
+            const int col = ((lane % S::CPR) ^ (row % S::CM)) * S::E;
+            voff[i] = col < d ? (int)(row % 16 * seq + col) * (int)sizeof(T) : 0x7ffffff0;   // in its 16-row group
         }
     }
-    // DMA of rows [k0, k0 + ROWS), zeros at and past `end` and where a page is bad; pages of 16 rows or more
+    // DMA of rows [k0, k0 + ROWS), zeros at and past `end` and where a page is bad; pages of 16 rows or more:
+    // a 16-row group lies in one page
     template <typename Cache>
     __device__ __forceinline__ void fill(T* dst, int k0, int end, const int (&page)[ROWS / 16], const Cache& c,
                                          int wave) const {
+        constexpr int kStep = NW * S::RPR;   // rows of the waves' i-th runs
+        __amdgpu_buffer_rsrc_t rs;
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
-            const int run = i * NW + wave, r0 = run * S::RPR, row = k0 + r0;
-            constexpr int kStep = NW * S::RPR;   // rows of the waves' i-th runs: in one 16-row group, or in two
-            int pg = page[i * kStep / 16];
-            if constexpr (kStep > 16) pg = wave * S::RPR >= 16 ? page[i * kStep / 16 + 1] : pg;
-            const int in = c.table ? row & c.page_mask : row;
-            const int n = pg < 0 ? 0 : max(0, min(S::RPR, end - row));
-            const T* src = base + (c.table && n > 0 ? pg * batch : 0) + (n > 0 ? in * seq : 0);
-            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-                const_cast<T*>(src), (short)0, (int)(n * seq) * (int)sizeof(T), 0x00020000);
+            if (i * kStep % 16 == 0 || kStep > 16) {
+                // the group of the wave's run
+                const int grp = kStep > 16 ? i * kStep / 16 + wave * S::RPR / 16 : i * kStep / 16;
+                int pg = page[i * kStep / 16];
+                if constexpr (kStep > 16) pg = wave * S::RPR >= 16 ? page[i * kStep / 16 + 1] : pg;
+                const int row = k0 + 16 * grp;
+                const int n = pg < 0 ? 0 : max(0, min(16, end - row));
+                const T* src = n == 0 ? base : c.table ? base + (pg * batch + (row & c.page_mask) * seq) : base + row * seq;
+                rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(src), (short)0, (int)(n * seq) * (int)sizeof(T),
+                                                       0x00020000);
+            }
+            const int run = i * NW + wave;
             __builtin_amdgcn_raw_ptr_buffer_load_lds(
                 rs, (__attribute__((address_space(3))) void*)(dst + run * 64 * S::E), 16, voff[i], 0, 0, 0);
         }
     }
     // the same element by element: any alignment, any page size.  Returns whether the thread met a bad page.
     template <typename Cache>
-    __device__ __forceinline__ bool fill_slow(T* dst, int k0, int end, const Cache& c, int d, bool vec, int tid) const {
+    __device__ __forceinline__ bool fill_slow(T* dst, int k0, int end, const Cache& c, int d, int tid) const {
         bool bad = false;
+#pragma unroll 1
         for (int pos = tid; pos < ROWS * (D / 8); pos += 64 * NW) {
             const int r = pos / (D / 8), col = 8 * (pos % (D / 8));
             const int64_t at = c.at(k0 + r, end, seq, batch);
             bad = bad || (at < 0 && k0 + r < end);
-            const typename Mma<T>::v8 x = global_row<T>(base + (at < 0 ? 0 : at), 0, 0, at >= 0, col, d, vec);
+            const typename Mma<T>::v8 x = global_row<T, false>(base + (at < 0 ? 0 : at), 0, 0, at >= 0, col, d);
             if constexpr (sizeof(T) == 2) {
                 *reinterpret_cast<typename Mma<T>::v8*>(dst + S::at(r, col)) = x;
             } else {
@@ -143,6 +150,10 @@ struct CachePages {
     }
 };
 
+__device__ __forceinline__ CachePages rows_pages(const RowsParams& p, int b) {
+    return {p.table ? p.table + (int64_t)b * p.pages_per_seq : nullptr, p.page_shift, (1 << p.page_shift) - 1, p.n_pages};
+}
+
 // What a workgroup of either kernel works on.
 struct RowsWork {
     int kv, split, rb, b, hk;
@@ -171,8 +182,8 @@ __device__ __forceinline__ RowsWork rows_work(const RowsParams& p, int rows) {
     w.docs = p.q_doc != nullptr;
     // keys of the sequence: all of the filled rows, then the drafted ones; every row sees
     // those before `open`
-    w.len = w.tree ? p.lens[w.b] : 0;
-    w.prefix = p.prefix ? p.prefix[w.b] : 0;
+    w.len = w.tree ? load_uniform(p.lens + w.b) : 0;
+    w.prefix = p.prefix ? load_uniform(p.prefix + w.b) : 0;
     int total;
     if (w.tree) {
         total = w.len < 0 ? 0 : (int)min((int64_t)w.len + p.n, (int64_t)p.sk);
@@ -205,7 +216,7 @@ __device__ __forceinline__ bool rows_see(const RowsParams& p, const RowsWork& w,
 }
 
 // MT 16-row tiles of a wave: their queries, and the running softmax over KB 16-key blocks at a time.
-template <typename T, int D, int MT, int KB, bool MOD>
+template <typename T, int D, int MT, int KB, bool MOD, bool VEC>
 struct RowTiles {
     using M = Mma<T>;
     using S = Swizzled<T, D>;
@@ -215,7 +226,7 @@ struct RowTiles {
     f32x4 o[MT][NDB], s[MT][KB];
     float m[MT], ref[MT], l[MT];   // l: the lane's share of the row's sum
     float slope[MT];
-    int token[MT], pos[MT];
+    int token[MT], pos[MT], qd[MT];
     uint64_t word[MT];             // the token's first mask word
     int g, li;
     float c;
@@ -232,8 +243,9 @@ struct RowTiles {
             const T* from = reinterpret_cast<const T*>(p.q) + w.b * p.qs.b + h * p.qs.h;
 #pragma unroll
             for (int dc = 0; dc < NDC; ++dc)
-                q[t][dc] = global_row<T>(from, p.qs.s, token[t], real ? p.n : 0, 32 * dc + 8 * g, p.d, p.vec);
+                q[t][dc] = global_row<T, VEC>(from, p.qs.s, token[t], real ? p.n : 0, 32 * dc + 8 * g, p.d);
             pos[t] = !w.tree ? p.q_start + token[t] : p.pos ? p.pos[w.b * p.n + token[t]] : w.len + token[t];
+            qd[t] = w.docs ? p.q_doc[(int64_t)w.b * p.n + token[t]] : 0;
             slope[t] = MOD && p.slopes ? p.slopes[h] * kLog2e : 0.0f;
             word[t] = 0;
             if (w.tree)
@@ -246,8 +258,8 @@ struct RowTiles {
         }
     }
     // Scores of KB blocks of keys from k0, relative to the references; hidden ones -inf.
-    __device__ __forceinline__ void scores(const RowsParams& p, const RowsWork& w, const CachePages& pages, const T* Ks,
-                                           int k0, bool masked, bool badpage) {
+    __device__ __forceinline__ void scores(const RowsParams& p, const RowsWork& w, const T* Ks, int k0, bool masked,
+                                           bool badpage) {
 #pragma unroll
         for (int t = 0; t < MT; ++t)
 #pragma unroll
@@ -282,37 +294,80 @@ struct RowTiles {
                         for (int r = 0; r < 4; ++r) s[t][b][r] = __builtin_fmaf(s[t][b][r], p.scale_log2e, -ref[t]);
                     }
                     if (p.slopes) {
+                        f32x4 x;
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            float x = dist - (float)(16 * b + r);
-                            const int key = k0 + 16 * b + 4 * g + r;
-                            if (masked && w.tree && p.pos && key >= w.len && key < w.kend)
-                                x = (float)(pos[t] - p.pos[w.b * p.n + key - w.len]);
-                            s[t][b][r] = __builtin_fmaf(-slope[t], fabsf(x), s[t][b][r]);
+                        for (int r = 0; r < 4; ++r) x[r] = dist - (float)(16 * b + r);
+                        if (masked && w.tree) {
+                            // drafted keys stand where the program says
+                            const RowsParams lp = late_params<RowsParams>();
+                            const int bit = k0 + 16 * b + 4 * g - w.len;
+#pragma unroll
+                            for (int r = 0; r < 4; ++r)
+                                if (lp.pos && bit + r >= 0)
+                                    x[r] = (float)(pos[t] - lp.pos[w.b * lp.n + min(bit + r, lp.n - 1)]);
                         }
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) s[t][b][r] = __builtin_fmaf(-slope[t], fabsf(x[r]), s[t][b][r]);
                     }
                 }
             }
         }
         if (masked) {
+            // keys k0 .. k0 + 16 KB - 1 as bits
+            const RowsParams lp = late_params<RowsParams>();
+            const uint64_t there = keys_there(lp, w, k0, badpage);
+            uint64_t see[MT];
 #pragma unroll
-            for (int b = 0; b < KB; ++b)
+            for (int t = 0; t < MT; ++t) see[t] = there & seen_bits(lp, w, t, k0);
+            if (w.docs) {
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int key = k0 + 16 * b + 4 * g + r;
-                    const bool there = key < w.kend && (!badpage || pages.at(key, w.kend, 0, 0) >= 0);
+                for (int b = 0; b < KB; ++b)
 #pragma unroll
-                    for (int t = 0; t < MT; ++t) {
-                        bool see = there;
-                        if (w.tree && key - w.len < 64) {
-                            see = see && (key < w.len || (word[t] >> (max(key - w.len, 0) & 63)) & 1);
-                        } else if (see) {
-                            see = rows_see(p, w, token[t], key);
-                        }
-                        if (!see) s[t][b][r] = OPS_NEG_INF;
+                    for (int r = 0; r < 4; ++r) {
+                        const int x = 16 * b + 4 * g + r;
+                        const int kd = lp.k_doc[(int64_t)w.b * lp.sk + min(k0 + x, lp.sk - 1)];
+#pragma unroll
+                        for (int t = 0; t < MT; ++t)
+                            if (kd != qd[t]) see[t] &= ~(1ull << x);
                     }
+            }
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+                for (int b = 0; b < KB; ++b) {
+                    const unsigned bits = (unsigned)(see[t] >> (16 * b + 4 * g));
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (!(bits & (1u << r))) s[t][b][r] = OPS_NEG_INF;
                 }
         }
+    }
+    // Bits of the keys that exist: before the run's end, in good pages (one lane a key).
+    __device__ __forceinline__ uint64_t keys_there(const RowsParams& p, const RowsWork& w, int k0, bool badpage) const {
+        const int lane = 16 * g + li, key = k0 + lane;
+        if (!badpage) return w.kend - k0 >= 64 ? ~0ull : (1ull << (w.kend - k0)) - 1;
+        const CachePages pages = rows_pages(p, w.b);
+        return __builtin_amdgcn_ballot_w64(key < w.kend && pages.at(key, w.kend, 0, 0) >= 0);
+    }
+    // Bits of the keys that the lane's row of tile t sees, as far as causal, prefix and tree tell.
+    __device__ __forceinline__ uint64_t seen_bits(const RowsParams& p, const RowsWork& w, int t, int k0) const {
+        if (!w.tree) {
+            const int n = (w.docs && qd[t] < 0 ? 0 : p.causal ? max(p.q_start + token[t] + 1, w.prefix) : 0x7fffffff) - k0;
+            return n >= 64 ? ~0ull : (1ull << max(n, 0)) - 1;
+        }
+        const int rel = k0 - w.len;   // the first key's number among the drafted ones
+        if (rel <= -64) return ~0ull;
+        if (rel < 0) return (mask_word(p, w, t, 0) << -rel) | ((1ull << -rel) - 1);
+        const int i = rel >> 6, sh = rel & 63;
+        const uint64_t lo = mask_word(p, w, t, i) >> sh;
+        return sh == 0 ? lo : lo | (mask_word(p, w, t, i + 1) << (64 - sh));
+    }
+    __device__ __forceinline__ uint64_t mask_word(const RowsParams& p, const RowsWork& w, int t, int i) const {
+        if (i == 0) return word[t];
+        if (i >= p.mask_words) return 0;
+        if (p.mask) return p.mask[((p.mask_shared ? 0 : (int64_t)w.b * p.n) + token[t]) * p.mask_words + i];
+        const int n = token[t] + 1 - 64 * i;   // a chain
+        return n >= 64 ? ~0ull : (1ull << max(n, 0)) - 1;
     }
     // the reference of a row moves only when a score passes it by more than kLazy, or at its first key
     __device__ __forceinline__ void softmax() {
@@ -372,8 +427,10 @@ struct RowTiles {
     }
     // Partial sums, or the rows themselves where the sequence is one run.  specials: V held
     // infinities or NaN in a masked block.
-    __device__ __forceinline__ void store(const RowsParams& p, const RowsWork& w, const CachePages& pages, const T* V,
-                                          int rfirst, int tile0, int lane, bool specials) {
+    __device__ __forceinline__ void store(const RowsWork& w, const T* V, int rfirst, int tile0, int lane,
+                                          bool specials) {
+        const RowsParams p = late_params<RowsParams>();
+        const CachePages pages = rows_pages(p, w.b);
         const int mine = min(16 * MT, w.nrows - rfirst);
         auto row_at = [&](int key) -> const T* {
             const int64_t at = pages.at(key, w.kend, p.vs.s, p.vs.b);
@@ -413,7 +470,7 @@ struct RowTiles {
             T* const out = out_row(16 * t + li);
             const float inv = l[t] == 0.0f ? 0.0f : 1.0f / l[t];
 #pragma unroll
-            for (int j = 0; j < NDB; ++j) store4<T>(out, 16 * j + 4 * g, p.d, p.ovec, o[t][j] * inv);
+            for (int j = 0; j < NDB; ++j) store4<T, VEC>(out, 16 * j + 4 * g, p.d, o[t][j] * inv);
             if (p.lse && g == 0)
                 p.lse[((int64_t)w.b * p.heads + w.hk * p.group + r % p.group) * p.n + token[t]] =
                     l[t] == 0.0f ? OPS_NEG_INF : (m[t] + __builtin_log2f(l[t]) - kProbLog2<T>) * kLn2;
@@ -424,10 +481,6 @@ struct RowTiles {
         }
     }
 };
-
-__device__ __forceinline__ CachePages rows_pages(const RowsParams& p, int b) {
-    return {p.table ? p.table + (int64_t)b * p.pages_per_seq : nullptr, p.page_shift, (1 << p.page_shift) - 1, p.n_pages};
-}
 
 template <int N>
 __device__ __forceinline__ void wait_vmcnt() {
@@ -440,10 +493,10 @@ __device__ __forceinline__ void wait_vmcnt() {
 // ---------------------------------------------------------------------------
 // Up to 16 MT rows, a wave 32-key blocks of its own.
 // ---------------------------------------------------------------------------
-template <typename T, int D, int MT, bool MOD>
+template <typename T, int D, int MT, bool MOD, bool VEC>
 __device__ __forceinline__ void rows_stream(const RowsParams& p) {
     constexpr int NW = kStreamWaves<D * (int)sizeof(T)>, SK = 32, TILE = SK * D;
-    using R = RowTiles<T, D, MT, 2, MOD>;
+    using R = RowTiles<T, D, MT, 2, MOD, VEC>;
     using Src = RowSource<T, D, SK, 1>;
     constexpr int RUNS = Src::RUNS, NDB = R::NDB;
     T* const K0 = lds_array<T, NW * TILE, 0>();
@@ -461,13 +514,13 @@ __device__ __forceinline__ void rows_stream(const RowsParams& p) {
     const Src ksrc(K, p.ks.s, p.ks.b, p.d, 0, lane), vsrc(V, p.vs.s, p.vs.b, p.d, 0, lane);
     const int k_first = w.kbeg + SK * wave;
     const int nblk = k_first < w.kend ? (w.kend - k_first + SK * NW - 1) / (SK * NW) : 0;
-    const bool dma = p.dma;
+    static_assert(VEC, "DMA only");
 
     bool special = false;
     R x;
     auto pages_of = [&](int blk, int (&pg)[2]) {
         const int k = k_first + blk * SK * NW;
-        const bool in = dma && blk < nblk;
+        const bool in = blk < nblk;
         pg[0] = in ? pages.page(k) : -1;
         pg[1] = in && k + 16 < w.kend ? pages.page(k + 16) : -1;
     };
@@ -477,12 +530,12 @@ __device__ __forceinline__ void rows_stream(const RowsParams& p) {
     int pg0[2], pg1[2], pg2[2];
     pages_of(0, pg0);
     pages_of(1, pg1);
-    if (dma && nblk > 0) {
+    if (nblk > 0) {
         fill(ksrc, K0, 0, pg0);
         fill(vsrc, V0, 0, pg0);
     }
     x.init(p, w, w.rfirst, lane);
-    if (dma && nblk > 0) {
+    if (nblk > 0) {
         // Q's loads are through before more DMA starts: only DMA is counted from here
         wait_vmcnt<0>();
         fill(ksrc, K1, 1, pg1);
@@ -492,32 +545,22 @@ __device__ __forceinline__ void rows_stream(const RowsParams& p) {
         T* const Ks = kb + wave * TILE;
         T* const Vs = vb + wave * TILE;
         const int k0 = k_first + i * SK * NW;
-        bool bad = false;
-        if (dma) {
-            bad = pg0[0] < 0 || (pg0[1] < 0 && k0 + 16 < w.kend);
-            pages_of(i + 2, pg2);
-            wait_vmcnt<3 * RUNS>();
-        } else {
-            bool b = ksrc.fill_slow(Ks, k0, w.kend, pages, p.d, p.vec, lane);
-            b = vsrc.fill_slow(Vs, k0, w.kend, pages, p.d, p.vec, lane) || b;
-            bad = __builtin_amdgcn_ballot_w64(b) != 0;
-            reread();
-        }
+        const bool bad = pg0[0] < 0 || (pg0[1] < 0 && k0 + 16 < w.kend);
+        pages_of(i + 2, pg2);
+        wait_vmcnt<3 * RUNS>();
         const bool masked = bad || k0 + SK > min(w.open, w.kend);
-        x.scores(p, w, pages, Ks, k0, masked, bad);
-        if (dma) {
-            reread();
-            fill(ksrc, kb, i + 2, pg2);
-        }
+        x.scores(p, w, Ks, k0, masked, bad);
+        reread();
+        fill(ksrc, kb, i + 2, pg2);
         x.softmax();
-        if (dma) wait_vmcnt<3 * RUNS>();
+        wait_vmcnt<3 * RUNS>();
         if (masked) {
             special = Swizzled<T, D>::template clean<SK, 64>(Vs, lane) || special;
             reread();
         }
         x.values(Vs);
         reread();
-        if (dma) fill(vsrc, vb, i + 2, pg2);
+        fill(vsrc, vb, i + 2, pg2);
         pg0[0] = pg1[0], pg0[1] = pg1[1];
         pg1[0] = pg2[0], pg1[1] = pg2[1];
     };
@@ -570,16 +613,16 @@ __device__ __forceinline__ void rows_stream(const RowsParams& p) {
     int specials = 0;
 #pragma unroll
     for (int i = 0; i < NW; ++i) specials |= any_special[i];
-    x.store(p, w, pages, V, w.rfirst, 0, lane, specials != 0);
+    x.store(w, V, w.rfirst, 0, lane, specials != 0);
 }
 
 // ---------------------------------------------------------------------------
 // Many rows: the waves share the keys.
 // ---------------------------------------------------------------------------
-template <typename T, int D, int MT, bool MOD>
+template <typename T, int D, int MT, bool MOD, bool VEC>
 __device__ __forceinline__ void rows_shared(const RowsParams& p) {
     constexpr int NW = 4, SK = sizeof(T) == 4 || D > 128 ? 32 : 64, TILE = SK * D, KB = SK / 16;
-    using R = RowTiles<T, D, MT, KB, MOD>;
+    using R = RowTiles<T, D, MT, KB, MOD, VEC>;
     using Src = RowSource<T, D, SK, NW>;
     T* const Kb0 = lds_array<T, TILE, 0>();
     T* const Vb0 = lds_array<T, TILE, 1>();
@@ -595,7 +638,8 @@ __device__ __forceinline__ void rows_shared(const RowsParams& p) {
     const Src ksrc(K, p.ks.s, p.ks.b, p.d, wave, lane), vsrc(V, p.vs.s, p.vs.b, p.d, wave, lane);
     const int nst = (w.kend - w.kbeg + SK - 1) / SK;
     const int rfirst = w.rfirst + 16 * MT * wave;
-    const bool dma = p.dma, act = rfirst < w.nrows;
+    constexpr bool dma = VEC;
+    const bool act = rfirst < w.nrows;
 
     int pgk[SK / 16], pgv[SK / 16], pgn[SK / 16];   // pages of the current, next and after-next stage
     auto pages_of = [&](int st, int (&pg)[SK / 16]) {
@@ -607,10 +651,10 @@ __device__ __forceinline__ void rows_shared(const RowsParams& p) {
     };
     auto fill = [&](const Src& src, T* dst, int st, const int (&pg)[SK / 16], int parity) {
         const int k0 = w.kbeg + st * SK;
-        if (dma) {
+        if constexpr (dma) {
             src.fill(dst, k0, w.kend, pg, pages, wave);
-        } else if (src.fill_slow(dst, k0, w.kend, pages, p.d, p.vec, tid)) {
-            bad_any[parity] = 1;
+        } else {
+            if (src.fill_slow(dst, k0, w.kend, pages, p.d, tid)) bad_any[parity] = 1;
         }
     };
     auto bad_stage = [&](int st, const int (&pg)[SK / 16], int parity) {
@@ -638,7 +682,7 @@ __device__ __forceinline__ void rows_shared(const RowsParams& p) {
         const int k0 = w.kbeg + st * SK;
         bad = bad_stage(st, pg, parity);
         masked = bad || k0 + SK > min(w.open, w.kend);
-        if (act) x.scores(p, w, pages, Ks, k0, masked, bad);
+        if (act) x.scores(p, w, Ks, k0, masked, bad);
     };
     if (nst > 0) score(0, Kb0, pgk, 0);
     __syncthreads();
@@ -667,37 +711,47 @@ __device__ __forceinline__ void rows_shared(const RowsParams& p) {
         if (st + 1 < nst) step(std::integral_constant<int, 1>{}, st + 1);
     }
     x.close();
-    if (act) x.store(p, w, pages, V, rfirst, MT * wave, lane, Special != 0);
+    if (act) x.store(w, V, rfirst, MT * wave, lane, Special != 0);
 }
 
-// Joins the partial sums of a row, a wave a row, four columns a lane.
-template <typename T, int D>
+// Joins the partial sums of a row: a workgroup a row, D / 4 lanes a run, the runs dealt to
+// the workgroup's groups of lanes, whose sums meet in LDS.
+template <typename T, int D, bool VEC>
 __device__ __forceinline__ void rows_merge(const RowsParams& p) {
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
-    const int nrows = p.n * p.group, rows = p.block_rows;
-    if (row >= (int64_t)p.batch * p.kv_heads * nrows) return;
-    const int kv = row / nrows, r = row % nrows;
+    constexpr int L = D / 4, G = 256 / L;
+    __shared__ f32x4 sums[G][L];
+    __shared__ float ls[G];
+    const int nrows = p.n * p.group, rows = p.block_rows, tid = threadIdx.x;
+    const int grp = tid / L, lane = tid % L;
+    const int kv = blockIdx.x / nrows, r = blockIdx.x % nrows;
     const int b = kv / p.kv_heads, h = kv % p.kv_heads * p.group + r % p.group, token = r / p.group;
     const int64_t part = ((int64_t)kv * p.nrb + r / rows) * p.num_splits;
     const float* const ml = p.part_ml + part * 2 * rows + r % rows;
     const float* const po = p.part_o + (part * rows + r % rows) * D + 4 * lane;
     float mx = OPS_NEG_INF;
-    for (int s = lane; s < p.num_splits; s += 64) mx = fmaxf(mx, ml[(int64_t)s * 2 * rows]);
+    for (int s = tid & 63; s < p.num_splits; s += 64) mx = fmaxf(mx, ml[(int64_t)s * 2 * rows]);
 #pragma unroll
     for (int s = 1; s < 64; s *= 2) mx = fmaxf(mx, __shfl_xor(mx, s));
     const float ref = mx == OPS_NEG_INF ? 0.0f : mx;
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
     float l = 0.0f;
 #pragma unroll 4
-    for (int s = 0; s < p.num_splits; ++s) {
+    for (int s = grp; s < p.num_splits; s += G) {
         const float c = ops_exp2(ml[(int64_t)s * 2 * rows] - ref);
         l += c * ml[(int64_t)s * 2 * rows + rows];
-        if (4 * lane < D) o += c * *reinterpret_cast<const f32x4*>(po + (int64_t)s * rows * D);
+        o += c * *reinterpret_cast<const f32x4*>(po + (int64_t)s * rows * D);
     }
-    if (4 * lane < D)
-        store4<T>(reinterpret_cast<T*>(p.out) + b * p.os.b + h * p.os.h + token * p.os.s, 4 * lane, p.d, p.ovec,
-                  o * (l == 0.0f ? 0.0f : 1.0f / l));
+    sums[grp][lane] = o;
+    if (lane == 0) ls[grp] = l;
+    __syncthreads();
+    if (grp != 0) return;
+#pragma unroll
+    for (int i = 1; i < G; ++i) {
+        o += sums[i][lane];
+        l += ls[i];
+    }
+    store4<T, VEC>(reinterpret_cast<T*>(p.out) + b * p.os.b + h * p.os.h + token * p.os.s, 4 * lane, p.d,
+                   o * (l == 0.0f ? 0.0f : 1.0f / l));
     if (p.lse && lane == 0)
         p.lse[((int64_t)b * p.heads + h) * p.n + token] =
             l == 0.0f ? OPS_NEG_INF : (mx + __builtin_log2f(l) - kProbLog2<T>) * kLn2;
@@ -705,38 +759,39 @@ __device__ __forceinline__ void rows_merge(const RowsParams& p) {
 
 #define PASTE_(a, b, c, d) a##b##c##d
 #define PASTE(a, b, c, d) PASTE_(a, b, c, d)
-#define KERNEL(F, BODY, D, MT, MOD, TAG, THREADS, WAVES)                                                       \
+#define KERNEL(F, BODY, D, MT, MOD, VEC, TAG, THREADS, WAVES)                                                  \
     extern "C" __global__ __launch_bounds__(THREADS, WAVES) void PASTE(F, OPS_NAME, _d##D##_t##MT, TAG)(RowsParams p) { \
-        BODY<OPS_T, D, MT, MOD>(p);                                                                            \
+        BODY<OPS_T, D, MT, MOD, VEC>(p);                                                                       \
     }
-#define STREAM(D, MT)                                                                                    \
-    KERNEL(fa_rows_stream_, rows_stream, D, MT, false, , (64 * kStreamWaves<D * (int)sizeof(OPS_T)>), 1) \
-    KERNEL(fa_rows_stream_, rows_stream, D, MT, true, m, (64 * kStreamWaves<D * (int)sizeof(OPS_T)>), 1)
-#define SHARED(D, MT, WAVES)                                             \
-    KERNEL(fa_rows_shared_, rows_shared, D, MT, false, , 256, WAVES)     \
-    KERNEL(fa_rows_shared_, rows_shared, D, MT, true, m, 256, WAVES)
-#define MERGE(D)                                                                                          \
-    extern "C" __global__ __launch_bounds__(256) void PASTE(fa_rows_merge_, OPS_NAME, _d##D, )(RowsParams p) { \
-        rows_merge<OPS_T, D>(p);                                                                          \
+// plain scores, modified ones (m), and any alignment and page size (s)
+#define STREAM_THREADS(D) (64 * kStreamWaves<D * (int)sizeof(OPS_T)>)
+#define STREAM(D, MT, WAVES)                                                              \
+    KERNEL(fa_rows_stream_, rows_stream, D, MT, false, true, , STREAM_THREADS(D), WAVES)  \
+    KERNEL(fa_rows_stream_, rows_stream, D, MT, true, true, m, STREAM_THREADS(D), WAVES)
+#define SHARED(D, MT, WAVES)                                                   \
+    KERNEL(fa_rows_shared_, rows_shared, D, MT, false, true, , 256, WAVES)     \
+    KERNEL(fa_rows_shared_, rows_shared, D, MT, true, true, m, 256, WAVES)
+#define COMMON(D)                                                                                               \
+    KERNEL(fa_rows_shared_, rows_shared, D, 1, true, false, s, 256, 1)                                          \
+    extern "C" __global__ __launch_bounds__(256) void PASTE(fa_rows_merge_, OPS_NAME, _d##D, )(RowsParams p) {  \
+        rows_merge<OPS_T, D, true>(p);                                                                          \
+    }                                                                                                           \
+    extern "C" __global__ __launch_bounds__(256) void PASTE(fa_rows_merge_, OPS_NAME, _d##D, s)(RowsParams p) { \
+        rows_merge<OPS_T, D, false>(p);                                                                         \
     }
-MERGE(64)
-MERGE(128)
-MERGE(256)
-STREAM(64, 1)
-STREAM(128, 1)
-STREAM(256, 1)
+COMMON(64)
+COMMON(128)
+COMMON(256)
+STREAM(64, 1, 2)
+STREAM(64, 2, 2)
+STREAM(128, 1, 2)
 #ifdef OPS_16BIT
-STREAM(64, 2)
-STREAM(64, 4)
-STREAM(128, 2)
-STREAM(128, 4)
-STREAM(256, 2)
+STREAM(128, 2, 2)
+STREAM(256, 1, 2)
 SHARED(64, 2, 2)
 SHARED(128, 2, 2)
 SHARED(256, 1, 2)
 #else
-STREAM(64, 2)
-STREAM(128, 2)
 SHARED(64, 1, 2)
 SHARED(128, 1, 2)
 SHARED(256, 1, 1)

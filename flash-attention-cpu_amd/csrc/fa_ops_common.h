@@ -30,6 +30,18 @@ constexpr float kLn2 = 0.693147180559945309f;
 // maximum of a row by this much (log2 units) before the sums are rescaled.
 constexpr float kLazy = 8.0f;
 
+// The kernel's parameters, read again where this stands: code that runs seldom (masked tiles, the
+// stores at the end) uses these, so that what only it needs does not occupy scalar
+// registers in the main loop.
+template <typename P>
+__device__ __forceinline__ P late_params() {
+    auto k = (const __attribute__((address_space(4))) char*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(k));
+    P p;
+    __builtin_memcpy(&p, (const char*)k, sizeof(P));
+    return p;
+}
+
 template <typename T>
 struct Mma;
 template <>
@@ -97,17 +109,20 @@ __device__ __forceinline__ typename Mma<T>::v8 col_op(const T* tile, int row0, i
     }
 }
 
+// Kernels come in two kinds: VEC, where rows are 16-byte aligned and d is a multiple of 8, and
+// one that takes any alignment and width element by element.
+
 // Rows row0 + li of a matrix in global memory as an operand: columns 32 dc + 8g.
 // Zero outside [0, rows) x [0, d).
-template <typename T>
+template <typename T, bool VEC>
 __device__ __forceinline__ typename Mma<T>::v8 global_row(const T* base, int64_t stride, int row, int rows, int col,
-                                                          int d, bool vec) {
+                                                          int d) {
     typename Mma<T>::v8 v;
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = T(0.0f);
     if (row < rows && col < d) {
         const T* p = base + row * stride + col;
-        if (vec) {
+        if constexpr (VEC) {
             v = *reinterpret_cast<const typename Mma<T>::v8*>(p);
         } else {
 #pragma unroll
@@ -119,13 +134,13 @@ __device__ __forceinline__ typename Mma<T>::v8 global_row(const T* base, int64_t
 }
 
 // The C layout's four consecutive columns of one row, to global memory.
-template <typename T>
-__device__ __forceinline__ void store4(T* row, int col, int d, bool wide, f32x4 x) {
+template <typename T, bool VEC>
+__device__ __forceinline__ void store4(T* row, int col, int d, f32x4 x) {
     typename Mma<T>::v4 y;
 #pragma unroll
     for (int r = 0; r < 4; ++r) y[r] = T(x[r]);
-    if (wide && col + 4 <= d) {
-        *reinterpret_cast<typename Mma<T>::v4*>(row + col) = y;
+    if constexpr (VEC) {
+        if (col < d) *reinterpret_cast<typename Mma<T>::v4*>(row + col) = y;
     } else {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
@@ -250,7 +265,7 @@ __device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0f70
 // tile's image (pad chunks included) with offsets fixed for the whole kernel -- the buffer's range ends at the
 // last row, and lanes past it, past column d or in the pad read zeros --
 // or, where rows are not 16-byte aligned, element by element.
-template <typename T, int D, int ROWS, int NW>
+template <typename T, int D, int ROWS, int NW, bool VEC>
 struct TileFill {
     static constexpr int LD = D + kPad<T>, E = 16 / (int)sizeof(T), RCH = LD / E;
     static constexpr int TOTAL = ROWS * RCH, RUNS = (TOTAL + 63) / 64, NI = (RUNS + NW - 1) / NW;
@@ -258,9 +273,8 @@ struct TileFill {
     int voff[NI];
     int wave, lane, d;
     int64_t stride;
-    bool vec;
-    __device__ __forceinline__ TileFill(int64_t stride_, int d_, bool vec_, int wave_, int lane_)
-        : wave(wave_), lane(lane_), d(d_), stride(stride_), vec(vec_) {
+    __device__ __forceinline__ TileFill(int64_t stride_, int d_, int wave_, int lane_)
+        : wave(wave_), lane(lane_), d(d_), stride(stride_) {
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
             const int pos = (i * NW + wave) * 64 + lane, r = pos / RCH, col = pos % RCH * E;
@@ -269,7 +283,7 @@ struct TileFill {
     }
     __device__ __forceinline__ void operator()(T* dst, const T* base, int row0, int rows) const {
         const T* src = base + row0 * stride;
-        if (vec) {
+        if constexpr (VEC) {
             const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
                 const_cast<T*>(src), (short)0, (int)(min(ROWS, rows - row0) * stride) * (int)sizeof(T), 0x00020000);
 #pragma unroll
@@ -280,20 +294,13 @@ struct TileFill {
                         rs, (__attribute__((address_space(3))) void*)(dst + run * 64 * E), 16, voff[i], 0, 0, 0);
             }
         } else {
+#pragma unroll 1
             for (int pos = wave * 64 + lane; pos < ROWS * (D / 8); pos += 64 * NW) {
                 const int r = pos / (D / 8), col = 8 * (pos % (D / 8));
                 *reinterpret_cast<typename Mma<T>::v8*>(dst + r * LD + col) =
-                    global_row<T>(src, stride, r, rows - row0, col, d, false);
+                    global_row<T, false>(src, stride, r, rows - row0, col, d);
             }
         }
-    }
-};
-
-// Visibility of key j to the query at position pos (score attention).
-struct ScoreMask {
-    int causal, prefix, sk;
-    __device__ __forceinline__ bool seen(int key, int pos) const {
-        return key < sk && (!causal || key <= pos || key < prefix);
     }
 };
 

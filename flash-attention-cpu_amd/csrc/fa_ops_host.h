@@ -188,53 +188,55 @@ constexpr size_t kOpsMaxGrid = size_t(1) << 22;   // workgroups: threads of a la
 
 size_t doc_tiles(size_t n) { return (n + kDocTile - 1) / kDocTile; }
 
-// Plan of the rows kernels: streaming waves up to 64 rows (as far as registers go), else
-// workgroups that share their keys; the keys in as many runs as fill the GPU.
+// Plan of the rows kernels: streaming waves up to 64 rows, else workgroups that share their
+// keys; the keys in as many runs as fill the GPU.
 struct RowsPlan {
     bool stream;
     int mt, threads, rows, nrb, splits;
     size_t floats;
 };
-RowsPlan plan_rows(int dtype, int D, size_t nkv, size_t rows, size_t keys, int num_cus) {
+RowsPlan plan_rows(int dtype, int D, bool vec, size_t nkv, size_t rows, size_t keys, int num_cus) {
     RowsPlan r{};
     const bool f32 = dtype == FA_DTYPE_F32;
     const int row_bytes = D * static_cast<int>(elem_size(dtype));
-    const int most = f32 ? (D > 128 ? 1 : 2) : (D > 128 ? 2 : 4);   // tiles a streaming wave
-    r.stream = rows <= static_cast<size_t>(16 * most);
+    r.stream = vec && rows <= 64 && row_bytes <= 512;
     size_t step;
     if (r.stream) {
-        r.mt = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-        const int waves = row_bytes <= 256 ? kStreamWaves<256> : row_bytes <= 512 ? kStreamWaves<512> : kStreamWaves<1024>;
+        // two tiles a wave as far as its registers hold them
+        r.mt = rows <= 16 || row_bytes > 256 ? 1 : 2;
+        const int waves = row_bytes <= 256 ? kStreamWaves<256> : kStreamWaves<512>;
         r.threads = 64 * waves;
         r.rows = 16 * r.mt;
         step = 32 * waves;
     } else {
-        r.mt = f32 || D > 128 ? 1 : 2;
+        r.mt = !vec || f32 || D > 128 ? 1 : 2;
         r.threads = 256;
         r.rows = 64 * r.mt;
         step = f32 || D > 128 ? 32 : 64;
     }
     r.nrb = static_cast<int>((rows + r.rows - 1) / r.rows);
     const size_t units = std::max<size_t>(nkv * r.nrb, 1);
-    size_t splits = std::max<size_t>(1, 2 * static_cast<size_t>(num_cus) / units);
+    // one round of resident workgroups: LDS holds one streaming workgroup a CU, two of short rows or of shared stages
+    const size_t resident = (r.stream && row_bytes > 128 ? 1 : 2) * static_cast<size_t>(num_cus);
+    size_t splits = std::max<size_t>(1, resident / units);
     splits = std::min(splits, std::max<size_t>(1, keys / step));
     r.splits = static_cast<int>(std::min<size_t>(splits, 256));
     r.floats = r.splits > 1 ? units * r.splits * r.rows * (D + 2) : 0;
     return r;
 }
 
-int run_rows(int dev, hipStream_t stream, int dtype, int D, RowsParams* p, size_t keys) {
+int run_rows(int dev, hipStream_t stream, int dtype, int D, bool vec, RowsParams* p, size_t keys) {
+    vec = vec && (!p->table || p->page_shift >= 4);   // DMA moves runs of rows of one page
     const OpsModule module = of_type(kCacheModule, dtype);
     int rc = ops_module(dev, module);
     if (rc != FA_OK) return rc;
     const size_t nkv = static_cast<size_t>(p->batch) * p->kv_heads;
     const size_t rows = static_cast<size_t>(p->n) * p->group;
-    const RowsPlan plan = plan_rows(dtype, D, nkv, rows, keys, g_dev[dev].num_cus);
+    const RowsPlan plan = plan_rows(dtype, D, vec, nkv, rows, keys, g_dev[dev].num_cus);
     p->nrb = plan.nrb;
     p->num_splits = plan.splits;
     p->block_rows = plan.rows;
-    p->dma = p->vec && (!p->table || p->page_shift >= 4);
-    const size_t grid = nkv * plan.nrb * plan.splits, mgrid = (nkv * rows + 3) / 4;
+    const size_t grid = nkv * plan.nrb * plan.splits, mgrid = nkv * rows;
     if (grid > kOpsMaxGrid || mgrid > kOpsMaxGrid) return FA_ERR_UNSUPPORTED;
     OpsWorkspace ws;
     if (plan.floats) {
@@ -244,10 +246,10 @@ int run_rows(int dev, hipStream_t stream, int dtype, int D, RowsParams* p, size_
     }
     char name[64];
     std::snprintf(name, sizeof(name), "fa_rows_%s_%s_d%d_t%d%s", plan.stream ? "stream" : "shared", dtype_name(dtype), D,
-                  plan.mt, p->slopes || p->cap_log2e != 0.0f ? "m" : "");
+                  plan.mt, !vec ? "s" : p->slopes || p->cap_log2e != 0.0f ? "m" : "");
     rc = ops_launch(dev, module, name, grid, plan.threads, p, stream);
     if (rc == FA_OK && plan.splits > 1) {
-        std::snprintf(name, sizeof(name), "fa_rows_merge_%s_d%d", dtype_name(dtype), D);
+        std::snprintf(name, sizeof(name), "fa_rows_merge_%s_d%d%s", dtype_name(dtype), D, vec ? "" : "s");
         rc = ops_launch(dev, module, name, mgrid, 256, p, stream);
     }
     return ws.done(stream, rc);
@@ -397,8 +399,7 @@ int fa_score_forward(void* stream_, const fa_score_config* c, const void* q, con
     int dev;
     if ((rc = ops_begin(&dev, of_type(kScoreModule, c->dtype))) != FA_OK) return rc;
     const hipStream_t stream = static_cast<hipStream_t>(stream_);
-    const bool vec = vec_ok(q, lq, d) && vec_ok(k, lk, d) && vec_ok(v, lv, d);
-    const bool ovec = ovec_ok(out, lo, es);
+    const bool vec = vec_ok(q, lq, d) && vec_ok(k, lk, d) && vec_ok(v, lv, d) && ovec_ok(out, lo, es);
 
     if (score_takes_rows(*c, g_dev[dev].num_cus)) {
         RowsParams p{};
@@ -409,16 +410,14 @@ int fa_score_forward(void* stream_, const fa_score_config* c, const void* q, con
         p.kv_heads = static_cast<int>(c->kv_heads), p.group = static_cast<int>(c->heads / c->kv_heads);
         p.n = static_cast<int>(c->seq_len_q), p.sk = static_cast<int>(c->seq_len_k), p.d = static_cast<int>(d);
         p.causal = c->causal ? 1 : 0, p.q_start = static_cast<int>(c->q_start);
-        p.vec = vec, p.ovec = ovec;
         p.scale = sc.scale, p.scale_log2e = sc.scale_log2e, p.cap_in = sc.cap_in, p.cap_log2e = sc.cap_log2e;
-        return run_rows(dev, stream, c->dtype, D, &p, c->seq_len_k);
+        return run_rows(dev, stream, c->dtype, D, vec, &p, c->seq_len_k);
     }
     ScoreParams p{};
     fill_score(*c, sc, &p);
     p.q = q, p.k = k, p.v = v, p.out = out, p.lse = lse;
     p.qs = lq.st, p.ks = lk.st, p.vs = lv.st, p.os = lo.st;
-    p.vec = vec, p.ovec = ovec;
-    const int mt = score_tiles(c->dtype, D, c->seq_len_q, c->batch * c->heads, 2, g_dev[dev].num_cus);
+    const int mt = vec ? score_tiles(c->dtype, D, c->seq_len_q, c->batch * c->heads, 2, g_dev[dev].num_cus) : 1;
     p.nqb = static_cast<int>((c->seq_len_q + 64 * mt - 1) / (64 * mt));
     OpsWorkspace ws;
     if (c->q_doc) {
@@ -428,7 +427,7 @@ int fa_score_forward(void* stream_, const fa_score_config* c, const void* q, con
     if (rc == FA_OK) {
         char name[64];
         std::snprintf(name, sizeof(name), "fa_score_forward_%s_d%d_t%d%s", dtype_name(c->dtype), D, mt,
-                      c->slopes || c->softcap > 0.0f ? "m" : "");
+                      !vec ? "s" : c->slopes || c->softcap > 0.0f ? "m" : "");
         rc = ops_launch(dev, of_type(kScoreModule, c->dtype), name, c->batch * c->heads * p.nqb, 256, &p, stream);
     }
     return ws.done(stream, rc);
@@ -469,8 +468,8 @@ int fa_score_backward(void* stream_, const fa_score_config* c, const void* q, co
     p.dq = dq, p.dk = dk, p.dv = dv;
     p.qs = lq.st, p.ks = lk.st, p.vs = lv.st, p.os = lo.st, p.dos = ldo.st;
     p.dqs = ldq.st, p.dks = ldk.st, p.dvs = ldv.st;
-    p.vec = vec_ok(q, lq, d) && vec_ok(k, lk, d) && vec_ok(v, lv, d) && vec_ok(out, lo, d) && vec_ok(dout, ldo, d);
-    p.ovec = ovec_ok(dq, ldq, es) && ovec_ok(dk, ldk, es) && ovec_ok(dv, ldv, es);
+    const bool vec = vec_ok(q, lq, d) && vec_ok(k, lk, d) && vec_ok(v, lv, d) && vec_ok(out, lo, d) &&
+                     vec_ok(dout, ldo, d) && ovec_ok(dq, ldq, es) && ovec_ok(dk, ldk, es) && ovec_ok(dv, ldv, es);
     OpsWorkspace ws;
     const size_t rng = doc_range_bytes(*c);
     if ((rc = ws.get(dev, stream, 2 * rows * sizeof(float) + rng + 16)) != FA_OK) return rc;
@@ -479,18 +478,18 @@ int fa_score_backward(void* stream_, const fa_score_config* c, const void* q, co
     char name[64];
     if (c->q_doc) rc = launch_doc_ranges(dev, of_type(kScoreModule, c->dtype), stream, &p, reinterpret_cast<int32_t*>(p.delta + rows));
     if (rc == FA_OK) {
-        std::snprintf(name, sizeof(name), "fa_score_delta_%s", dtype_name(c->dtype));
+        std::snprintf(name, sizeof(name), "fa_score_delta_%s%s", dtype_name(c->dtype), vec ? "" : "s");
         rc = ops_launch(dev, of_type(kScoreModule, c->dtype), name, dgrid, 256, &p, stream);
     }
-    const char* mod = c->slopes || c->softcap > 0.0f ? "m" : "";
+    const char* mod = !vec ? "s" : c->slopes || c->softcap > 0.0f ? "m" : "";
     if (rc == FA_OK && (dk || dv)) {
-        const int mt = score_tiles(c->dtype, D, sk, c->batch * c->kv_heads, 1, g_dev[dev].num_cus);
+        const int mt = vec ? score_tiles(c->dtype, D, sk, c->batch * c->kv_heads, 1, g_dev[dev].num_cus) : 1;
         p.nqb = static_cast<int>((sk + 64 * mt - 1) / (64 * mt));
         std::snprintf(name, sizeof(name), "fa_score_dkv_%s_d%d_t%d%s", dtype_name(c->dtype), D, mt, mod);
         rc = ops_launch(dev, of_type(kScoreModule, c->dtype), name, c->batch * c->kv_heads * p.nqb, 256, &p, stream);
     }
     if (rc == FA_OK && dq) {
-        const int mt = score_tiles(c->dtype, D, sq, c->batch * c->heads, 2, g_dev[dev].num_cus);
+        const int mt = vec ? score_tiles(c->dtype, D, sq, c->batch * c->heads, 2, g_dev[dev].num_cus) : 1;
         p.nqb = static_cast<int>((sq + 64 * mt - 1) / (64 * mt));
         std::snprintf(name, sizeof(name), "fa_score_dq_%s_d%d_t%d%s", dtype_name(c->dtype), D, mt, mod);
         rc = ops_launch(dev, of_type(kScoreModule, c->dtype), name, c->batch * c->heads * p.nqb, 256, &p, stream);
@@ -667,12 +666,11 @@ int fa_tree_attention(void* stream, const fa_tree_config* c, const fa_kv_cache* 
     p.page_shift = page_shift(*cache);
     p.n_pages = static_cast<int>(cache->n_pages), p.pages_per_seq = static_cast<int>(cache->pages_per_seq);
     p.mask_words = static_cast<int>((n + 63) / 64), p.mask_shared = c->mask_shared ? 1 : 0;
-    p.vec = vec_ok(q, lq, d) && vec_ok(cache->k, ck, d) && vec_ok(cache->v, cv, d);
-    p.ovec = ovec_ok(out, lo, es);
+    const bool vec = vec_ok(q, lq, d) && vec_ok(cache->k, ck, d) && vec_ok(cache->v, cv, d) && ovec_ok(out, lo, es);
     p.scale = sc.scale, p.scale_log2e = sc.scale_log2e, p.cap_in = sc.cap_in, p.cap_log2e = sc.cap_log2e;
     int dev;
     if ((rc = ops_begin(&dev, of_type(kCacheModule, cache->dtype))) != FA_OK) return rc;
-    return run_rows(dev, static_cast<hipStream_t>(stream), cache->dtype, ops_pad_d(d), &p, capacity);
+    return run_rows(dev, static_cast<hipStream_t>(stream), cache->dtype, ops_pad_d(d), vec, &p, capacity);
 }
 
 }  // extern "C"

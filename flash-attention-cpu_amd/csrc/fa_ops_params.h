@@ -27,18 +27,16 @@ struct ScoreParams {
     int batch, heads, kv_heads, group, sq, sk, d;
     int causal, q_start;
     int nqb;                  // query (dK/dV: key) blocks a slice
-    int vec;                  // 16-byte loads of Q, K, V, dO
-    int ovec;                 // wide stores of the outputs
     float scale;              // of the scores
     float scale_log2e;
     float cap_in;             // 2 log2(e) scale / softcap: exponent of the cap's tanh
     float cap_log2e;          // softcap * log2(e); 0: no cap
 };
 
-// Waves of a workgroup of the streaming rows kernel, by the bytes of a padded row: each has
+// Waves of a workgroup of the streaming rows kernel, by the bytes of a padded row (up to 512): each has
 // two slots of 32 rows of K and V in LDS.
 template <int ROW>
-constexpr int kStreamWaves = ROW <= 256 ? 4 : ROW <= 512 ? 2 : 1;
+constexpr int kStreamWaves = ROW <= 256 ? 4 : 2;
 
 // Attention of few rows over a long key range, keys split over workgroups.
 struct RowsParams {
@@ -56,9 +54,7 @@ struct RowsParams {
     int page_shift, n_pages, pages_per_seq;
     int mask_words, mask_shared;
     int nrb, num_splits;      // row blocks of a (batch, kv head), splits of its keys
-    int block_rows;
-    int vec, ovec;
-    int dma;                  // K and V by DMA: 16-byte aligned rows, pages of 16 rows or more
+    int block_rows;           // rows of a row block
     float scale, scale_log2e, cap_in, cap_log2e;
 };
 

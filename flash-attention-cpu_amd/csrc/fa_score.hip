@@ -88,9 +88,14 @@ __device__ __forceinline__ void each_masked(Test test, int count, int lane, F f)
         if (masked) f(st);
 }
 
+// Keys that causal and prefix bounds leave a query at position pos: those before this.
+__device__ __forceinline__ int key_limit(const ScoreParams& p, int prefix, int pos) {
+    return p.causal ? max(pos + 1, prefix) : 0x7fffffff;
+}
+
 // Whether query `row` sees key `key`.
-__device__ __forceinline__ bool pair_seen(const ScoreParams& p, const ScoreMask& mask, int b, int row, int key) {
-    if (!mask.seen(key, p.q_start + row)) return false;
+__device__ __forceinline__ bool pair_seen(const ScoreParams& p, int prefix, int b, int row, int key) {
+    if (key >= key_limit(p, prefix, p.q_start + row)) return false;
     if (!p.q_doc) return true;
     const int d = p.q_doc[(int64_t)b * p.sq + row];
     return d >= 0 && d == p.k_doc[(int64_t)b * p.sk + key];
@@ -137,14 +142,14 @@ constexpr int kStageKeys = sizeof(T) == 4 || D > 128 ? 32 : 64;
 // Whether queries [q0, q1), of the documents qr, see a key of stage st, and whether
 // some pair is hidden.
 template <int SK>
-__device__ __forceinline__ bool key_stage(const ScoreParams& p, const ScoreMask& mask, int st, int q0, int q1, bool docs,
+__device__ __forceinline__ bool key_stage(const ScoreParams& p, int prefix, int st, int q0, int q1, bool docs,
                                           const DocRange& qr, const int32_t* krng, bool* part) {
     const int k0 = st * SK, k1 = k0 + SK;
     bool v = true;
     if (k1 > p.sk) *part = true;
     if (p.causal) {
-        v = k0 <= p.q_start + q1 - 1 || k0 < mask.prefix;
-        if (!(k1 - 1 <= p.q_start + q0 || k1 <= mask.prefix)) *part = true;
+        v = k0 <= p.q_start + q1 - 1 || k0 < prefix;
+        if (!(k1 - 1 <= p.q_start + q0 || k1 <= prefix)) *part = true;
     }
     if (docs && v) v = docs_meet(qr, doc_range(krng, k0 / kDocTile), part);
     return v;
@@ -157,13 +162,13 @@ __device__ __forceinline__ bool key_stage(const ScoreParams& p, const ScoreMask&
 // a stage's softmax and PV product run, K of the stage after the next and V of
 // the next arrive; one barrier a stage.  The loop is unrolled by two so that each buffer is
 // an array of its own.
-template <typename T, int D, int MT, bool MOD>
+template <typename T, int D, int MT, bool MOD, bool VEC>
 __device__ __forceinline__ void score_forward(const ScoreParams& p) {
     using M = Mma<T>;
     using v8 = typename M::v8;
     constexpr int NW = 4, SK = kStageKeys<T, D>, BQ = 16 * MT * NW;
     constexpr int KB = SK / 16, NCH = SK / 32, NDC = D / 32, NDB = D / 16, LD = D + kPad<T>;
-    using Fill = TileFill<T, D, SK, NW>;
+    using Fill = TileFill<T, D, SK, NW, VEC>;
     T* const Kb0 = lds_array<T, Fill::SIZE, 0>();
     T* const Vb0 = lds_array<T, Fill::SIZE, 1>();
     T* const Kb1 = lds_array<T, Fill::SIZE, 2>();
@@ -182,22 +187,23 @@ __device__ __forceinline__ void score_forward(const ScoreParams& p) {
     const T* V = slice<T>(p.v, p.vs, w.b, w.hk);
     const bool docs = p.q_doc != nullptr;
     const int32_t* kdoc = docs ? p.k_doc + (int64_t)w.b * p.sk : nullptr;
-    const ScoreMask mask = {p.causal, p.prefix ? p.prefix[w.b] : 0, p.sk};
+    const int prefix = p.prefix ? p.prefix[w.b] : 0;
     const float slope = MOD && p.slopes ? p.slopes[h] * kLog2e : 0.0f;
     const bool cap = MOD && p.cap_log2e != 0.0f;
     // scores leave the QK^T chains raw, and the scale goes into the exponent; modified ones are in log2 units
     const float c = MOD ? 1.0f : p.scale_log2e;
 
     v8 qreg[MT][NDC];
-    int qd[MT];
+    int qd[MT], limit[MT];   // a row's document, and the keys before which it may see
     f32x4 o[MT][NDB];
     float m[MT], l[MT], ref[MT];   // l: the lane's share of the row's sum; ref: m, or 0 while m = -inf
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
         const int row = row0 + 16 * t + li;
 #pragma unroll
-        for (int dc = 0; dc < NDC; ++dc) qreg[t][dc] = global_row<T>(Q, p.qs.s, row, p.sq, 32 * dc + 8 * g, p.d, p.vec);
+        for (int dc = 0; dc < NDC; ++dc) qreg[t][dc] = global_row<T, VEC>(Q, p.qs.s, row, p.sq, 32 * dc + 8 * g, p.d);
         qd[t] = docs && row < p.sq ? p.q_doc[(int64_t)w.b * p.sq + row] : -1;
+        limit[t] = docs && qd[t] < 0 ? 0 : min(p.sk, key_limit(p, prefix, p.q_start + row));
 #pragma unroll
         for (int j = 0; j < NDB; ++j) o[t][j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
         m[t] = OPS_NEG_INF;
@@ -211,9 +217,9 @@ __device__ __forceinline__ void score_forward(const ScoreParams& p) {
         qr = doc_range(p.q_rng + (int64_t)w.b * 2 * ((p.sq + kDocTile - 1) / kDocTile), q0, q1);
         krng = p.k_rng + (int64_t)w.b * 2 * ((p.sk + kDocTile - 1) / kDocTile);
     }
-    auto test = [&](int st, bool* part) -> bool { return key_stage<SK>(p, mask, st, q0, q1, docs, qr, krng, part); };
+    auto test = [&](int st, bool* part) -> bool { return key_stage<SK>(p, prefix, st, q0, q1, docs, qr, krng, part); };
     Stages<decltype(test)> stages((p.sk + SK - 1) / SK, lane, test);
-    const Fill kfill(p.ks.s, p.d, p.vec, wave, lane), vfill(p.vs.s, p.d, p.vec, wave, lane);
+    const Fill kfill(p.ks.s, p.d, wave, lane), vfill(p.vs.s, p.d, wave, lane);
     auto fill_k = [&](int st, T* dst, int* ids) {
         kfill(dst, K, st * SK, p.sk);
         if (docs && wave == 0 && lane < SK) fill_words(ids, kdoc + st * SK, p.sk - st * SK, lane);
@@ -276,18 +282,20 @@ __device__ __forceinline__ void score_forward(const ScoreParams& p) {
     auto hide = [&](int k0, const int* ids) {
 #pragma unroll
         for (int b = 0; b < KB; ++b) {
-            i32x4 kd = {0, 0, 0, 0};
-            if (docs) kd = *reinterpret_cast<const i32x4*>(ids + 16 * b + 4 * g);
+            const int key = k0 + 16 * b + 4 * g;
+            if (docs) {
+                const i32x4 kd = *reinterpret_cast<const i32x4*>(ids + 16 * b + 4 * g);
 #pragma unroll
-            for (int t = 0; t < MT; ++t) {
-                const int pos = p.q_start + row0 + 16 * t + li;
+                for (int t = 0; t < MT; ++t)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    bool see = mask.seen(k0 + 16 * b + 4 * g + r, pos);
-                    if (docs) see = see && qd[t] >= 0 && kd[r] == qd[t];
-                    if (!see) s[t][b][r] = OPS_NEG_INF;
-                }
+                    for (int r = 0; r < 4; ++r)
+                        if (kd[r] != qd[t]) s[t][b][r] = OPS_NEG_INF;
             }
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (key + r >= limit[t]) s[t][b][r] = OPS_NEG_INF;
         }
     };
     v8 pb[MT][NCH];
@@ -347,7 +355,7 @@ __device__ __forceinline__ void score_forward(const ScoreParams& p) {
     // whether some row of the wave sees some key of the stage (as far as causal and prefix tell)
     auto active = [&](int st) -> bool {
         if (st < 0 || row0 >= p.sq) return false;
-        return !p.causal || st * SK <= p.q_start + row0 + 16 * MT - 1 || st * SK < mask.prefix;
+        return !p.causal || st * SK <= p.q_start + row0 + 16 * MT - 1 || st * SK < prefix;
     };
 
     bool masked, masked_next = false;
@@ -402,28 +410,29 @@ __device__ __forceinline__ void score_forward(const ScoreParams& p) {
         step(std::integral_constant<int, 1>{});
     }
 
-    T* O = slice<T>(p.out, p.os, w.b, h);
+    const ScoreParams lp = late_params<ScoreParams>();
+    T* O = slice<T>(lp.out, lp.os, w.b, h);
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
         const int row = row0 + 16 * t + li;
         const float lt = row4_sum(l[t]);
-        if (row >= p.sq) continue;
+        if (row >= lp.sq) continue;
         const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;
 #pragma unroll
-        for (int j = 0; j < NDB; ++j) store4<T>(O + row * p.os.s, 16 * j + 4 * g, p.d, p.ovec, o[t][j] * inv);
-        if (p.lse && g == 0) {
+        for (int j = 0; j < NDB; ++j) store4<T, VEC>(O + row * lp.os.s, 16 * j + 4 * g, lp.d, o[t][j] * inv);
+        if (lp.lse && g == 0) {
             const float lse = (m[t] * c + __builtin_log2f(lt) - kProbLog2<T>) * kLn2;
-            p.lse[((int64_t)w.b * p.heads + h) * p.sq + row] = lt == 0.0f ? OPS_NEG_INF : lse;
+            lp.lse[((int64_t)w.b * lp.heads + h) * lp.sq + row] = lt == 0.0f ? OPS_NEG_INF : lse;
         }
     }
     if (*Special) {
         __threadfence();
         each_masked(test, stages.count, lane, [&](int stage) {
             add_specials<T, T, true>(
-                stage * SK, min(stage * SK + SK, p.sk), min(16 * MT, p.sq - row0), p.d, lane,
-                [&](int key) { return V + key * p.vs.s; },
-                [&](int key, int r) { return pair_seen(p, mask, w.b, row0 + r, key); },
-                [&](int r) { return O + (row0 + r) * p.os.s; });
+                stage * SK, min(stage * SK + SK, lp.sk), min(16 * MT, lp.sq - row0), lp.d, lane,
+                [&](int key) { return V + key * lp.vs.s; },
+                [&](int key, int r) { return pair_seen(lp, prefix, w.b, row0 + r, key); },
+                [&](int r) { return O + (row0 + r) * lp.os.s; });
         });
     }
 }
@@ -434,7 +443,7 @@ __device__ __forceinline__ void score_forward(const ScoreParams& p) {
 
 // delta = dO . O and lse2 = lse log2(e) of every row, a group of 16 lanes a row.  Empty rows get lse2 = +inf: their
 // weights e^(z - lse) then come out as 0.
-template <typename T>
+template <typename T, bool VEC>
 __device__ __forceinline__ void score_delta(const ScoreParams& p) {
     const int64_t row = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 4;
     const int li = threadIdx.x & 15;
@@ -445,8 +454,8 @@ __device__ __forceinline__ void score_delta(const ScoreParams& p) {
     const T* g = slice<T>(p.dout, p.dos, b, h);
     float sum = 0.0f;
     for (int col = 8 * li; col < p.d; col += 128) {
-        const auto x = global_row<T>(o, p.os.s, i, p.sq, col, p.d, p.vec);
-        const auto y = global_row<T>(g, p.dos.s, i, p.sq, col, p.d, p.vec);
+        const auto x = global_row<T, VEC>(o, p.os.s, i, p.sq, col, p.d);
+        const auto y = global_row<T, VEC>(g, p.dos.s, i, p.sq, col, p.d);
 #pragma unroll
         for (int e = 0; e < 8; ++e) sum += float(x[e]) * float(y[e]);
     }
@@ -481,13 +490,13 @@ __device__ __forceinline__ void weigh(const ScoreParams& p, bool cap, f32x4 s, f
 }
 
 // dQ: query rows kept, keys walked.  Four waves of MT 16-row tiles; K and V tiles double-buffered, one barrier a stage.
-template <typename T, int D, int MT, bool MOD>
+template <typename T, int D, int MT, bool MOD, bool VEC>
 __device__ __forceinline__ void score_dq(const ScoreParams& p) {
     using M = Mma<T>;
     using v8 = typename M::v8;
     constexpr int NW = 4, SK = kStageKeys<T, D>, BQ = 16 * MT * NW;
     constexpr int NCH = SK / 32, NDC = D / 32, NDB = D / 16, LD = D + kPad<T>;
-    using Fill = TileFill<T, D, SK, NW>;
+    using Fill = TileFill<T, D, SK, NW, VEC>;
     T* const Kb0 = lds_array<T, Fill::SIZE, 0>();
     T* const Vb0 = lds_array<T, Fill::SIZE, 1>();
     T* const Kb1 = lds_array<T, Fill::SIZE, 2>();
@@ -507,12 +516,12 @@ __device__ __forceinline__ void score_dq(const ScoreParams& p) {
     const T* V = slice<T>(p.v, p.vs, w.b, w.hk);
     const bool docs = p.q_doc != nullptr;
     const int32_t* kdoc = docs ? p.k_doc + (int64_t)w.b * p.sk : nullptr;
-    const ScoreMask mask = {p.causal, p.prefix ? p.prefix[w.b] : 0, p.sk};
+    const int prefix = p.prefix ? p.prefix[w.b] : 0;
     const float slope = MOD && p.slopes ? p.slopes[h] * kLog2e : 0.0f;
     const bool cap = MOD && p.cap_log2e != 0.0f;
 
     v8 qreg[MT][NDC], doreg[MT][NDC];
-    int qd[MT];
+    int qd[MT], limit[MT];
     f32x4 dq[MT][NDB];
     float lse2[MT], delta[MT];
 #pragma unroll
@@ -521,12 +530,13 @@ __device__ __forceinline__ void score_dq(const ScoreParams& p) {
         const int64_t at = ((int64_t)w.b * p.heads + h) * p.sq + row;
 #pragma unroll
         for (int dc = 0; dc < NDC; ++dc) {
-            qreg[t][dc] = global_row<T>(Q, p.qs.s, row, p.sq, 32 * dc + 8 * g, p.d, p.vec);
-            doreg[t][dc] = global_row<T>(dO, p.dos.s, row, p.sq, 32 * dc + 8 * g, p.d, p.vec);
+            qreg[t][dc] = global_row<T, VEC>(Q, p.qs.s, row, p.sq, 32 * dc + 8 * g, p.d);
+            doreg[t][dc] = global_row<T, VEC>(dO, p.dos.s, row, p.sq, 32 * dc + 8 * g, p.d);
         }
         qd[t] = docs && row < p.sq ? p.q_doc[(int64_t)w.b * p.sq + row] : -1;
         lse2[t] = row < p.sq ? p.lse2[at] : -OPS_NEG_INF;
         delta[t] = row < p.sq ? p.delta[at] : 0.0f;
+        limit[t] = (docs && qd[t] < 0) || lse2[t] == -OPS_NEG_INF ? 0 : min(p.sk, key_limit(p, prefix, p.q_start + row));
 #pragma unroll
         for (int j = 0; j < NDB; ++j) dq[t][j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
     }
@@ -537,9 +547,9 @@ __device__ __forceinline__ void score_dq(const ScoreParams& p) {
         qr = doc_range(p.q_rng + (int64_t)w.b * 2 * ((p.sq + kDocTile - 1) / kDocTile), q0, q1);
         krng = p.k_rng + (int64_t)w.b * 2 * ((p.sk + kDocTile - 1) / kDocTile);
     }
-    auto test = [&](int st, bool* part) -> bool { return key_stage<SK>(p, mask, st, q0, q1, docs, qr, krng, part); };
+    auto test = [&](int st, bool* part) -> bool { return key_stage<SK>(p, prefix, st, q0, q1, docs, qr, krng, part); };
     Stages<decltype(test)> stages((p.sk + SK - 1) / SK, lane, test);
-    const Fill kfill(p.ks.s, p.d, p.vec, wave, lane), vfill(p.vs.s, p.d, p.vec, wave, lane);
+    const Fill kfill(p.ks.s, p.d, wave, lane), vfill(p.vs.s, p.d, wave, lane);
     auto fill = [&](int st, T* k, T* v, int* ids) {
         kfill(k, K, st * SK, p.sk);
         vfill(v, V, st * SK, p.sk);
@@ -547,7 +557,7 @@ __device__ __forceinline__ void score_dq(const ScoreParams& p) {
     };
     auto active = [&](int st) -> bool {
         if (row0 >= p.sq) return false;
-        return !p.causal || st * SK <= p.q_start + row0 + 16 * MT - 1 || st * SK < mask.prefix;
+        return !p.causal || st * SK <= p.q_start + row0 + 16 * MT - 1 || st * SK < prefix;
     };
 
     bool masked = false, masked_next = false;
@@ -598,14 +608,15 @@ __device__ __forceinline__ void score_dq(const ScoreParams& p) {
                         weigh<T, MOD>(p, cap, s[t][b], dp[t][b], (f32x4){lse2[t], lse2[t], lse2[t], lse2[t]},
                                       (f32x4){delta[t], delta[t], delta[t], delta[t]}, slope, (float)(pos - key), &x, &ds);
                         if (masked) {
-                            i32x4 kd = {0, 0, 0, 0};
-                            if (docs) kd = *reinterpret_cast<const i32x4*>(ids + 32 * i + 16 * b + 4 * g);
+                            if (docs) {
+                                const i32x4 kd = *reinterpret_cast<const i32x4*>(ids + 32 * i + 16 * b + 4 * g);
 #pragma unroll
-                            for (int r = 0; r < 4; ++r) {
-                                bool see = mask.seen(key + r, pos) && lse2[t] != -OPS_NEG_INF;
-                                if (docs) see = see && qd[t] >= 0 && kd[r] == qd[t];
-                                if (!see) ds[r] = 0.0f;
+                                for (int r = 0; r < 4; ++r)
+                                    if (kd[r] != qd[t]) ds[r] = 0.0f;
                             }
+#pragma unroll
+                            for (int r = 0; r < 4; ++r)
+                                if (key + r >= limit[t]) ds[r] = 0.0f;
                         }
 #pragma unroll
                         for (int r = 0; r < 4; ++r) db[t][0][4 * b + r] = T(ds[r]);
@@ -636,22 +647,23 @@ __device__ __forceinline__ void score_dq(const ScoreParams& p) {
         if (st < 0) break;
         step(std::integral_constant<int, 1>{});
     }
-    T* out = slice<T>(p.dq, p.dqs, w.b, h);
+    const ScoreParams lp = late_params<ScoreParams>();
+    T* out = slice<T>(lp.dq, lp.dqs, w.b, h);
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
         const int row = row0 + 16 * t + li;
-        if (row >= p.sq) continue;
+        if (row >= lp.sq) continue;
 #pragma unroll
-        for (int j = 0; j < NDB; ++j) store4<T>(out + row * p.dqs.s, 16 * j + 4 * g, p.d, p.ovec, dq[t][j] * p.scale);
+        for (int j = 0; j < NDB; ++j) store4<T, VEC>(out + row * lp.dqs.s, 16 * j + 4 * g, lp.d, dq[t][j] * lp.scale);
     }
     if (*Special) {
         __threadfence();
         each_masked(test, stages.count, lane, [&](int stage) {
             add_specials<T, T, false>(
-                stage * SK, min(stage * SK + SK, p.sk), min(16 * MT, p.sq - row0), p.d, lane,
-                [&](int key) { return K + key * p.ks.s; },
-                [&](int key, int r) { return pair_seen(p, mask, w.b, row0 + r, key); },
-                [&](int r) { return out + (row0 + r) * p.dqs.s; });
+                stage * SK, min(stage * SK + SK, lp.sk), min(16 * MT, lp.sq - row0), lp.d, lane,
+                [&](int key) { return K + key * lp.ks.s; },
+                [&](int key, int r) { return pair_seen(lp, prefix, w.b, row0 + r, key); },
+                [&](int r) { return out + (row0 + r) * lp.dqs.s; });
         });
     }
 }
@@ -659,13 +671,13 @@ __device__ __forceinline__ void score_dq(const ScoreParams& p) {
 // dK and dV: key rows kept, the queries of every head of the group walked.  Four waves
 // of MT 16-row tiles; Q and dO tiles double-buffered, one barrier a stage.  A kv head's sums over its
 // query heads are formed here, in head order.
-template <typename T, int D, int MT, bool MOD>
+template <typename T, int D, int MT, bool MOD, bool VEC>
 __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
     using M = Mma<T>;
     using v8 = typename M::v8;
     constexpr int NW = 4, SQ = kStageKeys<T, D>, BK = 16 * MT * NW;
     constexpr int NCH = SQ / 32, NDC = D / 32, NDB = D / 16, LD = D + kPad<T>;
-    using Fill = TileFill<T, D, SQ, NW>;
+    using Fill = TileFill<T, D, SQ, NW, VEC>;
     T* const Qb0 = lds_array<T, Fill::SIZE, 0>();
     T* const Ob0 = lds_array<T, Fill::SIZE, 1>();
     T* const Qb1 = lds_array<T, Fill::SIZE, 2>();
@@ -682,7 +694,7 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
     const T* K = slice<T>(p.k, p.ks, w.b, w.hk);
     const T* V = slice<T>(p.v, p.vs, w.b, w.hk);
     const bool docs = p.q_doc != nullptr;
-    const ScoreMask mask = {p.causal, p.prefix ? p.prefix[w.b] : 0, p.sk};
+    const int prefix = p.prefix ? p.prefix[w.b] : 0;
     const bool cap = MOD && p.cap_log2e != 0.0f;
 
     v8 kreg[MT][NDC], vreg[MT][NDC];
@@ -693,8 +705,8 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
         const int key = key0 + 16 * t + li;
 #pragma unroll
         for (int dc = 0; dc < NDC; ++dc) {
-            kreg[t][dc] = global_row<T>(K, p.ks.s, key, p.sk, 32 * dc + 8 * g, p.d, p.vec);
-            vreg[t][dc] = global_row<T>(V, p.vs.s, key, p.sk, 32 * dc + 8 * g, p.d, p.vec);
+            kreg[t][dc] = global_row<T, VEC>(K, p.ks.s, key, p.sk, 32 * dc + 8 * g, p.d);
+            vreg[t][dc] = global_row<T, VEC>(V, p.vs.s, key, p.sk, 32 * dc + 8 * g, p.d);
         }
         kd[t] = docs && key < p.sk ? p.k_doc[(int64_t)w.b * p.sk + key] : -1;
 #pragma unroll
@@ -711,15 +723,15 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
         const int q0 = st * SQ, q1 = min(q0 + SQ, p.sq);
         bool v = true;
         if (p.causal) {
-            v = p.q_start + q1 - 1 >= kbeg || kbeg < mask.prefix;
-            if (!(p.q_start + q0 >= kend - 1 || kend <= mask.prefix)) *part = true;
+            v = p.q_start + q1 - 1 >= kbeg || kbeg < prefix;
+            if (!(p.q_start + q0 >= kend - 1 || kend <= prefix)) *part = true;
         }
         if (docs && v) v = docs_meet(kr, doc_range(qrng, q0 / kDocTile), part);
         return v;
     };
     const int nst = (p.sq + SQ - 1) / SQ;
     Stages<decltype(test)> stages(nst, lane, test);
-    const Fill qfill(p.qs.s, p.d, p.vec, wave, lane), ofill(p.dos.s, p.d, p.vec, wave, lane);
+    const Fill qfill(p.qs.s, p.d, wave, lane), ofill(p.dos.s, p.d, wave, lane);
     // the next (head, stage): the stages of one head of the group after the other
     int head = 0;
     auto next = [&](bool* m) -> int {
@@ -745,7 +757,7 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
     };
     auto active = [&](int st) -> bool {
         if (key0 >= p.sk) return false;
-        return !p.causal || p.q_start + st * SQ + SQ - 1 >= key0 || key0 < mask.prefix;
+        return !p.causal || p.q_start + st * SQ + SQ - 1 >= key0 || key0 < prefix;
     };
 
     bool masked = false, masked_next = false;
@@ -799,14 +811,15 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
                         f32x4 x, ds;
                         weigh<T, MOD>(p, cap, s[t][b], dp[t][b], lse2, delta, slope, (float)(key - pos), &x, &ds);
                         if (masked) {
-                            i32x4 qd = {0, 0, 0, 0};
-                            if (docs) qd = *reinterpret_cast<const i32x4*>(words + 128 + at);
+                            if (docs) {
+                                const i32x4 qd = *reinterpret_cast<const i32x4*>(words + 128 + at);
 #pragma unroll
-                            for (int r = 0; r < 4; ++r) {
-                                bool see = mask.seen(key, pos + r) && lse2[r] != -OPS_NEG_INF;
-                                if (docs) see = see && kd[t] >= 0 && qd[r] == kd[t];
-                                if (!see) x[r] = ds[r] = 0.0f;
+                                for (int r = 0; r < 4; ++r)
+                                    if (qd[r] != kd[t] || kd[t] < 0) x[r] = ds[r] = 0.0f;
                             }
+#pragma unroll
+                            for (int r = 0; r < 4; ++r)
+                                if (key >= key_limit(p, prefix, pos + r) || lse2[r] == -OPS_NEG_INF) x[r] = ds[r] = 0.0f;
                         }
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
@@ -845,33 +858,34 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
         if (st < 0) break;
         step(std::integral_constant<int, 1>{});
     }
-    T* outk = p.dk ? slice<T>(p.dk, p.dks, w.b, w.hk) : nullptr;
-    T* outv = p.dv ? slice<T>(p.dv, p.dvs, w.b, w.hk) : nullptr;
+    const ScoreParams lp = late_params<ScoreParams>();
+    T* outk = lp.dk ? slice<T>(lp.dk, lp.dks, w.b, w.hk) : nullptr;
+    T* outv = lp.dv ? slice<T>(lp.dv, lp.dvs, w.b, w.hk) : nullptr;
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
         const int key = key0 + 16 * t + li;
-        if (key >= p.sk) continue;
+        if (key >= lp.sk) continue;
 #pragma unroll
         for (int j = 0; j < NDB; ++j) {
-            if (outk) store4<T>(outk + key * p.dks.s, 16 * j + 4 * g, p.d, p.ovec, dk[t][j] * p.scale);
-            if (outv) store4<T>(outv + key * p.dvs.s, 16 * j + 4 * g, p.d, p.ovec, dv[t][j]);
+            if (outk) store4<T, VEC>(outk + key * lp.dks.s, 16 * j + 4 * g, lp.d, dk[t][j] * lp.scale);
+            if (outv) store4<T, VEC>(outv + key * lp.dvs.s, 16 * j + 4 * g, lp.d, dv[t][j]);
         }
     }
     if (*Special) {
         __threadfence();
-        for (int x = 0; x < p.group; ++x) {
-            const int h = w.hk * p.group + x;
-            const T* Q = slice<T>(p.q, p.qs, w.b, h);
-            const T* dO = slice<T>(p.dout, p.dos, w.b, h);
+        for (int x = 0; x < lp.group; ++x) {
+            const int h = w.hk * lp.group + x;
+            const T* Q = slice<T>(lp.q, lp.qs, w.b, h);
+            const T* dO = slice<T>(lp.dout, lp.dos, w.b, h);
             each_masked(test, nst, lane, [&](int stage) {
-                const int from = stage * SQ, to = min(from + SQ, p.sq), n = min(16 * MT, p.sk - key0);
-                auto see = [&](int row, int r) { return pair_seen(p, mask, w.b, row, key0 + r); };
+                const int from = stage * SQ, to = min(from + SQ, lp.sq), n = min(16 * MT, lp.sk - key0);
+                auto see = [&](int row, int r) { return pair_seen(lp, prefix, w.b, row, key0 + r); };
                 if (outk)
-                    add_specials<T, T, false>(from, to, n, p.d, lane, [&](int row) { return Q + row * p.qs.s; }, see,
-                                              [&](int r) { return outk + (key0 + r) * p.dks.s; });
+                    add_specials<T, T, false>(from, to, n, lp.d, lane, [&](int row) { return Q + row * lp.qs.s; }, see,
+                                              [&](int r) { return outk + (key0 + r) * lp.dks.s; });
                 if (outv)
-                    add_specials<T, T, true>(from, to, n, p.d, lane, [&](int row) { return dO + row * p.dos.s; }, see,
-                                             [&](int r) { return outv + (key0 + r) * p.dvs.s; });
+                    add_specials<T, T, true>(from, to, n, lp.d, lane, [&](int row) { return dO + row * lp.dos.s; }, see,
+                                             [&](int r) { return outv + (key0 + r) * lp.dvs.s; });
             });
         }
     }
@@ -905,17 +919,21 @@ extern "C" __global__ __launch_bounds__(256) void fa_score_doc_ranges(ScoreParam
 
 #define PASTE_(a, b, c, d) a##b##c##d
 #define PASTE(a, b, c, d) PASTE_(a, b, c, d)
-extern "C" __global__ __launch_bounds__(256) void PASTE(fa_score_delta_, OPS_NAME, , )(ScoreParams p) {
-    score_delta<OPS_T>(p);
-}
-#define KERNEL(F, D, MT, MOD, TAG, WAVES)                                                             \
+#define DELTA(VEC, TAG)                                                                                       \
+    extern "C" __global__ __launch_bounds__(256) void PASTE(fa_score_delta_, OPS_NAME, , TAG)(ScoreParams p) { \
+        score_delta<OPS_T, VEC>(p);                                                                           \
+    }
+DELTA(true, )
+DELTA(false, s)
+#define KERNEL(F, D, MT, MOD, VEC, TAG, WAVES)                                                        \
     extern "C" __global__ __launch_bounds__(256, WAVES) void PASTE(fa_score_##F##_, OPS_NAME, _d##D##_t##MT, TAG)( \
         ScoreParams p) {                                                                              \
-        score_##F<OPS_T, D, MT, MOD>(p);                                                              \
+        score_##F<OPS_T, D, MT, MOD, VEC>(p);                                                         \
     }
-#define KERNELS(F, D, MT, WAVES)       \
-    KERNEL(F, D, MT, false, , WAVES)   \
-    KERNEL(F, D, MT, true, m, WAVES)
+// plain scores, modified ones (m), and any alignment (s)
+#define KERNELS(F, D, MT, WAVES)             \
+    KERNEL(F, D, MT, false, true, , WAVES)   \
+    KERNEL(F, D, MT, true, true, m, WAVES)
 KERNELS(forward, 64, 1, 2)
 KERNELS(forward, 128, 1, 2)
 KERNELS(dq, 64, 1, 2)
@@ -923,6 +941,13 @@ KERNELS(dq, 128, 1, 2)
 KERNELS(dkv, 64, 1, 2)
 KERNELS(dkv, 128, 1, 2)
 KERNELS(dkv, 256, 1, 1)
+#define SLOW(F, W64, W128, W256)              \
+    KERNEL(F, 64, 1, true, false, s, W64)     \
+    KERNEL(F, 128, 1, true, false, s, W128)   \
+    KERNEL(F, 256, 1, true, false, s, W256)
+SLOW(forward, 2, 1, 1)
+SLOW(dq, 2, 1, 1)
+SLOW(dkv, 2, 1, 1)
 #ifdef OPS_16BIT
 KERNELS(forward, 64, 2, 2)
 KERNELS(forward, 128, 2, 2)
