@@ -178,13 +178,35 @@ int resolve_scale(float scale, float softcap, size_t d, ScoreScale* out) {
     return FA_OK;
 }
 
-// 16-row tiles a wave of the score kernels, which have four waves: two where that makes at
-// least `least` workgroups for every CU (what a wave reads from LDS serves both tiles).
+// 16-row tiles a wave of the score kernels, which have four waves: two where that still makes
+// workgroups enough, `least` for every CU (what a wave reads from LDS serves both tiles).
 int score_tiles(int dtype, int D, size_t rows, size_t slices, size_t least, int num_cus) {
     if (dtype == FA_DTYPE_F32 || D > 128) return 1;
     return (rows + 127) / 128 * slices >= least * static_cast<size_t>(num_cus) ? 2 : 1;
 }
-constexpr size_t kOpsMaxGrid = size_t(1) << 22;   // workgroups: threads of a launch stay in 32 bits
+// Causal workgroups differ in length, so that a single round of them ends late.
+size_t score_rounds(const fa_score_config& c) { return c.causal ? 4 : 2; }
+
+// Plan of the dK / dV kernel: tiles a wave, and the workgroups that share the heads of a group.
+struct DkvPlan {
+    int mt, splits;
+    size_t blocks, floats;
+};
+DkvPlan plan_dkv(const fa_score_config& c, int D, bool vec, int num_cus) {
+    DkvPlan r{};
+    const size_t nkv = c.batch * c.kv_heads, group = c.heads / c.kv_heads;
+    r.mt = vec && D == 64 ? score_tiles(c.dtype, D, c.seq_len_k, nkv, 4, num_cus) : 1;
+    r.blocks = (c.seq_len_k + 64 * r.mt - 1) / (64 * r.mt);
+    size_t s = 1;
+    while (s < group && r.blocks * nkv * s < 4 * static_cast<size_t>(num_cus)) {
+        ++s;
+        while (group % s != 0) ++s;
+    }
+    r.splits = static_cast<int>(s);
+    r.floats = s > 1 ? 2 * s * nkv * c.seq_len_k * D : 0;
+    return r;
+}
+constexpr size_t kOpsMaxGrid = size_t(1) << 23;   // workgroups: threads of a launch stay in 32 bits
 
 size_t doc_tiles(size_t n) { return (n + kDocTile - 1) / kDocTile; }
 
@@ -368,7 +390,7 @@ int launch_rotary(int dev, hipStream_t stream, int dtype, RotParams* p, bool wid
     while (ht < static_cast<size_t>(heads) && tokens * p->cols * ht < fill) ht *= 2;
     p->hthreads = static_cast<int>(std::min<size_t>(ht, heads));
     const size_t grid = (tokens * p->cols * p->hthreads + 255) / 256;
-    if (grid > 2 * kOpsMaxGrid) return FA_ERR_UNSUPPORTED;
+    if (grid > kOpsMaxGrid) return FA_ERR_UNSUPPORTED;
     char name[64];
     std::snprintf(name, sizeof(name), "fa_rotary_%s_%d", dtype_name(dtype), wide ? 1 : 0);
     return ops_launch(dev, kRotaryModule, name, grid, 256, p, stream);
@@ -417,7 +439,7 @@ int fa_score_forward(void* stream_, const fa_score_config* c, const void* q, con
     fill_score(*c, sc, &p);
     p.q = q, p.k = k, p.v = v, p.out = out, p.lse = lse;
     p.qs = lq.st, p.ks = lk.st, p.vs = lv.st, p.os = lo.st;
-    const int mt = vec ? score_tiles(c->dtype, D, c->seq_len_q, c->batch * c->heads, 2, g_dev[dev].num_cus) : 1;
+    const int mt = vec ? score_tiles(c->dtype, D, c->seq_len_q, c->batch * c->heads, score_rounds(*c), g_dev[dev].num_cus) : 1;
     p.nqb = static_cast<int>((c->seq_len_q + 64 * mt - 1) / (64 * mt));
     OpsWorkspace ws;
     if (c->q_doc) {
@@ -457,7 +479,7 @@ int fa_score_backward(void* stream_, const fa_score_config* c, const void* q, co
     const int D = ops_pad_d(d);
     const size_t rows = c->batch * c->heads * sq, dgrid = (rows + 15) / 16;
     if (c->batch * c->heads > kOpsMaxGrid || (sq + 63) / 64 * c->batch * c->heads > kOpsMaxGrid ||
-        (sk + 63) / 64 * c->batch * c->kv_heads > kOpsMaxGrid || dgrid > 4 * kOpsMaxGrid)
+        (sk + 63) / 64 * c->batch * c->heads > kOpsMaxGrid || dgrid > kOpsMaxGrid)
         return FA_ERR_UNSUPPORTED;
     int dev;
     if ((rc = ops_begin(&dev, of_type(kScoreModule, c->dtype))) != FA_OK) return rc;
@@ -472,8 +494,12 @@ int fa_score_backward(void* stream_, const fa_score_config* c, const void* q, co
                      vec_ok(dout, ldo, d) && ovec_ok(dq, ldq, es) && ovec_ok(dk, ldk, es) && ovec_ok(dv, ldv, es);
     OpsWorkspace ws;
     const size_t rng = doc_range_bytes(*c);
-    if ((rc = ws.get(dev, stream, 2 * rows * sizeof(float) + rng + 16)) != FA_OK) return rc;
-    p.lse2 = static_cast<float*>(ws.ptr);
+    const DkvPlan dkv = plan_dkv(*c, D, vec, g_dev[dev].num_cus);
+    // partial sums first: they are read and written 16 bytes at a time
+    const size_t floats = dk || dv ? dkv.floats : 0;
+    if ((rc = ws.get(dev, stream, (floats + 2 * rows) * sizeof(float) + rng + 16)) != FA_OK) return rc;
+    p.part = static_cast<float*>(ws.ptr);
+    p.lse2 = p.part + floats;
     p.delta = p.lse2 + rows;
     char name[64];
     if (c->q_doc) rc = launch_doc_ranges(dev, of_type(kScoreModule, c->dtype), stream, &p, reinterpret_cast<int32_t*>(p.delta + rows));
@@ -483,13 +509,19 @@ int fa_score_backward(void* stream_, const fa_score_config* c, const void* q, co
     }
     const char* mod = !vec ? "s" : c->slopes || c->softcap > 0.0f ? "m" : "";
     if (rc == FA_OK && (dk || dv)) {
-        const int mt = vec ? score_tiles(c->dtype, D, sk, c->batch * c->kv_heads, 1, g_dev[dev].num_cus) : 1;
-        p.nqb = static_cast<int>((sk + 64 * mt - 1) / (64 * mt));
-        std::snprintf(name, sizeof(name), "fa_score_dkv_%s_d%d_t%d%s", dtype_name(c->dtype), D, mt, mod);
-        rc = ops_launch(dev, of_type(kScoreModule, c->dtype), name, c->batch * c->kv_heads * p.nqb, 256, &p, stream);
+        p.nqb = static_cast<int>(dkv.blocks);
+        p.splits = dkv.splits;
+        std::snprintf(name, sizeof(name), "fa_score_dkv_%s_d%d_t%d%s", dtype_name(c->dtype), D, dkv.mt, mod);
+        rc = ops_launch(dev, of_type(kScoreModule, c->dtype), name, dkv.blocks * c->batch * c->kv_heads * dkv.splits, 256, &p,
+                        stream);
+        if (rc == FA_OK && dkv.splits > 1) {
+            std::snprintf(name, sizeof(name), "fa_score_dkv_sum_%s_d%d%s", dtype_name(c->dtype), D, vec ? "" : "s");
+            const size_t threads = c->batch * c->kv_heads * sk * (D / 4);
+            rc = ops_launch(dev, of_type(kScoreModule, c->dtype), name, (threads + 255) / 256, 256, &p, stream);
+        }
     }
     if (rc == FA_OK && dq) {
-        const int mt = vec ? score_tiles(c->dtype, D, sq, c->batch * c->heads, 2, g_dev[dev].num_cus) : 1;
+        const int mt = vec ? score_tiles(c->dtype, D, sq, c->batch * c->heads, score_rounds(*c), g_dev[dev].num_cus) : 1;
         p.nqb = static_cast<int>((sq + 64 * mt - 1) / (64 * mt));
         std::snprintf(name, sizeof(name), "fa_score_dq_%s_d%d_t%d%s", dtype_name(c->dtype), D, mt, mod);
         rc = ops_launch(dev, of_type(kScoreModule, c->dtype), name, c->batch * c->heads * p.nqb, 256, &p, stream);

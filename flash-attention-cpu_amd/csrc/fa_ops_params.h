@@ -27,6 +27,8 @@ struct ScoreParams {
     int batch, heads, kv_heads, group, sq, sk, d;
     int causal, q_start;
     int nqb;                  // query (dK/dV: key) blocks a slice
+    int splits;               // dK/dV: workgroups that share a key block, each some heads of the group
+    float* part;              // their sums: [dK, dV][split][batch, kv head][key][padded d]
     float scale;              // of the scores
     float scale_log2e;
     float cap_in;             // 2 log2(e) scale / softcap: exponent of the cap's tanh

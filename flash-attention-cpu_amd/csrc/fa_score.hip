@@ -668,9 +668,31 @@ __device__ __forceinline__ void score_dq(const ScoreParams& p) {
     }
 }
 
+// What was cleaned from the Q and dO tiles of heads [first, first + count), to the n key rows from key0 that see it.
+template <typename T, typename O, int SQ, typename Test>
+__device__ __forceinline__ void dkv_specials(const ScoreParams& p, Test test, int nst, int prefix, int b, int first,
+                                             int count, int key0, int n, int lane, O* outk, int64_t sk, O* outv,
+                                             int64_t sv) {
+    __threadfence();
+    for (int h = first; h < first + count; ++h) {
+        const T* Q = slice<T>(p.q, p.qs, b, h);
+        const T* dO = slice<T>(p.dout, p.dos, b, h);
+        each_masked(test, nst, lane, [&](int stage) {
+            const int from = stage * SQ, to = min(from + SQ, p.sq), keys = min(n, p.sk - key0);
+            auto see = [&](int row, int r) { return pair_seen(p, prefix, b, row, key0 + r); };
+            if (outk)
+                add_specials<T, O, false>(from, to, keys, p.d, lane, [&](int row) { return Q + row * p.qs.s; }, see,
+                                          [&](int r) { return outk + (key0 + r) * sk; });
+            if (outv)
+                add_specials<T, O, true>(from, to, keys, p.d, lane, [&](int row) { return dO + row * p.dos.s; }, see,
+                                         [&](int r) { return outv + (key0 + r) * sv; });
+        });
+    }
+}
+
 // dK and dV: key rows kept, the queries of every head of the group walked.  Four waves
 // of MT 16-row tiles; Q and dO tiles double-buffered, one barrier a stage.  A kv head's sums over its
-// query heads are formed here, in head order.
+// query heads are formed here, in head order, or by score_dkv_sum where workgroups share them.
 template <typename T, int D, int MT, bool MOD, bool VEC>
 __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
     using M = Mma<T>;
@@ -688,8 +710,9 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, li = lane & 15;
-    // a workgroup owns whole (batch, kv head) columns: no group in the map; the first key blocks have most queries where causal
-    const Work w = find_work(gridDim.x - 1 - blockIdx.x, p.nqb, p.batch * p.kv_heads, 1, p.kv_heads);
+    // a workgroup takes heads first .. first + count - 1 of a kv head's group; the first key blocks have most queries where causal
+    const Work w = find_work(gridDim.x - 1 - blockIdx.x, p.nqb, p.batch * p.kv_heads, p.splits, p.kv_heads);
+    const int count = p.group / p.splits, first = w.hk * p.group + w.hq * count;
     const int kbeg = w.blk * BK, key0 = kbeg + 16 * MT * wave;
     const T* K = slice<T>(p.k, p.ks, w.b, w.hk);
     const T* V = slice<T>(p.v, p.vs, w.b, w.hk);
@@ -736,16 +759,16 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
     int head = 0;
     auto next = [&](bool* m) -> int {
         int s = stages.next(m);
-        while (s < 0 && head + 1 < p.group && stages.count > 0) {
+        while (s < 0 && head + 1 < count && stages.count > 0) {
             ++head;
             stages.base = -64;
             s = stages.next(m);
-            if (s < 0) head = p.group;   // no stage for one head is none for any
+            if (s < 0) head = count;   // no stage for one head is none for any
         }
         return s;
     };
     auto fill = [&](int hq, int st, T* q, T* o, int* words) {
-        const int h = w.hk * p.group + hq, q0 = st * SQ;
+        const int h = first + hq, q0 = st * SQ;
         qfill(q, slice<T>(p.q, p.qs, w.b, h), q0, p.sq);
         ofill(o, slice<T>(p.dout, p.dos, w.b, h), q0, p.sq);
         const int64_t at = ((int64_t)w.b * p.heads + h) * p.sq + q0;
@@ -776,7 +799,7 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
         if (nx >= 0) fill(hnx, nx, P ? Qb0 : Qb1, P ? Ob0 : Ob1, P ? Wb0 : Wb1);
         const int q0 = st * SQ;
         const bool act = active(st);
-        const float slope = MOD && p.slopes ? p.slopes[w.hk * p.group + hq] * kLog2e : 0.0f;
+        const float slope = MOD && p.slopes ? p.slopes[first + hq] * kLog2e : 0.0f;
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
             v8 pb[MT][1], db[MT][1];
@@ -859,8 +882,25 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
         step(std::integral_constant<int, 1>{});
     }
     const ScoreParams lp = late_params<ScoreParams>();
-    T* outk = lp.dk ? slice<T>(lp.dk, lp.dks, w.b, w.hk) : nullptr;
-    T* outv = lp.dv ? slice<T>(lp.dv, lp.dvs, w.b, w.hk) : nullptr;
+    if (lp.splits > 1) {
+        const int64_t rows = (int64_t)lp.batch * lp.kv_heads * lp.sk;   // of one split
+        float* const outk = lp.part + (w.hq * rows + ((int64_t)w.b * lp.kv_heads + w.hk) * lp.sk) * D;
+        float* const outv = outk + lp.splits * rows * D;
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            const int key = key0 + 16 * t + li;
+            if (key >= lp.sk) continue;
+#pragma unroll
+            for (int j = 0; j < NDB; ++j) {
+                *reinterpret_cast<f32x4*>(outk + (int64_t)key * D + 16 * j + 4 * g) = dk[t][j];
+                *reinterpret_cast<f32x4*>(outv + (int64_t)key * D + 16 * j + 4 * g) = dv[t][j];
+            }
+        }
+        if (*Special) dkv_specials<T, float, SQ>(lp, test, nst, prefix, w.b, first, count, key0, 16 * MT, lane, outk, D, outv, D);
+        return;
+    }
+    T* const outk = lp.dk ? slice<T>(lp.dk, lp.dks, w.b, w.hk) : nullptr;
+    T* const outv = lp.dv ? slice<T>(lp.dv, lp.dvs, w.b, w.hk) : nullptr;
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
         const int key = key0 + 16 * t + li;
@@ -871,24 +911,29 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
             if (outv) store4<T, VEC>(outv + key * lp.dvs.s, 16 * j + 4 * g, lp.d, dv[t][j]);
         }
     }
-    if (*Special) {
-        __threadfence();
-        for (int x = 0; x < lp.group; ++x) {
-            const int h = w.hk * lp.group + x;
-            const T* Q = slice<T>(lp.q, lp.qs, w.b, h);
-            const T* dO = slice<T>(lp.dout, lp.dos, w.b, h);
-            each_masked(test, nst, lane, [&](int stage) {
-                const int from = stage * SQ, to = min(from + SQ, lp.sq), n = min(16 * MT, lp.sk - key0);
-                auto see = [&](int row, int r) { return pair_seen(lp, prefix, w.b, row, key0 + r); };
-                if (outk)
-                    add_specials<T, T, false>(from, to, n, lp.d, lane, [&](int row) { return Q + row * lp.qs.s; }, see,
-                                              [&](int r) { return outk + (key0 + r) * lp.dks.s; });
-                if (outv)
-                    add_specials<T, T, true>(from, to, n, lp.d, lane, [&](int row) { return dO + row * lp.dos.s; }, see,
-                                             [&](int r) { return outv + (key0 + r) * lp.dvs.s; });
-            });
-        }
+    if (*Special)
+        dkv_specials<T, T, SQ>(lp, test, nst, prefix, w.b, first, count, key0, 16 * MT, lane, outk, lp.dks.s, outv, lp.dvs.s);
+}
+
+// Adds up the splits of a key block's heads: four columns a thread.
+template <typename T, int D, bool VEC>
+__device__ __forceinline__ void score_dkv_sum(const ScoreParams& p) {
+    constexpr int L = D / 4;
+    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, row = id / L;
+    const int col = id % L * 4;
+    const int64_t rows = (int64_t)p.batch * p.kv_heads * p.sk;
+    if (row >= rows) return;
+    const int key = row % p.sk, hk = row / p.sk % p.kv_heads, b = row / p.sk / p.kv_heads;
+    const float* at = p.part + row * D + col;
+    f32x4 k = {0.0f, 0.0f, 0.0f, 0.0f}, v = k;
+#pragma unroll 4
+    for (int s = 0; s < p.splits; ++s) {
+        k += *reinterpret_cast<const f32x4*>(at + s * rows * D);
+        v += *reinterpret_cast<const f32x4*>(at + (p.splits + s) * rows * D);
     }
+    if (p.dk) store4<T, VEC>(slice<T>(p.dk, p.dks, b, hk) + key * p.dks.s, col, p.d, k * p.scale);
+    if (p.dv) store4<T, VEC>(slice<T>(p.dv, p.dvs, b, hk) + key * p.dvs.s, col, p.d, v);
+
 }
 
 // ---------------------------------------------------------------------------
@@ -930,6 +975,16 @@ DELTA(false, s)
         ScoreParams p) {                                                                              \
         score_##F<OPS_T, D, MT, MOD, VEC>(p);                                                         \
     }
+#define SUM(D, VEC, TAG)                                                                                         \
+    extern "C" __global__ __launch_bounds__(256) void PASTE(fa_score_dkv_sum_, OPS_NAME, _d##D, TAG)(ScoreParams p) { \
+        score_dkv_sum<OPS_T, D, VEC>(p);                                                                        \
+    }
+SUM(64, true, )
+SUM(128, true, )
+SUM(256, true, )
+SUM(64, false, s)
+SUM(128, false, s)
+SUM(256, false, s)
 // plain scores, modified ones (m), and any alignment (s)
 #define KERNELS(F, D, MT, WAVES)             \
     KERNEL(F, D, MT, false, true, , WAVES)   \
@@ -956,7 +1011,6 @@ KERNELS(dq, 64, 2, 2)
 KERNELS(dq, 128, 2, 2)
 KERNELS(dq, 256, 1, 2)
 KERNELS(dkv, 64, 2, 2)
-KERNELS(dkv, 128, 2, 1)
 #else
 KERNELS(forward, 256, 1, 1)
 KERNELS(dq, 256, 1, 1)
