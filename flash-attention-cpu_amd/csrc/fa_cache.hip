@@ -3,13 +3,14 @@
 // attention (fa_score_forward).
 //
 // The rows of a (sequence, kv head) are its tokens times the query heads of the
-// group, so K and V are read once for all of them.  The keys of a sequence are cut into runs, one a
-// workgroup; more than one run leave partial sums that fa_rows_merge joins.
+// group, so K and V are read once for all of them.  The keys of all sequences are cut into runs of one length,
+// one a workgroup, so that sequences of different lengths keep all of the GPU busy; a sequence of more than one run leaves
+// partial sums that fa_rows_merge joins.
 //   stream: up to 64 rows.  Bound by memory: every wave walks 32-key blocks of its own
 //           through LDS that only it uses, two slots of K and V, one filled by DMA while the
 //           other is used; no barrier until the waves' sums are joined at the end.
-//   shared: more rows.  Four waves of two 16-row tiles share 64-key stages,
-//           double-buffered, so that K and V cross the L2 once for 128 rows.
+//   shared: more rows.  Eight waves of one or two 16-row tiles share the stages of a ring, two of which are on
+//           their way while one is used, so that K and V cross the L2 once for up to 256 rows.
 // Tiles in LDS have no padding, so that DMA instructions move 1 KiB of whole rows; row r keeps
 // 16-byte chunk x at position x ^ (r % 16), which spreads row reads and transposed
 // reads over the banks.
@@ -67,70 +68,6 @@ __device__ __forceinline__ int load_uniform(const int32_t* p) {
     return *(const __attribute__((address_space(4))) int32_t*)p;
 }
 
-// Rows of one sequence's K or V and their way into LDS.
-template <typename T, int D, int ROWS, int NW>
-struct RowSource {
-    using S = Swizzled<T, D>;
-    static constexpr int RUNS = ROWS / S::RPR, NI = (RUNS + NW - 1) / NW;
-    static_assert(RUNS % NW == 0 && 16 % S::RPR == 0 && NW * S::RPR <= 32, "runs of a wave lie in 16-row groups");
-    const T* base;
-    int64_t seq, batch;
-    int voff[NI];
-    __device__ __forceinline__ RowSource(const T* b, int64_t seq_, int64_t batch_, int d, int wave, int lane)
-        : base(b), seq(seq_), batch(batch_) {
-#pragma unroll
-        for (int i = 0; i < NI; ++i) {
-            const int row = (i * NW + wave) * S::RPR + lane / S::CPR;
-            const int col = ((lane % S::CPR) ^ (row % S::CM)) * S::E;
-            voff[i] = col < d ? (int)(row % 16 * seq + col) * (int)sizeof(T) : 0x7ffffff0;   // in its 16-row group
-        }
-    }
-    // DMA of rows [k0, k0 + ROWS), zeros at and past `end` and where a page is bad; pages of 16 rows or more:
-    // a 16-row group lies in one page
-    template <typename Cache>
-    __device__ __forceinline__ void fill(T* dst, int k0, int end, const int (&page)[ROWS / 16], const Cache& c,
-                                         int wave) const {
-        constexpr int kStep = NW * S::RPR;   // rows of the waves' i-th runs
-        __amdgpu_buffer_rsrc_t rs;
-#pragma unroll
-        for (int i = 0; i < NI; ++i) {
-            if (i * kStep % 16 == 0 || kStep > 16) {
-                // the group of the wave's run
-                const int grp = kStep > 16 ? i * kStep / 16 + wave * S::RPR / 16 : i * kStep / 16;
-                int pg = page[i * kStep / 16];
-                if constexpr (kStep > 16) pg = wave * S::RPR >= 16 ? page[i * kStep / 16 + 1] : pg;
-                const int row = k0 + 16 * grp;
-                const int n = pg < 0 ? 0 : max(0, min(16, end - row));
-                const T* src = n == 0 ? base : c.table ? base + (pg * batch + (row & c.page_mask) * seq) : base + row * seq;
-                rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(src), (short)0, (int)(n * seq) * (int)sizeof(T),
-                                                       0x00020000);
-            }
-            const int run = i * NW + wave;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                rs, (__attribute__((address_space(3))) void*)(dst + run * 64 * S::E), 16, voff[i], 0, 0, 0);
-        }
-    }
-    // the same element by element: any alignment, any page size.  Returns whether the thread met a bad page.
-    template <typename Cache>
-    __device__ __forceinline__ bool fill_slow(T* dst, int k0, int end, const Cache& c, int d, int tid) const {
-        bool bad = false;
-#pragma unroll 1
-        for (int pos = tid; pos < ROWS * (D / 8); pos += 64 * NW) {
-            const int r = pos / (D / 8), col = 8 * (pos % (D / 8));
-            const int64_t at = c.at(k0 + r, end, seq, batch);
-            bad = bad || (at < 0 && k0 + r < end);
-            const typename Mma<T>::v8 x = global_row<T, false>(base + (at < 0 ? 0 : at), 0, 0, at >= 0, col, d);
-            if constexpr (sizeof(T) == 2) {
-                *reinterpret_cast<typename Mma<T>::v8*>(dst + S::at(r, col)) = x;
-            } else {
-                *reinterpret_cast<f32x4*>(dst + S::at(r, col)) = __builtin_shufflevector(x, x, 0, 1, 2, 3);
-                *reinterpret_cast<f32x4*>(dst + S::at(r, col + 4)) = __builtin_shufflevector(x, x, 4, 5, 6, 7);
-            }
-        }
-        return bad;
-    }
-};
-
 // The pages of a sequence.
 struct CachePages {
     const int32_t* table;   // nullptr: rows one after another
@@ -150,54 +87,223 @@ struct CachePages {
     }
 };
 
+// Rows of one sequence's K or V and their way into LDS, ROWS at a time.
+template <typename T, int D, int ROWS, int NW>
+struct RowSource {
+    using S = Swizzled<T, D>;
+    static constexpr int RUNS = ROWS / S::RPR, NI = RUNS / NW;
+    static_assert(RUNS % NW == 0 && 16 % S::RPR == 0, "whole runs a wave, in 16-row groups");
+    const T* base;
+    int64_t seq, batch;
+    int voff[NI];
+    __device__ __forceinline__ RowSource(const T* b, int64_t seq_, int64_t batch_, int d, int wave, int lane)
+        : base(b), seq(seq_), batch(batch_) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            const int row = (i * NW + wave) * S::RPR + lane / S::CPR;
+            const int col = ((lane % S::CPR) ^ (row % S::CM)) * S::E;
+            voff[i] = col < d ? (int)(row * seq + col) * (int)sizeof(T) : 0x7ffffff0;
+        }
+    }
+    // DMA of rows [k0, k0 + ROWS), zeros at and past `end` and where a page is bad, in pages of 16 rows or
+    // more; pg: the pages of its 16-row groups, or of row k0 alone where a page holds all.
+    static constexpr int GROUPS = ROWS / 16;
+    __device__ __forceinline__ void fill(T* dst, int k0, int end, const int (&pg)[GROUPS], const CachePages& c,
+                                         int wave) const {
+        constexpr int kStep = NW * S::RPR;   // rows of the waves' i-th runs
+        if (kStep > 16 && (!c.table || c.page_mask >= ROWS - 1)) {
+            const int n = pg[0] < 0 ? 0 : max(0, min(ROWS, end - k0));
+            const T* src = n == 0 ? base : c.table ? base + (pg[0] * batch + (k0 & c.page_mask) * seq) : base + k0 * seq;
+            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+                const_cast<T*>(src), (short)0, (int)(n * seq) * (int)sizeof(T), 0x00020000);
+#pragma unroll
+            for (int i = 0; i < NI; ++i)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                    rs, (__attribute__((address_space(3))) void*)(dst + (i * NW + wave) * 64 * S::E), 16, voff[i], 0, 0, 0);
+            return;
+        }
+        // A 16-row group lies in one page; its rows are addressed as from row k0 on.
+        __amdgpu_buffer_rsrc_t rs;
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            const int run = i * NW + wave;
+            if (i * kStep % 16 == 0 || kStep > 16) {
+                const int grp = kStep > 16 ? run * S::RPR / 16 : i * kStep / 16, row = k0 + 16 * grp;
+                int page = pg[i * kStep / 16];
+#pragma unroll
+                for (int e = 1; e < kStep / 16; ++e) page = wave * S::RPR / 16 == e ? pg[i * kStep / 16 + e] : page;
+                const int n = page < 0 ? 0 : max(0, min(16, end - row));
+                const T* src = n == 0 ? base : base + (page * batch + ((c.table ? row & c.page_mask : row) - 16 * grp) * seq);
+                rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(src), (short)0,
+                                                       n == 0 ? 0 : (int)((16 * grp + n) * seq) * (int)sizeof(T), 0x00020000);
+            }
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                rs, (__attribute__((address_space(3))) void*)(dst + run * 64 * S::E), 16, voff[i], 0, 0, 0);
+        }
+    }
+    // The pages of rows [k0, k0 + ROWS) before `end`; returns whether one is bad.
+    static __device__ __forceinline__ bool look_up(const CachePages& c, int k0, int end, int (&pg)[GROUPS]) {
+        bool bad = false;
+        const bool whole = !c.table || c.page_mask >= ROWS - 1;
+#pragma unroll
+        for (int i = 0; i < GROUPS; ++i) {
+            const int row = k0 + 16 * i;
+            if (i > 0 && whole) {
+                pg[i] = pg[0];
+            } else {
+                pg[i] = row < end ? c.page(row) : -1;
+            }
+            bad = bad || (pg[i] < 0 && row < end);
+        }
+        return bad;
+    }
+    // the same element by element: any alignment, any page size.  Returns whether the thread met a bad page.
+    __device__ __forceinline__ bool fill_slow(T* dst, int k0, int end, const CachePages& c, int d, int tid) const {
+        bool bad = false;
+#pragma unroll 1
+        for (int pos = tid; pos < ROWS * (D / 8); pos += 64 * NW) {
+            const int r = pos / (D / 8), col = 8 * (pos % (D / 8));
+            const int64_t at = c.at(k0 + r, end, seq, batch);
+            bad = bad || (at < 0 && k0 + r < end);
+            const typename Mma<T>::v8 x = global_row<T, false>(base + (at < 0 ? 0 : at), 0, 0, at >= 0, col, d);
+            if constexpr (sizeof(T) == 2) {
+                *reinterpret_cast<typename Mma<T>::v8*>(dst + S::at(r, col)) = x;
+            } else {
+                *reinterpret_cast<f32x4*>(dst + S::at(r, col)) = __builtin_shufflevector(x, x, 0, 1, 2, 3);
+                *reinterpret_cast<f32x4*>(dst + S::at(r, col + 4)) = __builtin_shufflevector(x, x, 4, 5, 6, 7);
+            }
+        }
+        return bad;
+    }
+};
+
 __device__ __forceinline__ CachePages rows_pages(const RowsParams& p, int b) {
     return {p.table ? p.table + (int64_t)b * p.pages_per_seq : nullptr, p.page_shift, (1 << p.page_shift) - 1, p.n_pages};
 }
 
 // What a workgroup of either kernel works on.
 struct RowsWork {
-    int kv, split, rb, b, hk;
+    int run, rb, b, hk;
+    int runs;   // of the sequence
     int len, prefix, open, kbeg, kend, nrows, rfirst;
     bool tree, docs;
 };
-template <int STEP>
-__device__ __forceinline__ RowsWork rows_work(const RowsParams& p, int rows) {
-    RowsWork w;
+
+// Keys that any query of sequence b sees.
+__device__ __forceinline__ int rows_total(const RowsParams& p, int b) {
+    if (p.lens) {
+        const int len = p.lens[b];
+        return len < 0 ? 0 : (int)min((int64_t)len + p.n, (int64_t)p.sk);
+    }
+    return p.causal ? max(min(max(p.q_start + p.n, p.prefix ? p.prefix[b] : 0), p.sk), 0) : p.sk;
+}
+
+// The runs of a sequence: their length in steps, how many, and the first one's number.
+struct Runs {
+    int b, steps, count, first;
+};
+// All sequences' steps are shared out over p.share runs, and a sequence takes as many whole runs as hold
+// its own, one at least.  Every wave finds them for itself, a lane a sequence, 64 sequences at a
+// time: f(sequence, its runs, the end of its runs' numbers) on every lane.
+template <typename F>
+__device__ __forceinline__ int each_runs(const RowsParams& p, int lane, F f) {
+    auto steps_of = [&](int i) { return (rows_total(p, i) + p.step - 1) / p.step; };
+    int64_t all = 0;
+    for (int i = lane; i < p.batch; i += 64) all += steps_of(i);
+#pragma unroll
+    for (int s = 1; s < 64; s *= 2) all += __shfl_xor(all, s);
+    const int steps = (int)max((int64_t)1, (all + p.share - 1) / p.share);
+    int before = 0;   // runs of the sequences of earlier chunks
+    for (int base = 0; base < p.batch; base += 64) {
+        const int i = base + lane;
+        const int n = i < p.batch ? max(1, (steps_of(i) + steps - 1) / steps) : 0;
+        int end = n;
+#pragma unroll
+        for (int s = 1; s < 64; s *= 2) {
+            const int x = __shfl_up(end, s);
+            end += lane >= s ? x : 0;
+        }
+        end += before;
+        if (f(base, n, end)) break;
+        before = __builtin_amdgcn_readlane(end, 63);
+    }
+    return steps;
+}
+// The runs of a call of one sequence.
+__device__ __forceinline__ Runs runs_of_one(const RowsParams& p) {
+    const int all = (rows_total(p, 0) + p.step - 1) / p.step, steps = max(1, (all + p.share - 1) / p.share);
+    return {0, steps, max(1, (all + steps - 1) / steps), 0};
+}
+// The sequence that run `run` (the same on all lanes) belongs to; b < 0: no such run.
+__device__ __forceinline__ Runs runs_of_run(const RowsParams& p, int run, int lane) {
+    if (p.batch == 1) {
+        Runs r = runs_of_one(p);
+        if (run >= r.count) r.b = -1;
+        return r;
+    }
+    Runs r = {-1, 0, 0, 0};
+    r.steps = each_runs(p, lane, [&](int base, int n, int end) {
+        const uint64_t hit = __builtin_amdgcn_ballot_w64(n > 0 && run >= end - n && run < end);
+        if (hit == 0) return false;
+        const int at = __builtin_ctzll(hit);
+        r.b = base + at;
+        r.count = __builtin_amdgcn_readlane(n, at);
+        r.first = __builtin_amdgcn_readlane(end, at) - r.count;
+        return true;
+    });
+    return r;
+}
+// Those of sequence b, each lane its own.
+__device__ __forceinline__ Runs runs_of_sequence(const RowsParams& p, int b, int lane) {
+    if (p.batch == 1) return runs_of_one(p);
+    Runs r = {b, 0, 0, 0};
+    r.steps = each_runs(p, lane, [&](int base, int n, int end) {
+        const int count = __shfl(n, b - base), last = __shfl(end, b - base);
+        if (b >= base && b < base + 64) {
+            r.count = count;
+            r.first = last - count;
+        }
+        return false;
+    });
+    return r;
+}
+
+// Returns whether there is work.
+__device__ __forceinline__ bool rows_work(const RowsParams& p, int rows, int lane, RowsWork* out) {
+    RowsWork& w = *out;
     // the row blocks of one run of keys side by side on one XCD where the counts allow
-    const int nkv = p.batch * p.kv_heads, runs = nkv * p.num_splits;
-    int run;
-    if ((runs & 7) == 0) {
+    int rk;
+    if ((p.num_runs * p.kv_heads & 7) == 0) {
         const int t = blockIdx.x >> 3;
         w.rb = t % p.nrb;
-        run = t / p.nrb * 8 + (blockIdx.x & 7);
+        rk = t / p.nrb * 8 + (blockIdx.x & 7);
     } else {
         w.rb = blockIdx.x % p.nrb;
-        run = blockIdx.x / p.nrb;
+        rk = blockIdx.x / p.nrb;
     }
-    w.kv = run / p.num_splits;
-    w.split = run % p.num_splits;
-    w.b = w.kv / p.kv_heads;
-    w.hk = w.kv % p.kv_heads;
+    w.run = rk / p.kv_heads;
+    w.hk = rk % p.kv_heads;
+    const Runs r = runs_of_run(p, w.run, lane);
+    w.b = __builtin_amdgcn_readfirstlane(r.b);
+    if (w.b < 0) return false;
+    w.runs = __builtin_amdgcn_readfirstlane(r.count);
     w.tree = p.lens != nullptr;
     w.docs = p.q_doc != nullptr;
-    // keys of the sequence: all of the filled rows, then the drafted ones; every row sees
-    // those before `open`
+    // all of the filled rows, then the drafted ones; every row sees those before `open`
     w.len = w.tree ? load_uniform(p.lens + w.b) : 0;
     w.prefix = p.prefix ? load_uniform(p.prefix + w.b) : 0;
-    int total;
     if (w.tree) {
-        total = w.len < 0 ? 0 : (int)min((int64_t)w.len + p.n, (int64_t)p.sk);
         w.open = min(max(w.len, 0), p.sk);
     } else {
-        total = p.causal ? max(min(max(p.q_start + p.n, w.prefix), p.sk), 0) : p.sk;
         w.open = w.docs ? 0 : p.causal ? max(p.q_start + 1, w.prefix) : p.sk;
     }
-    const int per = ((total + p.num_splits - 1) / p.num_splits + STEP - 1) / STEP * STEP;
-    w.kbeg = min((int64_t)w.split * per, (int64_t)total);
-    w.kend = min(w.kbeg + per, total);
+    const int total = __builtin_amdgcn_readfirstlane(rows_total(p, w.b));
+    const int64_t per = (int64_t)__builtin_amdgcn_readfirstlane(r.steps) * p.step;
+    w.kbeg = (int)min((w.run - __builtin_amdgcn_readfirstlane(r.first)) * per, (int64_t)total);
+    w.kend = (int)min(w.kbeg + per, (int64_t)total);
     w.nrows = p.n * p.group;
     w.rfirst = w.rb * rows;
-    return w;
+    return true;
 }
 
 // Whether token `tok` sees key `key` < kend, as far as masks tell.
@@ -275,7 +381,7 @@ struct RowTiles {
 #pragma unroll
                 for (int t = 0; t < MT; ++t) s[t][b] = M::mma(k, q[t][dc], s[t][b]);
             }
-            if (dc % 2 == 1) __builtin_amdgcn_sched_barrier(0);
+            if (sizeof(T) == 4 || dc % 2 == 1) __builtin_amdgcn_sched_barrier(0);
         }
         if constexpr (MOD) {
 #pragma unroll
@@ -414,7 +520,7 @@ struct RowTiles {
                 const v8 a = S::col_op(Vs, 32 * i, 16 * j, g, li);
 #pragma unroll
                 for (int t = 0; t < MT; ++t) o[t][j] = M::mma(a, pb[t][i], o[t][j]);
-                if (j % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+                if (sizeof(T) == 4 || j % 4 == 3) __builtin_amdgcn_sched_barrier(0);
             }
     }
     // maxima in log2 units and whole row sums, before partial sums meet
@@ -437,8 +543,8 @@ struct RowTiles {
             return at < 0 ? nullptr : V + at;
         };
         auto row_sees = [&](int key, int r) { return rows_see(p, w, (rfirst + r) / p.group, key); };
-        if (p.num_splits > 1) {
-            const int64_t part = ((int64_t)w.kv * p.nrb + w.rb) * p.num_splits + w.split;
+        if (w.runs > 1) {
+            const int64_t part = ((int64_t)w.run * p.kv_heads + w.hk) * p.nrb + w.rb;
             const int rows = p.block_rows;
             float* const po = p.part_o + (part * rows + 16 * tile0) * D;
             float* const pm = p.part_ml + part * 2 * rows + 16 * tile0;
@@ -507,7 +613,8 @@ __device__ __forceinline__ void rows_stream(const RowsParams& p) {
     __shared__ int any_special[NW];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const RowsWork w = rows_work<SK>(p, 16 * MT);
+    RowsWork w;
+    if (!rows_work(p, 16 * MT, lane, &w)) return;
     const CachePages pages = rows_pages(p, w.b);
     const T* const K = reinterpret_cast<const T*>(p.k) + w.hk * p.ks.h + (p.table ? 0 : w.b * p.ks.b);
     const T* const V = reinterpret_cast<const T*>(p.v) + w.hk * p.vs.h + (p.table ? 0 : w.b * p.vs.b);
@@ -518,40 +625,43 @@ __device__ __forceinline__ void rows_stream(const RowsParams& p) {
 
     bool special = false;
     R x;
-    auto pages_of = [&](int blk, int (&pg)[2]) {
-        const int k = k_first + blk * SK * NW;
-        const bool in = blk < nblk;
-        pg[0] = in ? pages.page(k) : -1;
-        pg[1] = in && k + 16 < w.kend ? pages.page(k + 16) : -1;
+    // pages of the block to fill next are looked up a block ahead
+    int page[2];
+    bool bad0, bad1, bad2;
+    auto look_up = [&](int blk) {
+        const int k0 = k_first + blk * SK * NW;
+        return Src::look_up(pages, k0, blk < nblk ? w.kend : k0, page);
     };
-    auto fill = [&](const Src& src, T* dst, int blk, const int (&pg)[2]) {
-        src.fill(dst + wave * TILE, k_first + blk * SK * NW, w.kend, pg, pages, 0);
+    auto fill = [&](const Src& src, T* dst, int blk) {
+        const int k0 = k_first + blk * SK * NW;
+        src.fill(dst + wave * TILE, k0, blk < nblk ? w.kend : k0, page, pages, 0);
     };
-    int pg0[2], pg1[2], pg2[2];
-    pages_of(0, pg0);
-    pages_of(1, pg1);
+    bad0 = look_up(0);
     if (nblk > 0) {
-        fill(ksrc, K0, 0, pg0);
-        fill(vsrc, V0, 0, pg0);
+        fill(ksrc, K0, 0);
+        fill(vsrc, V0, 0);
     }
+    bad1 = look_up(1);
     x.init(p, w, w.rfirst, lane);
     if (nblk > 0) {
         // Q's loads are through before more DMA starts: only DMA is counted from here
         wait_vmcnt<0>();
-        fill(ksrc, K1, 1, pg1);
-        fill(vsrc, V1, 1, pg1);
+        fill(ksrc, K1, 1);
+        fill(vsrc, V1, 1);
     }
+    bad2 = look_up(2);
     auto block = [&](int i, T* kb, T* vb) {
         T* const Ks = kb + wave * TILE;
         T* const Vs = vb + wave * TILE;
         const int k0 = k_first + i * SK * NW;
-        const bool bad = pg0[0] < 0 || (pg0[1] < 0 && k0 + 16 < w.kend);
-        pages_of(i + 2, pg2);
+        const bool bad = bad0;
+        bad0 = bad1;
+        bad1 = bad2;
         wait_vmcnt<3 * RUNS>();
         const bool masked = bad || k0 + SK > min(w.open, w.kend);
         x.scores(p, w, Ks, k0, masked, bad);
         reread();
-        fill(ksrc, kb, i + 2, pg2);
+        fill(ksrc, kb, i + 2);
         x.softmax();
         wait_vmcnt<3 * RUNS>();
         if (masked) {
@@ -560,9 +670,8 @@ __device__ __forceinline__ void rows_stream(const RowsParams& p) {
         }
         x.values(Vs);
         reread();
-        fill(vsrc, vb, i + 2, pg2);
-        pg0[0] = pg1[0], pg0[1] = pg1[1];
-        pg1[0] = pg2[0], pg1[1] = pg2[1];
+        fill(vsrc, vb, i + 2);
+        bad2 = look_up(i + 3);
     };
     for (int i = 0; i < nblk; i += 2) {
         block(i, K0, V0);
@@ -621,134 +730,155 @@ __device__ __forceinline__ void rows_stream(const RowsParams& p) {
 // ---------------------------------------------------------------------------
 template <typename T, int D, int MT, bool MOD, bool VEC>
 __device__ __forceinline__ void rows_shared(const RowsParams& p) {
-    constexpr int NW = 4, SK = sizeof(T) == 4 || D > 128 ? 32 : 64, TILE = SK * D, KB = SK / 16;
+    constexpr int NW = 8, SK = sizeof(T) == 4 || D > 128 ? 32 : 64, TILE = SK * D, KB = SK / 16;
+    constexpr int RING = TILE * (int)sizeof(T) > 16384 ? 2 : 3;   // stages in LDS
     using R = RowTiles<T, D, MT, KB, MOD, VEC>;
     using Src = RowSource<T, D, SK, NW>;
-    T* const Kb0 = lds_array<T, TILE, 0>();
-    T* const Vb0 = lds_array<T, TILE, 1>();
-    T* const Kb1 = lds_array<T, TILE, 2>();
-    T* const Vb1 = lds_array<T, TILE, 3>();
-    __shared__ int bad_any[2], Special;
+    T* const K0 = lds_array<T, TILE, 0>();
+    T* const V0 = lds_array<T, TILE, 1>();
+    T* const K1 = lds_array<T, TILE, 2>();
+    T* const V1 = lds_array<T, TILE, 3>();
+    constexpr int THIRD = (RING > 2) ? TILE : 8;
+    T* const K2 = (RING > 2) ? lds_array<T, THIRD, 4>() : K0;
+    T* const V2 = (RING > 2) ? lds_array<T, THIRD, 5>() : V0;
+    __shared__ int bad_any, Special;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const RowsWork w = rows_work<SK>(p, 16 * MT * NW);
+    RowsWork w;
+    if (!rows_work(p, 16 * MT * NW, lane, &w)) return;
     const CachePages pages = rows_pages(p, w.b);
     const T* const K = reinterpret_cast<const T*>(p.k) + w.hk * p.ks.h + (p.table ? 0 : w.b * p.ks.b);
     const T* const V = reinterpret_cast<const T*>(p.v) + w.hk * p.vs.h + (p.table ? 0 : w.b * p.vs.b);
     const Src ksrc(K, p.ks.s, p.ks.b, p.d, wave, lane), vsrc(V, p.vs.s, p.vs.b, p.d, wave, lane);
     const int nst = (w.kend - w.kbeg + SK - 1) / SK;
     const int rfirst = w.rfirst + 16 * MT * wave;
-    constexpr bool dma = VEC;
     const bool act = rfirst < w.nrows;
 
-    int pgk[SK / 16], pgv[SK / 16], pgn[SK / 16];   // pages of the current, next and after-next stage
-    auto pages_of = [&](int st, int (&pg)[SK / 16]) {
-#pragma unroll
-        for (int i = 0; i < SK / 16; ++i) {
-            const int k = w.kbeg + st * SK + 16 * i;
-            pg[i] = dma && k < w.kend ? pages.page(k) : -1;
-        }
-    };
-    auto fill = [&](const Src& src, T* dst, int st, const int (&pg)[SK / 16], int parity) {
+    // whether the stages on their way have bad pages; those of the stage to fill next are looked up a stage ahead
+    bool bad_now = false, bad_1 = false, bad_2 = false, bad_next = false;
+    int page[SK / 16];
+    auto look_up = [&](int st) {
         const int k0 = w.kbeg + st * SK;
-        if constexpr (dma) {
-            src.fill(dst, k0, w.kend, pg, pages, wave);
-        } else {
-            if (src.fill_slow(dst, k0, w.kend, pages, p.d, tid)) bad_any[parity] = 1;
-        }
+        if (VEC) bad_next = Src::look_up(pages, k0, st < nst ? w.kend : k0, page);
     };
-    auto bad_stage = [&](int st, const int (&pg)[SK / 16], int parity) {
-        if (!dma) return bad_any[parity] != 0;
-        bool bad = false;
-#pragma unroll
-        for (int i = 0; i < SK / 16; ++i) bad = bad || (pg[i] < 0 && w.kbeg + st * SK + 16 * i < w.kend);
+    auto fill = [&](int st, T* k, T* v) -> bool {
+        const int k0 = w.kbeg + st * SK;
+        const bool bad = bad_next;
+        if constexpr (VEC) {
+            const int end = st < nst ? w.kend : k0;
+            ksrc.fill(k, k0, end, page, pages, wave);
+            vsrc.fill(v, k0, end, page, pages, wave);
+            look_up(st + 1);
+        } else if (k0 < w.kend) {
+            if (ksrc.fill_slow(k, k0, w.kend, pages, p.d, tid)) bad_any = 1;
+            vsrc.fill_slow(v, k0, w.kend, pages, p.d, tid);
+        }
         return bad;
     };
-    if (tid == 0) bad_any[0] = bad_any[1] = Special = 0;
+    look_up(0);
+    // All waves' share of a stage has landed, and all are done with the stage before; younger: DMA issued since.
+    auto arrive = [&](auto younger) {
+        if constexpr (VEC) {
+            wait_vmcnt<decltype(younger)::value>();
+            __builtin_amdgcn_s_barrier();
+            reread();
+        } else {
+            __syncthreads();
+        }
+    };
+    if (tid == 0) bad_any = Special = 0;
     R x;
     x.init(p, w, rfirst, lane);
-    if (!dma) __syncthreads();
-    pages_of(0, pgk);
-    pages_of(1, pgv);
-    if (nst > 0) {
-        fill(ksrc, Kb0, 0, pgk, 0);
-        fill(vsrc, Vb0, 0, pgk, 0);
-    }
-    if (nst > 1) fill(ksrc, Kb1, 1, pgv, 1);
-    wait_loads();
     __syncthreads();
-    bool bad = false, masked = false;
-    auto score = [&](int st, const T* Ks, const int (&pg)[SK / 16], int parity) {
+    // the two waves of a SIMD out of step: one multiplies while the other is in its softmax
+    if (wave < NW / 2) __builtin_amdgcn_s_setprio(1);
+    bad_now = fill(0, K0, V0);
+    if (RING > 2) bad_1 = fill(1, K1, V1);
+    auto step = [&](int st, T* k, T* v, T* kn, T* vn) {
+        arrive(std::integral_constant<int, (RING - 2) * 2 * Src::NI>{});
+        const bool filled = fill(st + RING - 1, kn, vn);
+        if (RING > 2) bad_2 = filled;
+        else bad_1 = filled;
         const int k0 = w.kbeg + st * SK;
-        bad = bad_stage(st, pg, parity);
-        masked = bad || k0 + SK > min(w.open, w.kend);
-        if (act) x.scores(p, w, Ks, k0, masked, bad);
+        const bool bad = VEC ? bad_now : bad_any != 0;
+        const bool masked = bad || k0 + SK > min(w.open, w.kend);
+        if (act) {
+            x.scores(p, w, k, k0, masked, bad);
+            x.softmax();
+        }
+        if (masked) {
+            if (Swizzled<T, D>::template clean<SK, 64 * NW>(v, tid)) Special = 1;
+            __syncthreads();
+        }
+        if (act) x.values(v);
+        bad_now = bad_1;
+        bad_1 = bad_2;
     };
-    if (nst > 0) score(0, Kb0, pgk, 0);
-    __syncthreads();
-    auto step = [&](auto parity, int st) {
-        constexpr int P = decltype(parity)::value;
-        T* const k_cur = P ? Kb1 : Kb0;
-        T* const k_next = P ? Kb0 : Kb1;
-        T* const v_cur = P ? Vb1 : Vb0;
-        T* const v_next = P ? Vb0 : Vb1;
-        // pgv: the next stage's pages
-        if (st + 1 < nst) fill(vsrc, v_next, st + 1, pgv, 1 - P);
-        pages_of(st + 2, pgn);
-        if (st + 2 < nst) fill(ksrc, k_cur, st + 2, pgn, P);
-        if (masked && Swizzled<T, D>::template clean<SK, 64 * NW>(v_cur, tid)) Special = 1;
-        if (act) x.softmax();
-        if (masked) __syncthreads();
-        if (act) x.values(v_cur);
-        if (st + 1 < nst) score(st + 1, k_next, pgv, 1 - P);
-        wait_loads();
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < SK / 16; ++i) pgv[i] = pgn[i];
-    };
-    for (int st = 0; st < nst; st += 2) {
-        step(std::integral_constant<int, 0>{}, st);
-        if (st + 1 < nst) step(std::integral_constant<int, 1>{}, st + 1);
+    if constexpr (RING == 3) {
+        for (int st = 0; st < nst; st += 3) {
+            step(st, K0, V0, K2, V2);
+            if (st + 1 < nst) step(st + 1, K1, V1, K0, V0);
+            if (st + 2 < nst) step(st + 2, K2, V2, K1, V1);
+        }
+    } else {
+        for (int st = 0; st < nst; st += 2) {
+            step(st, K0, V0, K1, V1);
+            if (st + 1 < nst) step(st + 1, K1, V1, K0, V0);
+        }
     }
+    __syncthreads();
     x.close();
     if (act) x.store(w, V, rfirst, MT * wave, lane, Special != 0);
 }
 
-// Joins the partial sums of a row: a workgroup a row, D / 4 lanes a run, the runs dealt to
-// the workgroup's groups of lanes, whose sums meet in LDS.
-template <typename T, int D, bool VEC>
+// Joins the partial sums of a row, D / 4 lanes a run.  WIDE: a workgroup a row, the runs dealt to
+// its groups of lanes, whose sums meet in LDS; else (few runs) a group of lanes a row.
+template <typename T, int D, bool VEC, bool WIDE>
 __device__ __forceinline__ void rows_merge(const RowsParams& p) {
-    constexpr int L = D / 4, G = 256 / L;
+    constexpr int L = D / 4, N = 256 / L, G = WIDE ? N : 1;
     __shared__ f32x4 sums[G][L];
     __shared__ float ls[G];
     const int nrows = p.n * p.group, rows = p.block_rows, tid = threadIdx.x;
-    const int grp = tid / L, lane = tid % L;
-    const int kv = blockIdx.x / nrows, r = blockIdx.x % nrows;
-    const int b = kv / p.kv_heads, h = kv % p.kv_heads * p.group + r % p.group, token = r / p.group;
-    const int64_t part = ((int64_t)kv * p.nrb + r / rows) * p.num_splits;
+    const int grp = WIDE ? tid / L : 0, lane = tid % L;
+    // past the last row: the last one again, so that all lanes take part in what follows
+    const int64_t last = (int64_t)p.batch * p.kv_heads * nrows - 1, at = (int64_t)blockIdx.x * N + tid / L;
+    const int64_t id = WIDE ? blockIdx.x : min(at, last);
+    const int kv = id / nrows, r = id % nrows;
+    const int b = kv / p.kv_heads, hk = kv % p.kv_heads, h = hk * p.group + r % p.group, token = r / p.group;
+    const Runs runs = runs_of_sequence(p, b, tid & 63);
+    if (runs.count == 1) return;   // written by its run
+    const int64_t next = (int64_t)p.kv_heads * p.nrb * rows;   // rows from one run's partial sums to the next's
+    const int64_t part = ((int64_t)runs.first * p.kv_heads + hk) * p.nrb + r / rows;
     const float* const ml = p.part_ml + part * 2 * rows + r % rows;
     const float* const po = p.part_o + (part * rows + r % rows) * D + 4 * lane;
     float mx = OPS_NEG_INF;
-    for (int s = tid & 63; s < p.num_splits; s += 64) mx = fmaxf(mx, ml[(int64_t)s * 2 * rows]);
+    if constexpr (WIDE) {
+        for (int s = tid & 63; s < runs.count; s += 64) mx = fmaxf(mx, ml[s * 2 * next]);
 #pragma unroll
-    for (int s = 1; s < 64; s *= 2) mx = fmaxf(mx, __shfl_xor(mx, s));
+        for (int s = 1; s < 64; s *= 2) mx = fmaxf(mx, __shfl_xor(mx, s));
+    } else {
+#pragma unroll 4
+        for (int s = 0; s < runs.count; ++s) mx = fmaxf(mx, ml[s * 2 * next]);
+    }
     const float ref = mx == OPS_NEG_INF ? 0.0f : mx;
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
     float l = 0.0f;
 #pragma unroll 4
-    for (int s = grp; s < p.num_splits; s += G) {
-        const float c = ops_exp2(ml[(int64_t)s * 2 * rows] - ref);
-        l += c * ml[(int64_t)s * 2 * rows + rows];
-        o += c * *reinterpret_cast<const f32x4*>(po + (int64_t)s * rows * D);
+    for (int s = grp; s < runs.count; s += G) {
+        const float c = ops_exp2(ml[s * 2 * next] - ref);
+        l += c * ml[s * 2 * next + rows];
+        o += c * *reinterpret_cast<const f32x4*>(po + s * next * D);
     }
-    sums[grp][lane] = o;
-    if (lane == 0) ls[grp] = l;
-    __syncthreads();
-    if (grp != 0) return;
+    if constexpr (WIDE) {
+        sums[grp][lane] = o;
+        if (lane == 0) ls[grp] = l;
+        __syncthreads();
+        if (grp != 0) return;
 #pragma unroll
-    for (int i = 1; i < G; ++i) {
-        o += sums[i][lane];
-        l += ls[i];
+        for (int i = 1; i < G; ++i) {
+            o += sums[i][lane];
+            l += ls[i];
+        }
     }
     store4<T, VEC>(reinterpret_cast<T*>(p.out) + b * p.os.b + h * p.os.h + token * p.os.s, 4 * lane, p.d,
                    o * (l == 0.0f ? 0.0f : 1.0f / l));
@@ -769,16 +899,17 @@ __device__ __forceinline__ void rows_merge(const RowsParams& p) {
     KERNEL(fa_rows_stream_, rows_stream, D, MT, false, true, , STREAM_THREADS(D), WAVES)  \
     KERNEL(fa_rows_stream_, rows_stream, D, MT, true, true, m, STREAM_THREADS(D), WAVES)
 #define SHARED(D, MT, WAVES)                                                   \
-    KERNEL(fa_rows_shared_, rows_shared, D, MT, false, true, , 256, WAVES)     \
-    KERNEL(fa_rows_shared_, rows_shared, D, MT, true, true, m, 256, WAVES)
-#define COMMON(D)                                                                                               \
-    KERNEL(fa_rows_shared_, rows_shared, D, 1, true, false, s, 256, 1)                                          \
-    extern "C" __global__ __launch_bounds__(256) void PASTE(fa_rows_merge_, OPS_NAME, _d##D, )(RowsParams p) {  \
-        rows_merge<OPS_T, D, true>(p);                                                                          \
-    }                                                                                                           \
-    extern "C" __global__ __launch_bounds__(256) void PASTE(fa_rows_merge_, OPS_NAME, _d##D, s)(RowsParams p) { \
-        rows_merge<OPS_T, D, false>(p);                                                                         \
+    KERNEL(fa_rows_shared_, rows_shared, D, MT, false, true, , 512, WAVES)     \
+    KERNEL(fa_rows_shared_, rows_shared, D, MT, true, true, m, 512, WAVES)
+#define MERGE(D, VEC, WIDE, TAG)                                                                                  \
+    extern "C" __global__ __launch_bounds__(256) void PASTE(fa_rows_merge_, OPS_NAME, _d##D, TAG)(RowsParams p) { \
+        rows_merge<OPS_T, D, VEC, WIDE>(p);                                                                       \
     }
+#define COMMON(D)                                                                                               \
+    KERNEL(fa_rows_shared_, rows_shared, D, 1, true, false, s, 512, 2)                                          \
+    MERGE(D, true, false, )                                                                                     \
+    MERGE(D, true, true, w)                                                                                     \
+    MERGE(D, false, true, s)
 COMMON(64)
 COMMON(128)
 COMMON(256)
@@ -790,9 +921,7 @@ STREAM(128, 2, 2)
 STREAM(256, 1, 2)
 SHARED(64, 2, 2)
 SHARED(128, 2, 2)
-SHARED(256, 1, 2)
-#else
+#endif
 SHARED(64, 1, 2)
 SHARED(128, 1, 2)
-SHARED(256, 1, 1)
-#endif
+SHARED(256, 1, 2)

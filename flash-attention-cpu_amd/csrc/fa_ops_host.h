@@ -178,30 +178,41 @@ int resolve_scale(float scale, float softcap, size_t d, ScoreScale* out) {
     return FA_OK;
 }
 
-// 16-row tiles a wave of the score kernels, which have four waves: two where that still makes
-// workgroups enough, `least` for every CU (what a wave reads from LDS serves both tiles).
-int score_tiles(int dtype, int D, size_t rows, size_t slices, size_t least, int num_cus) {
-    if (dtype == FA_DTYPE_F32 || D > 128) return 1;
-    return (rows + 127) / 128 * slices >= least * static_cast<size_t>(num_cus) ? 2 : 1;
+// How a score kernel's four waves share a block of rows: two 16-row tiles a wave where that still makes
+// workgroups enough (what a wave reads from LDS serves both tiles); on small grids two groups of
+// waves on the same rows, each with half of the walked rows.
+struct ScoreTiles {
+    int mt, groups, rows;   // rows of a block
+    const char* tag;
+};
+ScoreTiles score_tiles(const fa_score_config& c, int D, bool vec, size_t rows, size_t slices, int num_cus) {
+    const size_t cus = static_cast<size_t>(num_cus), blocks = (rows + 63) / 64 * slices;
+    // causal workgroups differ in length, so that a single round of them ends late
+    if (vec && c.dtype != FA_DTYPE_F32 && D <= 128 && (rows + 127) / 128 * slices >= (c.causal ? 4 : 2) * cus)
+        return {2, 1, 128, ""};
+    // measured (bf16, causal): 16 x 1024^2 d64 (256 blocks) 15.9 us against 18.7, 32 x 1024^2 (512) 19.3 against 19.6,
+    // 32 x 1024^2 d128 all visible (512) 38.2 against 27.2
+    if (vec && D <= 128 && 2 * blocks <= 3 * cus) return {1, 2, 32, "k"};
+    return {1, 1, 64, ""};
 }
-// Causal workgroups differ in length, so that a single round of them ends late.
-size_t score_rounds(const fa_score_config& c) { return c.causal ? 4 : 2; }
 
 // Plan of the dK / dV kernel: tiles a wave, and the workgroups that share the heads of a group.
 struct DkvPlan {
-    int mt, splits;
+    ScoreTiles tiles;
+    int splits;
     size_t blocks, floats;
 };
 DkvPlan plan_dkv(const fa_score_config& c, int D, bool vec, int num_cus) {
     DkvPlan r{};
     const size_t nkv = c.batch * c.kv_heads, group = c.heads / c.kv_heads;
-    r.mt = vec && D == 64 ? score_tiles(c.dtype, D, c.seq_len_k, nkv, 4, num_cus) : 1;
-    r.blocks = (c.seq_len_k + 64 * r.mt - 1) / (64 * r.mt);
     size_t s = 1;
-    while (s < group && r.blocks * nkv * s < 4 * static_cast<size_t>(num_cus)) {
+    while (s < group && (c.seq_len_k + 63) / 64 * nkv * s < 4 * static_cast<size_t>(num_cus)) {
         ++s;
         while (group % s != 0) ++s;
     }
+    r.tiles = score_tiles(c, D, vec, c.seq_len_k, nkv * s, num_cus);
+    if (D == 128 && r.tiles.mt == 2) r.tiles = {1, 1, 64, ""};   // two tiles' K, V, dK and dV leave one wave a SIMD: slower
+    r.blocks = (c.seq_len_k + r.tiles.rows - 1) / r.tiles.rows;
     r.splits = static_cast<int>(s);
     r.floats = s > 1 ? 2 * s * nkv * c.seq_len_k * D : 0;
     return r;
@@ -211,39 +222,47 @@ constexpr size_t kOpsMaxGrid = size_t(1) << 23;   // workgroups: threads of a la
 size_t doc_tiles(size_t n) { return (n + kDocTile - 1) / kDocTile; }
 
 // Plan of the rows kernels: streaming waves up to 64 rows, else workgroups that share their
-// keys; the keys in as many runs as fill the GPU.
+// keys; the keys of all sequences shared out over as many runs as fill the GPU once.
 struct RowsPlan {
     bool stream;
-    int mt, threads, rows, nrb, splits;
+    int mt, threads, rows, nrb, step, share, runs;
     size_t floats;
 };
-RowsPlan plan_rows(int dtype, int D, bool vec, size_t nkv, size_t rows, size_t keys, int num_cus) {
+RowsPlan plan_rows(int dtype, int D, bool vec, size_t batch, size_t kv_heads, size_t rows, size_t keys, int num_cus) {
     RowsPlan r{};
     const bool f32 = dtype == FA_DTYPE_F32;
     const int row_bytes = D * static_cast<int>(elem_size(dtype));
     r.stream = vec && rows <= 64 && row_bytes <= 512;
-    size_t step;
+    size_t resident = static_cast<size_t>(num_cus);
     if (r.stream) {
         // two tiles a wave as far as its registers hold them
         r.mt = rows <= 16 || row_bytes > 256 ? 1 : 2;
         const int waves = row_bytes <= 256 ? kStreamWaves<256> : kStreamWaves<512>;
         r.threads = 64 * waves;
         r.rows = 16 * r.mt;
-        step = 32 * waves;
+        r.step = 32 * waves;
+        if (row_bytes <= 128) resident *= 2;   // LDS holds one workgroup a CU, two of short rows
     } else {
-        r.mt = !vec || f32 || D > 128 ? 1 : 2;
-        r.threads = 256;
-        r.rows = 64 * r.mt;
-        step = f32 || D > 128 ? 32 : 64;
+        r.mt = !vec || f32 || D > 128 || rows <= 128 ? 1 : 2;
+        r.threads = 512;
+        r.rows = 128 * r.mt;
+        r.step = f32 || D > 128 ? 32 : 64;
     }
     r.nrb = static_cast<int>((rows + r.rows - 1) / r.rows);
-    const size_t units = std::max<size_t>(nkv * r.nrb, 1);
-    // one round of resident workgroups: LDS holds one streaming workgroup a CU, two of short rows or of shared stages
-    const size_t resident = (r.stream && row_bytes > 128 ? 1 : 2) * static_cast<size_t>(num_cus);
-    size_t splits = std::max<size_t>(1, resident / units);
-    splits = std::min(splits, std::max<size_t>(1, keys / step));
-    r.splits = static_cast<int>(std::min<size_t>(splits, 256));
-    r.floats = r.splits > 1 ? units * r.splits * r.rows * (D + 2) : 0;
+    const size_t units = kv_heads * r.nrb;   // workgroups a run
+    // One round of resident workgroups where the sequences' last, shorter runs (one a sequence)
+    // leave room, else several rounds of shorter runs.
+    const size_t slots = std::max<size_t>(1, resident / units);
+    size_t share = batch == 1 ? slots : 2 * (batch - 1) <= slots ? slots - (batch - 1) : 4 * slots;
+    share = std::min(share, batch * std::max<size_t>(1, (keys + r.step - 1) / r.step));
+    if (batch * units >= 4 * resident) share = 1;   // sequences enough: one run each
+    r.share = static_cast<int>(share);
+    // each sequence rounds its share up to whole runs; eight runs and heads more or less fall
+    // on the eight XCDs evenly
+    size_t runs = share == 1 ? batch : share + batch - 1;
+    while (runs * kv_heads % 8 != 0 && runs >= 8) ++runs;
+    r.runs = static_cast<int>(runs);
+    r.floats = share > 1 ? runs * units * r.rows * (D + 2) : 0;
     return r;
 }
 
@@ -252,27 +271,32 @@ int run_rows(int dev, hipStream_t stream, int dtype, int D, bool vec, RowsParams
     const OpsModule module = of_type(kCacheModule, dtype);
     int rc = ops_module(dev, module);
     if (rc != FA_OK) return rc;
-    const size_t nkv = static_cast<size_t>(p->batch) * p->kv_heads;
     const size_t rows = static_cast<size_t>(p->n) * p->group;
-    const RowsPlan plan = plan_rows(dtype, D, vec, nkv, rows, keys, g_dev[dev].num_cus);
+    const RowsPlan plan = plan_rows(dtype, D, vec, p->batch, p->kv_heads, rows, keys, g_dev[dev].num_cus);
     p->nrb = plan.nrb;
-    p->num_splits = plan.splits;
     p->block_rows = plan.rows;
-    const size_t grid = nkv * plan.nrb * plan.splits, mgrid = nkv * rows;
-    if (grid > kOpsMaxGrid || mgrid > kOpsMaxGrid) return FA_ERR_UNSUPPORTED;
+    p->num_runs = plan.runs;
+    p->share = plan.share;
+    p->step = plan.step;
+    const size_t grid = static_cast<size_t>(plan.runs) * p->kv_heads * plan.nrb;
+    const size_t mgrid = static_cast<size_t>(p->batch) * p->kv_heads * rows;
+    if (grid > kOpsMaxGrid / 2 || mgrid > kOpsMaxGrid) return FA_ERR_UNSUPPORTED;
     OpsWorkspace ws;
     if (plan.floats) {
         if ((rc = ws.get(dev, stream, plan.floats * sizeof(float))) != FA_OK) return rc;
         p->part_o = static_cast<float*>(ws.ptr);
-        p->part_ml = p->part_o + nkv * plan.nrb * plan.splits * plan.rows * D;
+        p->part_ml = p->part_o + grid * plan.rows * D;
     }
     char name[64];
     std::snprintf(name, sizeof(name), "fa_rows_%s_%s_d%d_t%d%s", plan.stream ? "stream" : "shared", dtype_name(dtype), D,
                   plan.mt, !vec ? "s" : p->slopes || p->cap_log2e != 0.0f ? "m" : "");
     rc = ops_launch(dev, module, name, grid, plan.threads, p, stream);
-    if (rc == FA_OK && plan.splits > 1) {
-        std::snprintf(name, sizeof(name), "fa_rows_merge_%s_d%d%s", dtype_name(dtype), D, vec ? "" : "s");
-        rc = ops_launch(dev, module, name, mgrid, 256, p, stream);
+    if (rc == FA_OK && plan.floats) {
+        // eight runs a sequence or more: a workgroup a row
+        const bool wide = !vec || plan.share > 8 * p->batch;
+        std::snprintf(name, sizeof(name), "fa_rows_merge_%s_d%d%s", dtype_name(dtype), D, !vec ? "s" : wide ? "w" : "");
+        const size_t per = wide ? 1 : 1024 / D;
+        rc = ops_launch(dev, module, name, (mgrid + per - 1) / per, 256, p, stream);
     }
     return ws.done(stream, rc);
 }
@@ -281,8 +305,9 @@ int run_rows(int dev, hipStream_t stream, int dtype, int D, bool vec, RowsParams
 bool score_takes_rows(const fa_score_config& c, int num_cus) {
     const size_t group = c.heads / c.kv_heads;
     if (c.seq_len_q * group <= 64) return true;
-    const size_t blocks = c.batch * c.heads * ((c.seq_len_q + 127) / 128);
-    return c.seq_len_k >= 512 && blocks * 4 <= static_cast<size_t>(num_cus);
+    // a workgroup of 32 rows takes some 0.6 us per 64 keys: above 2048 keys longer than the split and its merge
+    const size_t blocks = c.batch * c.heads * ((c.seq_len_q + 31) / 32);
+    return c.seq_len_k >= 2048 && 2 * blocks <= static_cast<size_t>(num_cus);
 }
 
 int check_score(const fa_score_config* c) {
@@ -416,7 +441,7 @@ int fa_score_forward(void* stream_, const fa_score_config* c, const void* q, con
         return rc;
     if (!q || !out || (c->seq_len_k > 0 && (!k || !v))) return FA_ERR_INVALID_ARG;
     const int D = ops_pad_d(d);
-    if (c->batch * c->heads > kOpsMaxGrid || (c->seq_len_q + 63) / 64 * c->batch * c->heads > kOpsMaxGrid)
+    if (c->batch * c->heads > kOpsMaxGrid || (c->seq_len_q + 31) / 32 * c->batch * c->heads > kOpsMaxGrid)
         return FA_ERR_UNSUPPORTED;
     int dev;
     if ((rc = ops_begin(&dev, of_type(kScoreModule, c->dtype))) != FA_OK) return rc;
@@ -439,8 +464,8 @@ int fa_score_forward(void* stream_, const fa_score_config* c, const void* q, con
     fill_score(*c, sc, &p);
     p.q = q, p.k = k, p.v = v, p.out = out, p.lse = lse;
     p.qs = lq.st, p.ks = lk.st, p.vs = lv.st, p.os = lo.st;
-    const int mt = vec ? score_tiles(c->dtype, D, c->seq_len_q, c->batch * c->heads, score_rounds(*c), g_dev[dev].num_cus) : 1;
-    p.nqb = static_cast<int>((c->seq_len_q + 64 * mt - 1) / (64 * mt));
+    const ScoreTiles tiles = score_tiles(*c, D, vec, c->seq_len_q, c->batch * c->heads, g_dev[dev].num_cus);
+    p.nqb = static_cast<int>((c->seq_len_q + tiles.rows - 1) / tiles.rows);
     OpsWorkspace ws;
     if (c->q_doc) {
         if ((rc = ws.get(dev, stream, doc_range_bytes(*c))) != FA_OK) return rc;
@@ -448,8 +473,8 @@ int fa_score_forward(void* stream_, const fa_score_config* c, const void* q, con
     }
     if (rc == FA_OK) {
         char name[64];
-        std::snprintf(name, sizeof(name), "fa_score_forward_%s_d%d_t%d%s", dtype_name(c->dtype), D, mt,
-                      !vec ? "s" : c->slopes || c->softcap > 0.0f ? "m" : "");
+        std::snprintf(name, sizeof(name), "fa_score_forward_%s_d%d_t%d%s%s", dtype_name(c->dtype), D, tiles.mt,
+                      tiles.tag, !vec ? "s" : c->slopes || c->softcap > 0.0f ? "m" : "");
         rc = ops_launch(dev, of_type(kScoreModule, c->dtype), name, c->batch * c->heads * p.nqb, 256, &p, stream);
     }
     return ws.done(stream, rc);
@@ -478,8 +503,8 @@ int fa_score_backward(void* stream_, const fa_score_config* c, const void* q, co
     if (sk > 0 && (!k || !v)) return FA_ERR_INVALID_ARG;
     const int D = ops_pad_d(d);
     const size_t rows = c->batch * c->heads * sq, dgrid = (rows + 15) / 16;
-    if (c->batch * c->heads > kOpsMaxGrid || (sq + 63) / 64 * c->batch * c->heads > kOpsMaxGrid ||
-        (sk + 63) / 64 * c->batch * c->heads > kOpsMaxGrid || dgrid > kOpsMaxGrid)
+    if (c->batch * c->heads > kOpsMaxGrid || (sq + 31) / 32 * c->batch * c->heads > kOpsMaxGrid ||
+        (sk + 31) / 32 * c->batch * c->heads > kOpsMaxGrid || dgrid > kOpsMaxGrid)
         return FA_ERR_UNSUPPORTED;
     int dev;
     if ((rc = ops_begin(&dev, of_type(kScoreModule, c->dtype))) != FA_OK) return rc;
@@ -511,7 +536,8 @@ int fa_score_backward(void* stream_, const fa_score_config* c, const void* q, co
     if (rc == FA_OK && (dk || dv)) {
         p.nqb = static_cast<int>(dkv.blocks);
         p.splits = dkv.splits;
-        std::snprintf(name, sizeof(name), "fa_score_dkv_%s_d%d_t%d%s", dtype_name(c->dtype), D, dkv.mt, mod);
+        std::snprintf(name, sizeof(name), "fa_score_dkv_%s_d%d_t%d%s%s", dtype_name(c->dtype), D, dkv.tiles.mt,
+                      dkv.tiles.tag, mod);
         rc = ops_launch(dev, of_type(kScoreModule, c->dtype), name, dkv.blocks * c->batch * c->kv_heads * dkv.splits, 256, &p,
                         stream);
         if (rc == FA_OK && dkv.splits > 1) {
@@ -521,9 +547,9 @@ int fa_score_backward(void* stream_, const fa_score_config* c, const void* q, co
         }
     }
     if (rc == FA_OK && dq) {
-        const int mt = vec ? score_tiles(c->dtype, D, sq, c->batch * c->heads, score_rounds(*c), g_dev[dev].num_cus) : 1;
-        p.nqb = static_cast<int>((sq + 64 * mt - 1) / (64 * mt));
-        std::snprintf(name, sizeof(name), "fa_score_dq_%s_d%d_t%d%s", dtype_name(c->dtype), D, mt, mod);
+        const ScoreTiles tiles = score_tiles(*c, D, vec, sq, c->batch * c->heads, g_dev[dev].num_cus);
+        p.nqb = static_cast<int>((sq + tiles.rows - 1) / tiles.rows);
+        std::snprintf(name, sizeof(name), "fa_score_dq_%s_d%d_t%d%s%s", dtype_name(c->dtype), D, tiles.mt, tiles.tag, mod);
         rc = ops_launch(dev, of_type(kScoreModule, c->dtype), name, c->batch * c->heads * p.nqb, 256, &p, stream);
     }
     return ws.done(stream, rc);

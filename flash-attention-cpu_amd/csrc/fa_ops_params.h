@@ -45,7 +45,7 @@ struct RowsParams {
     const void *q, *k, *v;
     void* out;
     float* lse;               // [batch, heads, n] or NULL
-    float *part_o, *part_ml;  // [slot][block_rows][D], [slot][2][block_rows]
+    float *part_o, *part_ml;  // [run][kv head][row block][block_rows][D], [..][2][block_rows]
     const float* slopes;
     const int32_t *q_doc, *k_doc, *prefix;   // score attention
     const int32_t *lens, *table, *pos;       // tree attention (lens != NULL)
@@ -55,8 +55,9 @@ struct RowsParams {
     int causal, q_start;
     int page_shift, n_pages, pages_per_seq;
     int mask_words, mask_shared;
-    int nrb, num_splits;      // row blocks of a (batch, kv head), splits of its keys
-    int block_rows;           // rows of a row block
+    int nrb, block_rows;      // row blocks of a (batch, kv head), and rows of one
+    int num_runs, share;      // runs of keys a kv head, all sequences together; what the keys are shared out over
+    int step;                 // keys that a run's length is a multiple of
     float scale, scale_log2e, cap_in, cap_log2e;
 };
 

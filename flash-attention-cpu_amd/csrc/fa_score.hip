@@ -135,9 +135,9 @@ __device__ __forceinline__ void fill_words(void* dst, const void* src, int n, in
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)dst, 4, 4 * lane, 0, 0, 0);
 }
 
-// Keys of a stage.
-template <typename T, int D>
-constexpr int kStageKeys = sizeof(T) == 4 || D > 128 ? 32 : 64;
+// Walked rows of a stage: 32 at least for each of the KG groups of waves that share them out.
+template <typename T, int D, int KG>
+constexpr int kStageRows = KG == 1 && (sizeof(T) == 4 || D > 128) ? 32 : 64;
 
 // Whether queries [q0, q1), of the documents qr, see a key of stage st, and whether
 // some pair is hidden.
@@ -158,16 +158,17 @@ __device__ __forceinline__ bool key_stage(const ScoreParams& p, int prefix, int 
 // ---------------------------------------------------------------------------
 // Forward
 // ---------------------------------------------------------------------------
-// Four waves of MT 16-row tiles.  K and V tiles are double-buffered and filled by DMA: while
+// Four waves of MT 16-row tiles (KG = 2: two groups of two waves keep the same rows, each with half of a
+// stage's keys, and their sums meet in LDS at the end: twice the workgroups, each half as long).  K and V tiles are double-buffered and filled by DMA: while
 // a stage's softmax and PV product run, K of the stage after the next and V of
 // the next arrive; one barrier a stage.  The loop is unrolled by two so that each buffer is
 // an array of its own.
-template <typename T, int D, int MT, bool MOD, bool VEC>
+template <typename T, int D, int MT, int KG, bool MOD, bool VEC>
 __device__ __forceinline__ void score_forward(const ScoreParams& p) {
     using M = Mma<T>;
     using v8 = typename M::v8;
-    constexpr int NW = 4, SK = kStageKeys<T, D>, BQ = 16 * MT * NW;
-    constexpr int KB = SK / 16, NCH = SK / 32, NDC = D / 32, NDB = D / 16, LD = D + kPad<T>;
+    constexpr int NW = 4, NR = NW / KG, SK = kStageRows<T, D, KG>, SW = SK / KG, BQ = 16 * MT * NR;
+    constexpr int KB = SW / 16, NCH = SW / 32, NDC = D / 32, NDB = D / 16, LD = D + kPad<T>;
     using Fill = TileFill<T, D, SK, NW, VEC>;
     T* const Kb0 = lds_array<T, Fill::SIZE, 0>();
     T* const Vb0 = lds_array<T, Fill::SIZE, 1>();
@@ -181,7 +182,8 @@ __device__ __forceinline__ void score_forward(const ScoreParams& p) {
     const int g = lane >> 4, li = lane & 15;
     const Work w = find_work(blockIdx.x, p.nqb, p.batch * p.kv_heads, p.group, p.kv_heads);
     const int h = w.hk * p.group + w.hq;
-    const int q0 = w.blk * BQ, row0 = q0 + 16 * MT * wave;
+    const int kg = wave / NR, koff = kg * SW;   // the wave's keys of a stage: koff .. koff + SW - 1
+    const int q0 = w.blk * BQ, row0 = q0 + 16 * MT * (wave % NR);
     const T* Q = slice<T>(p.q, p.qs, w.b, h);
     const T* K = slice<T>(p.k, p.ks, w.b, w.hk);
     const T* V = slice<T>(p.v, p.vs, w.b, w.hk);
@@ -234,7 +236,7 @@ __device__ __forceinline__ void score_forward(const ScoreParams& p) {
 #pragma unroll
         for (int dc = 0; dc < PRE_K && dc < NDC; ++dc)
 #pragma unroll
-            for (int b = 0; b < KB; ++b) kk[dc][b] = row_op<T, LD>(Ks, 16 * b, dc, g, li);
+            for (int b = 0; b < KB; ++b) kk[dc][b] = row_op<T, LD>(Ks, koff + 16 * b, dc, g, li);
 #pragma unroll
         for (int t = 0; t < MT; ++t)
 #pragma unroll
@@ -246,7 +248,7 @@ __device__ __forceinline__ void score_forward(const ScoreParams& p) {
         for (int dc = 0; dc < NDC; ++dc) {
             if (dc + PRE_K < NDC) {
 #pragma unroll
-                for (int b = 0; b < KB; ++b) kk[(dc + PRE_K) % KR][b] = row_op<T, LD>(Ks, 16 * b, dc + PRE_K, g, li);
+                for (int b = 0; b < KB; ++b) kk[(dc + PRE_K) % KR][b] = row_op<T, LD>(Ks, koff + 16 * b, dc + PRE_K, g, li);
             }
 #pragma unroll
             for (int b = 0; b < KB; ++b)
@@ -257,7 +259,7 @@ __device__ __forceinline__ void score_forward(const ScoreParams& p) {
         if constexpr (MOD) {
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
-                const float dist = (float)(p.q_start + row0 + 16 * t + li - k0 - 4 * g);
+                const float dist = (float)(p.q_start + row0 + 16 * t + li - k0 - koff - 4 * g);
 #pragma unroll
                 for (int b = 0; b < KB; ++b) {
                     if (cap) {
@@ -282,9 +284,9 @@ __device__ __forceinline__ void score_forward(const ScoreParams& p) {
     auto hide = [&](int k0, const int* ids) {
 #pragma unroll
         for (int b = 0; b < KB; ++b) {
-            const int key = k0 + 16 * b + 4 * g;
+            const int key = k0 + koff + 16 * b + 4 * g;
             if (docs) {
-                const i32x4 kd = *reinterpret_cast<const i32x4*>(ids + 16 * b + 4 * g);
+                const i32x4 kd = *reinterpret_cast<const i32x4*>(ids + koff + 16 * b + 4 * g);
 #pragma unroll
                 for (int t = 0; t < MT; ++t)
 #pragma unroll
@@ -338,7 +340,7 @@ __device__ __forceinline__ void score_forward(const ScoreParams& p) {
     };
     constexpr int PRE_V = NCH * NDB >= 4 ? 3 : 1, VR = PRE_V + 1;
     v8 va[VR];
-    auto v_op = [&](const T* Vs, int i) { return col_op<T, LD>(Vs, 32 * (i / NDB), 16 * (i % NDB), g, li); };
+    auto v_op = [&](const T* Vs, int i) { return col_op<T, LD>(Vs, koff + 32 * (i / NDB), 16 * (i % NDB), g, li); };
     auto pv_preload = [&](const T* Vs) {
 #pragma unroll
         for (int i = 0; i < PRE_V; ++i) va[i] = v_op(Vs, i);
@@ -355,7 +357,8 @@ __device__ __forceinline__ void score_forward(const ScoreParams& p) {
     // whether some row of the wave sees some key of the stage (as far as causal and prefix tell)
     auto active = [&](int st) -> bool {
         if (st < 0 || row0 >= p.sq) return false;
-        return !p.causal || st * SK <= p.q_start + row0 + 16 * MT - 1 || st * SK < prefix;
+        const int k0 = st * SK + koff;
+        return k0 < p.sk && (!p.causal || k0 <= p.q_start + row0 + 16 * MT - 1 || k0 < prefix);
     };
 
     bool masked, masked_next = false;
@@ -411,6 +414,26 @@ __device__ __forceinline__ void score_forward(const ScoreParams& p) {
     }
 
     const ScoreParams lp = late_params<ScoreParams>();
+    if constexpr (KG > 1) {
+        // the last stage's barrier freed the tiles
+        static_assert(MT == 1 && KG == 2 && NR * NDB * 64 * 16 <= Fill::SIZE * (int)sizeof(T), "sums fit a tile");
+        f32x4* const sums = reinterpret_cast<f32x4*>(Kb0) + wave % NR * NDB * 64;
+        float* const ml = reinterpret_cast<float*>(Vb0) + wave % NR * 128;
+        if (kg == 1) {
+#pragma unroll
+            for (int j = 0; j < NDB; ++j) sums[j * 64 + lane] = o[0][j];
+            ml[lane] = m[0];
+            ml[64 + lane] = l[0];
+        }
+        __syncthreads();
+        if (kg == 1) return;
+        const float m2 = ml[lane], mn = fmaxf(m[0], m2), top = mn == OPS_NEG_INF ? 0.0f : mn;
+        const float c1 = ops_exp2((m[0] - top) * c), c2 = ops_exp2((m2 - top) * c);
+        m[0] = mn;
+        l[0] = l[0] * c1 + ml[64 + lane] * c2;
+#pragma unroll
+        for (int j = 0; j < NDB; ++j) o[0][j] = o[0][j] * c1 + sums[j * 64 + lane] * c2;
+    }
     T* O = slice<T>(lp.out, lp.os, w.b, h);
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
@@ -490,12 +513,12 @@ __device__ __forceinline__ void weigh(const ScoreParams& p, bool cap, f32x4 s, f
 }
 
 // dQ: query rows kept, keys walked.  Four waves of MT 16-row tiles; K and V tiles double-buffered, one barrier a stage.
-template <typename T, int D, int MT, bool MOD, bool VEC>
+template <typename T, int D, int MT, int KG, bool MOD, bool VEC>
 __device__ __forceinline__ void score_dq(const ScoreParams& p) {
     using M = Mma<T>;
     using v8 = typename M::v8;
-    constexpr int NW = 4, SK = kStageKeys<T, D>, BQ = 16 * MT * NW;
-    constexpr int NCH = SK / 32, NDC = D / 32, NDB = D / 16, LD = D + kPad<T>;
+    constexpr int NW = 4, NR = NW / KG, SK = kStageRows<T, D, KG>, BQ = 16 * MT * NR;
+    constexpr int NCH = SK / 32 / KG, NDC = D / 32, NDB = D / 16, LD = D + kPad<T>;
     using Fill = TileFill<T, D, SK, NW, VEC>;
     T* const Kb0 = lds_array<T, Fill::SIZE, 0>();
     T* const Vb0 = lds_array<T, Fill::SIZE, 1>();
@@ -509,7 +532,8 @@ __device__ __forceinline__ void score_dq(const ScoreParams& p) {
     const int g = lane >> 4, li = lane & 15;
     const Work w = find_work(blockIdx.x, p.nqb, p.batch * p.kv_heads, p.group, p.kv_heads);
     const int h = w.hk * p.group + w.hq;
-    const int q0 = w.blk * BQ, row0 = q0 + 16 * MT * wave;
+    const int kg = wave / NR, koff = kg * 32 * NCH;   // the wave's keys of a stage
+    const int q0 = w.blk * BQ, row0 = q0 + 16 * MT * (wave % NR);
     const T* Q = slice<T>(p.q, p.qs, w.b, h);
     const T* dO = slice<T>(p.dout, p.dos, w.b, h);
     const T* K = slice<T>(p.k, p.ks, w.b, w.hk);
@@ -557,7 +581,8 @@ __device__ __forceinline__ void score_dq(const ScoreParams& p) {
     };
     auto active = [&](int st) -> bool {
         if (row0 >= p.sq) return false;
-        return !p.causal || st * SK <= p.q_start + row0 + 16 * MT - 1 || st * SK < prefix;
+        const int k0 = st * SK + koff;
+        return k0 < p.sk && (!p.causal || k0 <= p.q_start + row0 + 16 * MT - 1 || k0 < prefix);
     };
 
     bool masked = false, masked_next = false;
@@ -588,8 +613,8 @@ __device__ __forceinline__ void score_dq(const ScoreParams& p) {
                 for (int dc = 0; dc < NDC; ++dc) {
 #pragma unroll
                     for (int b = 0; b < 2; ++b) {
-                        const v8 ka = row_op<T, LD>(Ks, 32 * i + 16 * b, dc, g, li);
-                        const v8 va = row_op<T, LD>(Vs, 32 * i + 16 * b, dc, g, li);
+                        const v8 ka = row_op<T, LD>(Ks, koff + 32 * i + 16 * b, dc, g, li);
+                        const v8 va = row_op<T, LD>(Vs, koff + 32 * i + 16 * b, dc, g, li);
 #pragma unroll
                         for (int t = 0; t < MT; ++t) {
                             s[t][b] = M::mma(ka, qreg[t][dc], s[t][b]);
@@ -604,12 +629,12 @@ __device__ __forceinline__ void score_dq(const ScoreParams& p) {
 #pragma unroll
                     for (int b = 0; b < 2; ++b) {
                         f32x4 x, ds;
-                        const int key = k0 + 32 * i + 16 * b + 4 * g;
+                        const int key = k0 + koff + 32 * i + 16 * b + 4 * g;
                         weigh<T, MOD>(p, cap, s[t][b], dp[t][b], (f32x4){lse2[t], lse2[t], lse2[t], lse2[t]},
                                       (f32x4){delta[t], delta[t], delta[t], delta[t]}, slope, (float)(pos - key), &x, &ds);
                         if (masked) {
                             if (docs) {
-                                const i32x4 kd = *reinterpret_cast<const i32x4*>(ids + 32 * i + 16 * b + 4 * g);
+                                const i32x4 kd = *reinterpret_cast<const i32x4*>(ids + koff + 32 * i + 16 * b + 4 * g);
 #pragma unroll
                                 for (int r = 0; r < 4; ++r)
                                     if (kd[r] != qd[t]) ds[r] = 0.0f;
@@ -625,13 +650,13 @@ __device__ __forceinline__ void score_dq(const ScoreParams& p) {
             }
             if (masked) {
                 __syncthreads();
-                if (tile_clean<T, LD, D, 32, 64 * NW>(Ks + 32 * i * LD, tid)) *Special = 1;
+                if (tile_clean<T, LD, D, 32 * KG, 64 * NW>(Ks + 32 * i * LD, tid)) *Special = 1;
                 __syncthreads();
             }
             if (act) {
 #pragma unroll
                 for (int j = 0; j < NDB; ++j) {
-                    const v8 a = col_op<T, LD>(Ks, 32 * i, 16 * j, g, li);
+                    const v8 a = col_op<T, LD>(Ks, koff + 32 * i, 16 * j, g, li);
 #pragma unroll
                     for (int t = 0; t < MT; ++t) dq[t][j] = M::mma(a, db[t][0], dq[t][j]);
                     if (j % 4 == 3) __builtin_amdgcn_sched_barrier(0);
@@ -648,6 +673,18 @@ __device__ __forceinline__ void score_dq(const ScoreParams& p) {
         step(std::integral_constant<int, 1>{});
     }
     const ScoreParams lp = late_params<ScoreParams>();
+    if constexpr (KG > 1) {
+        static_assert(MT == 1 && KG == 2 && NCH == 1 && NR * NDB * 64 * 16 <= Fill::SIZE * (int)sizeof(T), "sums fit a tile");
+        f32x4* const sums = reinterpret_cast<f32x4*>(Kb0) + wave % NR * NDB * 64;
+        if (kg == 1) {
+#pragma unroll
+            for (int j = 0; j < NDB; ++j) sums[j * 64 + lane] = dq[0][j];
+        }
+        __syncthreads();
+        if (kg == 1) return;
+#pragma unroll
+        for (int j = 0; j < NDB; ++j) dq[0][j] += sums[j * 64 + lane];
+    }
     T* out = slice<T>(lp.dq, lp.dqs, w.b, h);
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
@@ -693,12 +730,12 @@ __device__ __forceinline__ void dkv_specials(const ScoreParams& p, Test test, in
 // dK and dV: key rows kept, the queries of every head of the group walked.  Four waves
 // of MT 16-row tiles; Q and dO tiles double-buffered, one barrier a stage.  A kv head's sums over its
 // query heads are formed here, in head order, or by score_dkv_sum where workgroups share them.
-template <typename T, int D, int MT, bool MOD, bool VEC>
+template <typename T, int D, int MT, int KG, bool MOD, bool VEC>
 __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
     using M = Mma<T>;
     using v8 = typename M::v8;
-    constexpr int NW = 4, SQ = kStageKeys<T, D>, BK = 16 * MT * NW;
-    constexpr int NCH = SQ / 32, NDC = D / 32, NDB = D / 16, LD = D + kPad<T>;
+    constexpr int NW = 4, NR = NW / KG, SQ = kStageRows<T, D, KG>, BK = 16 * MT * NR;
+    constexpr int NCH = SQ / 32 / KG, NDC = D / 32, NDB = D / 16, LD = D + kPad<T>;
     using Fill = TileFill<T, D, SQ, NW, VEC>;
     T* const Qb0 = lds_array<T, Fill::SIZE, 0>();
     T* const Ob0 = lds_array<T, Fill::SIZE, 1>();
@@ -713,7 +750,8 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
     // a workgroup takes heads first .. first + count - 1 of a kv head's group; the first key blocks have most queries where causal
     const Work w = find_work(gridDim.x - 1 - blockIdx.x, p.nqb, p.batch * p.kv_heads, p.splits, p.kv_heads);
     const int count = p.group / p.splits, first = w.hk * p.group + w.hq * count;
-    const int kbeg = w.blk * BK, key0 = kbeg + 16 * MT * wave;
+    const int kg = wave / NR, qoff = kg * 32 * NCH;   // the wave's queries of a stage
+    const int kbeg = w.blk * BK, key0 = kbeg + 16 * MT * (wave % NR);
     const T* K = slice<T>(p.k, p.ks, w.b, w.hk);
     const T* V = slice<T>(p.v, p.vs, w.b, w.hk);
     const bool docs = p.q_doc != nullptr;
@@ -780,7 +818,7 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
     };
     auto active = [&](int st) -> bool {
         if (key0 >= p.sk) return false;
-        return !p.causal || p.q_start + st * SQ + SQ - 1 >= key0 || key0 < prefix;
+        return st * SQ + qoff < p.sq && (!p.causal || p.q_start + st * SQ + qoff + 32 * NCH - 1 >= key0 || key0 < prefix);
     };
 
     bool masked = false, masked_next = false;
@@ -813,8 +851,8 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
                 for (int dc = 0; dc < NDC; ++dc) {
 #pragma unroll
                     for (int b = 0; b < 2; ++b) {
-                        const v8 qa = row_op<T, LD>(Qs, 32 * i + 16 * b, dc, g, li);
-                        const v8 oa = row_op<T, LD>(Os, 32 * i + 16 * b, dc, g, li);
+                        const v8 qa = row_op<T, LD>(Qs, qoff + 32 * i + 16 * b, dc, g, li);
+                        const v8 oa = row_op<T, LD>(Os, qoff + 32 * i + 16 * b, dc, g, li);
 #pragma unroll
                         for (int t = 0; t < MT; ++t) {
                             s[t][b] = M::mma(qa, kreg[t][dc], s[t][b]);
@@ -825,7 +863,7 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
                 }
 #pragma unroll
                 for (int b = 0; b < 2; ++b) {
-                    const int at = 32 * i + 16 * b + 4 * g, pos = p.q_start + q0 + at;
+                    const int at = qoff + 32 * i + 16 * b + 4 * g, pos = p.q_start + q0 + at;
                     const f32x4 lse2 = *reinterpret_cast<const f32x4*>(Ls + at);
                     const f32x4 delta = *reinterpret_cast<const f32x4*>(Ls + 64 + at);
 #pragma unroll
@@ -854,15 +892,15 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
             }
             if (masked) {
                 __syncthreads();
-                const bool bad = tile_clean<T, LD, D, 32, 64 * NW>(Qs + 32 * i * LD, tid);
-                if (tile_clean<T, LD, D, 32, 64 * NW>(Os + 32 * i * LD, tid) || bad) *Special = 1;
+                const bool bad = tile_clean<T, LD, D, 32 * KG, 64 * NW>(Qs + 32 * i * LD, tid);
+                if (tile_clean<T, LD, D, 32 * KG, 64 * NW>(Os + 32 * i * LD, tid) || bad) *Special = 1;
                 __syncthreads();
             }
             if (act) {
 #pragma unroll
                 for (int j = 0; j < NDB; ++j) {
-                    const v8 a = col_op<T, LD>(Os, 32 * i, 16 * j, g, li);
-                    const v8 c = col_op<T, LD>(Qs, 32 * i, 16 * j, g, li);
+                    const v8 a = col_op<T, LD>(Os, qoff + 32 * i, 16 * j, g, li);
+                    const v8 c = col_op<T, LD>(Qs, qoff + 32 * i, 16 * j, g, li);
 #pragma unroll
                     for (int t = 0; t < MT; ++t) {
                         dv[t][j] = M::mma(a, pb[t][0], dv[t][j]);
@@ -882,6 +920,25 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
         step(std::integral_constant<int, 1>{});
     }
     const ScoreParams lp = late_params<ScoreParams>();
+    if constexpr (KG > 1) {
+        static_assert(MT == 1 && KG == 2 && NCH == 1 && NR * NDB * 64 * 16 <= Fill::SIZE * (int)sizeof(T), "sums fit a tile");
+        f32x4* const ksum = reinterpret_cast<f32x4*>(Qb0) + wave % NR * NDB * 64;
+        f32x4* const vsum = reinterpret_cast<f32x4*>(Ob0) + wave % NR * NDB * 64;
+        if (kg == 1) {
+#pragma unroll
+            for (int j = 0; j < NDB; ++j) {
+                ksum[j * 64 + lane] = dk[0][j];
+                vsum[j * 64 + lane] = dv[0][j];
+            }
+        }
+        __syncthreads();
+        if (kg == 1) return;
+#pragma unroll
+        for (int j = 0; j < NDB; ++j) {
+            dk[0][j] += ksum[j * 64 + lane];
+            dv[0][j] += vsum[j * 64 + lane];
+        }
+    }
     if (lp.splits > 1) {
         const int64_t rows = (int64_t)lp.batch * lp.kv_heads * lp.sk;   // of one split
         float* const outk = lp.part + (w.hq * rows + ((int64_t)w.b * lp.kv_heads + w.hk) * lp.sk) * D;
@@ -970,10 +1027,10 @@ extern "C" __global__ __launch_bounds__(256) void fa_score_doc_ranges(ScoreParam
     }
 DELTA(true, )
 DELTA(false, s)
-#define KERNEL(F, D, MT, MOD, VEC, TAG, WAVES)                                                        \
+#define KERNEL(F, D, MT, KG, MOD, VEC, TAG, WAVES)                                                    \
     extern "C" __global__ __launch_bounds__(256, WAVES) void PASTE(fa_score_##F##_, OPS_NAME, _d##D##_t##MT, TAG)( \
         ScoreParams p) {                                                                              \
-        score_##F<OPS_T, D, MT, MOD, VEC>(p);                                                         \
+        score_##F<OPS_T, D, MT, KG, MOD, VEC>(p);                                                     \
     }
 #define SUM(D, VEC, TAG)                                                                                         \
     extern "C" __global__ __launch_bounds__(256) void PASTE(fa_score_dkv_sum_, OPS_NAME, _d##D, TAG)(ScoreParams p) { \
@@ -985,33 +1042,37 @@ SUM(256, true, )
 SUM(64, false, s)
 SUM(128, false, s)
 SUM(256, false, s)
-// plain scores, modified ones (m), and any alignment (s)
-#define KERNELS(F, D, MT, WAVES)             \
-    KERNEL(F, D, MT, false, true, , WAVES)   \
-    KERNEL(F, D, MT, true, true, m, WAVES)
-KERNELS(forward, 64, 1, 2)
-KERNELS(forward, 128, 1, 2)
-KERNELS(dq, 64, 1, 2)
-KERNELS(dq, 128, 1, 2)
-KERNELS(dkv, 64, 1, 2)
-KERNELS(dkv, 128, 1, 2)
-KERNELS(dkv, 256, 1, 1)
-#define SLOW(F, W64, W128, W256)              \
-    KERNEL(F, 64, 1, true, false, s, W64)     \
-    KERNEL(F, 128, 1, true, false, s, W128)   \
-    KERNEL(F, 256, 1, true, false, s, W256)
+// plain scores, modified ones (m), any alignment (s); two groups of waves on a stage (k)
+#define KERNELS(F, D, MT, WAVES)                \
+    KERNEL(F, D, MT, 1, false, true, , WAVES)   \
+    KERNEL(F, D, MT, 1, true, true, m, WAVES)
+#define GROUPS(F, D, WAVES)                     \
+    KERNEL(F, D, 1, 2, false, true, k, WAVES)   \
+    KERNEL(F, D, 1, 2, true, true, km, WAVES)
+#define SLOW(F, W64, W128, W256)                 \
+    KERNEL(F, 64, 1, 1, true, false, s, W64)     \
+    KERNEL(F, 128, 1, 1, true, false, s, W128)   \
+    KERNEL(F, 256, 1, 1, true, false, s, W256)
+#define ALL(F, W64, W128, W256)  \
+    KERNELS(F, 64, 1, W64)       \
+    KERNELS(F, 128, 1, W128)     \
+    KERNELS(F, 256, 1, W256)     \
+    GROUPS(F, 64, W64)           \
+    GROUPS(F, 128, W128)
 SLOW(forward, 2, 1, 1)
 SLOW(dq, 2, 1, 1)
 SLOW(dkv, 2, 1, 1)
 #ifdef OPS_16BIT
+ALL(forward, 2, 2, 2)
+ALL(dq, 2, 2, 2)
+ALL(dkv, 2, 2, 1)
 KERNELS(forward, 64, 2, 2)
 KERNELS(forward, 128, 2, 2)
-KERNELS(forward, 256, 1, 2)
 KERNELS(dq, 64, 2, 2)
 KERNELS(dq, 128, 2, 2)
-KERNELS(dq, 256, 1, 2)
 KERNELS(dkv, 64, 2, 2)
 #else
-KERNELS(forward, 256, 1, 1)
-KERNELS(dq, 256, 1, 1)
+ALL(forward, 2, 2, 1)
+ALL(dq, 2, 2, 1)
+ALL(dkv, 2, 2, 1)
 #endif
