@@ -63,11 +63,6 @@ struct Swizzled {
     }
 };
 
-__device__ __forceinline__ int load_uniform(const int32_t* p) {
-    // a scalar load: a vector load would wait for all of the wave's DMA
-    return *(const __attribute__((address_space(4))) int32_t*)p;
-}
-
 // The pages of a sequence.
 struct CachePages {
     const int32_t* table;   // nullptr: rows one after another

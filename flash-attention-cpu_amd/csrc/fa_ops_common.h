@@ -42,6 +42,13 @@ __device__ __forceinline__ P late_params() {
     return p;
 }
 
+// A scalar load of what all lanes want: a vector load would come back only after all of the
+// wave's DMA.
+template <typename V>
+__device__ __forceinline__ V load_uniform(const V* p) {
+    return *(const __attribute__((address_space(4))) V*)p;
+}
+
 template <typename T>
 struct Mma;
 template <>
@@ -191,37 +198,45 @@ __device__ __forceinline__ void reread() {
 
 // Tiles that hold hidden pairs: a hidden pair has the weight 0, and values of rows that a
 // query does not see must not reach its sum, not even as 0 * inf.  So before
-// such a tile is multiplied, its infinities and NaN are replaced by zeros in LDS, each
-// thread looking at its share; where there were any, the kernel adds them once its
-// sums are written, to the rows that see them.  Returns whether the thread found one.
+// such a tile is multiplied, its infinities and NaN are replaced by zeros in LDS; where there
+// were any, the kernel adds them once its sums are written, to the rows that see them.
+
+// Whether a chunk of 16 bytes holds an infinity or NaN.
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+template <typename T>
+__device__ __forceinline__ bool chunk_special(u32x4 u) {
+    if constexpr (sizeof(T) == 2) {
+        // half words: magnitude + (2^15 - infinity) reaches 2^15 where not finite
+        constexpr unsigned kAdd = (0x8000u - (std::is_same<T, __bf16>::value ? 0x7f80u : 0x7c00u)) * 0x10001u;
+        unsigned any = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) any |= (u[e] & 0x7fff7fffu) + kAdd;
+        return (any & 0x80008000u) != 0;
+    } else {
+        bool bad = false;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) bad = bad || (u[e] & 0x7f800000u) == 0x7f800000u;
+        return bad;
+    }
+}
+template <typename T>
+__device__ __forceinline__ void clean_chunk(T* at) {
+#pragma unroll 1
+    for (int e = 0; e < 16 / (int)sizeof(T); ++e)
+        if (not_finite(float(at[e]))) at[e] = T(0.0f);
+}
+
+// Cleans ROWS rows of D elements (LD apart), NT threads; returns whether the thread found something.
 template <typename T, int LD, int D, int ROWS, int NT>
 __device__ __forceinline__ bool tile_clean(T* tile, int tid) {
-    using v8 = typename Mma<T>::v8;
-    constexpr int CPR = D / 8;
+    constexpr int E = 16 / (int)sizeof(T), CPR = D / E;
     bool found = false;
 #pragma unroll 1
     for (int pos = tid; pos < ROWS * CPR; pos += NT) {
-        T* at = tile + pos / CPR * LD + 8 * (pos % CPR);
-        v8 x = *reinterpret_cast<v8*>(at);
-        bool bad = false;
-        if constexpr (sizeof(T) == 2) {
-            // half words: magnitude + (2^15 - infinity) reaches 2^15 where not finite
-            constexpr unsigned kAdd = (0x8000u - (std::is_same<T, __bf16>::value ? 0x7f80u : 0x7c00u)) * 0x10001u;
-            typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-            const u32x4 u = __builtin_bit_cast(u32x4, x);
-            unsigned any = 0;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) any |= (u[e] & 0x7fff7fffu) + kAdd;
-            bad = (any & 0x80008000u) != 0;
-        } else {
-            bad = any_not_finite<T>(x);
-        }
-        if (bad) {
+        T* const at = tile + pos / CPR * LD + E * (pos % CPR);
+        if (chunk_special<T>(*reinterpret_cast<const u32x4*>(at))) {
             found = true;
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (not_finite(float(x[e]))) x[e] = T(0.0f);
-            *reinterpret_cast<v8*>(at) = x;
+            clean_chunk<T>(at);
         }
     }
     return found;
@@ -301,6 +316,30 @@ struct TileFill {
                     global_row<T, false>(src, stride, r, rows - row0, col, d);
             }
         }
+    }
+    // Whether what the lane itself filled, and what has arrived, holds an infinity or NaN; CLEAN: they become zeros.
+    template <bool CLEAN>
+    __device__ __forceinline__ bool special(T* dst) const {
+        bool found = false;
+        auto look = [&](T* at) {
+            if (chunk_special<T>(*reinterpret_cast<const u32x4*>(at))) {
+                found = true;
+                if (CLEAN) clean_chunk<T>(at);
+            }
+        };
+        if constexpr (VEC) {
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                const int run = i * NW + wave;
+                if ((i + 1) * NW <= RUNS || run < RUNS) look(dst + (run * 64 + lane) * E);
+            }
+        } else {
+#pragma unroll 1
+            for (int pos = wave * 64 + lane; pos < ROWS * (D / 8); pos += 64 * NW)
+#pragma unroll
+                for (int c = 0; c < 8; c += E) look(dst + pos / (D / 8) * LD + 8 * (pos % (D / 8)) + c);
+        }
+        return found;
     }
 };
 

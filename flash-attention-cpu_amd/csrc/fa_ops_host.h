@@ -178,6 +178,11 @@ int resolve_scale(float scale, float softcap, size_t d, ScoreScale* out) {
     return FA_OK;
 }
 
+// Tag of the kernel for what happens to the scores.
+const char* score_tag(const fa_score_config& c, bool vec) {
+    return !vec ? "s" : c.softcap > 0.0f ? (c.slopes ? "cb" : "c") : c.slopes ? "b" : "";
+}
+
 // How a score kernel's four waves share a block of rows: two 16-row tiles a wave where that still makes
 // workgroups enough (what a wave reads from LDS serves both tiles); on small grids two groups of
 // waves on the same rows, each with half of the walked rows.
@@ -474,7 +479,7 @@ int fa_score_forward(void* stream_, const fa_score_config* c, const void* q, con
     if (rc == FA_OK) {
         char name[64];
         std::snprintf(name, sizeof(name), "fa_score_forward_%s_d%d_t%d%s%s", dtype_name(c->dtype), D, tiles.mt,
-                      tiles.tag, !vec ? "s" : c->slopes || c->softcap > 0.0f ? "m" : "");
+                      tiles.tag, score_tag(*c, vec));
         rc = ops_launch(dev, of_type(kScoreModule, c->dtype), name, c->batch * c->heads * p.nqb, 256, &p, stream);
     }
     return ws.done(stream, rc);
@@ -532,7 +537,7 @@ int fa_score_backward(void* stream_, const fa_score_config* c, const void* q, co
         std::snprintf(name, sizeof(name), "fa_score_delta_%s%s", dtype_name(c->dtype), vec ? "" : "s");
         rc = ops_launch(dev, of_type(kScoreModule, c->dtype), name, dgrid, 256, &p, stream);
     }
-    const char* mod = !vec ? "s" : c->slopes || c->softcap > 0.0f ? "m" : "";
+    const char* mod = score_tag(*c, vec);
     if (rc == FA_OK && (dk || dv)) {
         p.nqb = static_cast<int>(dkv.blocks);
         p.splits = dkv.splits;

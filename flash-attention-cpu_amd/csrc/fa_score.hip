@@ -17,6 +17,17 @@
 
 #include "fa_ops_common.h"
 
+// What happens to scores, fixed for a kernel: bits kCap and kBias, or kAny: looked up in the parameters.
+constexpr int kCap = 1, kBias = 2, kAny = 4;
+template <int MOD>
+__device__ __forceinline__ bool has_cap(const ScoreParams& p) {
+    return MOD == kAny ? p.cap_log2e != 0.0f : (MOD & kCap) != 0;
+}
+template <int MOD>
+__device__ __forceinline__ bool has_bias(const ScoreParams& p) {
+    return MOD == kAny ? p.slopes != nullptr : (MOD & kBias) != 0;
+}
+
 template <typename T>
 __device__ __forceinline__ const T* slice(const void* base, OpsStrides st, int b, int h) {
     return reinterpret_cast<const T*>(base) + b * st.b + h * st.h;
@@ -62,8 +73,8 @@ struct Stages {
     int base, count, lane;
     Test test;
     __device__ __forceinline__ Stages(int n, int lane_, Test t) : base(-64), count(n), lane(lane_), test(t) {}
-    // next stage (-1: none); *masked: it needs the mask
-    __device__ __forceinline__ int next(bool* masked) {
+    // next stage (-1: none); *masked: it needs the mask (an int: uniform flags stay in one scalar register)
+    __device__ __forceinline__ int next(int* masked) {
         while (vis == 0) {
             base += 64;
             if (base >= count) return -1;
@@ -74,7 +85,7 @@ struct Stages {
         }
         const int bit = __builtin_ctzll(vis);
         vis &= vis - 1;
-        *masked = (part >> bit) & 1;
+        *masked = (int)(part >> bit) & 1;
         return base + bit;
     }
 };
@@ -83,7 +94,7 @@ struct Stages {
 template <typename Test, typename F>
 __device__ __forceinline__ void each_masked(Test test, int count, int lane, F f) {
     Stages<Test> stages(count, lane, test);
-    bool masked;
+    int masked;
     for (int st = stages.next(&masked); st >= 0; st = stages.next(&masked))
         if (masked) f(st);
 }
@@ -163,7 +174,7 @@ __device__ __forceinline__ bool key_stage(const ScoreParams& p, int prefix, int 
 // a stage's softmax and PV product run, K of the stage after the next and V of
 // the next arrive; one barrier a stage.  The loop is unrolled by two so that each buffer is
 // an array of its own.
-template <typename T, int D, int MT, int KG, bool MOD, bool VEC>
+template <typename T, int D, int MT, int KG, int MOD, bool VEC>
 __device__ __forceinline__ void score_forward(const ScoreParams& p) {
     using M = Mma<T>;
     using v8 = typename M::v8;
@@ -189,11 +200,11 @@ __device__ __forceinline__ void score_forward(const ScoreParams& p) {
     const T* V = slice<T>(p.v, p.vs, w.b, w.hk);
     const bool docs = p.q_doc != nullptr;
     const int32_t* kdoc = docs ? p.k_doc + (int64_t)w.b * p.sk : nullptr;
-    const int prefix = p.prefix ? p.prefix[w.b] : 0;
-    const float slope = MOD && p.slopes ? p.slopes[h] * kLog2e : 0.0f;
-    const bool cap = MOD && p.cap_log2e != 0.0f;
+    const int prefix = p.prefix ? load_uniform(p.prefix + w.b) : 0;
+    const float slope = has_bias<MOD>(p) ? load_uniform(p.slopes + h) * kLog2e : 0.0f;
+    const bool cap = has_cap<MOD>(p);
     // scores leave the QK^T chains raw, and the scale goes into the exponent; modified ones are in log2 units
-    const float c = MOD ? 1.0f : p.scale_log2e;
+    const float c = MOD != 0 ? 1.0f : p.scale_log2e;
 
     v8 qreg[MT][NDC];
     int qd[MT], limit[MT];   // a row's document, and the keys before which it may see
@@ -241,7 +252,7 @@ __device__ __forceinline__ void score_forward(const ScoreParams& p) {
         for (int t = 0; t < MT; ++t)
 #pragma unroll
             for (int b = 0; b < KB; ++b) {
-                const float x = MOD ? 0.0f : -ref[t];
+                const float x = MOD != 0 ? 0.0f : -ref[t];
                 s[t][b] = (f32x4){x, x, x, x};
             }
 #pragma unroll
@@ -256,7 +267,7 @@ __device__ __forceinline__ void score_forward(const ScoreParams& p) {
                 for (int t = 0; t < MT; ++t) s[t][b] = M::mma(kk[dc % KR][b], qreg[t][dc], s[t][b]);
             __builtin_amdgcn_sched_barrier(0);
         }
-        if constexpr (MOD) {
+        if constexpr (MOD != 0) {
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
                 const float dist = (float)(p.q_start + row0 + 16 * t + li - k0 - koff - 4 * g);
@@ -272,7 +283,7 @@ __device__ __forceinline__ void score_forward(const ScoreParams& p) {
 #pragma unroll
                         for (int r = 0; r < 4; ++r) s[t][b][r] = __builtin_fmaf(s[t][b][r], p.scale_log2e, -ref[t]);
                     }
-                    if (p.slopes) {
+                    if (has_bias<MOD>(p)) {
 #pragma unroll
                         for (int r = 0; r < 4; ++r)
                             s[t][b][r] = __builtin_fmaf(-slope, fabsf(dist - (float)(16 * b + r)), s[t][b][r]);
@@ -355,13 +366,16 @@ __device__ __forceinline__ void score_forward(const ScoreParams& p) {
         }
     };
     // whether some row of the wave sees some key of the stage (as far as causal and prefix tell)
-    auto active = [&](int st) -> bool {
+    auto active = [&](int st) -> int {
         if (st < 0 || row0 >= p.sq) return false;
         const int k0 = st * SK + koff;
         return k0 < p.sk && (!p.causal || k0 <= p.q_start + row0 + 16 * MT - 1 || k0 < prefix);
     };
 
-    bool masked, masked_next = false;
+    // At 128 columns and more, waves in their products go before waves of the other workgroup in their softmax
+    // (16 heads x 4096^2 all visible, bf16: 286 -> 269 us; capped 411 -> 378; slower at 64 columns)
+    constexpr bool kPrio = D >= 128;
+    int masked = 0, masked_next = 0;
     int st = stages.next(&masked), nx = st < 0 ? -1 : stages.next(&masked_next);
     if (st >= 0) {
         fill_k(st, Kb0, Db0);
@@ -371,7 +385,8 @@ __device__ __forceinline__ void score_forward(const ScoreParams& p) {
     if (tid == 0) *Special = 0;
     wait_loads();
     __syncthreads();
-    bool act = active(st);
+    if (st >= 0 && masked && vfill.template special<true>(Vb0)) *Special = 1;
+    int act = active(st);
     if (act) {
         qk(Kb0, st * SK);
         if (masked) hide(st * SK, Db0);
@@ -383,26 +398,26 @@ __device__ __forceinline__ void score_forward(const ScoreParams& p) {
         T* const k_next = P ? Kb0 : Kb1;
         T* const v_cur = P ? Vb1 : Vb0;
         T* const v_next = P ? Vb0 : Vb1;
-        bool masked_after = false;
+        int masked_after = 0;
         const int after = nx < 0 ? -1 : stages.next(&masked_after);
         if (after >= 0) fill_k(after, k_cur, P ? Db1 : Db0);
         if (nx >= 0) vfill(v_next, V, nx * SK, p.sk);
-        if (masked && tile_clean<T, LD, D, SK, 64 * NW>(v_cur, tid)) *Special = 1;
         if (act) {
-            if (!masked) pv_preload(v_cur);
+            pv_preload(v_cur);
             softmax();
-        }
-        if (masked) __syncthreads();
-        if (act) {
-            if (masked) pv_preload(v_cur);
+            if (kPrio) __builtin_amdgcn_s_setprio(1);
             pv(v_cur);
+            if (kPrio) __builtin_amdgcn_s_setprio(0);
         }
         act = active(nx);
         if (act) {
+            if (kPrio) __builtin_amdgcn_s_setprio(1);
             qk(k_next, nx * SK);
+            if (kPrio) __builtin_amdgcn_s_setprio(0);
             if (masked_next) hide(nx * SK, P ? Db0 : Db1);
         }
         wait_loads();
+        if (masked_next && vfill.template special<true>(v_next)) *Special = 1;
         __syncthreads();
         st = nx, masked = masked_next;
         nx = after, masked_next = masked_after;
@@ -492,28 +507,28 @@ __device__ __forceinline__ void score_delta(const ScoreParams& p) {
 }
 
 // The weight p = e^(z - lse) and the gradient of the raw score (without the scale) of four scores.
-template <typename T, bool MOD>
+template <typename T, int MOD>
 __device__ __forceinline__ void weigh(const ScoreParams& p, bool cap, f32x4 s, f32x4 dp, f32x4 lse2, f32x4 delta,
                                       float slope, float dist, f32x4* w, f32x4* ds) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
         float z, th = 0.0f;
-        if (MOD && cap) {
+        if (cap) {
             z = capped<T>(s[r], p.cap_in, p.cap_log2e, &th) - lse2[r];
         } else {
             z = __builtin_fmaf(s[r], p.scale_log2e, -lse2[r]);
         }
-        if (MOD && p.slopes) z = __builtin_fmaf(-slope, fabsf(dist - (float)r), z);
+        if (has_bias<MOD>(p)) z = __builtin_fmaf(-slope, fabsf(dist - (float)r), z);
         const float x = ops_exp2(z);
         float y = x * (dp[r] - delta[r]);
-        if (MOD && cap) y = __builtin_fmaf(-th * th, y, y);
+        if (cap) y = __builtin_fmaf(-th * th, y, y);
         (*w)[r] = x;
         (*ds)[r] = y;
     }
 }
 
 // dQ: query rows kept, keys walked.  Four waves of MT 16-row tiles; K and V tiles double-buffered, one barrier a stage.
-template <typename T, int D, int MT, int KG, bool MOD, bool VEC>
+template <typename T, int D, int MT, int KG, int MOD, bool VEC>
 __device__ __forceinline__ void score_dq(const ScoreParams& p) {
     using M = Mma<T>;
     using v8 = typename M::v8;
@@ -526,7 +541,7 @@ __device__ __forceinline__ void score_dq(const ScoreParams& p) {
     T* const Vb1 = lds_array<T, Fill::SIZE, 3>();
     int* const Db0 = lds_array<int, 64, 4>();
     int* const Db1 = lds_array<int, 64, 5>();
-    int* const Special = lds_array<int, 1, 6>();
+    int* const Special = lds_array<int, 3, 6>();   // met any; and the tiles of either buffer hold some
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, li = lane & 15;
@@ -540,9 +555,9 @@ __device__ __forceinline__ void score_dq(const ScoreParams& p) {
     const T* V = slice<T>(p.v, p.vs, w.b, w.hk);
     const bool docs = p.q_doc != nullptr;
     const int32_t* kdoc = docs ? p.k_doc + (int64_t)w.b * p.sk : nullptr;
-    const int prefix = p.prefix ? p.prefix[w.b] : 0;
-    const float slope = MOD && p.slopes ? p.slopes[h] * kLog2e : 0.0f;
-    const bool cap = MOD && p.cap_log2e != 0.0f;
+    const int prefix = p.prefix ? load_uniform(p.prefix + w.b) : 0;
+    const float slope = has_bias<MOD>(p) ? load_uniform(p.slopes + h) * kLog2e : 0.0f;
+    const bool cap = has_cap<MOD>(p);
 
     v8 qreg[MT][NDC], doreg[MT][NDC];
     int qd[MT], limit[MT];
@@ -579,17 +594,19 @@ __device__ __forceinline__ void score_dq(const ScoreParams& p) {
         vfill(v, V, st * SK, p.sk);
         if (docs && wave == 0 && lane < SK) fill_words(ids, kdoc + st * SK, p.sk - st * SK, lane);
     };
-    auto active = [&](int st) -> bool {
+    auto active = [&](int st) -> int {
         if (row0 >= p.sq) return false;
         const int k0 = st * SK + koff;
         return k0 < p.sk && (!p.causal || k0 <= p.q_start + row0 + 16 * MT - 1 || k0 < prefix);
     };
 
-    bool masked = false, masked_next = false;
+    int masked = 0, masked_next = 0;
     int st = stages.next(&masked);
-    if (tid == 0) *Special = 0;
+    if (tid < 3) Special[tid] = 0;
     if (st >= 0) fill(st, Kb0, Vb0, Db0);
     wait_loads();
+    __syncthreads();
+    if (masked && kfill.template special<false>(Kb0)) Special[1] = 1;
     __syncthreads();
     auto step = [&](auto parity) {
         constexpr int P = decltype(parity)::value;
@@ -599,7 +616,7 @@ __device__ __forceinline__ void score_dq(const ScoreParams& p) {
         const int nx = stages.next(&masked_next);
         if (nx >= 0) fill(nx, P ? Kb0 : Kb1, P ? Vb0 : Vb1, P ? Db0 : Db1);
         const int k0 = st * SK;
-        const bool act = active(st);
+        const int act = active(st), dirty = masked ? __builtin_amdgcn_readfirstlane(Special[1 + P]) : 0;
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
             v8 db[MT][1];
@@ -648,7 +665,7 @@ __device__ __forceinline__ void score_dq(const ScoreParams& p) {
                     }
                 }
             }
-            if (masked) {
+            if (dirty) {   // the row products took K as it is, the column products may not
                 __syncthreads();
                 if (tile_clean<T, LD, D, 32 * KG, 64 * NW>(Ks + 32 * i * LD, tid)) *Special = 1;
                 __syncthreads();
@@ -664,6 +681,8 @@ __device__ __forceinline__ void score_dq(const ScoreParams& p) {
             }
         }
         wait_loads();
+        if (nx >= 0 && masked_next && kfill.template special<false>(P ? Kb0 : Kb1)) Special[2 - P] = 1;
+        if (dirty && tid == 0) Special[1 + P] = 0;
         __syncthreads();
         st = nx, masked = masked_next;
     };
@@ -730,7 +749,7 @@ __device__ __forceinline__ void dkv_specials(const ScoreParams& p, Test test, in
 // dK and dV: key rows kept, the queries of every head of the group walked.  Four waves
 // of MT 16-row tiles; Q and dO tiles double-buffered, one barrier a stage.  A kv head's sums over its
 // query heads are formed here, in head order, or by score_dkv_sum where workgroups share them.
-template <typename T, int D, int MT, int KG, bool MOD, bool VEC>
+template <typename T, int D, int MT, int KG, int MOD, bool VEC>
 __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
     using M = Mma<T>;
     using v8 = typename M::v8;
@@ -743,7 +762,7 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
     T* const Ob1 = lds_array<T, Fill::SIZE, 3>();
     int* const Wb0 = lds_array<int, 192, 4>();   // of the stage's queries: lse2, delta, document
     int* const Wb1 = lds_array<int, 192, 5>();
-    int* const Special = lds_array<int, 1, 6>();
+    int* const Special = lds_array<int, 3, 6>();   // met any; and the tiles of either buffer hold some
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, li = lane & 15;
@@ -755,8 +774,8 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
     const T* K = slice<T>(p.k, p.ks, w.b, w.hk);
     const T* V = slice<T>(p.v, p.vs, w.b, w.hk);
     const bool docs = p.q_doc != nullptr;
-    const int prefix = p.prefix ? p.prefix[w.b] : 0;
-    const bool cap = MOD && p.cap_log2e != 0.0f;
+    const int prefix = p.prefix ? load_uniform(p.prefix + w.b) : 0;
+    const bool cap = has_cap<MOD>(p);
 
     v8 kreg[MT][NDC], vreg[MT][NDC];
     f32x4 dk[MT][NDB], dv[MT][NDB];
@@ -795,7 +814,7 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
     const Fill qfill(p.qs.s, p.d, wave, lane), ofill(p.dos.s, p.d, wave, lane);
     // the next (head, stage): the stages of one head of the group after the other
     int head = 0;
-    auto next = [&](bool* m) -> int {
+    auto next = [&](int* m) -> int {
         int s = stages.next(m);
         while (s < 0 && head + 1 < count && stages.count > 0) {
             ++head;
@@ -805,27 +824,38 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
         }
         return s;
     };
+    const T* const Q = slice<T>(p.q, p.qs, w.b, first);
+    const T* const dO = slice<T>(p.dout, p.dos, w.b, first);
+    const float* const lse2 = p.lse2 + ((int64_t)w.b * p.heads + first) * p.sq;
+    const int64_t to_delta = p.delta - p.lse2;
+    const int32_t* const qdoc = docs ? p.q_doc + (int64_t)w.b * p.sq : nullptr;
     auto fill = [&](int hq, int st, T* q, T* o, int* words) {
-        const int h = first + hq, q0 = st * SQ;
-        qfill(q, slice<T>(p.q, p.qs, w.b, h), q0, p.sq);
-        ofill(o, slice<T>(p.dout, p.dos, w.b, h), q0, p.sq);
-        const int64_t at = ((int64_t)w.b * p.heads + h) * p.sq + q0;
+        const int q0 = st * SQ;
+        qfill(q, Q + hq * p.qs.h, q0, p.sq);
+        ofill(o, dO + hq * p.dos.h, q0, p.sq);
         if (lane < SQ) {
-            if (wave == 0) fill_words(words, p.lse2 + at, p.sq - q0, lane);
-            if (wave == 1) fill_words(words + 64, p.delta + at, p.sq - q0, lane);
-            if (wave == 2 && docs) fill_words(words + 128, p.q_doc + (int64_t)w.b * p.sq + q0, p.sq - q0, lane);
+            const float* const at = lse2 + (int64_t)hq * p.sq + q0;
+            if (wave == 0) fill_words(words, at, p.sq - q0, lane);
+            if (wave == 1) fill_words(words + 64, at + to_delta, p.sq - q0, lane);
+            if (wave == 2 && docs) fill_words(words + 128, qdoc + q0, p.sq - q0, lane);
         }
     };
-    auto active = [&](int st) -> bool {
+    auto active = [&](int st) -> int {
         if (key0 >= p.sk) return false;
         return st * SQ + qoff < p.sq && (!p.causal || p.q_start + st * SQ + qoff + 32 * NCH - 1 >= key0 || key0 < prefix);
     };
 
-    bool masked = false, masked_next = false;
+    int masked = 0, masked_next = 0;
     int st = next(&masked), hq = head;
-    if (tid == 0) *Special = 0;
+    if (tid < 3) Special[tid] = 0;
     if (st >= 0) fill(hq, st, Qb0, Ob0, Wb0);
     wait_loads();
+    __syncthreads();
+    auto special = [&](T* q, T* o) {
+        const bool found = qfill.template special<false>(q);
+        return ofill.template special<false>(o) || found;
+    };
+    if (masked && special(Qb0, Ob0)) Special[1] = 1;
     __syncthreads();
     auto step = [&](auto parity) {
         constexpr int P = decltype(parity)::value;
@@ -836,8 +866,8 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
         const int nx = next(&masked_next), hnx = head;
         if (nx >= 0) fill(hnx, nx, P ? Qb0 : Qb1, P ? Ob0 : Ob1, P ? Wb0 : Wb1);
         const int q0 = st * SQ;
-        const bool act = active(st);
-        const float slope = MOD && p.slopes ? p.slopes[first + hq] * kLog2e : 0.0f;
+        const int act = active(st), dirty = masked ? __builtin_amdgcn_readfirstlane(Special[1 + P]) : 0;
+        const float slope = has_bias<MOD>(p) ? load_uniform(p.slopes + first + hq) * kLog2e : 0.0f;
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
             v8 pb[MT][1], db[MT][1];
@@ -890,7 +920,7 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
                     }
                 }
             }
-            if (masked) {
+            if (dirty) {
                 __syncthreads();
                 const bool bad = tile_clean<T, LD, D, 32 * KG, 64 * NW>(Qs + 32 * i * LD, tid);
                 if (tile_clean<T, LD, D, 32 * KG, 64 * NW>(Os + 32 * i * LD, tid) || bad) *Special = 1;
@@ -911,6 +941,8 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
             }
         }
         wait_loads();
+        if (nx >= 0 && masked_next && special(P ? Qb0 : Qb1, P ? Ob0 : Ob1)) Special[2 - P] = 1;
+        if (dirty && tid == 0) Special[1 + P] = 0;
         __syncthreads();
         st = nx, hq = hnx, masked = masked_next;
     };
@@ -1042,17 +1074,21 @@ SUM(256, true, )
 SUM(64, false, s)
 SUM(128, false, s)
 SUM(256, false, s)
-// plain scores, modified ones (m), any alignment (s); two groups of waves on a stage (k)
-#define KERNELS(F, D, MT, WAVES)                \
-    KERNEL(F, D, MT, 1, false, true, , WAVES)   \
-    KERNEL(F, D, MT, 1, true, true, m, WAVES)
-#define GROUPS(F, D, WAVES)                     \
-    KERNEL(F, D, 1, 2, false, true, k, WAVES)   \
-    KERNEL(F, D, 1, 2, true, true, km, WAVES)
+// plain scores, capped (c), with a bias (b) or both (cb); any alignment (s); two groups of waves on a stage (k)
+#define KERNELS(F, D, MT, WAVES)                      \
+    KERNEL(F, D, MT, 1, 0, true, , WAVES)             \
+    KERNEL(F, D, MT, 1, kCap, true, c, WAVES)         \
+    KERNEL(F, D, MT, 1, kBias, true, b, WAVES)        \
+    KERNEL(F, D, MT, 1, kCap | kBias, true, cb, WAVES)
+#define GROUPS(F, D, WAVES)                           \
+    KERNEL(F, D, 1, 2, 0, true, k, WAVES)             \
+    KERNEL(F, D, 1, 2, kCap, true, kc, WAVES)         \
+    KERNEL(F, D, 1, 2, kBias, true, kb, WAVES)        \
+    KERNEL(F, D, 1, 2, kCap | kBias, true, kcb, WAVES)
 #define SLOW(F, W64, W128, W256)                 \
-    KERNEL(F, 64, 1, 1, true, false, s, W64)     \
-    KERNEL(F, 128, 1, 1, true, false, s, W128)   \
-    KERNEL(F, 256, 1, 1, true, false, s, W256)
+    KERNEL(F, 64, 1, 1, kAny, false, s, W64)     \
+    KERNEL(F, 128, 1, 1, kAny, false, s, W128)   \
+    KERNEL(F, 256, 1, 1, kAny, false, s, W256)
 #define ALL(F, W64, W128, W256)  \
     KERNELS(F, 64, 1, W64)       \
     KERNELS(F, 128, 1, W128)     \
