@@ -137,8 +137,8 @@ struct RowSource {
         }
     }
     // The pages of rows [k0, k0 + ROWS) before `end`; returns whether one is bad.
-    static __device__ __forceinline__ bool look_up(const CachePages& c, int k0, int end, int (&pg)[GROUPS]) {
-        bool bad = false;
+    static __device__ __forceinline__ int look_up(const CachePages& c, int k0, int end, int (&pg)[GROUPS]) {
+        int bad = 0;
         const bool whole = !c.table || c.page_mask >= ROWS - 1;
 #pragma unroll
         for (int i = 0; i < GROUPS; ++i) {
@@ -181,7 +181,7 @@ struct RowsWork {
     int run, rb, b, hk;
     int runs;   // of the sequence
     int len, prefix, open, kbeg, kend, nrows, rfirst;
-    bool tree, docs;
+    int tree, docs;
 };
 
 // Keys that any query of sequence b sees.
@@ -317,7 +317,7 @@ __device__ __forceinline__ bool rows_see(const RowsParams& p, const RowsWork& w,
 }
 
 // MT 16-row tiles of a wave: their queries, and the running softmax over KB 16-key blocks at a time.
-template <typename T, int D, int MT, int KB, bool MOD, bool VEC>
+template <typename T, int D, int MT, int KB, int MOD, bool VEC>
 struct RowTiles {
     using M = Mma<T>;
     using S = Swizzled<T, D>;
@@ -334,7 +334,7 @@ struct RowTiles {
 
     __device__ __forceinline__ void init(const RowsParams& p, const RowsWork& w, int rfirst, int lane) {
         g = lane >> 4, li = lane & 15;
-        c = MOD ? 1.0f : p.scale_log2e;
+        c = MOD != 0 ? 1.0f : p.scale_log2e;
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
             const int r = rfirst + 16 * t + li;
@@ -347,7 +347,7 @@ struct RowTiles {
                 q[t][dc] = global_row<T, VEC>(from, p.qs.s, token[t], real ? p.n : 0, 32 * dc + 8 * g, p.d);
             pos[t] = !w.tree ? p.q_start + token[t] : p.pos ? p.pos[w.b * p.n + token[t]] : w.len + token[t];
             qd[t] = w.docs ? p.q_doc[(int64_t)w.b * p.n + token[t]] : 0;
-            slope[t] = MOD && p.slopes ? p.slopes[h] * kLog2e : 0.0f;
+            slope[t] = has_bias<MOD>(p) ? p.slopes[h] * kLog2e : 0.0f;
             word[t] = 0;
             if (w.tree)
                 word[t] = p.mask ? p.mask[((p.mask_shared ? 0 : (int64_t)w.b * p.n) + token[t]) * p.mask_words]
@@ -365,7 +365,7 @@ struct RowTiles {
         for (int t = 0; t < MT; ++t)
 #pragma unroll
             for (int b = 0; b < KB; ++b) {
-                const float x = MOD ? 0.0f : -ref[t];
+                const float x = MOD != 0 ? 0.0f : -ref[t];
                 s[t][b] = (f32x4){x, x, x, x};
             }
 #pragma unroll
@@ -378,13 +378,13 @@ struct RowTiles {
             }
             if (sizeof(T) == 4 || dc % 2 == 1) __builtin_amdgcn_sched_barrier(0);
         }
-        if constexpr (MOD) {
+        if constexpr (MOD != 0) {
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
                 const float dist = (float)(pos[t] - k0 - 4 * g);
 #pragma unroll
                 for (int b = 0; b < KB; ++b) {
-                    if (p.cap_log2e != 0.0f) {
+                    if (has_cap<MOD>(p)) {
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
                             float th;
@@ -394,7 +394,7 @@ struct RowTiles {
 #pragma unroll
                         for (int r = 0; r < 4; ++r) s[t][b][r] = __builtin_fmaf(s[t][b][r], p.scale_log2e, -ref[t]);
                     }
-                    if (p.slopes) {
+                    if (has_bias<MOD>(p)) {
                         f32x4 x;
 #pragma unroll
                         for (int r = 0; r < 4; ++r) x[r] = dist - (float)(16 * b + r);
@@ -444,7 +444,7 @@ struct RowTiles {
         }
     }
     // Bits of the keys that exist: before the run's end, in good pages (one lane a key).
-    __device__ __forceinline__ uint64_t keys_there(const RowsParams& p, const RowsWork& w, int k0, bool badpage) const {
+    __device__ __forceinline__ uint64_t keys_there(const RowsParams& p, const RowsWork& w, int k0, int badpage) const {
         const int lane = 16 * g + li, key = k0 + lane;
         if (!badpage) return w.kend - k0 >= 64 ? ~0ull : (1ull << (w.kend - k0)) - 1;
         const CachePages pages = rows_pages(p, w.b);
@@ -594,7 +594,7 @@ __device__ __forceinline__ void wait_vmcnt() {
 // ---------------------------------------------------------------------------
 // Up to 16 MT rows, a wave 32-key blocks of its own.
 // ---------------------------------------------------------------------------
-template <typename T, int D, int MT, bool MOD, bool VEC>
+template <typename T, int D, int MT, int MOD, bool VEC>
 __device__ __forceinline__ void rows_stream(const RowsParams& p) {
     constexpr int NW = kStreamWaves<D * (int)sizeof(T)>, SK = 32, TILE = SK * D;
     using R = RowTiles<T, D, MT, 2, MOD, VEC>;
@@ -622,7 +622,7 @@ __device__ __forceinline__ void rows_stream(const RowsParams& p) {
     R x;
     // pages of the block to fill next are looked up a block ahead
     int page[2];
-    bool bad0, bad1, bad2;
+    int bad0, bad1, bad2;
     auto look_up = [&](int blk) {
         const int k0 = k_first + blk * SK * NW;
         return Src::look_up(pages, k0, blk < nblk ? w.kend : k0, page);
@@ -649,11 +649,11 @@ __device__ __forceinline__ void rows_stream(const RowsParams& p) {
         T* const Ks = kb + wave * TILE;
         T* const Vs = vb + wave * TILE;
         const int k0 = k_first + i * SK * NW;
-        const bool bad = bad0;
+        const int bad = bad0;
         bad0 = bad1;
         bad1 = bad2;
         wait_vmcnt<3 * RUNS>();
-        const bool masked = bad || k0 + SK > min(w.open, w.kend);
+        const int masked = bad || k0 + SK > min(w.open, w.kend);
         x.scores(p, w, Ks, k0, masked, bad);
         reread();
         fill(ksrc, kb, i + 2);
@@ -723,7 +723,7 @@ __device__ __forceinline__ void rows_stream(const RowsParams& p) {
 // ---------------------------------------------------------------------------
 // Many rows: the waves share the keys.
 // ---------------------------------------------------------------------------
-template <typename T, int D, int MT, bool MOD, bool VEC>
+template <typename T, int D, int MT, int MOD, bool VEC>
 __device__ __forceinline__ void rows_shared(const RowsParams& p) {
     constexpr int NW = 8, SK = sizeof(T) == 4 || D > 128 ? 32 : 64, TILE = SK * D, KB = SK / 16;
     constexpr int RING = TILE * (int)sizeof(T) > 16384 ? 2 : 3;   // stages in LDS
@@ -747,18 +747,18 @@ __device__ __forceinline__ void rows_shared(const RowsParams& p) {
     const Src ksrc(K, p.ks.s, p.ks.b, p.d, wave, lane), vsrc(V, p.vs.s, p.vs.b, p.d, wave, lane);
     const int nst = (w.kend - w.kbeg + SK - 1) / SK;
     const int rfirst = w.rfirst + 16 * MT * wave;
-    const bool act = rfirst < w.nrows;
+    const int act = rfirst < w.nrows;
 
     // whether the stages on their way have bad pages; those of the stage to fill next are looked up a stage ahead
-    bool bad_now = false, bad_1 = false, bad_2 = false, bad_next = false;
+    int bad_now = 0, bad_1 = 0, bad_2 = 0, bad_next = 0;
     int page[SK / 16];
     auto look_up = [&](int st) {
         const int k0 = w.kbeg + st * SK;
         if (VEC) bad_next = Src::look_up(pages, k0, st < nst ? w.kend : k0, page);
     };
-    auto fill = [&](int st, T* k, T* v) -> bool {
+    auto fill = [&](int st, T* k, T* v) -> int {
         const int k0 = w.kbeg + st * SK;
-        const bool bad = bad_next;
+        const int bad = bad_next;
         if constexpr (VEC) {
             const int end = st < nst ? w.kend : k0;
             ksrc.fill(k, k0, end, page, pages, wave);
@@ -791,12 +791,12 @@ __device__ __forceinline__ void rows_shared(const RowsParams& p) {
     if (RING > 2) bad_1 = fill(1, K1, V1);
     auto step = [&](int st, T* k, T* v, T* kn, T* vn) {
         arrive(std::integral_constant<int, (RING - 2) * 2 * Src::NI>{});
-        const bool filled = fill(st + RING - 1, kn, vn);
+        const int filled = fill(st + RING - 1, kn, vn);
         if (RING > 2) bad_2 = filled;
         else bad_1 = filled;
         const int k0 = w.kbeg + st * SK;
-        const bool bad = VEC ? bad_now : bad_any != 0;
-        const bool masked = bad || k0 + SK > min(w.open, w.kend);
+        const int bad = VEC ? bad_now : __builtin_amdgcn_readfirstlane(bad_any);
+        const int masked = bad || k0 + SK > min(w.open, w.kend);
         if (act) {
             x.scores(p, w, k, k0, masked, bad);
             x.softmax();
@@ -888,20 +888,20 @@ __device__ __forceinline__ void rows_merge(const RowsParams& p) {
     extern "C" __global__ __launch_bounds__(THREADS, WAVES) void PASTE(F, OPS_NAME, _d##D##_t##MT, TAG)(RowsParams p) { \
         BODY<OPS_T, D, MT, MOD, VEC>(p);                                                                       \
     }
-// plain scores, modified ones (m), and any alignment and page size (s)
-#define STREAM_THREADS(D) (64 * kStreamWaves<D * (int)sizeof(OPS_T)>)
-#define STREAM(D, MT, WAVES)                                                              \
-    KERNEL(fa_rows_stream_, rows_stream, D, MT, false, true, , STREAM_THREADS(D), WAVES)  \
-    KERNEL(fa_rows_stream_, rows_stream, D, MT, true, true, m, STREAM_THREADS(D), WAVES)
-#define SHARED(D, MT, WAVES)                                                   \
-    KERNEL(fa_rows_shared_, rows_shared, D, MT, false, true, , 512, WAVES)     \
-    KERNEL(fa_rows_shared_, rows_shared, D, MT, true, true, m, 512, WAVES)
+// plain scores, capped (c), with a bias (b) or both (cb); any alignment and page size (s)
+#define KINDS(F, BODY, D, MT, THREADS, WAVES)                            \
+    KERNEL(F, BODY, D, MT, 0, true, , THREADS, WAVES)                    \
+    KERNEL(F, BODY, D, MT, kCap, true, c, THREADS, WAVES)                \
+    KERNEL(F, BODY, D, MT, kBias, true, b, THREADS, WAVES)               \
+    KERNEL(F, BODY, D, MT, kCap | kBias, true, cb, THREADS, WAVES)
+#define STREAM(D, MT, WAVES) KINDS(fa_rows_stream_, rows_stream, D, MT, (64 * kStreamWaves<D * (int)sizeof(OPS_T)>), WAVES)
+#define SHARED(D, MT, WAVES) KINDS(fa_rows_shared_, rows_shared, D, MT, 512, WAVES)
 #define MERGE(D, VEC, WIDE, TAG)                                                                                  \
     extern "C" __global__ __launch_bounds__(256) void PASTE(fa_rows_merge_, OPS_NAME, _d##D, TAG)(RowsParams p) { \
         rows_merge<OPS_T, D, VEC, WIDE>(p);                                                                       \
     }
 #define COMMON(D)                                                                                               \
-    KERNEL(fa_rows_shared_, rows_shared, D, 1, true, false, s, 512, 2)                                          \
+    KERNEL(fa_rows_shared_, rows_shared, D, 1, kAny, false, s, 512, 2)                                          \
     MERGE(D, true, false, )                                                                                     \
     MERGE(D, true, true, w)                                                                                     \
     MERGE(D, false, true, s)

@@ -30,6 +30,17 @@ constexpr float kLn2 = 0.693147180559945309f;
 // maximum of a row by this much (log2 units) before the sums are rescaled.
 constexpr float kLazy = 8.0f;
 
+// What happens to scores, fixed for a kernel: bits kCap and kBias, or kAny: looked up in the parameters.
+constexpr int kCap = 1, kBias = 2, kAny = 4;
+template <int MOD, typename P>
+__device__ __forceinline__ bool has_cap(const P& p) {
+    return MOD == kAny ? p.cap_log2e != 0.0f : (MOD & kCap) != 0;
+}
+template <int MOD, typename P>
+__device__ __forceinline__ bool has_bias(const P& p) {
+    return MOD == kAny ? p.slopes != nullptr : (MOD & kBias) != 0;
+}
+
 // The kernel's parameters, read again where this stands: code that runs seldom (masked tiles, the
 // stores at the end) uses these, so that what only it needs does not occupy scalar
 // registers in the main loop.

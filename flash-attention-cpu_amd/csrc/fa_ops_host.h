@@ -294,7 +294,7 @@ int run_rows(int dev, hipStream_t stream, int dtype, int D, bool vec, RowsParams
     }
     char name[64];
     std::snprintf(name, sizeof(name), "fa_rows_%s_%s_d%d_t%d%s", plan.stream ? "stream" : "shared", dtype_name(dtype), D,
-                  plan.mt, !vec ? "s" : p->slopes || p->cap_log2e != 0.0f ? "m" : "");
+                  plan.mt, !vec ? "s" : p->cap_log2e != 0.0f ? (p->slopes ? "cb" : "c") : p->slopes ? "b" : "");
     rc = ops_launch(dev, module, name, grid, plan.threads, p, stream);
     if (rc == FA_OK && plan.floats) {
         // eight runs a sequence or more: a workgroup a row

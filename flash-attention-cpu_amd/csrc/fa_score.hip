@@ -17,17 +17,6 @@
 
 #include "fa_ops_common.h"
 
-// What happens to scores, fixed for a kernel: bits kCap and kBias, or kAny: looked up in the parameters.
-constexpr int kCap = 1, kBias = 2, kAny = 4;
-template <int MOD>
-__device__ __forceinline__ bool has_cap(const ScoreParams& p) {
-    return MOD == kAny ? p.cap_log2e != 0.0f : (MOD & kCap) != 0;
-}
-template <int MOD>
-__device__ __forceinline__ bool has_bias(const ScoreParams& p) {
-    return MOD == kAny ? p.slopes != nullptr : (MOD & kBias) != 0;
-}
-
 template <typename T>
 __device__ __forceinline__ const T* slice(const void* base, OpsStrides st, int b, int h) {
     return reinterpret_cast<const T*>(base) + b * st.b + h * st.h;
