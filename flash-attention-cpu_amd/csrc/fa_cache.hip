@@ -31,28 +31,35 @@ struct Swizzled {
     static __device__ __forceinline__ int at(int row, int col) {   // col: a multiple of E or inside its chunk
         return row * D + (((col / E) ^ (row % CM)) * E) + col % E;
     }
+    // An operand's chunk numbers are those of its first column block, exclusive-or the block's own (a
+    // multiple of what the lanes add), so its place is base ^ block; row0 (a multiple of 16) only adds whole rows.
     static __device__ __forceinline__ v8 row_op(const T* tile, int row0, int dc, int g, int li) {
-        const int r = row0 + li;
+        const int base = at(li, 8 * g);
+        const T* const t = tile + row0 * D;
         if constexpr (sizeof(T) == 2) {
-            return *reinterpret_cast<const v8*>(tile + at(r, 32 * dc + 8 * g));
+            return *reinterpret_cast<const v8*>(t + (base ^ (32 * dc)));
         } else {
-            const f32x4 a = *reinterpret_cast<const f32x4*>(tile + at(r, 32 * dc + 8 * g));
-            const f32x4 b = *reinterpret_cast<const f32x4*>(tile + at(r, 32 * dc + 8 * g + 4));
+            const f32x4 a = *reinterpret_cast<const f32x4*>(t + (base ^ (32 * dc)));
+            const f32x4 b = *reinterpret_cast<const f32x4*>(t + (base ^ (32 * dc + 4)));
             return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
         }
     }
     static __device__ __forceinline__ v8 col_op(const T* tile, int row0, int col0, int g, int li) {
+        const T* const t = tile + row0 * D;
         if constexpr (sizeof(T) == 2) {
             typedef __attribute__((address_space(3))) s16x4* lds4;
-            const int r = row0 + 4 * g + (li >> 2);
-            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4) const_cast<T*>(tile + at(r, col0 + 4 * (li & 3))));
-            const s16x4 hi =
-                __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4) const_cast<T*>(tile + at(r + 16, col0 + 4 * (li & 3))));
+            const int place = at(4 * g + (li >> 2), 4 * (li & 3)) ^ col0;
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4) const_cast<T*>(t + place));
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4) const_cast<T*>(t + 16 * D + place));
             return __builtin_bit_cast(v8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
         } else {
             v8 v;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = tile[at(row0 + (e < 4 ? 0 : 12) + 4 * g + e, col0 + li)];
+            for (int e = 0; e < 4; ++e) {
+                const int place = at(4 * g + e, li) ^ col0;
+                v[e] = t[place];
+                v[4 + e] = t[16 * D + place];
+            }
             return v;
         }
     }
