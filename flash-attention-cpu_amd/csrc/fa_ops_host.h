@@ -538,6 +538,14 @@ int fa_score_backward(void* stream_, const fa_score_config* c, const void* q, co
         rc = ops_launch(dev, of_type(kScoreModule, c->dtype), name, dgrid, 256, &p, stream);
     }
     const char* mod = score_tag(*c, vec);
+    // 16-bit types: the dQ kernel also corrects delta, which dK takes from it
+    if (rc == FA_OK && sq > 0 && (dq || (dk && c->dtype != FA_DTYPE_F32))) {
+        ScoreTiles tiles = score_tiles(*c, D, vec, sq, c->batch * c->heads, g_dev[dev].num_cus);
+        if (D == 128 && tiles.mt == 2) tiles = {1, 1, 64, ""};   // two tiles' Q, dO and sums leave one wave a SIMD
+        p.nqb = static_cast<int>((sq + tiles.rows - 1) / tiles.rows);
+        std::snprintf(name, sizeof(name), "fa_score_dq_%s_d%d_t%d%s%s", dtype_name(c->dtype), D, tiles.mt, tiles.tag, mod);
+        rc = ops_launch(dev, of_type(kScoreModule, c->dtype), name, c->batch * c->heads * p.nqb, 256, &p, stream);
+    }
     if (rc == FA_OK && (dk || dv)) {
         p.nqb = static_cast<int>(dkv.blocks);
         p.splits = dkv.splits;
@@ -550,12 +558,6 @@ int fa_score_backward(void* stream_, const fa_score_config* c, const void* q, co
             const size_t threads = c->batch * c->kv_heads * sk * (D / 4);
             rc = ops_launch(dev, of_type(kScoreModule, c->dtype), name, (threads + 255) / 256, 256, &p, stream);
         }
-    }
-    if (rc == FA_OK && dq) {
-        const ScoreTiles tiles = score_tiles(*c, D, vec, sq, c->batch * c->heads, g_dev[dev].num_cus);
-        p.nqb = static_cast<int>((sq + tiles.rows - 1) / tiles.rows);
-        std::snprintf(name, sizeof(name), "fa_score_dq_%s_d%d_t%d%s%s", dtype_name(c->dtype), D, tiles.mt, tiles.tag, mod);
-        rc = ops_launch(dev, of_type(kScoreModule, c->dtype), name, c->batch * c->heads * p.nqb, 256, &p, stream);
     }
     return ws.done(stream, rc);
 }

@@ -495,10 +495,11 @@ __device__ __forceinline__ void score_delta(const ScoreParams& p) {
     }
 }
 
-// The weight p = e^(z - lse) and the gradient of the raw score (without the scale) of four scores.
+// Of four scores: the weights p = e^(z - lse), the gradients y = p (dP - delta) of the modified scores z, and
+// what these have to be multiplied by for the raw ones (1 - tanh^2; 1 without a cap).
 template <typename T, int MOD>
 __device__ __forceinline__ void weigh(const ScoreParams& p, bool cap, f32x4 s, f32x4 dp, f32x4 lse2, f32x4 delta,
-                                      float slope, float dist, f32x4* w, f32x4* ds) {
+                                      float slope, float dist, f32x4* w, f32x4* y, f32x4* f) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
         float z, th = 0.0f;
@@ -509,18 +510,26 @@ __device__ __forceinline__ void weigh(const ScoreParams& p, bool cap, f32x4 s, f
         }
         if (has_bias<MOD>(p)) z = __builtin_fmaf(-slope, fabsf(dist - (float)r), z);
         const float x = ops_exp2(z);
-        float y = x * (dp[r] - delta[r]);
-        if (cap) y = __builtin_fmaf(-th * th, y, y);
         (*w)[r] = x;
-        (*ds)[r] = y;
+        (*y)[r] = x * (dp[r] - delta[r]);
+        (*f)[r] = cap ? __builtin_fmaf(-th, th, 1.0f) : 1.0f;
     }
 }
 
 // dQ: query rows kept, keys walked.  Four waves of MT 16-row tiles; K and V tiles double-buffered, one barrier a stage.
+//
+// 16-bit types: delta = dO . O comes from the rounded O, and an error of delta is common to all keys of a row, so
+// it does not average out: it was the largest error of dQ and dK (bf16, 2 x 4096 tokens, documents, capped scores:
+// 3.3e-3 relative, of which 1.7e-3 is the rounding of the results; 2.4e-3 now).  But sum_j p (dP - delta) is just
+// that error e.  It is summed on the way, as is sum_j p K_j (its operands are in registers anyway); dQ is corrected
+// by -e sum_j p K_j, and delta + e left for the dK / dV kernel, which runs after this one.  The third product takes
+// the kernel from 1089 to 764 TF/s (two products counted; 4096^2, 16 heads of 128 columns), the whole backward pass
+// of that shape from 1036 to 1171 us, and that of the documents above from 497 to 507.
 template <typename T, int D, int MT, int KG, int MOD, bool VEC>
 __device__ __forceinline__ void score_dq(const ScoreParams& p) {
     using M = Mma<T>;
     using v8 = typename M::v8;
+    constexpr bool kRefine = sizeof(T) == 2;
     constexpr int NW = 4, NR = NW / KG, SK = kStageRows<T, D, KG>, BQ = 16 * MT * NR;
     constexpr int NCH = SK / 32 / KG, NDC = D / 32, NDB = D / 16, LD = D + kPad<T>;
     using Fill = TileFill<T, D, SK, NW, VEC>;
@@ -550,8 +559,8 @@ __device__ __forceinline__ void score_dq(const ScoreParams& p) {
 
     v8 qreg[MT][NDC], doreg[MT][NDC];
     int qd[MT], limit[MT];
-    f32x4 dq[MT][NDB];
-    float lse2[MT], delta[MT];
+    f32x4 dq[MT][NDB], pk[MT][kRefine ? NDB : 1];
+    float lse2[MT], delta[MT], err[MT];
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
         const int row = row0 + 16 * t + li;
@@ -566,7 +575,11 @@ __device__ __forceinline__ void score_dq(const ScoreParams& p) {
         delta[t] = row < p.sq ? p.delta[at] : 0.0f;
         limit[t] = (docs && qd[t] < 0) || lse2[t] == -OPS_NEG_INF ? 0 : min(p.sk, key_limit(p, prefix, p.q_start + row));
 #pragma unroll
-        for (int j = 0; j < NDB; ++j) dq[t][j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+        for (int j = 0; j < NDB; ++j) {
+            dq[t][j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+            if (kRefine) pk[t][j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        err[t] = 0.0f;
     }
     const int q1 = min(q0 + BQ, p.sq);
     DocRange qr = {};
@@ -608,7 +621,7 @@ __device__ __forceinline__ void score_dq(const ScoreParams& p) {
         const int act = active(st), dirty = masked ? __builtin_amdgcn_readfirstlane(Special[1 + P]) : 0;
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
-            v8 db[MT][1];
+            v8 db[MT], pb[MT];
             if (act) {
                 f32x4 s[MT][2], dp[MT][2];
 #pragma unroll
@@ -634,23 +647,29 @@ __device__ __forceinline__ void score_dq(const ScoreParams& p) {
                     const int pos = p.q_start + row0 + 16 * t + li;
 #pragma unroll
                     for (int b = 0; b < 2; ++b) {
-                        f32x4 x, ds;
+                        f32x4 x, y, f;
                         const int key = k0 + koff + 32 * i + 16 * b + 4 * g;
                         weigh<T, MOD>(p, cap, s[t][b], dp[t][b], (f32x4){lse2[t], lse2[t], lse2[t], lse2[t]},
-                                      (f32x4){delta[t], delta[t], delta[t], delta[t]}, slope, (float)(pos - key), &x, &ds);
+                                      (f32x4){delta[t], delta[t], delta[t], delta[t]}, slope, (float)(pos - key), &x, &y, &f);
                         if (masked) {
                             if (docs) {
                                 const i32x4 kd = *reinterpret_cast<const i32x4*>(ids + koff + 32 * i + 16 * b + 4 * g);
 #pragma unroll
                                 for (int r = 0; r < 4; ++r)
-                                    if (kd[r] != qd[t]) ds[r] = 0.0f;
+                                    if (kd[r] != qd[t]) x[r] = y[r] = 0.0f;
                             }
 #pragma unroll
                             for (int r = 0; r < 4; ++r)
-                                if (key + r >= limit[t]) ds[r] = 0.0f;
+                                if (key + r >= limit[t]) x[r] = y[r] = 0.0f;
                         }
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) db[t][0][4 * b + r] = T(ds[r]);
+                        for (int r = 0; r < 4; ++r) {
+                            db[t][4 * b + r] = T(y[r] * f[r]);
+                            if (kRefine) {
+                                pb[t][4 * b + r] = T(x[r] * f[r]);
+                                err[t] += y[r];
+                            }
+                        }
                     }
                 }
             }
@@ -664,7 +683,10 @@ __device__ __forceinline__ void score_dq(const ScoreParams& p) {
                 for (int j = 0; j < NDB; ++j) {
                     const v8 a = col_op<T, LD>(Ks, koff + 32 * i, 16 * j, g, li);
 #pragma unroll
-                    for (int t = 0; t < MT; ++t) dq[t][j] = M::mma(a, db[t][0], dq[t][j]);
+                    for (int t = 0; t < MT; ++t) {
+                        dq[t][j] = M::mma(a, db[t], dq[t][j]);
+                        if (kRefine) pk[t][j] = M::mma(a, pb[t], pk[t][j]);
+                    }
                     if (j % 4 == 3) __builtin_amdgcn_sched_barrier(0);
                 }
             }
@@ -684,15 +706,37 @@ __device__ __forceinline__ void score_dq(const ScoreParams& p) {
     if constexpr (KG > 1) {
         static_assert(MT == 1 && KG == 2 && NCH == 1 && NR * NDB * 64 * 16 <= Fill::SIZE * (int)sizeof(T), "sums fit a tile");
         f32x4* const sums = reinterpret_cast<f32x4*>(Kb0) + wave % NR * NDB * 64;
+        f32x4* const psums = reinterpret_cast<f32x4*>(Vb0) + wave % NR * NDB * 64;
+        float* const errs = reinterpret_cast<float*>(Kb1) + wave % NR * 64;
         if (kg == 1) {
 #pragma unroll
-            for (int j = 0; j < NDB; ++j) sums[j * 64 + lane] = dq[0][j];
+            for (int j = 0; j < NDB; ++j) {
+                sums[j * 64 + lane] = dq[0][j];
+                if (kRefine) psums[j * 64 + lane] = pk[0][j];
+            }
+            if (kRefine) errs[lane] = err[0];
         }
         __syncthreads();
         if (kg == 1) return;
 #pragma unroll
-        for (int j = 0; j < NDB; ++j) dq[0][j] += sums[j * 64 + lane];
+        for (int j = 0; j < NDB; ++j) {
+            dq[0][j] += sums[j * 64 + lane];
+            if (kRefine) pk[0][j] += psums[j * 64 + lane];
+        }
+        if (kRefine) err[0] += errs[lane];
     }
+    if constexpr (kRefine) {
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            const int row = row0 + 16 * t + li;
+            const float e = row4_sum(err[t]);
+            if (row < lp.sq && g == 0)
+                lp.delta[((int64_t)w.b * lp.heads + h) * lp.sq + row] = delta[t] + e;
+#pragma unroll
+            for (int j = 0; j < NDB; ++j) dq[t][j] -= pk[t][j] * e;
+        }
+    }
+    if (!lp.dq) return;
     T* out = slice<T>(lp.dq, lp.dqs, w.b, h);
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
@@ -888,8 +932,8 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
 #pragma unroll
                     for (int t = 0; t < MT; ++t) {
                         const int key = key0 + 16 * t + li;
-                        f32x4 x, ds;
-                        weigh<T, MOD>(p, cap, s[t][b], dp[t][b], lse2, delta, slope, (float)(key - pos), &x, &ds);
+                        f32x4 x, ds, f;
+                        weigh<T, MOD>(p, cap, s[t][b], dp[t][b], lse2, delta, slope, (float)(key - pos), &x, &ds, &f);
                         if (masked) {
                             if (docs) {
                                 const i32x4 qd = *reinterpret_cast<const i32x4*>(words + 128 + at);
@@ -904,7 +948,7 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
                             pb[t][0][4 * b + r] = T(x[r]);
-                            db[t][0][4 * b + r] = T(ds[r]);
+                            db[t][0][4 * b + r] = T(ds[r] * f[r]);
                         }
                     }
                 }
@@ -1094,7 +1138,6 @@ ALL(dkv, 2, 2, 1)
 KERNELS(forward, 64, 2, 2)
 KERNELS(forward, 128, 2, 2)
 KERNELS(dq, 64, 2, 2)
-KERNELS(dq, 128, 2, 2)
 KERNELS(dkv, 64, 2, 2)
 #else
 ALL(forward, 2, 2, 1)
