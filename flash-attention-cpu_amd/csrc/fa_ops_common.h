@@ -189,6 +189,17 @@ __device__ __forceinline__ float capped(float x, float cap_in, float cap_log2e, 
     return cap_log2e * *t;
 }
 
+// The same less ref, where the tanh itself is not wanted.
+template <typename T>
+__device__ __forceinline__ float capped_over(float x, float cap_in, float cap_log2e, float ref) {
+    if constexpr (sizeof(T) == 2) {
+        return __builtin_fmaf(-2.0f * cap_log2e, __builtin_amdgcn_rcpf(ops_exp2(x * cap_in) + 1.0f), cap_log2e - ref);
+    } else {
+        float t;
+        return capped<T>(x, cap_in, cap_log2e, &t) - ref;
+    }
+}
+
 __device__ __forceinline__ bool not_finite(float x) {
     return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u;
 }

@@ -192,8 +192,9 @@ struct ScoreTiles {
 };
 ScoreTiles score_tiles(const fa_score_config& c, int D, bool vec, size_t rows, size_t slices, int num_cus) {
     const size_t cus = static_cast<size_t>(num_cus), blocks = (rows + 63) / 64 * slices;
-    // causal workgroups differ in length, so that a single round of them ends late
-    if (vec && c.dtype != FA_DTYPE_F32 && D <= 128 && (rows + 127) / 128 * slices >= (c.causal ? 4 : 2) * cus)
+    // causal workgroups differ in length, so that a single round of them ends late (2048^2, d128: 32 heads 60 us
+    // with one tile a wave, 70 with two; 48 heads 86 and 73)
+    if (vec && c.dtype != FA_DTYPE_F32 && D <= 128 && (rows + 127) / 128 * slices >= (c.causal ? 3 : 2) * cus)
         return {2, 1, 128, ""};
     // measured (bf16, causal): 16 x 1024^2 d64 (256 blocks) 15.9 us against 18.7, 32 x 1024^2 (512) 19.3 against 19.6,
     // 32 x 1024^2 d128 all visible (512) 38.2 against 27.2
@@ -346,14 +347,37 @@ void fill_score(const fa_score_config& c, const ScoreScale& sc, ScoreParams* p) 
     p->cap_log2e = sc.cap_log2e;
 }
 
-int launch_doc_ranges(int dev, OpsModule module, hipStream_t stream, ScoreParams* p, int32_t* ws) {
-    const size_t tiles = static_cast<size_t>(p->batch) * (doc_tiles(p->sq) + doc_tiles(p->sk));
-    p->q_rng = ws;
-    p->k_rng = ws + 2 * static_cast<size_t>(p->batch) * doc_tiles(p->sq);
-    return ops_launch(dev, module, "fa_score_doc_ranges", (tiles + 3) / 4, 256, p, stream);
+// Tables of the documents: ranges of the tiles, and the order of the blocks (of q_rows queries and k_rows keys; 0:
+// that side's is not needed).  Order where the workgroups of a side are more than run at once.
+struct DocPlan {
+    bool q_order, k_order;
+    size_t q_blocks, k_blocks, bytes;
+};
+DocPlan plan_docs(const fa_score_config& c, size_t q_rows, size_t q_slices, size_t k_rows, size_t k_slices, int num_cus) {
+    DocPlan r{};
+    if (!c.q_doc) return r;
+    const size_t qt = c.batch * doc_tiles(c.seq_len_q), kt = c.batch * doc_tiles(c.seq_len_k);
+    r.q_blocks = q_rows ? c.batch * ((c.seq_len_q + q_rows - 1) / q_rows) : 0;
+    r.k_blocks = k_rows ? c.batch * ((c.seq_len_k + k_rows - 1) / k_rows) : 0;
+    const size_t fits = 2 * static_cast<size_t>(num_cus);
+    r.q_order = r.q_blocks <= kOrderBlocks && kt <= kOrderTiles && r.q_blocks * q_slices > fits;
+    r.k_order = r.k_blocks <= kOrderBlocks && qt <= kOrderTiles && r.k_blocks * k_slices > fits;
+    r.bytes = sizeof(int32_t) * (2 * (qt + kt) + r.q_blocks + r.k_blocks);
+    return r;
 }
-size_t doc_range_bytes(const fa_score_config& c) {
-    return c.q_doc ? 2 * sizeof(int32_t) * c.batch * (doc_tiles(c.seq_len_q) + doc_tiles(c.seq_len_k)) : 0;
+int launch_docs(int dev, OpsModule module, hipStream_t stream, const DocPlan& plan, size_t q_rows, size_t k_rows,
+                ScoreParams* p, int32_t* ws) {
+    const size_t qt = p->batch * doc_tiles(p->sq), kt = p->batch * doc_tiles(p->sk);
+    p->q_rng = ws;
+    p->k_rng = ws + 2 * qt;
+    int rc = ops_launch(dev, module, "fa_score_doc_ranges", (qt + kt + 3) / 4, 256, p, stream);
+    int32_t* const q_order = ws + 2 * (qt + kt);
+    if (rc != FA_OK || (!plan.q_order && !plan.k_order)) return rc;
+    p->q_order = plan.q_order ? q_order : nullptr;
+    p->k_order = plan.k_order ? q_order + plan.q_blocks : nullptr;
+    p->q_rows = static_cast<int>(q_rows);
+    p->k_rows = static_cast<int>(k_rows);
+    return ops_launch(dev, module, "fa_score_doc_order", 2, 1024, p, stream);
 }
 
 int check_cache(const fa_kv_cache* c, OpsLayout* k, OpsLayout* v, size_t* capacity) {
@@ -473,8 +497,9 @@ int fa_score_forward(void* stream_, const fa_score_config* c, const void* q, con
     p.nqb = static_cast<int>((c->seq_len_q + tiles.rows - 1) / tiles.rows);
     OpsWorkspace ws;
     if (c->q_doc) {
-        if ((rc = ws.get(dev, stream, doc_range_bytes(*c))) != FA_OK) return rc;
-        rc = launch_doc_ranges(dev, of_type(kScoreModule, c->dtype), stream, &p, static_cast<int32_t*>(ws.ptr));
+        const DocPlan docs = plan_docs(*c, tiles.rows, c->heads, 0, 0, g_dev[dev].num_cus);
+        if ((rc = ws.get(dev, stream, docs.bytes)) != FA_OK) return rc;
+        rc = launch_docs(dev, of_type(kScoreModule, c->dtype), stream, docs, tiles.rows, 0, &p, static_cast<int32_t*>(ws.ptr));
     }
     if (rc == FA_OK) {
         char name[64];
@@ -523,16 +548,20 @@ int fa_score_backward(void* stream_, const fa_score_config* c, const void* q, co
     const bool vec = vec_ok(q, lq, d) && vec_ok(k, lk, d) && vec_ok(v, lv, d) && vec_ok(out, lo, d) &&
                      vec_ok(dout, ldo, d) && ovec_ok(dq, ldq, es) && ovec_ok(dk, ldk, es) && ovec_ok(dv, ldv, es);
     OpsWorkspace ws;
-    const size_t rng = doc_range_bytes(*c);
     const DkvPlan dkv = plan_dkv(*c, D, vec, g_dev[dev].num_cus);
+    ScoreTiles tiles = score_tiles(*c, D, vec, sq, c->batch * c->heads, g_dev[dev].num_cus);
+    if (D == 128 && tiles.mt == 2) tiles = {1, 1, 64, ""};   // two tiles' Q, dO and sums leave one wave a SIMD
+    const DocPlan docs = plan_docs(*c, tiles.rows, c->heads, dkv.tiles.rows, c->kv_heads * dkv.splits, g_dev[dev].num_cus);
     // partial sums first: they are read and written 16 bytes at a time
     const size_t floats = dk || dv ? dkv.floats : 0;
-    if ((rc = ws.get(dev, stream, (floats + 2 * rows) * sizeof(float) + rng + 16)) != FA_OK) return rc;
+    if ((rc = ws.get(dev, stream, (floats + 2 * rows) * sizeof(float) + docs.bytes + 16)) != FA_OK) return rc;
     p.part = static_cast<float*>(ws.ptr);
     p.lse2 = p.part + floats;
     p.delta = p.lse2 + rows;
     char name[64];
-    if (c->q_doc) rc = launch_doc_ranges(dev, of_type(kScoreModule, c->dtype), stream, &p, reinterpret_cast<int32_t*>(p.delta + rows));
+    if (c->q_doc)
+        rc = launch_docs(dev, of_type(kScoreModule, c->dtype), stream, docs, tiles.rows, dkv.tiles.rows, &p,
+                         reinterpret_cast<int32_t*>(p.delta + rows));
     if (rc == FA_OK) {
         std::snprintf(name, sizeof(name), "fa_score_delta_%s%s", dtype_name(c->dtype), vec ? "" : "s");
         rc = ops_launch(dev, of_type(kScoreModule, c->dtype), name, dgrid, 256, &p, stream);
@@ -540,8 +569,6 @@ int fa_score_backward(void* stream_, const fa_score_config* c, const void* q, co
     const char* mod = score_tag(*c, vec);
     // 16-bit types: the dQ kernel also corrects delta, which dK takes from it
     if (rc == FA_OK && sq > 0 && (dq || (dk && c->dtype != FA_DTYPE_F32))) {
-        ScoreTiles tiles = score_tiles(*c, D, vec, sq, c->batch * c->heads, g_dev[dev].num_cus);
-        if (D == 128 && tiles.mt == 2) tiles = {1, 1, 64, ""};   // two tiles' Q, dO and sums leave one wave a SIMD
         p.nqb = static_cast<int>((sq + tiles.rows - 1) / tiles.rows);
         std::snprintf(name, sizeof(name), "fa_score_dq_%s_d%d_t%d%s%s", dtype_name(c->dtype), D, tiles.mt, tiles.tag, mod);
         rc = ops_launch(dev, of_type(kScoreModule, c->dtype), name, c->batch * c->heads * p.nqb, 256, &p, stream);

@@ -13,6 +13,8 @@ struct OpsStrides {
 
 // Tokens per entry of the document range tables.
 constexpr int kDocTile = 64;
+// What fa_score_doc_order takes: blocks to order, and tiles of the other side, of all batches.
+constexpr int kOrderBlocks = 1024, kOrderTiles = 4096;
 
 struct ScoreParams {
     const void *q, *k, *v, *out_in, *dout;
@@ -23,6 +25,8 @@ struct ScoreParams {
     const float* slopes;
     const int32_t *q_doc, *k_doc, *prefix;
     int32_t *q_rng, *k_rng;   // (min, max) id of each kDocTile tokens
+    int32_t *q_order, *k_order;   // batch * blocks + block, in the order of their workgroups; NULL: none
+    int q_rows, k_rows;       // rows of a block (for fa_score_doc_order)
     OpsStrides qs, ks, vs, os, dos, dqs, dks, dvs;
     int batch, heads, kv_heads, group, sq, sk, d;
     int causal, q_start;

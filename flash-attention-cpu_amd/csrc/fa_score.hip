@@ -26,15 +26,27 @@ __device__ __forceinline__ T* slice(void* base, OpsStrides st, int b, int h) {
     return reinterpret_cast<T*>(base) + b * st.b + h * st.h;
 }
 
-// (slice, block) of a workgroup: the slices of a kv head share its K and V, so all
-// its workgroups go to one XCD where the counts allow (workgroups go round-robin over the eight); blocks in
-// falling order, the longest first where causal.
+// (slice, block) of a workgroup.  Without documents: the slices of a kv head share its K and V, so all its
+// workgroups go to one XCD where the counts allow (workgroups go round-robin over the eight), blocks in falling
+// order, the longest first where causal.  With `order` (of documents): the blocks of all batches, the longest
+// first, and of every block the same heads to each XCD, so that all have the same amount of work.
 struct Work {
     int b, hk, hq, blk;   // hq: head within the group
 };
-__device__ __forceinline__ Work find_work(unsigned id, int nblk, int nkv, int group, int kv_heads) {
+__device__ __forceinline__ Work find_work(unsigned id, int nblk, int nkv, int group, int kv_heads, const int32_t* order) {
     Work w;
     int kv;
+    if (order) {
+        const int per = kv_heads * group;
+        const int item = load_uniform(order + id / per);
+        int s = id % per;
+        if ((per & 7) == 0) s = (s & 7) * (per >> 3) + (s >> 3);
+        w.b = item / nblk;
+        w.blk = item % nblk;
+        w.hk = s / group;
+        w.hq = s % group;
+        return w;
+    }
     if ((nkv & 7) == 0) {
         const int per = (nkv >> 3) * group;   // slices an XCD
         const int x = id & 7, t = id >> 3;
@@ -180,7 +192,7 @@ __device__ __forceinline__ void score_forward(const ScoreParams& p) {
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, li = lane & 15;
-    const Work w = find_work(blockIdx.x, p.nqb, p.batch * p.kv_heads, p.group, p.kv_heads);
+    const Work w = find_work(blockIdx.x, p.nqb, p.batch * p.kv_heads, p.group, p.kv_heads, p.q_order);
     const int h = w.hk * p.group + w.hq;
     const int kg = wave / NR, koff = kg * SW;   // the wave's keys of a stage: koff .. koff + SW - 1
     const int q0 = w.blk * BQ, row0 = q0 + 16 * MT * (wave % NR);
@@ -227,8 +239,10 @@ __device__ __forceinline__ void score_forward(const ScoreParams& p) {
         if (docs && wave == 0 && lane < SK) fill_words(ids, kdoc + st * SK, p.sk - st * SK, lane);
     };
 
-    // S^T of a stage, relative to the rows' references (log2 units where modified)
+    // S^T of a stage, relative to the rows' references (modified: log2 units, and what 16-bit weights are taken
+    // larger by)
     constexpr int PRE_K = NDC > 1 ? 2 : 1;
+    constexpr float kUp = MOD != 0 ? kProbLog2<T> : 0.0f;
     f32x4 s[MT][KB];
     auto qk = [&](const T* Ks, int k0) {
         constexpr int KR = PRE_K + 1;
@@ -264,13 +278,11 @@ __device__ __forceinline__ void score_forward(const ScoreParams& p) {
                 for (int b = 0; b < KB; ++b) {
                     if (cap) {
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            float th;
-                            s[t][b][r] = capped<T>(s[t][b][r], p.cap_in, p.cap_log2e, &th) - ref[t];
-                        }
+                        for (int r = 0; r < 4; ++r)
+                            s[t][b][r] = capped_over<T>(s[t][b][r], p.cap_in, p.cap_log2e, ref[t] - kUp);
                     } else {
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) s[t][b][r] = __builtin_fmaf(s[t][b][r], p.scale_log2e, -ref[t]);
+                        for (int r = 0; r < 4; ++r) s[t][b][r] = __builtin_fmaf(s[t][b][r], p.scale_log2e, kUp - ref[t]);
                     }
                     if (has_bias<MOD>(p)) {
 #pragma unroll
@@ -301,6 +313,24 @@ __device__ __forceinline__ void score_forward(const ScoreParams& p) {
         }
     };
     v8 pb[MT][NCH];
+    float sum[MT];
+    // At 128 columns the weights of a stage's second 32 keys are taken between the products of the first
+    // (16 heads x 2 x 4096^2, bf16: 314 -> 287 us all visible, 172 -> 158 causal; nothing at 64 columns).
+    constexpr bool kMix = D == 128 && NCH == 2;
+    // The weights of two scores a lane of 32 keys, pair e of its 4 MT, in two steps.
+    auto weigh2 = [&](int ch, int e, int step) {
+        const int t = e / 4, b = 2 * ch + e % 4 / 2;
+#pragma unroll
+        for (int r = 2 * (e & 1); r < 2 * (e & 1) + 2; ++r) {
+            const float x = s[t][b][r];
+            if (step == 0) {
+                s[t][b][r] = ops_exp2(MOD != 0 ? x : __builtin_fmaf(x, c, kProbLog2<T>));
+            } else {
+                pb[t][ch][4 * (b & 1) + r] = T(x);
+                sum[t] += x;
+            }
+        }
+    };
     auto softmax = [&] {
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
@@ -308,7 +338,8 @@ __device__ __forceinline__ void score_forward(const ScoreParams& p) {
 #pragma unroll
             for (int b = 0; b < KB; ++b)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) mt = fmaxf(mt, s[t][b][r]);
+                for (int r = 0; r < 4; ++r) mt = __builtin_elementwise_maximum(mt, s[t][b][r]);
+            mt -= kUp;
             // the reference moves only when a score passes it by more than kLazy, or at a row's first key
             const bool seen = m[t] != OPS_NEG_INF;
             const float limit = seen ? kLazy : OPS_NEG_INF;
@@ -326,17 +357,10 @@ __device__ __forceinline__ void score_forward(const ScoreParams& p) {
                     for (int j = 0; j < NDB; ++j) o[t][j] *= corr;
                 }
             }
-            float sum = 0.0f;
-#pragma unroll
-            for (int b = 0; b < KB; ++b)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float x = ops_exp2(__builtin_fmaf(s[t][b][r], c, kProbLog2<T>));
-                    pb[t][b / 2][4 * (b & 1) + r] = T(x);
-                    sum += x;
-                }
-            l[t] += sum;
+            sum[t] = 0.0f;
         }
+#pragma unroll
+        for (int e = 0; e < 8 * MT * (kMix ? 1 : NCH); ++e) weigh2(e / (8 * MT), e / 2 % (4 * MT), e & 1);
     };
     constexpr int PRE_V = NCH * NDB >= 4 ? 3 : 1, VR = PRE_V + 1;
     v8 va[VR];
@@ -350,9 +374,20 @@ __device__ __forceinline__ void score_forward(const ScoreParams& p) {
         for (int i = 0; i < NCH * NDB; ++i) {
             if (i + PRE_V < NCH * NDB) va[(i + PRE_V) % VR] = v_op(Vs, i + PRE_V);
 #pragma unroll
-            for (int t = 0; t < MT; ++t) o[t][i % NDB] = M::mma(va[i % VR], pb[t][i / NDB], o[t][i % NDB]);
+            for (int t = 0; t < MT; ++t) {
+                o[t][i % NDB] = M::mma(va[i % VR], pb[t][i / NDB], o[t][i % NDB]);
+                if (kMix && i < NDB) {
+                    constexpr int PER = NDB / 4;   // products a pair
+                    const int n = i % NDB * MT + t;
+                    if (n % PER == 0) weigh2(NCH - 1, n / PER, 0);
+                    if (n % PER == PER - 1) weigh2(NCH - 1, n / PER, 1);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
             __builtin_amdgcn_sched_barrier(0);
         }
+#pragma unroll
+        for (int t = 0; t < MT; ++t) l[t] += sum[t];
     };
     // whether some row of the wave sees some key of the stage (as far as causal and prefix tell)
     auto active = [&](int st) -> int {
@@ -543,7 +578,7 @@ __device__ __forceinline__ void score_dq(const ScoreParams& p) {
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, li = lane & 15;
-    const Work w = find_work(blockIdx.x, p.nqb, p.batch * p.kv_heads, p.group, p.kv_heads);
+    const Work w = find_work(blockIdx.x, p.nqb, p.batch * p.kv_heads, p.group, p.kv_heads, p.q_order);
     const int h = w.hk * p.group + w.hq;
     const int kg = wave / NR, koff = kg * 32 * NCH;   // the wave's keys of a stage
     const int q0 = w.blk * BQ, row0 = q0 + 16 * MT * (wave % NR);
@@ -800,7 +835,8 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, li = lane & 15;
     // a workgroup takes heads first .. first + count - 1 of a kv head's group; the first key blocks have most queries where causal
-    const Work w = find_work(gridDim.x - 1 - blockIdx.x, p.nqb, p.batch * p.kv_heads, p.splits, p.kv_heads);
+    const Work w = find_work(p.k_order ? blockIdx.x : gridDim.x - 1 - blockIdx.x, p.nqb, p.batch * p.kv_heads, p.splits,
+                             p.kv_heads, p.k_order);
     const int count = p.group / p.splits, first = w.hk * p.group + w.hq * count;
     const int kg = wave / NR, qoff = kg * 32 * NCH;   // the wave's queries of a stage
     const int kbeg = w.blk * BK, key0 = kbeg + 16 * MT * (wave % NR);
@@ -1084,6 +1120,62 @@ extern "C" __global__ __launch_bounds__(256) void fa_score_doc_ranges(ScoreParam
     }
 }
 
+// Orders the blocks of all batches by the number of tiles of the other side that they meet, the most first:
+// workgroup 0 the query blocks, 1 the key blocks.  Documents make blocks differ in length by far more than causal
+// bounds do, and a long one that starts late ends alone (bf16, 2 x 4096 tokens, 16 heads of 128 columns, documents
+// up to 2550 tokens, forward 155 -> 137 us; in
+// 16384 tokens of documents up to 3400: 237 -> 222).
+extern "C" __global__ __launch_bounds__(1024) void fa_score_doc_order(ScoreParams p) {
+    __shared__ int2 walked[kOrderTiles];
+    __shared__ int2 kept[kOrderBlocks];
+    __shared__ int padded[kOrderBlocks];
+    __shared__ int key[kOrderBlocks];
+    const bool isq = blockIdx.x == 0;
+    if (!(isq ? p.q_order : p.k_order)) return;
+    const int n = isq ? p.sq : p.sk, rows = isq ? p.q_rows : p.k_rows;
+    const int nt = ((isq ? p.sq : p.sk) + kDocTile - 1) / kDocTile, wt = ((isq ? p.sk : p.sq) + kDocTile - 1) / kDocTile;
+    const int nblk = (n + rows - 1) / rows, items = p.batch * nblk;
+    const int32_t *krng = isq ? p.q_rng : p.k_rng, *wrng = isq ? p.k_rng : p.q_rng;
+    const int tid = threadIdx.x, lane = tid & 63;
+    for (int i = tid; i < p.batch * wt; i += 1024) walked[i] = make_int2(wrng[2 * i], wrng[2 * i + 1]);
+    if (tid < items) {
+        const int r0 = tid % nblk * rows;
+        const DocRange x = doc_range(krng + 2 * (tid / nblk * nt), r0, min(r0 + rows, n));
+        kept[tid] = make_int2(x.lo, x.hi);
+        padded[tid] = x.padding;
+    }
+    __syncthreads();
+    for (int i = tid >> 6; i < items; i += 16) {
+        const int b = i / nblk, r0 = i % nblk * rows, r1 = min(r0 + rows, n);
+        const int prefix = p.prefix ? load_uniform(p.prefix + b) : 0;
+        const DocRange x = {kept[i].x, kept[i].y, padded[i] != 0};
+        int count = 0;
+        for (int t0 = 0; t0 < wt; t0 += 64) {
+            const int t = t0 + lane, w0 = t * kDocTile;
+            bool v = t < wt;
+            if (v) {
+                const int lo = walked[b * wt + t].x;
+                bool part;
+                v = docs_meet(x, DocRange{lo < 0 ? ~lo : lo, walked[b * wt + t].y, lo < 0}, &part);
+                if (p.causal) {
+                    const int last = isq ? r1 : min(w0 + kDocTile, p.sq), first = isq ? w0 : r0;   // query, key
+                    v = v && (first <= p.q_start + last - 1 || first < prefix);
+                }
+            }
+            count += __builtin_popcountll(__builtin_amdgcn_ballot_w64(v));
+        }
+        if (lane == 0) key[i] = (count << 10) + i;   // kOrderBlocks = 2^10: no two alike
+    }
+    __syncthreads();
+    if (tid < items) {
+        int rank = 0;
+        const int mine = key[tid];
+#pragma unroll 8
+        for (int i = 0; i < items; ++i) rank += key[i] > mine;
+        (isq ? p.q_order : p.k_order)[rank] = tid;
+    }
+}
+
 #define PASTE_(a, b, c, d) a##b##c##d
 #define PASTE(a, b, c, d) PASTE_(a, b, c, d)
 #define DELTA(VEC, TAG)                                                                                       \
@@ -1135,7 +1227,12 @@ SLOW(dkv, 2, 1, 1)
 ALL(forward, 2, 2, 2)
 ALL(dq, 2, 2, 2)
 ALL(dkv, 2, 2, 1)
-KERNELS(forward, 64, 2, 2)
+// two tiles of 64 columns: three waves a SIMD, except where a cap would spill (bf16, 16 heads x 4 x 4096^2, causal,
+// plain 200 -> 172 us, bias 282 -> 248, capped 287 -> 318)
+KERNEL(forward, 64, 2, 1, 0, true, , 3)
+KERNEL(forward, 64, 2, 1, kCap, true, c, 2)
+KERNEL(forward, 64, 2, 1, kBias, true, b, 3)
+KERNEL(forward, 64, 2, 1, kCap | kBias, true, cb, 2)
 KERNELS(forward, 128, 2, 2)
 KERNELS(dq, 64, 2, 2)
 KERNELS(dkv, 64, 2, 2)
