@@ -204,14 +204,6 @@ __device__ __forceinline__ bool not_finite(float x) {
     return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u;
 }
 
-template <typename T>
-__device__ __forceinline__ bool any_not_finite(typename Mma<T>::v8 v) {
-    bool bad = false;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) bad = bad || not_finite(float(v[e]));
-    return bad;
-}
-
 // LDS reads do not move over this, nor are their values kept in registers for a second use.
 __device__ __forceinline__ void reread() {
     asm volatile("" ::: "memory");

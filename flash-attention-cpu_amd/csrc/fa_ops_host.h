@@ -28,6 +28,8 @@ constexpr size_t kOpsMaxD = 256;
 constexpr int64_t kOpsMaxRowStride = int64_t(1) << 22;   // elements: a tile's byte offsets stay in 32 bits
 constexpr int64_t kOpsMaxStride = int64_t(1) << 44;
 constexpr size_t kTreeMaxTokens = 256;
+constexpr size_t kOpsMaxGrid = size_t(1) << 23;   // workgroups: threads of a launch stay in 32 bits
+constexpr size_t kOpsMaxTokens = size_t(1) << 31;   // of a rotary launch: a thread for each at least
 
 int ops_module(int dev, OpsModule which) {
     static const char* const files[] = {"fa_rotary.hsaco",     "fa_score_f32.hsaco",  "fa_score_bf16.hsaco",
@@ -130,6 +132,7 @@ int resolve_layout(const fa_strides& in, size_t batch, size_t seq, size_t heads,
     if (b == 0 && s == 0 && h == 0) {
         s = row;
         h = static_cast<int64_t>(seq) * row;
+        if (h > 0 && static_cast<int64_t>(heads) > kOpsMaxStride / h) return FA_ERR_UNSUPPORTED;
         b = static_cast<int64_t>(heads) * h;
     }
     // strides of single entries are never used
@@ -148,7 +151,9 @@ int resolve_layout(const fa_strides& in, size_t batch, size_t seq, size_t heads,
         for (const Dim& x : dims) {
             if (x.n <= 1) continue;
             if (x.stride < extent) return FA_ERR_INVALID_ARG;
-            extent = x.stride * static_cast<int64_t>(x.n);
+            // a stride of 2^44 over 2^30 entries would pass 64 bits; none is larger than 2^44
+            extent = x.n > static_cast<size_t>(kOpsMaxStride / x.stride) ? 2 * kOpsMaxStride
+                                                                          : x.stride * static_cast<int64_t>(x.n);
         }
     }
     out->st = {b, s, h};
@@ -223,7 +228,6 @@ DkvPlan plan_dkv(const fa_score_config& c, int D, bool vec, int num_cus) {
     r.floats = s > 1 ? 2 * s * nkv * c.seq_len_k * D : 0;
     return r;
 }
-constexpr size_t kOpsMaxGrid = size_t(1) << 23;   // workgroups: threads of a launch stay in 32 bits
 
 size_t doc_tiles(size_t n) { return (n + kDocTile - 1) / kDocTile; }
 
@@ -455,7 +459,7 @@ int launch_rotary(int dev, hipStream_t stream, int dtype, RotParams* p, bool wid
 extern "C" {
 
 int fa_score_forward(void* stream_, const fa_score_config* c, const void* q, const void* k, const void* v, void* out,
-                     float* lse) {
+                     float* lse) try {
     int rc = check_score(c);
     if (rc != FA_OK) return rc;
     if (c->batch == 0 || c->heads == 0 || c->seq_len_q == 0 || c->d_head == 0) return FA_OK;
@@ -486,7 +490,7 @@ int fa_score_forward(void* stream_, const fa_score_config* c, const void* q, con
         p.kv_heads = static_cast<int>(c->kv_heads), p.group = static_cast<int>(c->heads / c->kv_heads);
         p.n = static_cast<int>(c->seq_len_q), p.sk = static_cast<int>(c->seq_len_k), p.d = static_cast<int>(d);
         p.causal = c->causal ? 1 : 0, p.q_start = static_cast<int>(c->q_start);
-        p.scale = sc.scale, p.scale_log2e = sc.scale_log2e, p.cap_in = sc.cap_in, p.cap_log2e = sc.cap_log2e;
+        p.scale_log2e = sc.scale_log2e, p.cap_in = sc.cap_in, p.cap_log2e = sc.cap_log2e;
         return run_rows(dev, stream, c->dtype, D, vec, &p, c->seq_len_k);
     }
     ScoreParams p{};
@@ -508,10 +512,12 @@ int fa_score_forward(void* stream_, const fa_score_config* c, const void* q, con
         rc = ops_launch(dev, of_type(kScoreModule, c->dtype), name, c->batch * c->heads * p.nqb, 256, &p, stream);
     }
     return ws.done(stream, rc);
+} catch (...) {   // no memory for the tables of modules, kernels and workspaces
+    return FA_ERR_ALLOC;
 }
 
 int fa_score_backward(void* stream_, const fa_score_config* c, const void* q, const void* k, const void* v,
-                      const void* out, const float* lse, const void* dout, void* dq, void* dk, void* dv) {
+                      const void* out, const float* lse, const void* dout, void* dq, void* dk, void* dv) try {
     int rc = check_score(c);
     if (rc != FA_OK) return rc;
     if (c->batch == 0 || c->heads == 0 || c->d_head == 0) return FA_OK;
@@ -587,6 +593,8 @@ int fa_score_backward(void* stream_, const fa_score_config* c, const void* q, co
         }
     }
     return ws.done(stream, rc);
+} catch (...) {   // no memory for the tables of modules, kernels and workspaces
+    return FA_ERR_ALLOC;
 }
 
 int fa_rotary_init(fa_rotary_config* cfg, int dtype, size_t d_head, size_t rot_dim, int interleaved, double base,
@@ -630,12 +638,12 @@ int fa_rotary_init(fa_rotary_config* cfg, int dtype, size_t d_head, size_t rot_d
 
 int fa_rotary(void* stream, const fa_rotary_config* cfg, size_t batch, size_t seq_len, const int32_t* positions,
               int inverse, const fa_rotary_tensor* ql, const void* q, void* q_out, const fa_rotary_tensor* kl,
-              const void* k, void* k_out) {
+              const void* k, void* k_out) try {
     int rc = check_rotary(cfg);
     if (rc != FA_OK) return rc;
     if (!ql) return FA_ERR_INVALID_ARG;
     if (batch == 0 || seq_len == 0) return FA_OK;
-    if (batch > kOpsMaxSeq || seq_len > kOpsMaxSeq) return FA_ERR_UNSUPPORTED;
+    if (batch > kOpsMaxSeq || seq_len > kOpsMaxSeq || batch * seq_len > kOpsMaxTokens) return FA_ERR_UNSUPPORTED;
     if (!positions) return FA_ERR_INVALID_ARG;
     RotParams p{};
     bool wide = true;
@@ -669,10 +677,12 @@ int fa_rotary(void* stream, const fa_rotary_config* cfg, size_t batch, size_t se
     int dev;
     if ((rc = ops_begin(&dev, kRotaryModule)) != FA_OK) return rc;
     return launch_rotary(dev, static_cast<hipStream_t>(stream), cfg->dtype, &p, wide);
+} catch (...) {   // no memory for the tables of modules, kernels and workspaces
+    return FA_ERR_ALLOC;
 }
 
 int fa_cache_append(void* stream, const fa_kv_cache* cache, const fa_append_config* cfg, const void* k, const void* v,
-                    const int32_t* positions, const void* q, void* q_out) {
+                    const int32_t* positions, const void* q, void* q_out) try {
     OpsLayout ck, cv, lk, lv;
     size_t capacity = 0;
     int rc = check_cache(cache, &ck, &cv, &capacity);
@@ -684,7 +694,7 @@ int fa_cache_append(void* stream, const fa_kv_cache* cache, const fa_append_conf
     if (cfg->q_layout && !rot) return FA_ERR_INVALID_ARG;
     if (cache->batch == 0 || cache->kv_heads == 0 || cache->d_head == 0 || cfg->n_tokens == 0) return FA_OK;
     const size_t es = elem_size(cache->dtype), d = cache->d_head, n = cfg->n_tokens;
-    if (n > kOpsMaxSeq) return FA_ERR_UNSUPPORTED;
+    if (n > kOpsMaxSeq || cache->batch * n > kOpsMaxTokens) return FA_ERR_UNSUPPORTED;
     if ((rc = resolve_layout(cfg->k, cache->batch, n, cache->kv_heads, d, es, false, &lk)) != FA_OK ||
         (rc = resolve_layout(cfg->v, cache->batch, n, cache->kv_heads, d, es, false, &lv)) != FA_OK)
         return rc;
@@ -727,10 +737,12 @@ int fa_cache_append(void* stream, const fa_kv_cache* cache, const fa_append_conf
     int dev;
     if ((rc = ops_begin(&dev, kRotaryModule)) != FA_OK) return rc;
     return launch_rotary(dev, static_cast<hipStream_t>(stream), cache->dtype, &p, wide);
+} catch (...) {   // no memory for the tables of modules, kernels and workspaces
+    return FA_ERR_ALLOC;
 }
 
 int fa_tree_attention(void* stream, const fa_tree_config* c, const fa_kv_cache* cache, const void* q, void* out,
-                      float* lse) {
+                      float* lse) try {
     OpsLayout ck, cv, lq, lo;
     size_t capacity = 0;
     int rc = check_cache(cache, &ck, &cv, &capacity);
@@ -759,10 +771,12 @@ int fa_tree_attention(void* stream, const fa_tree_config* c, const fa_kv_cache* 
     p.n_pages = static_cast<int>(cache->n_pages), p.pages_per_seq = static_cast<int>(cache->pages_per_seq);
     p.mask_words = static_cast<int>((n + 63) / 64), p.mask_shared = c->mask_shared ? 1 : 0;
     const bool vec = vec_ok(q, lq, d) && vec_ok(cache->k, ck, d) && vec_ok(cache->v, cv, d) && ovec_ok(out, lo, es);
-    p.scale = sc.scale, p.scale_log2e = sc.scale_log2e, p.cap_in = sc.cap_in, p.cap_log2e = sc.cap_log2e;
+    p.scale_log2e = sc.scale_log2e, p.cap_in = sc.cap_in, p.cap_log2e = sc.cap_log2e;
     int dev;
     if ((rc = ops_begin(&dev, of_type(kCacheModule, cache->dtype))) != FA_OK) return rc;
     return run_rows(dev, static_cast<hipStream_t>(stream), cache->dtype, ops_pad_d(d), vec, &p, capacity);
+} catch (...) {   // no memory for the tables of modules, kernels and workspaces
+    return FA_ERR_ALLOC;
 }
 
 }  // extern "C"

@@ -62,7 +62,7 @@ struct RowsParams {
     int nrb, block_rows;      // row blocks of a (batch, kv head), and rows of one
     int num_runs, share;      // runs of keys a kv head, all sequences together; what the keys are shared out over
     int step;                 // keys that a run's length is a multiple of
-    float scale, scale_log2e, cap_in, cap_log2e;
+    float scale_log2e, cap_in, cap_log2e;   // as in ScoreParams
 };
 
 // One tensor of a rotary or append launch.

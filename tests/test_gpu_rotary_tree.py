@@ -467,3 +467,43 @@ def test_chains_longer_than_a_mask_word(n):
     c = Tree("bf16", [40, 7], 2, 2, n, 64, mask="chain", seed=n)
     c.run()
     c.check()
+
+
+@pytest.mark.parametrize("dtype", ("f32", "bf16"))
+@pytest.mark.parametrize("n", (3, 40))
+def test_more_sequences_than_lanes(dtype, n):
+    """70 and 140 sequences of all lengths, idle ones among them."""
+    for b in (70, 140):
+        lens = [(37 * i) % 300 if i % 9 else -1 for i in range(b)]
+        c = Tree(dtype, lens, 2, 1, n, 64, page=16, seed=b)
+        c.run()
+        c.check()
+
+
+@pytest.mark.parametrize("n", (4, 48))
+def test_pages_far_into_the_pool(n):
+    """Pages whose offsets pass 2^32 elements give what the same pages at the start of a small pool give."""
+    c = Tree("bf16", [1500, 700], 4, 2, n, 128, page=256, seed=17)
+    g = torch.Generator().manual_seed(18)
+    new_k, new_v = (torch.randn(2, 2, n, 128, generator=g).bfloat16().cuda() for _ in range(2))
+    cfg = fa.append_config(n)
+    fa.cache_append_device(c.cache, cfg, new_k.data_ptr(), new_v.data_ptr(), stream=stream())
+    c.run()
+    torch.cuda.synchronize()
+    want, want_lse = c.out.clone(), c.lse.clone()
+    pages = c.gk.shape[0]
+    total = 2 ** 32 // (256 * 2 * 128) + pages
+    at = total - pages
+    far = [torch.empty((total, 256, 2, 128), dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    for pool, small in zip(far, (c.kc, c.vc)):
+        pool[at:].copy_(small)
+    assert far[0][at:].storage_offset() >= 2 ** 32
+    c.keep[3].add_(at)
+    c.cache.k, c.cache.v, c.cache.n_pages = far[0].data_ptr(), far[1].data_ptr(), total
+    c.out.fill_(7.0)
+    fa.cache_append_device(c.cache, cfg, new_k.data_ptr(), new_v.data_ptr(), stream=stream())
+    c.run()
+    torch.cuda.synchronize()
+    assert torch.equal(c.out, want) and torch.equal(c.lse, want_lse)
+    for pool, small in zip(far, (c.gk, c.gv)):
+        assert torch.equal(pool[at:].nan_to_num(0), small.nan_to_num(0))

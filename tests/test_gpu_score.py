@@ -427,3 +427,111 @@ def test_two_streams_at_once():
     for c, grads in ((a, True), (b, False)):
         for n, (x, e) in c.expect(grads).items():
             check(n, c.lse if n == "lse" else c.outs[n], x, e)
+
+
+def check_batch(c, i, grads=True):
+    """One batch entry of a larger call."""
+    one = Call.__new__(Call)
+    one.__dict__.update(c.__dict__)
+    for n in ("q", "k", "v", "dout"):
+        setattr(one, n, getattr(c, n)[i:i + 1])
+    one.see = c.see[i:i + 1]
+    for n, (x, e) in one.expect(grads).items():
+        check(n, (c.lse if n == "lse" else c.outs[n])[i:i + 1], x, e)
+
+
+@pytest.mark.parametrize("dtype,d", (("bf16", 64), ("f16", 64), ("bf16", 128), ("f16", 128)))
+@pytest.mark.parametrize("mods", ({}, {"cap": 20.0}, {"alibi": True}, {"cap": 20.0, "alibi": True}))
+def test_many_blocks(dtype, d, mods):
+    """Workgroups enough for two tiles a wave, and gradients whose group is not split."""
+    c = Call(dtype, 8, 16, 4, 500, 500, d, causal=d == 64, seed=26, **mods)
+    c.forward()
+    c.backward()
+    torch.cuda.synchronize()
+    check_batch(c, 7)
+
+
+@pytest.mark.parametrize("causal", (False, True))
+@pytest.mark.parametrize("sq,sk", ((770, 770), (770, 500), (400, 1100)))
+def test_many_blocks_of_documents(causal, sq, sk):
+    """More blocks than run at once: they go in the order of their lengths.  Every entry has documents of its own."""
+    lengths = ([300, 20, 450], [5, 700], [64, 64, 128, 192, 322], [sk])
+    ids = [doc_ids(4, n, lengths, pad=n // 9) for n in (sq, sk)]
+    c = Call("bf16", 4, 16, 8, sq, sk, 64, causal=causal, q_doc=ids[0], k_doc=ids[1], seed=27)
+    c.forward()
+    c.backward()
+    torch.cuda.synchronize()
+    for i in range(4):
+        check_batch(c, i)
+
+
+def test_more_blocks_of_documents_than_are_ordered():
+    """1100 blocks of 128 queries: the tables of their order hold 1024."""
+    ids = doc_ids(220, 640, ([100, 300, 90, 150], [640], [7, 600]))
+    c = Call("bf16", 220, 2, 1, 640, 640, 64, causal=True, q_doc=ids, k_doc=ids, seed=28)
+    c.forward()
+    c.backward()
+    torch.cuda.synchronize()
+    for i in (0, 1, 219):
+        check_batch(c, i)
+
+
+@pytest.mark.parametrize("dtype", ("f32", "bf16", "f16"))
+@pytest.mark.parametrize("h,hk,sq", ((4, 1, 70), (4, 4, 90), (2, 1, 40)))
+@pytest.mark.parametrize("mods", ({}, {"cap": 20.0, "alibi": True}))
+def test_blocks_of_rows_that_share_a_long_range(dtype, h, hk, sq, mods):
+    """Few workgroups of queries over many keys: the keys are split, one block of rows or several."""
+    Call(dtype, 1, h, hk, sq, 2500, 64, causal=True, q_start=2430, seed=29, **mods).run_and_check(grads=False)
+
+
+def test_small_gradients_in_f16():
+    """dO of 1e-4: products with weights below the normal numbers of the type."""
+    c = Call("f16", 1, 2, 1, 300, 300, 64, causal=True, seed=30)
+    c.dout = (c.dout.float() * 1e-4).half()
+    c.gpu["dout"] = to_gpu(c.dout)
+    c.forward()
+    c.backward()
+    torch.cuda.synchronize()
+    tiny = 2.0 ** -24   # half a step of the numbers below 2^-14, times 2 for the two factors of a product
+    x = c.expect()
+    for n in ("dq", "dk", "dv"):
+        # each of up to 300 products carries a rounding of its weight's gradient (dS), up to `tiny` / 2 absolutely,
+        # against an operand below 4.5 times the scale, once for each of the group's two heads
+        slack = 300 * 2 * tiny * 4.5 * (c.scale if n != "dv" else 1e-4)
+        check(n, c.outs[n], x[n][0], x[n][1] + slack)
+
+
+def test_two_graphs_and_eager_calls_at_once():
+    """Two captured steps replay on streams of their own while an eager one runs: each has its own workspace."""
+    ids = doc_ids(4, 600, ([200, 400], [500, 90]))
+    cases = [Call("bf16", 4, 16, 4, 600, 600, 64, causal=True, q_doc=ids, k_doc=ids, seed=s) for s in (31, 32, 33)]
+    side, graphs = torch.cuda.Stream(), []
+    for c in cases[:2]:
+        with torch.cuda.stream(side):
+            c.forward()
+            c.backward()
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            c.forward()
+            c.backward()
+        graphs.append(graph)
+    first = None
+    for _ in range(3):
+        for c in cases:
+            for x in c.outs.values():
+                x.fill_(7.0)
+        torch.cuda.synchronize()
+        for stream, graph in zip((side, torch.cuda.Stream()), graphs):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        cases[2].forward()
+        cases[2].backward()
+        torch.cuda.synchronize()
+        if first is None:
+            first = [{n: x.clone() for n, x in c.outs.items()} for c in cases]
+            for c in cases:
+                check_batch(c, 3)
+        for c, f in zip(cases, first):
+            for n, x in c.outs.items():
+                assert torch.equal(x, f[n]), n

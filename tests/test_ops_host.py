@@ -221,3 +221,13 @@ def test_structs_match_the_header(tmp_path):
     subprocess.run(["gcc", "-std=c11", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(exe)], check=True)
     got = [int(x) for x in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()]
     assert got == want
+
+
+def test_sizes_whose_products_pass_64_bits():
+    big = 1 << 30
+    assert rotary(batch=big, seq=big) == UNSUPPORTED
+    assert rotary(layout=fa.rotary_tensor(big), batch=2, seq=big) == UNSUPPORTED
+    assert score(batch=big, heads=big, kv_heads=1, sq=big) == UNSUPPORTED
+    assert tree(c=cache(batch=big, kv_heads=2, capacity=big)) == UNSUPPORTED
+    # heads 2^44 apart, 2^30 of them, inside a batch stride that they pass
+    assert score(heads=big, kv_heads=1, out=PTR, strides={"out": (1 << 44, 64, 1 << 44)}) in (INVALID, UNSUPPORTED)
