@@ -6,7 +6,7 @@
 // group, so K and V are read once for all of them.  The keys of all sequences are cut into runs of one length,
 // one a workgroup, so that sequences of different lengths keep all of the GPU busy; a sequence of more than one run leaves
 // partial sums that fa_rows_merge joins.
-//   stream: up to 64 rows.  Bound by memory: every wave walks 32-key blocks of its own
+//   stream: up to 16 rows, up to 64 where a row of K has 128 bytes.  Bound by memory: every wave walks 32-key blocks of its own
 //           through LDS that only it uses, two slots of K and V, one filled by DMA while the
 //           other is used; no barrier until the waves' sums are joined at the end.
 //   shared: more rows.  Eight waves of one or two 16-row tiles share the stages of a ring, two of which are on
@@ -365,7 +365,9 @@ struct RowTiles {
             l[t] = ref[t] = 0.0f;
         }
     }
-    // Scores of KB blocks of keys from k0, relative to the references; hidden ones -inf.
+    // Scores of KB blocks of keys from k0, relative to the references (modified: log2 units, and what 16-bit weights
+    // are taken larger by); hidden ones -inf.
+    static constexpr float kUp = MOD != 0 ? kProbLog2<T> : 0.0f;
     __device__ __forceinline__ void scores(const RowsParams& p, const RowsWork& w, const T* Ks, int k0, bool masked,
                                            bool badpage) {
 #pragma unroll
@@ -393,13 +395,11 @@ struct RowTiles {
                 for (int b = 0; b < KB; ++b) {
                     if (has_cap<MOD>(p)) {
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            float th;
-                            s[t][b][r] = capped<T>(s[t][b][r], p.cap_in, p.cap_log2e, &th) - ref[t];
-                        }
+                        for (int r = 0; r < 4; ++r)
+                            s[t][b][r] = capped_over<T>(s[t][b][r], p.cap_in, p.cap_log2e, ref[t] - kUp);
                     } else {
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) s[t][b][r] = __builtin_fmaf(s[t][b][r], p.scale_log2e, -ref[t]);
+                        for (int r = 0; r < 4; ++r) s[t][b][r] = __builtin_fmaf(s[t][b][r], p.scale_log2e, kUp - ref[t]);
                     }
                     if (has_bias<MOD>(p)) {
                         f32x4 x;
@@ -485,7 +485,8 @@ struct RowTiles {
 #pragma unroll
             for (int b = 0; b < KB; ++b)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) mt = fmaxf(mt, s[t][b][r]);
+                for (int r = 0; r < 4; ++r) mt = __builtin_elementwise_maximum(mt, s[t][b][r]);
+            mt -= kUp;
             const bool seen = m[t] != OPS_NEG_INF;
             const float limit = seen ? kLazy : OPS_NEG_INF;
             if (__builtin_amdgcn_ballot_w64(mt * c > limit) != 0) {
@@ -507,7 +508,7 @@ struct RowTiles {
             for (int b = 0; b < KB; ++b)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const float x = ops_exp2(__builtin_fmaf(s[t][b][r], c, kProbLog2<T>));
+                    const float x = ops_exp2(MOD != 0 ? s[t][b][r] : __builtin_fmaf(s[t][b][r], c, kProbLog2<T>));
                     pb[t][b / 2][4 * (b & 1) + r] = T(x);
                     sum += x;
                 }
@@ -916,10 +917,9 @@ COMMON(64)
 COMMON(128)
 COMMON(256)
 STREAM(64, 1, 2)
-STREAM(64, 2, 2)
 STREAM(128, 1, 2)
 #ifdef OPS_16BIT
-STREAM(128, 2, 2)
+STREAM(64, 2, 2)
 STREAM(256, 1, 2)
 SHARED(64, 2, 2)
 SHARED(128, 2, 2)

@@ -231,7 +231,7 @@ DkvPlan plan_dkv(const fa_score_config& c, int D, bool vec, int num_cus) {
 
 size_t doc_tiles(size_t n) { return (n + kDocTile - 1) / kDocTile; }
 
-// Plan of the rows kernels: streaming waves up to 64 rows, else workgroups that share their
+// Plan of the rows kernels: streaming waves for few rows, else workgroups that share their
 // keys; the keys of all sequences shared out over as many runs as fill the GPU once.
 struct RowsPlan {
     bool stream;
@@ -242,18 +242,23 @@ RowsPlan plan_rows(int dtype, int D, bool vec, size_t batch, size_t kv_heads, si
     RowsPlan r{};
     const bool f32 = dtype == FA_DTYPE_F32;
     const int row_bytes = D * static_cast<int>(elem_size(dtype));
-    r.stream = vec && rows <= 64 && row_bytes <= 512;
+    // A streaming wave reads a block's K and V for 16 or 32 rows only; with more rows it reads them again (8 sequences
+    // of 8000 keys, bf16: 64 rows of 128 columns 102 us streamed, 60 shared, of 256 columns 312 and 107; 16 rows of 128
+    // columns 45 and 57; 64 rows of 64 columns 42 and 47)
+    r.stream = vec && rows <= (row_bytes <= 128 ? 64 : 16) && row_bytes <= 512;
     size_t resident = static_cast<size_t>(num_cus);
     if (r.stream) {
-        // two tiles a wave as far as its registers hold them
-        r.mt = rows <= 16 || row_bytes > 256 ? 1 : 2;
+        r.mt = rows <= 16 ? 1 : 2;
         const int waves = row_bytes <= 256 ? kStreamWaves<256> : kStreamWaves<512>;
         r.threads = 64 * waves;
         r.rows = 16 * r.mt;
         r.step = 32 * waves;
         if (row_bytes <= 128) resident *= 2;   // LDS holds one workgroup a CU, two of short rows
     } else {
-        r.mt = !vec || f32 || D > 128 || rows <= 128 ? 1 : 2;
+        // Two tiles a wave halve what is read from LDS and L2, but start and end later: where each CU gets 16 stages or
+        // more (d128: 8 sequences of 16384 keys, 256 rows 308 us with one, 210 with two; 4 of 3000, 200 rows 32 and 39)
+        const size_t stages = batch * keys * kv_heads * ((rows + 127) / 128) / 64;
+        r.mt = !vec || f32 || D > 128 || rows <= 128 || stages < 16 * resident ? 1 : 2;
         r.threads = 512;
         r.rows = 128 * r.mt;
         r.step = f32 || D > 128 ? 32 : 64;
@@ -266,6 +271,9 @@ RowsPlan plan_rows(int dtype, int D, bool vec, size_t batch, size_t kv_heads, si
     size_t share = batch == 1 ? slots : 2 * (batch - 1) <= slots ? slots - (batch - 1) : 4 * slots;
     share = std::min(share, batch * std::max<size_t>(1, (keys + r.step - 1) / r.step));
     if (batch * units >= 4 * resident) share = 1;   // sequences enough: one run each
+    // Few keys: one run each too, which saves the merge, some 4 us, unless walking them costs as much (measured: 8
+    // sequences of 250 keys, bf16, 7 rows of 64 columns 13.1 us split, 9.7 whole; 3 of 250, f32, 8 rows of 80 17.6 and 23.6)
+    if (keys <= static_cast<size_t>(r.step) * (f32 || D > 128 ? 1 : 4)) share = 1;
     r.share = static_cast<int>(share);
     // each sequence rounds its share up to whole runs; eight runs and heads more or less fall
     // on the eight XCDs evenly
