@@ -546,9 +546,9 @@ int fa_score_backward(void* stream_, const fa_score_config* c, const void* q, co
     if (sq > 0 && (!q || !out || !lse || !dout)) return FA_ERR_INVALID_ARG;
     if (sk > 0 && (!k || !v)) return FA_ERR_INVALID_ARG;
     const int D = ops_pad_d(d);
-    const size_t rows = c->batch * c->heads * sq, dgrid = (rows + 15) / 16;
+    const size_t rows = c->batch * c->heads * sq;
     if (c->batch * c->heads > kOpsMaxGrid || (sq + 31) / 32 * c->batch * c->heads > kOpsMaxGrid ||
-        (sk + 31) / 32 * c->batch * c->heads > kOpsMaxGrid || dgrid > kOpsMaxGrid)
+        (sk + 31) / 32 * c->batch * c->heads > kOpsMaxGrid)
         return FA_ERR_UNSUPPORTED;
     int dev;
     if ((rc = ops_begin(&dev, of_type(kScoreModule, c->dtype))) != FA_OK) return rc;
@@ -576,13 +576,9 @@ int fa_score_backward(void* stream_, const fa_score_config* c, const void* q, co
     if (c->q_doc)
         rc = launch_docs(dev, of_type(kScoreModule, c->dtype), stream, docs, tiles.rows, dkv.tiles.rows, &p,
                          reinterpret_cast<int32_t*>(p.delta + rows));
-    if (rc == FA_OK) {
-        std::snprintf(name, sizeof(name), "fa_score_delta_%s%s", dtype_name(c->dtype), vec ? "" : "s");
-        rc = ops_launch(dev, of_type(kScoreModule, c->dtype), name, dgrid, 256, &p, stream);
-    }
     const char* mod = score_tag(*c, vec);
-    // 16-bit types: the dQ kernel also corrects delta, which dK takes from it
-    if (rc == FA_OK && sq > 0 && (dq || (dk && c->dtype != FA_DTYPE_F32))) {
+    // the dQ kernel also forms delta and lse2, and with 16-bit types corrects delta, for the other one
+    if (rc == FA_OK && sq > 0) {
         p.nqb = static_cast<int>((sq + tiles.rows - 1) / tiles.rows);
         std::snprintf(name, sizeof(name), "fa_score_dq_%s_d%d_t%d%s%s", dtype_name(c->dtype), D, tiles.mt, tiles.tag, mod);
         rc = ops_launch(dev, of_type(kScoreModule, c->dtype), name, c->batch * c->heads * p.nqb, 256, &p, stream);

@@ -503,33 +503,6 @@ __device__ __forceinline__ void score_forward(const ScoreParams& p) {
 // Backward
 // ---------------------------------------------------------------------------
 
-// delta = dO . O and lse2 = lse log2(e) of every row, a group of 16 lanes a row.  Empty rows get lse2 = +inf: their
-// weights e^(z - lse) then come out as 0.
-template <typename T, bool VEC>
-__device__ __forceinline__ void score_delta(const ScoreParams& p) {
-    const int64_t row = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 4;
-    const int li = threadIdx.x & 15;
-    const int64_t total = (int64_t)p.batch * p.heads * p.sq;
-    if (row >= total) return;
-    const int i = row % p.sq, h = row / p.sq % p.heads, b = row / p.sq / p.heads;
-    const T* o = slice<T>(p.out_in, p.os, b, h);
-    const T* g = slice<T>(p.dout, p.dos, b, h);
-    float sum = 0.0f;
-    for (int col = 8 * li; col < p.d; col += 128) {
-        const auto x = global_row<T, VEC>(o, p.os.s, i, p.sq, col, p.d);
-        const auto y = global_row<T, VEC>(g, p.dos.s, i, p.sq, col, p.d);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sum += float(x[e]) * float(y[e]);
-    }
-#pragma unroll
-    for (int s = 1; s < 16; s *= 2) sum += __shfl_xor(sum, s);
-    if (li == 0) {
-        const float lse = p.lse_in[row];
-        p.delta[row] = sum;
-        p.lse2[row] = lse == OPS_NEG_INF ? -OPS_NEG_INF : lse == -OPS_NEG_INF ? __builtin_nanf("") : lse * kLog2e;
-    }
-}
-
 // Of four scores: the weights p = e^(z - lse), the gradients y = p (dP - delta) of the modified scores z, and
 // what these have to be multiplied by for the raw ones (1 - tanh^2; 1 without a cap).
 template <typename T, int MOD>
@@ -552,6 +525,8 @@ __device__ __forceinline__ void weigh(const ScoreParams& p, bool cap, f32x4 s, f
 }
 
 // dQ: query rows kept, keys walked.  Four waves of MT 16-row tiles; K and V tiles double-buffered, one barrier a stage.
+// On the way in a wave leaves delta = dO . O and lse2 = lse log2(e) of its rows for the dK / dV kernel.  Empty rows get
+// lse2 = +inf: their weights e^(z - lse) then come out as 0.
 //
 // 16-bit types: delta = dO . O comes from the rounded O, and an error of delta is common to all keys of a row, so
 // it does not average out: it was the largest error of dQ and dK (bf16, 2 x 4096 tokens, documents, capped scores:
@@ -606,8 +581,21 @@ __device__ __forceinline__ void score_dq(const ScoreParams& p) {
             doreg[t][dc] = global_row<T, VEC>(dO, p.dos.s, row, p.sq, 32 * dc + 8 * g, p.d);
         }
         qd[t] = docs && row < p.sq ? p.q_doc[(int64_t)w.b * p.sq + row] : -1;
-        lse2[t] = row < p.sq ? p.lse2[at] : -OPS_NEG_INF;
-        delta[t] = row < p.sq ? p.delta[at] : 0.0f;
+        const T* O = slice<T>(p.out_in, p.os, w.b, h);
+        float sum = 0.0f;
+#pragma unroll
+        for (int dc = 0; dc < NDC; ++dc) {
+            const v8 o = global_row<T, VEC>(O, p.os.s, row, p.sq, 32 * dc + 8 * g, p.d);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum += float(o[e]) * float(doreg[t][dc][e]);
+        }
+        delta[t] = row4_sum(sum);
+        const float lse = row < p.sq ? p.lse_in[at] : OPS_NEG_INF;
+        lse2[t] = lse == OPS_NEG_INF ? -OPS_NEG_INF : lse == -OPS_NEG_INF ? __builtin_nanf("") : lse * kLog2e;
+        if (row < p.sq && g == 0 && kg == 0) {
+            p.lse2[at] = lse2[t];
+            p.delta[at] = delta[t];
+        }
         limit[t] = (docs && qd[t] < 0) || lse2[t] == -OPS_NEG_INF ? 0 : min(p.sk, key_limit(p, prefix, p.q_start + row));
 #pragma unroll
         for (int j = 0; j < NDB; ++j) {
@@ -616,6 +604,7 @@ __device__ __forceinline__ void score_dq(const ScoreParams& p) {
         }
         err[t] = 0.0f;
     }
+    if (!p.dq && !(kRefine && p.dk)) return;   // the dK / dV kernel wants lse2 and delta alone
     const int q1 = min(q0 + BQ, p.sq);
     DocRange qr = {};
     const int32_t* krng = nullptr;
@@ -1178,12 +1167,6 @@ extern "C" __global__ __launch_bounds__(1024) void fa_score_doc_order(ScoreParam
 
 #define PASTE_(a, b, c, d) a##b##c##d
 #define PASTE(a, b, c, d) PASTE_(a, b, c, d)
-#define DELTA(VEC, TAG)                                                                                       \
-    extern "C" __global__ __launch_bounds__(256) void PASTE(fa_score_delta_, OPS_NAME, , TAG)(ScoreParams p) { \
-        score_delta<OPS_T, VEC>(p);                                                                           \
-    }
-DELTA(true, )
-DELTA(false, s)
 #define KERNEL(F, D, MT, KG, MOD, VEC, TAG, WAVES)                                                    \
     extern "C" __global__ __launch_bounds__(256, WAVES) void PASTE(fa_score_##F##_, OPS_NAME, _d##D##_t##MT, TAG)( \
         ScoreParams p) {                                                                              \
