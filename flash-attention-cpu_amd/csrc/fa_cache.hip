@@ -12,7 +12,7 @@
 //   shared: more rows.  Eight waves of one or two 16-row tiles share the stages of a ring, two of which are on
 //           their way while one is used, so that K and V cross the L2 once for up to 256 rows.
 // Tiles in LDS have no padding, so that DMA instructions move 1 KiB of whole rows; row r keeps
-// 16-byte chunk x at position x ^ (r % 16), which spreads row reads and transposed
+// 16-byte chunk x at position x ^ turn(r), which spreads row reads and transposed
 // reads over the banks.
 //
 // Built once a type: OPS_T the element type, OPS_NAME its name in the kernels'.
@@ -28,8 +28,20 @@ struct Swizzled {
     static constexpr int CM = CPR < 16 ? CPR : 16;
     static constexpr int RPR = 64 / CPR > 0 ? 64 / CPR : 1;   // rows of a 1 KiB run
     static_assert(CPR <= 64, "a run holds whole rows");
+    // What row `row` adds to its chunk numbers: the same for rows 16 apart.  16-bit types: 16 rows (eight of 128 bytes)
+    // get different values, and eight that follow each other values that differ above the lowest bit, since a
+    // transposed read takes two chunks of eight rows at a time.
+    static __device__ __forceinline__ int turn(int row) {
+        if constexpr (sizeof(T) == 4) {
+            return row % CM;
+        } else if constexpr (CPR == 8) {
+            return (row >> 1 & 3) << 1 | (row >> 3 & 1);
+        } else {
+            return (row & 7) << 1 | (row >> 3 & 1);
+        }
+    }
     static __device__ __forceinline__ int at(int row, int col) {   // col: a multiple of E or inside its chunk
-        return row * D + (((col / E) ^ (row % CM)) * E) + col % E;
+        return row * D + (((col / E) ^ turn(row)) * E) + col % E;
     }
     // An operand's chunk numbers are those of its first column block, exclusive-or the block's own (a
     // multiple of what the lanes add), so its place is base ^ block; row0 (a multiple of 16) only adds whole rows.
@@ -103,7 +115,7 @@ struct RowSource {
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
             const int row = (i * NW + wave) * S::RPR + lane / S::CPR;
-            const int col = ((lane % S::CPR) ^ (row % S::CM)) * S::E;
+            const int col = ((lane % S::CPR) ^ S::turn(row)) * S::E;
             voff[i] = col < d ? (int)(row * seq + col) * (int)sizeof(T) : 0x7ffffff0;
         }
     }

@@ -524,6 +524,12 @@ __device__ __forceinline__ void weigh(const ScoreParams& p, bool cap, f32x4 s, f
     }
 }
 
+// Operands of the gradient kernels' products that are read from LDS ahead of their use: PRE steps, and the first ones of
+// the column products before the weights are formed (bf16, 2 x 4096 tokens, 16 heads of 128 columns, documents, capped:
+// forward and backward 644 -> 606 us; 16 heads x 2 x 4096^2 all visible, backward 1207 -> 1132; three steps: no more).
+template <typename T>
+constexpr int kAhead = sizeof(T) == 2 ? 2 : 1;
+
 // dQ: query rows kept, keys walked.  Four waves of MT 16-row tiles; K and V tiles double-buffered, one barrier a stage.
 // On the way in a wave leaves delta = dO . O and lse2 = lse log2(e) of its rows for the dK / dV kernel.  Empty rows get
 // lse2 = +inf: their weights e^(z - lse) then come out as 0.
@@ -542,6 +548,7 @@ __device__ __forceinline__ void score_dq(const ScoreParams& p) {
     constexpr bool kRefine = sizeof(T) == 2;
     constexpr int NW = 4, NR = NW / KG, SK = kStageRows<T, D, KG>, BQ = 16 * MT * NR;
     constexpr int NCH = SK / 32 / KG, NDC = D / 32, NDB = D / 16, LD = D + kPad<T>;
+    constexpr int PRE = D > 128 ? 1 : kAhead<T>;   // (at 256 columns registers are short)
     using Fill = TileFill<T, D, SK, NW, VEC>;
     T* const Kb0 = lds_array<T, Fill::SIZE, 0>();
     T* const Vb0 = lds_array<T, Fill::SIZE, 1>();
@@ -643,6 +650,12 @@ __device__ __forceinline__ void score_dq(const ScoreParams& p) {
         if (nx >= 0) fill(nx, P ? Kb0 : Kb1, P ? Vb0 : Vb1, P ? Db0 : Db1);
         const int k0 = st * SK;
         const int act = active(st), dirty = masked ? __builtin_amdgcn_readfirstlane(Special[1 + P]) : 0;
+        v8 ca[PRE + 1];
+        auto col = [&](int i, int j) { ca[j % (PRE + 1)] = col_op<T, LD>(Ks, koff + 32 * i, 16 * j, g, li); };
+        auto preload = [&](int i) {
+#pragma unroll
+            for (int j = 0; j < PRE; ++j) col(i, j);
+        };
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
             v8 db[MT], pb[MT];
@@ -652,20 +665,24 @@ __device__ __forceinline__ void score_dq(const ScoreParams& p) {
                 for (int t = 0; t < MT; ++t)
 #pragma unroll
                     for (int b = 0; b < 2; ++b) s[t][b] = dp[t][b] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+                v8 ka[PRE + 1], va[PRE + 1];
+                auto load = [&](int n) {   // operands of key block n % 2, columns 32 (n / 2)
+                    ka[n % (PRE + 1)] = row_op<T, LD>(Ks, koff + 32 * i + 16 * (n % 2), n / 2, g, li);
+                    va[n % (PRE + 1)] = row_op<T, LD>(Vs, koff + 32 * i + 16 * (n % 2), n / 2, g, li);
+                };
 #pragma unroll
-                for (int dc = 0; dc < NDC; ++dc) {
+                for (int n = 0; n < PRE; ++n) load(n);
 #pragma unroll
-                    for (int b = 0; b < 2; ++b) {
-                        const v8 ka = row_op<T, LD>(Ks, koff + 32 * i + 16 * b, dc, g, li);
-                        const v8 va = row_op<T, LD>(Vs, koff + 32 * i + 16 * b, dc, g, li);
+                for (int n = 0; n < 2 * NDC; ++n) {
+                    if (n + PRE < 2 * NDC) load(n + PRE);
 #pragma unroll
-                        for (int t = 0; t < MT; ++t) {
-                            s[t][b] = M::mma(ka, qreg[t][dc], s[t][b]);
-                            dp[t][b] = M::mma(va, doreg[t][dc], dp[t][b]);
-                        }
+                    for (int t = 0; t < MT; ++t) {
+                        s[t][n % 2] = M::mma(ka[n % (PRE + 1)], qreg[t][n / 2], s[t][n % 2]);
+                        dp[t][n % 2] = M::mma(va[n % (PRE + 1)], doreg[t][n / 2], dp[t][n % 2]);
                     }
-                    if (NDC > 4 || MT > 1) __builtin_amdgcn_sched_barrier(0);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
+                if (!dirty) preload(i);
 #pragma unroll
                 for (int t = 0; t < MT; ++t) {
                     const int pos = p.q_start + row0 + 16 * t + li;
@@ -701,17 +718,18 @@ __device__ __forceinline__ void score_dq(const ScoreParams& p) {
                 __syncthreads();
                 if (tile_clean<T, LD, D, 32 * KG, 64 * NW>(Ks + 32 * i * LD, tid)) *Special = 1;
                 __syncthreads();
+                if (act) preload(i);
             }
             if (act) {
 #pragma unroll
                 for (int j = 0; j < NDB; ++j) {
-                    const v8 a = col_op<T, LD>(Ks, koff + 32 * i, 16 * j, g, li);
+                    if (j + PRE < NDB) col(i, j + PRE);
 #pragma unroll
                     for (int t = 0; t < MT; ++t) {
-                        dq[t][j] = M::mma(a, db[t], dq[t][j]);
-                        if (kRefine) pk[t][j] = M::mma(a, pb[t], pk[t][j]);
+                        dq[t][j] = M::mma(ca[j % (PRE + 1)], db[t], dq[t][j]);
+                        if (kRefine) pk[t][j] = M::mma(ca[j % (PRE + 1)], pb[t], pk[t][j]);
                     }
-                    if (j % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
         }
@@ -812,6 +830,7 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
     using v8 = typename M::v8;
     constexpr int NW = 4, NR = NW / KG, SQ = kStageRows<T, D, KG>, BK = 16 * MT * NR;
     constexpr int NCH = SQ / 32 / KG, NDC = D / 32, NDB = D / 16, LD = D + kPad<T>;
+    constexpr int PRE = kAhead<T>;
     using Fill = TileFill<T, D, SQ, NW, VEC>;
     T* const Qb0 = lds_array<T, Fill::SIZE, 0>();
     T* const Ob0 = lds_array<T, Fill::SIZE, 1>();
@@ -926,6 +945,15 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
         const int q0 = st * SQ;
         const int act = active(st), dirty = masked ? __builtin_amdgcn_readfirstlane(Special[1 + P]) : 0;
         const float slope = has_bias<MOD>(p) ? load_uniform(p.slopes + first + hq) * kLog2e : 0.0f;
+        v8 co[PRE + 1], cq[PRE + 1];
+        auto col = [&](int i, int j) {
+            co[j % (PRE + 1)] = col_op<T, LD>(Os, qoff + 32 * i, 16 * j, g, li);
+            cq[j % (PRE + 1)] = col_op<T, LD>(Qs, qoff + 32 * i, 16 * j, g, li);
+        };
+        auto preload = [&](int i) {
+#pragma unroll
+            for (int j = 0; j < PRE; ++j) col(i, j);
+        };
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
             v8 pb[MT][1], db[MT][1];
@@ -935,20 +963,24 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
                 for (int t = 0; t < MT; ++t)
 #pragma unroll
                     for (int b = 0; b < 2; ++b) s[t][b] = dp[t][b] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+                v8 qa[PRE + 1], oa[PRE + 1];
+                auto load = [&](int n) {   // operands of query block n % 2, columns 32 (n / 2)
+                    qa[n % (PRE + 1)] = row_op<T, LD>(Qs, qoff + 32 * i + 16 * (n % 2), n / 2, g, li);
+                    oa[n % (PRE + 1)] = row_op<T, LD>(Os, qoff + 32 * i + 16 * (n % 2), n / 2, g, li);
+                };
 #pragma unroll
-                for (int dc = 0; dc < NDC; ++dc) {
+                for (int n = 0; n < PRE; ++n) load(n);
 #pragma unroll
-                    for (int b = 0; b < 2; ++b) {
-                        const v8 qa = row_op<T, LD>(Qs, qoff + 32 * i + 16 * b, dc, g, li);
-                        const v8 oa = row_op<T, LD>(Os, qoff + 32 * i + 16 * b, dc, g, li);
+                for (int n = 0; n < 2 * NDC; ++n) {
+                    if (n + PRE < 2 * NDC) load(n + PRE);
 #pragma unroll
-                        for (int t = 0; t < MT; ++t) {
-                            s[t][b] = M::mma(qa, kreg[t][dc], s[t][b]);
-                            dp[t][b] = M::mma(oa, vreg[t][dc], dp[t][b]);
-                        }
+                    for (int t = 0; t < MT; ++t) {
+                        s[t][n % 2] = M::mma(qa[n % (PRE + 1)], kreg[t][n / 2], s[t][n % 2]);
+                        dp[t][n % 2] = M::mma(oa[n % (PRE + 1)], vreg[t][n / 2], dp[t][n % 2]);
                     }
-                    if (NDC > 4 || MT > 1) __builtin_amdgcn_sched_barrier(0);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
+                if (!dirty) preload(i);
 #pragma unroll
                 for (int b = 0; b < 2; ++b) {
                     const int at = qoff + 32 * i + 16 * b + 4 * g, pos = p.q_start + q0 + at;
@@ -983,18 +1015,18 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
                 const bool bad = tile_clean<T, LD, D, 32 * KG, 64 * NW>(Qs + 32 * i * LD, tid);
                 if (tile_clean<T, LD, D, 32 * KG, 64 * NW>(Os + 32 * i * LD, tid) || bad) *Special = 1;
                 __syncthreads();
+                if (act) preload(i);
             }
             if (act) {
 #pragma unroll
                 for (int j = 0; j < NDB; ++j) {
-                    const v8 a = col_op<T, LD>(Os, qoff + 32 * i, 16 * j, g, li);
-                    const v8 c = col_op<T, LD>(Qs, qoff + 32 * i, 16 * j, g, li);
+                    if (j + PRE < NDB) col(i, j + PRE);
 #pragma unroll
                     for (int t = 0; t < MT; ++t) {
-                        dv[t][j] = M::mma(a, pb[t][0], dv[t][j]);
-                        dk[t][j] = M::mma(c, db[t][0], dk[t][j]);
+                        dv[t][j] = M::mma(co[j % (PRE + 1)], pb[t][0], dv[t][j]);
+                        dk[t][j] = M::mma(cq[j % (PRE + 1)], db[t][0], dk[t][j]);
                     }
-                    if (j % 2 == 1) __builtin_amdgcn_sched_barrier(0);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
         }
