@@ -389,15 +389,21 @@ struct RowTiles {
                 const float x = MOD != 0 ? 0.0f : -ref[t];
                 s[t][b] = (f32x4){x, x, x, x};
             }
+        constexpr int PRE = sizeof(T) == 2 ? 1 : 0;   // 32-column steps read ahead
+        v8 k[PRE + 1][KB];
+        auto load = [&](int dc) {
+#pragma unroll
+            for (int b = 0; b < KB; ++b) k[dc % (PRE + 1)][b] = S::row_op(Ks, 16 * b, dc, g, li);
+        };
+        if (PRE) load(0);
 #pragma unroll
         for (int dc = 0; dc < NDC; ++dc) {
+            if (dc + PRE < NDC) load(dc + PRE);
 #pragma unroll
-            for (int b = 0; b < KB; ++b) {
-                const v8 k = S::row_op(Ks, 16 * b, dc, g, li);
+            for (int b = 0; b < KB; ++b)
 #pragma unroll
-                for (int t = 0; t < MT; ++t) s[t][b] = M::mma(k, q[t][dc], s[t][b]);
-            }
-            if (sizeof(T) == 4 || dc % 2 == 1) __builtin_amdgcn_sched_barrier(0);
+                for (int t = 0; t < MT; ++t) s[t][b] = M::mma(k[dc % (PRE + 1)][b], q[t][dc], s[t][b]);
+            __builtin_amdgcn_sched_barrier(0);
         }
         if constexpr (MOD != 0) {
 #pragma unroll
@@ -528,15 +534,18 @@ struct RowTiles {
         }
     }
     __device__ __forceinline__ void values(const T* Vs) {
+        constexpr int PRE = sizeof(T) == 2 ? 3 : 0;
+        v8 a[PRE + 1];
+        auto load = [&](int n) { a[n % (PRE + 1)] = S::col_op(Vs, 32 * (n / NDB), 16 * (n % NDB), g, li); };
 #pragma unroll
-        for (int i = 0; i < NCH; ++i)
+        for (int n = 0; n < PRE; ++n) load(n);
 #pragma unroll
-            for (int j = 0; j < NDB; ++j) {
-                const v8 a = S::col_op(Vs, 32 * i, 16 * j, g, li);
+        for (int n = 0; n < NCH * NDB; ++n) {
+            if (n + PRE < NCH * NDB) load(n + PRE);
 #pragma unroll
-                for (int t = 0; t < MT; ++t) o[t][j] = M::mma(a, pb[t][i], o[t][j]);
-                if (sizeof(T) == 4 || j % 4 == 3) __builtin_amdgcn_sched_barrier(0);
-            }
+            for (int t = 0; t < MT; ++t) o[t][n % NDB] = M::mma(a[n % (PRE + 1)], pb[t][n / NDB], o[t][n % NDB]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
     }
     // maxima in log2 units and whole row sums, before partial sums meet
     __device__ __forceinline__ void close() {
