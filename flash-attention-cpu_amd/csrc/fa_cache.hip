@@ -2,15 +2,18 @@
 // over a key / value cache (fa_tree_attention) and short query blocks of score
 // attention (fa_score_forward).
 //
-// The rows of a (sequence, kv head) are its tokens times the query heads of the
-// group, so K and V are read once for all of them.  The keys of all sequences are cut into runs of one length,
-// one a workgroup, so that sequences of different lengths keep all of the GPU busy; a sequence of more than one run leaves
-// partial sums that fa_rows_merge joins.
-//   stream: up to 16 rows, up to 64 where a row of K has 128 bytes.  Bound by memory: every wave walks 32-key blocks of its own
-//           through LDS that only it uses, two slots of K and V, one filled by DMA while the
-//           other is used; no barrier until the waves' sums are joined at the end.
+// The rows of a (sequence, kv head) are its tokens times the query heads of the group, so K and V are read once for
+// all of them.  The keys of all sequences are cut into runs of one length, one a workgroup, so that sequences of
+// different lengths keep all of the GPU busy; a sequence of more than one run leaves partial sums that fa_rows_merge
+// joins.
+//   stream: up to 16 rows, up to 64 where a row of K has 128 bytes.  Bound by memory: every wave walks 32-key blocks
+//           of its own through LDS that only it uses, two slots of K and V, one filled by DMA while the
+//           other is used; no barrier until the waves' sums are joined at the end.  (bf16, 8 sequences of
+//           32768 keys, 1 token of 32 / 8 heads of 128 columns: 208 us, 5.2 TB/s; one such sequence 31 us.)
 //   shared: more rows.  Eight waves of one or two 16-row tiles share the stages of a ring, two of which are on
 //           their way while one is used, so that K and V cross the L2 once for up to 256 rows.
+//           Bound by vector and matrix instructions in turn and by start-up where runs are short.  (bf16, 8
+//           sequences of up to 16384 keys, 64 tokens of 32 / 8 heads of 128 columns: 169 us, 600 TF/s.)
 // Tiles in LDS have no padding, so that DMA instructions move 1 KiB of whole rows; row r keeps
 // 16-byte chunk x at position x ^ turn(r), which spreads row reads and transposed
 // reads over the banks.
@@ -28,10 +31,11 @@ struct Swizzled {
     static constexpr int CM = CPR < 16 ? CPR : 16;
     static constexpr int RPR = 64 / CPR > 0 ? 64 / CPR : 1;   // rows of a 1 KiB run
     static_assert(CPR <= 64, "a run holds whole rows");
-    // What row `row` adds to its chunk numbers: the same for rows 16 apart.  16-bit types: a transposed read takes two
-    // neighbouring chunks of eight rows in a row at a time, so these get values that differ above the lowest bit; a
-    // row read takes a chunk of rows 0 - 3 and 12 - 15 and the next chunk of rows 4 - 11, so the values 2x and 2x + 1
-    // go to rows r and 15 - r (measured: 520 and 470 bytes/ns a CU; values r alone 510 and 285, 2r | r / 8 290 and 470).
+    // What row `row` adds to its chunk numbers: the same for rows 16 apart.  16-bit types: a transposed read takes
+    // two neighbouring chunks of eight rows in a row at a time, so these get values that differ above the lowest bit;
+    // a row read takes a chunk of rows 0 - 3 and 12 - 15 and the next chunk of rows 4 - 11, so the values 2x and 2x +
+    // 1 go to rows r and 15 - r: no bank conflicts are counted (with r itself the transposed reads reach 285 bytes/ns
+    // a CU instead of 470, with 2r | r / 8 the row reads 290 instead of 510).
     static __device__ __forceinline__ int turn(int row) {
         if constexpr (sizeof(T) == 4) {
             return row % CM;
@@ -858,7 +862,7 @@ __device__ __forceinline__ void rows_shared(const RowsParams& p) {
     if (act) x.store(w, V, rfirst, MT * wave, lane, Special != 0);
 }
 
-// Joins the partial sums of a row, D / 4 lanes a run.  WIDE: a workgroup a row, the runs dealt to
+// Joins the partial sums of a row, D / 4 lanes a run (some 4 us for 512 rows of 9 runs: a launch's time).  WIDE: a workgroup a row, the runs dealt to
 // its groups of lanes, whose sums meet in LDS; else (few runs) a group of lanes a row.
 template <typename T, int D, bool VEC, bool WIDE>
 __device__ __forceinline__ void rows_merge(const RowsParams& p) {

@@ -256,8 +256,8 @@ __device__ __forceinline__ bool tile_clean(T* tile, int tid) {
     return found;
 }
 
-// Adds what tile_clean took out: rows [from, to) of src (a row's address: at(row), nullptr: none) that hold infinities or NaN, to
-// the rows r < n of the wave that see them.  POSITIVE weights: as they are, else as NaN.
+// Adds what tile_clean took out: rows [from, to) of src (a row's address: at(row), nullptr: none) that hold
+// infinities or NaN, to the rows r < n of the wave that see them.  POSITIVE weights: as they are, else as NaN.
 template <typename T, typename O, bool POSITIVE, typename At, typename See, typename Out>
 __device__ __forceinline__ void add_specials(int from, int to, int n, int d, int lane, At at, See see, Out out) {
 #pragma unroll 1

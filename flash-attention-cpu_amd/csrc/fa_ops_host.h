@@ -272,7 +272,8 @@ RowsPlan plan_rows(int dtype, int D, bool vec, size_t batch, size_t kv_heads, si
     share = std::min(share, batch * std::max<size_t>(1, (keys + r.step - 1) / r.step));
     if (batch * units >= 4 * resident) share = 1;   // sequences enough: one run each
     // Few keys: one run each too, which saves the merge, some 4 us, unless walking them costs as much (measured: 8
-    // sequences of 250 keys, bf16, 7 rows of 64 columns 13.1 us split, 9.7 whole; 3 of 250, f32, 8 rows of 80 17.6 and 23.6)
+    // sequences of 250 keys, bf16, 7 rows of 64 columns 13.1 us split, 9.7 whole; 3 of 250, f32, 8 rows of 80 17.6
+    // and 23.6)
     if (keys <= static_cast<size_t>(r.step) * (f32 || D > 128 ? 1 : 4)) share = 1;
     r.share = static_cast<int>(share);
     // each sequence rounds its share up to whole runs; eight runs and heads more or less fall

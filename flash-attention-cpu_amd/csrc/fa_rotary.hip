@@ -6,7 +6,8 @@
 // rotary columns further; else one pair or one copied column), finds the
 // sines and cosines of its pairs once and runs over the heads of all tensors with
 // them.  Angles are position * turns in 64 bits, of which only the fraction
-// goes into sin and cos.
+// goes into sin and cos.  (bf16, 8192 tokens of 32 + 8 heads of 128 columns: 37 us, 4.5 TB/s; f32, 2 x 1000 tokens of
+// 16 + 16 heads of 80 columns, 40 of them rotary: 10 us.)
 
 #include "fa_ops_common.h"
 

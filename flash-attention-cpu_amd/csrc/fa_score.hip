@@ -170,11 +170,14 @@ __device__ __forceinline__ bool key_stage(const ScoreParams& p, int prefix, int 
 // ---------------------------------------------------------------------------
 // Forward
 // ---------------------------------------------------------------------------
-// Four waves of MT 16-row tiles (KG = 2: two groups of two waves keep the same rows, each with half of a
-// stage's keys, and their sums meet in LDS at the end: twice the workgroups, each half as long).  K and V tiles are double-buffered and filled by DMA: while
-// a stage's softmax and PV product run, K of the stage after the next and V of
-// the next arrive; one barrier a stage.  The loop is unrolled by two so that each buffer is
-// an array of its own.
+// Four waves of MT 16-row tiles (KG = 2: two groups of two waves keep the same rows, each with half of a stage's
+// keys, and their sums meet in LDS at the end: twice the workgroups, each half as long).  K and V tiles are
+// double-buffered and filled by DMA: while a stage's softmax and PV product run, K of the stage after the next and V
+// of the next arrive; one barrier a stage.  The loop is unrolled by two so that each buffer is an array of its own.
+//
+// Bound by the issue of vector instructions (five a score, ten with a cap, transcendental ones counted twice) and of
+// products, which overlap little with two waves a SIMD: bf16, 2 x 16 x 4096^2 all visible, 128 columns 281 us
+// (978 TF/s), capped 339 us (810); causal 140 us (980); 64 columns, 4 x 16 x 4096^2 causal 183 us (750).
 template <typename T, int D, int MT, int KG, int MOD, bool VEC>
 __device__ __forceinline__ void score_forward(const ScoreParams& p) {
     using M = Mma<T>;
@@ -524,9 +527,10 @@ __device__ __forceinline__ void weigh(const ScoreParams& p, bool cap, f32x4 s, f
     }
 }
 
-// Operands of the gradient kernels' products that are read from LDS ahead of their use: PRE steps, and the first ones of
-// the column products before the weights are formed (bf16, 2 x 4096 tokens, 16 heads of 128 columns, documents, capped:
-// forward and backward 644 -> 606 us; 16 heads x 2 x 4096^2 all visible, backward 1207 -> 1132; three steps: no more).
+// Operands of the gradient kernels' products that are read from LDS ahead of their use: PRE steps, and the first ones
+// of the column products before the weights are formed (bf16, 2 x 4096 tokens, 16 heads of 128 columns, documents,
+// capped: forward and backward 644 -> 606 us; 16 heads x 2 x 4096^2 all visible, backward 1207 -> 1132; three steps:
+// no more).
 template <typename T>
 constexpr int kAhead = sizeof(T) == 2 ? 2 : 1;
 
@@ -824,6 +828,8 @@ __device__ __forceinline__ void dkv_specials(const ScoreParams& p, Test test, in
 // dK and dV: key rows kept, the queries of every head of the group walked.  Four waves
 // of MT 16-row tiles; Q and dO tiles double-buffered, one barrier a stage.  A kv head's sums over its
 // query heads are formed here, in head order, or by score_dkv_sum where workgroups share them.
+// Bound as the forward kernel, with LDS read at half of its rate besides: bf16, 2 x 16 x 4096^2 all visible, 128
+// columns some 615 us (four products, 890 TF/s), dQ 515 us.
 template <typename T, int D, int MT, int KG, int MOD, bool VEC>
 __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
     using M = Mma<T>;
@@ -842,7 +848,8 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, li = lane & 15;
-    // a workgroup takes heads first .. first + count - 1 of a kv head's group; the first key blocks have most queries where causal
+    // a workgroup takes heads first .. first + count - 1 of a kv head's group; the first key blocks have most queries
+    // where causal
     const Work w = find_work(p.k_order ? blockIdx.x : gridDim.x - 1 - blockIdx.x, p.nqb, p.batch * p.kv_heads, p.splits,
                              p.kv_heads, p.k_order);
     const int count = p.group / p.splits, first = w.hk * p.group + w.hq * count;
