@@ -1178,17 +1178,15 @@ extern "C" __global__ __launch_bounds__(1024) void fa_score_doc_order(ScoreParam
         const int prefix = p.prefix ? load_uniform(p.prefix + b) : 0;
         const DocRange x = {kept[i].x, kept[i].y, padded[i] != 0};
         int count = 0;
+#pragma unroll 4
         for (int t0 = 0; t0 < wt; t0 += 64) {
             const int t = t0 + lane, w0 = t * kDocTile;
-            bool v = t < wt;
-            if (v) {
-                const int lo = walked[b * wt + t].x;
-                bool part;
-                v = docs_meet(x, DocRange{lo < 0 ? ~lo : lo, walked[b * wt + t].y, lo < 0}, &part);
-                if (p.causal) {
-                    const int last = isq ? r1 : min(w0 + kDocTile, p.sq), first = isq ? w0 : r0;   // query, key
-                    v = v && (first <= p.q_start + last - 1 || first < prefix);
-                }
+            const int2 y = walked[b * wt + min(t, wt - 1)];
+            bool part;
+            bool v = t < wt && docs_meet(x, DocRange{y.x < 0 ? ~y.x : y.x, y.y, y.x < 0}, &part);
+            if (p.causal) {
+                const int last = isq ? r1 : min(w0 + kDocTile, p.sq), first = isq ? w0 : r0;   // query, key
+                v = v && (first <= p.q_start + last - 1 || first < prefix);
             }
             count += __builtin_popcountll(__builtin_amdgcn_ballot_w64(v));
         }
