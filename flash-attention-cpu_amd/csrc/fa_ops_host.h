@@ -324,9 +324,11 @@ int run_rows(int dev, hipStream_t stream, int dtype, int D, bool vec, RowsParams
 bool score_takes_rows(const fa_score_config& c, int num_cus) {
     const size_t group = c.heads / c.kv_heads;
     if (c.seq_len_q * group <= 64) return true;
-    // a workgroup of 32 rows takes some 0.6 us per 64 keys: above 2048 keys longer than the split and its merge
+    // a workgroup of 32 rows takes some 0.6 us per 64 keys: above 2048 keys longer than the split and its merge, at
+    // 256 columns above 1024 (1 head, 1900^2 causal: bf16 53 us whole, 35 split, f32 277 and 97; 2 heads of 128
+    // columns, 1500^2: bf16 21 and 30, f32 72 and 78)
     const size_t blocks = c.batch * c.heads * ((c.seq_len_q + 31) / 32);
-    return c.seq_len_k >= 2048 && 2 * blocks <= static_cast<size_t>(num_cus);
+    return c.seq_len_k >= (c.d_head > 128 ? 1024 : 2048) && 2 * blocks <= static_cast<size_t>(num_cus);
 }
 
 int check_score(const fa_score_config* c) {

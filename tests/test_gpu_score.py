@@ -535,3 +535,9 @@ def test_two_graphs_and_eager_calls_at_once():
         for c, f in zip(cases, first):
             for n, x in c.outs.items():
                 assert torch.equal(x, f[n]), n
+
+
+@pytest.mark.parametrize("dtype", ("f32", "bf16", "f16"))
+def test_wide_blocks_of_rows_that_share_a_range(dtype):
+    """256 columns: keys are split from 1024 on; the gradients take the forward pass's lse."""
+    Call(dtype, 1, 2, 2, 150, 1100, 256, causal=True, q_start=950, seed=34).run_and_check()
