@@ -886,6 +886,7 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
     auto test = [&](int st, bool* part) -> bool {
         const int q0 = st * SQ, q1 = min(q0 + SQ, p.sq);
         bool v = true;
+        if (q0 + SQ > p.sq) *part = true;
         if (p.causal) {
             v = p.q_start + q1 - 1 >= kbeg || kbeg < prefix;
             if (!(p.q_start + q0 >= kend - 1 || kend <= prefix)) *part = true;
@@ -924,6 +925,12 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
             if (wave == 2 && docs) fill_words(words + 128, qdoc + q0, p.sq - q0, lane);
         }
     };
+    // Rows past the last query arrive as zeros.  With an lse2 of 0 their weight would be e^bias, which overflows with
+    // negative slopes, and times the zeros of Q and dO that is NaN; so they get that of empty rows.  By the wave whose
+    // DMA it was, once that has arrived.
+    auto end_rows = [&](int st, int* words) {
+        if (wave == 0 && lane < SQ && st * SQ + lane >= p.sq) words[lane] = 0x7f800000;
+    };
     auto active = [&](int st) -> int {
         if (key0 >= p.sk) return false;
         return st * SQ + qoff < p.sq && (!p.causal || p.q_start + st * SQ + qoff + 32 * NCH - 1 >= key0 || key0 < prefix);
@@ -934,6 +941,7 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
     if (tid < 3) Special[tid] = 0;
     if (st >= 0) fill(hq, st, Qb0, Ob0, Wb0);
     wait_loads();
+    if (st >= 0) end_rows(st, Wb0);
     __syncthreads();
     auto special = [&](T* q, T* o) {
         const bool found = qfill.template special<false>(q);
@@ -1038,7 +1046,10 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
             }
         }
         wait_loads();
-        if (nx >= 0 && masked_next && special(P ? Qb0 : Qb1, P ? Ob0 : Ob1)) Special[2 - P] = 1;
+        if (nx >= 0 && masked_next) {
+            end_rows(nx, P ? Wb0 : Wb1);
+            if (special(P ? Qb0 : Qb1, P ? Ob0 : Ob1)) Special[2 - P] = 1;
+        }
         if (dirty && tid == 0) Special[1 + P] = 0;
         __syncthreads();
         st = nx, hq = hnx, masked = masked_next;
