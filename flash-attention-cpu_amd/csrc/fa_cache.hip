@@ -178,14 +178,12 @@ struct RowSource {
         }
         return bad;
     }
-    // the same element by element: any alignment, any page size.  Returns whether the thread met a bad page.
-    __device__ __forceinline__ bool fill_slow(T* dst, int k0, int end, const CachePages& c, int d, int tid) const {
-        bool bad = false;
+    // the same element by element: any alignment, any page size
+    __device__ __forceinline__ void fill_slow(T* dst, int k0, int end, const CachePages& c, int d, int tid) const {
 #pragma unroll 1
         for (int pos = tid; pos < ROWS * (D / 8); pos += 64 * NW) {
             const int r = pos / (D / 8), col = 8 * (pos % (D / 8));
             const int64_t at = c.at(k0 + r, end, seq, batch);
-            bad = bad || (at < 0 && k0 + r < end);
             const typename Mma<T>::v8 x = global_row<T, false>(base + (at < 0 ? 0 : at), 0, 0, at >= 0, col, d);
             if constexpr (sizeof(T) == 2) {
                 *reinterpret_cast<typename Mma<T>::v8*>(dst + S::at(r, col)) = x;
@@ -194,7 +192,13 @@ struct RowSource {
                 *reinterpret_cast<f32x4*>(dst + S::at(r, col + 4)) = __builtin_shufflevector(x, x, 4, 5, 6, 7);
             }
         }
-        return bad;
+    }
+    // Whether a row of [k0, k0 + ROWS) before `end` lies in a bad page, a lane a row: what look_up returns, for any page
+    // size.  Every wave looks for itself, so all come to the same answer.
+    static __device__ __forceinline__ int bad_rows(const CachePages& c, int k0, int end, int lane) {
+        static_assert(ROWS <= 64, "a lane a row");
+        if (!c.table) return 0;
+        return __builtin_amdgcn_ballot_w64(lane < ROWS && k0 + lane < end && c.at(k0 + lane, end, 0, 0) < 0) != 0;
     }
 };
 
@@ -772,7 +776,7 @@ __device__ __forceinline__ void rows_shared(const RowsParams& p) {
     constexpr int THIRD = (RING > 2) ? TILE : 8;
     T* const K2 = (RING > 2) ? lds_array<T, THIRD, 4>() : K0;
     T* const V2 = (RING > 2) ? lds_array<T, THIRD, 5>() : V0;
-    __shared__ int bad_any, Special;
+    __shared__ int Special;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     RowsWork w;
@@ -801,7 +805,7 @@ __device__ __forceinline__ void rows_shared(const RowsParams& p) {
             vsrc.fill(v, k0, end, page, pages, wave);
             look_up(st + 1);
         } else if (k0 < w.kend) {
-            if (ksrc.fill_slow(k, k0, w.kend, pages, p.d, tid)) bad_any = 1;
+            ksrc.fill_slow(k, k0, w.kend, pages, p.d, tid);
             vsrc.fill_slow(v, k0, w.kend, pages, p.d, tid);
         }
         return bad;
@@ -817,7 +821,7 @@ __device__ __forceinline__ void rows_shared(const RowsParams& p) {
             __syncthreads();
         }
     };
-    if (tid == 0) bad_any = Special = 0;
+    if (tid == 0) Special = 0;
     R x;
     x.init(p, w, rfirst, lane);
     __syncthreads();
@@ -826,12 +830,13 @@ __device__ __forceinline__ void rows_shared(const RowsParams& p) {
     bad_now = fill(0, K0, V0);
     if (RING > 2) bad_1 = fill(1, K1, V1);
     auto step = [&](int st, T* k, T* v, T* kn, T* vn) {
+        const int k0 = w.kbeg + st * SK;
+        // the same on all waves: a barrier hangs on it
+        const int bad = VEC ? bad_now : Src::bad_rows(pages, k0, w.kend, lane);
         arrive(std::integral_constant<int, (RING - 2) * 2 * Src::NI>{});
         const int filled = fill(st + RING - 1, kn, vn);
         if (RING > 2) bad_2 = filled;
         else bad_1 = filled;
-        const int k0 = w.kbeg + st * SK;
-        const int bad = VEC ? bad_now : __builtin_amdgcn_readfirstlane(bad_any);
         const int masked = bad || k0 + SK > min(w.open, w.kend);
         if (act) {
             x.scores(p, w, k, k0, masked, bad);
