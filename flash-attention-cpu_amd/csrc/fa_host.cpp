@@ -92,9 +92,11 @@ struct DeviceState {
         void* cap_ptr = nullptr;      // the buffer that the capture cap_id took over (one of the retired)
         size_t cap_bytes = 0;
         unsigned long long cap_id = 0;
+        std::shared_ptr<std::mutex> call = std::make_shared<std::mutex>();   // WorkspaceCall
     };
     std::mutex ws_mu;
     std::unordered_map<std::string, Workspace> ws;   // freed by fa_release_stream_workspace
+    std::mutex scratch_call;   // as Workspace::call, for the one scratch array of the allocation-free calls
     // Host-slice calls: up to kIoContexts contexts, created as concurrent
     // callers need them and kept; a caller takes a free one for its call.
     std::mutex io_mu;
@@ -1011,6 +1013,34 @@ std::string workspace_key(hipStream_t stream) {
     return key;
 }
 
+// A call of several kernels that meet in the stream's workspace: held from before the buffer is
+// fetched until the call's last launch is queued, so that another thread's call on the same stream
+// comes wholly before or after it and not between its kernels.
+class WorkspaceCall {
+public:
+    WorkspaceCall() = default;
+    WorkspaceCall(int dev, hipStream_t stream) {
+        DeviceState& s = g_dev[dev];
+        const std::string key = workspace_key(stream);
+        for (;;) {
+            {
+                std::lock_guard<std::mutex> lock(s.ws_mu);
+                mu_ = s.ws[key].call;
+            }
+            lock_ = std::unique_lock<std::mutex>(*mu_);
+            // the entry may have been released, and made anew by another thread, meanwhile
+            std::lock_guard<std::mutex> lock(s.ws_mu);
+            auto it = s.ws.find(key);
+            if (it != s.ws.end() && it->second.call == mu_) return;
+            lock_.unlock();
+        }
+    }
+
+private:
+    std::shared_ptr<std::mutex> mu_;   // before lock_, which is gone first
+    std::unique_lock<std::mutex> lock_;
+};
+
 // Device memory free right now (0 when the query fails).
 size_t free_device_bytes() {
     size_t free_b = 0, total_b = 0;
@@ -1107,7 +1137,10 @@ int run_device(int variant, hipStream_t stream, const void* q, const void* k, co
     const size_t bytes = plan.ws_floats * sizeof(float);
     float* ws = nullptr;
     const bool cached = noalloc || bytes <= kWorkspaceCacheMax;
+    const WorkspaceCall call = cached && !noalloc ? WorkspaceCall(dev, stream) : WorkspaceCall();
+    std::unique_lock<std::mutex> scratch_call(g_dev[dev].scratch_call, std::defer_lock);
     if (noalloc) {
+        scratch_call.lock();
         ws = static_cast<float*>(fa_scratch_ptr(dev));
         if (!ws || bytes > FA_SCRATCH_BYTES) return FA_ERR_SCRATCH;
     } else if (cached) {
@@ -1575,11 +1608,13 @@ int fa_release_stream_workspace(void* stream) {
     if (rc != FA_OK) return rc;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     DeviceState& s = g_dev[dev];
-    // Take the stream's buffers out of the table under the lock, then drain
-    // the stream and free them without it, so split calls on other streams
-    // of this device do not wait for this stream.
+    // Take the stream's buffers out of the table under the lock, once no call
+    // is between its launches, then drain the stream and free them without
+    // it, so split calls on other streams of this device do not wait for this
+    // stream.
     std::vector<void*> bufs;
     {
+        const WorkspaceCall call(dev, st);
         std::lock_guard<std::mutex> lock(s.ws_mu);
         auto it = s.ws.find(workspace_key(st));
         if (it == s.ws.end()) return FA_OK;

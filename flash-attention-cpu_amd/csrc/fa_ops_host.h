@@ -89,12 +89,17 @@ int ops_begin(int* dev, OpsModule which) {
     return rc;
 }
 
-// A call's scratch memory: the stream's workspace, or an allocation around the call above its limit.
+// A call's scratch memory: the stream's workspace, which is the call's until this object goes, or an
+// allocation around the call above its limit.
 struct OpsWorkspace {
     void* ptr = nullptr;
     bool own = false;
+    WorkspaceCall call;
     int get(int dev, hipStream_t stream, size_t bytes) {
-        if (bytes <= kWorkspaceCacheMax) return stream_workspace(dev, stream, bytes, &ptr);
+        if (bytes <= kWorkspaceCacheMax) {
+            call = WorkspaceCall(dev, stream);
+            return stream_workspace(dev, stream, bytes, &ptr);
+        }
         if (bytes > free_device_bytes() || hipMallocAsync(&ptr, bytes, stream) != hipSuccess) {
             (void)hipGetLastError();
             return FA_ERR_ALLOC;

@@ -20,6 +20,8 @@
  * once (the crate's functions are Sync).  Up to four host-slice calls per
  * device run concurrently, each on its own stream, device staging buffer and
  * pinned copy ring; further callers wait until one of those four finishes.
+ * Calls that several threads make on one stream are queued one after the
+ * other, all kernels of one before those of the next.
  */
 #ifndef FA_HIP_H
 #define FA_HIP_H

@@ -5,9 +5,12 @@ Bounds: tests/ops_reference.py.
 """
 from __future__ import annotations
 
+import threading
+
 import pytest
 import torch
 
+from test_gpu_rotary_tree import Tree
 from test_gpu_score import Call, check_batch, doc_ids
 
 pytestmark = pytest.mark.gpu
@@ -41,3 +44,39 @@ def test_negative_slopes_with_documents_and_many_blocks(dtype):
     c.backward()
     torch.cuda.synchronize()
     check_batch(c, 6)
+
+
+def test_threads_that_share_a_stream():
+    """Calls of several kernels from three threads on one stream: each gets what it gets alone."""
+    ids = [doc_ids(4, 600, x) for x in (([200, 400], [500, 90]), ([64, 300], [7, 580]))]
+    train = [Call("bf16", 4, 64, 8, 600, 600, 64, causal=True, q_doc=x, k_doc=x, seed=s) for s, x in zip((3, 4), ids)]
+    tree = Tree("bf16", [3000, 1700], 8, 2, 4, 64, seed=5)
+
+    def step(c):
+        if c is tree:
+            c.run()
+        else:
+            c.forward()
+            c.backward()
+
+    def results(c):
+        return [c.out, c.lse] if c is tree else [*c.outs.values(), c.lse]
+
+    cases = train + [tree]
+    for c in cases:
+        step(c)
+    torch.cuda.synchronize()
+    alone = [[x.clone() for x in results(c)] for c in cases]
+    for c in cases:
+        for x in results(c):
+            x.fill_(7.0)
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=lambda c=c: [step(c) for _ in range(20)]) for c in cases]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for c, want in zip(cases, alone):
+        for x, y in zip(results(c), want):
+            assert torch.equal(x, y)
