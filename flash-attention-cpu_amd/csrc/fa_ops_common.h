@@ -17,6 +17,8 @@
 
 #include "fa_ops_params.h"
 
+extern "C" __global__ void OPS_STAMP_KERNEL() {}
+
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));

@@ -23,6 +23,10 @@ struct OpsState {
 
 OpsState g_ops[kMaxDevices];
 
+#define OPS_STRING_(x) #x
+#define OPS_STRING(x) OPS_STRING_(x)
+constexpr char kStampKernel[] = OPS_STRING(OPS_STAMP_KERNEL);
+
 constexpr size_t kOpsMaxSeq = size_t(1) << 30;      // tokens: positions and their sums stay in 32 bits
 constexpr size_t kOpsMaxD = 256;
 constexpr int64_t kOpsMaxRowStride = int64_t(1) << 22;   // elements: a tile's byte offsets stay in 32 bits
@@ -42,7 +46,9 @@ int ops_module(int dev, OpsModule which) {
         path = (pos == std::string::npos ? std::string() : path.substr(0, pos + 1)) + files[which];
         FILE* f = std::fopen(path.c_str(), "rb");
         if (f) std::fclose(f);
-        if (!f || hipModuleLoad(&s.module[which], path.c_str()) != hipSuccess) {
+        hipFunction_t of_this_build;
+        if (!f || hipModuleLoad(&s.module[which], path.c_str()) != hipSuccess ||
+            hipModuleGetFunction(&of_this_build, s.module[which], kStampKernel) != hipSuccess) {
             (void)hipGetLastError();
             s.status[which] = FA_ERR_MODULE;
         }

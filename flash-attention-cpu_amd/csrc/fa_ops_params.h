@@ -6,6 +6,15 @@
 
 #include <stdint.h>
 
+// Every code object of the operators holds an (empty) kernel of this name: fa_ops_params_ and the build's stamp of this
+// file.  The host loads none that lacks it, since kernels of other parameter blocks would read pointers from wrong places.
+#ifndef OPS_STAMP
+#define OPS_STAMP none
+#endif
+#define OPS_PASTE2_(a, b) a##b
+#define OPS_PASTE2(a, b) OPS_PASTE2_(a, b)
+#define OPS_STAMP_KERNEL OPS_PASTE2(fa_ops_params_, OPS_STAMP)
+
 // Element strides between batches, tokens and heads.
 struct OpsStrides {
     int64_t b, s, h;

@@ -45,7 +45,8 @@ extern "C" {
                                  size beyond 32-bit row indexing (f32 heads of any width run the
                                  flash kernels) */
 #define FA_ERR_NO_DEVICE 7    /* no HIP device visible */
-#define FA_ERR_MODULE 8       /* code object missing / unloadable (FA_HIP_MODULE) */
+#define FA_ERR_MODULE 8       /* code object missing / unloadable (FA_HIP_MODULE), or an operator's
+                                 that another build of the library made */
 #define FA_ERR_ALLOC 9        /* device allocation failed, or the request exceeds the free
                                  device memory (checked before anything is queued) */
 #define FA_ERR_LAUNCH 10      /* kernel launch failed */
