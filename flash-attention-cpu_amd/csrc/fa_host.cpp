@@ -1058,7 +1058,14 @@ size_t free_device_bytes() {
 // next eager call on the stream gets a new one.  So replays of the graph --
 // on any stream -- never share partials with later eager calls on the
 // capture stream, nor with another graph captured there.
-int stream_workspace(int dev, hipStream_t stream, size_t bytes, void** out) {
+//
+// Buffers are whole units of 2 MiB, in which the driver hands memory out, and one unit larger than
+// the call needs: partials that grow a little from step to step keep their buffer, and the free
+// memory that the driver reports falls by the call's need at least (it counts units, and some
+// units short: of 20 allocations of 50 MiB one is seen as 48).
+constexpr size_t kWorkspaceUnit = size_t(2) << 20;
+int stream_workspace(int dev, hipStream_t stream, size_t need, void** out) {
+    const size_t bytes = (need + kWorkspaceUnit - 1) / kWorkspaceUnit * kWorkspaceUnit + kWorkspaceUnit;
     DeviceState& s = g_dev[dev];
     const std::string key = workspace_key(stream);
     hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
@@ -1071,12 +1078,12 @@ int stream_workspace(int dev, hipStream_t stream, size_t bytes, void** out) {
     std::lock_guard<std::mutex> lock(s.ws_mu);
     DeviceState::Workspace& w = s.ws[key];
     if (capturing) {
-        if (w.cap_ptr && w.cap_id == id && w.cap_bytes >= bytes) {   // a later call of the same capture
+        if (w.cap_ptr && w.cap_id == id && w.cap_bytes >= need) {   // a later call of the same capture
             *out = w.cap_ptr;
             return FA_OK;
         }
         void* ptr = nullptr;
-        if (w.ptr && w.bytes >= bytes) {
+        if (w.ptr && w.bytes >= need) {
             ptr = w.ptr;
             w.cap_bytes = w.bytes;
             w.ptr = nullptr;
@@ -1099,11 +1106,11 @@ int stream_workspace(int dev, hipStream_t stream, size_t bytes, void** out) {
         *out = ptr;
         return FA_OK;
     }
-    if (w.ptr && w.bytes >= bytes) {
+    if (w.ptr && w.bytes >= need) {
         *out = w.ptr;
         return FA_OK;
     }
-    const size_t want = std::max({bytes, 2 * w.bytes, size_t(1) << 20});
+    const size_t want = std::max(bytes, 2 * w.bytes);
     void* ptr = nullptr;
     if (hipMalloc(&ptr, want) != hipSuccess) {
         (void)hipGetLastError();

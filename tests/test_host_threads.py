@@ -100,3 +100,35 @@ def test_kernels_of_a_call_are_queued_together(program, kinds, per):
     r = subprocess.run([exe, *map(str, kinds)], capture_output=True, text=True, env=env, timeout=120)
     assert r.returncode == 0, (r.returncode, r.stdout, r.stderr)
     assert r.stdout.startswith(f"{200 * sum(per)} launches of {200 * len(kinds)} calls, apart 0"), r.stdout
+
+
+SIZES = r"""
+int main() {
+    static char mem[64] __attribute__((aligned(64)));
+    float* const f = reinterpret_cast<float*>(mem);
+    char text[256];
+    int i = 0;
+    for (size_t sk : {3000, 20000, 100000, 1000000}) {   // each on a stream of its own, twice
+        if (fa_describe_launch(2, 1, 16, 1, sk, 128, 0, nullptr, text, sizeof(text)) != FA_OK) return 2;
+        ++i;
+        for (int n = 0; n < 2; ++n)
+            if (fa_device_ex(2, reinterpret_cast<hipStream_t>(mem + i), f, f, f, 1, 16, 1, sk, 128, nullptr, nullptr, f) !=
+                FA_OK)
+                return 2;
+        std::printf("%zu %s\n", stub::allocations.back(), std::strstr(text, "workspace=") + 10);
+    }
+    std::printf("%zu allocations\n", stub::allocations.size());
+    return 0;
+}
+"""
+
+
+def test_workspaces_are_whole_units_and_one_more_than_needed(tmp_path):
+    """Units of 2 MiB, in which free memory is reported."""
+    exe, env = compile_with_stub(tmp_path, SIZES)
+    out = subprocess.run([exe], capture_output=True, text=True, env=env, check=True, timeout=60).stdout.splitlines()
+    unit = 2 << 20
+    for line in out[:-1]:
+        size, need = (int(x) for x in line.split()[:2])
+        assert size % unit == 0 and need + unit <= size < need + 2 * unit, line
+    assert out[-1] == "4 allocations"
