@@ -534,6 +534,61 @@ __device__ __forceinline__ void weigh(const ScoreParams& p, bool cap, f32x4 s, f
 template <typename T>
 constexpr int kAhead = sizeof(T) == 2 ? 2 : 1;
 
+// f16: weights p and score gradients enter their products 2^kGradLog2 times larger, so that those down to 2^-26 round as
+// normal numbers (gradients of a mean over many tokens are that small): p by an lse2 that is smaller by kGradLog2,
+// and the gradients with it.  Gradients that would then pass the type's range are scaled down, each kept row's by itself,
+// with its sums so far: GradScale.  Looking for them takes a vector instruction a score (backward, f16, 2 x 16 x 4096^2:
+// 128 columns, all visible 1142 us without, 1175 with it; 64 columns, 4 kv heads, causal 382 and 407).
+template <typename T>
+constexpr float kGradLog2 = std::is_same<T, _Float16>::value ? 12.0f : 0.0f;
+template <typename T>
+constexpr float kGradInv = std::is_same<T, _Float16>::value ? 0x1p-12f : 1.0f;
+
+// What a kept row's score gradients are scaled down by, a power of two u (1 where T has the range of f32).
+template <typename T, int D, int MT>
+struct GradScale {
+    static constexpr bool kOn = std::is_same<T, _Float16>::value;
+    float limit[MT];   // 2^15 / u: larger ones are brought down
+    int any = 0;       // some row's u is not 1
+    __device__ __forceinline__ GradScale() {
+#pragma unroll
+        for (int t = 0; t < MT; ++t) limit[t] = 0x1p15f;
+    }
+    // Brings the gradients of two blocks of rows into range; where they pass it, down to 2^13 .. 2^14 with the sums.
+    template <int N>
+    __device__ __forceinline__ void fit(int t, f32x4 (&y)[2], f32x4 (&sums)[N]) {
+        if constexpr (kOn) {
+            float mx = 0.0f;
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) mx = fmaxf(mx, fabsf(y[b][r]));
+            // (at 256 columns, where registers are short, dQ takes 170 us without these two hints and the second
+            // branch, which spares a product a score, and 192 with them)
+            constexpr bool kShort = D > 128;
+            const bool pass = __builtin_amdgcn_ballot_w64(mx > limit[t]) != 0;
+            if (kShort ? pass : __builtin_expect(pass, 0)) {
+                any = 1;
+                mx = row4_max(mx);
+                if (mx > limit[t] && !not_finite(mx)) {
+                    // 2^15 / u from the exponent of mx, and its inverse
+                    const unsigned larger = (min(__float_as_uint(mx) >> 23, 250u) + 2) << 23;
+                    const float by = limit[t] * __uint_as_float((254u << 23) - larger);
+                    limit[t] = __uint_as_float(larger);
+#pragma unroll
+                    for (int j = 0; j < N; ++j) sums[j] *= by;
+                }
+            }
+            if (kShort || __builtin_expect(any, 0)) {
+                const float u = __uint_as_float(((254u + 15u) << 23) - __float_as_uint(limit[t]));   // 2^15 / limit
+                y[0] *= u;
+                y[1] *= u;
+            }
+        }
+    }
+    __device__ __forceinline__ float inverse(int t) const { return kOn ? limit[t] * 0x1p-15f : 1.0f; }
+};
+
 // dQ: query rows kept, keys walked.  Four waves of MT 16-row tiles; K and V tiles double-buffered, one barrier a stage.
 // On the way in a wave leaves delta = dO . O and lse2 = lse log2(e) of its rows for the dK / dV kernel.  Empty rows get
 // lse2 = +inf: their weights e^(z - lse) then come out as 0.
@@ -582,6 +637,7 @@ __device__ __forceinline__ void score_dq(const ScoreParams& p) {
     int qd[MT], limit[MT];
     f32x4 dq[MT][NDB], pk[MT][kRefine ? NDB : 1];
     float lse2[MT], delta[MT], err[MT];
+    GradScale<T, D, MT> down;
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
         const int row = row0 + 16 * t + li;
@@ -602,7 +658,9 @@ __device__ __forceinline__ void score_dq(const ScoreParams& p) {
         }
         delta[t] = row4_sum(sum);
         const float lse = row < p.sq ? p.lse_in[at] : OPS_NEG_INF;
-        lse2[t] = lse == OPS_NEG_INF ? -OPS_NEG_INF : lse == -OPS_NEG_INF ? __builtin_nanf("") : lse * kLog2e;
+        lse2[t] = lse == OPS_NEG_INF    ? -OPS_NEG_INF
+                  : lse == -OPS_NEG_INF ? __builtin_nanf("")
+                                        : lse * kLog2e - kGradLog2<T>;
         if (row < p.sq && g == 0 && kg == 0) {
             p.lse2[at] = lse2[t];
             p.delta[at] = delta[t];
@@ -690,32 +748,39 @@ __device__ __forceinline__ void score_dq(const ScoreParams& p) {
 #pragma unroll
                 for (int t = 0; t < MT; ++t) {
                     const int pos = p.q_start + row0 + 16 * t + li;
+                    f32x4 x[2], y[2];   // y: gradients of the raw scores
 #pragma unroll
                     for (int b = 0; b < 2; ++b) {
-                        f32x4 x, y, f;
+                        f32x4 f;
                         const int key = k0 + koff + 32 * i + 16 * b + 4 * g;
                         weigh<T, MOD>(p, cap, s[t][b], dp[t][b], (f32x4){lse2[t], lse2[t], lse2[t], lse2[t]},
-                                      (f32x4){delta[t], delta[t], delta[t], delta[t]}, slope, (float)(pos - key), &x, &y, &f);
+                                      (f32x4){delta[t], delta[t], delta[t], delta[t]}, slope, (float)(pos - key), &x[b],
+                                      &y[b], &f);
                         if (masked) {
                             if (docs) {
                                 const i32x4 kd = *reinterpret_cast<const i32x4*>(ids + koff + 32 * i + 16 * b + 4 * g);
 #pragma unroll
                                 for (int r = 0; r < 4; ++r)
-                                    if (kd[r] != qd[t]) x[r] = y[r] = 0.0f;
+                                    if (kd[r] != qd[t]) x[b][r] = y[b][r] = 0.0f;
                             }
 #pragma unroll
                             for (int r = 0; r < 4; ++r)
-                                if (key + r >= limit[t]) x[r] = y[r] = 0.0f;
+                                if (key + r >= limit[t]) x[b][r] = y[b][r] = 0.0f;
                         }
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
-                            db[t][4 * b + r] = T(y[r] * f[r]);
                             if (kRefine) {
-                                pb[t][4 * b + r] = T(x[r] * f[r]);
-                                err[t] += y[r];
+                                pb[t][4 * b + r] = T(x[b][r] * f[r]);
+                                err[t] += y[b][r];
                             }
+                            y[b][r] *= f[r];
                         }
                     }
+                    down.fit(t, y, dq[t]);
+#pragma unroll
+                    for (int b = 0; b < 2; ++b)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) db[t][4 * b + r] = T(y[b][r]);
                 }
             }
             if (dirty) {   // the row products took K as it is, the column products may not
@@ -749,6 +814,18 @@ __device__ __forceinline__ void score_dq(const ScoreParams& p) {
         step(std::integral_constant<int, 1>{});
     }
     const ScoreParams lp = late_params<ScoreParams>();
+    if constexpr (down.kOn) {
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            const float by = down.inverse(t) * kGradInv<T>;
+            err[t] *= kGradInv<T>;
+#pragma unroll
+            for (int j = 0; j < NDB; ++j) {
+                dq[t][j] *= by;
+                pk[t][j] *= kGradInv<T>;
+            }
+        }
+    }
     if constexpr (KG > 1) {
         static_assert(MT == 1 && KG == 2 && NCH == 1 && NR * NDB * 64 * 16 <= Fill::SIZE * (int)sizeof(T), "sums fit a tile");
         f32x4* const sums = reinterpret_cast<f32x4*>(Kb0) + wave % NR * NDB * 64;
@@ -863,6 +940,7 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
 
     v8 kreg[MT][NDC], vreg[MT][NDC];
     f32x4 dk[MT][NDB], dv[MT][NDB];
+    GradScale<T, D, MT> down;
     int kd[MT];
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
@@ -996,6 +1074,7 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
                     __builtin_amdgcn_sched_barrier(0);
                 }
                 if (!dirty) preload(i);
+                f32x4 ds[MT][2];   // gradients of the raw scores
 #pragma unroll
                 for (int b = 0; b < 2; ++b) {
                     const int at = qoff + 32 * i + 16 * b + 4 * g, pos = p.q_start + q0 + at;
@@ -1004,25 +1083,33 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
 #pragma unroll
                     for (int t = 0; t < MT; ++t) {
                         const int key = key0 + 16 * t + li;
-                        f32x4 x, ds, f;
-                        weigh<T, MOD>(p, cap, s[t][b], dp[t][b], lse2, delta, slope, (float)(key - pos), &x, &ds, &f);
+                        f32x4 x, y, f;
+                        weigh<T, MOD>(p, cap, s[t][b], dp[t][b], lse2, delta, slope, (float)(key - pos), &x, &y, &f);
                         if (masked) {
                             if (docs) {
                                 const i32x4 qd = *reinterpret_cast<const i32x4*>(words + 128 + at);
 #pragma unroll
                                 for (int r = 0; r < 4; ++r)
-                                    if (qd[r] != kd[t] || kd[t] < 0) x[r] = ds[r] = 0.0f;
+                                    if (qd[r] != kd[t] || kd[t] < 0) x[r] = y[r] = 0.0f;
                             }
 #pragma unroll
                             for (int r = 0; r < 4; ++r)
-                                if (key >= key_limit(p, prefix, pos + r) || lse2[r] == -OPS_NEG_INF) x[r] = ds[r] = 0.0f;
+                                if (key >= key_limit(p, prefix, pos + r) || lse2[r] == -OPS_NEG_INF) x[r] = y[r] = 0.0f;
                         }
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
                             pb[t][0][4 * b + r] = T(x[r]);
-                            db[t][0][4 * b + r] = T(ds[r] * f[r]);
+                            ds[t][b][r] = y[r] * f[r];
                         }
                     }
+                }
+#pragma unroll
+                for (int t = 0; t < MT; ++t) {
+                    down.fit(t, ds[t], dk[t]);
+#pragma unroll
+                    for (int b = 0; b < 2; ++b)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) db[t][0][4 * b + r] = T(ds[t][b][r]);
                 }
             }
             if (dirty) {
@@ -1060,6 +1147,17 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
         step(std::integral_constant<int, 1>{});
     }
     const ScoreParams lp = late_params<ScoreParams>();
+    if constexpr (down.kOn) {
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            const float by = down.inverse(t) * kGradInv<T>;
+#pragma unroll
+            for (int j = 0; j < NDB; ++j) {
+                dk[t][j] *= by;
+                dv[t][j] *= kGradInv<T>;
+            }
+        }
+    }
     if constexpr (KG > 1) {
         static_assert(MT == 1 && KG == 2 && NCH == 1 && NR * NDB * 64 * 16 <= Fill::SIZE * (int)sizeof(T), "sums fit a tile");
         f32x4* const ksum = reinterpret_cast<f32x4*>(Qb0) + wave % NR * NDB * 64;

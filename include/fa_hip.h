@@ -269,7 +269,9 @@ int fa_multihead_lp(int dtype, const void* q, size_t q_len, const void* k, size_
  * heads is a multiple of kv_heads: query head h reads key / value head
  * h / (heads / kv_heads).  Q, K, V, O and all gradients have the type `dtype`
  * (products accumulate in f32; 16-bit inputs: probabilities and score
- * gradients are rounded to the type for the products they enter).  slopes, prefix
+ * gradients are rounded to the type for the products they enter, f16 ones
+ * scaled by powers of two so that neither small nor large ones leave the
+ * type's range there).  slopes, prefix
  * and lse are f32 / int32 / f32 whatever the type.  d_head <= 256.
  *
  * Layouts: element strides between batches, tokens and heads, columns next to

@@ -10,8 +10,9 @@ import threading
 import pytest
 import torch
 
+from ops_reference import attend, check, round_bound
 from test_gpu_rotary_tree import Tree
-from test_gpu_score import Call, check_batch, doc_ids
+from test_gpu_score import Call, check_batch, doc_ids, to_gpu
 
 pytestmark = pytest.mark.gpu
 
@@ -80,3 +81,97 @@ def test_threads_that_share_a_stream():
     for c, want in zip(cases, alone):
         for x, y in zip(results(c), want):
             assert torch.equal(x, y)
+
+
+def f16_gradients(c):
+    """Gradients of a call in f16 and their bounds, as ops_reference.attend has them, but for the absolute part of the
+    roundings of weights and score gradients.  There it is 2^-25, half a step of the smallest numbers of f16.  Weights are
+    taken 2^12 larger: 2^-37.  Score gradients too, and where the largest of a kept row (a query's for dQ, a key's for
+    dK) would pass 2^15 so, all of that row are brought down with it to 2^13 at least: 2^-25 times max / 2^13."""
+    b, h = c.q.shape[:2]
+    sums = {"dq": [], "dk": [], "dv": []}
+    for i in range(b):
+        rows = {n: [] for n in sums}
+        for j in range(h):
+            k, v, q, do = c.k[i, j // c.group], c.v[i, j // c.group], c.q[i, j].double(), c.dout[i, j].double()
+            see = c.see[i].double()
+            r = attend(c.q[i, j], k, v, c.see[i], c.scale, c.cap, c.bias[j], c.t, c.dout[i, j])
+            x = q @ k.double().T * c.scale
+            t = torch.tanh(x / c.cap) if c.cap else torch.zeros_like(x)
+            z = (c.cap * t if c.cap else x) + (0 if c.bias[j] is None else c.bias[j])
+            p = torch.softmax(z.masked_fill(~c.see[i], float("-inf")), 1).nan_to_num(0)
+            ds = (p * (do @ v.double().T - (do * (p @ v.double())).sum(1, keepdim=True)) * (1 - t * t)).abs()
+            less = {n: (2.0 ** -25 - (2.0 ** -38 * ds.amax(d, keepdim=True)).clamp_min(2.0 ** -37)) * see
+                    for n, d in (("dq", 1), ("dk", 0))}
+            less = {"dq": less["dq"] @ k.double().abs() * c.scale, "dk": less["dk"].T @ q.abs() * c.scale,
+                    "dv": (2.0 ** -25 - 2.0 ** -37) * see.T @ do.abs()}
+            for n in sums:
+                x, e = r[n][0], r[n][1] - less[n]
+                if n != "dq" and j % c.group:
+                    rows[n][-1] = (rows[n][-1][0] + x, rows[n][-1][1] + e)
+                else:
+                    rows[n].append((x, e))
+        for n in sums:
+            sums[n].append([torch.stack([y[m] for y in rows[n]]) for m in (0, 1)])
+    full = {n: [torch.stack([y[m] for y in x]) for m in (0, 1)] for n, x in sums.items()}
+    return {n: (x, round_bound(x, e, c.t)) for n, (x, e) in full.items()}
+
+
+def check_f16_gradients(c):
+    c.gpu["dout"] = to_gpu(c.dout)
+    c.forward()
+    c.backward()
+    torch.cuda.synchronize()
+    for n, (x, e) in f16_gradients(c).items():
+        # zeros would not pass
+        assert (e < x.abs()).double().mean() > 0.75, (n, (e / x.abs()).median())
+        check(n, c.outs[n], x, e)
+        # All values together: errors of independent roundings, each within u of its term (u / sqrt(3) on average), add
+        # up as the terms do, to u / sqrt(3) of the sum; the result is rounded once more.
+        off, rounded = ((y - x).norm() for y in (c.outs[n].double().cpu(), x.to(c.t).double()))
+        assert off <= 2 * (rounded + 2.0 ** -11 * x.norm()), (n, off, rounded, x.norm())
+
+
+@pytest.mark.parametrize("size", (1e-2, 3e-4))
+@pytest.mark.parametrize("sq,sk,d,mods", ((300, 300, 64, {"causal": True}), (300, 3000, 64, {}), (3000, 300, 64, {"alibi": True}),
+                                          (400, 1300, 128, {"cap": 5.0}), (150, 1000, 256, {}), (100, 1000, 36, {})))
+def test_small_f16_gradients_keep_their_accuracy(size, sq, sk, d, mods):
+    """Score gradients far below the normal numbers of the type, down to parts of its smallest."""
+    c = Call("f16", 1, 4, 2, sq, sk, d, seed=6, **mods)
+    c.dout = (c.dout.float() * size).half()
+    check_f16_gradients(c)
+
+
+@pytest.mark.parametrize("sq,sk,d,mods", ((6, 3, 64, {}), (6, 3, 128, {"cap": 2.0}), (70, 40, 64, {"causal": True}), (40, 70, 256, {}),
+                                          (7, 5, 36, {"alibi": True})))
+def test_large_f16_gradients_stay_in_range(sq, sk, d, mods):
+    """Score gradients beyond the type's largest number, whose sums are not."""
+    c = Call("f16", 1, 4, 2, sq, sk, d, scale=0.01, seed=7, **mods)
+    c.dout = (c.dout.float() * 1e4).half()
+    check_f16_gradients(c)
+
+
+def test_f16_gradients_of_all_sizes_at_once():
+    """Rows of dO from 1e-3 to 1e3: each query's gradient has its own range, each key's that of its largest."""
+    c = Call("f16", 2, 16, 4, 500, 500, 64, causal=True, seed=8)
+    g = torch.Generator().manual_seed(9)
+    size = 10.0 ** (6 * torch.rand(2, 16, 500, 1, generator=g) - 3)
+    c.dout = (c.dout.float() * size).half()
+    check_f16_gradients(c)
+
+
+def test_many_blocks_of_small_f16_gradients():
+    """Two tiles a wave."""
+    c = Call("f16", 8, 16, 4, 500, 500, 64, seed=10)
+    c.dout = (c.dout.float() * 1e-3).half()
+    c.gpu["dout"] = to_gpu(c.dout)
+    c.forward()
+    c.backward()
+    torch.cuda.synchronize()
+    one = Call.__new__(Call)
+    one.__dict__.update(c.__dict__)
+    for n in ("q", "k", "v", "dout"):
+        setattr(one, n, getattr(c, n)[7:])
+    one.see = c.see[7:]
+    for n, (x, e) in f16_gradients(one).items():
+        check(n, c.outs[n][7:], x, e)
