@@ -425,7 +425,7 @@ struct RowTiles {
                     if (has_cap<MOD>(p)) {
 #pragma unroll
                         for (int r = 0; r < 4; ++r)
-                            s[t][b][r] = capped_over<T>(s[t][b][r], p.cap_in, p.cap_log2e, ref[t] - kUp);
+                            s[t][b][r] = capped_over<T, MOD>(s[t][b][r], p.cap_in, p.cap_log2e, ref[t] - kUp);
                     } else {
 #pragma unroll
                         for (int r = 0; r < 4; ++r) s[t][b][r] = __builtin_fmaf(s[t][b][r], p.scale_log2e, kUp - ref[t]);

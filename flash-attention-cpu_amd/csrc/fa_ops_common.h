@@ -179,11 +179,16 @@ __device__ __forceinline__ float row4_sum(float x) {
 }
 
 // log2(e) * softcap * tanh(scale x / softcap); t: the tanh.
-// 16-bit: 1 - 2 / (e^2y + 1), within 2e-7 absolutely.  f32 takes the library's tanh,
-// whose relative error is small also near 0.
-template <typename T>
+// 16-bit: 1 - 2 / (e^2y + 1), within 2e-7 absolutely, so the score is within 2e-7 of the cap: enough up to
+// kFastCap.  f32, and 16-bit types with larger caps, take the library's tanh, whose relative error is small
+// also near 0; the latter in the kernels of any alignment only (kAny), where the host sends them.
+template <typename T, int MOD>
+__device__ __forceinline__ bool fast_cap(float cap_log2e) {
+    return sizeof(T) == 2 && (MOD != kAny || cap_log2e <= kFastCap * kLog2e);
+}
+template <typename T, int MOD>
 __device__ __forceinline__ float capped(float x, float cap_in, float cap_log2e, float* t) {
-    if constexpr (sizeof(T) == 2) {
+    if (fast_cap<T, MOD>(cap_log2e)) {
         *t = 1.0f - 2.0f * __builtin_amdgcn_rcpf(ops_exp2(x * cap_in) + 1.0f);
     } else {
         *t = tanhf(x * (cap_in * (0.5f * kLn2)));
@@ -192,14 +197,12 @@ __device__ __forceinline__ float capped(float x, float cap_in, float cap_log2e, 
 }
 
 // The same less ref, where the tanh itself is not wanted.
-template <typename T>
+template <typename T, int MOD>
 __device__ __forceinline__ float capped_over(float x, float cap_in, float cap_log2e, float ref) {
-    if constexpr (sizeof(T) == 2) {
+    if (fast_cap<T, MOD>(cap_log2e))
         return __builtin_fmaf(-2.0f * cap_log2e, __builtin_amdgcn_rcpf(ops_exp2(x * cap_in) + 1.0f), cap_log2e - ref);
-    } else {
-        float t;
-        return capped<T>(x, cap_in, cap_log2e, &t) - ref;
-    }
+    float t;
+    return capped<T, MOD>(x, cap_in, cap_log2e, &t) - ref;
 }
 
 __device__ __forceinline__ bool not_finite(float x) {

@@ -191,8 +191,13 @@ int resolve_scale(float scale, float softcap, size_t d, ScoreScale* out) {
     out->scale_log2e = scale * log2e;
     out->cap_in = softcap > 0.0f ? 2.0f * log2e * scale / softcap : 0.0f;
     out->cap_log2e = softcap * log2e;
+    // a cap, or its ratio to the scale, at the ends of f32's range
+    if (softcap > 0.0f && (!std::isnormal(out->cap_in) || !std::isnormal(out->cap_log2e))) return FA_ERR_UNSUPPORTED;
     return FA_OK;
 }
+
+// Large caps of 16-bit types need the longer tanh, which only the kernels of any alignment have.
+bool cap_ok(int dtype, float softcap) { return dtype == FA_DTYPE_F32 || softcap <= kFastCap; }
 
 // Tag of the kernel for what happens to the scores.
 const char* score_tag(const fa_score_config& c, bool vec) {
@@ -501,7 +506,8 @@ int fa_score_forward(void* stream_, const fa_score_config* c, const void* q, con
     int dev;
     if ((rc = ops_begin(&dev, of_type(kScoreModule, c->dtype))) != FA_OK) return rc;
     const hipStream_t stream = static_cast<hipStream_t>(stream_);
-    const bool vec = vec_ok(q, lq, d) && vec_ok(k, lk, d) && vec_ok(v, lv, d) && ovec_ok(out, lo, es);
+    const bool vec = vec_ok(q, lq, d) && vec_ok(k, lk, d) && vec_ok(v, lv, d) && ovec_ok(out, lo, es) &&
+                     cap_ok(c->dtype, c->softcap);
 
     if (score_takes_rows(*c, g_dev[dev].num_cus)) {
         RowsParams p{};
@@ -574,7 +580,8 @@ int fa_score_backward(void* stream_, const fa_score_config* c, const void* q, co
     p.qs = lq.st, p.ks = lk.st, p.vs = lv.st, p.os = lo.st, p.dos = ldo.st;
     p.dqs = ldq.st, p.dks = ldk.st, p.dvs = ldv.st;
     const bool vec = vec_ok(q, lq, d) && vec_ok(k, lk, d) && vec_ok(v, lv, d) && vec_ok(out, lo, d) &&
-                     vec_ok(dout, ldo, d) && ovec_ok(dq, ldq, es) && ovec_ok(dk, ldk, es) && ovec_ok(dv, ldv, es);
+                     vec_ok(dout, ldo, d) && ovec_ok(dq, ldq, es) && ovec_ok(dk, ldk, es) && ovec_ok(dv, ldv, es) &&
+                     cap_ok(c->dtype, c->softcap);
     OpsWorkspace ws;
     const DkvPlan dkv = plan_dkv(*c, D, vec, g_dev[dev].num_cus);
     ScoreTiles tiles = score_tiles(*c, D, vec, sq, c->batch * c->heads, g_dev[dev].num_cus);
@@ -788,7 +795,8 @@ int fa_tree_attention(void* stream, const fa_tree_config* c, const fa_kv_cache* 
     p.page_shift = page_shift(*cache);
     p.n_pages = static_cast<int>(cache->n_pages), p.pages_per_seq = static_cast<int>(cache->pages_per_seq);
     p.mask_words = static_cast<int>((n + 63) / 64), p.mask_shared = c->mask_shared ? 1 : 0;
-    const bool vec = vec_ok(q, lq, d) && vec_ok(cache->k, ck, d) && vec_ok(cache->v, cv, d) && ovec_ok(out, lo, es);
+    const bool vec = vec_ok(q, lq, d) && vec_ok(cache->k, ck, d) && vec_ok(cache->v, cv, d) && ovec_ok(out, lo, es) &&
+                     cap_ok(cache->dtype, c->softcap);
     p.scale_log2e = sc.scale_log2e, p.cap_in = sc.cap_in, p.cap_log2e = sc.cap_log2e;
     int dev;
     if ((rc = ops_begin(&dev, of_type(kCacheModule, cache->dtype))) != FA_OK) return rc;

@@ -22,6 +22,9 @@ struct OpsStrides {
 
 // Tokens per entry of the document range tables.
 constexpr int kDocTile = 64;
+// The largest cap whose scores 16-bit kernels take with the short formula (within 1e-4, a quarter of f16's rounding of
+// the weights).
+constexpr float kFastCap = 512.0f;
 // What fa_score_doc_order takes: blocks to order, and tiles of the other side, of all batches.
 constexpr int kOrderBlocks = 1024, kOrderTiles = 4096;
 

@@ -282,7 +282,7 @@ __device__ __forceinline__ void score_forward(const ScoreParams& p) {
                     if (cap) {
 #pragma unroll
                         for (int r = 0; r < 4; ++r)
-                            s[t][b][r] = capped_over<T>(s[t][b][r], p.cap_in, p.cap_log2e, ref[t] - kUp);
+                            s[t][b][r] = capped_over<T, MOD>(s[t][b][r], p.cap_in, p.cap_log2e, ref[t] - kUp);
                     } else {
 #pragma unroll
                         for (int r = 0; r < 4; ++r) s[t][b][r] = __builtin_fmaf(s[t][b][r], p.scale_log2e, kUp - ref[t]);
@@ -515,7 +515,7 @@ __device__ __forceinline__ void weigh(const ScoreParams& p, bool cap, f32x4 s, f
     for (int r = 0; r < 4; ++r) {
         float z, th = 0.0f;
         if (cap) {
-            z = capped<T>(s[r], p.cap_in, p.cap_log2e, &th) - lse2[r];
+            z = capped<T, MOD>(s[r], p.cap_in, p.cap_log2e, &th) - lse2[r];
         } else {
             z = __builtin_fmaf(s[r], p.scale_log2e, -lse2[r]);
         }

@@ -289,7 +289,8 @@ typedef struct fa_score_config {
     size_t batch, heads, kv_heads, seq_len_q, seq_len_k, d_head;
     int64_t q_start;           /* position of query 0 (a decode step: the cache length) */
     float softmax_scale;       /* <= 0 or NaN: 1/sqrt(d_head) */
-    float softcap;             /* 0: none */
+    float softcap;             /* 0: none; 16-bit inputs: above 512 slower.  One whose ratio to the
+                                  scale, or itself times log2(e), is no normal f32 is refused */
     const float* slopes;       /* [heads], device memory; NULL: no bias */
     const int32_t* q_doc;      /* [batch, seq_len_q], device memory; both or neither */
     const int32_t* k_doc;      /* [batch, seq_len_k] */

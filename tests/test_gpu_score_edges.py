@@ -175,3 +175,64 @@ def test_many_blocks_of_small_f16_gradients():
     one.see = c.see[7:]
     for n, (x, e) in f16_gradients(one).items():
         check(n, c.outs[n][7:], x, e)
+
+
+def check_cap(c, grads=True):
+    """Against the capped definition, with the bounds of uncapped scores and a quarter: scores of at most 8 differ from
+    capped ones by x^3 / (3 cap^2), which changes those bounds by less than 1e-3 of them, and the rounding of the tanh adds
+    8 2^-24 |x| to the error of a score, a quarter of that of its dot product at most."""
+    want, cap = c.expect(grads), c.cap
+    bounds = want
+    if cap > 512:   # below, 16-bit types take the short tanh: ops_reference has its error, 4e-7 of the cap
+        c.cap = 0.0
+        bounds = c.expect(grads)
+        c.cap = cap
+    for n, (x, _) in want.items():
+        check(n, c.lse if n == "lse" else c.outs[n], x, 1.25 * bounds[n][1])
+
+
+CAPS = (500.0, 520.0, 1e4, 1e6, 1e12, 1e30)
+
+
+@pytest.mark.parametrize("dtype", ("f32", "bf16", "f16"))
+@pytest.mark.parametrize("cap", CAPS)
+@pytest.mark.parametrize("d,alibi", ((64, False), (128, True), (36, False)))
+def test_large_caps(dtype, cap, d, alibi):
+    c = Call(dtype, 1, 4, 2, 140, 140, d, causal=True, cap=cap, alibi=alibi, seed=11)
+    c.forward()
+    c.backward()
+    torch.cuda.synchronize()
+    check_cap(c)
+
+
+@pytest.mark.parametrize("dtype", ("f32", "bf16", "f16"))
+@pytest.mark.parametrize("cap", CAPS)
+def test_large_caps_over_long_ranges(dtype, cap):
+    c = Call(dtype, 1, 8, 2, 3, 900, 64, causal=True, q_start=880, cap=cap, seed=12)
+    c.forward()
+    torch.cuda.synchronize()
+    check_cap(c, grads=False)
+    # a tree's check has the capped bound, which allows 4e-7 of the cap: against the same call without a cap instead
+    results = []
+    for x in (cap, 0.0):
+        t = Tree(dtype, [700, 60], 4, 2, 7, 64, page=16, cap=x, seed=13)
+        t.run()
+        results.append(t)
+    torch.cuda.synchronize()
+    if cap < 1e4:   # capped scores differ
+        results[0].check()
+        return
+    results[1].out, results[1].lse = results[0].out, results[0].lse
+    results[1].check()
+
+
+@pytest.mark.parametrize("dtype", ("f32", "bf16", "f16"))
+def test_tiny_caps(dtype):
+    """All scores are within the cap: every visible key weighs the same."""
+    c = Call(dtype, 1, 2, 1, 70, 70, 64, causal=True, cap=1e-30, seed=14)
+    c.forward()
+    torch.cuda.synchronize()
+    v = c.v.double().repeat_interleave(2, 1)
+    want = v.cumsum(2) / torch.arange(1, 71)[:, None]
+    u = torch.finfo(c.t).eps / 2
+    check("out", c.outs["out"], want, 2 * u * (v.abs().cumsum(2) / torch.arange(1, 71)[:, None]) + 70 * 2.0 ** -24 + 2.0 ** -25)
