@@ -138,7 +138,6 @@ int resolve_layout(const fa_strides& in, size_t batch, size_t seq, size_t heads,
                    OpsLayout* out) {
     int64_t b = in.batch, s = in.seq, h = in.head;
     if (b < 0 || s < 0 || h < 0) return FA_ERR_INVALID_ARG;
-    if (b > kOpsMaxStride || h > kOpsMaxStride || s >= kOpsMaxRowStride) return FA_ERR_UNSUPPORTED;
     const int64_t row = static_cast<int64_t>(d);
     if (b == 0 && s == 0 && h == 0) {
         s = row;
@@ -146,10 +145,11 @@ int resolve_layout(const fa_strides& in, size_t batch, size_t seq, size_t heads,
         if (h > 0 && static_cast<int64_t>(heads) > kOpsMaxStride / h) return FA_ERR_UNSUPPORTED;
         b = static_cast<int64_t>(heads) * h;
     }
-    // strides of single entries are never used
+    // strides of single entries are never used, whatever they are
     if (seq <= 1) s = row;
     if (heads <= 1) h = 0;
     if (batch <= 1) b = 0;
+    if (b > kOpsMaxStride || h > kOpsMaxStride || s >= kOpsMaxRowStride) return FA_ERR_UNSUPPORTED;
     if (s < row) return FA_ERR_INVALID_ARG;
     if (writable) {
         // no two rows overlap: each dimension steps over all of the smaller ones

@@ -276,7 +276,8 @@ int fa_multihead_lp(int dtype, const void* q, size_t q_len, const void* k, size_
  *
  * Layouts: element strides between batches, tokens and heads, columns next to
  * each other; all three 0 means contiguous [batch, heads, seq, d_head].  The
- * token stride is at least d_head.  Inputs may share memory between batches or heads
+ * token stride is at least d_head and below 2^22 (FA_ERR_UNSUPPORTED beyond);
+ * strides of dimensions of one entry are not looked at.  Inputs may share memory between batches or heads
  * (stride 0); outputs may not overlap.  Any alignment works; 16-byte aligned
  * rows (pointers, strides and d_head) are faster. */
 typedef struct fa_strides {
