@@ -267,6 +267,10 @@ __device__ __forceinline__ Runs runs_of_run(const RowsParams& p, int run, int la
         return r;
     }
     Runs r = {-1, 0, 0, 0};
+    if (p.share == 1) {   // a run each: with many sequences every workgroup would look through all of them
+        if (run < p.batch) r = {run, (rows_total(p, run) + p.step - 1) / p.step, 1, run};
+        return r;
+    }
     r.steps = each_runs(p, lane, [&](int base, int n, int end) {
         const uint64_t hit = __builtin_amdgcn_ballot_w64(n > 0 && run >= end - n && run < end);
         if (hit == 0) return false;

@@ -10,6 +10,7 @@ import threading
 import pytest
 import torch
 
+import flash_attention_amd as fa
 from ops_reference import attend, check, round_bound
 from test_gpu_rotary_tree import Tree
 from test_gpu_score import Call, check_batch, doc_ids, to_gpu
@@ -236,3 +237,22 @@ def test_tiny_caps(dtype):
     want = v.cumsum(2) / torch.arange(1, 71)[:, None]
     u = torch.finfo(c.t).eps / 2
     check("out", c.outs["out"], want, 2 * u * (v.abs().cumsum(2) / torch.arange(1, 71)[:, None]) + 70 * 2.0 ** -24 + 2.0 ** -25)
+
+
+@pytest.mark.parametrize("batch,sq,sk,d", ((131073, 64, 20, 8), (300007, 49, 49, 32), (600011, 1, 5, 64)))
+def test_very_many_small_calls_in_one(batch, sq, sk, d):
+    """More than 2^23 query rows in short blocks, all on the same keys: each weight and the result are rounded once, 2 u of
+    the largest value, and f32 errors are far below a quarter of that."""
+    g = torch.Generator(device="cuda").manual_seed(15)
+    q = torch.randn(batch, 1, sq, d, generator=g, device="cuda").bfloat16()
+    k, v = (torch.randn(sk, d, generator=g, device="cuda").bfloat16() for _ in range(2))
+    out, lse = torch.full_like(q, 7.0), torch.full((batch, 1, sq), 7.0, device="cuda")
+    c = fa.score_config(fa.DTYPE_BF16, batch, 1, 1, sq, sk, d, strides={"k": (0, d, 0), "v": (0, d, 0)})
+    fa.score_attention_device(c, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
+                              torch.cuda.current_stream().cuda_stream)
+    kt, vd = k.double().t().contiguous(), v.double()
+    for lo in range(0, batch, 40000):
+        z = q[lo:lo + 40000].reshape(-1, d).double() @ kt / d ** 0.5
+        want = torch.softmax(z, 1) @ vd
+        assert (out[lo:lo + 40000].reshape(-1, d) - want).abs().max() <= 2.25 * 2.0 ** -8 * vd.abs().max()
+        assert (lse[lo:lo + 40000].reshape(-1) - torch.logsumexp(z, 1)).abs().max() <= 1e-4
