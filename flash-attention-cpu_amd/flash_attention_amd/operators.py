@@ -83,15 +83,19 @@ def declare(lib: ctypes.CDLL) -> None:
         "fa_cache_append": [_P, ptr(KvCache), ptr(AppendConfig), _P, _P, _P, _P, _P],
         "fa_tree_attention": [_P, ptr(TreeConfig), ptr(KvCache), _P, _P, _P],
     }.items():
-        f = getattr(lib, name)
-        f.argtypes = args
-        f.restype = _I
+        f = getattr(lib, name, None)   # None: a library built before there were operators
+        if f is not None:
+            f.argtypes = args
+            f.restype = _I
 
 
 def _lib():
     global _lib
     from . import lib
     loaded = lib()
+    if not hasattr(loaded, "fa_score_forward"):
+        from . import FA_ERR_MODULE, LIB_PATH, FaError
+        raise FaError(FA_ERR_MODULE, f"{LIB_PATH} has no operators; build it anew with flash-attention-cpu_amd/build.py")
 
     def known():
         return loaded
