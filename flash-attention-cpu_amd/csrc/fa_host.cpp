@@ -189,8 +189,6 @@ CopyPool& copy_pool() {
 
 DeviceState g_dev[kMaxDevices];
 
-void ops_init(int dev);   // fa_ops_host.h
-
 std::string module_path() {
     const char* env = std::getenv("FA_HIP_MODULE");
     if (env && *env) return std::string(env);
@@ -1518,11 +1516,9 @@ fa_config fa_config_default(void) {
 
 int fa_init(void) {
     int dev;
-    int rc = current_device(&dev);
+    const int rc = current_device(&dev);
     if (rc != FA_OK) return rc;
-    rc = ensure_loaded(dev);
-    if (rc == FA_OK) ops_init(dev);   // a missing operator module concerns only its entry points
-    return rc;
+    return ensure_loaded(dev);
 }
 
 int fa_v1(const float* q, size_t q_len, const float* k, size_t k_len, const float* v, size_t v_len, size_t sq,

@@ -6,6 +6,7 @@ import subprocess
 import sys
 
 import flash_attention_amd as fa
+from test_host_threads import compile_with_stub
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 OPERATORS = ("fa_score_forward", "fa_score_backward", "fa_rotary_init", "fa_rotary", "fa_cache_append", "fa_tree_attention")
@@ -25,3 +26,31 @@ def test_a_library_without_operators_still_loads(tmp_path):
                PYTHONPATH=os.path.join(ROOT, "flash-attention-cpu_amd"))
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, env=env, timeout=120)
     assert r.stdout.splitlines() == ["loaded", "8 True", "8 True"], (r.stdout, r.stderr)
+
+
+DRIVER = r"""
+int main() {
+    static char mem[64] __attribute__((aligned(64)));
+    void* p = mem;
+    if (fa_init() != FA_OK) return 2;
+    std::printf("%zu\n", stub::loaded.size());
+    fa_rotary_config r;
+    fa_rotary_init(&r, FA_DTYPE_F16, 64, 64, 0, 10000.0, 0, 1.0, 0.0);
+    fa_rotary_tensor x{};
+    x.heads = 2;
+    for (int i = 0; i < 2; ++i)
+        if (fa_rotary(nullptr, &r, 1, 4, static_cast<const int32_t*>(p), 0, &x, p, p, nullptr, nullptr, nullptr) != FA_OK) return 3;
+    fa_score_config c{};
+    c.dtype = FA_DTYPE_F16, c.batch = 1, c.heads = c.kv_heads = 2, c.seq_len_q = c.seq_len_k = 200, c.d_head = 64;
+    if (fa_score_forward(nullptr, &c, p, p, p, p, nullptr) != FA_OK) return 4;
+    for (const std::string& s : stub::loaded) std::printf("%s\n", s.substr(s.rfind('/') + 1).c_str());
+    return 0;
+}
+"""
+
+
+def test_operators_are_loaded_by_the_calls_that_need_them(tmp_path):
+    """fa_init loads what programs without operators use, and no more."""
+    exe, env = compile_with_stub(tmp_path, DRIVER)
+    out = subprocess.run([exe], capture_output=True, text=True, env=env, check=True, timeout=60).stdout.split()
+    assert out == ["1", "fa_kernels.hsaco", "fa_rotary.hsaco", "fa_score_f16.hsaco"]
