@@ -142,8 +142,9 @@ __device__ __forceinline__ bool docs_meet(const DocRange& a, const DocRange& b, 
 
 // One value a lane from global memory into LDS, zero past n.
 __device__ __forceinline__ void fill_words(void* dst, const void* src, int n, int lane) {
+    const int bytes = 4 * min(max(n, 0), 64);   // (of 2^30 words the size would not fit)
     const __amdgpu_buffer_rsrc_t rs =
-        __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(src), (short)0, 4 * max(n, 0), 0x00020000);
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(src), (short)0, bytes, 0x00020000);
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)dst, 4, 4 * lane, 0, 0, 0);
 }
 
