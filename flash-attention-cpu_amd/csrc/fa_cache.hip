@@ -427,9 +427,7 @@ struct RowTiles {
 #pragma unroll
                 for (int b = 0; b < KB; ++b) {
                     if (has_cap<MOD>(p)) {
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            s[t][b][r] = capped_over<T, MOD>(s[t][b][r], p.cap_in, p.cap_log2e, ref[t] - kUp);
+                        s[t][b] = capped_over<T, MOD>(s[t][b], p.cap_in, p.cap_log2e, ref[t] - kUp);
                     } else {
 #pragma unroll
                         for (int r = 0; r < 4; ++r) s[t][b][r] = __builtin_fmaf(s[t][b][r], p.scale_log2e, kUp - ref[t]);

@@ -187,22 +187,29 @@ __device__ __forceinline__ bool fast_cap(float cap_log2e) {
     return sizeof(T) == 2 && (MOD != kAny || cap_log2e <= kFastCap * kLog2e);
 }
 template <typename T, int MOD>
-__device__ __forceinline__ float capped(float x, float cap_in, float cap_log2e, float* t) {
+__device__ __forceinline__ f32x4 capped(f32x4 x, float cap_in, float cap_log2e, f32x4* t) {
     if (fast_cap<T, MOD>(cap_log2e)) {
-        *t = 1.0f - 2.0f * __builtin_amdgcn_rcpf(ops_exp2(x * cap_in) + 1.0f);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) (*t)[r] = 1.0f - 2.0f * __builtin_amdgcn_rcpf(ops_exp2(x[r] * cap_in) + 1.0f);
     } else {
-        *t = tanhf(x * (cap_in * (0.5f * kLn2)));
+#pragma unroll
+        for (int r = 0; r < 4; ++r) (*t)[r] = tanhf(x[r] * (cap_in * (0.5f * kLn2)));
     }
-    return cap_log2e * *t;
+    return *t * cap_log2e;
 }
 
 // The same less ref, where the tanh itself is not wanted.
 template <typename T, int MOD>
-__device__ __forceinline__ float capped_over(float x, float cap_in, float cap_log2e, float ref) {
-    if (fast_cap<T, MOD>(cap_log2e))
-        return __builtin_fmaf(-2.0f * cap_log2e, __builtin_amdgcn_rcpf(ops_exp2(x * cap_in) + 1.0f), cap_log2e - ref);
-    float t;
-    return capped<T, MOD>(x, cap_in, cap_log2e, &t) - ref;
+__device__ __forceinline__ f32x4 capped_over(f32x4 x, float cap_in, float cap_log2e, float ref) {
+    if (fast_cap<T, MOD>(cap_log2e)) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            x[r] = __builtin_fmaf(-2.0f * cap_log2e, __builtin_amdgcn_rcpf(ops_exp2(x[r] * cap_in) + 1.0f), cap_log2e - ref);
+    } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] = cap_log2e * tanhf(x[r] * (cap_in * (0.5f * kLn2))) - ref;
+    }
+    return x;
 }
 
 __device__ __forceinline__ bool not_finite(float x) {

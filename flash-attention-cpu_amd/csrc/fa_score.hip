@@ -281,9 +281,7 @@ __device__ __forceinline__ void score_forward(const ScoreParams& p) {
 #pragma unroll
                 for (int b = 0; b < KB; ++b) {
                     if (cap) {
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            s[t][b][r] = capped_over<T, MOD>(s[t][b][r], p.cap_in, p.cap_log2e, ref[t] - kUp);
+                        s[t][b] = capped_over<T, MOD>(s[t][b], p.cap_in, p.cap_log2e, ref[t] - kUp);
                     } else {
 #pragma unroll
                         for (int r = 0; r < 4; ++r) s[t][b][r] = __builtin_fmaf(s[t][b][r], p.scale_log2e, kUp - ref[t]);
@@ -512,19 +510,16 @@ __device__ __forceinline__ void score_forward(const ScoreParams& p) {
 template <typename T, int MOD>
 __device__ __forceinline__ void weigh(const ScoreParams& p, bool cap, f32x4 s, f32x4 dp, f32x4 lse2, f32x4 delta,
                                       float slope, float dist, f32x4* w, f32x4* y, f32x4* f) {
+    f32x4 th, capped_s;
+    if (cap) capped_s = capped<T, MOD>(s, p.cap_in, p.cap_log2e, &th);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-        float z, th = 0.0f;
-        if (cap) {
-            z = capped<T, MOD>(s[r], p.cap_in, p.cap_log2e, &th) - lse2[r];
-        } else {
-            z = __builtin_fmaf(s[r], p.scale_log2e, -lse2[r]);
-        }
+        float z = cap ? capped_s[r] - lse2[r] : __builtin_fmaf(s[r], p.scale_log2e, -lse2[r]);
         if (has_bias<MOD>(p)) z = __builtin_fmaf(-slope, fabsf(dist - (float)r), z);
         const float x = ops_exp2(z);
         (*w)[r] = x;
         (*y)[r] = x * (dp[r] - delta[r]);
-        (*f)[r] = cap ? __builtin_fmaf(-th, th, 1.0f) : 1.0f;
+        (*f)[r] = cap ? __builtin_fmaf(-th[r], th[r], 1.0f) : 1.0f;
     }
 }
 
