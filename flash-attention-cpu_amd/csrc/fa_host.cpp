@@ -1057,9 +1057,9 @@ size_t free_device_bytes() {
 // on any stream -- never share partials with later eager calls on the
 // capture stream, nor with another graph captured there.
 //
-// Buffers are whole units of 2 MiB, in which the driver hands memory out, and one unit larger than
+// Buffers are whole units of 2 MiB, in which device memory is handed out, and one unit larger than
 // the call needs: partials that grow a little from step to step keep their buffer, and the free
-// memory that the driver reports falls by the call's need at least (it counts units, and some
+// memory that hipMemGetInfo reports falls by the call's need at least (it counts units, and some
 // units short: of 20 allocations of 50 MiB one is seen as 48).
 constexpr size_t kWorkspaceUnit = size_t(2) << 20;
 int stream_workspace(int dev, hipStream_t stream, size_t need, void** out) {

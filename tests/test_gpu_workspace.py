@@ -1,4 +1,4 @@
-"""What a stream's workspace takes of the device's free memory, as the driver reports it."""
+"""What a stream's workspace takes of the device's free memory, as hipMemGetInfo reports it."""
 from __future__ import annotations
 
 import ctypes
@@ -18,7 +18,7 @@ def hip_runtime():
 
 
 def test_a_workspace_takes_its_size_whatever_was_allocated_before():
-    """The free memory that the driver reports falls by a workspace's size at least, also where the report is a unit of
+    """The free memory that is reported falls by a workspace's size at least, also where the report is a unit of
     2 MiB short (once in 1000 MiB of allocations of 50 MiB).  Other allocations in steps of 40 MiB, smaller than the
     workspace of 48.25 MiB, move it over more than 1000 MiB."""
     import torch
