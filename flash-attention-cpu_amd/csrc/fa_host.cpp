@@ -1617,6 +1617,10 @@ int fa_release_stream_workspace(void* stream) {
     // stream.
     std::vector<void*> bufs;
     {
+        std::lock_guard<std::mutex> lock(s.ws_mu);
+        if (s.ws.find(workspace_key(st)) == s.ws.end()) return FA_OK;
+    }
+    {
         const WorkspaceCall call(dev, st);
         std::lock_guard<std::mutex> lock(s.ws_mu);
         auto it = s.ws.find(workspace_key(st));

@@ -26,6 +26,7 @@ inline std::string absent;             // functions whose names start with this 
 inline int yields = 1;
 inline std::vector<std::string> loaded;
 inline std::vector<size_t> allocations;
+inline int synchronized = 0;           // streams, by hipStreamSynchronize
 }  // namespace stub
 
 extern "C" {
@@ -54,7 +55,10 @@ hipError_t hipEventDestroy(hipEvent_t) { return hipSuccess; }
 hipError_t hipEventRecord(hipEvent_t, hipStream_t) { return hipSuccess; }
 hipError_t hipEventSynchronize(hipEvent_t) { return hipSuccess; }
 hipError_t hipStreamCreateWithFlags(hipStream_t* s, unsigned) { return *s = nullptr, hipSuccess; }
-hipError_t hipStreamSynchronize(hipStream_t) { return hipSuccess; }
+hipError_t hipStreamSynchronize(hipStream_t) {
+    std::lock_guard<std::mutex> lock(stub::mu);
+    return ++stub::synchronized, hipSuccess;
+}
 hipError_t hipStreamGetCaptureInfo(hipStream_t, hipStreamCaptureStatus* st, unsigned long long* id) {
     return *st = hipStreamCaptureStatusNone, *id = 0, hipSuccess;
 }

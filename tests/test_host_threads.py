@@ -132,3 +132,26 @@ def test_workspaces_are_whole_units_and_one_more_than_needed(tmp_path):
         size, need = (int(x) for x in line.split()[:2])
         assert size % unit == 0 and need + unit <= size < need + 2 * unit, line
     assert out[-1] == "4 allocations"
+
+
+RELEASE = r"""
+int main() {
+    static char mem[64] __attribute__((aligned(64)));
+    float* const f = reinterpret_cast<float*>(mem);
+    const hipStream_t s = reinterpret_cast<hipStream_t>(mem);
+    if (fa_init() != FA_OK || fa_release_stream_workspace(s) != FA_OK) return 2;
+    std::printf("%d\n", stub::synchronized);
+    if (fa_device_ex(2, s, f, f, f, 1, 16, 1, 20000, 128, nullptr, nullptr, f) != FA_OK) return 2;
+    for (int i = 0; i < 2; ++i)
+        if (fa_release_stream_workspace(s) != FA_OK) return 2;
+    std::printf("%d\n", stub::synchronized);
+    return 0;
+}
+"""
+
+
+def test_a_stream_without_a_workspace_is_left_alone(tmp_path):
+    """Releasing the workspace of a stream that has none does not wait for the stream (which may be capturing)."""
+    exe, env = compile_with_stub(tmp_path, RELEASE)
+    out = subprocess.run([exe], capture_output=True, text=True, env=env, check=True, timeout=60).stdout.split()
+    assert out == ["0", "1"]
