@@ -212,17 +212,44 @@ struct RowsWork {
     int run, rb, b, hk;
     int runs;   // of the sequence
     int len, prefix, open, kbeg, kend, nrows, rfirst;
+    int kwalk;        // keys to walk, from kbeg on, without those that are left out
+    int gap, skip;    // keys from `gap` on are left out, `skip` of them
+    int low;          // a window's: keys before this and not before p.sinks are hidden from some row
     int tree, docs;
+    // the key that stands `i` behind kbeg (a multiple of 16) among those walked
+    __device__ __forceinline__ int key(int i) const {
+        const int k = kfirst + i;
+        return k + (k >= gap ? skip : 0);
+    }
+    int kfirst;       // kbeg among those walked
 };
 
-// Keys that any query of sequence b sees.
-__device__ __forceinline__ int rows_total(const RowsParams& p, int b) {
+// Keys that any query of sequence b sees: those before `total`, without `skip` ones from `gap` on where a window
+// leaves them out (multiples of 64, so that blocks of keys start where they do without).
+struct Walk {
+    int total, gap, skip;
+    __device__ __forceinline__ int walked() const { return total - skip; }
+};
+__device__ __forceinline__ Walk rows_walk(const RowsParams& p, int b) {
+    Walk w = {0, 0x7fffffff, 0};
+    int first;   // position of the first query
     if (p.lens) {
         const int len = p.lens[b];
-        return len < 0 ? 0 : (int)min((int64_t)len + p.n, (int64_t)p.sk);
+        w.total = len < 0 ? 0 : (int)min((int64_t)len + p.n, (int64_t)p.sk);
+        first = len;
+    } else {
+        w.total = p.causal ? max(min(max(p.q_start + p.n, p.prefix ? p.prefix[b] : 0), p.sk), 0) : p.sk;
+        first = p.q_start;
     }
-    return p.causal ? max(min(max(p.q_start + p.n, p.prefix ? p.prefix[b] : 0), p.sk), 0) : p.sk;
+    if (p.window) {
+        if (!p.lens) w.total = min(w.total, max(max(first + p.n - 1 + p.window, p.sinks), 0));
+        w.gap = (p.sinks + 63) & ~63;
+        const int low = min(first - p.window + 1, w.total);
+        w.skip = max((max(low, 0) & ~63) - w.gap, 0);
+    }
+    return w;
 }
+__device__ __forceinline__ int rows_total(const RowsParams& p, int b) { return rows_walk(p, b).walked(); }
 
 // The runs of a sequence: their length in steps, how many, and the first one's number.
 struct Runs {
@@ -327,17 +354,56 @@ __device__ __forceinline__ bool rows_work(const RowsParams& p, int rows, int lan
     } else {
         w.open = w.docs ? 0 : p.causal ? max(p.q_start + 1, w.prefix) : p.sk;
     }
-    const int total = __builtin_amdgcn_readfirstlane(rows_total(p, w.b));
+    w.low = INT32_MIN;
+    if (p.window) {
+        int last = p.q_start + p.n - 1;   // position of the last query
+        if (w.tree) {
+            last = p.pos ? w.len : (int)min((int64_t)w.len + p.n - 1, (int64_t)kWindowMaxPos);
+            for (int i = lane; p.pos && i < p.n; i += 64) last = max(last, p.pos[(int64_t)w.b * p.n + i]);
+#pragma unroll
+            for (int s = 1; s < 64; s *= 2) last = max(last, __shfl_xor(last, s));
+            last = min(__builtin_amdgcn_readfirstlane(last), kWindowMaxPos);
+        } else {
+            w.open = min(w.open, max(p.q_start + p.window, 0));
+        }
+        w.low = last - p.window + 1;
+    }
+    const Walk walk = rows_walk(p, w.b);
+    w.gap = __builtin_amdgcn_readfirstlane(walk.gap);
+    w.skip = __builtin_amdgcn_readfirstlane(walk.skip);
+    const int total = __builtin_amdgcn_readfirstlane(walk.walked());
     const int64_t per = (int64_t)__builtin_amdgcn_readfirstlane(r.steps) * p.step;
-    w.kbeg = (int)min((w.run - __builtin_amdgcn_readfirstlane(r.first)) * per, (int64_t)total);
-    w.kend = (int)min(w.kbeg + per, (int64_t)total);
+    w.kfirst = (int)min((w.run - __builtin_amdgcn_readfirstlane(r.first)) * per, (int64_t)total);
+    const int last = (int)min(w.kfirst + per, (int64_t)total);
+    w.kwalk = last - w.kfirst;
+    w.kbeg = w.key(0);
+    w.kend = last + (last > w.gap ? w.skip : 0);
     w.nrows = p.n * p.group;
     w.rfirst = w.rb * rows;
     return true;
 }
 
+// Whether the keys of a block need the mask: [k0, k0 + n).
+__device__ __forceinline__ int rows_masked(const RowsParams& p, const RowsWork& w, int k0, int n) {
+    return k0 + n > min(w.open, w.kend) || (k0 < w.low && k0 + n > p.sinks);
+}
+
+// Position of a token for windows, which drafted tokens do not stand before their sequence's filled rows for.
+__device__ __forceinline__ int window_position(const RowsParams& p, const RowsWork& w, int tok) {
+    if (!w.tree) return p.q_start + tok;
+    return min(p.pos ? max(p.pos[(int64_t)w.b * p.n + tok], w.len) : w.len + tok, kWindowMaxPos);
+}
+// Whether the window hides key `key` from a token that stands at `pos`.
+__device__ __forceinline__ bool window_hides(const RowsParams& p, const RowsWork& w, int pos, int key) {
+    if (key < p.sinks) return false;
+    if (!w.tree) return key <= pos - p.window || key >= pos + p.window;
+    const int bit = key - w.len;
+    return pos - (bit >= 0 ? window_position(p, w, min(bit, p.n - 1)) : key) >= p.window;
+}
+
 // Whether token `tok` sees key `key` < kend, as far as masks tell.
 __device__ __forceinline__ bool rows_see(const RowsParams& p, const RowsWork& w, int tok, int key) {
+    if (p.window && window_hides(p, w, window_position(p, w, tok), key)) return false;
     if (!w.tree) {
         if (p.causal && !(key <= p.q_start + tok || key < w.prefix)) return false;
         if (!w.docs) return true;
@@ -459,6 +525,10 @@ struct RowTiles {
             uint64_t see[MT];
 #pragma unroll
             for (int t = 0; t < MT; ++t) see[t] = there & seen_bits(lp, w, t, k0);
+            if (lp.window) {
+#pragma unroll
+                for (int t = 0; t < MT; ++t) see[t] &= window_bits(lp, w, t, k0);
+            }
             if (w.docs) {
 #pragma unroll
                 for (int b = 0; b < KB; ++b)
@@ -501,6 +571,26 @@ struct RowTiles {
         const int i = rel >> 6, sh = rel & 63;
         const uint64_t lo = mask_word(p, w, t, i) >> sh;
         return sh == 0 ? lo : lo | (mask_word(p, w, t, i + 1) << (64 - sh));
+    }
+    // Those of the 16 KB keys that the window leaves the lane's row of tile t; drafted keys that stand where the program
+    // says: of the keys whose scores the lane holds.
+    __device__ __forceinline__ uint64_t window_bits(const RowsParams& p, const RowsWork& w, int t, int k0) const {
+        auto before = [](int n) -> uint64_t { return n >= 64 ? ~0ull : (1ull << max(n, 0)) - 1; };
+        const int at = w.tree ? min(max(pos[t], w.len), kWindowMaxPos) : pos[t];
+        uint64_t bits = ~before(at - p.window + 1 - k0);
+        if (!w.tree) bits &= before(at + p.window - k0);
+        bits |= before(p.sinks - k0);
+        if (w.tree && p.pos && k0 + 16 * KB > w.len) {
+#pragma unroll 1
+            for (int b = 0; b < KB; ++b)
+#pragma unroll 1
+                for (int r = 0; r < 4; ++r) {
+                    const int x = 16 * b + 4 * g + r;
+                    if (k0 + x < w.len) continue;
+                    bits = window_hides(p, w, at, k0 + x) ? bits & ~(1ull << x) : bits | 1ull << x;
+                }
+        }
+        return bits;
     }
     __device__ __forceinline__ uint64_t mask_word(const RowsParams& p, const RowsWork& w, int t, int i) const {
         if (i == 0) return word[t];
@@ -577,6 +667,7 @@ struct RowTiles {
         const CachePages pages = rows_pages(p, w.b);
         const int mine = min(16 * MT, w.nrows - rfirst);
         auto row_at = [&](int key) -> const T* {
+            if (key >= w.gap && key - w.gap < w.skip) return nullptr;
             const int64_t at = pages.at(key, w.kend, p.vs.s, p.vs.b);
             return at < 0 ? nullptr : V + at;
         };
@@ -657,8 +748,8 @@ __device__ __forceinline__ void rows_stream(const RowsParams& p) {
     const T* const K = reinterpret_cast<const T*>(p.k) + w.hk * p.ks.h + (p.table ? 0 : w.b * p.ks.b);
     const T* const V = reinterpret_cast<const T*>(p.v) + w.hk * p.vs.h + (p.table ? 0 : w.b * p.vs.b);
     const Src ksrc(K, p.ks.s, p.ks.b, p.d, 0, lane), vsrc(V, p.vs.s, p.vs.b, p.d, 0, lane);
-    const int k_first = w.kbeg + SK * wave;
-    const int nblk = k_first < w.kend ? (w.kend - k_first + SK * NW - 1) / (SK * NW) : 0;
+    const int k_first = SK * wave;   // of the walked keys
+    const int nblk = k_first < w.kwalk ? (w.kwalk - k_first + SK * NW - 1) / (SK * NW) : 0;
     static_assert(VEC, "DMA only");
 
     bool special = false;
@@ -667,11 +758,11 @@ __device__ __forceinline__ void rows_stream(const RowsParams& p) {
     int page[2];
     int bad0, bad1, bad2;
     auto look_up = [&](int blk) {
-        const int k0 = k_first + blk * SK * NW;
+        const int k0 = w.key(k_first + blk * SK * NW);
         return Src::look_up(pages, k0, blk < nblk ? w.kend : k0, page);
     };
     auto fill = [&](const Src& src, T* dst, int blk) {
-        const int k0 = k_first + blk * SK * NW;
+        const int k0 = w.key(k_first + blk * SK * NW);
         src.fill(dst + wave * TILE, k0, blk < nblk ? w.kend : k0, page, pages, 0);
     };
     bad0 = look_up(0);
@@ -691,12 +782,12 @@ __device__ __forceinline__ void rows_stream(const RowsParams& p) {
     auto block = [&](int i, T* kb, T* vb) {
         T* const Ks = kb + wave * TILE;
         T* const Vs = vb + wave * TILE;
-        const int k0 = k_first + i * SK * NW;
+        const int k0 = w.key(k_first + i * SK * NW);
         const int bad = bad0;
         bad0 = bad1;
         bad1 = bad2;
         wait_vmcnt<3 * RUNS>();
-        const int masked = bad || k0 + SK > min(w.open, w.kend);
+        const int masked = bad || rows_masked(p, w, k0, SK);
         x.scores(p, w, Ks, k0, masked, bad);
         reread();
         fill(ksrc, kb, i + 2);
@@ -788,7 +879,7 @@ __device__ __forceinline__ void rows_shared(const RowsParams& p) {
     const T* const K = reinterpret_cast<const T*>(p.k) + w.hk * p.ks.h + (p.table ? 0 : w.b * p.ks.b);
     const T* const V = reinterpret_cast<const T*>(p.v) + w.hk * p.vs.h + (p.table ? 0 : w.b * p.vs.b);
     const Src ksrc(K, p.ks.s, p.ks.b, p.d, wave, lane), vsrc(V, p.vs.s, p.vs.b, p.d, wave, lane);
-    const int nst = (w.kend - w.kbeg + SK - 1) / SK;
+    const int nst = (w.kwalk + SK - 1) / SK;
     const int rfirst = w.rfirst + 16 * MT * wave;
     const int act = rfirst < w.nrows;
 
@@ -796,11 +887,11 @@ __device__ __forceinline__ void rows_shared(const RowsParams& p) {
     int bad_now = 0, bad_1 = 0, bad_2 = 0, bad_next = 0;
     int page[SK / 16];
     auto look_up = [&](int st) {
-        const int k0 = w.kbeg + st * SK;
+        const int k0 = w.key(st * SK);
         if (VEC) bad_next = Src::look_up(pages, k0, st < nst ? w.kend : k0, page);
     };
     auto fill = [&](int st, T* k, T* v) -> int {
-        const int k0 = w.kbeg + st * SK;
+        const int k0 = w.key(st * SK);
         const int bad = bad_next;
         if constexpr (VEC) {
             const int end = st < nst ? w.kend : k0;
@@ -833,14 +924,14 @@ __device__ __forceinline__ void rows_shared(const RowsParams& p) {
     bad_now = fill(0, K0, V0);
     if (RING > 2) bad_1 = fill(1, K1, V1);
     auto step = [&](int st, T* k, T* v, T* kn, T* vn) {
-        const int k0 = w.kbeg + st * SK;
+        const int k0 = w.key(st * SK);
         // the same on all waves: a barrier hangs on it
         const int bad = VEC ? bad_now : Src::bad_rows(pages, k0, w.kend, lane);
         arrive(std::integral_constant<int, (RING - 2) * 2 * Src::NI>{});
         const int filled = fill(st + RING - 1, kn, vn);
         if (RING > 2) bad_2 = filled;
         else bad_1 = filled;
-        const int masked = bad || k0 + SK > min(w.open, w.kend);
+        const int masked = bad || rows_masked(p, w, k0, SK);
         if (act) {
             x.scores(p, w, k, k0, masked, bad);
             x.softmax();

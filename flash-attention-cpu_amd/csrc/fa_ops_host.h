@@ -334,15 +334,33 @@ int run_rows(int dev, hipStream_t stream, int dtype, int D, bool vec, RowsParams
     return ws.done(stream, rc);
 }
 
+// A window's size and sinks as kernels take them (size 0: hides nothing); farthest: the largest distance there is.
+int resolve_window(const fa_window* w, bool docs, int64_t farthest, int* size, int* sinks) {
+    *size = *sinks = 0;
+    if (!w) return FA_OK;
+    if (w->size < 1 || w->sinks < 0) return FA_ERR_INVALID_ARG;
+    if (w->sinks > 0 && docs) return FA_ERR_UNSUPPORTED;   // the first keys are another document's
+    if (w->size > farthest) return FA_OK;
+    if (farthest > kWindowMaxPos) return FA_ERR_UNSUPPORTED;   // positions plus or minus a window stay in 32 bits
+    *size = static_cast<int>(w->size);
+    *sinks = static_cast<int>(std::min<int64_t>(w->sinks, kWindowMaxPos));
+    return FA_OK;
+}
+// The most keys that n consecutive queries of a window walk.
+size_t window_keys(size_t keys, int size, int sinks, size_t n, bool both_sides) {
+    if (size == 0) return keys;
+    return std::min(keys, (both_sides ? 2 : 1) * static_cast<size_t>(size) + sinks + n + 128);
+}
+
 // Short query blocks, and few workgroups over many keys, run on the rows kernel, which splits the keys.
-bool score_takes_rows(const fa_score_config& c, int num_cus) {
+bool score_takes_rows(const fa_score_config& c, size_t keys, int num_cus) {
     const size_t group = c.heads / c.kv_heads;
     if (c.seq_len_q * group <= 64) return true;
     // a workgroup of 32 rows takes some 0.6 us per 64 keys: above 2048 keys longer than the split and its merge, at
     // 256 columns above 1024 (1 head, 1900^2 causal: bf16 53 us whole, 35 split, f32 277 and 97; 2 heads of 128
     // columns, 1500^2: bf16 21 and 30, f32 72 and 78)
     const size_t blocks = c.batch * c.heads * ((c.seq_len_q + 31) / 32);
-    return c.seq_len_k >= (c.d_head > 128 ? 1024 : 2048) && 2 * blocks <= static_cast<size_t>(num_cus);
+    return keys >= (c.d_head > 128 ? 1024 : 2048) && 2 * blocks <= static_cast<size_t>(num_cus);
 }
 
 int check_score(const fa_score_config* c) {
@@ -481,10 +499,16 @@ int launch_rotary(int dev, hipStream_t stream, int dtype, RotParams* p, bool wid
 
 }  // namespace
 
-extern "C" {
+namespace {
 
-int fa_score_forward(void* stream_, const fa_score_config* c, const void* q, const void* k, const void* v, void* out,
-                     float* lse) try {
+// The largest distance between a query and a key, and of the rows that fill up a block.
+int64_t score_farthest(const fa_score_config& c) {
+    const int64_t first = c.q_start, last = first + static_cast<int64_t>(c.seq_len_q) - 1;
+    return std::max(std::abs(last), std::abs(first - (static_cast<int64_t>(c.seq_len_k) - 1))) + 4096;
+}
+
+int score_forward(void* stream_, const fa_score_config* c, const fa_window* window, const void* q, const void* k,
+                  const void* v, void* out, float* lse) {
     int rc = check_score(c);
     if (rc != FA_OK) return rc;
     if (c->batch == 0 || c->heads == 0 || c->seq_len_q == 0 || c->d_head == 0) return FA_OK;
@@ -497,6 +521,8 @@ int fa_score_forward(void* stream_, const fa_score_config* c, const void* q, con
         (rc = resolve_layout(c->v, c->batch, c->seq_len_k, c->kv_heads, d, es, false, &lv)) != FA_OK ||
         (rc = resolve_layout(c->out, c->batch, c->seq_len_q, c->heads, d, es, true, &lo)) != FA_OK)
         return rc;
+    int size, sinks;
+    if ((rc = resolve_window(window, c->q_doc, score_farthest(*c), &size, &sinks)) != FA_OK) return rc;
     if (!q || !out || (c->seq_len_k > 0 && (!k || !v))) return FA_ERR_INVALID_ARG;
     const int D = ops_pad_d(d);
     if (c->batch * c->heads > kOpsMaxGrid || (c->seq_len_q + 31) / 32 * c->batch * c->heads > kOpsMaxGrid)
@@ -507,7 +533,8 @@ int fa_score_forward(void* stream_, const fa_score_config* c, const void* q, con
     const bool vec = vec_ok(q, lq, d) && vec_ok(k, lk, d) && vec_ok(v, lv, d) && ovec_ok(out, lo, es) &&
                      cap_ok(c->dtype, c->softcap);
 
-    if (score_takes_rows(*c, g_dev[dev].num_cus)) {
+    const size_t keys = window_keys(c->seq_len_k, size, sinks, c->seq_len_q, !c->causal || c->prefix);
+    if (score_takes_rows(*c, keys, g_dev[dev].num_cus)) {
         RowsParams p{};
         p.q = q, p.k = k, p.v = v, p.out = out, p.lse = lse;
         p.slopes = c->slopes, p.q_doc = c->q_doc, p.k_doc = c->k_doc, p.prefix = c->causal ? c->prefix : nullptr;
@@ -517,10 +544,12 @@ int fa_score_forward(void* stream_, const fa_score_config* c, const void* q, con
         p.n = static_cast<int>(c->seq_len_q), p.sk = static_cast<int>(c->seq_len_k), p.d = static_cast<int>(d);
         p.causal = c->causal ? 1 : 0, p.q_start = static_cast<int>(c->q_start);
         p.scale_log2e = sc.scale_log2e, p.cap_in = sc.cap_in, p.cap_log2e = sc.cap_log2e;
-        return run_rows(dev, stream, c->dtype, D, vec, &p, c->seq_len_k);
+        p.window = size, p.sinks = sinks;
+        return run_rows(dev, stream, c->dtype, D, vec, &p, keys);
     }
     ScoreParams p{};
     fill_score(*c, sc, &p);
+    p.window = size, p.sinks = sinks;
     p.q = q, p.k = k, p.v = v, p.out = out, p.lse = lse;
     p.qs = lq.st, p.ks = lk.st, p.vs = lv.st, p.os = lo.st;
     const ScoreTiles tiles = score_tiles(*c, D, vec, c->seq_len_q, c->batch * c->heads, g_dev[dev].num_cus);
@@ -538,12 +567,10 @@ int fa_score_forward(void* stream_, const fa_score_config* c, const void* q, con
         rc = ops_launch(dev, of_type(kScoreModule, c->dtype), name, c->batch * c->heads * p.nqb, 256, &p, stream);
     }
     return ws.done(stream, rc);
-} catch (...) {   // no memory for the tables of modules, kernels and workspaces
-    return FA_ERR_ALLOC;
 }
 
-int fa_score_backward(void* stream_, const fa_score_config* c, const void* q, const void* k, const void* v,
-                      const void* out, const float* lse, const void* dout, void* dq, void* dk, void* dv) try {
+int score_backward(void* stream_, const fa_score_config* c, const fa_window* window, const void* q, const void* k,
+                   const void* v, const void* out, const float* lse, const void* dout, void* dq, void* dk, void* dv) {
     int rc = check_score(c);
     if (rc != FA_OK) return rc;
     if (c->batch == 0 || c->heads == 0 || c->d_head == 0) return FA_OK;
@@ -561,6 +588,8 @@ int fa_score_backward(void* stream_, const fa_score_config* c, const void* q, co
         (rc = resolve_layout(c->dk, c->batch, sk, c->kv_heads, d, es, true, &ldk)) != FA_OK ||
         (rc = resolve_layout(c->dv, c->batch, sk, c->kv_heads, d, es, true, &ldv)) != FA_OK)
         return rc;
+    int size, sinks;
+    if ((rc = resolve_window(window, c->q_doc, score_farthest(*c), &size, &sinks)) != FA_OK) return rc;
     if (sq > 0 && (!q || !out || !lse || !dout)) return FA_ERR_INVALID_ARG;
     if (sk > 0 && (!k || !v)) return FA_ERR_INVALID_ARG;
     const int D = ops_pad_d(d);
@@ -573,6 +602,7 @@ int fa_score_backward(void* stream_, const fa_score_config* c, const void* q, co
     const hipStream_t stream = static_cast<hipStream_t>(stream_);
     ScoreParams p{};
     fill_score(*c, sc, &p);
+    p.window = size, p.sinks = sinks;
     p.q = q, p.k = k, p.v = v, p.out_in = out, p.dout = dout, p.lse_in = lse;
     p.dq = dq, p.dk = dk, p.dv = dv;
     p.qs = lq.st, p.ks = lk.st, p.vs = lv.st, p.os = lo.st, p.dos = ldo.st;
@@ -616,6 +646,78 @@ int fa_score_backward(void* stream_, const fa_score_config* c, const void* q, co
         }
     }
     return ws.done(stream, rc);
+}
+
+int tree_attention(void* stream, const fa_tree_config* c, const fa_window* window, const fa_kv_cache* cache,
+                   const void* q, void* out, float* lse) {
+    OpsLayout ck, cv, lq, lo;
+    size_t capacity = 0;
+    int rc = check_cache(cache, &ck, &cv, &capacity);
+    if (rc != FA_OK) return rc;
+    if (!c) return FA_ERR_INVALID_ARG;
+    if (cache->batch == 0 || c->heads == 0 || c->n_tokens == 0 || cache->d_head == 0) return FA_OK;
+    if (cache->kv_heads == 0 || c->heads % cache->kv_heads != 0) return FA_ERR_INVALID_ARG;
+    if (c->heads > kOpsMaxSeq || c->n_tokens > kTreeMaxTokens) return FA_ERR_UNSUPPORTED;
+    const size_t es = elem_size(cache->dtype), d = cache->d_head, n = c->n_tokens;
+    ScoreScale sc;
+    if ((rc = resolve_scale(c->softmax_scale, c->softcap, d, &sc)) != FA_OK ||
+        (rc = resolve_layout(c->q, cache->batch, n, c->heads, d, es, false, &lq)) != FA_OK ||
+        (rc = resolve_layout(c->out, cache->batch, n, c->heads, d, es, true, &lo)) != FA_OK)
+        return rc;
+    int size, sinks;
+    if ((rc = resolve_window(window, false, kWindowMaxPos, &size, &sinks)) != FA_OK) return rc;
+    if (!q || !out) return FA_ERR_INVALID_ARG;
+    if (cache->batch * c->heads > kOpsMaxGrid) return FA_ERR_UNSUPPORTED;
+    RowsParams p{};
+    p.q = q, p.k = cache->k, p.v = cache->v, p.out = out, p.lse = lse;
+    p.slopes = c->slopes, p.lens = cache->lens, p.table = cache->block_table;
+    p.pos = c->positions, p.mask = c->mask;
+    p.qs = lq.st, p.ks = ck.st, p.vs = cv.st, p.os = lo.st;
+    p.batch = static_cast<int>(cache->batch), p.heads = static_cast<int>(c->heads);
+    p.kv_heads = static_cast<int>(cache->kv_heads), p.group = static_cast<int>(c->heads / cache->kv_heads);
+    p.n = static_cast<int>(n), p.sk = static_cast<int>(capacity), p.d = static_cast<int>(d);
+    p.page_shift = page_shift(*cache);
+    p.n_pages = static_cast<int>(cache->n_pages), p.pages_per_seq = static_cast<int>(cache->pages_per_seq);
+    p.mask_words = static_cast<int>((n + 63) / 64), p.mask_shared = c->mask_shared ? 1 : 0;
+    p.window = size, p.sinks = sinks;
+    const bool vec = vec_ok(q, lq, d) && vec_ok(cache->k, ck, d) && vec_ok(cache->v, cv, d) && ovec_ok(out, lo, es) &&
+                     cap_ok(cache->dtype, c->softcap);
+    p.scale_log2e = sc.scale_log2e, p.cap_in = sc.cap_in, p.cap_log2e = sc.cap_log2e;
+    int dev;
+    if ((rc = ops_begin(&dev, of_type(kCacheModule, cache->dtype))) != FA_OK) return rc;
+    return run_rows(dev, static_cast<hipStream_t>(stream), cache->dtype, ops_pad_d(d), vec, &p,
+                    window_keys(capacity, size, sinks, n, false));
+}
+
+}  // namespace
+
+extern "C" {
+
+int fa_score_forward(void* stream, const fa_score_config* c, const void* q, const void* k, const void* v, void* out,
+                     float* lse) try {
+    return score_forward(stream, c, nullptr, q, k, v, out, lse);
+} catch (...) {   // no memory for the tables of modules, kernels and workspaces
+    return FA_ERR_ALLOC;
+}
+
+int fa_window_forward(void* stream, const fa_score_config* c, const fa_window* window, const void* q, const void* k,
+                      const void* v, void* out, float* lse) try {
+    return score_forward(stream, c, window, q, k, v, out, lse);
+} catch (...) {   // no memory for the tables of modules, kernels and workspaces
+    return FA_ERR_ALLOC;
+}
+
+int fa_score_backward(void* stream, const fa_score_config* c, const void* q, const void* k, const void* v,
+                      const void* out, const float* lse, const void* dout, void* dq, void* dk, void* dv) try {
+    return score_backward(stream, c, nullptr, q, k, v, out, lse, dout, dq, dk, dv);
+} catch (...) {   // no memory for the tables of modules, kernels and workspaces
+    return FA_ERR_ALLOC;
+}
+
+int fa_window_backward(void* stream, const fa_score_config* c, const fa_window* window, const void* q, const void* k,
+                       const void* v, const void* out, const float* lse, const void* dout, void* dq, void* dk,
+                       void* dv) try {
+    return score_backward(stream, c, window, q, k, v, out, lse, dout, dq, dk, dv);
 } catch (...) {   // no memory for the tables of modules, kernels and workspaces
     return FA_ERR_ALLOC;
 }
@@ -766,39 +868,14 @@ int fa_cache_append(void* stream, const fa_kv_cache* cache, const fa_append_conf
 
 int fa_tree_attention(void* stream, const fa_tree_config* c, const fa_kv_cache* cache, const void* q, void* out,
                       float* lse) try {
-    OpsLayout ck, cv, lq, lo;
-    size_t capacity = 0;
-    int rc = check_cache(cache, &ck, &cv, &capacity);
-    if (rc != FA_OK) return rc;
-    if (!c) return FA_ERR_INVALID_ARG;
-    if (cache->batch == 0 || c->heads == 0 || c->n_tokens == 0 || cache->d_head == 0) return FA_OK;
-    if (cache->kv_heads == 0 || c->heads % cache->kv_heads != 0) return FA_ERR_INVALID_ARG;
-    if (c->heads > kOpsMaxSeq || c->n_tokens > kTreeMaxTokens) return FA_ERR_UNSUPPORTED;
-    const size_t es = elem_size(cache->dtype), d = cache->d_head, n = c->n_tokens;
-    ScoreScale sc;
-    if ((rc = resolve_scale(c->softmax_scale, c->softcap, d, &sc)) != FA_OK ||
-        (rc = resolve_layout(c->q, cache->batch, n, c->heads, d, es, false, &lq)) != FA_OK ||
-        (rc = resolve_layout(c->out, cache->batch, n, c->heads, d, es, true, &lo)) != FA_OK)
-        return rc;
-    if (!q || !out) return FA_ERR_INVALID_ARG;
-    if (cache->batch * c->heads > kOpsMaxGrid) return FA_ERR_UNSUPPORTED;
-    RowsParams p{};
-    p.q = q, p.k = cache->k, p.v = cache->v, p.out = out, p.lse = lse;
-    p.slopes = c->slopes, p.lens = cache->lens, p.table = cache->block_table;
-    p.pos = c->positions, p.mask = c->mask;
-    p.qs = lq.st, p.ks = ck.st, p.vs = cv.st, p.os = lo.st;
-    p.batch = static_cast<int>(cache->batch), p.heads = static_cast<int>(c->heads);
-    p.kv_heads = static_cast<int>(cache->kv_heads), p.group = static_cast<int>(c->heads / cache->kv_heads);
-    p.n = static_cast<int>(n), p.sk = static_cast<int>(capacity), p.d = static_cast<int>(d);
-    p.page_shift = page_shift(*cache);
-    p.n_pages = static_cast<int>(cache->n_pages), p.pages_per_seq = static_cast<int>(cache->pages_per_seq);
-    p.mask_words = static_cast<int>((n + 63) / 64), p.mask_shared = c->mask_shared ? 1 : 0;
-    const bool vec = vec_ok(q, lq, d) && vec_ok(cache->k, ck, d) && vec_ok(cache->v, cv, d) && ovec_ok(out, lo, es) &&
-                     cap_ok(cache->dtype, c->softcap);
-    p.scale_log2e = sc.scale_log2e, p.cap_in = sc.cap_in, p.cap_log2e = sc.cap_log2e;
-    int dev;
-    if ((rc = ops_begin(&dev, of_type(kCacheModule, cache->dtype))) != FA_OK) return rc;
-    return run_rows(dev, static_cast<hipStream_t>(stream), cache->dtype, ops_pad_d(d), vec, &p, capacity);
+    return tree_attention(stream, c, nullptr, cache, q, out, lse);
+} catch (...) {   // no memory for the tables of modules, kernels and workspaces
+    return FA_ERR_ALLOC;
+}
+
+int fa_window_tree_attention(void* stream, const fa_tree_config* c, const fa_window* window, const fa_kv_cache* cache,
+                             const void* q, void* out, float* lse) try {
+    return tree_attention(stream, c, window, cache, q, out, lse);
 } catch (...) {   // no memory for the tables of modules, kernels and workspaces
     return FA_ERR_ALLOC;
 }

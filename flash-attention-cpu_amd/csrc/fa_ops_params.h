@@ -42,6 +42,7 @@ struct ScoreParams {
     OpsStrides qs, ks, vs, os, dos, dqs, dks, dvs;
     int batch, heads, kv_heads, group, sq, sk, d;
     int causal, q_start;
+    int window, sinks;        // window 0: none
     int nqb;                  // query (dK/dV: key) blocks a slice
     int splits;               // dK/dV: workgroups that share a key block, each some heads of the group
     float* part;              // their sums: [dK, dV][split][batch, kv head][key][padded d]
@@ -50,6 +51,9 @@ struct ScoreParams {
     float cap_in;             // 2 log2(e) scale / softcap: exponent of the cap's tanh
     float cap_log2e;          // softcap * log2(e); 0: no cap
 };
+
+// Largest position of a token over a cache where a window looks at it, and largest window that hides anything.
+constexpr int kWindowMaxPos = 1 << 30;
 
 // Waves of a workgroup of the streaming rows kernel, by the bytes of a padded row (up to 512): each has
 // two slots of 32 rows of K and V in LDS.
@@ -69,6 +73,7 @@ struct RowsParams {
     OpsStrides qs, ks, vs, os;
     int batch, heads, kv_heads, group, n, sk, d;   // n: tokens; sk: keys (tree: capacity)
     int causal, q_start;
+    int window, sinks;        // window 0: none
     int page_shift, n_pages, pages_per_seq;
     int mask_words, mask_shared;
     int nrb, block_rows;      // row blocks of a (batch, kv head), and rows of one

@@ -72,12 +72,14 @@ template <typename Test>
 struct Stages {
     uint64_t vis = 0, part = 0;
     int base, count, lane;
+    int skip_from = 0, skip_to = 0;   // 64-stage runs that start in here hold no visible pair
     Test test;
     __device__ __forceinline__ Stages(int n, int lane_, Test t) : base(-64), count(n), lane(lane_), test(t) {}
     // next stage (-1: none); *masked: it needs the mask (an int: uniform flags stay in one scalar register)
     __device__ __forceinline__ int next(int* masked) {
         while (vis == 0) {
             base += 64;
+            if (base >= skip_from && base < skip_to) base = skip_to;
             if (base >= count) return -1;
             bool p = false, v = false;
             if (base + lane < count) v = test(base + lane, &p);
@@ -105,9 +107,15 @@ __device__ __forceinline__ int key_limit(const ScoreParams& p, int prefix, int p
     return p.causal ? max(pos + 1, prefix) : 0x7fffffff;
 }
 
+// Whether the window hides key `key` from a query at position pos.
+__device__ __forceinline__ bool window_hides(const ScoreParams& p, int pos, int key) {
+    return key >= p.sinks && (key <= pos - p.window || key >= pos + p.window);
+}
+
 // Whether query `row` sees key `key`.
 __device__ __forceinline__ bool pair_seen(const ScoreParams& p, int prefix, int b, int row, int key) {
     if (key >= key_limit(p, prefix, p.q_start + row)) return false;
+    if (p.window && window_hides(p, p.q_start + row, key)) return false;
     if (!p.q_doc) return true;
     const int d = p.q_doc[(int64_t)b * p.sq + row];
     return d >= 0 && d == p.k_doc[(int64_t)b * p.sk + key];
@@ -140,6 +148,21 @@ __device__ __forceinline__ bool docs_meet(const DocRange& a, const DocRange& b, 
     return a.lo <= b.hi && b.lo <= a.hi;
 }
 
+// Whether the windows of queries at positions [lo, hi] reach keys [k0, k1); *part: whether they hide some pair.
+__device__ __forceinline__ bool window_meets(const ScoreParams& p, int lo, int hi, int k0, int k1, bool* part) {
+    if (k1 > p.sinks && (k0 <= hi - p.window || k1 - 1 >= lo + p.window)) *part = true;
+    return k0 < p.sinks || (k1 - 1 > lo - p.window && k0 < hi + p.window);
+}
+// The walked stages that a window leaves: rows before `sinks` (where they are walked for their own sake) and rows
+// [lo, hi], of n stages of ROWS.
+template <int ROWS, typename S>
+__device__ __forceinline__ void window_stages(S* s, int sinks, int lo, int hi, int n) {
+    const int first = (sinks + ROWS - 1) / ROWS;
+    s->count = min(n, max(first, hi < 0 ? 0 : hi / ROWS + 1));
+    s->skip_from = (first + 63) & ~63;
+    s->skip_to = lo <= 0 ? 0 : lo / ROWS & ~63;
+}
+
 // One value a lane from global memory into LDS, zero past n.
 __device__ __forceinline__ void fill_words(void* dst, const void* src, int n, int lane) {
     const int bytes = 4 * min(max(n, 0), 64);   // (of 2^30 words the size would not fit)
@@ -164,8 +187,21 @@ __device__ __forceinline__ bool key_stage(const ScoreParams& p, int prefix, int 
         v = k0 <= p.q_start + q1 - 1 || k0 < prefix;
         if (!(k1 - 1 <= p.q_start + q0 || k1 <= prefix)) *part = true;
     }
+    if (p.window && v) v = window_meets(p, p.q_start + q0, p.q_start + q1 - 1, k0, k1, part);
     if (docs && v) v = docs_meet(qr, doc_range(krng, k0 / kDocTile), part);
     return v;
+}
+// The stages of keys that the windows of queries [q0, q1) leave.
+template <int SK, typename S>
+__device__ __forceinline__ void window_keys(const ScoreParams& p, S* s, int q0, int q1) {
+    if (!p.window) return;
+    const int up = p.causal && !p.prefix ? 0 : p.window - 1;
+    window_stages<SK>(s, p.sinks, p.q_start + q0 - p.window + 1, p.q_start + q1 - 1 + up, s->count);
+}
+// Whether rows of a wave at positions [lo, hi] see a key of [k0, k1), as far as the window tells.
+__device__ __forceinline__ bool window_active(const ScoreParams& p, int lo, int hi, int k0, int k1) {
+    bool part;
+    return !p.window || window_meets(p, lo, hi, k0, k1, &part);
 }
 
 // ---------------------------------------------------------------------------
@@ -237,6 +273,7 @@ __device__ __forceinline__ void score_forward(const ScoreParams& p) {
     }
     auto test = [&](int st, bool* part) -> bool { return key_stage<SK>(p, prefix, st, q0, q1, docs, qr, krng, part); };
     Stages<decltype(test)> stages((p.sk + SK - 1) / SK, lane, test);
+    window_keys<SK>(p, &stages, q0, q1);
     const Fill kfill(p.ks.s, p.d, wave, lane), vfill(p.vs.s, p.d, wave, lane);
     auto fill_k = [&](int st, T* dst, int* ids) {
         kfill(dst, K, st * SK, p.sk);
@@ -312,6 +349,17 @@ __device__ __forceinline__ void score_forward(const ScoreParams& p) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
                     if (key + r >= limit[t]) s[t][b][r] = OPS_NEG_INF;
+        }
+        if (p.window) {
+            const ScoreParams lp = late_params<ScoreParams>();
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+                for (int b = 0; b < KB; ++b)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (window_hides(lp, lp.q_start + row0 + 16 * t + li, k0 + koff + 16 * b + 4 * g + r))
+                            s[t][b][r] = OPS_NEG_INF;
         }
     };
     v8 pb[MT][NCH];
@@ -395,7 +443,8 @@ __device__ __forceinline__ void score_forward(const ScoreParams& p) {
     auto active = [&](int st) -> int {
         if (st < 0 || row0 >= p.sq) return false;
         const int k0 = st * SK + koff;
-        return k0 < p.sk && (!p.causal || k0 <= p.q_start + row0 + 16 * MT - 1 || k0 < prefix);
+        return k0 < p.sk && (!p.causal || k0 <= p.q_start + row0 + 16 * MT - 1 || k0 < prefix) &&
+               window_active(p, p.q_start + row0, p.q_start + row0 + 16 * MT - 1, k0, k0 + SW);
     };
 
     // At 128 columns and more, waves in their products go before waves of the other workgroup in their softmax
@@ -679,6 +728,7 @@ __device__ __forceinline__ void score_dq(const ScoreParams& p) {
     }
     auto test = [&](int st, bool* part) -> bool { return key_stage<SK>(p, prefix, st, q0, q1, docs, qr, krng, part); };
     Stages<decltype(test)> stages((p.sk + SK - 1) / SK, lane, test);
+    window_keys<SK>(p, &stages, q0, q1);
     const Fill kfill(p.ks.s, p.d, wave, lane), vfill(p.vs.s, p.d, wave, lane);
     auto fill = [&](int st, T* k, T* v, int* ids) {
         kfill(k, K, st * SK, p.sk);
@@ -688,7 +738,8 @@ __device__ __forceinline__ void score_dq(const ScoreParams& p) {
     auto active = [&](int st) -> int {
         if (row0 >= p.sq) return false;
         const int k0 = st * SK + koff;
-        return k0 < p.sk && (!p.causal || k0 <= p.q_start + row0 + 16 * MT - 1 || k0 < prefix);
+        return k0 < p.sk && (!p.causal || k0 <= p.q_start + row0 + 16 * MT - 1 || k0 < prefix) &&
+               window_active(p, p.q_start + row0, p.q_start + row0 + 16 * MT - 1, k0, k0 + 32 * NCH);
     };
 
     int masked = 0, masked_next = 0;
@@ -762,6 +813,12 @@ __device__ __forceinline__ void score_dq(const ScoreParams& p) {
 #pragma unroll
                             for (int r = 0; r < 4; ++r)
                                 if (key + r >= limit[t]) x[b][r] = y[b][r] = 0.0f;
+                            if (p.window) {
+                                const ScoreParams lp = late_params<ScoreParams>();
+#pragma unroll
+                                for (int r = 0; r < 4; ++r)
+                                    if (window_hides(lp, pos, key + r)) x[b][r] = y[b][r] = 0.0f;
+                            }
                         }
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
@@ -965,11 +1022,15 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
             v = p.q_start + q1 - 1 >= kbeg || kbeg < prefix;
             if (!(p.q_start + q0 >= kend - 1 || kend <= prefix)) *part = true;
         }
+        if (p.window && v) v = window_meets(p, p.q_start + q0, p.q_start + q1 - 1, kbeg, kend, part);
         if (docs && v) v = docs_meet(kr, doc_range(qrng, q0 / kDocTile), part);
         return v;
     };
     const int nst = (p.sq + SQ - 1) / SQ;
     Stages<decltype(test)> stages(nst, lane, test);
+    if (p.window && kbeg >= p.sinks)
+        window_stages<SQ>(&stages, 0, kbeg - p.q_start - (p.causal && !p.prefix ? 0 : p.window - 1),
+                          kend - 1 - p.q_start + p.window - 1, nst);
     const Fill qfill(p.qs.s, p.d, wave, lane), ofill(p.dos.s, p.d, wave, lane);
     // the next (head, stage): the stages of one head of the group after the other
     int head = 0;
@@ -1007,7 +1068,9 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
     };
     auto active = [&](int st) -> int {
         if (key0 >= p.sk) return false;
-        return st * SQ + qoff < p.sq && (!p.causal || p.q_start + st * SQ + qoff + 32 * NCH - 1 >= key0 || key0 < prefix);
+        const int lo = p.q_start + st * SQ + qoff, hi = lo + 32 * NCH - 1;
+        return st * SQ + qoff < p.sq && (!p.causal || hi >= key0 || key0 < prefix) &&
+               window_active(p, lo, hi, key0, key0 + 16 * MT);
     };
 
     int masked = 0, masked_next = 0;
@@ -1091,6 +1154,12 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
 #pragma unroll
                             for (int r = 0; r < 4; ++r)
                                 if (key >= key_limit(p, prefix, pos + r) || lse2[r] == -OPS_NEG_INF) x[r] = y[r] = 0.0f;
+                            if (p.window) {
+                                const ScoreParams lp = late_params<ScoreParams>();
+#pragma unroll
+                                for (int r = 0; r < 4; ++r)
+                                    if (window_hides(lp, pos + r, key)) x[r] = y[r] = 0.0f;
+                            }
                         }
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {

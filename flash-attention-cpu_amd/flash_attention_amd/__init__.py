@@ -73,6 +73,7 @@ EXPORTED_SYMBOLS = (
     "fa_naive_attention", "fa_naive_device",
     "fa_init", "fa_describe_launch", "fa_probe_launch",
     "fa_score_forward", "fa_score_backward", "fa_rotary_init", "fa_rotary", "fa_cache_append", "fa_tree_attention",
+    "fa_window_forward", "fa_window_backward", "fa_window_tree_attention",
 )
 
 
@@ -419,6 +420,6 @@ def init() -> None:
 # Attention with modified scores, rotary positions, key / value cache (operators.py)
 ROTARY_NONE, ROTARY_LINEAR, ROTARY_NTK, ROTARY_YARN = 0, 1, 2, 3
 from .operators import (  # noqa: E402
-    AppendConfig, KvCache, RotaryConfig, RotaryTensor, ScoreConfig, Strides, TreeConfig, append_config,
+    AppendConfig, KvCache, RotaryConfig, RotaryTensor, ScoreConfig, Strides, TreeConfig, Window, append_config,
     cache_append_device, kv_cache, rotary_config, rotary_device, rotary_tensor, score_attention_backward_device,
-    score_attention_device, score_config, tree_attention_device, tree_config)
+    score_attention_device, score_config, tree_attention_device, tree_config, window)

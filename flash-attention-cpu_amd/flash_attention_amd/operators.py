@@ -1,6 +1,6 @@
 """Attention with modified scores, rotary positions and the key / value cache.
 
-Python view of the fa_score_*, fa_rotary*, fa_cache_append and
+Python view of the fa_score_*, fa_window_*, fa_rotary*, fa_cache_append and
 fa_tree_attention entry points of include/fa_hip.h, which defines what they
 compute.  They have no counterpart in the reference crate.
 
@@ -34,6 +34,12 @@ class ScoreConfig(ctypes.Structure):
                 ("seq_len_k", _SZ), ("d_head", _SZ), ("q_start", ctypes.c_int64), ("softmax_scale", _F),
                 ("softcap", _F), ("slopes", _P), ("q_doc", _P), ("k_doc", _P), ("prefix", _P),
                 *((n, Strides) for n in ("q", "k", "v", "out", "dout", "dq", "dk", "dv"))]
+
+
+class Window(ctypes.Structure):
+    """fa_window."""
+
+    _fields_ = [("size", ctypes.c_int64), ("sinks", ctypes.c_int64)]
 
 
 class RotaryConfig(ctypes.Structure):
@@ -82,6 +88,9 @@ def declare(lib: ctypes.CDLL) -> None:
         "fa_rotary": [_P, ptr(RotaryConfig), _SZ, _SZ, _P, _I, ptr(RotaryTensor), _P, _P, ptr(RotaryTensor), _P, _P],
         "fa_cache_append": [_P, ptr(KvCache), ptr(AppendConfig), _P, _P, _P, _P, _P],
         "fa_tree_attention": [_P, ptr(TreeConfig), ptr(KvCache), _P, _P, _P],
+        "fa_window_forward": [_P, ptr(ScoreConfig), ptr(Window), _P, _P, _P, _P, _P],
+        "fa_window_backward": [_P, ptr(ScoreConfig), ptr(Window)] + [_P] * 9,
+        "fa_window_tree_attention": [_P, ptr(TreeConfig), ptr(Window), ptr(KvCache), _P, _P, _P],
     }.items():
         f = getattr(lib, name, None)   # None: a library built before there were operators
         if f is not None:
@@ -135,18 +144,30 @@ def score_config(dtype: int, batch: int, heads: int, kv_heads: int, seq_len_q: i
     return c
 
 
+def window(size: int, sinks: int = 0) -> Window:
+    """A sliding window: a query sees keys less than `size` away, and the first `sinks`."""
+    return Window(int(size), int(sinks))
+
+
 def score_attention_device(cfg: ScoreConfig, q_ptr: int, k_ptr: int, v_ptr: int, out_ptr: int, lse_ptr: int = 0,
-                           stream: int = 0) -> None:
-    """Queue softmax attention with modified scores (fa_score_forward)."""
-    _check(_lib().fa_score_forward(stream, cfg, q_ptr, k_ptr, v_ptr, out_ptr, lse_ptr))
+                           stream: int = 0, window: Window | None = None) -> None:
+    """Queue softmax attention with modified scores (fa_score_forward; in a window: fa_window_forward)."""
+    if window is None:
+        _check(_lib().fa_score_forward(stream, cfg, q_ptr, k_ptr, v_ptr, out_ptr, lse_ptr))
+    else:
+        _check(_lib().fa_window_forward(stream, cfg, window, q_ptr, k_ptr, v_ptr, out_ptr, lse_ptr))
 
 
 def score_attention_backward_device(cfg: ScoreConfig, q_ptr: int, k_ptr: int, v_ptr: int, out_ptr: int, lse_ptr: int,
-                                    dout_ptr: int, dq_ptr: int, dk_ptr: int, dv_ptr: int, stream: int = 0) -> None:
-    """Queue its gradients (fa_score_backward); out and lse are the forward's.  A
+                                    dout_ptr: int, dq_ptr: int, dk_ptr: int, dv_ptr: int, stream: int = 0,
+                                    window: Window | None = None) -> None:
+    """Queue its gradients (fa_score_backward, fa_window_backward); out and lse are the forward's.  A
     gradient whose pointer is 0 is not computed."""
-    _check(_lib().fa_score_backward(stream, cfg, q_ptr, k_ptr, v_ptr, out_ptr, lse_ptr, dout_ptr, dq_ptr, dk_ptr,
-                                    dv_ptr))
+    args = (q_ptr, k_ptr, v_ptr, out_ptr, lse_ptr, dout_ptr, dq_ptr, dk_ptr, dv_ptr)
+    if window is None:
+        _check(_lib().fa_score_backward(stream, cfg, *args))
+    else:
+        _check(_lib().fa_window_backward(stream, cfg, window, *args))
 
 
 def rotary_config(dtype: int, d_head: int, rot_dim: int | None = None, interleaved: bool = False,
@@ -208,6 +229,9 @@ def tree_config(heads: int, n_tokens: int, mask_ptr: int = 0, mask_shared: bool 
 
 
 def tree_attention_device(cfg: TreeConfig, cache: KvCache, q_ptr: int, out_ptr: int, lse_ptr: int = 0,
-                          stream: int = 0) -> None:
-    """Queue attention of drafted tokens over the cache (fa_tree_attention)."""
-    _check(_lib().fa_tree_attention(stream, cfg, cache, q_ptr, out_ptr, lse_ptr))
+                          stream: int = 0, window: Window | None = None) -> None:
+    """Queue attention of drafted tokens over the cache (fa_tree_attention, fa_window_tree_attention)."""
+    if window is None:
+        _check(_lib().fa_tree_attention(stream, cfg, cache, q_ptr, out_ptr, lse_ptr))
+    else:
+        _check(_lib().fa_window_tree_attention(stream, cfg, window, cache, q_ptr, out_ptr, lse_ptr))

@@ -311,6 +311,30 @@ int fa_score_forward(void* stream, const fa_score_config* cfg, const void* q, co
 int fa_score_backward(void* stream, const fa_score_config* cfg, const void* q, const void* k, const void* v,
                       const void* out, const float* lse, const void* dout, void* dq, void* dk, void* dv);
 
+/* ---- sliding windows -------------------------------------------------------
+ * No counterpart in the reference.  The calls above and fa_tree_attention
+ * where a query besides sees only keys near it and the first ones (sinks):
+ *     |i' - j| < size  or  j < sinks
+ * (causal: the last `size` keys, its own among them; not causal: both sides).
+ * Keys out of reach are not read.  Results of a window that hides nothing are those
+ * of the plain calls, and so are those of window NULL.  Sinks and documents
+ * together are refused (FA_ERR_UNSUPPORTED): the first keys belong to the first document alone;
+ * so are, with a window that hides something, distances that may pass 2^30.
+ *
+ * Over a cache the position of filled rows is their row number, that of
+ * drafted ones positions[b][t], at least lens[b] (smaller ones count as that), and
+ * a token sees what its mask shows if it lies less than `size` behind it or is a
+ * row before `sinks` (positions past 2^30 count as that).  Pages that no token reaches may be gone from the table. */
+typedef struct fa_window {
+    int64_t size;    /* at least 1 */
+    int64_t sinks;   /* 0: none */
+} fa_window;
+int fa_window_forward(void* stream, const fa_score_config* cfg, const fa_window* window, const void* q, const void* k,
+                      const void* v, void* out, float* lse);
+int fa_window_backward(void* stream, const fa_score_config* cfg, const fa_window* window, const void* q,
+                       const void* k, const void* v, const void* out, const float* lse, const void* dout, void* dq,
+                       void* dk, void* dv);
+
 /* ---- rotary positions -------------------------------------------------------
  * No counterpart in the reference.  Column pairs of the first rot_dim columns
  * of each head row are rotated by position * 2 pi * turns[c]:
@@ -408,6 +432,9 @@ typedef struct fa_tree_config {
 } fa_tree_config;
 int fa_tree_attention(void* stream, const fa_tree_config* cfg, const fa_kv_cache* cache, const void* q, void* out,
                       float* lse);
+/* The same in a sliding window (see there). */
+int fa_window_tree_attention(void* stream, const fa_tree_config* cfg, const fa_window* window,
+                             const fa_kv_cache* cache, const void* q, void* out, float* lse);
 
 /* ---- naive attention (materialised scores) -------------------------------
  * naive_attention -- src/naive.rs:14-75: the textbook O(seq_q * seq_k)
