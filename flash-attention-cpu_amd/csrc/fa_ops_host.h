@@ -11,7 +11,7 @@
 namespace {
 
 // Code objects: those of score attention and of the cache one a type (FA_DTYPE_*).
-enum OpsModule { kRotaryModule, kScoreModule, kCacheModule = kScoreModule + 3, kOpsModules = kCacheModule + 3 };
+enum OpsModule { kRotaryModule, kScoreModule, kCacheModule = kScoreModule + 3, kNormModule = kCacheModule + 3, kOpsModules };
 OpsModule of_type(OpsModule m, int dtype) { return static_cast<OpsModule>(m + dtype); }
 
 struct OpsState {
@@ -39,7 +39,7 @@ constexpr size_t kOpsMaxTokens = size_t(1) << 31;   // of a rotary launch: a thr
 int ops_module(int dev, OpsModule which) {
     static const char* const files[] = {"fa_rotary.hsaco",     "fa_score_f32.hsaco",  "fa_score_bf16.hsaco",
                                         "fa_score_f16.hsaco",  "fa_cache_f32.hsaco",  "fa_cache_bf16.hsaco",
-                                        "fa_cache_f16.hsaco"};
+                                        "fa_cache_f16.hsaco",  "fa_norm.hsaco"};
     OpsState& s = g_ops[dev];
     std::call_once(s.once[which], [&] {
         std::string path = module_path();
@@ -689,6 +689,82 @@ int tree_attention(void* stream, const fa_tree_config* c, const fa_window* windo
                     window_keys(capacity, size, sinks, n, false));
 }
 
+// Norms with rotary positions: one tensor of a launch, checked.
+struct NormCheck {
+    bool wide = true;
+    int heads = 0;   // of all tensors
+};
+int add_norm_tensor(NormParams* p, NormCheck* check, size_t batch, size_t seq, size_t d, size_t es, size_t heads,
+                    const void* x, const fa_strides& xs, const void* dy, const fa_strides* dys, void* out,
+                    const OpsLayout& lo, bool norm, const void* w, bool cache) {
+    OpsLayout lx, ldy;
+    int rc = resolve_layout(xs, batch, seq, heads, d, es, false, &lx);
+    if (rc == FA_OK && dys) rc = resolve_layout(*dys, batch, seq, heads, d, es, false, &ldy);
+    if (rc != FA_OK) return rc;
+    NormTensor& t = p->t[p->nt++];
+    t.x = x, t.dy = dy, t.w = w, t.out = out;
+    t.xs = lx.st, t.dys = ldy.st, t.outs = lo.st;
+    t.heads = static_cast<int>(heads);
+    t.norm = norm ? 1 : 0, t.cache = cache ? 1 : 0;
+    check->wide = check->wide && lx.aligned16 && ldy.aligned16 && lo.aligned16 && aligned16(x) && aligned16(dy) && aligned16(out);
+    check->heads += t.heads;
+    return FA_OK;
+}
+bool same_strides(const OpsStrides& a, const OpsStrides& b) { return a.b == b.b && a.s == b.s && a.h == b.h; }
+
+void fill_norm(const fa_rotary_config& c, const fa_head_norm& norm, size_t batch, size_t seq, const int32_t* positions,
+               NormParams* p) {
+    p->batch = static_cast<int>(batch);
+    p->seq = static_cast<int>(seq);
+    p->d = static_cast<int>(c.d_head);
+    p->rot = static_cast<int>(c.rot_dim);
+    p->interleaved = c.interleaved ? 1 : 0;
+    p->pos = positions;
+    p->gain = c.gain;
+    p->eps = norm.eps;
+    std::memcpy(p->turns, c.turns, sizeof(p->turns));
+}
+int check_norm(const fa_rotary_config* c, const fa_head_norm* n) {
+    const int rc = check_rotary(c);
+    if (rc != FA_OK) return rc;
+    return n && n->eps > 0.0f && std::isfinite(n->eps) ? FA_OK : FA_ERR_INVALID_ARG;
+}
+
+// Lanes of a row and tokens of a workgroup.
+int plan_norm(int dev, int dtype, bool wide, NormParams* p, bool* wide_out, size_t* grid) {
+    const int w = static_cast<int>(16 / elem_size(dtype));
+    const int run = p->interleaved ? p->rot : p->rot / 2;
+    wide = wide && run % w == 0 && (p->d - p->rot) % w == 0;
+    p->units = wide ? run / w + (p->d - p->rot) / w : p->rot / 2 + p->d - p->rot;
+    p->lanes = 1;
+    while (p->lanes < 64 && p->lanes < p->units) p->lanes *= 2;
+    const size_t slots = 256 / p->lanes, all = static_cast<size_t>(p->batch) * p->seq;
+    *grid = 0;
+    for (int i = 0; i < p->nt; ++i) {
+        NormTensor& t = p->t[i];
+        // some four rows a slot where that leaves workgroups enough
+        size_t tokens = 1;
+        while (tokens < kNormTokens && tokens * t.heads < 4 * slots &&
+               (all + 2 * tokens - 1) / (2 * tokens) >= 4 * static_cast<size_t>(g_dev[dev].num_cus))
+            tokens *= 2;
+        t.tokens = static_cast<int>(tokens);
+        const size_t blocks = (all + tokens - 1) / tokens;
+        if (blocks > kOpsMaxGrid) return FA_ERR_UNSUPPORTED;
+        t.blocks = static_cast<int>(blocks);
+        *grid += blocks;
+    }
+    *wide_out = wide;
+    return *grid > kOpsMaxGrid ? FA_ERR_UNSUPPORTED : FA_OK;
+}
+int launch_norm(int dev, hipStream_t stream, int dtype, NormParams* p, bool wide) {
+    size_t grid;
+    int rc = plan_norm(dev, dtype, wide, p, &wide, &grid);
+    if (rc != FA_OK) return rc;
+    char name[64];
+    std::snprintf(name, sizeof(name), "fa_norm_%s_%d", dtype_name(dtype), wide ? 1 : 0);
+    return ops_launch(dev, kNormModule, name, grid, kNormThreads, p, stream);
+}
+
 }  // namespace
 
 extern "C" {
@@ -802,6 +878,171 @@ int fa_rotary(void* stream, const fa_rotary_config* cfg, size_t batch, size_t se
     int dev;
     if ((rc = ops_begin(&dev, kRotaryModule)) != FA_OK) return rc;
     return launch_rotary(dev, static_cast<hipStream_t>(stream), cfg->dtype, &p, wide);
+} catch (...) {   // no memory for the tables of modules, kernels and workspaces
+    return FA_ERR_ALLOC;
+}
+
+int fa_norm_rotary(void* stream, const fa_rotary_config* cfg, const fa_head_norm* norm, size_t batch, size_t seq_len,
+                   const int32_t* positions, const fa_rotary_tensor* ql, const void* q, void* q_out,
+                   const fa_rotary_tensor* kl, const void* k, void* k_out) try {
+    int rc = check_norm(cfg, norm);
+    if (rc != FA_OK) return rc;
+    if (!ql) return FA_ERR_INVALID_ARG;
+    if (batch == 0 || seq_len == 0) return FA_OK;
+    if (batch > kOpsMaxSeq || seq_len > kOpsMaxSeq || batch * seq_len > kOpsMaxTokens) return FA_ERR_UNSUPPORTED;
+    if (!positions) return FA_ERR_INVALID_ARG;
+    NormParams p{};
+    NormCheck check;
+    const size_t d = cfg->d_head, es = elem_size(cfg->dtype);
+    for (int n = 0; n < (kl ? 2 : 1); ++n) {
+        const fa_rotary_tensor* t = n ? kl : ql;
+        const void* src = n ? k : q;
+        void* dst = n ? k_out : q_out;
+        if (t->heads == 0) continue;
+        if (t->heads > kOpsMaxSeq) return FA_ERR_UNSUPPORTED;
+        OpsLayout out;
+        if ((rc = resolve_layout(t->out, batch, seq_len, t->heads, d, es, true, &out)) != FA_OK) return rc;
+        if (!src || !dst) return FA_ERR_INVALID_ARG;
+        if ((rc = add_norm_tensor(&p, &check, batch, seq_len, d, es, t->heads, src, t->in, nullptr, nullptr, dst, out, true,
+                                  n ? norm->k_weight : norm->q_weight, false)) != FA_OK)
+            return rc;
+        // in place the layouts have to agree: a lane reads what it writes
+        if (src == dst && !same_strides(p.t[p.nt - 1].xs, out.st)) return FA_ERR_INVALID_ARG;
+    }
+    if (p.nt == 0) return FA_OK;
+    fill_norm(*cfg, *norm, batch, seq_len, positions, &p);
+    int dev;
+    if ((rc = ops_begin(&dev, kNormModule)) != FA_OK) return rc;
+    return launch_norm(dev, static_cast<hipStream_t>(stream), cfg->dtype, &p, check.wide);
+} catch (...) {   // no memory for the tables of modules, kernels and workspaces
+    return FA_ERR_ALLOC;
+}
+
+int fa_norm_rotary_backward(void* stream_, const fa_rotary_config* cfg, const fa_head_norm* norm, size_t batch,
+                            size_t seq_len, const int32_t* positions, const fa_norm_grad* qg, const void* q,
+                            const void* dq_out, void* dq, float* dq_weight, const fa_norm_grad* kg, const void* k,
+                            const void* dk_out, void* dk, float* dk_weight) try {
+    int rc = check_norm(cfg, norm);
+    if (rc != FA_OK) return rc;
+    if (!qg) return FA_ERR_INVALID_ARG;
+    if (batch > kOpsMaxSeq || seq_len > kOpsMaxSeq || (seq_len > 0 && batch > kOpsMaxTokens / seq_len))
+        return FA_ERR_UNSUPPORTED;
+    const bool any = batch > 0 && seq_len > 0;
+    if (any && !positions) return FA_ERR_INVALID_ARG;
+    NormParams p{};
+    NormCheck check;
+    const size_t d = cfg->d_head, es = elem_size(cfg->dtype);
+    bool weights = false;
+    for (int n = 0; n < (kg ? 2 : 1); ++n) {
+        const fa_norm_grad* t = n ? kg : qg;
+        const void *x = n ? k : q, *dy = n ? dk_out : dq_out;
+        void* dx = n ? dk : dq;
+        float* dw = n ? dk_weight : dq_weight;
+        if (t->heads > kOpsMaxSeq) return FA_ERR_UNSUPPORTED;
+        if (!dx && !dw) continue;
+        if (!any || t->heads == 0) {   // the sums of no rows: zeros
+            p.t[p.nt++].dw = dw;
+            weights = weights || dw;
+            continue;
+        }
+        OpsLayout out;
+        if ((rc = resolve_layout(t->dx, batch, seq_len, t->heads, d, es, true, &out)) != FA_OK) return rc;
+        if (!x || !dy) return FA_ERR_INVALID_ARG;
+        if ((rc = add_norm_tensor(&p, &check, batch, seq_len, d, es, t->heads, x, t->x, dy, &t->dout, dx, out, true,
+                                  n ? norm->k_weight : norm->q_weight, false)) != FA_OK)
+            return rc;
+        NormTensor& added = p.t[p.nt - 1];
+        if ((dx && dx == x && !same_strides(added.xs, out.st)) || (dx && dx == dy && !same_strides(added.dys, out.st)))
+            return FA_ERR_INVALID_ARG;
+        added.dw = dw;
+        weights = weights || dw;
+    }
+    if (p.nt == 0) return FA_OK;
+    fill_norm(*cfg, *norm, batch, seq_len, positions, &p);
+    int dev;
+    if ((rc = ops_begin(&dev, kNormModule)) != FA_OK) return rc;
+    const hipStream_t stream = static_cast<hipStream_t>(stream_);
+    // tensors without rows are left out of the first launch
+    NormParams rows = p;
+    rows.nt = 0;
+    int from[3];
+    for (int i = 0; i < p.nt; ++i)
+        if (p.t[i].heads > 0) {
+            from[rows.nt] = i;
+            rows.t[rows.nt++] = p.t[i];
+        }
+    OpsWorkspace ws;
+    if (rows.nt > 0) {
+        size_t grid;
+        bool wide;
+        if ((rc = plan_norm(dev, cfg->dtype, check.wide, &rows, &wide, &grid)) != FA_OK) return rc;
+        if (weights) {
+            if ((rc = ws.get(dev, stream, grid * d * sizeof(float))) != FA_OK) return rc;
+            float* part = static_cast<float*>(ws.ptr);
+            for (int i = 0; i < rows.nt; ++i) {
+                rows.t[i].part = rows.t[i].dw ? part : nullptr;
+                part += rows.t[i].blocks * d;
+                p.t[from[i]] = rows.t[i];
+            }
+        }
+        char name[64];
+        std::snprintf(name, sizeof(name), "fa_norm_back_%s_%d", dtype_name(cfg->dtype), wide ? 1 : 0);
+        rc = ops_launch(dev, kNormModule, name, grid, kNormThreads, &rows, stream);
+    }
+    if (rc == FA_OK && weights) rc = ops_launch(dev, kNormModule, "fa_norm_weights", p.nt * ((d + 15) / 16), 1024, &p, stream);
+    return ws.done(stream, rc);
+} catch (...) {   // no memory for the tables of modules, kernels and workspaces
+    return FA_ERR_ALLOC;
+}
+
+int fa_norm_cache_append(void* stream, const fa_kv_cache* cache, const fa_append_config* cfg, const fa_head_norm* norm,
+                         const void* k, const void* v, const int32_t* positions, const void* q, void* q_out) try {
+    OpsLayout ck, cv;
+    size_t capacity = 0;
+    int rc = check_cache(cache, &ck, &cv, &capacity);
+    if (rc != FA_OK) return rc;
+    if (!cfg) return FA_ERR_INVALID_ARG;
+    const fa_rotary_config* rot = cfg->rotary;
+    if ((rc = check_norm(rot, norm)) != FA_OK) return rc;
+    if (rot->dtype != cache->dtype || rot->d_head != cache->d_head) return FA_ERR_INVALID_ARG;
+    if (cache->batch == 0 || cache->kv_heads == 0 || cache->d_head == 0 || cfg->n_tokens == 0) return FA_OK;
+    const size_t es = elem_size(cache->dtype), d = cache->d_head, n = cfg->n_tokens;
+    if (n > kOpsMaxSeq || cache->batch * n > kOpsMaxTokens) return FA_ERR_UNSUPPORTED;
+    if (!k || !v || !positions) return FA_ERR_INVALID_ARG;
+    NormParams p{};
+    NormCheck check;
+    // checked also where there is no room for a row
+    if ((rc = add_norm_tensor(&p, &check, cache->batch, n, d, es, cache->kv_heads, k, cfg->k, nullptr, nullptr, cache->k,
+                              ck, true, norm->k_weight, true)) != FA_OK ||
+        (rc = add_norm_tensor(&p, &check, cache->batch, n, d, es, cache->kv_heads, v, cfg->v, nullptr, nullptr, cache->v,
+                              cv, false, nullptr, true)) != FA_OK)
+        return rc;
+    if (capacity == 0) {
+        p.nt = 0;
+        check = NormCheck();
+    }
+    if (cfg->q_layout && cfg->q_layout->heads > 0) {
+        const fa_rotary_tensor* t = cfg->q_layout;
+        OpsLayout out;
+        if (t->heads > kOpsMaxSeq) return FA_ERR_UNSUPPORTED;
+        if ((rc = resolve_layout(t->out, cache->batch, n, t->heads, d, es, true, &out)) != FA_OK) return rc;
+        if (!q || !q_out) return FA_ERR_INVALID_ARG;
+        if ((rc = add_norm_tensor(&p, &check, cache->batch, n, d, es, t->heads, q, t->in, nullptr, nullptr, q_out, out,
+                                  true, norm->q_weight, false)) != FA_OK)
+            return rc;
+        if (q == q_out && !same_strides(p.t[p.nt - 1].xs, out.st)) return FA_ERR_INVALID_ARG;
+    }
+    if (p.nt == 0) return FA_OK;
+    fill_norm(*rot, *norm, cache->batch, n, positions, &p);
+    p.lens = cache->lens;
+    p.table = cache->block_table;
+    p.capacity = static_cast<int>(capacity);
+    p.page_shift = page_shift(*cache);
+    p.n_pages = static_cast<int>(cache->n_pages);
+    p.pages_per_seq = static_cast<int>(cache->pages_per_seq);
+    int dev;
+    if ((rc = ops_begin(&dev, kNormModule)) != FA_OK) return rc;
+    return launch_norm(dev, static_cast<hipStream_t>(stream), cache->dtype, &p, check.wide);
 } catch (...) {   // no memory for the tables of modules, kernels and workspaces
     return FA_ERR_ALLOC;
 }

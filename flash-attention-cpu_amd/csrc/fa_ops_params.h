@@ -104,4 +104,29 @@ struct RotParams {
     double turns[128];
 };
 
+// One tensor of a launch of norms with rotary positions.
+constexpr int kNormThreads = 256;
+constexpr int kNormTokens = 16;   // most tokens of a workgroup
+struct NormTensor {
+    const void *x, *dy, *w;   // w: NULL: ones
+    void* out;                // y, or dx (NULL: not wanted)
+    float *dw, *part;         // backward: the weights' gradient, and its partial sums [blocks][d]
+    OpsStrides xs, dys, outs;
+    int heads;
+    int norm;                 // 0: copied
+    int cache;                // out is a cache: rows lens[b] + token
+    int tokens, blocks;       // of a workgroup; workgroups
+};
+
+struct NormParams {
+    NormTensor t[3];
+    int nt;
+    int batch, seq, d, rot, interleaved;
+    int units, lanes;         // units of columns of a row, and the lanes that keep them
+    const int32_t *pos, *lens, *table;
+    int capacity, page_shift, n_pages, pages_per_seq;
+    float gain, eps;
+    double turns[128];
+};
+
 #endif  // FA_OPS_PARAMS_H

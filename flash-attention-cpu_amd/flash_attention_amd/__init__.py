@@ -74,6 +74,7 @@ EXPORTED_SYMBOLS = (
     "fa_init", "fa_describe_launch", "fa_probe_launch",
     "fa_score_forward", "fa_score_backward", "fa_rotary_init", "fa_rotary", "fa_cache_append", "fa_tree_attention",
     "fa_window_forward", "fa_window_backward", "fa_window_tree_attention",
+    "fa_norm_rotary", "fa_norm_rotary_backward", "fa_norm_cache_append",
 )
 
 
@@ -420,6 +421,7 @@ def init() -> None:
 # Attention with modified scores, rotary positions, key / value cache (operators.py)
 ROTARY_NONE, ROTARY_LINEAR, ROTARY_NTK, ROTARY_YARN = 0, 1, 2, 3
 from .operators import (  # noqa: E402
-    AppendConfig, KvCache, RotaryConfig, RotaryTensor, ScoreConfig, Strides, TreeConfig, Window, append_config,
-    cache_append_device, kv_cache, rotary_config, rotary_device, rotary_tensor, score_attention_backward_device,
+    AppendConfig, HeadNorm, KvCache, NormGrad, RotaryConfig, RotaryTensor, ScoreConfig, Strides, TreeConfig, Window,
+    append_config, cache_append_device, head_norm, kv_cache, norm_grad, norm_rotary_backward_device,
+    norm_rotary_device, rotary_config, rotary_device, rotary_tensor, score_attention_backward_device,
     score_attention_device, score_config, tree_attention_device, tree_config, window)

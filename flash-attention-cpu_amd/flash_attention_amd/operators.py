@@ -1,6 +1,6 @@
 """Attention with modified scores, rotary positions and the key / value cache.
 
-Python view of the fa_score_*, fa_window_*, fa_rotary*, fa_cache_append and
+Python view of the fa_score_*, fa_window_*, fa_rotary*, fa_norm_*, fa_cache_append and
 fa_tree_attention entry points of include/fa_hip.h, which defines what they
 compute.  They have no counterpart in the reference crate.
 
@@ -55,6 +55,18 @@ class RotaryTensor(ctypes.Structure):
     _fields_ = [("heads", _SZ), ("src", Strides), ("dst", Strides)]
 
 
+class HeadNorm(ctypes.Structure):
+    """fa_head_norm."""
+
+    _fields_ = [("q_weight", _P), ("k_weight", _P), ("eps", _F)]
+
+
+class NormGrad(ctypes.Structure):
+    """fa_norm_grad."""
+
+    _fields_ = [("heads", _SZ), ("x", Strides), ("dout", Strides), ("dx", Strides)]
+
+
 class KvCache(ctypes.Structure):
     """fa_kv_cache."""
 
@@ -86,6 +98,11 @@ def declare(lib: ctypes.CDLL) -> None:
         "fa_rotary_init": [ptr(RotaryConfig), _I, _SZ, _SZ, _I, ctypes.c_double, _I, ctypes.c_double,
                            ctypes.c_double],
         "fa_rotary": [_P, ptr(RotaryConfig), _SZ, _SZ, _P, _I, ptr(RotaryTensor), _P, _P, ptr(RotaryTensor), _P, _P],
+        "fa_norm_rotary": [_P, ptr(RotaryConfig), ptr(HeadNorm), _SZ, _SZ, _P, ptr(RotaryTensor), _P, _P,
+                           ptr(RotaryTensor), _P, _P],
+        "fa_norm_rotary_backward": [_P, ptr(RotaryConfig), ptr(HeadNorm), _SZ, _SZ, _P, ptr(NormGrad), _P, _P, _P, _P,
+                                    ptr(NormGrad), _P, _P, _P, _P],
+        "fa_norm_cache_append": [_P, ptr(KvCache), ptr(AppendConfig), ptr(HeadNorm), _P, _P, _P, _P, _P],
         "fa_cache_append": [_P, ptr(KvCache), ptr(AppendConfig), _P, _P, _P, _P, _P],
         "fa_tree_attention": [_P, ptr(TreeConfig), ptr(KvCache), _P, _P, _P],
         "fa_window_forward": [_P, ptr(ScoreConfig), ptr(Window), _P, _P, _P, _P, _P],
@@ -193,6 +210,33 @@ def rotary_device(cfg: RotaryConfig, batch: int, seq_len: int, positions_ptr: in
                             q_out_ptr, k_layout, k_ptr, k_out_ptr))
 
 
+def head_norm(q_weight_ptr: int = 0, k_weight_ptr: int = 0, eps: float = 1e-6) -> HeadNorm:
+    """Norms of queries and keys; weights: one a column, 0: ones."""
+    return HeadNorm(_ptr(q_weight_ptr), _ptr(k_weight_ptr), float(eps))
+
+
+def norm_rotary_device(cfg: RotaryConfig, norm: HeadNorm, batch: int, seq_len: int, positions_ptr: int,
+                       q_layout: RotaryTensor, q_ptr: int, q_out_ptr: int, k_layout: RotaryTensor | None = None,
+                       k_ptr: int = 0, k_out_ptr: int = 0, stream: int = 0) -> None:
+    """Queue the norms of the head rows of one or two tensors and their rotary positions (fa_norm_rotary)."""
+    _check(_lib().fa_norm_rotary(stream, cfg, norm, batch, seq_len, positions_ptr, q_layout, q_ptr, q_out_ptr,
+                                 k_layout, k_ptr, k_out_ptr))
+
+
+def norm_grad(heads: int, x_strides=None, dout_strides=None, dx_strides=None) -> NormGrad:
+    """Head rows a token and layouts of one tensor of a backward call: input, its output's gradient, its gradient."""
+    return NormGrad(heads, _strides(x_strides), _strides(dout_strides), _strides(dx_strides))
+
+
+def norm_rotary_backward_device(cfg: RotaryConfig, norm: HeadNorm, batch: int, seq_len: int, positions_ptr: int,
+                                q_grad: NormGrad, q_ptr: int, dq_out_ptr: int, dq_ptr: int, dq_weight_ptr: int = 0,
+                                k_grad: NormGrad | None = None, k_ptr: int = 0, dk_out_ptr: int = 0, dk_ptr: int = 0,
+                                dk_weight_ptr: int = 0, stream: int = 0) -> None:
+    """Queue its gradients (fa_norm_rotary_backward); those whose pointer is 0 are not computed."""
+    _check(_lib().fa_norm_rotary_backward(stream, cfg, norm, batch, seq_len, positions_ptr, q_grad, q_ptr, dq_out_ptr,
+                                          dq_ptr, dq_weight_ptr, k_grad, k_ptr, dk_out_ptr, dk_ptr, dk_weight_ptr))
+
+
 def kv_cache(dtype: int, batch: int, kv_heads: int, d_head: int, k_ptr: int, v_ptr: int, lens_ptr: int,
              k_strides=None, v_strides=None, capacity: int = 0, block_table_ptr: int = 0, page_size: int = 0,
              n_pages: int = 0, pages_per_seq: int = 0) -> KvCache:
@@ -214,9 +258,13 @@ def append_config(n_tokens: int, rotary: RotaryConfig | None = None, k_strides=N
 
 
 def cache_append_device(cache: KvCache, cfg: AppendConfig, k_ptr: int, v_ptr: int, positions_ptr: int = 0,
-                        q_ptr: int = 0, q_out_ptr: int = 0, stream: int = 0) -> None:
-    """Queue the append of drafted keys and values behind each sequence's rows (fa_cache_append)."""
-    _check(_lib().fa_cache_append(stream, cache, cfg, k_ptr, v_ptr, positions_ptr, q_ptr, q_out_ptr))
+                        q_ptr: int = 0, q_out_ptr: int = 0, stream: int = 0, norm: HeadNorm | None = None) -> None:
+    """Queue the append of drafted keys and values behind each sequence's rows (fa_cache_append; norm: keys and
+    queries are normed before their rotation, fa_norm_cache_append)."""
+    if norm is None:
+        _check(_lib().fa_cache_append(stream, cache, cfg, k_ptr, v_ptr, positions_ptr, q_ptr, q_out_ptr))
+    else:
+        _check(_lib().fa_norm_cache_append(stream, cache, cfg, norm, k_ptr, v_ptr, positions_ptr, q_ptr, q_out_ptr))
 
 
 def tree_config(heads: int, n_tokens: int, mask_ptr: int = 0, mask_shared: bool = False,

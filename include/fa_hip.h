@@ -377,6 +377,34 @@ int fa_rotary(void* stream, const fa_rotary_config* cfg, size_t batch, size_t se
               int inverse, const fa_rotary_tensor* q_layout, const void* q, void* q_out,
               const fa_rotary_tensor* k_layout, const void* k, void* k_out);
 
+/* ---- norms of queries and keys ------------------------------------------------
+ * No counterpart in the reference.  Each head row is divided by its root mean
+ * square, multiplied by weights (one a column, shared by all heads) and
+ * rotated as fa_rotary does, in one pass:
+ *     y = R(position) (x r w),   r = 1 / sqrt(mean over d_head of x^2 + eps)
+ * with sums in f32 and one rounding at the end (rows whose sum of squares
+ * passes f32's range give zeros).  In place where pointers and strides are the same. */
+typedef struct fa_head_norm {
+    const void *q_weight, *k_weight;   /* [d_head] of the config's dtype, device memory; NULL: ones */
+    float eps;                         /* above 0 */
+} fa_head_norm;
+int fa_norm_rotary(void* stream, const fa_rotary_config* cfg, const fa_head_norm* norm, size_t batch, size_t seq_len,
+                   const int32_t* positions, const fa_rotary_tensor* q_layout, const void* q, void* q_out,
+                   const fa_rotary_tensor* k_layout, const void* k, void* k_out);
+/* Its gradients from its inputs and the gradients of its outputs: dx in the
+ * inputs' type, those of the weights (summed over all rows) f32 [d_head].  Each of
+ * dq, dk and the weights' may be NULL where it is not wanted, kg where there is
+ * one tensor.  dq may be q or dq_out where the strides are the same.  Results do not depend on the order in which
+ * workgroups run.  With no rows the weights' gradients are zeros. */
+typedef struct fa_norm_grad {
+    size_t heads;
+    fa_strides x, dout, dx;
+} fa_norm_grad;
+int fa_norm_rotary_backward(void* stream, const fa_rotary_config* cfg, const fa_head_norm* norm, size_t batch,
+                            size_t seq_len, const int32_t* positions, const fa_norm_grad* qg, const void* q,
+                            const void* dq_out, void* dq, float* dq_weight, const fa_norm_grad* kg, const void* k,
+                            const void* dk_out, void* dk, float* dk_weight);
+
 /* ---- key / value cache and attention of drafted trees -----------------------
  * No counterpart in the reference.  A cache holds capacity rows a sequence,
  * either one after another (block_table NULL: row r of sequence b at
@@ -412,6 +440,10 @@ typedef struct fa_append_config {
 } fa_append_config;
 int fa_cache_append(void* stream, const fa_kv_cache* cache, const fa_append_config* cfg, const void* k, const void* v,
                     const int32_t* positions, const void* q, void* q_out);
+/* The same with the norms of fa_norm_rotary before the rotation (cfg->rotary
+ * and positions have to be given). */
+int fa_norm_cache_append(void* stream, const fa_kv_cache* cache, const fa_append_config* cfg, const fa_head_norm* norm,
+                         const void* k, const void* v, const int32_t* positions, const void* q, void* q_out);
 
 /* Attention of n drafted tokens a sequence: token i sees the rows before
  * lens[b] and the drafted row lens[b] + t iff bit t % 64 of
