@@ -1,0 +1,717 @@
+// fa_cache4.hip -- gfx950 kernels of the key / value cache held in 4 bits:
+// append, rows read back, and attention of query rows over it (fa_cache4_*).
+//
+// A row's columns come in groups of 32.  A group has a step S / 16 and an offset O, both f16, and its code c
+// stands for the value O + (1 + c / 16) S:  c in the upper bits of the fraction of an f16 in [1, 2) makes that one
+// multiply-add of two values, and no subtraction of a constant is needed.
+//
+// Keys lie in rows of d / 8 words, 8 columns a word; values in words of 8 rows of one column, d such words for the
+// 8 rows.  Both are then operands of 16 x 16 x 32 matrix products as they come from memory, a word's eight codes
+// being the eight elements that a lane holds, and nothing goes through LDS or is transposed.
+// Entry e of a word stands at bits 4 (e / 2) + 16 (e % 2), so that pairs of neighbours leave it together.
+//
+// Built once a type: OPS_T the type of queries, outputs and rows (16 bits), OPS_NAME its name in the kernels'.
+
+#include "fa_rows.h"
+
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+
+// Block of memory and row in it of a sequence's row, -1: there is none.
+struct Place {
+    int64_t block;
+    int row;
+};
+__device__ __forceinline__ Place cache4_place(const Cache4Params& p, int b, int64_t row) {
+    if (row < 0 || row >= p.capacity) return {-1, 0};
+    if (!p.table) return {b, (int)row};
+    const int page = p.table[(int64_t)b * p.pages_per_seq + (row >> p.page_shift)];
+    return {(unsigned)page < (unsigned)p.n_pages ? page : -1, (int)row & ((1 << p.page_shift) - 1)};
+}
+
+__device__ __forceinline__ unsigned half_bits(_Float16 x) { return __builtin_bit_cast(unsigned short, x); }
+__device__ __forceinline__ _Float16 bits_half(unsigned x) { return __builtin_bit_cast(_Float16, (unsigned short)x); }
+
+// ---------------------------------------------------------------------------
+// Append: a workgroup takes a few runs of 8 rows of one head of K or V.  A thread quantises 8 columns of a row, four
+// neighbours a group.  Keys are words then; values meet in LDS, where a thread a column makes a word of
+// 8 rows, with what is there already of rows that are not new.
+// Bound by memory and, for short runs, by the launch.
+// ---------------------------------------------------------------------------
+template <typename T>
+__device__ __forceinline__ void cache4_append(const Cache4Params& p) {
+    __shared__ __attribute__((aligned(16))) unsigned char codes[256 * 8];   // [run][8 rows][d]
+    __shared__ int fresh[32];
+    typedef T run8 __attribute__((ext_vector_type(8)));
+    const int tid = threadIdx.x, words = p.d / 8, per = 256 / p.d;   // runs of 8 rows a workgroup
+    unsigned id = blockIdx.x;
+    const int part = id % p.nparts;
+    id /= p.nparts;
+    const int h = id % p.kv_heads;
+    id /= p.kv_heads;
+    const bool isv = id & 1;
+    const int b = id >> 1;
+    const int len = p.lens[b];
+    if (len < 0) return;
+    const int64_t first = len / 8 + (int64_t)part * per;   // run of 8 rows
+    const T* const src = reinterpret_cast<const T*>(isv ? p.v : p.k) + (isv ? b * p.vs.b + h * p.vs.h : b * p.ks.b + h * p.ks.h);
+    const int64_t seq = isv ? p.vs.s : p.ks.s;
+
+    const bool mine = tid < per * p.d;
+    const int run = tid / p.d, r = tid % p.d / words, word = tid % words;
+    const int64_t row = (first + run) * 8 + r, token = row - len;
+    Place at = {-1, 0};
+    if (mine && token >= 0 && token < p.n) at = cache4_place(p, b, row);
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = 0.0f;
+    if (at.block >= 0) {
+        const T* const from = src + token * seq + 8 * word;
+        if (p.vec) {
+            const run8 y = *reinterpret_cast<const run8*>(from);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = float(y[e]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = float(from[e]);
+        }
+    }
+    float lo = INFINITY, hi = -INFINITY;
+    int bad = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        bad |= not_finite(x[e]);
+        x[e] = fminf(fmaxf(x[e], -kCache4Max), kCache4Max);
+        lo = fminf(lo, x[e]);
+        hi = fmaxf(hi, x[e]);
+    }
+#pragma unroll
+    for (int m = 1; m < 4; m *= 2) {
+        lo = fminf(lo, __shfl_xor(lo, m));
+        hi = fmaxf(hi, __shfl_xor(hi, m));
+        bad |= __shfl_xor(bad, m);
+    }
+    // as the header defines them, each operation rounded once
+    constexpr float kTop = 65504.0f;
+    const _Float16 big = bad ? bits_half(0x7e00) : _Float16(fminf((hi - lo) * 16.0f / 15.0f, kTop));
+    const _Float16 off = bad ? bits_half(0x7e00) : _Float16(fmaxf(lo - float(big), -kTop));
+    const float step = float(big) * 0.0625f;
+    unsigned code[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float y = rintf((x[e] - float(off)) / step - 16.0f);
+        code[e] = bad || step == 0.0f ? 0u : (unsigned)fminf(fmaxf(y, 0.0f), 15.0f);
+    }
+    const int groups = p.d / 32;
+    if (!isv) {
+        if (at.block < 0) return;
+        const int64_t to = (at.block * p.kv_heads + h) * p.block_rows + at.row;
+        unsigned w = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w |= code[e] << (4 * (e / 2) + 16 * (e % 2));
+        p.k4[to * words + word] = w;
+        if (word % 4 == 0) reinterpret_cast<unsigned*>(p.kscale)[to * groups + word / 4] = half_bits(big) | half_bits(off) << 16;
+        return;
+    }
+    if (tid < per) fresh[tid] = 0;
+    __syncthreads();
+    if (at.block >= 0) {
+        if (word == 0) atomicOr(&fresh[run], 1 << r);
+        u32x2 c = {code[0] | code[1] << 8 | code[2] << 16 | code[3] << 24, code[4] | code[5] << 8 | code[6] << 16 | code[7] << 24};
+        *reinterpret_cast<u32x2*>(codes + (run * 8 + r) * p.d + 8 * word) = c;
+        if (word % 4 == 0) {
+            const int64_t to = (at.block * p.kv_heads + h) * (p.block_rows / 8) + at.row / 8;
+            unsigned short* const s = p.vscale + (to * groups + word / 4) * 16 + r;
+            s[0] = half_bits(big);
+            s[8] = half_bits(off);
+        }
+    }
+    __syncthreads();
+    const int run2 = tid / p.d, col = tid % p.d;
+    if (!mine || fresh[run2] == 0) return;
+    const Place to = cache4_place(p, b, (first + run2) * 8 + __builtin_ctz(fresh[run2]));
+    if (to.block < 0) return;
+    unsigned* const word8 = p.v4 + ((to.block * p.kv_heads + h) * (p.block_rows / 8) + to.row / 8) * p.d + col;
+    unsigned w = fresh[run2] == 0xff ? 0u : *word8;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const int sh = 4 * (e / 2) + 16 * (e % 2);
+        if (fresh[run2] >> e & 1) w = (w & ~(15u << sh)) | (unsigned)codes[(run2 * 8 + e) * p.d + col] << sh;
+    }
+    *word8 = w;
+}
+
+// Rows of the cache in the type: 8 columns of a row a thread, K and V.
+template <typename T>
+__device__ __forceinline__ void cache4_read(const Cache4Params& p) {
+    typedef T run8 __attribute__((ext_vector_type(8)));
+    const int words = p.d / 8, groups = p.d / 32;
+    int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int word = id % words;
+    id /= words;
+    const int i = id % p.n;
+    id /= p.n;
+    const int h = id % p.kv_heads;
+    id /= p.kv_heads;
+    const bool isv = id & 1;
+    const int b = id >> 1;
+    if (b >= p.batch || !(isv ? p.vo : p.ko)) return;
+    const Place at = cache4_place(p, b, p.rows[(int64_t)b * p.n + i]);
+    run8 y = {};
+    if (at.block >= 0) {
+        const int64_t head = at.block * p.kv_heads + h;
+        if (!isv) {
+            const int64_t row = head * p.block_rows + at.row;
+            const unsigned w = p.k4[row * words + word];
+            const unsigned s = reinterpret_cast<const unsigned*>(p.kscale)[row * groups + word / 4];
+            const float big = float(bits_half(s & 0xffff)), off = float(bits_half(s >> 16));
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                y[e] = T(__builtin_fmaf(1.0f + (float)(w >> (4 * (e / 2) + 16 * (e % 2)) & 15) * 0.0625f, big, off));
+        } else {
+            const int64_t run = head * (p.block_rows / 8) + at.row / 8;
+            const int r = at.row % 8, sh = 4 * (r / 2) + 16 * (r % 2);
+            const unsigned short* const s = p.vscale + (run * groups + word / 4) * 16 + r;
+            const float big = float(bits_half(s[0])), off = float(bits_half(s[8]));
+            const u32x4* const from = reinterpret_cast<const u32x4*>(p.v4 + run * p.d + 8 * word);
+            const u32x4 w[2] = {from[0], from[1]};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = T(__builtin_fmaf(1.0f + (float)(w[e / 4][e % 4] >> sh & 15) * 0.0625f, big, off));
+        }
+    }
+    T* const to = reinterpret_cast<T*>(isv ? p.vo : p.ko) +
+                  (isv ? b * p.vs.b + h * p.vs.h + i * p.vs.s : b * p.ks.b + h * p.ks.h + i * p.ks.s) + 8 * word;
+    if (p.vec) {
+        *reinterpret_cast<run8*>(to) = y;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) to[e] = y[e];
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Attention
+// ---------------------------------------------------------------------------
+// Eight values of a word: codes to the fraction of f16 numbers in [1, 2), times S, plus O.  big(i), off(i): those of
+// pair i.
+template <typename B, typename O>
+__device__ __forceinline__ h8 dequant(unsigned w, B big, O off) {
+    h8 v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const unsigned bits = (4 * i < 6 ? w << (6 - 4 * i) : w >> (4 * i - 6)) & 0x03c003c0u;
+        const h2 t = __builtin_bit_cast(h2, bits | 0x3c003c00u);
+        const h2 y = __builtin_elementwise_fma(t, big(i), off(i));
+        v[2 * i] = y[0];
+        v[2 * i + 1] = y[1];
+    }
+    return v;
+}
+
+template <int N>
+struct Words {
+    unsigned w[N];
+};
+// N words at a byte offset of a buffer (zeros past its end)
+template <int N>
+__device__ __forceinline__ Words<N> buffer_words(__amdgpu_buffer_rsrc_t rs, int at) {
+    Words<N> r;
+    if constexpr (N == 4) {
+        const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(rs, at, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r.w[i] = x[i];
+    } else if constexpr (N == 2) {
+        const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(rs, at, 0, 0);
+        r.w[0] = x[0];
+        r.w[1] = x[1];
+    } else {
+        r.w[0] = __builtin_amdgcn_raw_buffer_load_b32(rs, at, 0, 0);
+    }
+    return r;
+}
+
+// The matrix product over f16, whose other operands are the values that codes stand for.
+using M4 = Mma<_Float16>;
+
+// Waves walk blocks of 32 keys of their own, two blocks in registers or on their way while one is used.  MT 16-row
+// tiles of queries; SMALL: pages of less than 32 rows, whose rows are found lane by lane.
+// A lane (g = l / 16, li = l % 16) has of K the rows 8 (li / 4) + 4 b + li % 4, b < 2, of a block, so that the scores
+// it gets are those of keys 8 g .. 8 g + 7, the eight rows of a word of V.
+template <typename T, int NDC, int MT, int MOD, bool SMALL>
+__device__ __forceinline__ void rows4(const RowsParams& p) {
+    constexpr int NW = kRows4Waves, SK = 32, D = 32 * NDC;
+    constexpr int KW = NDC % 4 == 0 ? 4 : NDC % 2 == 0 ? 2 : 1, NK = NDC / KW;   // words of a load of K, and loads a row
+    constexpr int VW = NDC % 2 == 0 ? 4 : 2, NV = D / (16 * VW);                  // columns of a load of V, and loads
+    constexpr int NO = D / 16, PD = D <= 64 ? 64 : D <= 128 ? 128 : 256;          // PD: a row of partial sums
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = lane >> 4, li = lane & 15;
+    RowsWork w;
+    if (!rows_work(p, 16 * MT, lane, &w)) return;
+    const CachePages pages = rows_pages(p, w.b);
+    const int page_rows = p.block4;   // rows of a block of memory
+    const unsigned* const K = reinterpret_cast<const unsigned*>(p.k);
+    const unsigned* const KS = reinterpret_cast<const unsigned*>(p.k_scale);
+    const unsigned* const V = reinterpret_cast<const unsigned*>(p.v);
+    const unsigned* const VS = reinterpret_cast<const unsigned*>(p.v_scale);
+    const int nblk = SK * wave < w.kwalk ? (w.kwalk - SK * wave + SK * NW - 1) / (SK * NW) : 0;
+    auto key_of = [&](int i) { return w.key(SK * wave + i * SK * NW); };   // first key of the wave's i-th block
+
+    // byte offsets of the lane's loads in a block of 32 rows
+    int kat[2], kpat[2], vat, vpat;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+        const int row = 8 * (li >> 2) + 4 * b + (li & 3);
+        kat[b] = row * (D / 2) + g * 4 * KW;
+        kpat[b] = row * NDC * 4 + (g * KW / 4) * 4;
+    }
+    vat = g * D * 4 + li * 4 * VW;
+    vpat = g * NDC * 32 + (VW == 4 ? (li >> 3) * 32 : 0);
+    struct Block {
+        Words<KW> k[2][NK];
+        unsigned ks[2][NK];
+        Words<VW> v[NV];
+        Words<4> big[NV], off[NV];
+    };
+    // the page of a block of 32 keys (0 without pages), -1: bad or past the end
+    auto look_up = [&](int i) {
+        if (SMALL || i >= nblk) return -1;
+        return pages.page(key_of(i));
+    };
+    auto rows_at = [&](int i, int page) -> int64_t {   // rows before the block's first, of its head
+        const int k0 = key_of(i);
+        const int64_t blk = p.table ? page : w.b;
+        return (blk * p.kv_heads + w.hk) * page_rows + (p.table ? k0 & pages.page_mask : k0);
+    };
+    auto buffer = [&](const unsigned* base, int64_t word, int words) {
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned*>(words > 0 ? base + word : base), (short)0, 4 * words,
+                                                 0x00020000);
+    };
+    // SMALL: the rows before row `row` of its head, where it is one
+    auto lane_rows = [&](int row, bool* real) -> int64_t {
+        *real = row < w.kend;
+        int page = *real ? pages.table[row >> pages.shift] : 0;
+        if ((unsigned)page >= (unsigned)pages.n_pages) *real = false;
+        return ((int64_t)page * p.kv_heads + w.hk) * page_rows + (row & pages.page_mask);
+    };
+    auto load_k = [&](Block& x, int i, int page) {
+        const int k0 = key_of(i);
+        if constexpr (SMALL) {
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                bool real = false;
+                int64_t at = 0;
+                if (i < nblk) at = lane_rows(k0 + 8 * (li >> 2) + 4 * b + (li & 3), &real);
+#pragma unroll
+                for (int q = 0; q < NK; ++q) {
+                    x.k[b][q] = {};
+                    x.ks[b][q] = 0;
+                    if (!real) continue;
+#pragma unroll
+                    for (int e = 0; e < KW; ++e) x.k[b][q].w[e] = K[at * (D / 8) + q * 4 * KW + g * KW + e];
+                    x.ks[b][q] = KS[at * NDC + q * KW + g * KW / 4];
+                }
+            }
+        } else {
+            const int n = page < 0 || i >= nblk ? 0 : max(0, min(SK, w.kend - k0));
+            const int64_t at = n ? rows_at(i, page) : 0;
+            const __amdgpu_buffer_rsrc_t rk = buffer(K, at * (D / 8), n * (D / 8)), rs = buffer(KS, at * NDC, n * NDC);
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int q = 0; q < NK; ++q) {
+                    x.k[b][q] = buffer_words<KW>(rk, kat[b] + q * 16 * KW);
+                    x.ks[b][q] = buffer_words<1>(rs, kpat[b] + q * 4 * KW).w[0];
+                }
+        }
+    };
+    auto load_v = [&](Block& x, int i, int page) {
+        const int k0 = key_of(i);
+        if constexpr (SMALL) {
+            bool real = false;
+            int64_t at = 0;
+            if (i < nblk) at = lane_rows(k0 + 8 * g, &real) / 8;
+#pragma unroll
+            for (int q = 0; q < NV; ++q) {
+                x.v[q] = {};
+                x.big[q] = x.off[q] = {};
+                if (!real) continue;
+#pragma unroll
+                for (int e = 0; e < VW; ++e) x.v[q].w[e] = V[at * D + q * 16 * VW + li * VW + e];
+                const unsigned* const s = VS + (at * NDC + (q * 16 + li) * VW / 32) * 8;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    x.big[q].w[e] = s[e];
+                    x.off[q].w[e] = s[4 + e];
+                }
+            }
+        } else {
+            const int n = page < 0 || i >= nblk ? 0 : (max(0, min(SK, w.kend - k0)) + 7) / 8;   // runs of 8 rows
+            const int64_t at = n ? rows_at(i, page) / 8 : 0;
+            const __amdgpu_buffer_rsrc_t rv = buffer(V, at * D, n * D), rs = buffer(VS, at * NDC * 8, n * NDC * 8);
+#pragma unroll
+            for (int q = 0; q < NV; ++q) {
+                x.v[q] = buffer_words<VW>(rv, vat + q * 64 * VW);
+                x.big[q] = buffer_words<4>(rs, vpat + q * 16 * VW);
+                x.off[q] = buffer_words<4>(rs, vpat + q * 16 * VW + 16);
+            }
+        }
+    };
+
+    Block A, B;
+    int page0 = look_up(0), page1 = look_up(1), page2;
+    load_k(A, 0, page0);
+    load_v(A, 0, page0);
+    load_k(B, 1, page1);
+    load_v(B, 1, page1);
+    page2 = look_up(2);
+
+    // Queries as f16.  bf16 rows are brought into its range by a power of two, exactly but for entries 2^29 below the
+    // row's largest; qs takes it back.
+    h8 q[MT][NDC];
+    f32x4 o[MT][NO], s[MT][2];
+    float m[MT], ref[MT], l[MT], qs[MT], c[MT], slope[MT];
+    RowToken tok[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        const int r = w.rfirst + 16 * t + li;
+        const bool real = r < w.nrows;
+        const int token = real ? r / p.group : 0, h = w.hk * p.group + (real ? r % p.group : 0);
+        tok[t] = row_token(p, w, token);
+        slope[t] = has_bias<MOD>(p) ? p.slopes[h] * kLog2e : 0.0f;
+        const T* const from = reinterpret_cast<const T*>(p.q) + w.b * p.qs.b + h * p.qs.h + token * p.qs.s;
+        typename Mma<T>::v8 x[NDC];
+        float mx = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NDC; ++j) {
+            const int col = j / KW * 32 * KW + g * 8 * KW + j % KW * 8;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[j][e] = T(0.0f);
+            if (real) {
+                if (p.vec4) {
+                    x[j] = *reinterpret_cast<const typename Mma<T>::v8*>(from + col);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[j][e] = from[col + e];
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(float(x[j][e])));
+        }
+        qs[t] = 1.0f;
+        float up = 1.0f;
+        if constexpr (std::is_same<T, __bf16>::value) {
+            mx = row4_max(mx);
+            const unsigned ex = __float_as_uint(mx) >> 23;
+            if (ex > 0 && ex < 255) {
+                const unsigned e = max(ex, 15u);
+                up = __uint_as_float((268u - e) << 23);   // the largest to 2^14 .. 2^15
+                qs[t] = __uint_as_float((e - 14u) << 23);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < NDC; ++j)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) q[t][j][e] = _Float16(float(x[j][e]) * up);
+        c[t] = MOD != 0 ? 1.0f : p.scale_log2e * qs[t];
+#pragma unroll
+        for (int j = 0; j < NO; ++j) o[t][j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+        m[t] = OPS_NEG_INF;
+        l[t] = ref[t] = 0.0f;
+    }
+    constexpr float kProb = kProbLog2<_Float16>, kUp = MOD != 0 ? kProb : 0.0f;
+    int special = 0;
+
+    auto block = [&](int i, Block& x, int page) {
+        const int k0 = key_of(i);
+        // S^T of the block, relative to the rows' references
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            const float r = MOD != 0 ? 0.0f : -ref[t];
+            s[t][0] = s[t][1] = (f32x4){r, r, r, r};
+        }
+#pragma unroll
+        for (int n = 0; n < NK; ++n)
+#pragma unroll
+            for (int j = 0; j < KW; ++j)
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    const h2 so = __builtin_bit_cast(h2, x.ks[b][n]);
+                    const h8 k = dequant(x.k[b][n].w[j], [&](int) { return (h2){so[0], so[0]}; },
+                                         [&](int) { return (h2){so[1], so[1]}; });
+#pragma unroll
+                    for (int t = 0; t < MT; ++t) s[t][b] = M4::mma(k, q[t][n * KW + j], s[t][b]);
+                }
+        __builtin_amdgcn_sched_barrier(0);
+        load_k(x, i + 2, page2);
+        int bad = page < 0;
+        if constexpr (SMALL) {
+            const int row = k0 + lane;
+            bad = __builtin_amdgcn_ballot_w64(lane < SK && row < w.kend && pages.at(row, w.kend, 0, 0) < 0) != 0;
+        }
+        const int masked = bad || rows_masked(p, w, k0, SK);
+        if constexpr (MOD != 0) {
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                const float dist = (float)(tok[t].pos - k0 - 8 * g);
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    s[t][b] *= qs[t];
+                    if (has_cap<MOD>(p)) {
+                        s[t][b] = capped_over<_Float16, MOD>(s[t][b], p.cap_in, p.cap_log2e, ref[t] - kUp);
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) s[t][b][r] = __builtin_fmaf(s[t][b][r], p.scale_log2e, kUp - ref[t]);
+                    }
+                    if (has_bias<MOD>(p)) {
+                        f32x4 y;
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) y[r] = dist - (float)(4 * b + r);
+                        if (masked && p.pos) {
+                            // drafted keys stand where the program says
+                            const int bit = k0 + 8 * g + 4 * b - w.len;
+#pragma unroll
+                            for (int r = 0; r < 4; ++r)
+                                if (bit + r >= 0)
+                                    y[r] = (float)(tok[t].pos - p.pos[w.b * p.n + min(bit + r, p.n - 1)]);
+                        }
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) s[t][b][r] = __builtin_fmaf(-slope[t], fabsf(y[r]), s[t][b][r]);
+                    }
+                }
+            }
+        }
+        if (masked) {
+            const RowsParams lp = late_params<RowsParams>();
+            const uint64_t there = keys_there(lp, w, k0, lane, bad);
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                uint64_t see = there & seen_bits(lp, w, tok[t], k0);
+                if (lp.window) see &= window_bits<SK>(lp, w, tok[t], k0, [&](int b, int r) { return 8 * g + 4 * b + r; });
+                const unsigned bits = (unsigned)(see >> (8 * g));
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (!(bits & (1u << (4 * b + r)))) s[t][b][r] = OPS_NEG_INF;
+            }
+            // rows that are not there, or are no numbers, weigh nothing: what those that see them get comes at the end
+            const unsigned mine = (unsigned)(there >> (8 * g));
+#pragma unroll
+            for (int n = 0; n < NV; ++n)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const unsigned sh = 16 * (e % 2), keep = ~(0xffffu << sh);
+                    const unsigned hb = x.big[n].w[e / 2] >> sh & 0x7c00u, ho = x.off[n].w[e / 2] >> sh & 0x7c00u;
+                    const bool nan = hb == 0x7c00u || ho == 0x7c00u, there_ = mine >> e & 1;
+                    if (nan && there_) special = 1;
+                    if (nan || !there_) {
+                        x.big[n].w[e / 2] &= keep;
+                        x.off[n].w[e / 2] &= keep;
+                    }
+                }
+        }
+        // softmax: the reference of a row moves only when a score passes it by more than kLazy, or at its first key
+        h8 pb[MT];
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            float mt = s[t][0][0];
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) mt = __builtin_elementwise_maximum(mt, s[t][b][r]);
+            mt -= kUp;
+            const bool seen = m[t] != OPS_NEG_INF;
+            const float limit = seen ? kLazy : OPS_NEG_INF;
+            if (__builtin_amdgcn_ballot_w64(mt * c[t] > limit) != 0) {
+                mt = row4_max(mt);
+                const bool grow = mt * c[t] > limit;
+                const float delta = grow ? mt : 0.0f;
+#pragma unroll
+                for (int b = 0; b < 2; ++b) s[t][b] -= delta;
+                if (grow) m[t] = ref[t] = ref[t] + delta;
+                if (__builtin_amdgcn_ballot_w64(grow && seen) != 0) {
+                    const float corr = grow && seen ? ops_exp2(-delta * c[t]) : 1.0f;
+                    l[t] *= corr;
+#pragma unroll
+                    for (int j = 0; j < NO; ++j) o[t][j] *= corr;
+                }
+            }
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float y = ops_exp2(MOD != 0 ? s[t][b][r] : __builtin_fmaf(s[t][b][r], c[t], kProb));
+                    pb[t][4 * b + r] = _Float16(y);   // (11 bits; the row's sum takes them unrounded)
+                    l[t] += y;
+                }
+        }
+#pragma unroll
+        for (int n = 0; n < NV; ++n)
+#pragma unroll
+            for (int j = 0; j < VW; ++j) {
+                const h8 v = dequant(x.v[n].w[j], [&](int e) { return __builtin_bit_cast(h2, x.big[n].w[e]); },
+                                     [&](int e) { return __builtin_bit_cast(h2, x.off[n].w[e]); });
+#pragma unroll
+                for (int t = 0; t < MT; ++t) o[t][n * VW + j] = M4::mma(v, pb[t], o[t][n * VW + j]);
+            }
+        __builtin_amdgcn_sched_barrier(0);
+        load_v(x, i + 2, page2);
+        page0 = page1;
+        page1 = page2;
+        page2 = look_up(i + 3);
+    };
+    for (int i = 0; i < nblk; i += 2) {
+        block(i, A, page0);
+        if (i + 1 < nblk) block(i + 1, B, page0);
+    }
+
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        m[t] *= c[t];   // log2 units
+        l[t] = row4_sum(l[t]);
+    }
+    // Join the waves' sums: the upper half leaves its own in LDS, the lower half adds them, and again.
+    __shared__ f32x4 sums[NW / 2][MT * NO * 64];
+    __shared__ float Ml[NW / 2][MT][2][16];
+    __shared__ int any_special;
+    if (threadIdx.x == 0) any_special = 0;
+    __syncthreads();
+    if (special) any_special = 1;
+#pragma unroll
+    for (int half = NW / 2; half >= 1; half /= 2) {
+        __syncthreads();
+        if (wave >= half && wave < 2 * half) {
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+#pragma unroll
+                for (int j = 0; j < NO; ++j) sums[wave - half][(t * NO + j) * 64 + lane] = o[t][j];
+                if (g == 0) {
+                    Ml[wave - half][t][0][li] = m[t];
+                    Ml[wave - half][t][1][li] = l[t];
+                }
+            }
+        }
+        __syncthreads();
+        if (wave < half) {
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                const float m2 = Ml[wave][t][0][li], l2 = Ml[wave][t][1][li];
+                const float mn = fmaxf(m[t], m2), top = mn == OPS_NEG_INF ? 0.0f : mn;
+                const float c1 = ops_exp2(m[t] - top), c2 = ops_exp2(m2 - top);
+                m[t] = mn;
+                l[t] = l[t] * c1 + l2 * c2;
+#pragma unroll
+                for (int j = 0; j < NO; ++j) o[t][j] = o[t][j] * c1 + sums[wave][(t * NO + j) * 64 + lane] * c2;
+            }
+        }
+    }
+    if (wave != 0) return;
+
+    // Partial sums, or the rows themselves where the sequence is one run.  The lane's columns: 4 VW in a row of each load.
+    const RowsParams lp = late_params<RowsParams>();
+    const int64_t part = ((int64_t)w.run * lp.kv_heads + w.hk) * lp.nrb + w.rb;
+    float* const po = lp.part_o + part * lp.block_rows * PD;
+    float* const pm = lp.part_ml + part * 2 * lp.block_rows;
+    auto out_row = [&](int r) {
+        const int h = w.hk * lp.group + (w.rfirst + r) % lp.group;
+        return reinterpret_cast<T*>(lp.out) + w.b * lp.os.b + h * lp.os.h + (w.rfirst + r) / lp.group * lp.os.s;
+    };
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        const int r = 16 * t + li;
+        if (w.runs > 1) {
+#pragma unroll
+            for (int n = 0; n < NV; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int j = 0; j < VW; ++j) po[r * PD + n * 16 * VW + 4 * VW * g + VW * e + j] = o[t][n * VW + j][e];
+            if (g == 0) {
+                pm[r] = m[t] - (kProb - kProbLog2<T>);   // as the joining kernel of the type takes them
+                pm[lp.block_rows + r] = l[t];
+            }
+            continue;
+        }
+        if (w.rfirst + r >= w.nrows) continue;
+        const float inv = l[t] == 0.0f ? 0.0f : 1.0f / l[t];
+        T* const out = out_row(r);
+#pragma unroll
+        for (int n = 0; n < NV; ++n)
+#pragma unroll
+            for (int e = 0; e < VW; ++e) {   // the e-th four of the columns
+                f32x4 y;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) y[j] = o[t][n * VW + (4 * e + j) % VW][(4 * e + j) / VW] * inv;
+                const int col = n * 16 * VW + 4 * VW * g + 4 * e;
+                if (lp.vec4) store4<T, true>(out, col, D, y);
+                else store4<T, false>(out, col, D, y);
+            }
+        if (lp.lse && g == 0)
+            lp.lse[((int64_t)w.b * lp.heads + w.hk * lp.group + (w.rfirst + r) % lp.group) * lp.n + tok[t].token] =
+                l[t] == 0.0f ? OPS_NEG_INF : (m[t] + __builtin_log2f(l[t]) - kProb) * kLn2;
+    }
+    if (!any_special) return;
+    // values that are no numbers, to the rows that see them
+    __threadfence();
+    const int mine = min(16 * MT, w.nrows - w.rfirst);
+#pragma unroll 1
+    for (int key = w.kbeg; key < w.kend; ++key) {
+        if (key >= w.gap && key - w.gap < w.skip) continue;
+        const int page = pages.page(key);
+        if (page < 0) continue;
+        const int64_t at = ((int64_t)(lp.table ? page : w.b) * lp.kv_heads + w.hk) * page_rows + (lp.table ? key & pages.page_mask : key);
+#pragma unroll 1
+        for (int col = lane; col < D; col += 64) {
+            const unsigned short* const sv =
+                reinterpret_cast<const unsigned short*>(VS) + (at / 8 * NDC + col / 32) * 16 + at % 8;
+            const unsigned code = V[at / 8 * D + col] >> (4 * (at % 8 / 2) + 16 * (at % 2)) & 15;
+            const float y = __builtin_fmaf(1.0f + (float)code * 0.0625f, float(bits_half(sv[0])), float(bits_half(sv[8])));
+            if (!not_finite(y)) continue;
+#pragma unroll 1
+            for (int r = 0; r < mine; ++r) {
+                if (!rows_see(lp, w, (w.rfirst + r) / lp.group, key)) continue;
+                if (w.runs > 1) po[r * PD + col] += y;
+                else out_row(r)[col] = T(float(out_row(r)[col]) + y);
+            }
+        }
+    }
+}
+
+#define PASTE_(a, b, c, d) a##b##c##d
+#define PASTE(a, b, c, d) PASTE_(a, b, c, d)
+#define KERNEL(NDC, MT, MOD, SMALL, TAG, WAVES)                                                         \
+    extern "C" __global__ __launch_bounds__(64 * kRows4Waves, WAVES)                                    \
+    void PASTE(fa_rows4_, OPS_NAME, _c##NDC##_t##MT, TAG)(RowsParams p) {                               \
+        rows4<OPS_T, NDC, MT, MOD, SMALL>(p);                                                           \
+    }
+// plain scores, or looked up (m); pages of less than 32 rows (p)
+#define KINDS(NDC, MT, WAVES)                  \
+    KERNEL(NDC, MT, 0, false, , WAVES)         \
+    KERNEL(NDC, MT, kAny, false, m, WAVES)     \
+    KERNEL(NDC, MT, kAny, true, p, WAVES)
+KINDS(2, 1, 2)
+KINDS(2, 2, 2)
+KINDS(2, 4, 2)
+KINDS(4, 1, 2)
+KINDS(4, 2, 2)
+KINDS(4, 4, 1)
+KINDS(8, 1, 2)
+KINDS(8, 2, 1)
+// other widths
+KERNEL(1, 1, kAny, false, m, 2)
+KERNEL(3, 1, kAny, false, m, 2)
+KERNEL(5, 1, kAny, false, m, 2)
+KERNEL(6, 1, kAny, false, m, 2)
+KERNEL(7, 1, kAny, false, m, 2)
+KERNEL(1, 1, kAny, true, p, 2)
+KERNEL(3, 1, kAny, true, p, 2)
+KERNEL(5, 1, kAny, true, p, 2)
+KERNEL(6, 1, kAny, true, p, 2)
+KERNEL(7, 1, kAny, true, p, 2)
+extern "C" __global__ __launch_bounds__(256) void PASTE(fa_cache4_append_, OPS_NAME, , )(Cache4Params p) {
+    cache4_append<OPS_T>(p);
+}
+extern "C" __global__ __launch_bounds__(256) void PASTE(fa_cache4_read_, OPS_NAME, , )(Cache4Params p) {
+    cache4_read<OPS_T>(p);
+}

@@ -11,7 +11,9 @@
 namespace {
 
 // Code objects: those of score attention and of the cache one a type (FA_DTYPE_*).
-enum OpsModule { kRotaryModule, kScoreModule, kCacheModule = kScoreModule + 3, kNormModule = kCacheModule + 3, kOpsModules };
+enum OpsModule { kRotaryModule, kScoreModule, kCacheModule = kScoreModule + 3, kNormModule = kCacheModule + 3,
+                 kCache4Module,   // bf16, f16
+                 kOpsModules = kCache4Module + 2 };
 OpsModule of_type(OpsModule m, int dtype) { return static_cast<OpsModule>(m + dtype); }
 
 struct OpsState {
@@ -39,7 +41,8 @@ constexpr size_t kOpsMaxTokens = size_t(1) << 31;   // of a rotary launch: a thr
 int ops_module(int dev, OpsModule which) {
     static const char* const files[] = {"fa_rotary.hsaco",     "fa_score_f32.hsaco",  "fa_score_bf16.hsaco",
                                         "fa_score_f16.hsaco",  "fa_cache_f32.hsaco",  "fa_cache_bf16.hsaco",
-                                        "fa_cache_f16.hsaco",  "fa_norm.hsaco"};
+                                        "fa_cache_f16.hsaco",  "fa_norm.hsaco",      "fa_cache4_bf16.hsaco",
+                                        "fa_cache4_f16.hsaco"};
     OpsState& s = g_ops[dev];
     std::call_once(s.once[which], [&] {
         std::string path = module_path();
@@ -252,6 +255,28 @@ struct RowsPlan {
     int mt, threads, rows, nrb, step, share, runs;
     size_t floats;
 };
+// Shares the keys of all sequences out over runs; up to `whole` keys a sequence are one.  D: columns of a row of
+// partial sums.
+void share_keys(RowsPlan* plan, size_t batch, size_t kv_heads, size_t rows, size_t keys, size_t resident, size_t whole,
+                int D) {
+    RowsPlan& r = *plan;
+    r.nrb = static_cast<int>((rows + r.rows - 1) / r.rows);
+    const size_t units = kv_heads * r.nrb;   // workgroups a run
+    // One round of resident workgroups where the sequences' last, shorter runs (one a sequence)
+    // leave room, else several rounds of shorter runs.
+    const size_t slots = std::max<size_t>(1, resident / units);
+    size_t share = batch == 1 ? slots : 2 * (batch - 1) <= slots ? slots - (batch - 1) : 4 * slots;
+    share = std::min(share, batch * std::max<size_t>(1, (keys + r.step - 1) / r.step));
+    if (batch * units >= 4 * resident) share = 1;   // sequences enough: one run each
+    if (keys <= whole) share = 1;
+    r.share = static_cast<int>(share);
+    // each sequence rounds its share up to whole runs; eight runs and heads more or less fall
+    // on the eight XCDs evenly
+    size_t runs = share == 1 ? batch : share + batch - 1;
+    while (runs * kv_heads % 8 != 0 && runs >= 8) ++runs;
+    r.runs = static_cast<int>(runs);
+    r.floats = share > 1 ? runs * units * r.rows * (D + 2) : 0;
+}
 RowsPlan plan_rows(int dtype, int D, bool vec, size_t batch, size_t kv_heads, size_t rows, size_t keys, int num_cus) {
     RowsPlan r{};
     const bool f32 = dtype == FA_DTYPE_F32;
@@ -277,35 +302,17 @@ RowsPlan plan_rows(int dtype, int D, bool vec, size_t batch, size_t kv_heads, si
         r.rows = 128 * r.mt;
         r.step = f32 || D > 128 ? 32 : 64;
     }
-    r.nrb = static_cast<int>((rows + r.rows - 1) / r.rows);
-    const size_t units = kv_heads * r.nrb;   // workgroups a run
-    // One round of resident workgroups where the sequences' last, shorter runs (one a sequence)
-    // leave room, else several rounds of shorter runs.
-    const size_t slots = std::max<size_t>(1, resident / units);
-    size_t share = batch == 1 ? slots : 2 * (batch - 1) <= slots ? slots - (batch - 1) : 4 * slots;
-    share = std::min(share, batch * std::max<size_t>(1, (keys + r.step - 1) / r.step));
-    if (batch * units >= 4 * resident) share = 1;   // sequences enough: one run each
-    // Few keys: one run each too, which saves the merge, some 4 us, unless walking them costs as much (measured: 8
+    // Few keys: one run each, which saves the merge, some 4 us, unless walking them costs as much (measured: 8
     // sequences of 250 keys, bf16, 7 rows of 64 columns 13.1 us split, 9.7 whole; 3 of 250, f32, 8 rows of 80 17.6
     // and 23.6)
-    if (keys <= static_cast<size_t>(r.step) * (f32 || D > 128 ? 1 : 4)) share = 1;
-    r.share = static_cast<int>(share);
-    // each sequence rounds its share up to whole runs; eight runs and heads more or less fall
-    // on the eight XCDs evenly
-    size_t runs = share == 1 ? batch : share + batch - 1;
-    while (runs * kv_heads % 8 != 0 && runs >= 8) ++runs;
-    r.runs = static_cast<int>(runs);
-    r.floats = share > 1 ? runs * units * r.rows * (D + 2) : 0;
+    share_keys(&r, batch, kv_heads, rows, keys, resident, static_cast<size_t>(r.step) * (f32 || D > 128 ? 1 : 4), D);
     return r;
 }
 
-int run_rows(int dev, hipStream_t stream, int dtype, int D, bool vec, RowsParams* p, size_t keys) {
-    vec = vec && (!p->table || p->page_shift >= 4);   // DMA moves runs of rows of one page
-    const OpsModule module = of_type(kCacheModule, dtype);
-    int rc = ops_module(dev, module);
-    if (rc != FA_OK) return rc;
+// Launches a rows kernel, and the one that joins its partial sums (of D columns).
+int launch_rows(int dev, hipStream_t stream, int dtype, OpsModule module, const char* kernel, const RowsPlan& plan, int D,
+                bool vec, RowsParams* p) {
     const size_t rows = static_cast<size_t>(p->n) * p->group;
-    const RowsPlan plan = plan_rows(dtype, D, vec, p->batch, p->kv_heads, rows, keys, g_dev[dev].num_cus);
     p->nrb = plan.nrb;
     p->block_rows = plan.rows;
     p->num_runs = plan.runs;
@@ -314,24 +321,36 @@ int run_rows(int dev, hipStream_t stream, int dtype, int D, bool vec, RowsParams
     const size_t grid = static_cast<size_t>(plan.runs) * p->kv_heads * plan.nrb;
     const size_t mgrid = static_cast<size_t>(p->batch) * p->kv_heads * rows;
     if (grid > kOpsMaxGrid / 2 || (plan.floats && mgrid > kOpsMaxGrid)) return FA_ERR_UNSUPPORTED;
+    int rc;
     OpsWorkspace ws;
     if (plan.floats) {
         if ((rc = ws.get(dev, stream, plan.floats * sizeof(float))) != FA_OK) return rc;
         p->part_o = static_cast<float*>(ws.ptr);
         p->part_ml = p->part_o + grid * plan.rows * D;
     }
-    char name[64];
-    std::snprintf(name, sizeof(name), "fa_rows_%s_%s_d%d_t%d%s", plan.stream ? "stream" : "shared", dtype_name(dtype), D,
-                  plan.mt, !vec ? "s" : p->cap_log2e != 0.0f ? (p->slopes ? "cb" : "c") : p->slopes ? "b" : "");
-    rc = ops_launch(dev, module, name, grid, plan.threads, p, stream);
+    rc = ops_launch(dev, module, kernel, grid, plan.threads, p, stream);
     if (rc == FA_OK && plan.floats) {
         // eight runs a sequence or more: a workgroup a row
         const bool wide = !vec || plan.share > 8 * p->batch;
+        char name[64];
         std::snprintf(name, sizeof(name), "fa_rows_merge_%s_d%d%s", dtype_name(dtype), D, !vec ? "s" : wide ? "w" : "");
         const size_t per = wide ? 1 : 1024 / D;
-        rc = ops_launch(dev, module, name, (mgrid + per - 1) / per, 256, p, stream);
+        rc = ops_launch(dev, of_type(kCacheModule, dtype), name, (mgrid + per - 1) / per, 256, p, stream);
     }
     return ws.done(stream, rc);
+}
+
+int run_rows(int dev, hipStream_t stream, int dtype, int D, bool vec, RowsParams* p, size_t keys) {
+    vec = vec && (!p->table || p->page_shift >= 4);   // DMA moves runs of rows of one page
+    const OpsModule module = of_type(kCacheModule, dtype);
+    const int rc = ops_module(dev, module);
+    if (rc != FA_OK) return rc;
+    const RowsPlan plan =
+        plan_rows(dtype, D, vec, p->batch, p->kv_heads, static_cast<size_t>(p->n) * p->group, keys, g_dev[dev].num_cus);
+    char name[64];
+    std::snprintf(name, sizeof(name), "fa_rows_%s_%s_d%d_t%d%s", plan.stream ? "stream" : "shared", dtype_name(dtype), D,
+                  plan.mt, !vec ? "s" : p->cap_log2e != 0.0f ? (p->slopes ? "cb" : "c") : p->slopes ? "b" : "");
+    return launch_rows(dev, stream, dtype, module, name, plan, D, vec, p);
 }
 
 // A window's size and sinks as kernels take them (size 0: hides nothing); farthest: the largest distance there is.
@@ -765,6 +784,59 @@ int launch_norm(int dev, hipStream_t stream, int dtype, NormParams* p, bool wide
     return ops_launch(dev, kNormModule, name, grid, kNormThreads, p, stream);
 }
 
+// A cache in 4 bits: rows of a block of memory, and of a sequence.
+int check_cache4(const fa_kv_cache4* c, size_t* block_rows, size_t* capacity) {
+    if (!c || !valid_dtype(c->dtype)) return FA_ERR_INVALID_ARG;
+    if (c->batch == 0 || c->kv_heads == 0 || c->d_head == 0) return FA_OK;
+    if (c->dtype == FA_DTYPE_F32 || c->d_head > kOpsMaxD || c->d_head % 32 != 0 || c->batch > kOpsMaxSeq ||
+        c->kv_heads > kOpsMaxSeq)
+        return FA_ERR_UNSUPPORTED;
+    if (!c->lens) return FA_ERR_INVALID_ARG;
+    if (c->block_table) {
+        if (c->page_size < 8 || (c->page_size & (c->page_size - 1)) != 0) return FA_ERR_INVALID_ARG;
+        if (c->page_size > kOpsMaxSeq || c->pages_per_seq > kOpsMaxSeq || c->n_pages > kOpsMaxSeq)
+            return FA_ERR_UNSUPPORTED;
+        *block_rows = c->page_size;
+        *capacity = c->page_size * c->pages_per_seq;
+    } else {
+        if (c->capacity % 8 != 0) return FA_ERR_INVALID_ARG;
+        *block_rows = *capacity = c->capacity;
+    }
+    if (*capacity > kOpsMaxSeq) return FA_ERR_UNSUPPORTED;
+    if (*capacity > 0 && (!c->k || !c->v || !c->k_scale || !c->v_scale)) return FA_ERR_INVALID_ARG;
+    // the kernels load words of it, 16 bytes at a time
+    if (!aligned16(c->k) || !aligned16(c->v) || !aligned16(c->k_scale) || !aligned16(c->v_scale)) return FA_ERR_INVALID_ARG;
+    return FA_OK;
+}
+int page_shift4(const fa_kv_cache4& c) {
+    int s = 0;
+    while (c.block_table && (size_t(1) << s) < c.page_size) ++s;
+    return s;
+}
+void fill_cache4(const fa_kv_cache4& c, size_t block_rows, size_t capacity, Cache4Params* p) {
+    p->k4 = c.k, p->v4 = c.v, p->kscale = c.k_scale, p->vscale = c.v_scale;
+    p->lens = c.lens, p->table = c.block_table;
+    p->batch = static_cast<int>(c.batch), p->kv_heads = static_cast<int>(c.kv_heads), p->d = static_cast<int>(c.d_head);
+    p->capacity = static_cast<int>(capacity), p->block_rows = static_cast<int>(block_rows);
+    p->page_shift = page_shift4(c);
+    p->n_pages = static_cast<int>(c.n_pages), p->pages_per_seq = static_cast<int>(c.pages_per_seq);
+}
+OpsModule cache4_module(int dtype) { return static_cast<OpsModule>(kCache4Module + (dtype == FA_DTYPE_BF16 ? 0 : 1)); }
+
+// Plan of attention over a cache in 4 bits: more tiles a wave where there are rows for them, since what a code costs
+// to become a number is then shared.
+RowsPlan plan_rows4(size_t d, size_t batch, size_t kv_heads, size_t rows, size_t keys, int num_cus) {
+    RowsPlan r{};
+    const bool widths = d == 64 || d == 128 || d == 256;
+    r.mt = !widths || rows <= 16 ? 1 : rows <= 32 || d == 256 ? 2 : 4;
+    r.threads = 64 * kRows4Waves;
+    r.rows = 16 * r.mt;
+    r.step = 32 * kRows4Waves;
+    const size_t resident = static_cast<size_t>(num_cus) * (r.mt * d >= 512 ? 1 : 2);
+    share_keys(&r, batch, kv_heads, rows, keys, resident, 4 * r.step, ops_pad_d(d));
+    return r;
+}
+
 }  // namespace
 
 extern "C" {
@@ -1117,6 +1189,124 @@ int fa_tree_attention(void* stream, const fa_tree_config* c, const fa_kv_cache* 
 int fa_window_tree_attention(void* stream, const fa_tree_config* c, const fa_window* window, const fa_kv_cache* cache,
                              const void* q, void* out, float* lse) try {
     return tree_attention(stream, c, window, cache, q, out, lse);
+} catch (...) {   // no memory for the tables of modules, kernels and workspaces
+    return FA_ERR_ALLOC;
+}
+
+int fa_cache4_append(void* stream, const fa_kv_cache4* cache, const fa_append_config* cfg, const void* k,
+                     const void* v) try {
+    size_t block_rows = 0, capacity = 0;
+    int rc = check_cache4(cache, &block_rows, &capacity);
+    if (rc != FA_OK) return rc;
+    if (!cfg) return FA_ERR_INVALID_ARG;
+    if (cfg->rotary || cfg->q_layout) return FA_ERR_UNSUPPORTED;   // rows come as they are to be kept
+    if (cache->batch == 0 || cache->kv_heads == 0 || cache->d_head == 0 || cfg->n_tokens == 0) return FA_OK;
+    const size_t d = cache->d_head, n = cfg->n_tokens;
+    if (n > kOpsMaxSeq || cache->batch * n > kOpsMaxTokens) return FA_ERR_UNSUPPORTED;
+    OpsLayout lk, lv;
+    if ((rc = resolve_layout(cfg->k, cache->batch, n, cache->kv_heads, d, 2, false, &lk)) != FA_OK ||
+        (rc = resolve_layout(cfg->v, cache->batch, n, cache->kv_heads, d, 2, false, &lv)) != FA_OK)
+        return rc;
+    if (!k || !v) return FA_ERR_INVALID_ARG;
+    if (capacity == 0) return FA_OK;
+    Cache4Params p{};
+    fill_cache4(*cache, block_rows, capacity, &p);
+    p.k = k, p.v = v, p.ks = lk.st, p.vs = lv.st;
+    p.n = static_cast<int>(n);
+    p.vec = vec_ok(k, lk, d) && vec_ok(v, lv, d);
+    const size_t runs = (n + 7) / 8 + 1, per = 256 / d;   // n rows touch that many runs of 8 at most
+    const size_t parts = (runs + per - 1) / per, heads = 2 * cache->batch * cache->kv_heads;
+    if (heads > kOpsMaxGrid / parts) return FA_ERR_UNSUPPORTED;
+    p.nparts = static_cast<int>(parts);
+    int dev;
+    const OpsModule module = cache4_module(cache->dtype);
+    if ((rc = ops_begin(&dev, module)) != FA_OK) return rc;
+    return ops_launch(dev, module, cache->dtype == FA_DTYPE_BF16 ? "fa_cache4_append_bf16" : "fa_cache4_append_f16",
+                      heads * parts, 256, &p, static_cast<hipStream_t>(stream));
+} catch (...) {   // no memory for the tables of modules, kernels and workspaces
+    return FA_ERR_ALLOC;
+}
+
+int fa_cache4_read(void* stream, const fa_kv_cache4* cache, const fa_read_config* cfg, const int32_t* rows, void* k_out,
+                   void* v_out) try {
+    size_t block_rows = 0, capacity = 0;
+    int rc = check_cache4(cache, &block_rows, &capacity);
+    if (rc != FA_OK) return rc;
+    if (!cfg) return FA_ERR_INVALID_ARG;
+    if (cache->batch == 0 || cache->kv_heads == 0 || cache->d_head == 0 || cfg->n_rows == 0) return FA_OK;
+    const size_t d = cache->d_head, n = cfg->n_rows;
+    if (n > kOpsMaxSeq || cache->batch * n > kOpsMaxTokens) return FA_ERR_UNSUPPORTED;
+    OpsLayout lk, lv;
+    if ((rc = resolve_layout(cfg->k, cache->batch, n, cache->kv_heads, d, 2, true, &lk)) != FA_OK ||
+        (rc = resolve_layout(cfg->v, cache->batch, n, cache->kv_heads, d, 2, true, &lv)) != FA_OK)
+        return rc;
+    if (!rows) return FA_ERR_INVALID_ARG;
+    if (!k_out && !v_out) return FA_OK;
+    const size_t heads = 2 * cache->batch * cache->kv_heads, words = n * (d / 8);
+    if (heads > kOpsMaxGrid * 256 / words) return FA_ERR_UNSUPPORTED;
+    Cache4Params p{};
+    fill_cache4(*cache, block_rows, capacity, &p);
+    p.ko = k_out, p.vo = v_out, p.ks = lk.st, p.vs = lv.st, p.rows = rows;
+    p.n = static_cast<int>(n);
+    p.vec = vec_ok(k_out, lk, d) && vec_ok(v_out, lv, d);
+    int dev;
+    const OpsModule module = cache4_module(cache->dtype);
+    if ((rc = ops_begin(&dev, module)) != FA_OK) return rc;
+    return ops_launch(dev, module, cache->dtype == FA_DTYPE_BF16 ? "fa_cache4_read_bf16" : "fa_cache4_read_f16",
+                      (heads * words + 255) / 256, 256, &p, static_cast<hipStream_t>(stream));
+} catch (...) {   // no memory for the tables of modules, kernels and workspaces
+    return FA_ERR_ALLOC;
+}
+
+int fa_cache4_attention(void* stream_, const fa_tree_config* c, const fa_window* window, const fa_kv_cache4* cache,
+                        const void* q, void* out, float* lse) try {
+    size_t block_rows = 0, capacity = 0;
+    int rc = check_cache4(cache, &block_rows, &capacity);
+    if (rc != FA_OK) return rc;
+    if (!c) return FA_ERR_INVALID_ARG;
+    if (cache->batch == 0 || c->heads == 0 || c->n_tokens == 0 || cache->d_head == 0) return FA_OK;
+    if (cache->kv_heads == 0 || c->heads % cache->kv_heads != 0) return FA_ERR_INVALID_ARG;
+    if (c->heads > kOpsMaxSeq || c->n_tokens > kTreeMaxTokens) return FA_ERR_UNSUPPORTED;
+    const size_t d = cache->d_head, n = c->n_tokens;
+    ScoreScale sc;
+    OpsLayout lq, lo;
+    if ((rc = resolve_scale(c->softmax_scale, c->softcap, d, &sc)) != FA_OK ||
+        (rc = resolve_layout(c->q, cache->batch, n, c->heads, d, 2, false, &lq)) != FA_OK ||
+        (rc = resolve_layout(c->out, cache->batch, n, c->heads, d, 2, true, &lo)) != FA_OK)
+        return rc;
+    int size, sinks;
+    if ((rc = resolve_window(window, false, kWindowMaxPos, &size, &sinks)) != FA_OK) return rc;
+    if (!q || !out) return FA_ERR_INVALID_ARG;
+    if (cache->batch * c->heads > kOpsMaxGrid) return FA_ERR_UNSUPPORTED;
+    RowsParams p{};
+    p.q = q, p.k = cache->k, p.v = cache->v, p.k_scale = cache->k_scale, p.v_scale = cache->v_scale;
+    p.out = out, p.lse = lse;
+    p.slopes = c->slopes, p.lens = cache->lens, p.table = cache->block_table;
+    p.pos = c->positions, p.mask = c->mask;
+    p.qs = lq.st, p.os = lo.st;
+    p.batch = static_cast<int>(cache->batch), p.heads = static_cast<int>(c->heads);
+    p.kv_heads = static_cast<int>(cache->kv_heads), p.group = static_cast<int>(c->heads / cache->kv_heads);
+    p.n = static_cast<int>(n), p.sk = static_cast<int>(capacity), p.d = static_cast<int>(d);
+    p.page_shift = page_shift4(*cache);
+    p.n_pages = static_cast<int>(cache->n_pages), p.pages_per_seq = static_cast<int>(cache->pages_per_seq);
+    p.mask_words = static_cast<int>((n + 63) / 64), p.mask_shared = c->mask_shared ? 1 : 0;
+    p.window = size, p.sinks = sinks;
+    p.scale_log2e = sc.scale_log2e, p.cap_in = sc.cap_in, p.cap_log2e = sc.cap_log2e;
+    p.block4 = static_cast<int>(block_rows);
+    p.vec4 = vec_ok(q, lq, d) && ovec_ok(out, lo, 2);
+    int dev;
+    const OpsModule module = cache4_module(cache->dtype), joins = of_type(kCacheModule, cache->dtype);
+    if ((rc = ops_begin(&dev, module)) != FA_OK || (rc = ops_module(dev, joins)) != FA_OK) return rc;
+    const hipStream_t stream = static_cast<hipStream_t>(stream_);
+    const size_t rows = n * static_cast<size_t>(p.group);
+    const RowsPlan plan = plan_rows4(d, cache->batch, cache->kv_heads, rows, window_keys(capacity, size, sinks, n, false),
+                                     g_dev[dev].num_cus);
+    char name[64];
+    std::snprintf(name, sizeof(name), "fa_rows4_%s_c%d_t%d%s", dtype_name(cache->dtype), static_cast<int>(d / 32), plan.mt,
+                  cache->block_table && cache->page_size < 32                       ? "p"
+                  : c->softcap > 0.0f || c->slopes || (d != 64 && d != 128 && d != 256) ? "m"
+                                                                                    : "");
+    return launch_rows(dev, stream, cache->dtype, module, name, plan, ops_pad_d(d), p.vec4, &p);
 } catch (...) {   // no memory for the tables of modules, kernels and workspaces
     return FA_ERR_ALLOC;
 }

@@ -80,6 +80,27 @@ struct RowsParams {
     int num_runs, share;      // runs of keys a kv head, all sequences together; what the keys are shared out over
     int step;                 // keys that a run's length is a multiple of
     float scale_log2e, cap_in, cap_log2e;   // as in ScoreParams
+    const void *k_scale, *v_scale;          // a cache in 4 bits: its steps and offsets,
+    int block4;               // the rows of a page (without pages: of a sequence),
+    int vec4;                 // and whether rows of q and out are aligned
+};
+
+// Waves of a workgroup of the kernel over a cache in 4 bits.
+constexpr int kRows4Waves = 4;
+// Largest size of a value in such a cache: larger ones count as that, and what codes stand for stays in f16's range.
+constexpr float kCache4Max = 60000.0f;
+// Append to and rows out of such a cache.
+struct Cache4Params {
+    const void *k, *v;        // append
+    void *ko, *vo;            // read; NULL: not wanted
+    OpsStrides ks, vs;
+    uint32_t *k4, *v4;        // [blocks, kv_heads, rows, d / 8], [blocks, kv_heads, rows / 8, d]
+    uint16_t *kscale, *vscale;   // [blocks, kv_heads, rows, d / 32, (S, O)], [blocks, kv_heads, rows / 8, d / 32, (S, O), 8]
+    const int32_t *lens, *table, *rows;
+    int batch, kv_heads, n, d;
+    int capacity, block_rows, page_shift, n_pages, pages_per_seq;
+    int nparts;               // workgroups of a head's rows (append)
+    int vec;                  // rows of k, v (ko, vo) are aligned
 };
 
 // One tensor of a rotary or append launch.

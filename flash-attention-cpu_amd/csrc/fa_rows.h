@@ -1,0 +1,305 @@
+// fa_rows.h -- what the kernels for query rows over a cache have in common
+// (fa_cache.hip, fa_cache4.hip): pages, the runs that the keys of all sequences are cut into, and
+// what a row sees.
+#ifndef FA_ROWS_H
+#define FA_ROWS_H
+
+#include "fa_ops_common.h"
+
+// The pages of a sequence.
+struct CachePages {
+    const int32_t* table;   // nullptr: rows one after another
+    int shift, page_mask, n_pages;
+    // page of a row, -1: bad (0 without pages)
+    __device__ __forceinline__ int page(int row) const {
+        if (!table) return 0;
+        const int pg = load_uniform(table + (row >> shift));
+        return (unsigned)pg < (unsigned)n_pages ? pg : -1;
+    }
+    // element offset of a row, or -1
+    __device__ __forceinline__ int64_t at(int row, int end, int64_t seq, int64_t batch) const {
+        if (row >= end) return -1;
+        if (!table) return row * seq;
+        const int pg = table[row >> shift];
+        return (unsigned)pg < (unsigned)n_pages ? pg * batch + (row & page_mask) * seq : -1;
+    }
+};
+
+__device__ __forceinline__ CachePages rows_pages(const RowsParams& p, int b) {
+    return {p.table ? p.table + (int64_t)b * p.pages_per_seq : nullptr, p.page_shift, (1 << p.page_shift) - 1, p.n_pages};
+}
+
+// What a workgroup of either kernel works on.
+struct RowsWork {
+    int run, rb, b, hk;
+    int runs;   // of the sequence
+    int len, prefix, open, kbeg, kend, nrows, rfirst;
+    int kwalk;        // keys to walk, from kbeg on, without those that are left out
+    int gap, skip;    // keys from `gap` on are left out, `skip` of them
+    int low;          // a window's: keys before this and not before p.sinks are hidden from some row
+    int tree, docs;
+    // the key that stands `i` behind kbeg (a multiple of 16) among those walked
+    __device__ __forceinline__ int key(int i) const {
+        const int k = kfirst + i;
+        return k + (k >= gap ? skip : 0);
+    }
+    int kfirst;       // kbeg among those walked
+};
+
+// Keys that any query of sequence b sees: those before `total`, without `skip` ones from `gap` on where a window
+// leaves them out (multiples of 64, so that blocks of keys start where they do without).
+struct Walk {
+    int total, gap, skip;
+    __device__ __forceinline__ int walked() const { return total - skip; }
+};
+__device__ __forceinline__ Walk rows_walk(const RowsParams& p, int b) {
+    Walk w = {0, 0x7fffffff, 0};
+    int first;   // position of the first query
+    if (p.lens) {
+        const int len = p.lens[b];
+        w.total = len < 0 ? 0 : (int)min((int64_t)len + p.n, (int64_t)p.sk);
+        first = len;
+    } else {
+        w.total = p.causal ? max(min(max(p.q_start + p.n, p.prefix ? p.prefix[b] : 0), p.sk), 0) : p.sk;
+        first = p.q_start;
+    }
+    if (p.window) {
+        if (!p.lens) w.total = min(w.total, max(max(first + p.n - 1 + p.window, p.sinks), 0));
+        w.gap = (p.sinks + 63) & ~63;
+        const int low = min(first - p.window + 1, w.total);
+        w.skip = max((max(low, 0) & ~63) - w.gap, 0);
+    }
+    return w;
+}
+__device__ __forceinline__ int rows_total(const RowsParams& p, int b) { return rows_walk(p, b).walked(); }
+
+// The runs of a sequence: their length in steps, how many, and the first one's number.
+struct Runs {
+    int b, steps, count, first;
+};
+// All sequences' steps are shared out over p.share runs, and a sequence takes as many whole runs as hold
+// its own, one at least.  Every wave finds them for itself, a lane a sequence, 64 sequences at a
+// time: f(sequence, its runs, the end of its runs' numbers) on every lane.
+template <typename F>
+__device__ __forceinline__ int each_runs(const RowsParams& p, int lane, F f) {
+    auto steps_of = [&](int i) { return (rows_total(p, i) + p.step - 1) / p.step; };
+    int64_t all = 0;
+    for (int i = lane; i < p.batch; i += 64) all += steps_of(i);
+#pragma unroll
+    for (int s = 1; s < 64; s *= 2) all += __shfl_xor(all, s);
+    const int steps = (int)max((int64_t)1, (all + p.share - 1) / p.share);
+    int before = 0;   // runs of the sequences of earlier chunks
+    for (int base = 0; base < p.batch; base += 64) {
+        const int i = base + lane;
+        const int n = i < p.batch ? max(1, (steps_of(i) + steps - 1) / steps) : 0;
+        int end = n;
+#pragma unroll
+        for (int s = 1; s < 64; s *= 2) {
+            const int x = __shfl_up(end, s);
+            end += lane >= s ? x : 0;
+        }
+        end += before;
+        if (f(base, n, end)) break;
+        before = __builtin_amdgcn_readlane(end, 63);
+    }
+    return steps;
+}
+// The runs of a call of one sequence.
+__device__ __forceinline__ Runs runs_of_one(const RowsParams& p) {
+    const int all = (rows_total(p, 0) + p.step - 1) / p.step, steps = max(1, (all + p.share - 1) / p.share);
+    return {0, steps, max(1, (all + steps - 1) / steps), 0};
+}
+// The sequence that run `run` (the same on all lanes) belongs to; b < 0: no such run.
+__device__ __forceinline__ Runs runs_of_run(const RowsParams& p, int run, int lane) {
+    if (p.batch == 1) {
+        Runs r = runs_of_one(p);
+        if (run >= r.count) r.b = -1;
+        return r;
+    }
+    Runs r = {-1, 0, 0, 0};
+    if (p.share == 1) {   // a run each: with many sequences every workgroup would look through all of them
+        if (run < p.batch) r = {run, (rows_total(p, run) + p.step - 1) / p.step, 1, run};
+        return r;
+    }
+    r.steps = each_runs(p, lane, [&](int base, int n, int end) {
+        const uint64_t hit = __builtin_amdgcn_ballot_w64(n > 0 && run >= end - n && run < end);
+        if (hit == 0) return false;
+        const int at = __builtin_ctzll(hit);
+        r.b = base + at;
+        r.count = __builtin_amdgcn_readlane(n, at);
+        r.first = __builtin_amdgcn_readlane(end, at) - r.count;
+        return true;
+    });
+    return r;
+}
+// Those of sequence b, each lane its own.
+__device__ __forceinline__ Runs runs_of_sequence(const RowsParams& p, int b, int lane) {
+    if (p.batch == 1) return runs_of_one(p);
+    Runs r = {b, 0, 0, 0};
+    r.steps = each_runs(p, lane, [&](int base, int n, int end) {
+        const int count = __shfl(n, b - base), last = __shfl(end, b - base);
+        if (b >= base && b < base + 64) {
+            r.count = count;
+            r.first = last - count;
+        }
+        return false;
+    });
+    return r;
+}
+
+// Returns whether there is work.
+__device__ __forceinline__ bool rows_work(const RowsParams& p, int rows, int lane, RowsWork* out) {
+    RowsWork& w = *out;
+    // the row blocks of one run of keys side by side on one XCD where the counts allow
+    int rk;
+    if ((p.num_runs * p.kv_heads & 7) == 0) {
+        const int t = blockIdx.x >> 3;
+        w.rb = t % p.nrb;
+        rk = t / p.nrb * 8 + (blockIdx.x & 7);
+    } else {
+        w.rb = blockIdx.x % p.nrb;
+        rk = blockIdx.x / p.nrb;
+    }
+    w.run = rk / p.kv_heads;
+    w.hk = rk % p.kv_heads;
+    const Runs r = runs_of_run(p, w.run, lane);
+    w.b = __builtin_amdgcn_readfirstlane(r.b);
+    if (w.b < 0) return false;
+    w.runs = __builtin_amdgcn_readfirstlane(r.count);
+    w.tree = p.lens != nullptr;
+    w.docs = p.q_doc != nullptr;
+    // all of the filled rows, then the drafted ones; every row sees those before `open`
+    w.len = w.tree ? load_uniform(p.lens + w.b) : 0;
+    w.prefix = p.prefix ? load_uniform(p.prefix + w.b) : 0;
+    if (w.tree) {
+        w.open = min(max(w.len, 0), p.sk);
+    } else {
+        w.open = w.docs ? 0 : p.causal ? max(p.q_start + 1, w.prefix) : p.sk;
+    }
+    w.low = INT32_MIN;
+    if (p.window) {
+        int last = p.q_start + p.n - 1;   // position of the last query
+        if (w.tree) {
+            last = p.pos ? w.len : (int)min((int64_t)w.len + p.n - 1, (int64_t)kWindowMaxPos);
+            for (int i = lane; p.pos && i < p.n; i += 64) last = max(last, p.pos[(int64_t)w.b * p.n + i]);
+#pragma unroll
+            for (int s = 1; s < 64; s *= 2) last = max(last, __shfl_xor(last, s));
+            last = min(__builtin_amdgcn_readfirstlane(last), kWindowMaxPos);
+        } else {
+            w.open = min(w.open, max(p.q_start + p.window, 0));
+        }
+        w.low = last - p.window + 1;
+    }
+    const Walk walk = rows_walk(p, w.b);
+    w.gap = __builtin_amdgcn_readfirstlane(walk.gap);
+    w.skip = __builtin_amdgcn_readfirstlane(walk.skip);
+    const int total = __builtin_amdgcn_readfirstlane(walk.walked());
+    const int64_t per = (int64_t)__builtin_amdgcn_readfirstlane(r.steps) * p.step;
+    w.kfirst = (int)min((w.run - __builtin_amdgcn_readfirstlane(r.first)) * per, (int64_t)total);
+    const int last = (int)min(w.kfirst + per, (int64_t)total);
+    w.kwalk = last - w.kfirst;
+    w.kbeg = w.key(0);
+    w.kend = last + (last > w.gap ? w.skip : 0);
+    w.nrows = p.n * p.group;
+    w.rfirst = w.rb * rows;
+    return true;
+}
+
+// Whether the keys of a block need the mask: [k0, k0 + n).
+__device__ __forceinline__ int rows_masked(const RowsParams& p, const RowsWork& w, int k0, int n) {
+    return k0 + n > min(w.open, w.kend) || (k0 < w.low && k0 + n > p.sinks);
+}
+
+// Position of a token for windows, which drafted tokens do not stand before their sequence's filled rows for.
+__device__ __forceinline__ int window_position(const RowsParams& p, const RowsWork& w, int tok) {
+    if (!w.tree) return p.q_start + tok;
+    return min(p.pos ? max(p.pos[(int64_t)w.b * p.n + tok], w.len) : w.len + tok, kWindowMaxPos);
+}
+// Whether the window hides key `key` from a token that stands at `pos`.
+__device__ __forceinline__ bool window_hides(const RowsParams& p, const RowsWork& w, int pos, int key) {
+    if (key < p.sinks) return false;
+    if (!w.tree) return key <= pos - p.window || key >= pos + p.window;
+    const int bit = key - w.len;
+    return pos - (bit >= 0 ? window_position(p, w, min(bit, p.n - 1)) : key) >= p.window;
+}
+
+// Whether token `tok` sees key `key` < kend, as far as masks tell.
+__device__ __forceinline__ bool rows_see(const RowsParams& p, const RowsWork& w, int tok, int key) {
+    if (p.window && window_hides(p, w, window_position(p, w, tok), key)) return false;
+    if (!w.tree) {
+        if (p.causal && !(key <= p.q_start + tok || key < w.prefix)) return false;
+        if (!w.docs) return true;
+        const int id = p.q_doc[(int64_t)w.b * p.n + tok];
+        return id >= 0 && p.k_doc[(int64_t)w.b * p.sk + key] == id;
+    }
+    if (key < w.len) return true;
+    const int bit = key - w.len;
+    if (!p.mask) return bit <= tok;
+    const int64_t row = (p.mask_shared ? 0 : (int64_t)w.b * p.n) + tok;
+    return (p.mask[row * p.mask_words + (bit >> 6)] >> (bit & 63)) & 1;
+}
+
+// A row's token: its number, position, document, and first mask word.
+struct RowToken {
+    int token, pos, doc;
+    uint64_t word;
+};
+__device__ __forceinline__ RowToken row_token(const RowsParams& p, const RowsWork& w, int token) {
+    RowToken r;
+    r.token = token;
+    r.pos = !w.tree ? p.q_start + token : p.pos ? p.pos[w.b * p.n + token] : w.len + token;
+    r.doc = w.docs ? p.q_doc[(int64_t)w.b * p.n + token] : 0;
+    r.word = 0;
+    if (w.tree)
+        r.word = p.mask ? p.mask[((p.mask_shared ? 0 : (int64_t)w.b * p.n) + token) * p.mask_words]
+                        : token < 63 ? (2ull << token) - 1 : ~0ull;
+    return r;
+}
+__device__ __forceinline__ uint64_t bits_before(int n) { return n >= 64 ? ~0ull : (1ull << max(n, 0)) - 1; }
+
+// Bits of the keys from k0 that exist: before the run's end, in good pages (one lane a key).
+__device__ __forceinline__ uint64_t keys_there(const RowsParams& p, const RowsWork& w, int k0, int lane, int badpage) {
+    const int key = k0 + lane;
+    if (!badpage) return w.kend - k0 >= 64 ? ~0ull : (1ull << (w.kend - k0)) - 1;
+    const CachePages pages = rows_pages(p, w.b);
+    return __builtin_amdgcn_ballot_w64(key < w.kend && pages.at(key, w.kend, 0, 0) >= 0);
+}
+__device__ __forceinline__ uint64_t mask_word(const RowsParams& p, const RowsWork& w, const RowToken& r, int i) {
+    if (i == 0) return r.word;
+    if (i >= p.mask_words) return 0;
+    if (p.mask) return p.mask[((p.mask_shared ? 0 : (int64_t)w.b * p.n) + r.token) * p.mask_words + i];
+    return bits_before(r.token + 1 - 64 * i);   // a chain
+}
+// Bits of the keys that a row sees, as far as causal, prefix and tree tell.
+__device__ __forceinline__ uint64_t seen_bits(const RowsParams& p, const RowsWork& w, const RowToken& r, int k0) {
+    if (!w.tree)
+        return bits_before((w.docs && r.doc < 0 ? 0 : p.causal ? max(p.q_start + r.token + 1, w.prefix) : 0x7fffffff) - k0);
+    const int rel = k0 - w.len;   // the first key's number among the drafted ones
+    if (rel <= -64) return ~0ull;
+    if (rel < 0) return (mask_word(p, w, r, 0) << -rel) | ((1ull << -rel) - 1);
+    const int i = rel >> 6, sh = rel & 63;
+    const uint64_t lo = mask_word(p, w, r, i) >> sh;
+    return sh == 0 ? lo : lo | (mask_word(p, w, r, i + 1) << (64 - sh));
+}
+// Those of the N keys that the window leaves a row; drafted keys that stand where the program says: of the keys
+// at(b, r), b < N / 16, whose scores the lane holds.
+template <int N, typename At>
+__device__ __forceinline__ uint64_t window_bits(const RowsParams& p, const RowsWork& w, const RowToken& row, int k0, At at_) {
+    const int at = w.tree ? min(max(row.pos, w.len), kWindowMaxPos) : row.pos;
+    uint64_t bits = ~bits_before(at - p.window + 1 - k0);
+    if (!w.tree) bits &= bits_before(at + p.window - k0);
+    bits |= bits_before(p.sinks - k0);
+    if (w.tree && p.pos && k0 + N > w.len) {
+#pragma unroll 1
+        for (int b = 0; b < N / 16; ++b)
+#pragma unroll 1
+            for (int r = 0; r < 4; ++r) {
+                const int x = at_(b, r);
+                if (k0 + x < w.len) continue;
+                bits = window_hides(p, w, at, k0 + x) ? bits & ~(1ull << x) : bits | 1ull << x;
+            }
+    }
+    return bits;
+}
+
+#endif  // FA_ROWS_H

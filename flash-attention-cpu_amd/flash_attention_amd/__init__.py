@@ -75,6 +75,7 @@ EXPORTED_SYMBOLS = (
     "fa_score_forward", "fa_score_backward", "fa_rotary_init", "fa_rotary", "fa_cache_append", "fa_tree_attention",
     "fa_window_forward", "fa_window_backward", "fa_window_tree_attention",
     "fa_norm_rotary", "fa_norm_rotary_backward", "fa_norm_cache_append",
+    "fa_cache4_append", "fa_cache4_read", "fa_cache4_attention",
 )
 
 
@@ -421,7 +422,8 @@ def init() -> None:
 # Attention with modified scores, rotary positions, key / value cache (operators.py)
 ROTARY_NONE, ROTARY_LINEAR, ROTARY_NTK, ROTARY_YARN = 0, 1, 2, 3
 from .operators import (  # noqa: E402
-    AppendConfig, HeadNorm, KvCache, NormGrad, RotaryConfig, RotaryTensor, ScoreConfig, Strides, TreeConfig, Window,
-    append_config, cache_append_device, head_norm, kv_cache, norm_grad, norm_rotary_backward_device,
-    norm_rotary_device, rotary_config, rotary_device, rotary_tensor, score_attention_backward_device,
-    score_attention_device, score_config, tree_attention_device, tree_config, window)
+    AppendConfig, HeadNorm, KvCache, KvCache4, NormGrad, ReadConfig, RotaryConfig, RotaryTensor, ScoreConfig, Strides,
+    TreeConfig, Window, append_config, cache4_append_device, cache4_attention_device, cache4_read_device, cache4_shapes,
+    cache_append_device, head_norm, kv_cache, kv_cache4, norm_grad, norm_rotary_backward_device, norm_rotary_device,
+    read_config, rotary_config, rotary_device, rotary_tensor, score_attention_backward_device, score_attention_device,
+    score_config, tree_attention_device, tree_config, window)

@@ -1,7 +1,7 @@
 """Attention with modified scores, rotary positions and the key / value cache.
 
-Python view of the fa_score_*, fa_window_*, fa_rotary*, fa_norm_*, fa_cache_append and
-fa_tree_attention entry points of include/fa_hip.h, which defines what they
+Python view of the fa_score_*, fa_window_*, fa_rotary*, fa_norm_*, fa_cache_append,
+fa_tree_attention and fa_cache4_* entry points of include/fa_hip.h, which defines what they
 compute.  They have no counterpart in the reference crate.
 
 Calls take raw device pointers and a HIP stream, as attention_device does,
@@ -75,6 +75,20 @@ class KvCache(ctypes.Structure):
                 ("page_size", _SZ), ("n_pages", _SZ), ("pages_per_seq", _SZ)]
 
 
+class KvCache4(ctypes.Structure):
+    """fa_kv_cache4."""
+
+    _fields_ = [("dtype", _I), ("batch", _SZ), ("kv_heads", _SZ), ("d_head", _SZ), ("k", _P), ("k_scale", _P), ("v", _P),
+                ("v_scale", _P), ("lens", _P), ("capacity", _SZ), ("block_table", _P), ("page_size", _SZ),
+                ("n_pages", _SZ), ("pages_per_seq", _SZ)]
+
+
+class ReadConfig(ctypes.Structure):
+    """fa_read_config."""
+
+    _fields_ = [("n_rows", _SZ), ("k", Strides), ("v", Strides)]
+
+
 class AppendConfig(ctypes.Structure):
     """fa_append_config."""
 
@@ -105,28 +119,44 @@ def declare(lib: ctypes.CDLL) -> None:
         "fa_norm_cache_append": [_P, ptr(KvCache), ptr(AppendConfig), ptr(HeadNorm), _P, _P, _P, _P, _P],
         "fa_cache_append": [_P, ptr(KvCache), ptr(AppendConfig), _P, _P, _P, _P, _P],
         "fa_tree_attention": [_P, ptr(TreeConfig), ptr(KvCache), _P, _P, _P],
+        "fa_cache4_append": [_P, ptr(KvCache4), ptr(AppendConfig), _P, _P],
+        "fa_cache4_read": [_P, ptr(KvCache4), ptr(ReadConfig), _P, _P, _P],
+        "fa_cache4_attention": [_P, ptr(TreeConfig), ptr(Window), ptr(KvCache4), _P, _P, _P],
         "fa_window_forward": [_P, ptr(ScoreConfig), ptr(Window), _P, _P, _P, _P, _P],
         "fa_window_backward": [_P, ptr(ScoreConfig), ptr(Window)] + [_P] * 9,
         "fa_window_tree_attention": [_P, ptr(TreeConfig), ptr(Window), ptr(KvCache), _P, _P, _P],
     }.items():
-        f = getattr(lib, name, None)   # None: a library built before there were operators
+        f = getattr(lib, name, None)   # None: a library built before there was this operator
         if f is not None:
             f.argtypes = args
             f.restype = _I
 
 
+class _Entries:
+    """The library's entry points; those that it lacks are reported as calls of them fail."""
+
+    def __init__(self, loaded):
+        self._loaded = loaded
+
+    def __getattr__(self, name):
+        f = getattr(self._loaded, name, None)
+        if f is None:
+            from . import FA_ERR_MODULE, LIB_PATH, FaError
+            raise FaError(FA_ERR_MODULE, f"{LIB_PATH} has no operators of the name {name}; build it anew with "
+                                         "flash-attention-cpu_amd/build.py")
+        setattr(self, name, f)
+        return f
+
+
 def _lib():
     global _lib
     from . import lib
-    loaded = lib()
-    if not hasattr(loaded, "fa_score_forward"):
-        from . import FA_ERR_MODULE, LIB_PATH, FaError
-        raise FaError(FA_ERR_MODULE, f"{LIB_PATH} has no operators; build it anew with flash-attention-cpu_amd/build.py")
+    entries = _Entries(lib())
 
     def known():
-        return loaded
+        return entries
     _lib = known
-    return loaded
+    return entries
 
 
 def _check(status: int) -> None:
@@ -283,3 +313,40 @@ def tree_attention_device(cfg: TreeConfig, cache: KvCache, q_ptr: int, out_ptr: 
         _check(_lib().fa_tree_attention(stream, cfg, cache, q_ptr, out_ptr, lse_ptr))
     else:
         _check(_lib().fa_window_tree_attention(stream, cfg, window, cache, q_ptr, out_ptr, lse_ptr))
+
+
+def kv_cache4(dtype: int, batch: int, kv_heads: int, d_head: int, k_ptr: int, k_scale_ptr: int, v_ptr: int,
+              v_scale_ptr: int, lens_ptr: int, capacity: int = 0, block_table_ptr: int = 0, page_size: int = 0,
+              n_pages: int = 0, pages_per_seq: int = 0) -> KvCache4:
+    """A cache in 4 bits, of capacity rows a sequence or (block_table_ptr) in pages; buffers: cache4_shapes."""
+    return KvCache4(int(dtype), batch, kv_heads, d_head, _ptr(k_ptr), _ptr(k_scale_ptr), _ptr(v_ptr), _ptr(v_scale_ptr),
+                    _ptr(lens_ptr), capacity, _ptr(block_table_ptr), page_size, n_pages, pages_per_seq)
+
+
+def cache4_shapes(blocks: int, kv_heads: int, rows: int, d_head: int) -> dict:
+    """Shapes of its buffers: k and v of 32-bit words, k_scale and v_scale of f16; blocks: sequences, or pages of `rows`
+    rows."""
+    return {"k": (blocks, kv_heads, rows, d_head // 8), "k_scale": (blocks, kv_heads, rows, d_head // 32, 2),
+            "v": (blocks, kv_heads, rows // 8, d_head), "v_scale": (blocks, kv_heads, rows // 8, d_head // 32, 2, 8)}
+
+
+def cache4_append_device(cache: KvCache4, cfg: AppendConfig, k_ptr: int, v_ptr: int, stream: int = 0) -> None:
+    """Queue the append of keys and values behind each sequence's rows, in 4 bits (fa_cache4_append)."""
+    _check(_lib().fa_cache4_append(stream, cache, cfg, k_ptr, v_ptr))
+
+
+def read_config(n_rows: int, k_strides=None, v_strides=None) -> ReadConfig:
+    """Rows read back a sequence, and the layouts that they get."""
+    return ReadConfig(n_rows, _strides(k_strides), _strides(v_strides))
+
+
+def cache4_read_device(cache: KvCache4, cfg: ReadConfig, rows_ptr: int, k_out_ptr: int, v_out_ptr: int,
+                       stream: int = 0) -> None:
+    """Queue rows of a cache in 4 bits, as its 16-bit type (fa_cache4_read); 0: keys or values not wanted."""
+    _check(_lib().fa_cache4_read(stream, cache, cfg, rows_ptr, k_out_ptr, v_out_ptr))
+
+
+def cache4_attention_device(cfg: TreeConfig, cache: KvCache4, q_ptr: int, out_ptr: int, lse_ptr: int = 0,
+                            stream: int = 0, window: Window | None = None) -> None:
+    """Queue attention of drafted tokens over a cache in 4 bits (fa_cache4_attention)."""
+    _check(_lib().fa_cache4_attention(stream, cfg, window, cache, q_ptr, out_ptr, lse_ptr))

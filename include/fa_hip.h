@@ -468,6 +468,55 @@ int fa_tree_attention(void* stream, const fa_tree_config* cfg, const fa_kv_cache
 int fa_window_tree_attention(void* stream, const fa_tree_config* cfg, const fa_window* window,
                              const fa_kv_cache* cache, const void* q, void* out, float* lse);
 
+/* ---- key / value cache in 4 bits --------------------------------------------
+ * No counterpart in the reference.  A cache that keeps each row of a head in
+ * groups of 32 columns: 4 bits a column, and an f16 pair (S, O) a group; code
+ * c stands for O + (1 + c / 16) S.  Of a group's values, the smallest lo, the
+ * largest hi, with f32 operations:
+ *     S = f16((hi - lo) * 16 / 15),  O = f16(lo - S),
+ *     c = round((x - O) / (S / 16) - 16), halves to even, within 0 .. 15  (0 where S = 0)
+ * so a value is kept within half a step S / 16 and the rounding of O.  Sizes
+ * above 60000 count as that, S ends at 65504 and O at -65504 (a group between -20000 and 20000 meets
+ * neither); a group with an infinity or NaN reads back as NaN.  16-bit types,
+ * d_head a multiple of 32 (FA_ERR_UNSUPPORTED otherwise).
+ *
+ * Sequences, pages, lens and what is seen are as in fa_kv_cache; pages hold 8
+ * rows or more, and capacity is a multiple of 8 (FA_ERR_INVALID_ARG).  Buffers are the program's, 16-byte
+ * aligned, contiguous, and filled by fa_cache4_append:
+ *     k        [pages or batch, kv_heads, rows, d_head / 8] words, 8 columns each
+ *     k_scale  [pages or batch, kv_heads, rows, d_head / 32, 2] f16: S, O
+ *     v        [pages or batch, kv_heads, rows / 8, d_head] words, 8 rows each
+ *     v_scale  [pages or batch, kv_heads, rows / 8, d_head / 32, 2, 8] f16: S of 8 rows, O of 8 rows
+ * (rows: of a page, or the capacity).  Entry e of a word stands at bits 4 (e / 2) + 16 (e % 2). */
+typedef struct fa_kv_cache4 {
+    int dtype;                         /* of queries, outputs and rows: FA_DTYPE_BF16 or FA_DTYPE_F16 */
+    size_t batch, kv_heads, d_head;
+    uint32_t* k;
+    uint16_t* k_scale;
+    uint32_t* v;
+    uint16_t* v_scale;
+    const int32_t* lens;               /* [batch] */
+    size_t capacity;                   /* rows a sequence, without pages */
+    const int32_t* block_table;        /* [batch, pages_per_seq] or NULL */
+    size_t page_size, n_pages, pages_per_seq;
+} fa_kv_cache4;
+/* fa_cache_append for such a cache; rows come as they are to be kept (a
+ * config with rotary or q_layout is refused). */
+int fa_cache4_append(void* stream, const fa_kv_cache4* cache, const fa_append_config* cfg, const void* k,
+                     const void* v);
+/* Rows of the cache in its dtype: rows[b][i] of sequence b, i < n_rows (int32,
+ * device memory; any order, also past lens[b]; zeros where there is no such row).  k_out or v_out may be NULL. */
+typedef struct fa_read_config {
+    size_t n_rows;
+    fa_strides k, v;                   /* of k_out and v_out, [batch, kv_heads, n_rows, d_head] by default */
+} fa_read_config;
+int fa_cache4_read(void* stream, const fa_kv_cache4* cache, const fa_read_config* cfg, const int32_t* rows, void* k_out,
+                   void* v_out);
+/* fa_tree_attention over such a cache, in a sliding window if window != NULL.
+ * Values enter the products as f16 (rounded once), and so do probabilities and, by powers of two a row, queries. */
+int fa_cache4_attention(void* stream, const fa_tree_config* cfg, const fa_window* window, const fa_kv_cache4* cache,
+                        const void* q, void* out, float* lse);
+
 /* ---- naive attention (materialised scores) -------------------------------
  * naive_attention -- src/naive.rs:14-75: the textbook O(seq_q * seq_k)
  * memory form (scores, row softmax, PV) that the crate keeps as its
