@@ -4,7 +4,8 @@ Outputs, next to this file (git-ignored, used in place):
   fa_kernels.hsaco  gfx950 code object with the attention kernels (hipcc --genco)
   fa_score_*.hsaco, fa_cache_*.hsaco (f32, bf16, f16), fa_cache4_*.hsaco (bf16, f16), fa_rotary.hsaco, fa_norm.hsaco
                     code objects of attention with modified scores, of the
-                    key / value cache, of one held in 4 bits, of rotary positions and of norms with them
+                    key / value cache, of one held in 4 bits, of rotary positions and of norms with them;
+                    fa_score_w_*, fa_cache_w_*, fa_cache4_w_*: those of calls in a sliding window
   libfa_hip.so      C ABI of include/fa_hip.h over the HIP runtime
 
 All are written aside and moved into place together once every one of them has
@@ -33,8 +34,9 @@ ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 TYPES = {"f32": ("-DOPS_T=float", "-DOPS_NAME=f32"), "bf16": ("-DOPS_T=__bf16", "-DOPS_NAME=bf16", "-DOPS_16BIT"),
          "f16": ("-DOPS_T=_Float16", "-DOPS_NAME=f16", "-DOPS_16BIT")}
 OBJECTS = {"fa_kernels": ("fa_kernels", ()), "fa_rotary": ("fa_rotary", ()), "fa_norm": ("fa_norm", ()),
-           **{f"{src}_{t}": (src, flags) for src in ("fa_score", "fa_cache") for t, flags in TYPES.items()},
-           **{f"fa_cache4_{t}": ("fa_cache4", TYPES[t]) for t in ("bf16", "f16")}}
+           **{f"{src}{tag}_{t}": (src, flags + window) for src in ("fa_score", "fa_cache", "fa_cache4")
+              for tag, window in (("", ()), ("_w", ("-DOPS_WINDOW",))) for t, flags in TYPES.items()
+              if src != "fa_cache4" or t != "f32"}}
 LIB = os.path.join(HERE, "libfa_hip.so")
 BUILD = os.path.join(HERE, "_build")   # intermediate objects, and outputs until all are there (git-ignored)
 

@@ -290,7 +290,7 @@ struct RowTiles {
             uint64_t see[MT];
 #pragma unroll
             for (int t = 0; t < MT; ++t) see[t] = there & seen_bits(lp, w, {token[t], pos[t], qd[t], word[t]}, k0);
-            if (lp.window) {
+            if constexpr (kWindow) {
 #pragma unroll
                 for (int t = 0; t < MT; ++t)
                     see[t] &= window_bits<16 * KB>(lp, w, {token[t], pos[t], qd[t], word[t]}, k0,
@@ -387,7 +387,7 @@ struct RowTiles {
         const CachePages pages = rows_pages(p, w.b);
         const int mine = min(16 * MT, w.nrows - rfirst);
         auto row_at = [&](int key) -> const T* {
-            if (key >= w.gap && key - w.gap < w.skip) return nullptr;
+            if (kWindow && key >= w.gap && key - w.gap < w.skip) return nullptr;
             const int64_t at = pages.at(key, w.kend, p.vs.s, p.vs.b);
             return at < 0 ? nullptr : V + at;
         };
@@ -744,11 +744,18 @@ __device__ __forceinline__ void rows_merge(const RowsParams& p) {
         BODY<OPS_T, D, MT, MOD, VEC>(p);                                                                       \
     }
 // plain scores, capped (c), with a bias (b) or both (cb); any alignment and page size (s)
+// windows: plain scores, or looked up (m)
+#ifdef OPS_WINDOW
+#define KINDS(F, BODY, D, MT, THREADS, WAVES)                            \
+    KERNEL(F, BODY, D, MT, 0, true, , THREADS, WAVES)                    \
+    KERNEL(F, BODY, D, MT, kAny, true, m, THREADS, WAVES)
+#else
 #define KINDS(F, BODY, D, MT, THREADS, WAVES)                            \
     KERNEL(F, BODY, D, MT, 0, true, , THREADS, WAVES)                    \
     KERNEL(F, BODY, D, MT, kCap, true, c, THREADS, WAVES)                \
     KERNEL(F, BODY, D, MT, kBias, true, b, THREADS, WAVES)               \
     KERNEL(F, BODY, D, MT, kCap | kBias, true, cb, THREADS, WAVES)
+#endif
 #define STREAM(D, MT, WAVES) KINDS(fa_rows_stream_, rows_stream, D, MT, (64 * kStreamWaves<D * (int)sizeof(OPS_T)>), WAVES)
 #define SHARED(D, MT, WAVES) KINDS(fa_rows_shared_, rows_shared, D, MT, 512, WAVES)
 #define MERGE(D, VEC, WIDE, TAG)                                                                                  \

@@ -487,7 +487,7 @@ __device__ __forceinline__ void rows4(const RowsParams& p) {
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
                 uint64_t see = there & seen_bits(lp, w, tok[t], k0);
-                if (lp.window) see &= window_bits<SK>(lp, w, tok[t], k0, [&](int b, int r) { return 8 * g + 4 * b + r; });
+                if constexpr (kWindow) see &= window_bits<SK>(lp, w, tok[t], k0, [&](int b, int r) { return 8 * g + 4 * b + r; });
                 const unsigned bits = (unsigned)(see >> (8 * g));
 #pragma unroll
                 for (int b = 0; b < 2; ++b)
@@ -657,7 +657,7 @@ __device__ __forceinline__ void rows4(const RowsParams& p) {
     const int mine = min(16 * MT, w.nrows - w.rfirst);
 #pragma unroll 1
     for (int key = w.kbeg; key < w.kend; ++key) {
-        if (key >= w.gap && key - w.gap < w.skip) continue;
+        if (kWindow && key >= w.gap && key - w.gap < w.skip) continue;
         const int page = pages.page(key);
         if (page < 0) continue;
         const int64_t at = ((int64_t)(lp.table ? page : w.b) * lp.kv_heads + w.hk) * page_rows + (lp.table ? key & pages.page_mask : key);
@@ -709,9 +709,11 @@ KERNEL(3, 1, kAny, true, p, 2)
 KERNEL(5, 1, kAny, true, p, 2)
 KERNEL(6, 1, kAny, true, p, 2)
 KERNEL(7, 1, kAny, true, p, 2)
+#ifndef OPS_WINDOW
 extern "C" __global__ __launch_bounds__(256) void PASTE(fa_cache4_append_, OPS_NAME, , )(Cache4Params p) {
     cache4_append<OPS_T>(p);
 }
 extern "C" __global__ __launch_bounds__(256) void PASTE(fa_cache4_read_, OPS_NAME, , )(Cache4Params p) {
     cache4_read<OPS_T>(p);
 }
+#endif

@@ -32,6 +32,14 @@ constexpr float kLn2 = 0.693147180559945309f;
 // maximum of a row by this much (log2 units) before the sums are rescaled.
 constexpr float kLazy = 8.0f;
 
+// Kernels of calls with a sliding window are code objects of their own (the same sources built with OPS_WINDOW): what
+// they need besides would take scalar registers from the others.
+#ifdef OPS_WINDOW
+constexpr bool kWindow = true;
+#else
+constexpr bool kWindow = false;
+#endif
+
 // What happens to scores, fixed for a kernel: bits kCap and kBias, or kAny: looked up in the parameters.
 constexpr int kCap = 1, kBias = 2, kAny = 4;
 template <int MOD, typename P>

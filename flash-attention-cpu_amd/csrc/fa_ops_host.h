@@ -10,10 +10,19 @@
 
 namespace {
 
-// Code objects: those of score attention and of the cache one a type (FA_DTYPE_*).
-enum OpsModule { kRotaryModule, kScoreModule, kCacheModule = kScoreModule + 3, kNormModule = kCacheModule + 3,
-                 kCache4Module,   // bf16, f16
-                 kOpsModules = kCache4Module + 2 };
+// Code objects: those of score attention and of the cache one a type (FA_DTYPE_*), those of a cache in 4 bits for bf16
+// and f16; calls in a window have their own.
+enum OpsModule {
+    kRotaryModule,
+    kNormModule,
+    kScoreModule,
+    kCacheModule = kScoreModule + 3,
+    kCache4Module = kCacheModule + 3,
+    kScoreWindowModule = kCache4Module + 2,
+    kCacheWindowModule = kScoreWindowModule + 3,
+    kCache4WindowModule = kCacheWindowModule + 3,
+    kOpsModules = kCache4WindowModule + 2
+};
 OpsModule of_type(OpsModule m, int dtype) { return static_cast<OpsModule>(m + dtype); }
 
 struct OpsState {
@@ -39,10 +48,12 @@ constexpr size_t kOpsMaxGrid = size_t(1) << 23;   // workgroups: threads of a la
 constexpr size_t kOpsMaxTokens = size_t(1) << 31;   // of a rotary launch: a thread for each at least
 
 int ops_module(int dev, OpsModule which) {
-    static const char* const files[] = {"fa_rotary.hsaco",     "fa_score_f32.hsaco",  "fa_score_bf16.hsaco",
-                                        "fa_score_f16.hsaco",  "fa_cache_f32.hsaco",  "fa_cache_bf16.hsaco",
-                                        "fa_cache_f16.hsaco",  "fa_norm.hsaco",      "fa_cache4_bf16.hsaco",
-                                        "fa_cache4_f16.hsaco"};
+    static const char* const files[kOpsModules] = {
+        "fa_rotary.hsaco",       "fa_norm.hsaco",          "fa_score_f32.hsaco",    "fa_score_bf16.hsaco",
+        "fa_score_f16.hsaco",    "fa_cache_f32.hsaco",     "fa_cache_bf16.hsaco",   "fa_cache_f16.hsaco",
+        "fa_cache4_bf16.hsaco",  "fa_cache4_f16.hsaco",    "fa_score_w_f32.hsaco",  "fa_score_w_bf16.hsaco",
+        "fa_score_w_f16.hsaco",  "fa_cache_w_f32.hsaco",   "fa_cache_w_bf16.hsaco", "fa_cache_w_f16.hsaco",
+        "fa_cache4_w_bf16.hsaco", "fa_cache4_w_f16.hsaco"};
     OpsState& s = g_ops[dev];
     std::call_once(s.once[which], [&] {
         std::string path = module_path();
@@ -201,7 +212,8 @@ int resolve_scale(float scale, float softcap, size_t d, ScoreScale* out) {
 bool cap_ok(int dtype, float softcap) { return dtype == FA_DTYPE_F32 || softcap <= kFastCap; }
 
 // Tag of the kernel for what happens to the scores.
-const char* score_tag(const fa_score_config& c, bool vec) {
+const char* score_tag(const fa_score_config& c, bool vec, bool window) {
+    if (window) return !vec ? "s" : c.softcap > 0.0f || c.slopes ? "m" : "";
     return !vec ? "s" : c.softcap > 0.0f ? (c.slopes ? "cb" : "c") : c.slopes ? "b" : "";
 }
 
@@ -243,6 +255,45 @@ DkvPlan plan_dkv(const fa_score_config& c, int D, bool vec, int num_cus) {
     r.blocks = (c.seq_len_k + r.tiles.rows - 1) / r.tiles.rows;
     r.splits = static_cast<int>(s);
     r.floats = s > 1 ? 2 * s * nkv * c.seq_len_k * D : 0;
+    return r;
+}
+
+// A window's size and sinks as kernels take them (size 0: hides nothing); farthest: the largest distance there is.
+int resolve_window(const fa_window* w, bool docs, int64_t farthest, int* size, int* sinks) {
+    *size = *sinks = 0;
+    if (!w) return FA_OK;
+    if (w->size < 1 || w->sinks < 0) return FA_ERR_INVALID_ARG;
+    if (w->sinks > 0 && docs) return FA_ERR_UNSUPPORTED;   // the first keys are another document's
+    if (w->size > farthest) return FA_OK;
+    if (farthest > kWindowMaxPos) return FA_ERR_UNSUPPORTED;   // positions plus or minus a window stay in 32 bits
+    *size = static_cast<int>(w->size);
+    *sinks = static_cast<int>(std::min<int64_t>(w->sinks, kWindowMaxPos));
+    return FA_OK;
+}
+// The most keys that n consecutive queries of a window walk.
+size_t window_keys(size_t keys, int size, int sinks, size_t n, bool both_sides) {
+    if (size == 0) return keys;
+    return std::min(keys, (both_sides ? 2 : 1) * static_cast<size_t>(size) + sinks + n + 128);
+}
+
+// In a window: key blocks that hold sinks, and the chunks in which other workgroups take the queries that see them from
+// afar; as long as what the other key blocks have, so that none ends late (sinks or not: 2 x 16 / 4 heads x 4096^2,
+// 128 columns, window 512, bf16).
+struct FarPlan {
+    int stages, chunks, blocks;
+    size_t floats;
+};
+FarPlan plan_far(const fa_score_config& c, int D, const DkvPlan& dkv, int size, int sinks) {
+    FarPlan r{};
+    if (size == 0 || sinks == 0 || c.seq_len_k == 0) return r;
+    const size_t step = dkv.tiles.groups == 1 && (c.dtype == FA_DTYPE_F32 || D > 128) ? 32 : 64;   // queries of a stage
+    const size_t nst = (c.seq_len_q + step - 1) / step;
+    r.blocks = static_cast<int>((std::min<size_t>(sinks, c.seq_len_k) + dkv.tiles.rows - 1) / dkv.tiles.rows);
+    const size_t reach = window_keys(c.seq_len_q, size, 0, dkv.tiles.rows, !c.causal || c.prefix) / step + 1;
+    // (a workspace of 2^15 such chunks at most, of the workgroups of ever longer rows)
+    r.stages = static_cast<int>(std::max({reach, size_t(4), nst / 1024 + 1}));
+    r.chunks = static_cast<int>((nst + r.stages - 1) / r.stages);
+    r.floats = size_t(2) * (r.chunks + 1) * dkv.splits * c.batch * c.kv_heads * r.blocks * dkv.tiles.rows * D;
     return r;
 }
 
@@ -309,6 +360,8 @@ RowsPlan plan_rows(int dtype, int D, bool vec, size_t batch, size_t kv_heads, si
     return r;
 }
 
+OpsModule cache_module(int dtype, const RowsParams& p) { return of_type(p.window ? kCacheWindowModule : kCacheModule, dtype); }
+
 // Launches a rows kernel, and the one that joins its partial sums (of D columns).
 int launch_rows(int dev, hipStream_t stream, int dtype, OpsModule module, const char* kernel, const RowsPlan& plan, int D,
                 bool vec, RowsParams* p) {
@@ -335,40 +388,23 @@ int launch_rows(int dev, hipStream_t stream, int dtype, OpsModule module, const 
         char name[64];
         std::snprintf(name, sizeof(name), "fa_rows_merge_%s_d%d%s", dtype_name(dtype), D, !vec ? "s" : wide ? "w" : "");
         const size_t per = wide ? 1 : 1024 / D;
-        rc = ops_launch(dev, of_type(kCacheModule, dtype), name, (mgrid + per - 1) / per, 256, p, stream);
+        rc = ops_launch(dev, cache_module(dtype, *p), name, (mgrid + per - 1) / per, 256, p, stream);
     }
     return ws.done(stream, rc);
 }
 
 int run_rows(int dev, hipStream_t stream, int dtype, int D, bool vec, RowsParams* p, size_t keys) {
     vec = vec && (!p->table || p->page_shift >= 4);   // DMA moves runs of rows of one page
-    const OpsModule module = of_type(kCacheModule, dtype);
+    const OpsModule module = cache_module(dtype, *p);
     const int rc = ops_module(dev, module);
     if (rc != FA_OK) return rc;
     const RowsPlan plan =
         plan_rows(dtype, D, vec, p->batch, p->kv_heads, static_cast<size_t>(p->n) * p->group, keys, g_dev[dev].num_cus);
     char name[64];
     std::snprintf(name, sizeof(name), "fa_rows_%s_%s_d%d_t%d%s", plan.stream ? "stream" : "shared", dtype_name(dtype), D,
-                  plan.mt, !vec ? "s" : p->cap_log2e != 0.0f ? (p->slopes ? "cb" : "c") : p->slopes ? "b" : "");
+                  plan.mt, !vec ? "s" : p->window ? (p->cap_log2e != 0.0f || p->slopes ? "m" : "")
+                                  : p->cap_log2e != 0.0f ? (p->slopes ? "cb" : "c") : p->slopes ? "b" : "");
     return launch_rows(dev, stream, dtype, module, name, plan, D, vec, p);
-}
-
-// A window's size and sinks as kernels take them (size 0: hides nothing); farthest: the largest distance there is.
-int resolve_window(const fa_window* w, bool docs, int64_t farthest, int* size, int* sinks) {
-    *size = *sinks = 0;
-    if (!w) return FA_OK;
-    if (w->size < 1 || w->sinks < 0) return FA_ERR_INVALID_ARG;
-    if (w->sinks > 0 && docs) return FA_ERR_UNSUPPORTED;   // the first keys are another document's
-    if (w->size > farthest) return FA_OK;
-    if (farthest > kWindowMaxPos) return FA_ERR_UNSUPPORTED;   // positions plus or minus a window stay in 32 bits
-    *size = static_cast<int>(w->size);
-    *sinks = static_cast<int>(std::min<int64_t>(w->sinks, kWindowMaxPos));
-    return FA_OK;
-}
-// The most keys that n consecutive queries of a window walk.
-size_t window_keys(size_t keys, int size, int sinks, size_t n, bool both_sides) {
-    if (size == 0) return keys;
-    return std::min(keys, (both_sides ? 2 : 1) * static_cast<size_t>(size) + sinks + n + 128);
 }
 
 // Short query blocks, and few workgroups over many keys, run on the rows kernel, which splits the keys.
@@ -547,7 +583,8 @@ int score_forward(void* stream_, const fa_score_config* c, const fa_window* wind
     if (c->batch * c->heads > kOpsMaxGrid || (c->seq_len_q + 31) / 32 * c->batch * c->heads > kOpsMaxGrid)
         return FA_ERR_UNSUPPORTED;
     int dev;
-    if ((rc = ops_begin(&dev, of_type(kScoreModule, c->dtype))) != FA_OK) return rc;
+    const OpsModule module = of_type(size ? kScoreWindowModule : kScoreModule, c->dtype);
+    if ((rc = ops_begin(&dev, module)) != FA_OK) return rc;
     const hipStream_t stream = static_cast<hipStream_t>(stream_);
     const bool vec = vec_ok(q, lq, d) && vec_ok(k, lk, d) && vec_ok(v, lv, d) && ovec_ok(out, lo, es) &&
                      cap_ok(c->dtype, c->softcap);
@@ -577,13 +614,13 @@ int score_forward(void* stream_, const fa_score_config* c, const fa_window* wind
     if (c->q_doc) {
         const DocPlan docs = plan_docs(*c, tiles.rows, c->heads, 0, 0, g_dev[dev].num_cus);
         if ((rc = ws.get(dev, stream, docs.bytes)) != FA_OK) return rc;
-        rc = launch_docs(dev, of_type(kScoreModule, c->dtype), stream, docs, tiles.rows, 0, &p, static_cast<int32_t*>(ws.ptr));
+        rc = launch_docs(dev, module, stream, docs, tiles.rows, 0, &p, static_cast<int32_t*>(ws.ptr));
     }
     if (rc == FA_OK) {
         char name[64];
         std::snprintf(name, sizeof(name), "fa_score_forward_%s_d%d_t%d%s%s", dtype_name(c->dtype), D, tiles.mt,
-                      tiles.tag, score_tag(*c, vec));
-        rc = ops_launch(dev, of_type(kScoreModule, c->dtype), name, c->batch * c->heads * p.nqb, 256, &p, stream);
+                      tiles.tag, score_tag(*c, vec, size > 0));
+        rc = ops_launch(dev, module, name, c->batch * c->heads * p.nqb, 256, &p, stream);
     }
     return ws.done(stream, rc);
 }
@@ -617,7 +654,8 @@ int score_backward(void* stream_, const fa_score_config* c, const fa_window* win
         (sk + 31) / 32 * c->batch * c->heads > kOpsMaxGrid)
         return FA_ERR_UNSUPPORTED;
     int dev;
-    if ((rc = ops_begin(&dev, of_type(kScoreModule, c->dtype))) != FA_OK) return rc;
+    const OpsModule module = of_type(size ? kScoreWindowModule : kScoreModule, c->dtype);
+    if ((rc = ops_begin(&dev, module)) != FA_OK) return rc;
     const hipStream_t stream = static_cast<hipStream_t>(stream_);
     ScoreParams p{};
     fill_score(*c, sc, &p);
@@ -635,33 +673,38 @@ int score_backward(void* stream_, const fa_score_config* c, const fa_window* win
     if (D == 128 && tiles.mt == 2) tiles = {1, 1, 64, ""};   // two tiles' Q, dO and sums leave one wave a SIMD
     const DocPlan docs = plan_docs(*c, tiles.rows, c->heads, dkv.tiles.rows, c->kv_heads * dkv.splits, g_dev[dev].num_cus);
     // partial sums first: they are read and written 16 bytes at a time
+    const FarPlan far = dk || dv ? plan_far(*c, D, dkv, size, sinks) : FarPlan{};
     const size_t floats = dk || dv ? dkv.floats : 0;
-    if ((rc = ws.get(dev, stream, (floats + 2 * rows) * sizeof(float) + docs.bytes + 16)) != FA_OK) return rc;
+    if ((rc = ws.get(dev, stream, (floats + far.floats + 2 * rows) * sizeof(float) + docs.bytes + 16)) != FA_OK) return rc;
     p.part = static_cast<float*>(ws.ptr);
-    p.lse2 = p.part + floats;
+    p.far_part = p.part + floats;
+    p.lse2 = p.far_part + far.floats;
     p.delta = p.lse2 + rows;
     char name[64];
     if (c->q_doc)
-        rc = launch_docs(dev, of_type(kScoreModule, c->dtype), stream, docs, tiles.rows, dkv.tiles.rows, &p,
+        rc = launch_docs(dev, module, stream, docs, tiles.rows, dkv.tiles.rows, &p,
                          reinterpret_cast<int32_t*>(p.delta + rows));
-    const char* mod = score_tag(*c, vec);
+    const char* mod = score_tag(*c, vec, size > 0);
     // the dQ kernel also forms delta and lse2, and with 16-bit types corrects delta, for the other one
     if (rc == FA_OK && sq > 0) {
         p.nqb = static_cast<int>((sq + tiles.rows - 1) / tiles.rows);
         std::snprintf(name, sizeof(name), "fa_score_dq_%s_d%d_t%d%s%s", dtype_name(c->dtype), D, tiles.mt, tiles.tag, mod);
-        rc = ops_launch(dev, of_type(kScoreModule, c->dtype), name, c->batch * c->heads * p.nqb, 256, &p, stream);
+        rc = ops_launch(dev, module, name, c->batch * c->heads * p.nqb, 256, &p, stream);
     }
     if (rc == FA_OK && (dk || dv)) {
         p.nqb = static_cast<int>(dkv.blocks);
         p.splits = dkv.splits;
         std::snprintf(name, sizeof(name), "fa_score_dkv_%s_d%d_t%d%s%s", dtype_name(c->dtype), D, dkv.tiles.mt,
                       dkv.tiles.tag, mod);
-        rc = ops_launch(dev, of_type(kScoreModule, c->dtype), name, dkv.blocks * c->batch * c->kv_heads * dkv.splits, 256, &p,
-                        stream);
-        if (rc == FA_OK && dkv.splits > 1) {
+        const size_t slices = c->batch * c->kv_heads, grid = dkv.blocks * slices * dkv.splits;
+        p.far_first = static_cast<int>(grid);
+        p.far_stages = far.stages, p.far_chunks = far.chunks, p.far_blocks = far.blocks;
+        p.far_rows = far.blocks * dkv.tiles.rows;
+        rc = ops_launch(dev, module, name, grid + slices * dkv.splits * far.blocks * far.chunks, 256, &p, stream);
+        if (rc == FA_OK && (dkv.splits > 1 || far.blocks)) {
             std::snprintf(name, sizeof(name), "fa_score_dkv_sum_%s_d%d%s", dtype_name(c->dtype), D, vec ? "" : "s");
-            const size_t threads = c->batch * c->kv_heads * sk * (D / 4);
-            rc = ops_launch(dev, of_type(kScoreModule, c->dtype), name, (threads + 255) / 256, 256, &p, stream);
+            const size_t threads = slices * (dkv.splits > 1 ? sk : std::min<size_t>(sk, p.far_rows)) * (D / 4);
+            rc = ops_launch(dev, module, name, (threads + 255) / 256, 256, &p, stream);
         }
     }
     return ws.done(stream, rc);
@@ -703,7 +746,7 @@ int tree_attention(void* stream, const fa_tree_config* c, const fa_window* windo
                      cap_ok(cache->dtype, c->softcap);
     p.scale_log2e = sc.scale_log2e, p.cap_in = sc.cap_in, p.cap_log2e = sc.cap_log2e;
     int dev;
-    if ((rc = ops_begin(&dev, of_type(kCacheModule, cache->dtype))) != FA_OK) return rc;
+    if ((rc = ops_begin(&dev, cache_module(cache->dtype, p))) != FA_OK) return rc;
     return run_rows(dev, static_cast<hipStream_t>(stream), cache->dtype, ops_pad_d(d), vec, &p,
                     window_keys(capacity, size, sinks, n, false));
 }
@@ -821,7 +864,9 @@ void fill_cache4(const fa_kv_cache4& c, size_t block_rows, size_t capacity, Cach
     p->page_shift = page_shift4(c);
     p->n_pages = static_cast<int>(c.n_pages), p->pages_per_seq = static_cast<int>(c.pages_per_seq);
 }
-OpsModule cache4_module(int dtype) { return static_cast<OpsModule>(kCache4Module + (dtype == FA_DTYPE_BF16 ? 0 : 1)); }
+OpsModule cache4_module(int dtype, int window) {
+    return static_cast<OpsModule>((window ? kCache4WindowModule : kCache4Module) + (dtype == FA_DTYPE_BF16 ? 0 : 1));
+}
 
 // Plan of attention over a cache in 4 bits: more tiles a wave where there are rows for them, since what a code costs
 // to become a number is then shared.
@@ -1219,7 +1264,7 @@ int fa_cache4_append(void* stream, const fa_kv_cache4* cache, const fa_append_co
     if (heads > kOpsMaxGrid / parts) return FA_ERR_UNSUPPORTED;
     p.nparts = static_cast<int>(parts);
     int dev;
-    const OpsModule module = cache4_module(cache->dtype);
+    const OpsModule module = cache4_module(cache->dtype, 0);
     if ((rc = ops_begin(&dev, module)) != FA_OK) return rc;
     return ops_launch(dev, module, cache->dtype == FA_DTYPE_BF16 ? "fa_cache4_append_bf16" : "fa_cache4_append_f16",
                       heads * parts, 256, &p, static_cast<hipStream_t>(stream));
@@ -1250,7 +1295,7 @@ int fa_cache4_read(void* stream, const fa_kv_cache4* cache, const fa_read_config
     p.n = static_cast<int>(n);
     p.vec = vec_ok(k_out, lk, d) && vec_ok(v_out, lv, d);
     int dev;
-    const OpsModule module = cache4_module(cache->dtype);
+    const OpsModule module = cache4_module(cache->dtype, 0);
     if ((rc = ops_begin(&dev, module)) != FA_OK) return rc;
     return ops_launch(dev, module, cache->dtype == FA_DTYPE_BF16 ? "fa_cache4_read_bf16" : "fa_cache4_read_f16",
                       (heads * words + 255) / 256, 256, &p, static_cast<hipStream_t>(stream));
@@ -1295,7 +1340,7 @@ int fa_cache4_attention(void* stream_, const fa_tree_config* c, const fa_window*
     p.block4 = static_cast<int>(block_rows);
     p.vec4 = vec_ok(q, lq, d) && ovec_ok(out, lo, 2);
     int dev;
-    const OpsModule module = cache4_module(cache->dtype), joins = of_type(kCacheModule, cache->dtype);
+    const OpsModule module = cache4_module(cache->dtype, size), joins = cache_module(cache->dtype, p);
     if ((rc = ops_begin(&dev, module)) != FA_OK || (rc = ops_module(dev, joins)) != FA_OK) return rc;
     const hipStream_t stream = static_cast<hipStream_t>(stream_);
     const size_t rows = n * static_cast<size_t>(p.group);

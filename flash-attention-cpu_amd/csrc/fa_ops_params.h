@@ -46,6 +46,10 @@ struct ScoreParams {
     int nqb;                  // query (dK/dV: key) blocks a slice
     int splits;               // dK/dV: workgroups that share a key block, each some heads of the group
     float* part;              // their sums: [dK, dV][split][batch, kv head][key][padded d]
+    // dK/dV in a window: workgroups from far_first on take far_stages stages each of the queries that see the first
+    // far_blocks key blocks (far_rows rows) as sinks alone
+    int far_first, far_stages, far_chunks, far_blocks, far_rows;
+    float* far_part;          // [dK, dV][chunk + 1][split][batch, kv head][far_rows][padded d]
     float scale;              // of the scores
     float scale_log2e;
     float cap_in;             // 2 log2(e) scale / softcap: exponent of the cap's tanh

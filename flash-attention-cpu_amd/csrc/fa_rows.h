@@ -41,7 +41,7 @@ struct RowsWork {
     // the key that stands `i` behind kbeg (a multiple of 16) among those walked
     __device__ __forceinline__ int key(int i) const {
         const int k = kfirst + i;
-        return k + (k >= gap ? skip : 0);
+        return kWindow ? k + (k >= gap ? skip : 0) : k;
     }
     int kfirst;       // kbeg among those walked
 };
@@ -63,7 +63,7 @@ __device__ __forceinline__ Walk rows_walk(const RowsParams& p, int b) {
         w.total = p.causal ? max(min(max(p.q_start + p.n, p.prefix ? p.prefix[b] : 0), p.sk), 0) : p.sk;
         first = p.q_start;
     }
-    if (p.window) {
+    if (kWindow) {
         if (!p.lens) w.total = min(w.total, max(max(first + p.n - 1 + p.window, p.sinks), 0));
         w.gap = (p.sinks + 63) & ~63;
         const int low = min(first - p.window + 1, w.total);
@@ -177,7 +177,7 @@ __device__ __forceinline__ bool rows_work(const RowsParams& p, int rows, int lan
         w.open = w.docs ? 0 : p.causal ? max(p.q_start + 1, w.prefix) : p.sk;
     }
     w.low = INT32_MIN;
-    if (p.window) {
+    if (kWindow) {
         int last = p.q_start + p.n - 1;   // position of the last query
         if (w.tree) {
             last = p.pos ? w.len : (int)min((int64_t)w.len + p.n - 1, (int64_t)kWindowMaxPos);
@@ -199,7 +199,7 @@ __device__ __forceinline__ bool rows_work(const RowsParams& p, int rows, int lan
     const int last = (int)min(w.kfirst + per, (int64_t)total);
     w.kwalk = last - w.kfirst;
     w.kbeg = w.key(0);
-    w.kend = last + (last > w.gap ? w.skip : 0);
+    w.kend = kWindow ? last + (last > w.gap ? w.skip : 0) : last;
     w.nrows = p.n * p.group;
     w.rfirst = w.rb * rows;
     return true;
@@ -207,7 +207,7 @@ __device__ __forceinline__ bool rows_work(const RowsParams& p, int rows, int lan
 
 // Whether the keys of a block need the mask: [k0, k0 + n).
 __device__ __forceinline__ int rows_masked(const RowsParams& p, const RowsWork& w, int k0, int n) {
-    return k0 + n > min(w.open, w.kend) || (k0 < w.low && k0 + n > p.sinks);
+    return k0 + n > min(w.open, w.kend) || (kWindow && k0 < w.low && k0 + n > p.sinks);
 }
 
 // Position of a token for windows, which drafted tokens do not stand before their sequence's filled rows for.
@@ -225,7 +225,7 @@ __device__ __forceinline__ bool window_hides(const RowsParams& p, const RowsWork
 
 // Whether token `tok` sees key `key` < kend, as far as masks tell.
 __device__ __forceinline__ bool rows_see(const RowsParams& p, const RowsWork& w, int tok, int key) {
-    if (p.window && window_hides(p, w, window_position(p, w, tok), key)) return false;
+    if (kWindow && window_hides(p, w, window_position(p, w, tok), key)) return false;
     if (!w.tree) {
         if (p.causal && !(key <= p.q_start + tok || key < w.prefix)) return false;
         if (!w.docs) return true;

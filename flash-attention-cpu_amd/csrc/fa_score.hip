@@ -79,7 +79,7 @@ struct Stages {
     __device__ __forceinline__ int next(int* masked) {
         while (vis == 0) {
             base += 64;
-            if (base >= skip_from && base < skip_to) base = skip_to;
+            if (kWindow && base >= skip_from && base < skip_to) base = skip_to;
             if (base >= count) return -1;
             bool p = false, v = false;
             if (base + lane < count) v = test(base + lane, &p);
@@ -108,14 +108,17 @@ __device__ __forceinline__ int key_limit(const ScoreParams& p, int prefix, int p
 }
 
 // Whether the window hides key `key` from a query at position pos.
+__device__ __forceinline__ bool window_hides(const ScoreParams& p, int pos, int key, int sinks) {
+    return key >= sinks && (key <= pos - p.window || key >= pos + p.window);
+}
 __device__ __forceinline__ bool window_hides(const ScoreParams& p, int pos, int key) {
-    return key >= p.sinks && (key <= pos - p.window || key >= pos + p.window);
+    return window_hides(p, pos, key, p.sinks);
 }
 
 // Whether query `row` sees key `key`.
 __device__ __forceinline__ bool pair_seen(const ScoreParams& p, int prefix, int b, int row, int key) {
     if (key >= key_limit(p, prefix, p.q_start + row)) return false;
-    if (p.window && window_hides(p, p.q_start + row, key)) return false;
+    if (kWindow && window_hides(p, p.q_start + row, key)) return false;
     if (!p.q_doc) return true;
     const int d = p.q_doc[(int64_t)b * p.sq + row];
     return d >= 0 && d == p.k_doc[(int64_t)b * p.sk + key];
@@ -187,21 +190,21 @@ __device__ __forceinline__ bool key_stage(const ScoreParams& p, int prefix, int 
         v = k0 <= p.q_start + q1 - 1 || k0 < prefix;
         if (!(k1 - 1 <= p.q_start + q0 || k1 <= prefix)) *part = true;
     }
-    if (p.window && v) v = window_meets(p, p.q_start + q0, p.q_start + q1 - 1, k0, k1, part);
+    if (kWindow && v) v = window_meets(p, p.q_start + q0, p.q_start + q1 - 1, k0, k1, part);
     if (docs && v) v = docs_meet(qr, doc_range(krng, k0 / kDocTile), part);
     return v;
 }
 // The stages of keys that the windows of queries [q0, q1) leave.
 template <int SK, typename S>
 __device__ __forceinline__ void window_keys(const ScoreParams& p, S* s, int q0, int q1) {
-    if (!p.window) return;
+    if (!kWindow) return;
     const int up = p.causal && !p.prefix ? 0 : p.window - 1;
     window_stages<SK>(s, p.sinks, p.q_start + q0 - p.window + 1, p.q_start + q1 - 1 + up, s->count);
 }
 // Whether rows of a wave at positions [lo, hi] see a key of [k0, k1), as far as the window tells.
 __device__ __forceinline__ bool window_active(const ScoreParams& p, int lo, int hi, int k0, int k1) {
     bool part;
-    return !p.window || window_meets(p, lo, hi, k0, k1, &part);
+    return !kWindow || window_meets(p, lo, hi, k0, k1, &part);
 }
 
 // ---------------------------------------------------------------------------
@@ -350,16 +353,16 @@ __device__ __forceinline__ void score_forward(const ScoreParams& p) {
                 for (int r = 0; r < 4; ++r)
                     if (key + r >= limit[t]) s[t][b][r] = OPS_NEG_INF;
         }
-        if (p.window) {
-            const ScoreParams lp = late_params<ScoreParams>();
+        if constexpr (kWindow) {
 #pragma unroll
-            for (int t = 0; t < MT; ++t)
+            for (int t = 0; t < MT; ++t) {
+                const int pos = p.q_start + row0 + 16 * t + li - k0 - koff - 4 * g;
 #pragma unroll
                 for (int b = 0; b < KB; ++b)
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
-                        if (window_hides(lp, lp.q_start + row0 + 16 * t + li, k0 + koff + 16 * b + 4 * g + r))
-                            s[t][b][r] = OPS_NEG_INF;
+                        if (window_hides(p, pos, 16 * b + r, p.sinks - k0 - koff - 4 * g)) s[t][b][r] = OPS_NEG_INF;
+            }
         }
     };
     v8 pb[MT][NCH];
@@ -813,11 +816,10 @@ __device__ __forceinline__ void score_dq(const ScoreParams& p) {
 #pragma unroll
                             for (int r = 0; r < 4; ++r)
                                 if (key + r >= limit[t]) x[b][r] = y[b][r] = 0.0f;
-                            if (p.window) {
-                                const ScoreParams lp = late_params<ScoreParams>();
+                            if constexpr (kWindow) {
 #pragma unroll
                                 for (int r = 0; r < 4; ++r)
-                                    if (window_hides(lp, pos, key + r)) x[b][r] = y[b][r] = 0.0f;
+                                    if (window_hides(p, pos, key + r)) x[b][r] = y[b][r] = 0.0f;
                             }
                         }
 #pragma unroll
@@ -955,9 +957,20 @@ __device__ __forceinline__ void dkv_specials(const ScoreParams& p, Test test, in
     }
 }
 
+// Of the stages of queries: those in [first, last) but not in [out_first, out_last).
+struct FarStages {
+    int first, last, out_first, out_last;
+    __device__ __forceinline__ bool takes(int st) const {
+        return st >= first && st < last && !(st >= out_first && st < out_last);
+    }
+};
+
 // dK and dV: key rows kept, the queries of every head of the group walked.  Four waves
 // of MT 16-row tiles; Q and dO tiles double-buffered, one barrier a stage.  A kv head's sums over its
 // query heads are formed here, in head order, or by score_dkv_sum where workgroups share them.
+// Windows: key blocks that hold sinks are seen by all queries.  Those whose window does not reach them are dealt out in
+// chunks to workgroups of their own (blockIdx >= p.far_first), whose sums score_dkv_sum adds, since the few long
+// blocks would end long after all others.
 // Bound as the forward kernel, with LDS read at half of its rate besides: bf16, 2 x 16 x 4096^2 all visible, 128
 // columns some 615 us (four products, 890 TF/s), dQ 515 us.
 template <typename T, int D, int MT, int KG, int MOD, bool VEC>
@@ -980,8 +993,23 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
     const int g = lane >> 4, li = lane & 15;
     // a workgroup takes heads first .. first + count - 1 of a kv head's group; the first key blocks have most queries
     // where causal
-    const Work w = find_work(p.k_order ? blockIdx.x : gridDim.x - 1 - blockIdx.x, p.nqb, p.batch * p.kv_heads, p.splits,
-                             p.kv_heads, p.k_order);
+    Work w;
+    int chunk = -1;
+    if (kWindow && (int)blockIdx.x >= p.far_first) {
+        int id = blockIdx.x - p.far_first;
+        chunk = id % p.far_chunks;
+        id /= p.far_chunks;
+        w.hq = id % p.splits;
+        id /= p.splits;
+        w.blk = id % p.far_blocks;
+        id /= p.far_blocks;
+        w.hk = id % p.kv_heads;
+        w.b = id / p.kv_heads;
+    } else {
+        const unsigned grid = kWindow ? p.far_first : gridDim.x;
+        w = find_work(p.k_order ? blockIdx.x : grid - 1 - blockIdx.x, p.nqb, p.batch * p.kv_heads, p.splits, p.kv_heads,
+                      p.k_order);
+    }
     const int count = p.group / p.splits, first = w.hk * p.group + w.hq * count;
     const int kg = wave / NR, qoff = kg * 32 * NCH;   // the wave's queries of a stage
     const int kbeg = w.blk * BK, key0 = kbeg + 16 * MT * (wave % NR);
@@ -1014,6 +1042,15 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
         kr = doc_range(p.k_rng + (int64_t)w.b * 2 * ((p.sk + kDocTile - 1) / kDocTile), kbeg, kend);
         qrng = p.q_rng + (int64_t)w.b * 2 * ((p.sq + kDocTile - 1) / kDocTile);
     }
+    const int nst = (p.sq + SQ - 1) / SQ;
+    // the stages of queries whose window reaches the keys, or of a chunk of the others
+    FarStages far = {0, nst, 0, 0};
+    if constexpr (kWindow) {
+        const int lo = kbeg - p.q_start - (p.causal && !p.prefix ? 0 : p.window - 1), hi = kend - 1 - p.q_start + p.window - 1;
+        const int first = lo <= 0 ? 0 : min(nst, lo / SQ), last = hi < 0 ? 0 : min(nst, hi / SQ + 1);
+        if (chunk < 0) far = {first, last, 0, 0};
+        else far = {chunk * p.far_stages, min(nst, (chunk + 1) * p.far_stages), first, last};
+    }
     auto test = [&](int st, bool* part) -> bool {
         const int q0 = st * SQ, q1 = min(q0 + SQ, p.sq);
         bool v = true;
@@ -1022,15 +1059,16 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
             v = p.q_start + q1 - 1 >= kbeg || kbeg < prefix;
             if (!(p.q_start + q0 >= kend - 1 || kend <= prefix)) *part = true;
         }
-        if (p.window && v) v = window_meets(p, p.q_start + q0, p.q_start + q1 - 1, kbeg, kend, part);
+        if (kWindow && v)
+            v = window_meets(p, p.q_start + q0, p.q_start + q1 - 1, kbeg, kend, part) && far.takes(st);
         if (docs && v) v = docs_meet(kr, doc_range(qrng, q0 / kDocTile), part);
         return v;
     };
-    const int nst = (p.sq + SQ - 1) / SQ;
     Stages<decltype(test)> stages(nst, lane, test);
-    if (p.window && kbeg >= p.sinks)
-        window_stages<SQ>(&stages, 0, kbeg - p.q_start - (p.causal && !p.prefix ? 0 : p.window - 1),
-                          kend - 1 - p.q_start + p.window - 1, nst);
+    if constexpr (kWindow) {
+        stages.count = far.last;
+        stages.skip_to = far.first & ~63;
+    }
     const Fill qfill(p.qs.s, p.d, wave, lane), ofill(p.dos.s, p.d, wave, lane);
     // the next (head, stage): the stages of one head of the group after the other
     int head = 0;
@@ -1154,11 +1192,10 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
 #pragma unroll
                             for (int r = 0; r < 4; ++r)
                                 if (key >= key_limit(p, prefix, pos + r) || lse2[r] == -OPS_NEG_INF) x[r] = y[r] = 0.0f;
-                            if (p.window) {
-                                const ScoreParams lp = late_params<ScoreParams>();
+                            if constexpr (kWindow) {
 #pragma unroll
                                 for (int r = 0; r < 4; ++r)
-                                    if (window_hides(lp, pos + r, key)) x[r] = y[r] = 0.0f;
+                                    if (window_hides(p, pos + r, key)) x[r] = y[r] = 0.0f;
                             }
                         }
 #pragma unroll
@@ -1242,10 +1279,21 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
             dv[0][j] += vsum[j * 64 + lane];
         }
     }
-    if (lp.splits > 1) {
-        const int64_t rows = (int64_t)lp.batch * lp.kv_heads * lp.sk;   // of one split
-        float* const outk = lp.part + (w.hq * rows + ((int64_t)w.b * lp.kv_heads + w.hk) * lp.sk) * D;
-        float* const outv = outk + lp.splits * rows * D;
+    // to partial sums where several workgroups share the keys: those of the heads of the group, those of far queries,
+    // and (far chunk 0) a block of sinks that otherwise one workgroup has
+    const bool far_sums = kWindow && (chunk >= 0 || (lp.splits == 1 && w.blk < lp.far_blocks));
+    if (lp.splits > 1 || far_sums) {
+        const int64_t slices = (int64_t)lp.batch * lp.kv_heads, at = (int64_t)w.b * lp.kv_heads + w.hk;
+        const int64_t rows = slices * lp.sk;   // of one split
+        float *outk, *outv;
+        if (far_sums) {
+            const int64_t per = slices * lp.far_blocks * BK;
+            outk = lp.far_part + (((chunk + 1) * lp.splits + w.hq) * per + at * lp.far_blocks * BK) * D;
+            outv = outk + (lp.far_chunks + 1) * lp.splits * per * D;
+        } else {
+            outk = lp.part + (w.hq * rows + at * lp.sk) * D;
+            outv = outk + lp.splits * rows * D;
+        }
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
             const int key = key0 + 16 * t + li;
@@ -1275,21 +1323,34 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
         dkv_specials<T, T, SQ>(lp, test, nst, prefix, w.b, first, count, key0, 16 * MT, lane, outk, lp.dks.s, outv, lp.dvs.s);
 }
 
-// Adds up the splits of a key block's heads: four columns a thread.
+// Adds up the splits of a key block's heads and, of sinks, the chunks of far queries: four columns a thread.  Without
+// splits only rows of sinks come here.
 template <typename T, int D, bool VEC>
 __device__ __forceinline__ void score_dkv_sum(const ScoreParams& p) {
     constexpr int L = D / 4;
     const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, row = id / L;
-    const int col = id % L * 4;
+    const int col = id % L * 4, far_rows = kWindow ? p.far_rows : 0, n = p.splits > 1 ? p.sk : min(far_rows, p.sk);
+    if (row >= (int64_t)p.batch * p.kv_heads * n) return;
+    const int key = row % n, hk = row / n % p.kv_heads, b = row / n / p.kv_heads;
     const int64_t rows = (int64_t)p.batch * p.kv_heads * p.sk;
-    if (row >= rows) return;
-    const int key = row % p.sk, hk = row / p.sk % p.kv_heads, b = row / p.sk / p.kv_heads;
-    const float* at = p.part + row * D + col;
     f32x4 k = {0.0f, 0.0f, 0.0f, 0.0f}, v = k;
+    if (p.splits > 1) {
+        const float* at = p.part + row * D + col;
 #pragma unroll 4
-    for (int s = 0; s < p.splits; ++s) {
-        k += *reinterpret_cast<const f32x4*>(at + s * rows * D);
-        v += *reinterpret_cast<const f32x4*>(at + (p.splits + s) * rows * D);
+        for (int s = 0; s < p.splits; ++s) {
+            k += *reinterpret_cast<const f32x4*>(at + s * rows * D);
+            v += *reinterpret_cast<const f32x4*>(at + (p.splits + s) * rows * D);
+        }
+    }
+    if (kWindow && key < far_rows) {
+        const int64_t per = (int64_t)p.batch * p.kv_heads * far_rows;
+        const float* at = p.far_part + ((int64_t)(b * p.kv_heads + hk) * far_rows + key) * D + col;
+        const int all = (p.far_chunks + 1) * p.splits;
+#pragma unroll 4
+        for (int s = p.splits > 1 ? p.splits : 0; s < all; ++s) {   // (chunk 0 is used without splits only)
+            k += *reinterpret_cast<const f32x4*>(at + s * per * D);
+            v += *reinterpret_cast<const f32x4*>(at + (all + s) * per * D);
+        }
     }
     if (p.dk) store4<T, VEC>(slice<T>(p.dk, p.dks, b, hk) + key * p.dks.s, col, p.d, k * p.scale);
     if (p.dv) store4<T, VEC>(slice<T>(p.dv, p.dvs, b, hk) + key * p.dvs.s, col, p.d, v);
@@ -1394,6 +1455,15 @@ SUM(64, false, s)
 SUM(128, false, s)
 SUM(256, false, s)
 // plain scores, capped (c), with a bias (b) or both (cb); any alignment (s); two groups of waves on a stage (k)
+// windows: plain scores, or looked up (m)
+#ifdef OPS_WINDOW
+#define KERNELS(F, D, MT, WAVES)                      \
+    KERNEL(F, D, MT, 1, 0, true, , WAVES)             \
+    KERNEL(F, D, MT, 1, kAny, true, m, WAVES)
+#define GROUPS(F, D, WAVES)                           \
+    KERNEL(F, D, 1, 2, 0, true, k, WAVES)             \
+    KERNEL(F, D, 1, 2, kAny, true, km, WAVES)
+#else
 #define KERNELS(F, D, MT, WAVES)                      \
     KERNEL(F, D, MT, 1, 0, true, , WAVES)             \
     KERNEL(F, D, MT, 1, kCap, true, c, WAVES)         \
@@ -1404,6 +1474,7 @@ SUM(256, false, s)
     KERNEL(F, D, 1, 2, kCap, true, kc, WAVES)         \
     KERNEL(F, D, 1, 2, kBias, true, kb, WAVES)        \
     KERNEL(F, D, 1, 2, kCap | kBias, true, kcb, WAVES)
+#endif
 #define SLOW(F, W64, W128, W256)                 \
     KERNEL(F, 64, 1, 1, kAny, false, s, W64)     \
     KERNEL(F, 128, 1, 1, kAny, false, s, W128)   \
@@ -1423,10 +1494,14 @@ ALL(dq, 2, 2, 2)
 ALL(dkv, 2, 2, 1)
 // two tiles of 64 columns: three waves a SIMD, except where a cap would spill (bf16, 16 heads x 4 x 4096^2, causal,
 // plain 200 -> 172 us, bias 282 -> 248, capped 287 -> 318)
+#ifdef OPS_WINDOW
+KERNELS(forward, 64, 2, 2)
+#else
 KERNEL(forward, 64, 2, 1, 0, true, , 3)
 KERNEL(forward, 64, 2, 1, kCap, true, c, 2)
 KERNEL(forward, 64, 2, 1, kBias, true, b, 3)
 KERNEL(forward, 64, 2, 1, kCap | kBias, true, cb, 2)
+#endif
 KERNELS(forward, 128, 2, 2)
 KERNELS(dq, 64, 2, 2)
 KERNELS(dkv, 64, 2, 2)
