@@ -792,22 +792,34 @@ int check_norm(const fa_rotary_config* c, const fa_head_norm* n) {
     return n && n->eps > 0.0f && std::isfinite(n->eps) ? FA_OK : FA_ERR_INVALID_ARG;
 }
 
-// Lanes of a row and tokens of a workgroup.
-int plan_norm(int dev, int dtype, bool wide, NormParams* p, bool* wide_out, size_t* grid) {
+// The kernel's kind, lanes of a row and tokens of a workgroup.
+int plan_norm(int dev, int dtype, bool wide, NormParams* p, const char** kind, size_t* grid) {
     const int w = static_cast<int>(16 / elem_size(dtype));
     const int run = p->interleaved ? p->rot : p->rot / 2;
     wide = wide && run % w == 0 && (p->d - p->rot) % w == 0;
     p->units = wide ? run / w + (p->d - p->rot) / w : p->rot / 2 + p->d - p->rot;
-    p->lanes = 1;
-    while (p->lanes < 64 && p->lanes < p->units) p->lanes *= 2;
-    const size_t slots = 256 / p->lanes, all = static_cast<size_t>(p->batch) * p->seq;
+    auto power = [](int n) {
+        int l = 1;
+        while (l < 64 && l < n) l *= 2;
+        return l;
+    };
+    p->lanes = power(p->units);
+    // three units a lane where that leaves fewer lanes idle (20 units: 24 places instead of 32; 2 x 1000 tokens of 16 + 16
+    // heads of 80 columns, 40 of them rotary, f32)
+    const bool three = wide && (p->interleaved || dtype == FA_DTYPE_F32) && p->units > 2 && 3 * power((p->units + 2) / 3) < p->lanes;
+    if (three) p->lanes = power((p->units + 2) / 3);
+    const bool full = wide && !three && p->rot == p->d && p->units == p->lanes;
+    *kind = !wide ? "0" : full ? (p->interleaved ? "fi" : "f") : three ? (p->interleaved ? "3i" : "3") : p->interleaved ? "1i" : "1";
+    const size_t slots = kNormThreads / p->lanes, all = static_cast<size_t>(p->batch) * p->seq;
     *grid = 0;
     for (int i = 0; i < p->nt; ++i) {
         NormTensor& t = p->t[i];
-        // some four rows a slot where that leaves workgroups enough
+        // some four rows a slot, so that the next is on its way while one is worked on, where that leaves two workgroups a
+        // CU; a row for each slot where it leaves one
         size_t tokens = 1;
+        const size_t cus = static_cast<size_t>(g_dev[dev].num_cus);
         while (tokens < kNormTokens && tokens * t.heads < 4 * slots &&
-               (all + 2 * tokens - 1) / (2 * tokens) >= 4 * static_cast<size_t>(g_dev[dev].num_cus))
+               all / (2 * tokens) >= (tokens * t.heads < slots ? 1 : 2) * cus)
             tokens *= 2;
         t.tokens = static_cast<int>(tokens);
         const size_t blocks = (all + tokens - 1) / tokens;
@@ -815,15 +827,15 @@ int plan_norm(int dev, int dtype, bool wide, NormParams* p, bool* wide_out, size
         t.blocks = static_cast<int>(blocks);
         *grid += blocks;
     }
-    *wide_out = wide;
     return *grid > kOpsMaxGrid ? FA_ERR_UNSUPPORTED : FA_OK;
 }
 int launch_norm(int dev, hipStream_t stream, int dtype, NormParams* p, bool wide) {
     size_t grid;
-    int rc = plan_norm(dev, dtype, wide, p, &wide, &grid);
+    const char* kind;
+    const int rc = plan_norm(dev, dtype, wide, p, &kind, &grid);
     if (rc != FA_OK) return rc;
     char name[64];
-    std::snprintf(name, sizeof(name), "fa_norm_%s_%d", dtype_name(dtype), wide ? 1 : 0);
+    std::snprintf(name, sizeof(name), "fa_norm_%s_%s", dtype_name(dtype), kind);
     return ops_launch(dev, kNormModule, name, grid, kNormThreads, p, stream);
 }
 
@@ -1091,8 +1103,8 @@ int fa_norm_rotary_backward(void* stream_, const fa_rotary_config* cfg, const fa
     OpsWorkspace ws;
     if (rows.nt > 0) {
         size_t grid;
-        bool wide;
-        if ((rc = plan_norm(dev, cfg->dtype, check.wide, &rows, &wide, &grid)) != FA_OK) return rc;
+        const char* kind;
+        if ((rc = plan_norm(dev, cfg->dtype, check.wide, &rows, &kind, &grid)) != FA_OK) return rc;
         if (weights) {
             if ((rc = ws.get(dev, stream, grid * d * sizeof(float))) != FA_OK) return rc;
             float* part = static_cast<float*>(ws.ptr);
@@ -1103,10 +1115,11 @@ int fa_norm_rotary_backward(void* stream_, const fa_rotary_config* cfg, const fa
             }
         }
         char name[64];
-        std::snprintf(name, sizeof(name), "fa_norm_back_%s_%d", dtype_name(cfg->dtype), wide ? 1 : 0);
+        std::snprintf(name, sizeof(name), "fa_norm_back_%s_%s", dtype_name(cfg->dtype), kind);
         rc = ops_launch(dev, kNormModule, name, grid, kNormThreads, &rows, stream);
     }
-    if (rc == FA_OK && weights) rc = ops_launch(dev, kNormModule, "fa_norm_weights", p.nt * ((d + 15) / 16), 1024, &p, stream);
+    if (rc == FA_OK && weights) rc = ops_launch(dev, kNormModule, "fa_norm_weights", p.nt * ((d + kNormColumns - 1) / kNormColumns), 1024, &p,
+                                              stream);
     return ws.done(stream, rc);
 } catch (...) {   // no memory for the tables of modules, kernels and workspaces
     return FA_ERR_ALLOC;

@@ -132,6 +132,7 @@ struct RotParams {
 // One tensor of a launch of norms with rotary positions.
 constexpr int kNormThreads = 256;
 constexpr int kNormTokens = 16;   // most tokens of a workgroup
+constexpr int kNormColumns = 8;   // of a workgroup of fa_norm_weights
 struct NormTensor {
     const void *x, *dy, *w;   // w: NULL: ones
     void* out;                // y, or dx (NULL: not wanted)
