@@ -12,6 +12,7 @@
 //
 // Built once a type: OPS_T the type of queries, outputs and rows (16 bits), OPS_NAME its name in the kernels'.
 
+#define ROWS_EVEN
 #include "fa_rows.h"
 
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
@@ -196,12 +197,14 @@ __device__ __forceinline__ void cache4_read(const Cache4Params& p) {
 // Eight values of a word: codes to the fraction of f16 numbers in [1, 2), times S, plus O.  big(i), off(i): those of
 // pair i.
 template <typename B, typename O>
-__device__ __forceinline__ h8 dequant(unsigned w, B big, O off) {
+__device__ __forceinline__ h8 dequant(unsigned w, unsigned one, B big, O off) {
     h8 v;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const unsigned bits = (4 * i < 6 ? w << (6 - 4 * i) : w >> (4 * i - 6)) & 0x03c003c0u;
-        const h2 t = __builtin_bit_cast(h2, bits | 0x3c003c00u);
+        unsigned bits = 4 * i < 6 ? w << (6 - 4 * i) : w >> (4 * i - 6);
+        // (bits & mask) | one: the compiler makes two instructions of it, since it takes both constants for literals
+        asm("v_and_or_b32 %0, %0, %1, %2" : "+v"(bits) : "s"(0x03c003c0u), "v"(one));
+        const h2 t = __builtin_bit_cast(h2, bits);
         const h2 y = __builtin_elementwise_fma(t, big(i), off(i));
         v[2 * i] = y[0];
         v[2 * i + 1] = y[1];
@@ -273,35 +276,54 @@ __device__ __forceinline__ void rows4(const RowsParams& p) {
         Words<VW> v[NV];
         Words<4> big[NV], off[NV];
     };
-    // the page of a block of 32 keys (0 without pages), -1: bad or past the end
-    auto look_up = [&](int i) {
-        if (SMALL || i >= nblk) return -1;
-        return pages.page(key_of(i));
+    // the page of a block of 32 keys (0 without pages; SMALL: of each of its runs of 8), -1: bad or past the end
+    struct Pages {
+        int p[SMALL ? 4 : 1];
     };
-    auto rows_at = [&](int i, int page) -> int64_t {   // rows before the block's first, of its head
+    auto look_up = [&](int i) {
+        Pages r;
+#pragma unroll
+        for (int e = 0; e < (SMALL ? 4 : 1); ++e) {
+            r.p[e] = -1;
+            if (i < nblk && key_of(i) + 8 * e < w.kend) r.p[e] = pages.page(key_of(i) + 8 * e);
+        }
+        return r;
+    };
+    auto any_bad = [&](const Pages& pg, int k0) {
+        int bad = 0;
+#pragma unroll
+        for (int e = 0; e < (SMALL ? 4 : 1); ++e) bad |= pg.p[e] < 0 && k0 + 8 * e < w.kend;
+        return bad;
+    };
+    // Of a block of 32 keys: the rows before it in memory, and those that are there.
+    struct Source {
+        int64_t at;
+        int n;
+    };
+    const int64_t head_rows = ((int64_t)(p.table ? 0 : w.b) * p.kv_heads + w.hk) * page_rows;
+    const int64_t page_stride = (int64_t)p.kv_heads * page_rows;
+    auto source = [&](int i, int page) -> Source {
+        if (page < 0 || i >= nblk) return {0, 0};
         const int k0 = key_of(i);
-        const int64_t blk = p.table ? page : w.b;
-        return (blk * p.kv_heads + w.hk) * page_rows + (p.table ? k0 & pages.page_mask : k0);
+        return {head_rows + (p.table ? page * page_stride + (k0 & pages.page_mask) : (int64_t)k0), min(SK, w.kend - k0)};
     };
     auto buffer = [&](const unsigned* base, int64_t word, int words) {
-        return __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned*>(words > 0 ? base + word : base), (short)0, 4 * words,
-                                                 0x00020000);
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned*>(base + word), (short)0, 4 * words, 0x00020000);
     };
-    // SMALL: the rows before row `row` of its head, where it is one
-    auto lane_rows = [&](int row, bool* real) -> int64_t {
-        *real = row < w.kend;
-        int page = *real ? pages.table[row >> pages.shift] : 0;
-        if ((unsigned)page >= (unsigned)pages.n_pages) *real = false;
-        return ((int64_t)page * p.kv_heads + w.hk) * page_rows + (row & pages.page_mask);
+    // SMALL: the rows before row `row` of its head, in run `run` of 8 of the block, where it is one
+    auto lane_rows = [&](const Pages& pg, int row, int run, bool* real) -> int64_t {
+        int page = pg.p[0];
+        if constexpr (SMALL) page = run == 0 ? pg.p[0] : run == 1 ? pg.p[1] : run == 2 ? pg.p[2] : pg.p[3];
+        *real = page >= 0 && row < w.kend;
+        return head_rows + page * page_stride + (row & pages.page_mask);
     };
-    auto load_k = [&](Block& x, int i, int page) {
-        const int k0 = key_of(i);
+    auto load_k = [&](Block& x, int i, const Source& src, const Pages& pg) {
         if constexpr (SMALL) {
+            const int k0 = key_of(i);
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
-                bool real = false;
-                int64_t at = 0;
-                if (i < nblk) at = lane_rows(k0 + 8 * (li >> 2) + 4 * b + (li & 3), &real);
+                bool real;
+                const int64_t at = lane_rows(pg, k0 + 8 * (li >> 2) + 4 * b + (li & 3), li >> 2, &real);
 #pragma unroll
                 for (int q = 0; q < NK; ++q) {
                     x.k[b][q] = {};
@@ -313,9 +335,8 @@ __device__ __forceinline__ void rows4(const RowsParams& p) {
                 }
             }
         } else {
-            const int n = page < 0 || i >= nblk ? 0 : max(0, min(SK, w.kend - k0));
-            const int64_t at = n ? rows_at(i, page) : 0;
-            const __amdgpu_buffer_rsrc_t rk = buffer(K, at * (D / 8), n * (D / 8)), rs = buffer(KS, at * NDC, n * NDC);
+            const int n = src.n;
+            const __amdgpu_buffer_rsrc_t rk = buffer(K, src.at * (D / 8), n * (D / 8)), rs = buffer(KS, src.at * NDC, n * NDC);
 #pragma unroll
             for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -325,12 +346,11 @@ __device__ __forceinline__ void rows4(const RowsParams& p) {
                 }
         }
     };
-    auto load_v = [&](Block& x, int i, int page) {
-        const int k0 = key_of(i);
+    auto load_v = [&](Block& x, int i, const Source& src, const Pages& pg) {
         if constexpr (SMALL) {
-            bool real = false;
-            int64_t at = 0;
-            if (i < nblk) at = lane_rows(k0 + 8 * g, &real) / 8;
+            const int k0 = key_of(i);
+            bool real;
+            const int64_t at = lane_rows(pg, k0 + 8 * g, g, &real) >> 3;
 #pragma unroll
             for (int q = 0; q < NV; ++q) {
                 x.v[q] = {};
@@ -346,8 +366,8 @@ __device__ __forceinline__ void rows4(const RowsParams& p) {
                 }
             }
         } else {
-            const int n = page < 0 || i >= nblk ? 0 : (max(0, min(SK, w.kend - k0)) + 7) / 8;   // runs of 8 rows
-            const int64_t at = n ? rows_at(i, page) / 8 : 0;
+            const int n = (src.n + 7) >> 3;   // runs of 8 rows
+            const int64_t at = src.at >> 3;
             const __amdgpu_buffer_rsrc_t rv = buffer(V, at * D, n * D), rs = buffer(VS, at * NDC * 8, n * NDC * 8);
 #pragma unroll
             for (int q = 0; q < NV; ++q) {
@@ -359,11 +379,14 @@ __device__ __forceinline__ void rows4(const RowsParams& p) {
     };
 
     Block A, B;
-    int page0 = look_up(0), page1 = look_up(1), page2;
-    load_k(A, 0, page0);
-    load_v(A, 0, page0);
-    load_k(B, 1, page1);
-    load_v(B, 1, page1);
+    Pages page2 = look_up(0);
+    int bad0 = any_bad(page2, key_of(0));   // of the block to work on, and of the next
+    load_k(A, 0, source(0, page2.p[0]), page2);
+    load_v(A, 0, source(0, page2.p[0]), page2);
+    page2 = look_up(1);
+    int bad1 = any_bad(page2, key_of(1));
+    load_k(B, 1, source(1, page2.p[0]), page2);
+    load_v(B, 1, source(1, page2.p[0]), page2);
     page2 = look_up(2);
 
     // Queries as f16.  bf16 rows are brought into its range by a power of two, exactly but for entries 2^29 below the
@@ -421,9 +444,11 @@ __device__ __forceinline__ void rows4(const RowsParams& p) {
     }
     constexpr float kProb = kProbLog2<_Float16>, kUp = MOD != 0 ? kProb : 0.0f;
     int special = 0;
+    const unsigned one = 0x3c003c00u;   // two f16 ones
 
-    auto block = [&](int i, Block& x, int page) {
-        const int k0 = key_of(i);
+    auto block = [&](int i, Block& x) {
+        const int k0 = key_of(i), bad = bad0;
+        const Source next = source(i + 2, page2.p[0]);
         // S^T of the block, relative to the rows' references
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
@@ -437,18 +462,13 @@ __device__ __forceinline__ void rows4(const RowsParams& p) {
 #pragma unroll
                 for (int b = 0; b < 2; ++b) {
                     const h2 so = __builtin_bit_cast(h2, x.ks[b][n]);
-                    const h8 k = dequant(x.k[b][n].w[j], [&](int) { return (h2){so[0], so[0]}; },
+                    const h8 k = dequant(x.k[b][n].w[j], one, [&](int) { return (h2){so[0], so[0]}; },
                                          [&](int) { return (h2){so[1], so[1]}; });
 #pragma unroll
                     for (int t = 0; t < MT; ++t) s[t][b] = M4::mma(k, q[t][n * KW + j], s[t][b]);
                 }
         __builtin_amdgcn_sched_barrier(0);
-        load_k(x, i + 2, page2);
-        int bad = page < 0;
-        if constexpr (SMALL) {
-            const int row = k0 + lane;
-            bad = __builtin_amdgcn_ballot_w64(lane < SK && row < w.kend && pages.at(row, w.kend, 0, 0) < 0) != 0;
-        }
+        load_k(x, i + 2, next, page2);
         const int masked = bad || rows_masked(p, w, k0, SK);
         if constexpr (MOD != 0) {
 #pragma unroll
@@ -550,20 +570,20 @@ __device__ __forceinline__ void rows4(const RowsParams& p) {
         for (int n = 0; n < NV; ++n)
 #pragma unroll
             for (int j = 0; j < VW; ++j) {
-                const h8 v = dequant(x.v[n].w[j], [&](int e) { return __builtin_bit_cast(h2, x.big[n].w[e]); },
+                const h8 v = dequant(x.v[n].w[j], one, [&](int e) { return __builtin_bit_cast(h2, x.big[n].w[e]); },
                                      [&](int e) { return __builtin_bit_cast(h2, x.off[n].w[e]); });
 #pragma unroll
                 for (int t = 0; t < MT; ++t) o[t][n * VW + j] = M4::mma(v, pb[t], o[t][n * VW + j]);
             }
         __builtin_amdgcn_sched_barrier(0);
-        load_v(x, i + 2, page2);
-        page0 = page1;
-        page1 = page2;
+        load_v(x, i + 2, next, page2);
+        bad0 = bad1;
+        bad1 = any_bad(page2, key_of(i + 2));
         page2 = look_up(i + 3);
     };
     for (int i = 0; i < nblk; i += 2) {
-        block(i, A, page0);
-        if (i + 1 < nblk) block(i + 1, B, page0);
+        block(i, A);
+        if (i + 1 < nblk) block(i + 1, B);
     }
 
 #pragma unroll
@@ -686,29 +706,27 @@ __device__ __forceinline__ void rows4(const RowsParams& p) {
         rows4<OPS_T, NDC, MT, MOD, SMALL>(p);                                                           \
     }
 // plain scores, or looked up (m); pages of less than 32 rows (p)
-#define KINDS(NDC, MT, WAVES)                  \
-    KERNEL(NDC, MT, 0, false, , WAVES)         \
-    KERNEL(NDC, MT, kAny, false, m, WAVES)     \
-    KERNEL(NDC, MT, kAny, true, p, WAVES)
-KINDS(2, 1, 2)
-KINDS(2, 2, 2)
-KINDS(2, 4, 2)
-KINDS(4, 1, 2)
-KINDS(4, 2, 2)
-KINDS(4, 4, 1)
-KINDS(8, 1, 2)
-KINDS(8, 2, 1)
+#define KINDS(NDC, MT, WAVES, MWAVES)           \
+    KERNEL(NDC, MT, 0, false, , WAVES)          \
+    KERNEL(NDC, MT, kAny, false, m, MWAVES)     \
+    KERNEL(NDC, MT, kAny, true, p, MWAVES)
+KINDS(2, 1, 4, 3)
+KINDS(2, 2, 2, 2)
+KINDS(2, 4, 2, 1)
+KINDS(4, 1, 3, 2)
+KINDS(4, 2, 2, 2)
+KINDS(4, 4, 1, 1)
+KINDS(8, 1, 1, 1)
+KINDS(8, 2, 1, 1)
 // other widths
-KERNEL(1, 1, kAny, false, m, 2)
-KERNEL(3, 1, kAny, false, m, 2)
-KERNEL(5, 1, kAny, false, m, 2)
-KERNEL(6, 1, kAny, false, m, 2)
-KERNEL(7, 1, kAny, false, m, 2)
-KERNEL(1, 1, kAny, true, p, 2)
-KERNEL(3, 1, kAny, true, p, 2)
-KERNEL(5, 1, kAny, true, p, 2)
-KERNEL(6, 1, kAny, true, p, 2)
-KERNEL(7, 1, kAny, true, p, 2)
+#define WIDTHS(NDC, WAVES)                  \
+    KERNEL(NDC, 1, kAny, false, m, WAVES)   \
+    KERNEL(NDC, 1, kAny, true, p, WAVES)
+WIDTHS(1, 4)
+WIDTHS(3, 2)
+WIDTHS(5, 1)
+WIDTHS(6, 1)
+WIDTHS(7, 1)
 #ifndef OPS_WINDOW
 extern "C" __global__ __launch_bounds__(256) void PASTE(fa_cache4_append_, OPS_NAME, , )(Cache4Params p) {
     cache4_append<OPS_T>(p);

@@ -882,14 +882,15 @@ OpsModule cache4_module(int dtype, int window) {
 
 // Plan of attention over a cache in 4 bits: more tiles a wave where there are rows for them, since what a code costs
 // to become a number is then shared.
-RowsPlan plan_rows4(size_t d, size_t batch, size_t kv_heads, size_t rows, size_t keys, int num_cus) {
+RowsPlan plan_rows4(size_t d, bool plain, size_t batch, size_t kv_heads, size_t rows, size_t keys, int num_cus) {
     RowsPlan r{};
     const bool widths = d == 64 || d == 128 || d == 256;
     r.mt = !widths || rows <= 16 ? 1 : rows <= 32 || d == 256 ? 2 : 4;
     r.threads = 64 * kRows4Waves;
     r.rows = 16 * r.mt;
     r.step = 32 * kRows4Waves;
-    const size_t resident = static_cast<size_t>(num_cus) * (r.mt * d >= 512 ? 1 : 2);
+    // workgroups a CU that the registers leave room for
+    const size_t resident = static_cast<size_t>(num_cus) * (r.mt * d >= 512 || d > 128 ? 1 : r.mt > 1 || !plain ? 2 : d > 64 ? 3 : 4);
     share_keys(&r, batch, kv_heads, rows, keys, resident, 4 * r.step, ops_pad_d(d));
     return r;
 }
@@ -1357,13 +1358,13 @@ int fa_cache4_attention(void* stream_, const fa_tree_config* c, const fa_window*
     if ((rc = ops_begin(&dev, module)) != FA_OK || (rc = ops_module(dev, joins)) != FA_OK) return rc;
     const hipStream_t stream = static_cast<hipStream_t>(stream_);
     const size_t rows = n * static_cast<size_t>(p.group);
-    const RowsPlan plan = plan_rows4(d, cache->batch, cache->kv_heads, rows, window_keys(capacity, size, sinks, n, false),
-                                     g_dev[dev].num_cus);
+    const char* kind = cache->block_table && cache->page_size < 32                           ? "p"
+                       : c->softcap > 0.0f || c->slopes || (d != 64 && d != 128 && d != 256) ? "m"
+                                                                                              : "";
+    const RowsPlan plan = plan_rows4(d, !*kind, cache->batch, cache->kv_heads, rows,
+                                     window_keys(capacity, size, sinks, n, false), g_dev[dev].num_cus);
     char name[64];
-    std::snprintf(name, sizeof(name), "fa_rows4_%s_c%d_t%d%s", dtype_name(cache->dtype), static_cast<int>(d / 32), plan.mt,
-                  cache->block_table && cache->page_size < 32                       ? "p"
-                  : c->softcap > 0.0f || c->slopes || (d != 64 && d != 128 && d != 256) ? "m"
-                                                                                    : "");
+    std::snprintf(name, sizeof(name), "fa_rows4_%s_c%d_t%d%s", dtype_name(cache->dtype), static_cast<int>(d / 32), plan.mt, kind);
     return launch_rows(dev, stream, cache->dtype, module, name, plan, ops_pad_d(d), p.vec4, &p);
 } catch (...) {   // no memory for the tables of modules, kernels and workspaces
     return FA_ERR_ALLOC;

@@ -147,6 +147,14 @@ __device__ __forceinline__ Runs runs_of_sequence(const RowsParams& p, int b, int
     return r;
 }
 
+// (16 sequences of 33 steps, 17 of them a run's share: 31 + 2 steps each, or 17 + 16; bf16, 16 decode steps in a window of
+// 4096 keys)
+#if defined(ROWS_EVEN) || defined(OPS_WINDOW)
+constexpr bool kEvenRuns = true;
+#else
+constexpr bool kEvenRuns = false;
+#endif
+
 // Returns whether there is work.
 __device__ __forceinline__ bool rows_work(const RowsParams& p, int rows, int lane, RowsWork* out) {
     RowsWork& w = *out;
@@ -194,7 +202,9 @@ __device__ __forceinline__ bool rows_work(const RowsParams& p, int rows, int lan
     w.gap = __builtin_amdgcn_readfirstlane(walk.gap);
     w.skip = __builtin_amdgcn_readfirstlane(walk.skip);
     const int total = __builtin_amdgcn_readfirstlane(walk.walked());
-    const int64_t per = (int64_t)__builtin_amdgcn_readfirstlane(r.steps) * p.step;
+    int64_t per = (int64_t)__builtin_amdgcn_readfirstlane(r.steps) * p.step;
+    // a sequence's runs of one length, rather than all but its last
+    if (kEvenRuns) per = (int64_t)((total + p.step * w.runs - 1) / (p.step * w.runs)) * p.step;
     w.kfirst = (int)min((w.run - __builtin_amdgcn_readfirstlane(r.first)) * per, (int64_t)total);
     const int last = (int)min(w.kfirst + per, (int64_t)total);
     w.kwalk = last - w.kfirst;
