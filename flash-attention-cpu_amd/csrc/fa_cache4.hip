@@ -712,12 +712,9 @@ __device__ __forceinline__ void rows4(const RowsParams& p) {
     KERNEL(NDC, MT, kAny, true, p, MWAVES)
 KINDS(2, 1, 4, 3)
 KINDS(2, 2, 2, 2)
-KINDS(2, 4, 2, 1)
 KINDS(4, 1, 3, 2)
 KINDS(4, 2, 2, 2)
-KINDS(4, 4, 1, 1)
 KINDS(8, 1, 1, 1)
-KINDS(8, 2, 1, 1)
 // other widths
 #define WIDTHS(NDC, WAVES)                  \
     KERNEL(NDC, 1, kAny, false, m, WAVES)   \

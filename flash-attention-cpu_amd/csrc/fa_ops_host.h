@@ -880,17 +880,19 @@ OpsModule cache4_module(int dtype, int window) {
     return static_cast<OpsModule>((window ? kCache4WindowModule : kCache4Module) + (dtype == FA_DTYPE_BF16 ? 0 : 1));
 }
 
-// Plan of attention over a cache in 4 bits: more tiles a wave where there are rows for them, since what a code costs
-// to become a number is then shared.
+// Plan of attention over a cache in 4 bits.
 RowsPlan plan_rows4(size_t d, bool plain, size_t batch, size_t kv_heads, size_t rows, size_t keys, int num_cus) {
     RowsPlan r{};
-    const bool widths = d == 64 || d == 128 || d == 256;
-    r.mt = !widths || rows <= 16 ? 1 : rows <= 32 || d == 256 ? 2 : 4;
+    // Two tiles a wave share what a code costs to become a number, but there are half as many workgroups: from more than
+    // four steps of 128 keys a resident one on (d128, 8 sequences of up to 8000 keys, 256 rows 134 us with two, 156 with
+    // one; 4 of 3000, 200 rows 26 and 24; four tiles, or two of 256 columns, leave one wave a SIMD: 252 us)
+    const size_t cus = static_cast<size_t>(num_cus), steps = batch * keys * kv_heads * ((rows + 31) / 32) / (32 * kRows4Waves);
+    r.mt = (d == 64 || d == 128) && rows > 16 && steps > 4 * 2 * cus ? 2 : 1;
     r.threads = 64 * kRows4Waves;
     r.rows = 16 * r.mt;
     r.step = 32 * kRows4Waves;
     // workgroups a CU that the registers leave room for
-    const size_t resident = static_cast<size_t>(num_cus) * (r.mt * d >= 512 || d > 128 ? 1 : r.mt > 1 || !plain ? 2 : d > 64 ? 3 : 4);
+    const size_t resident = cus * (d > 128 ? 1 : r.mt > 1 || !plain ? 2 : d > 64 ? 3 : 4);
     share_keys(&r, batch, kv_heads, rows, keys, resident, 4 * r.step, ops_pad_d(d));
     return r;
 }
