@@ -34,11 +34,16 @@ __device__ __forceinline__ Place cache4_place(const Cache4Params& p, int b, int6
 __device__ __forceinline__ unsigned half_bits(_Float16 x) { return __builtin_bit_cast(unsigned short, x); }
 __device__ __forceinline__ _Float16 bits_half(unsigned x) { return __builtin_bit_cast(_Float16, (unsigned short)x); }
 
+// x / d of numbers below 2^16, d given as its inverse
+__device__ __forceinline__ int small_div(int x, float inv) { return (int)(((float)x + 0.5f) * inv); }
+
 // ---------------------------------------------------------------------------
 // Append: a workgroup takes a few runs of 8 rows of one head of K or V.  A thread quantises 8 columns of a row, four
 // neighbours a group.  Keys are words then; values meet in LDS, where a thread a column makes a word of
 // 8 rows, with what is there already of rows that are not new.
-// Bound by memory and, for short runs, by the launch.
+// Bound by vector instructions (a quotient by the group's inverse and one correction, which rounds it as a division
+// does: the inverse of an 11-bit number is rounded right by one step from the approximate one, since it lies no nearer than
+// 2^-36 to the middle of two f32 numbers, and from a right inverse the corrected quotient is right).
 // ---------------------------------------------------------------------------
 template <typename T>
 __device__ __forceinline__ void cache4_append(const Cache4Params& p) {
@@ -46,6 +51,7 @@ __device__ __forceinline__ void cache4_append(const Cache4Params& p) {
     __shared__ int fresh[32];
     typedef T run8 __attribute__((ext_vector_type(8)));
     const int tid = threadIdx.x, words = p.d / 8, per = 256 / p.d;   // runs of 8 rows a workgroup
+    const float inv_d = 1.0f / (float)p.d, inv_words = 1.0f / (float)words;
     unsigned id = blockIdx.x;
     const int part = id % p.nparts;
     id /= p.nparts;
@@ -55,139 +61,176 @@ __device__ __forceinline__ void cache4_append(const Cache4Params& p) {
     const int b = id >> 1;
     const int len = p.lens[b];
     if (len < 0) return;
-    const int64_t first = len / 8 + (int64_t)part * per;   // run of 8 rows
     const T* const src = reinterpret_cast<const T*>(isv ? p.v : p.k) + (isv ? b * p.vs.b + h * p.vs.h : b * p.ks.b + h * p.ks.h);
     const int64_t seq = isv ? p.vs.s : p.ks.s;
-
     const bool mine = tid < per * p.d;
-    const int run = tid / p.d, r = tid % p.d / words, word = tid % words;
-    const int64_t row = (first + run) * 8 + r, token = row - len;
-    Place at = {-1, 0};
-    if (mine && token >= 0 && token < p.n) at = cache4_place(p, b, row);
-    float x[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = 0.0f;
-    if (at.block >= 0) {
-        const T* const from = src + token * seq + 8 * word;
-        if (p.vec) {
-            const run8 y = *reinterpret_cast<const run8*>(from);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = float(y[e]);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = float(from[e]);
-        }
-    }
-    float lo = INFINITY, hi = -INFINITY;
-    int bad = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        bad |= not_finite(x[e]);
-        x[e] = fminf(fmaxf(x[e], -kCache4Max), kCache4Max);
-        lo = fminf(lo, x[e]);
-        hi = fmaxf(hi, x[e]);
-    }
-#pragma unroll
-    for (int m = 1; m < 4; m *= 2) {
-        lo = fminf(lo, __shfl_xor(lo, m));
-        hi = fmaxf(hi, __shfl_xor(hi, m));
-        bad |= __shfl_xor(bad, m);
-    }
-    // as the header defines them, each operation rounded once
-    constexpr float kTop = 65504.0f;
-    const _Float16 big = bad ? bits_half(0x7e00) : _Float16(fminf((hi - lo) * 16.0f / 15.0f, kTop));
-    const _Float16 off = bad ? bits_half(0x7e00) : _Float16(fmaxf(lo - float(big), -kTop));
-    const float step = float(big) * 0.0625f;
-    unsigned code[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const float y = rintf((x[e] - float(off)) / step - 16.0f);
-        code[e] = bad || step == 0.0f ? 0u : (unsigned)fminf(fmaxf(y, 0.0f), 15.0f);
-    }
+    const int run = small_div(tid, inv_d), col = tid - run * p.d, r = small_div(col, inv_words), word = col - r * words;
     const int groups = p.d / 32;
-    if (!isv) {
-        if (at.block < 0) return;
-        const int64_t to = (at.block * p.kv_heads + h) * p.block_rows + at.row;
-        unsigned w = 0;
+
+    // what a thread takes of the workgroup's u-th few runs: its place in the cache, and its columns
+    struct Piece {
+        Place at;
+        run8 y;
+    };
+    auto first_of = [&](int u) { return len / 8 + ((int64_t)part * p.loops + u) * per; };
+    auto fetch = [&](Piece& x, int u) {
+        const int64_t row = (first_of(u) + run) * 8 + r, token = row - len;
+        x.at = {-1, 0};
+        x.y = run8{};
+        if (mine && token >= 0 && token < p.n) {
+            x.at = cache4_place(p, b, row);
+            const T* const from = src + token * seq + 8 * word;
+            if (p.vec) {
+                x.y = *reinterpret_cast<const run8*>(from);
+            } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) w |= code[e] << (4 * (e / 2) + 16 * (e % 2));
-        p.k4[to * words + word] = w;
-        if (word % 4 == 0) reinterpret_cast<unsigned*>(p.kscale)[to * groups + word / 4] = half_bits(big) | half_bits(off) << 16;
-        return;
-    }
-    if (tid < per) fresh[tid] = 0;
-    __syncthreads();
-    if (at.block >= 0) {
-        if (word == 0) atomicOr(&fresh[run], 1 << r);
-        u32x2 c = {code[0] | code[1] << 8 | code[2] << 16 | code[3] << 24, code[4] | code[5] << 8 | code[6] << 16 | code[7] << 24};
-        *reinterpret_cast<u32x2*>(codes + (run * 8 + r) * p.d + 8 * word) = c;
-        if (word % 4 == 0) {
-            const int64_t to = (at.block * p.kv_heads + h) * (p.block_rows / 8) + at.row / 8;
-            unsigned short* const s = p.vscale + (to * groups + word / 4) * 16 + r;
-            s[0] = half_bits(big);
-            s[8] = half_bits(off);
+                for (int e = 0; e < 8; ++e) x.y[e] = from[e];
+            }
         }
-    }
-    __syncthreads();
-    const int run2 = tid / p.d, col = tid % p.d;
-    if (!mine || fresh[run2] == 0) return;
-    const Place to = cache4_place(p, b, (first + run2) * 8 + __builtin_ctz(fresh[run2]));
-    if (to.block < 0) return;
-    unsigned* const word8 = p.v4 + ((to.block * p.kv_heads + h) * (p.block_rows / 8) + to.row / 8) * p.d + col;
-    unsigned w = fresh[run2] == 0xff ? 0u : *word8;
+    };
+    auto keep = [&](const Piece& piece, int u) {
+        const Place at = piece.at;
+        float x[8], lo = kCache4Max, hi = -kCache4Max;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const int sh = 4 * (e / 2) + 16 * (e % 2);
-        if (fresh[run2] >> e & 1) w = (w & ~(15u << sh)) | (unsigned)codes[(run2 * 8 + e) * p.d + col] << sh;
+        for (int e = 0; e < 8; ++e) {
+            x[e] = __builtin_amdgcn_fmed3f(float(piece.y[e]), -kCache4Max, kCache4Max);
+            lo = fminf(lo, x[e]);
+            hi = fmaxf(hi, x[e]);
+        }
+        int bad = chunk_special<T>(__builtin_bit_cast(u32x4, piece.y));
+#pragma unroll
+        for (int m = 1; m < 4; m *= 2) {
+            lo = fminf(lo, __shfl_xor(lo, m));
+            hi = fmaxf(hi, __shfl_xor(hi, m));
+            bad |= __shfl_xor(bad, m);
+        }
+        // as the header defines them, each operation rounded once
+        constexpr float kTop = 65504.0f;
+        const _Float16 big = bad ? bits_half(0x7e00) : _Float16(fminf((hi - lo) * 16.0f / 15.0f, kTop));
+        const _Float16 off = bad ? bits_half(0x7e00) : _Float16(fmaxf(lo - float(big), -kTop));
+        const float o = float(off), step = float(big) * 0.0625f;
+        const bool flat = bad || step == 0.0f;
+        const float near = __builtin_amdgcn_rcpf(flat ? 1.0f : step);
+        const float inv = __builtin_fmaf(__builtin_fmaf(-near, flat ? 1.0f : step, 1.0f), near, near);
+        unsigned code[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float a = x[e] - o, q = a * inv, z = __builtin_fmaf(__builtin_fmaf(-q, step, a), inv, q);
+            code[e] = flat ? 0u : (unsigned)__builtin_amdgcn_fmed3f(rintf(z), 16.0f, 31.0f) & 15u;
+        }
+        if (!isv) {
+            if (at.block < 0) return;
+            const int64_t to = (at.block * p.kv_heads + h) * p.block_rows + at.row;
+            unsigned w = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w |= code[e] << (4 * (e / 2) + 16 * (e % 2));
+            p.k4[to * words + word] = w;
+            if (word % 4 == 0)
+                reinterpret_cast<unsigned*>(p.kscale)[to * groups + word / 4] = half_bits(big) | half_bits(off) << 16;
+            return;
+        }
+        __syncthreads();
+        if (tid < per) fresh[tid] = 0;
+        __syncthreads();
+        if (at.block >= 0) {
+            if (word == 0) atomicOr(&fresh[run], 1 << r);
+            u32x2 c = {code[0] | code[1] << 8 | code[2] << 16 | code[3] << 24,
+                       code[4] | code[5] << 8 | code[6] << 16 | code[7] << 24};
+            *reinterpret_cast<u32x2*>(codes + (run * 8 + r) * p.d + 8 * word) = c;
+            if (word % 4 == 0) {
+                const int64_t to = (at.block * p.kv_heads + h) * (p.block_rows / 8) + at.row / 8;
+                unsigned short* const s = p.vscale + (to * groups + word / 4) * 16 + r;
+                s[0] = half_bits(big);
+                s[8] = half_bits(off);
+            }
+        }
+        __syncthreads();
+        const int have = mine ? fresh[run] : 0;
+        if (have == 0) return;
+        const Place to = cache4_place(p, b, (first_of(u) + run) * 8 + __builtin_ctz(have));
+        if (to.block < 0) return;
+        unsigned* const word8 = p.v4 + ((to.block * p.kv_heads + h) * (p.block_rows / 8) + to.row / 8) * p.d + col;
+        unsigned w = have == 0xff ? 0u : *word8;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int sh = 4 * (e / 2) + 16 * (e % 2);
+            if (have >> e & 1) w = (w & ~(15u << sh)) | (unsigned)codes[(run * 8 + e) * p.d + col] << sh;
+        }
+        *word8 = w;
+    };
+    Piece now, next;
+    fetch(now, 0);
+    for (int u = 0; u < p.loops; ++u) {
+        if (u + 1 < p.loops) fetch(next, u + 1);
+        keep(now, u);
+        now = next;
     }
-    *word8 = w;
 }
 
-// Rows of the cache in the type: 8 columns of a row a thread, K and V.
+// Rows of the cache in the type: 8 columns of a row a thread, a head of K or V a workgroup.
 template <typename T>
 __device__ __forceinline__ void cache4_read(const Cache4Params& p) {
     typedef T run8 __attribute__((ext_vector_type(8)));
-    const int words = p.d / 8, groups = p.d / 32;
-    int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int word = id % words;
-    id /= words;
-    const int i = id % p.n;
-    id /= p.n;
+    const int tid = threadIdx.x, words = p.d / 8, groups = p.d / 32, per = 256 / words;   // rows a workgroup
+    unsigned id = blockIdx.x;
+    const int part = id % p.nparts;
+    id /= p.nparts;
     const int h = id % p.kv_heads;
     id /= p.kv_heads;
     const bool isv = id & 1;
     const int b = id >> 1;
-    if (b >= p.batch || !(isv ? p.vo : p.ko)) return;
-    const Place at = cache4_place(p, b, p.rows[(int64_t)b * p.n + i]);
-    run8 y = {};
-    if (at.block >= 0) {
-        const int64_t head = at.block * p.kv_heads + h;
+    const int r = small_div(tid, 1.0f / (float)words), word = tid - r * words;
+    if (r >= per || !(isv ? p.vo : p.ko)) return;
+    constexpr int N = kCache4ReadRows;   // rows of a thread: their loads overlap
+    const int64_t i0 = (int64_t)part * per * N + r;
+    Place at[N];
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+        const int64_t i = i0 + u * per;
+        at[u] = i < p.n ? cache4_place(p, b, p.rows[(int64_t)b * p.n + i]) : Place{-1, 0};
+    }
+    u32x4 w[N][2];
+    unsigned sc[N];   // S and O
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+        w[u][0] = w[u][1] = (u32x4){0, 0, 0, 0};
+        sc[u] = 0;
+        if (at[u].block < 0) continue;
+        const int64_t head = at[u].block * p.kv_heads + h;
         if (!isv) {
-            const int64_t row = head * p.block_rows + at.row;
-            const unsigned w = p.k4[row * words + word];
-            const unsigned s = reinterpret_cast<const unsigned*>(p.kscale)[row * groups + word / 4];
-            const float big = float(bits_half(s & 0xffff)), off = float(bits_half(s >> 16));
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                y[e] = T(__builtin_fmaf(1.0f + (float)(w >> (4 * (e / 2) + 16 * (e % 2)) & 15) * 0.0625f, big, off));
+            const int64_t row = head * p.block_rows + at[u].row;
+            w[u][0][0] = p.k4[row * words + word];
+            sc[u] = reinterpret_cast<const unsigned*>(p.kscale)[row * groups + word / 4];
         } else {
-            const int64_t run = head * (p.block_rows / 8) + at.row / 8;
-            const int r = at.row % 8, sh = 4 * (r / 2) + 16 * (r % 2);
-            const unsigned short* const s = p.vscale + (run * groups + word / 4) * 16 + r;
-            const float big = float(bits_half(s[0])), off = float(bits_half(s[8]));
+            const int64_t run = head * (p.block_rows / 8) + at[u].row / 8;
+            const unsigned short* const s = p.vscale + (run * groups + word / 4) * 16 + at[u].row % 8;
+            sc[u] = s[0] | (unsigned)s[8] << 16;
             const u32x4* const from = reinterpret_cast<const u32x4*>(p.v4 + run * p.d + 8 * word);
-            const u32x4 w[2] = {from[0], from[1]};
-#pragma unroll
-            for (int e = 0; e < 8; ++e) y[e] = T(__builtin_fmaf(1.0f + (float)(w[e / 4][e % 4] >> sh & 15) * 0.0625f, big, off));
+            w[u][0] = from[0];
+            w[u][1] = from[1];
         }
     }
-    T* const to = reinterpret_cast<T*>(isv ? p.vo : p.ko) +
-                  (isv ? b * p.vs.b + h * p.vs.h + i * p.vs.s : b * p.ks.b + h * p.ks.h + i * p.ks.s) + 8 * word;
-    if (p.vec) {
-        *reinterpret_cast<run8*>(to) = y;
-    } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) to[e] = y[e];
+    for (int u = 0; u < N; ++u) {
+        const int64_t i = i0 + u * per;
+        if (i >= p.n) break;
+        const float big = float(bits_half(sc[u] & 0xffff)), off = float(bits_half(sc[u] >> 16));
+        const int e8 = at[u].row % 8, sh = 4 * (e8 / 2) + 16 * (e8 % 2);
+        run8 y;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const unsigned c = isv ? w[u][e / 4][e % 4] >> sh : w[u][0][0] >> (4 * (e / 2) + 16 * (e % 2));
+            // (no such row: 0)
+            y[e] = T(__builtin_fmaf(1.0f + (float)(c & 15) * 0.0625f, big, off));
+        }
+        T* const to = reinterpret_cast<T*>(isv ? p.vo : p.ko) +
+                      (isv ? b * p.vs.b + h * p.vs.h + i * p.vs.s : b * p.ks.b + h * p.ks.h + i * p.ks.s) + 8 * word;
+        if (p.vec) {
+            *reinterpret_cast<run8*>(to) = y;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) to[e] = y[e];
+        }
     }
 }
 

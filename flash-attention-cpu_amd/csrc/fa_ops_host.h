@@ -242,11 +242,12 @@ struct DkvPlan {
     int splits;
     size_t blocks, floats;
 };
-DkvPlan plan_dkv(const fa_score_config& c, int D, bool vec, int num_cus) {
+DkvPlan plan_dkv(const fa_score_config& c, int D, bool vec, int size, int num_cus) {
     DkvPlan r{};
     const size_t nkv = c.batch * c.kv_heads, group = c.heads / c.kv_heads;
     size_t s = 1;
-    while (s < group && (c.seq_len_k + 63) / 64 * nkv * s < 4 * static_cast<size_t>(num_cus)) {
+    // (in a window all are of one length, and one round of them will do)
+    while (s < group && (c.seq_len_k + 63) / 64 * nkv * s < (size ? 2 : 4) * static_cast<size_t>(num_cus)) {
         ++s;
         while (group % s != 0) ++s;
     }
@@ -276,24 +277,26 @@ size_t window_keys(size_t keys, int size, int sinks, size_t n, bool both_sides) 
     return std::min(keys, (both_sides ? 2 : 1) * static_cast<size_t>(size) + sinks + n + 128);
 }
 
-// In a window: key blocks that hold sinks, and the chunks in which other workgroups take the queries that see them from
-// afar; as long as what the other key blocks have, so that none ends late (sinks or not: 2 x 16 / 4 heads x 4096^2,
-// 128 columns, window 512, bf16).
+// In a window: key blocks that hold sinks, and the workgroups that take the queries that see them from afar.  These
+// are shorter than those of the other key blocks, which run first and all end at about the same time: a head of the
+// group each, and two thirds of the stages that a window reaches (2 x 16 / 4 heads x 4096^2, 128 columns, window 512,
+// 64 sinks, bf16: dK and dV).
 struct FarPlan {
-    int stages, chunks, blocks;
+    int stages, chunks, splits, blocks;
     size_t floats;
 };
 FarPlan plan_far(const fa_score_config& c, int D, const DkvPlan& dkv, int size, int sinks) {
     FarPlan r{};
-    if (size == 0 || sinks == 0 || c.seq_len_k == 0) return r;
+    if (size == 0 || sinks == 0 || c.seq_len_k == 0 || c.seq_len_q == 0) return r;
     const size_t step = dkv.tiles.groups == 1 && (c.dtype == FA_DTYPE_F32 || D > 128) ? 32 : 64;   // queries of a stage
     const size_t nst = (c.seq_len_q + step - 1) / step;
     r.blocks = static_cast<int>((std::min<size_t>(sinks, c.seq_len_k) + dkv.tiles.rows - 1) / dkv.tiles.rows);
     const size_t reach = window_keys(c.seq_len_q, size, 0, dkv.tiles.rows, !c.causal || c.prefix) / step + 1;
-    // (a workspace of 2^15 such chunks at most, of the workgroups of ever longer rows)
-    r.stages = static_cast<int>(std::max({reach, size_t(4), nst / 1024 + 1}));
+    // (of very long rows 256 chunks at most)
+    r.stages = static_cast<int>(std::max({2 * reach / 3, size_t(4), nst / 256 + 1}));
     r.chunks = static_cast<int>((nst + r.stages - 1) / r.stages);
-    r.floats = size_t(2) * (r.chunks + 1) * dkv.splits * c.batch * c.kv_heads * r.blocks * dkv.tiles.rows * D;
+    r.splits = static_cast<int>(c.heads / c.kv_heads);
+    r.floats = size_t(2) * (r.chunks * r.splits + 1) * c.batch * c.kv_heads * r.blocks * dkv.tiles.rows * D;
     return r;
 }
 
@@ -668,7 +671,7 @@ int score_backward(void* stream_, const fa_score_config* c, const fa_window* win
                      vec_ok(dout, ldo, d) && ovec_ok(dq, ldq, es) && ovec_ok(dk, ldk, es) && ovec_ok(dv, ldv, es) &&
                      cap_ok(c->dtype, c->softcap);
     OpsWorkspace ws;
-    const DkvPlan dkv = plan_dkv(*c, D, vec, g_dev[dev].num_cus);
+    const DkvPlan dkv = plan_dkv(*c, D, vec, size, g_dev[dev].num_cus);
     ScoreTiles tiles = score_tiles(*c, D, vec, sq, c->batch * c->heads, g_dev[dev].num_cus);
     if (D == 128 && tiles.mt == 2) tiles = {1, 1, 64, ""};   // two tiles' Q, dO and sums leave one wave a SIMD
     const DocPlan docs = plan_docs(*c, tiles.rows, c->heads, dkv.tiles.rows, c->kv_heads * dkv.splits, g_dev[dev].num_cus);
@@ -698,9 +701,9 @@ int score_backward(void* stream_, const fa_score_config* c, const fa_window* win
                       dkv.tiles.tag, mod);
         const size_t slices = c->batch * c->kv_heads, grid = dkv.blocks * slices * dkv.splits;
         p.far_first = static_cast<int>(grid);
-        p.far_stages = far.stages, p.far_chunks = far.chunks, p.far_blocks = far.blocks;
+        p.far_stages = far.stages, p.far_chunks = far.chunks, p.far_splits = far.splits, p.far_blocks = far.blocks;
         p.far_rows = far.blocks * dkv.tiles.rows;
-        rc = ops_launch(dev, module, name, grid + slices * dkv.splits * far.blocks * far.chunks, 256, &p, stream);
+        rc = ops_launch(dev, module, name, grid + slices * far.splits * far.blocks * far.chunks, 256, &p, stream);
         if (rc == FA_OK && (dkv.splits > 1 || far.blocks)) {
             std::snprintf(name, sizeof(name), "fa_score_dkv_sum_%s_d%d%s", dtype_name(c->dtype), D, vec ? "" : "s");
             const size_t threads = slices * (dkv.splits > 1 ? sk : std::min<size_t>(sk, p.far_rows)) * (D / 4);
@@ -1276,12 +1279,17 @@ int fa_cache4_append(void* stream, const fa_kv_cache4* cache, const fa_append_co
     p.n = static_cast<int>(n);
     p.vec = vec_ok(k, lk, d) && vec_ok(v, lv, d);
     const size_t runs = (n + 7) / 8 + 1, per = 256 / d;   // n rows touch that many runs of 8 at most
-    const size_t parts = (runs + per - 1) / per, heads = 2 * cache->batch * cache->kv_heads;
-    if (heads > kOpsMaxGrid / parts) return FA_ERR_UNSUPPORTED;
-    p.nparts = static_cast<int>(parts);
+    const size_t heads = 2 * cache->batch * cache->kv_heads;
     int dev;
     const OpsModule module = cache4_module(cache->dtype, 0);
+    if (heads > kOpsMaxGrid / ((runs + per - 1) / per)) return FA_ERR_UNSUPPORTED;
     if ((rc = ops_begin(&dev, module)) != FA_OK) return rc;
+    // some pieces a workgroup, so that the next is on its way while one is worked on, where that leaves eight a CU
+    size_t loops = 1;
+    while (loops < 8 && heads * (runs / (2 * loops * per)) >= 8 * static_cast<size_t>(g_dev[dev].num_cus)) loops *= 2;
+    const size_t parts = (runs + loops * per - 1) / (loops * per);
+    p.nparts = static_cast<int>(parts);
+    p.loops = static_cast<int>(loops);
     return ops_launch(dev, module, cache->dtype == FA_DTYPE_BF16 ? "fa_cache4_append_bf16" : "fa_cache4_append_f16",
                       heads * parts, 256, &p, static_cast<hipStream_t>(stream));
 } catch (...) {   // no memory for the tables of modules, kernels and workspaces
@@ -1303,18 +1311,19 @@ int fa_cache4_read(void* stream, const fa_kv_cache4* cache, const fa_read_config
         return rc;
     if (!rows) return FA_ERR_INVALID_ARG;
     if (!k_out && !v_out) return FA_OK;
-    const size_t heads = 2 * cache->batch * cache->kv_heads, words = n * (d / 8);
-    if (heads > kOpsMaxGrid * 256 / words) return FA_ERR_UNSUPPORTED;
+    const size_t heads = 2 * cache->batch * cache->kv_heads, per = 256 / (d / 8) * kCache4ReadRows, parts = (n + per - 1) / per;
+    if (heads > kOpsMaxGrid / parts) return FA_ERR_UNSUPPORTED;
     Cache4Params p{};
     fill_cache4(*cache, block_rows, capacity, &p);
     p.ko = k_out, p.vo = v_out, p.ks = lk.st, p.vs = lv.st, p.rows = rows;
     p.n = static_cast<int>(n);
+    p.nparts = static_cast<int>(parts);
     p.vec = vec_ok(k_out, lk, d) && vec_ok(v_out, lv, d);
     int dev;
     const OpsModule module = cache4_module(cache->dtype, 0);
     if ((rc = ops_begin(&dev, module)) != FA_OK) return rc;
     return ops_launch(dev, module, cache->dtype == FA_DTYPE_BF16 ? "fa_cache4_read_bf16" : "fa_cache4_read_f16",
-                      (heads * words + 255) / 256, 256, &p, static_cast<hipStream_t>(stream));
+                      heads * parts, 256, &p, static_cast<hipStream_t>(stream));
 } catch (...) {   // no memory for the tables of modules, kernels and workspaces
     return FA_ERR_ALLOC;
 }

@@ -48,8 +48,9 @@ struct ScoreParams {
     float* part;              // their sums: [dK, dV][split][batch, kv head][key][padded d]
     // dK/dV in a window: workgroups from far_first on take far_stages stages each of the queries that see the first
     // far_blocks key blocks (far_rows rows) as sinks alone
-    int far_first, far_stages, far_chunks, far_blocks, far_rows;
-    float* far_part;          // [dK, dV][chunk + 1][split][batch, kv head][far_rows][padded d]
+    // (shared out over far_chunks chunks of stages and far_splits parts of the group's heads)
+    int far_first, far_stages, far_chunks, far_splits, far_blocks, far_rows;
+    float* far_part;          // [dK, dV][1 + chunk, split][batch, kv head][far_rows][padded d]
     float scale;              // of the scores
     float scale_log2e;
     float cap_in;             // 2 log2(e) scale / softcap: exponent of the cap's tanh
@@ -93,6 +94,8 @@ struct RowsParams {
 constexpr int kRows4Waves = 4;
 // Largest size of a value in such a cache: larger ones count as that, and what codes stand for stays in f16's range.
 constexpr float kCache4Max = 60000.0f;
+// Rows that a thread reads back.
+constexpr int kCache4ReadRows = 2;
 // Append to and rows out of such a cache.
 struct Cache4Params {
     const void *k, *v;        // append
@@ -103,7 +106,8 @@ struct Cache4Params {
     const int32_t *lens, *table, *rows;
     int batch, kv_heads, n, d;
     int capacity, block_rows, page_shift, n_pages, pages_per_seq;
-    int nparts;               // workgroups of a head's rows (append)
+    int nparts;               // workgroups of a head's rows
+    int loops;                // append: how often a workgroup takes 256 / d runs of 8 rows
     int vec;                  // rows of k, v (ko, vo) are aligned
 };
 

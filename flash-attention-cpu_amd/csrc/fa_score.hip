@@ -999,8 +999,8 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
         int id = blockIdx.x - p.far_first;
         chunk = id % p.far_chunks;
         id /= p.far_chunks;
-        w.hq = id % p.splits;
-        id /= p.splits;
+        w.hq = id % p.far_splits;
+        id /= p.far_splits;
         w.blk = id % p.far_blocks;
         id /= p.far_blocks;
         w.hk = id % p.kv_heads;
@@ -1010,7 +1010,7 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
         w = find_work(p.k_order ? blockIdx.x : grid - 1 - blockIdx.x, p.nqb, p.batch * p.kv_heads, p.splits, p.kv_heads,
                       p.k_order);
     }
-    const int count = p.group / p.splits, first = w.hk * p.group + w.hq * count;
+    const int count = p.group / (kWindow && chunk >= 0 ? p.far_splits : p.splits), first = w.hk * p.group + w.hq * count;
     const int kg = wave / NR, qoff = kg * 32 * NCH;   // the wave's queries of a stage
     const int kbeg = w.blk * BK, key0 = kbeg + 16 * MT * (wave % NR);
     const T* K = slice<T>(p.k, p.ks, w.b, w.hk);
@@ -1280,7 +1280,7 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
         }
     }
     // to partial sums where several workgroups share the keys: those of the heads of the group, those of far queries,
-    // and (far chunk 0) a block of sinks that otherwise one workgroup has
+    // and (the first of these sums) a block of sinks that otherwise one workgroup has
     const bool far_sums = kWindow && (chunk >= 0 || (lp.splits == 1 && w.blk < lp.far_blocks));
     if (lp.splits > 1 || far_sums) {
         const int64_t slices = (int64_t)lp.batch * lp.kv_heads, at = (int64_t)w.b * lp.kv_heads + w.hk;
@@ -1288,8 +1288,9 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
         float *outk, *outv;
         if (far_sums) {
             const int64_t per = slices * lp.far_blocks * BK;
-            outk = lp.far_part + (((chunk + 1) * lp.splits + w.hq) * per + at * lp.far_blocks * BK) * D;
-            outv = outk + (lp.far_chunks + 1) * lp.splits * per * D;
+            const int sum = chunk < 0 ? 0 : 1 + chunk * lp.far_splits + w.hq;
+            outk = lp.far_part + (sum * per + at * lp.far_blocks * BK) * D;
+            outv = outk + (lp.far_chunks * lp.far_splits + 1) * per * D;
         } else {
             outk = lp.part + (w.hq * rows + at * lp.sk) * D;
             outv = outk + lp.splits * rows * D;
@@ -1345,9 +1346,9 @@ __device__ __forceinline__ void score_dkv_sum(const ScoreParams& p) {
     if (kWindow && key < far_rows) {
         const int64_t per = (int64_t)p.batch * p.kv_heads * far_rows;
         const float* at = p.far_part + ((int64_t)(b * p.kv_heads + hk) * far_rows + key) * D + col;
-        const int all = (p.far_chunks + 1) * p.splits;
-#pragma unroll 4
-        for (int s = p.splits > 1 ? p.splits : 0; s < all; ++s) {   // (chunk 0 is used without splits only)
+        const int all = p.far_chunks * p.far_splits + 1;
+#pragma unroll 8
+        for (int s = p.splits > 1 ? 1 : 0; s < all; ++s) {   // (the first is there without splits only)
             k += *reinterpret_cast<const f32x4*>(at + s * per * D);
             v += *reinterpret_cast<const f32x4*>(at + (all + s) * per * D);
         }
