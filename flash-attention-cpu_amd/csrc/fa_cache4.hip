@@ -19,16 +19,30 @@ typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
-// Block of memory and row in it of a sequence's row, -1: there is none.
+// A sequence's row among all rows of its head's kind in memory ([blocks, kv_heads, rows]: fewer than 2^32), if there is one.
 struct Place {
-    int64_t block;
-    int row;
+    unsigned at;
+    bool there;
 };
-__device__ __forceinline__ Place cache4_place(const Cache4Params& p, int b, int64_t row) {
-    if (row < 0 || row >= p.capacity) return {-1, 0};
-    if (!p.table) return {b, (int)row};
-    const int page = p.table[(int64_t)b * p.pages_per_seq + (row >> p.page_shift)];
-    return {(unsigned)page < (unsigned)p.n_pages ? page : -1, (int)row & ((1 << p.page_shift) - 1)};
+__device__ __forceinline__ Place cache4_place(const Cache4Params& p, int b, int h, int64_t row) {
+    if (row < 0 || row >= p.capacity) return {0, false};
+    const unsigned head = (unsigned)h * (unsigned)p.block_rows, block = (unsigned)p.kv_heads * (unsigned)p.block_rows;
+    if (!p.table) return {(unsigned)b * block + head + (unsigned)row, true};
+    const int page = p.table[(int64_t)b * p.pages_per_seq + ((int)row >> p.page_shift)];
+    if ((unsigned)page >= (unsigned)p.n_pages) return {0, false};
+    return {(unsigned)page * block + head + ((unsigned)row & ((1u << p.page_shift) - 1)), true};
+}
+
+// The neighbour at lane ^ M, M = 1 or 2
+template <int M, typename V>
+__device__ __forceinline__ V neighbour(V x) {
+    constexpr int kPerm = M == 1 ? 0xb1 : 0x4e;
+    return __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), kPerm, 0xf, 0xf, true));
+}
+// a / b, rounded as a division is, from the inverse of b rounded right
+__device__ __forceinline__ float divided(float a, float b, float inv) {
+    const float q = a * inv;
+    return __builtin_fmaf(__builtin_fmaf(-q, b, a), inv, q);
 }
 
 __device__ __forceinline__ unsigned half_bits(_Float16 x) { return __builtin_bit_cast(unsigned short, x); }
@@ -48,7 +62,8 @@ __device__ __forceinline__ int small_div(int x, float inv) { return (int)(((floa
 template <typename T>
 __device__ __forceinline__ void cache4_append(const Cache4Params& p) {
     __shared__ __attribute__((aligned(16))) unsigned char codes[256 * 8];   // [run][8 rows][d]
-    __shared__ int fresh[32];
+    __shared__ int fresh[8];       // rows of a run that are new
+    __shared__ unsigned where[8];   // and its place among the runs in memory
     typedef T run8 __attribute__((ext_vector_type(8)));
     const int tid = threadIdx.x, words = p.d / 8, per = 256 / p.d;   // runs of 8 rows a workgroup
     const float inv_d = 1.0f / (float)p.d, inv_words = 1.0f / (float)words;
@@ -65,7 +80,7 @@ __device__ __forceinline__ void cache4_append(const Cache4Params& p) {
     const int64_t seq = isv ? p.vs.s : p.ks.s;
     const bool mine = tid < per * p.d;
     const int run = small_div(tid, inv_d), col = tid - run * p.d, r = small_div(col, inv_words), word = col - r * words;
-    const int groups = p.d / 32;
+    const int groups = words / 4;
 
     // what a thread takes of the workgroup's u-th few runs: its place in the cache, and its columns
     struct Piece {
@@ -75,10 +90,10 @@ __device__ __forceinline__ void cache4_append(const Cache4Params& p) {
     auto first_of = [&](int u) { return len / 8 + ((int64_t)part * p.loops + u) * per; };
     auto fetch = [&](Piece& x, int u) {
         const int64_t row = (first_of(u) + run) * 8 + r, token = row - len;
-        x.at = {-1, 0};
+        x.at = {0, false};
         x.y = run8{};
         if (mine && token >= 0 && token < p.n) {
-            x.at = cache4_place(p, b, row);
+            x.at = cache4_place(p, b, h, row);
             const T* const from = src + token * seq + 8 * word;
             if (p.vec) {
                 x.y = *reinterpret_cast<const run8*>(from);
@@ -90,56 +105,64 @@ __device__ __forceinline__ void cache4_append(const Cache4Params& p) {
     };
     auto keep = [&](const Piece& piece, int u) {
         const Place at = piece.at;
-        float x[8], lo = kCache4Max, hi = -kCache4Max;
+        float x[8], lo = INFINITY, hi = -INFINITY;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            x[e] = __builtin_amdgcn_fmed3f(float(piece.y[e]), -kCache4Max, kCache4Max);
+            x[e] = float(piece.y[e]);
             lo = fminf(lo, x[e]);
             hi = fmaxf(hi, x[e]);
         }
         int bad = chunk_special<T>(__builtin_bit_cast(u32x4, piece.y));
+        lo = fminf(lo, neighbour<1>(lo));
+        hi = fmaxf(hi, neighbour<1>(hi));
+        bad |= neighbour<1>(bad);
+        lo = fminf(lo, neighbour<2>(lo));
+        hi = fmaxf(hi, neighbour<2>(hi));
+        bad |= neighbour<2>(bad);
+        if (__builtin_amdgcn_ballot_w64(lo < -kCache4Max || hi > kCache4Max) != 0) {
+            lo = __builtin_amdgcn_fmed3f(lo, -kCache4Max, kCache4Max);
+            hi = __builtin_amdgcn_fmed3f(hi, -kCache4Max, kCache4Max);
 #pragma unroll
-        for (int m = 1; m < 4; m *= 2) {
-            lo = fminf(lo, __shfl_xor(lo, m));
-            hi = fmaxf(hi, __shfl_xor(hi, m));
-            bad |= __shfl_xor(bad, m);
+            for (int e = 0; e < 8; ++e) x[e] = __builtin_amdgcn_fmed3f(x[e], -kCache4Max, kCache4Max);
         }
         // as the header defines them, each operation rounded once
         constexpr float kTop = 65504.0f;
-        const _Float16 big = bad ? bits_half(0x7e00) : _Float16(fminf((hi - lo) * 16.0f / 15.0f, kTop));
+        const float size = fminf(divided((hi - lo) * 16.0f, 15.0f, 1.0f / 15.0f), kTop);
+        const _Float16 big = bad ? bits_half(0x7e00) : _Float16(size);
         const _Float16 off = bad ? bits_half(0x7e00) : _Float16(fmaxf(lo - float(big), -kTop));
-        const float o = float(off), step = float(big) * 0.0625f;
-        const bool flat = bad || step == 0.0f;
-        const float near = __builtin_amdgcn_rcpf(flat ? 1.0f : step);
-        const float inv = __builtin_fmaf(__builtin_fmaf(-near, flat ? 1.0f : step, 1.0f), near, near);
-        unsigned code[8];
+        const float o = bad ? 0.0f : float(off), step = bad ? 0.0f : float(big) * 0.0625f;
+        const float near = __builtin_amdgcn_rcpf(step);
+        // (no step: an inverse of 0 gives codes of 0)
+        const float inv = step == 0.0f ? 0.0f : __builtin_fmaf(__builtin_fmaf(-near, step, 1.0f), near, near);
+        // Codes plus 16 as bytes, rounded to even: entries 0, 4, 1, 5 of the word's, and 2, 6, 3, 7.
+        unsigned even = 0, odd = 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const float a = x[e] - o, q = a * inv, z = __builtin_fmaf(__builtin_fmaf(-q, step, a), inv, q);
-            code[e] = flat ? 0u : (unsigned)__builtin_amdgcn_fmed3f(rintf(z), 16.0f, 31.0f) & 15u;
+            const float z = __builtin_amdgcn_fmed3f(divided(x[e] - o, step, inv), 16.0f, 31.0f);
+            unsigned& to = e / 2 % 2 == 0 ? even : odd;
+            to = __builtin_amdgcn_cvt_pk_u8_f32(z, e / 4 + 2 * (e % 2), to);
         }
+        even &= 0x0f0f0f0fu;
+        odd &= 0x0f0f0f0fu;
         if (!isv) {
-            if (at.block < 0) return;
-            const int64_t to = (at.block * p.kv_heads + h) * p.block_rows + at.row;
-            unsigned w = 0;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) w |= code[e] << (4 * (e / 2) + 16 * (e % 2));
-            p.k4[to * words + word] = w;
+            if (!at.there) return;
+            p.k4[(uint64_t)at.at * (unsigned)words + (unsigned)word] = even | odd << 4;
             if (word % 4 == 0)
-                reinterpret_cast<unsigned*>(p.kscale)[to * groups + word / 4] = half_bits(big) | half_bits(off) << 16;
+                reinterpret_cast<unsigned*>(p.kscale)[(uint64_t)at.at * (unsigned)groups + (unsigned)word / 4] =
+                    half_bits(big) | half_bits(off) << 16;
             return;
         }
         __syncthreads();
         if (tid < per) fresh[tid] = 0;
         __syncthreads();
-        if (at.block >= 0) {
-            if (word == 0) atomicOr(&fresh[run], 1 << r);
-            u32x2 c = {code[0] | code[1] << 8 | code[2] << 16 | code[3] << 24,
-                       code[4] | code[5] << 8 | code[6] << 16 | code[7] << 24};
-            *reinterpret_cast<u32x2*>(codes + (run * 8 + r) * p.d + 8 * word) = c;
+        if (at.there) {
+            if (word == 0) {
+                atomicOr(&fresh[run], 1 << r);
+                where[run] = at.at >> 3;   // (all rows of a run lie in one page)
+            }
+            *reinterpret_cast<u32x2*>(codes + (run * 8 + r) * p.d + 8 * word) = (u32x2){even, odd};
             if (word % 4 == 0) {
-                const int64_t to = (at.block * p.kv_heads + h) * (p.block_rows / 8) + at.row / 8;
-                unsigned short* const s = p.vscale + (to * groups + word / 4) * 16 + r;
+                unsigned short* const s = p.vscale + ((uint64_t)(at.at >> 3) * (unsigned)groups + (unsigned)word / 4) * 16 + r;
                 s[0] = half_bits(big);
                 s[8] = half_bits(off);
             }
@@ -147,23 +170,28 @@ __device__ __forceinline__ void cache4_append(const Cache4Params& p) {
         __syncthreads();
         const int have = mine ? fresh[run] : 0;
         if (have == 0) return;
-        const Place to = cache4_place(p, b, (first_of(u) + run) * 8 + __builtin_ctz(have));
-        if (to.block < 0) return;
-        unsigned* const word8 = p.v4 + ((to.block * p.kv_heads + h) * (p.block_rows / 8) + to.row / 8) * p.d + col;
+        const int byte = (col & ~7) + (col / 2 % 2) * 4 + (col / 4 % 2) + 2 * (col % 2);   // of the column's codes
+        unsigned* const word8 = p.v4 + (uint64_t)where[run] * (unsigned)p.d + (unsigned)col;
         unsigned w = have == 0xff ? 0u : *word8;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const int sh = 4 * (e / 2) + 16 * (e % 2);
-            if (have >> e & 1) w = (w & ~(15u << sh)) | (unsigned)codes[(run * 8 + e) * p.d + col] << sh;
+            const unsigned c = (unsigned)codes[(run * 8 + e) * p.d + byte] << sh, keep = ~(15u << sh);
+            if (have >> e & 1) w = (w & keep) | c;
         }
         *word8 = w;
     };
-    Piece now, next;
+    // three pieces on their way while one is worked on
+    Piece now, second, third, last;
     fetch(now, 0);
+    if (p.loops > 1) fetch(second, 1);
+    if (p.loops > 2) fetch(third, 2);
     for (int u = 0; u < p.loops; ++u) {
-        if (u + 1 < p.loops) fetch(next, u + 1);
+        if (u + 3 < p.loops) fetch(last, u + 3);
         keep(now, u);
-        now = next;
+        now = second;
+        second = third;
+        third = last;
     }
 }
 
@@ -181,13 +209,13 @@ __device__ __forceinline__ void cache4_read(const Cache4Params& p) {
     const int b = id >> 1;
     const int r = small_div(tid, 1.0f / (float)words), word = tid - r * words;
     if (r >= per || !(isv ? p.vo : p.ko)) return;
-    constexpr int N = kCache4ReadRows;   // rows of a thread: their loads overlap
+    constexpr int N = kCache4ReadRows;   // rows of a thread, whose loads overlap
     const int64_t i0 = (int64_t)part * per * N + r;
     Place at[N];
 #pragma unroll
     for (int u = 0; u < N; ++u) {
         const int64_t i = i0 + u * per;
-        at[u] = i < p.n ? cache4_place(p, b, p.rows[(int64_t)b * p.n + i]) : Place{-1, 0};
+        at[u] = i < p.n ? cache4_place(p, b, h, p.rows[(int64_t)b * p.n + i]) : Place{0, false};
     }
     u32x4 w[N][2];
     unsigned sc[N];   // S and O
@@ -195,17 +223,16 @@ __device__ __forceinline__ void cache4_read(const Cache4Params& p) {
     for (int u = 0; u < N; ++u) {
         w[u][0] = w[u][1] = (u32x4){0, 0, 0, 0};
         sc[u] = 0;
-        if (at[u].block < 0) continue;
-        const int64_t head = at[u].block * p.kv_heads + h;
+        if (!at[u].there) continue;
         if (!isv) {
-            const int64_t row = head * p.block_rows + at[u].row;
-            w[u][0][0] = p.k4[row * words + word];
-            sc[u] = reinterpret_cast<const unsigned*>(p.kscale)[row * groups + word / 4];
+            w[u][0][0] = p.k4[(uint64_t)at[u].at * (unsigned)words + (unsigned)word];
+            sc[u] = reinterpret_cast<const unsigned*>(p.kscale)[(uint64_t)at[u].at * (unsigned)groups + (unsigned)word / 4];
         } else {
-            const int64_t run = head * (p.block_rows / 8) + at[u].row / 8;
-            const unsigned short* const s = p.vscale + (run * groups + word / 4) * 16 + at[u].row % 8;
+            const unsigned run = at[u].at >> 3;
+            const unsigned short* const s =
+                p.vscale + ((uint64_t)run * (unsigned)groups + (unsigned)word / 4) * 16 + (at[u].at & 7);
             sc[u] = s[0] | (unsigned)s[8] << 16;
-            const u32x4* const from = reinterpret_cast<const u32x4*>(p.v4 + run * p.d + 8 * word);
+            const u32x4* const from = reinterpret_cast<const u32x4*>(p.v4 + (uint64_t)run * (unsigned)p.d + 8 * word);
             w[u][0] = from[0];
             w[u][1] = from[1];
         }
@@ -215,7 +242,7 @@ __device__ __forceinline__ void cache4_read(const Cache4Params& p) {
         const int64_t i = i0 + u * per;
         if (i >= p.n) break;
         const float big = float(bits_half(sc[u] & 0xffff)), off = float(bits_half(sc[u] >> 16));
-        const int e8 = at[u].row % 8, sh = 4 * (e8 / 2) + 16 * (e8 % 2);
+        const int e8 = at[u].at & 7, sh = 4 * (e8 / 2) + 16 * (e8 % 2);
         run8 y;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {

@@ -861,6 +861,9 @@ int check_cache4(const fa_kv_cache4* c, size_t* block_rows, size_t* capacity) {
         *block_rows = *capacity = c->capacity;
     }
     if (*capacity > kOpsMaxSeq) return FA_ERR_UNSUPPORTED;
+    // rows of all heads are numbered in 32 bits (2^32 of 64 columns have 172 GB)
+    const size_t heads = (c->block_table ? c->n_pages : c->batch) * c->kv_heads;
+    if (*block_rows > 0 && heads >= (size_t(1) << 32) / *block_rows) return FA_ERR_UNSUPPORTED;
     if (*capacity > 0 && (!c->k || !c->v || !c->k_scale || !c->v_scale)) return FA_ERR_INVALID_ARG;
     // the kernels load words of it, 16 bytes at a time
     if (!aligned16(c->k) || !aligned16(c->v) || !aligned16(c->k_scale) || !aligned16(c->v_scale)) return FA_ERR_INVALID_ARG;
@@ -1284,9 +1287,10 @@ int fa_cache4_append(void* stream, const fa_kv_cache4* cache, const fa_append_co
     const OpsModule module = cache4_module(cache->dtype, 0);
     if (heads > kOpsMaxGrid / ((runs + per - 1) / per)) return FA_ERR_UNSUPPORTED;
     if ((rc = ops_begin(&dev, module)) != FA_OK) return rc;
-    // some pieces a workgroup, so that the next is on its way while one is worked on, where that leaves eight a CU
-    size_t loops = 1;
-    while (loops < 8 && heads * (runs / (2 * loops * per)) >= 8 * static_cast<size_t>(g_dev[dev].num_cus)) loops *= 2;
+    // pieces enough a workgroup that all run at once, eight a CU: a last round of few costs as much as a full one (4 x 2048
+    // rows of 8 heads of 128 columns, 64 workgroups of 2112 in a second round: 20 us)
+    const size_t resident = 8 * static_cast<size_t>(g_dev[dev].num_cus), pieces = heads * ((runs + per - 1) / per);
+    const size_t loops = std::min<size_t>(16, (pieces + resident - 1) / resident);
     const size_t parts = (runs + loops * per - 1) / (loops * per);
     p.nparts = static_cast<int>(parts);
     p.loops = static_cast<int>(loops);

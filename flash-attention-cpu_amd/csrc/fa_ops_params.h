@@ -95,7 +95,7 @@ constexpr int kRows4Waves = 4;
 // Largest size of a value in such a cache: larger ones count as that, and what codes stand for stays in f16's range.
 constexpr float kCache4Max = 60000.0f;
 // Rows that a thread reads back.
-constexpr int kCache4ReadRows = 2;
+constexpr int kCache4ReadRows = 4;
 // Append to and rows out of such a cache.
 struct Cache4Params {
     const void *k, *v;        // append
