@@ -818,11 +818,11 @@ int plan_norm(int dev, int dtype, bool wide, NormParams* p, const char** kind, s
     for (int i = 0; i < p->nt; ++i) {
         NormTensor& t = p->t[i];
         // some four rows a slot, so that the next is on its way while one is worked on, where that leaves two workgroups a
-        // CU; a row for each slot where it leaves one
+        // CU, all tensors together; a row for each slot where it leaves one
         size_t tokens = 1;
         const size_t cus = static_cast<size_t>(g_dev[dev].num_cus);
         while (tokens < kNormTokens && tokens * t.heads < 4 * slots &&
-               all / (2 * tokens) >= (tokens * t.heads < slots ? 1 : 2) * cus)
+               all * p->nt / (2 * tokens) >= (tokens * t.heads < slots ? 1 : 2) * cus)
             tokens *= 2;
         t.tokens = static_cast<int>(tokens);
         const size_t blocks = (all + tokens - 1) / tokens;
