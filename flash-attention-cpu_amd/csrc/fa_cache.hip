@@ -213,11 +213,13 @@ struct RowTiles {
 #pragma unroll
             for (int dc = 0; dc < NDC; ++dc)
                 q[t][dc] = global_row<T, VEC>(from, p.qs.s, token[t], real ? p.n : 0, 32 * dc + 8 * g, p.d);
-            const RowToken row = row_token(p, w, token[t]);
-            pos[t] = row.pos;
-            qd[t] = row.doc;
-            word[t] = row.word;
+            pos[t] = !w.tree ? p.q_start + token[t] : p.pos ? p.pos[w.b * p.n + token[t]] : w.len + token[t];
+            qd[t] = w.docs ? p.q_doc[(int64_t)w.b * p.n + token[t]] : 0;
             slope[t] = has_bias<MOD>(p) ? p.slopes[h] * kLog2e : 0.0f;
+            word[t] = 0;
+            if (w.tree)
+                word[t] = p.mask ? p.mask[((p.mask_shared ? 0 : (int64_t)w.b * p.n) + token[t]) * p.mask_words]
+                                 : token[t] < 63 ? (2ull << token[t]) - 1 : ~0ull;
 #pragma unroll
             for (int j = 0; j < NDB; ++j) o[t][j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
             m[t] = OPS_NEG_INF;
@@ -286,15 +288,14 @@ struct RowTiles {
         if (masked) {
             // keys k0 .. k0 + 16 KB - 1 as bits
             const RowsParams lp = late_params<RowsParams>();
-            const uint64_t there = keys_there(lp, w, k0, 16 * g + li, badpage);
+            const uint64_t there = keys_there(lp, w, k0, badpage);
             uint64_t see[MT];
 #pragma unroll
-            for (int t = 0; t < MT; ++t) see[t] = there & seen_bits(lp, w, {token[t], pos[t], qd[t], word[t]}, k0);
+            for (int t = 0; t < MT; ++t) see[t] = there & seen_bits(lp, w, t, k0);
             if constexpr (kWindow) {
 #pragma unroll
                 for (int t = 0; t < MT; ++t)
-                    see[t] &= window_bits<16 * KB>(lp, w, {token[t], pos[t], qd[t], word[t]}, k0,
-                                                   [&](int b, int r) { return 16 * b + 4 * g + r; });
+                    see[t] &= window_bits<16 * KB>(lp, w, pos[t], k0, [&](int b, int r) { return 16 * b + 4 * g + r; });
             }
             if (w.docs) {
 #pragma unroll
@@ -318,6 +319,33 @@ struct RowTiles {
                         if (!(bits & (1u << r))) s[t][b][r] = OPS_NEG_INF;
                 }
         }
+    }
+    // Bits of the keys that exist: before the run's end, in good pages (one lane a key).
+    __device__ __forceinline__ uint64_t keys_there(const RowsParams& p, const RowsWork& w, int k0, int badpage) const {
+        const int lane = 16 * g + li, key = k0 + lane;
+        if (!badpage) return w.kend - k0 >= 64 ? ~0ull : (1ull << (w.kend - k0)) - 1;
+        const CachePages pages = rows_pages(p, w.b);
+        return __builtin_amdgcn_ballot_w64(key < w.kend && pages.at(key, w.kend, 0, 0) >= 0);
+    }
+    // Bits of the keys that the lane's row of tile t sees, as far as causal, prefix and tree tell.
+    __device__ __forceinline__ uint64_t seen_bits(const RowsParams& p, const RowsWork& w, int t, int k0) const {
+        if (!w.tree) {
+            const int n = (w.docs && qd[t] < 0 ? 0 : p.causal ? max(p.q_start + token[t] + 1, w.prefix) : 0x7fffffff) - k0;
+            return n >= 64 ? ~0ull : (1ull << max(n, 0)) - 1;
+        }
+        const int rel = k0 - w.len;   // the first key's number among the drafted ones
+        if (rel <= -64) return ~0ull;
+        if (rel < 0) return (mask_word(p, w, t, 0) << -rel) | ((1ull << -rel) - 1);
+        const int i = rel >> 6, sh = rel & 63;
+        const uint64_t lo = mask_word(p, w, t, i) >> sh;
+        return sh == 0 ? lo : lo | (mask_word(p, w, t, i + 1) << (64 - sh));
+    }
+    __device__ __forceinline__ uint64_t mask_word(const RowsParams& p, const RowsWork& w, int t, int i) const {
+        if (i == 0) return word[t];
+        if (i >= p.mask_words) return 0;
+        if (p.mask) return p.mask[((p.mask_shared ? 0 : (int64_t)w.b * p.n) + token[t]) * p.mask_words + i];
+        const int n = token[t] + 1 - 64 * i;   // a chain
+        return n >= 64 ? ~0ull : (1ull << max(n, 0)) - 1;
     }
     // the reference of a row moves only when a score passes it by more than kLazy, or at its first key
     __device__ __forceinline__ void softmax() {
@@ -469,7 +497,7 @@ __device__ __forceinline__ void rows_stream(const RowsParams& p) {
     const T* const V = reinterpret_cast<const T*>(p.v) + w.hk * p.vs.h + (p.table ? 0 : w.b * p.vs.b);
     const Src ksrc(K, p.ks.s, p.ks.b, p.d, 0, lane), vsrc(V, p.vs.s, p.vs.b, p.d, 0, lane);
     const int k_first = SK * wave;   // of the walked keys
-    const int nblk = k_first < w.kwalk ? (w.kwalk - k_first + SK * NW - 1) / (SK * NW) : 0;
+    const int nblk = k_first < w.kwalk() ? (w.kwalk() - k_first + SK * NW - 1) / (SK * NW) : 0;
     static_assert(VEC, "DMA only");
 
     bool special = false;
@@ -599,7 +627,7 @@ __device__ __forceinline__ void rows_shared(const RowsParams& p) {
     const T* const K = reinterpret_cast<const T*>(p.k) + w.hk * p.ks.h + (p.table ? 0 : w.b * p.ks.b);
     const T* const V = reinterpret_cast<const T*>(p.v) + w.hk * p.vs.h + (p.table ? 0 : w.b * p.vs.b);
     const Src ksrc(K, p.ks.s, p.ks.b, p.d, wave, lane), vsrc(V, p.vs.s, p.vs.b, p.d, wave, lane);
-    const int nst = (w.kwalk + SK - 1) / SK;
+    const int nst = (w.kwalk() + SK - 1) / SK;
     const int rfirst = w.rfirst + 16 * MT * wave;
     const int act = rfirst < w.nrows;
 

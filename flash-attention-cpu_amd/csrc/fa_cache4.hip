@@ -327,7 +327,7 @@ __device__ __forceinline__ void rows4(const RowsParams& p) {
     const unsigned* const KS = reinterpret_cast<const unsigned*>(p.k_scale);
     const unsigned* const V = reinterpret_cast<const unsigned*>(p.v);
     const unsigned* const VS = reinterpret_cast<const unsigned*>(p.v_scale);
-    const int nblk = SK * wave < w.kwalk ? (w.kwalk - SK * wave + SK * NW - 1) / (SK * NW) : 0;
+    const int nblk = SK * wave < w.kwalk() ? (w.kwalk() - SK * wave + SK * NW - 1) / (SK * NW) : 0;
     auto key_of = [&](int i) { return w.key(SK * wave + i * SK * NW); };   // first key of the wave's i-th block
 
     // byte offsets of the lane's loads in a block of 32 rows
@@ -470,7 +470,7 @@ __device__ __forceinline__ void rows4(const RowsParams& p) {
         const int r = w.rfirst + 16 * t + li;
         const bool real = r < w.nrows;
         const int token = real ? r / p.group : 0, h = w.hk * p.group + (real ? r % p.group : 0);
-        tok[t] = row_token(p, w, token);
+        tok[t] = {token, token_position(p, w, token), 0, first_word(p, w, token)};
         slope[t] = has_bias<MOD>(p) ? p.slopes[h] * kLog2e : 0.0f;
         const T* const from = reinterpret_cast<const T*>(p.q) + w.b * p.qs.b + h * p.qs.h + token * p.qs.s;
         typename Mma<T>::v8 x[NDC];
@@ -577,7 +577,7 @@ __device__ __forceinline__ void rows4(const RowsParams& p) {
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
                 uint64_t see = there & seen_bits(lp, w, tok[t], k0);
-                if constexpr (kWindow) see &= window_bits<SK>(lp, w, tok[t], k0, [&](int b, int r) { return 8 * g + 4 * b + r; });
+                if constexpr (kWindow) see &= window_bits<SK>(lp, w, tok[t].pos, k0, [&](int b, int r) { return 8 * g + 4 * b + r; });
                 const unsigned bits = (unsigned)(see >> (8 * g));
 #pragma unroll
                 for (int b = 0; b < 2; ++b)

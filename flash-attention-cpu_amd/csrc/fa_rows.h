@@ -34,16 +34,16 @@ struct RowsWork {
     int run, rb, b, hk;
     int runs;   // of the sequence
     int len, prefix, open, kbeg, kend, nrows, rfirst;
-    int kwalk;        // keys to walk, from kbeg on, without those that are left out
-    int gap, skip;    // keys from `gap` on are left out, `skip` of them
+    int kfirst, gap, skip;   // windows: kbeg among the keys that are walked; keys from `gap` on are left out, `skip` of them
     int low;          // a window's: keys before this and not before p.sinks are hidden from some row
     int tree, docs;
-    // the key that stands `i` behind kbeg (a multiple of 16) among those walked
+    // how many keys are walked, and the one that stands `i` behind kbeg (a multiple of 16) among them
+    __device__ __forceinline__ int kwalk() const { return kend - kbeg - (kWindow && kbeg < gap && kend > gap ? skip : 0); }
     __device__ __forceinline__ int key(int i) const {
+        if (!kWindow) return kbeg + i;
         const int k = kfirst + i;
-        return kWindow ? k + (k >= gap ? skip : 0) : k;
+        return k + (k >= gap ? skip : 0);
     }
-    int kfirst;       // kbeg among those walked
 };
 
 // Keys that any query of sequence b sees: those before `total`, without `skip` ones from `gap` on where a window
@@ -53,7 +53,7 @@ struct Walk {
     __device__ __forceinline__ int walked() const { return total - skip; }
 };
 __device__ __forceinline__ Walk rows_walk(const RowsParams& p, int b) {
-    Walk w = {0, 0x7fffffff, 0};
+    Walk w = {0, 0, 0};
     int first;   // position of the first query
     if (p.lens) {
         const int len = p.lens[b];
@@ -184,7 +184,6 @@ __device__ __forceinline__ bool rows_work(const RowsParams& p, int rows, int lan
     } else {
         w.open = w.docs ? 0 : p.causal ? max(p.q_start + 1, w.prefix) : p.sk;
     }
-    w.low = INT32_MIN;
     if (kWindow) {
         int last = p.q_start + p.n - 1;   // position of the last query
         if (w.tree) {
@@ -199,17 +198,21 @@ __device__ __forceinline__ bool rows_work(const RowsParams& p, int rows, int lan
         w.low = last - p.window + 1;
     }
     const Walk walk = rows_walk(p, w.b);
-    w.gap = __builtin_amdgcn_readfirstlane(walk.gap);
-    w.skip = __builtin_amdgcn_readfirstlane(walk.skip);
+    if (kWindow) {
+        w.gap = __builtin_amdgcn_readfirstlane(walk.gap);
+        w.skip = __builtin_amdgcn_readfirstlane(walk.skip);
+    }
     const int total = __builtin_amdgcn_readfirstlane(walk.walked());
     int64_t per = (int64_t)__builtin_amdgcn_readfirstlane(r.steps) * p.step;
     // a sequence's runs of one length, rather than all but its last
     if (kEvenRuns) per = (int64_t)((total + p.step * w.runs - 1) / (p.step * w.runs)) * p.step;
-    w.kfirst = (int)min((w.run - __builtin_amdgcn_readfirstlane(r.first)) * per, (int64_t)total);
-    const int last = (int)min(w.kfirst + per, (int64_t)total);
-    w.kwalk = last - w.kfirst;
-    w.kbeg = w.key(0);
-    w.kend = kWindow ? last + (last > w.gap ? w.skip : 0) : last;
+    w.kbeg = (int)min((w.run - __builtin_amdgcn_readfirstlane(r.first)) * per, (int64_t)total);
+    w.kend = (int)min(w.kbeg + per, (int64_t)total);
+    if (kWindow) {
+        w.kfirst = w.kbeg;
+        w.kbeg = w.key(0);
+        w.kend += w.kend > w.gap ? w.skip : 0;
+    }
     w.nrows = p.n * p.group;
     w.rfirst = w.rb * rows;
     return true;
@@ -249,21 +252,18 @@ __device__ __forceinline__ bool rows_see(const RowsParams& p, const RowsWork& w,
     return (p.mask[row * p.mask_words + (bit >> 6)] >> (bit & 63)) & 1;
 }
 
-// A row's token: its number, position, document, and first mask word.
+// A row's token: its number, position, document, and first mask word.  (RowTiles has the following as members: through
+// these its kernels take 3 % longer, 176 us instead of 171 for 8 trees of 64 tokens over up to 16384 rows.)
 struct RowToken {
     int token, pos, doc;
     uint64_t word;
 };
-__device__ __forceinline__ RowToken row_token(const RowsParams& p, const RowsWork& w, int token) {
-    RowToken r;
-    r.token = token;
-    r.pos = !w.tree ? p.q_start + token : p.pos ? p.pos[w.b * p.n + token] : w.len + token;
-    r.doc = w.docs ? p.q_doc[(int64_t)w.b * p.n + token] : 0;
-    r.word = 0;
-    if (w.tree)
-        r.word = p.mask ? p.mask[((p.mask_shared ? 0 : (int64_t)w.b * p.n) + token) * p.mask_words]
-                        : token < 63 ? (2ull << token) - 1 : ~0ull;
-    return r;
+__device__ __forceinline__ int token_position(const RowsParams& p, const RowsWork& w, int token) {
+    return !w.tree ? p.q_start + token : p.pos ? p.pos[w.b * p.n + token] : w.len + token;
+}
+__device__ __forceinline__ uint64_t first_word(const RowsParams& p, const RowsWork& w, int token) {
+    if (p.mask) return p.mask[((p.mask_shared ? 0 : (int64_t)w.b * p.n) + token) * p.mask_words];
+    return token < 63 ? (2ull << token) - 1 : ~0ull;
 }
 __device__ __forceinline__ uint64_t bits_before(int n) { return n >= 64 ? ~0ull : (1ull << max(n, 0)) - 1; }
 
@@ -294,8 +294,8 @@ __device__ __forceinline__ uint64_t seen_bits(const RowsParams& p, const RowsWor
 // Those of the N keys that the window leaves a row; drafted keys that stand where the program says: of the keys
 // at(b, r), b < N / 16, whose scores the lane holds.
 template <int N, typename At>
-__device__ __forceinline__ uint64_t window_bits(const RowsParams& p, const RowsWork& w, const RowToken& row, int k0, At at_) {
-    const int at = w.tree ? min(max(row.pos, w.len), kWindowMaxPos) : row.pos;
+__device__ __forceinline__ uint64_t window_bits(const RowsParams& p, const RowsWork& w, int pos, int k0, At at_) {
+    const int at = w.tree ? min(max(pos, w.len), kWindowMaxPos) : pos;
     uint64_t bits = ~bits_before(at - p.window + 1 - k0);
     if (!w.tree) bits &= bits_before(at + p.window - k0);
     bits |= bits_before(p.sinks - k0);
