@@ -282,6 +282,40 @@ __device__ __forceinline__ h8 dequant(unsigned w, unsigned one, B big, O off) {
     return v;
 }
 
+// A row's token: its number, position and first mask word.  (The following are what RowTiles of fa_cache.hip has as members,
+// for trees alone; its kernels take 3 % longer through functions like these: 176 us instead of 171 for 8 trees of 64
+// tokens over up to 16384 rows.)
+struct RowToken {
+    int token, pos;
+    uint64_t word;
+};
+__device__ __forceinline__ RowToken row_token(const RowsParams& p, const RowsWork& w, int token) {
+    const int64_t at = (int64_t)w.b * p.n + token;
+    return {token, p.pos ? p.pos[at] : w.len + token,
+            p.mask ? p.mask[(p.mask_shared ? token : at) * p.mask_words] : bits_before(token + 1)};
+}
+__device__ __forceinline__ uint64_t mask_word(const RowsParams& p, const RowsWork& w, const RowToken& r, int i) {
+    if (i == 0) return r.word;
+    if (i >= p.mask_words) return 0;
+    if (p.mask) return p.mask[((p.mask_shared ? 0 : (int64_t)w.b * p.n) + r.token) * p.mask_words + i];
+    return bits_before(r.token + 1 - 64 * i);   // a chain
+}
+// Bits of the keys from k0 that the row sees, as far as the tree tells.
+__device__ __forceinline__ uint64_t seen_bits(const RowsParams& p, const RowsWork& w, const RowToken& r, int k0) {
+    const int rel = k0 - w.len;   // the first key's number among the drafted ones
+    if (rel <= -64) return ~0ull;
+    if (rel < 0) return (mask_word(p, w, r, 0) << -rel) | ((1ull << -rel) - 1);
+    const int i = rel >> 6, sh = rel & 63;
+    const uint64_t lo = mask_word(p, w, r, i) >> sh;
+    return sh == 0 ? lo : lo | (mask_word(p, w, r, i + 1) << (64 - sh));
+}
+// Bits of the 32 keys from k0 that exist: before the run's end, in good pages (one lane a key).
+__device__ __forceinline__ uint64_t keys_there(const RowsParams& p, const RowsWork& w, int k0, int lane, int badpage) {
+    if (!badpage) return bits_before(w.kend - k0);
+    const CachePages pages = rows_pages(p, w.b);
+    return __builtin_amdgcn_ballot_w64(k0 + lane < w.kend && pages.at(k0 + lane, w.kend, 0, 0) >= 0);
+}
+
 template <int N>
 struct Words {
     unsigned w[N];
@@ -470,7 +504,7 @@ __device__ __forceinline__ void rows4(const RowsParams& p) {
         const int r = w.rfirst + 16 * t + li;
         const bool real = r < w.nrows;
         const int token = real ? r / p.group : 0, h = w.hk * p.group + (real ? r % p.group : 0);
-        tok[t] = {token, token_position(p, w, token), 0, first_word(p, w, token)};
+        tok[t] = row_token(p, w, token);
         slope[t] = has_bias<MOD>(p) ? p.slopes[h] * kLog2e : 0.0f;
         const T* const from = reinterpret_cast<const T*>(p.q) + w.b * p.qs.b + h * p.qs.h + token * p.qs.s;
         typename Mma<T>::v8 x[NDC];

@@ -292,12 +292,16 @@ FarPlan plan_far(const fa_score_config& c, int D, const DkvPlan& dkv, int size, 
     const size_t nst = (c.seq_len_q + step - 1) / step;
     r.blocks = static_cast<int>((std::min<size_t>(sinks, c.seq_len_k) + dkv.tiles.rows - 1) / dkv.tiles.rows);
     const size_t reach = window_keys(c.seq_len_q, size, 0, dkv.tiles.rows, !c.causal || c.prefix) / step + 1;
-    // (of very long rows 256 chunks at most)
-    r.stages = static_cast<int>(std::max({2 * reach / 3, size_t(4), nst / 256 + 1}));
-    r.chunks = static_cast<int>((nst + r.stages - 1) / r.stages);
+    // Where sinks are many, key blocks are of like length without; and the partial sums get 64 MiB at most.
+    if (4 * static_cast<size_t>(r.blocks) > dkv.blocks) return FarPlan{};
     r.splits = static_cast<int>(c.heads / c.kv_heads);
-    r.floats = size_t(2) * (r.chunks * r.splits + 1) * c.batch * c.kv_heads * r.blocks * dkv.tiles.rows * D;
-    return r;
+    for (size_t stages = std::max(2 * reach / 3, size_t(4)); stages < nst; stages *= 2) {
+        r.stages = static_cast<int>(stages);
+        r.chunks = static_cast<int>((nst + stages - 1) / stages);
+        r.floats = size_t(2) * (r.chunks * size_t(r.splits) + 1) * c.batch * c.kv_heads * r.blocks * dkv.tiles.rows * D;
+        if (r.floats <= size_t(16) << 20) return r;
+    }
+    return FarPlan{};
 }
 
 size_t doc_tiles(size_t n) { return (n + kDocTile - 1) / kDocTile; }

@@ -58,7 +58,7 @@ __device__ __forceinline__ Walk rows_walk(const RowsParams& p, int b) {
     if (p.lens) {
         const int len = p.lens[b];
         w.total = len < 0 ? 0 : (int)min((int64_t)len + p.n, (int64_t)p.sk);
-        first = len;
+        first = min(len, kWindowMaxPos);
     } else {
         w.total = p.causal ? max(min(max(p.q_start + p.n, p.prefix ? p.prefix[b] : 0), p.sk), 0) : p.sk;
         first = p.q_start;
@@ -252,46 +252,9 @@ __device__ __forceinline__ bool rows_see(const RowsParams& p, const RowsWork& w,
     return (p.mask[row * p.mask_words + (bit >> 6)] >> (bit & 63)) & 1;
 }
 
-// A row's token: its number, position, document, and first mask word.  (RowTiles has the following as members: through
-// these its kernels take 3 % longer, 176 us instead of 171 for 8 trees of 64 tokens over up to 16384 rows.)
-struct RowToken {
-    int token, pos, doc;
-    uint64_t word;
-};
-__device__ __forceinline__ int token_position(const RowsParams& p, const RowsWork& w, int token) {
-    return !w.tree ? p.q_start + token : p.pos ? p.pos[w.b * p.n + token] : w.len + token;
-}
-__device__ __forceinline__ uint64_t first_word(const RowsParams& p, const RowsWork& w, int token) {
-    if (p.mask) return p.mask[((p.mask_shared ? 0 : (int64_t)w.b * p.n) + token) * p.mask_words];
-    return token < 63 ? (2ull << token) - 1 : ~0ull;
-}
 __device__ __forceinline__ uint64_t bits_before(int n) { return n >= 64 ? ~0ull : (1ull << max(n, 0)) - 1; }
 
-// Bits of the keys from k0 that exist: before the run's end, in good pages (one lane a key).
-__device__ __forceinline__ uint64_t keys_there(const RowsParams& p, const RowsWork& w, int k0, int lane, int badpage) {
-    const int key = k0 + lane;
-    if (!badpage) return w.kend - k0 >= 64 ? ~0ull : (1ull << (w.kend - k0)) - 1;
-    const CachePages pages = rows_pages(p, w.b);
-    return __builtin_amdgcn_ballot_w64(key < w.kend && pages.at(key, w.kend, 0, 0) >= 0);
-}
-__device__ __forceinline__ uint64_t mask_word(const RowsParams& p, const RowsWork& w, const RowToken& r, int i) {
-    if (i == 0) return r.word;
-    if (i >= p.mask_words) return 0;
-    if (p.mask) return p.mask[((p.mask_shared ? 0 : (int64_t)w.b * p.n) + r.token) * p.mask_words + i];
-    return bits_before(r.token + 1 - 64 * i);   // a chain
-}
-// Bits of the keys that a row sees, as far as causal, prefix and tree tell.
-__device__ __forceinline__ uint64_t seen_bits(const RowsParams& p, const RowsWork& w, const RowToken& r, int k0) {
-    if (!w.tree)
-        return bits_before((w.docs && r.doc < 0 ? 0 : p.causal ? max(p.q_start + r.token + 1, w.prefix) : 0x7fffffff) - k0);
-    const int rel = k0 - w.len;   // the first key's number among the drafted ones
-    if (rel <= -64) return ~0ull;
-    if (rel < 0) return (mask_word(p, w, r, 0) << -rel) | ((1ull << -rel) - 1);
-    const int i = rel >> 6, sh = rel & 63;
-    const uint64_t lo = mask_word(p, w, r, i) >> sh;
-    return sh == 0 ? lo : lo | (mask_word(p, w, r, i + 1) << (64 - sh));
-}
-// Those of the N keys that the window leaves a row; drafted keys that stand where the program says: of the keys
+// Bits of the N keys from k0 that the window leaves a row at position pos; drafted keys that stand where the program says: of the keys
 // at(b, r), b < N / 16, whose scores the lane holds.
 template <int N, typename At>
 __device__ __forceinline__ uint64_t window_bits(const RowsParams& p, const RowsWork& w, int pos, int k0, At at_) {

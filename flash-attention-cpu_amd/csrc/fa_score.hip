@@ -1048,8 +1048,8 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
     if constexpr (kWindow) {
         const int lo = kbeg - p.q_start - (p.causal && !p.prefix ? 0 : p.window - 1), hi = kend - 1 - p.q_start + p.window - 1;
         const int first = lo <= 0 ? 0 : min(nst, lo / SQ), last = hi < 0 ? 0 : min(nst, hi / SQ + 1);
-        if (chunk < 0) far = {first, last, 0, 0};
-        else far = {chunk * p.far_stages, min(nst, (chunk + 1) * p.far_stages), first, last};
+        if (chunk < 0 && (kbeg >= p.sinks || p.far_blocks)) far = {first, last, 0, 0};
+        if (chunk >= 0) far = {chunk * p.far_stages, min(nst, (chunk + 1) * p.far_stages), first, last};
     }
     auto test = [&](int st, bool* part) -> bool {
         const int q0 = st * SQ, q1 = min(q0 + SQ, p.sq);

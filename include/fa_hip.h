@@ -481,7 +481,8 @@ int fa_window_tree_attention(void* stream, const fa_tree_config* cfg, const fa_w
  * d_head a multiple of 32 (FA_ERR_UNSUPPORTED otherwise).
  *
  * Sequences, pages, lens and what is seen are as in fa_kv_cache; pages hold 8
- * rows or more, and capacity is a multiple of 8 (FA_ERR_INVALID_ARG).  Buffers are the program's, 16-byte
+ * rows or more, and capacity is a multiple of 8 (FA_ERR_INVALID_ARG); all rows of K's heads together are fewer than 2^32.
+ * Eight rows of V share words, so a page that is appended to belongs to one place of one sequence.  Buffers are the program's, 16-byte
  * aligned, contiguous, and filled by fa_cache4_append:
  *     k        [pages or batch, kv_heads, rows, d_head / 8] words, 8 columns each
  *     k_scale  [pages or batch, kv_heads, rows, d_head / 32, 2] f16: S, O

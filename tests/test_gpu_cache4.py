@@ -523,3 +523,22 @@ def test_a_layer_as_it_is_served():
                 check("out", out[x, y], o, e)
         done += n
         lens.fill_(done)
+
+
+@pytest.mark.parametrize("page", (0, 8, 32))
+def test_a_cache_without_rows(page):
+    """No capacity, or no pages at all: nothing is seen, and nothing is read or written."""
+    t, code = DT["bf16"]
+    lens = torch.tensor([3, 0], dtype=torch.int32, device="cuda")
+    table = torch.zeros(2, 4, dtype=torch.int32, device="cuda")
+    paged = {"block_table_ptr": table.data_ptr(), "page_size": page, "n_pages": 0, "pages_per_seq": 4} if page else {}
+    some = torch.full((1024,), 7.0, device="cuda")
+    buffers = [some.data_ptr()] * 4 if page else [0] * 4
+    cache = fa.kv_cache4(code, 2, 1, 64, *buffers, lens.data_ptr(), capacity=0, **paged)
+    q = torch.randn(2, 2, 3, 64, device="cuda").to(t)
+    out, lse = torch.full_like(q, 7.0), torch.full((2, 2, 3), 7.0, device="cuda")
+    k = torch.ones(2, 1, 3, 64, dtype=t, device="cuda")
+    fa.cache4_append_device(cache, fa.append_config(3), k.data_ptr(), k.data_ptr(), stream())
+    fa.cache4_attention_device(fa.tree_config(2, 3), cache, q.data_ptr(), out.data_ptr(), lse.data_ptr(), stream())
+    torch.cuda.synchronize()
+    assert (out == 0).all() and (lse == -math.inf).all() and (some == 7).all()

@@ -89,6 +89,15 @@ def test_long(dtype, heads, d, n, size, sinks):
     Window(dtype, 1, heads, heads // 2, n, n, d, size, sinks, causal=True, seed=n).run_and_check()
 
 
+@pytest.mark.parametrize("dtype", ("f32", "bf16"))
+@pytest.mark.parametrize("sinks", (60, 200, 512, 100000))
+@pytest.mark.parametrize("causal", (True, False))
+def test_many_sinks(dtype, sinks, causal):
+    """From a few blocks of keys to all of them; as many queries as keys, and fewer."""
+    Window(dtype, 1, 4, 2, 512, 512, 64, 40, sinks, causal=causal, seed=sinks).run_and_check()
+    Window(dtype, 1, 16, 2, 70, 512, 64, 40, sinks, q_start=400, causal=causal, seed=sinks).run_and_check()
+
+
 @pytest.mark.parametrize("value", (math.nan, math.inf))
 @pytest.mark.parametrize("sq,start", ((400, 0), (3, 397)))
 def test_what_lies_outside_does_not_reach_a_row(value, sq, start):
@@ -255,6 +264,21 @@ def test_pages_out_of_reach_may_be_gone():
     c.keep[3].copy_(table)
     c.run()
     c.check()
+
+
+def test_lengths_beyond_the_capacity():
+    """Tokens stand so far behind that their window reaches no row but the sinks."""
+    c = WindowTree("bf16", [300], 2, 1, 4, 64, 100, 3, spare=0, seed=11)
+    for length in (10 ** 9, 2 ** 31 - 1):
+        c.keep[0].fill_(length)
+        c.run()
+        torch.cuda.synchronize()
+        see = torch.zeros(4, 304, dtype=torch.bool)
+        see[:, :3] = True
+        for j in range(2):
+            r = attend(c.q[0, j], c.k[0][0], c.v[0][0], see, c.scale, dtype=c.t)
+            check("out", c.out[0, j], *r["out"])
+            check("lse", c.lse[0, j], *r["lse"])
 
 
 @pytest.mark.parametrize("page", (0, 16))

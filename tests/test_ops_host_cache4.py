@@ -54,6 +54,7 @@ def test_refusals():
     assert append(c=cache(batch=big), n=8) == UNSUPPORTED and read(c=cache(batch=big), n=8) == UNSUPPORTED
     assert append(c=cache(batch=1 << 20, kv_heads=1 << 20), n=8) == UNSUPPORTED
     assert attention(c=cache(batch=big, kv_heads=2)) == UNSUPPORTED
+    assert attention(c=cache(**dict(PAGES, page_size=1 << 20, pages_per_seq=1, n_pages=1 << 11))) == UNSUPPORTED   # 2^32 rows
     lib = fa.lib()
     assert lib.fa_cache4_append(None, cache(), None, PTR, PTR) == INVALID
     assert lib.fa_cache4_append(None, None, fa.append_config(1), PTR, PTR) == INVALID
