@@ -323,7 +323,8 @@ struct RowTiles {
     // Bits of the keys that exist: before the run's end, in good pages (one lane a key).
     __device__ __forceinline__ uint64_t keys_there(const RowsParams& p, const RowsWork& w, int k0, int badpage) const {
         const int lane = 16 * g + li, key = k0 + lane;
-        if (!badpage) return w.kend - k0 >= 64 ? ~0ull : (1ull << (w.kend - k0)) - 1;
+        const int n = kWindow ? max(w.kend - k0, 0) : w.kend - k0;   // (windows: a block may start past the end)
+        if (!badpage) return n >= 64 ? ~0ull : (1ull << n) - 1;
         const CachePages pages = rows_pages(p, w.b);
         return __builtin_amdgcn_ballot_w64(key < w.kend && pages.at(key, w.kend, 0, 0) >= 0);
     }
@@ -415,7 +416,7 @@ struct RowTiles {
         const CachePages pages = rows_pages(p, w.b);
         const int mine = min(16 * MT, w.nrows - rfirst);
         auto row_at = [&](int key) -> const T* {
-            if (kWindow && key >= w.gap && key - w.gap < w.skip) return nullptr;
+            if (w.out(key)) return nullptr;
             const int64_t at = pages.at(key, w.kend, p.vs.s, p.vs.b);
             return at < 0 ? nullptr : V + at;
         };

@@ -781,7 +781,7 @@ __device__ __forceinline__ void rows4(const RowsParams& p) {
     const int mine = min(16 * MT, w.nrows - w.rfirst);
 #pragma unroll 1
     for (int key = w.kbeg; key < w.kend; ++key) {
-        if (kWindow && key >= w.gap && key - w.gap < w.skip) continue;
+        if (w.out(key)) continue;
         const int page = pages.page(key);
         if (page < 0) continue;
         const int64_t at = ((int64_t)(lp.table ? page : w.b) * lp.kv_heads + w.hk) * page_rows + (lp.table ? key & pages.page_mask : key);

@@ -259,14 +259,15 @@ DkvPlan plan_dkv(const fa_score_config& c, int D, bool vec, int size, int num_cu
     return r;
 }
 
-// A window's size and sinks as kernels take them (size 0: hides nothing); farthest: the largest distance there is.
-int resolve_window(const fa_window* w, bool docs, int64_t farthest, int* size, int* sinks) {
+// A window's size and sinks as kernels take them (size 0: hides nothing); farthest: the largest distance there is; past:
+// how far beyond it kernels may reckon.
+int resolve_window(const fa_window* w, bool docs, int64_t farthest, int past, int* size, int* sinks) {
     *size = *sinks = 0;
     if (!w) return FA_OK;
     if (w->size < 1 || w->sinks < 0) return FA_ERR_INVALID_ARG;
     if (w->sinks > 0 && docs) return FA_ERR_UNSUPPORTED;   // the first keys are another document's
     if (w->size > farthest) return FA_OK;
-    if (farthest > kWindowMaxPos) return FA_ERR_UNSUPPORTED;   // positions plus or minus a window stay in 32 bits
+    if (farthest + past > kWindowMaxPos) return FA_ERR_UNSUPPORTED;   // positions plus or minus a window stay in 32 bits
     *size = static_cast<int>(w->size);
     *sinks = static_cast<int>(std::min<int64_t>(w->sinks, kWindowMaxPos));
     return FA_OK;
@@ -563,10 +564,11 @@ int launch_rotary(int dev, hipStream_t stream, int dtype, RotParams* p, bool wid
 
 namespace {
 
-// The largest distance between a query and a key, and of the rows that fill up a block.
+// The largest distance between a query and a key, and how much that of the rows that fill up a block passes it.
+constexpr int kWindowPast = 4096;
 int64_t score_farthest(const fa_score_config& c) {
     const int64_t first = c.q_start, last = first + static_cast<int64_t>(c.seq_len_q) - 1;
-    return std::max(std::abs(last), std::abs(first - (static_cast<int64_t>(c.seq_len_k) - 1))) + 4096;
+    return std::max(std::abs(last), std::abs(first - (static_cast<int64_t>(c.seq_len_k) - 1)));
 }
 
 int score_forward(void* stream_, const fa_score_config* c, const fa_window* window, const void* q, const void* k,
@@ -584,7 +586,7 @@ int score_forward(void* stream_, const fa_score_config* c, const fa_window* wind
         (rc = resolve_layout(c->out, c->batch, c->seq_len_q, c->heads, d, es, true, &lo)) != FA_OK)
         return rc;
     int size, sinks;
-    if ((rc = resolve_window(window, c->q_doc, score_farthest(*c), &size, &sinks)) != FA_OK) return rc;
+    if ((rc = resolve_window(window, c->q_doc, score_farthest(*c), kWindowPast, &size, &sinks)) != FA_OK) return rc;
     if (!q || !out || (c->seq_len_k > 0 && (!k || !v))) return FA_ERR_INVALID_ARG;
     const int D = ops_pad_d(d);
     if (c->batch * c->heads > kOpsMaxGrid || (c->seq_len_q + 31) / 32 * c->batch * c->heads > kOpsMaxGrid)
@@ -652,7 +654,7 @@ int score_backward(void* stream_, const fa_score_config* c, const fa_window* win
         (rc = resolve_layout(c->dv, c->batch, sk, c->kv_heads, d, es, true, &ldv)) != FA_OK)
         return rc;
     int size, sinks;
-    if ((rc = resolve_window(window, c->q_doc, score_farthest(*c), &size, &sinks)) != FA_OK) return rc;
+    if ((rc = resolve_window(window, c->q_doc, score_farthest(*c), kWindowPast, &size, &sinks)) != FA_OK) return rc;
     if (sq > 0 && (!q || !out || !lse || !dout)) return FA_ERR_INVALID_ARG;
     if (sk > 0 && (!k || !v)) return FA_ERR_INVALID_ARG;
     const int D = ops_pad_d(d);
@@ -734,7 +736,7 @@ int tree_attention(void* stream, const fa_tree_config* c, const fa_window* windo
         (rc = resolve_layout(c->out, cache->batch, n, c->heads, d, es, true, &lo)) != FA_OK)
         return rc;
     int size, sinks;
-    if ((rc = resolve_window(window, false, kWindowMaxPos, &size, &sinks)) != FA_OK) return rc;
+    if ((rc = resolve_window(window, false, kWindowMaxPos, 0, &size, &sinks)) != FA_OK) return rc;
     if (!q || !out) return FA_ERR_INVALID_ARG;
     if (cache->batch * c->heads > kOpsMaxGrid) return FA_ERR_UNSUPPORTED;
     RowsParams p{};
@@ -1353,7 +1355,7 @@ int fa_cache4_attention(void* stream_, const fa_tree_config* c, const fa_window*
         (rc = resolve_layout(c->out, cache->batch, n, c->heads, d, 2, true, &lo)) != FA_OK)
         return rc;
     int size, sinks;
-    if ((rc = resolve_window(window, false, kWindowMaxPos, &size, &sinks)) != FA_OK) return rc;
+    if ((rc = resolve_window(window, false, kWindowMaxPos, 0, &size, &sinks)) != FA_OK) return rc;
     if (!q || !out) return FA_ERR_INVALID_ARG;
     if (cache->batch * c->heads > kOpsMaxGrid) return FA_ERR_UNSUPPORTED;
     RowsParams p{};

@@ -34,23 +34,29 @@ struct RowsWork {
     int run, rb, b, hk;
     int runs;   // of the sequence
     int len, prefix, open, kbeg, kend, nrows, rfirst;
-    int kfirst, gap, skip;   // windows: kbeg among the keys that are walked; keys from `gap` on are left out, `skip` of them
+    // windows: kfirst and klast, the run's ends among the keys that are walked: first those from `near` on (near_keys of
+    // them), then the sinks; keys [out_lo, out_hi) lie between kbeg and kend but are not the run's
+    int kfirst, klast, near, near_keys, out_lo, out_hi;
     int low;          // a window's: keys before this and not before p.sinks are hidden from some row
     int tree, docs;
-    // how many keys are walked, and the one that stands `i` behind kbeg (a multiple of 16) among them
-    __device__ __forceinline__ int kwalk() const { return kend - kbeg - (kWindow && kbeg < gap && kend > gap ? skip : 0); }
+    // how many keys are walked, and the i-th (a multiple of 16) of them
+    __device__ __forceinline__ int kwalk() const { return kWindow ? klast - kfirst : kend - kbeg; }
     __device__ __forceinline__ int key(int i) const {
         if (!kWindow) return kbeg + i;
         const int k = kfirst + i;
-        return k + (k >= gap ? skip : 0);
+        return k < near_keys ? near + k : k - near_keys;
     }
+    __device__ __forceinline__ bool out(int k) const { return kWindow && k >= out_lo && k < out_hi; }
 };
 
-// Keys that any query of sequence b sees: those before `total`, without `skip` ones from `gap` on where a window
-// leaves them out (multiples of 64, so that blocks of keys start where they do without).
+// Keys that any query of sequence b sees: those before `total`.  In a window, those from `near` on and, after them, those
+// before `sinks`, all three but `total` multiples of 64, so that blocks of keys start where they do without.  (Sinks
+// last: their scores may be so far below the others, by a bias, that those would lose their low bits against a reference
+// that starts there.)
 struct Walk {
-    int total, gap, skip;
-    __device__ __forceinline__ int walked() const { return total - skip; }
+    int total, near, sinks;
+    __device__ __forceinline__ int near_keys() const { return (total - near + 63) & ~63; }
+    __device__ __forceinline__ int walked() const { return sinks ? near_keys() + sinks : total - near; }
 };
 __device__ __forceinline__ Walk rows_walk(const RowsParams& p, int b) {
     Walk w = {0, 0, 0};
@@ -65,9 +71,8 @@ __device__ __forceinline__ Walk rows_walk(const RowsParams& p, int b) {
     }
     if (kWindow) {
         if (!p.lens) w.total = min(w.total, max(max(first + p.n - 1 + p.window, p.sinks), 0));
-        w.gap = (p.sinks + 63) & ~63;
-        const int low = min(first - p.window + 1, w.total);
-        w.skip = max((max(low, 0) & ~63) - w.gap, 0);
+        w.near = max(min(first - p.window + 1, w.total), 0) & ~63;
+        w.sinks = min((p.sinks + 63) & ~63, w.near);
     }
     return w;
 }
@@ -198,10 +203,6 @@ __device__ __forceinline__ bool rows_work(const RowsParams& p, int rows, int lan
         w.low = last - p.window + 1;
     }
     const Walk walk = rows_walk(p, w.b);
-    if (kWindow) {
-        w.gap = __builtin_amdgcn_readfirstlane(walk.gap);
-        w.skip = __builtin_amdgcn_readfirstlane(walk.skip);
-    }
     const int total = __builtin_amdgcn_readfirstlane(walk.walked());
     int64_t per = (int64_t)__builtin_amdgcn_readfirstlane(r.steps) * p.step;
     // a sequence's runs of one length, rather than all but its last
@@ -210,8 +211,23 @@ __device__ __forceinline__ bool rows_work(const RowsParams& p, int rows, int lan
     w.kend = (int)min(w.kbeg + per, (int64_t)total);
     if (kWindow) {
         w.kfirst = w.kbeg;
-        w.kbeg = w.key(0);
-        w.kend += w.kend > w.gap ? w.skip : 0;
+        w.klast = w.kend;
+        w.near = __builtin_amdgcn_readfirstlane(walk.near);
+        const int end = __builtin_amdgcn_readfirstlane(walk.total), nk = __builtin_amdgcn_readfirstlane(walk.near_keys());
+        w.near_keys = nk;
+        w.out_lo = w.out_hi = 0;
+        if (w.kfirst < nk) {
+            w.kbeg = w.near + w.kfirst;
+            w.kend = w.near + min(w.klast, end - w.near);
+            if (w.klast > nk) {   // sinks too
+                w.out_lo = w.klast - nk;
+                w.out_hi = w.kbeg;
+                w.kbeg = 0;
+            }
+        } else {
+            w.kbeg = w.kfirst - nk;
+            w.kend = w.klast - nk;
+        }
     }
     w.nrows = p.n * p.group;
     w.rfirst = w.rb * rows;

@@ -72,17 +72,26 @@ template <typename Test>
 struct Stages {
     uint64_t vis = 0, part = 0;
     int base, count, lane;
-    int skip_from = 0, skip_to = 0;   // 64-stage runs that start in here hold no visible pair
+    // Windows: 64-stage runs that start in here hold no visible pair, and the first `last` stages (of sinks) come
+    // last: their scores may be so far below the others (a bias by distance) that those would lose their low bits
+    // against a reference that starts there.
+    int skip_from = 0, skip_to = 0, last = 0, pass = 0;
     Test test;
     __device__ __forceinline__ Stages(int n, int lane_, Test t) : base(-64), count(n), lane(lane_), test(t) {}
     // next stage (-1: none); *masked: it needs the mask (an int: uniform flags stay in one scalar register)
     __device__ __forceinline__ int next(int* masked) {
         while (vis == 0) {
             base += 64;
-            if (kWindow && base >= skip_from && base < skip_to) base = skip_to;
-            if (base >= count) return -1;
+            if (kWindow && pass == 0 && base >= skip_from && base < skip_to) base = skip_to;
+            if (base >= (kWindow && pass ? last : count)) {
+                if (!kWindow || pass || last == 0) return -1;
+                pass = 1;
+                base = -64;
+                continue;
+            }
             bool p = false, v = false;
             if (base + lane < count) v = test(base + lane, &p);
+            if (kWindow) v = v && (base + lane < last) == (pass != 0);
             vis = __builtin_amdgcn_ballot_w64(v);
             part = __builtin_amdgcn_ballot_w64(v && p);
         }
@@ -161,6 +170,7 @@ __device__ __forceinline__ bool window_meets(const ScoreParams& p, int lo, int h
 template <int ROWS, typename S>
 __device__ __forceinline__ void window_stages(S* s, int sinks, int lo, int hi, int n) {
     const int first = (sinks + ROWS - 1) / ROWS;
+    s->last = first;
     s->count = min(n, max(first, hi < 0 ? 0 : hi / ROWS + 1));
     s->skip_from = (first + 63) & ~63;
     s->skip_to = lo <= 0 ? 0 : lo / ROWS & ~63;

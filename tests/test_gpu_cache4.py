@@ -378,6 +378,16 @@ def test_windows(dtype, size, sinks, n, mask, page):
     c.check()
 
 
+@pytest.mark.parametrize("page", (0, 8))
+@pytest.mark.parametrize("length", (449, 480, 6000))
+def test_windows_with_sinks_far_below(length, page):
+    """A bias by distance leaves sinks thousands below; last and first keys anywhere in a block of 64."""
+    for size, sinks in ((100, 4), (33, 70), (5, 3)):
+        c = Attention("f16", [length], 8, 8, 3, 64, page=page, alibi=True, window=(size, sinks), seed=length)
+        c.run()
+        c.check()
+
+
 @pytest.mark.parametrize("big", (1e-30, 1e-3, 1e5, 1e30))
 def test_bf16_queries_of_any_size(big):
     """Brought into f16's range by powers of two, a row each."""

@@ -98,6 +98,37 @@ def test_many_sinks(dtype, sinks, causal):
     Window(dtype, 1, 16, 2, 70, 512, 64, 40, sinks, q_start=400, causal=causal, seed=sinks).run_and_check()
 
 
+def by_row(see, q, k, v, scale, bias, dout=None):
+    """attend of each row with the keys that it sees alone: bounds of sums over those."""
+    rows = [attend(q[i:i + 1], k[see[i]], v[see[i]], torch.ones(1, int(see[i].sum()), dtype=torch.bool), scale,
+                   bias=bias[i:i + 1, see[i]], dout=None if dout is None else dout[i:i + 1]) for i in range(q.shape[0])]
+    return {n: tuple(torch.cat([r[n][i] for r in rows]) for i in (0, 1))
+            for n in (("out", "lse") if dout is None else ("out", "lse", "dq"))}
+
+
+@pytest.mark.parametrize("sq", (4, 600))
+@pytest.mark.parametrize("sinks", (4, 70))
+def test_sinks_far_below_the_other_scores(sq, sinks):
+    """A bias by distance leaves sinks thousands below: what weighs is as exact as without them."""
+    c = Window("f32", 1, 8, 8, sq, 6000, 64, 100, sinks, q_start=6000 - sq, causal=True, alibi=True, seed=sq)
+    c.forward()
+    c.backward()
+    torch.cuda.synchronize()
+    rows = torch.arange(0, sq, 37 if sq > 4 else 1)
+    for h in range(8):
+        e = by_row(c.see[0][rows], c.q[0, h, rows], c.k[0, h], c.v[0, h], c.scale, c.bias[h][rows], c.dout[0, h, rows])
+        for n, (x, bound) in e.items():
+            check(n, (c.lse if n == "lse" else c.outs[n])[0, h, rows.cuda()], x, bound)
+    # The weights of sinks reach down to 0.  One below f32's smallest normal number, 2^-126, may count as 0, and so may its
+    # product with what it weighs: sq terms of a sum, each off by 2^-126 (1 + its factor).  Of dV that is |dO|, of dK
+    # |dP - delta| |q| scale, where |dP| and |delta| are at most |dO| times the longest row of V.
+    full, tiny = c.expect(), 2.0 ** -126
+    long_v = c.v.norm(dim=-1).max().double()
+    for n, factor in (("dv", c.dout.double().abs().amax()),
+                      ("dk", 2 * c.dout.double().norm(dim=-1).max() * long_v * c.q.double().abs().amax())):
+        check(n, c.outs[n], full[n][0], full[n][1] + sq * tiny * (1 + factor))
+
+
 @pytest.mark.parametrize("value", (math.nan, math.inf))
 @pytest.mark.parametrize("sq,start", ((400, 0), (3, 397)))
 def test_what_lies_outside_does_not_reach_a_row(value, sq, start):
@@ -264,6 +295,31 @@ def test_pages_out_of_reach_may_be_gone():
     c.keep[3].copy_(table)
     c.run()
     c.check()
+
+
+@pytest.mark.parametrize("n,h,d", ((1, 8, 64), (40, 8, 64), (3, 8, 36)))
+@pytest.mark.parametrize("sinks", (4, 70))
+def test_sinks_far_below_in_a_cache(n, h, d, sinks):
+    c = WindowTree("f32", [6000, 300, 90], h, 8, n, d, 100, sinks, alibi=True, seed=12)
+    c.run()
+    torch.cuda.synchronize()
+    for i, x in enumerate(c.lens):
+        pos = c.pos[i].double()
+        dist = (pos[:, None] - torch.cat((torch.arange(x), pos))[None, :]).abs()
+        for j in range(h):
+            for name, (value, bound) in by_row(c.seen(i), c.q[i, j], c.k[i][j], c.v[i][j], c.scale,
+                                               -c.slopes[j].double() * dist).items():
+                check(f"{name} {i} {j}", (c.lse if name == "lse" else c.out)[i, j], value, bound)
+
+
+@pytest.mark.parametrize("size", (1, 5, 30, 64, 65, 97))
+@pytest.mark.parametrize("length", (449, 480, 512, 513))
+def test_ends_of_the_window(size, length):
+    """Last keys and first ones anywhere in a block of 64, with sinks walked after them."""
+    for dtype, d, n in (("f32", 64, 20), ("bf16", 256, 20), ("bf16", 64, 3)):
+        c = WindowTree(dtype, [length], 2, 1, n, d, size, 3, seed=13)
+        c.run()
+        c.check()
 
 
 def test_lengths_beyond_the_capacity():
