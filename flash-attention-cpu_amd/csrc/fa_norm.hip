@@ -10,7 +10,11 @@
 // two), each with one unit of columns (W > 1: 16 bytes of a column run and, in the half layout, the 16 bytes half the
 // rotary columns further; W = 1: up to four pairs or copied columns), so that the sums over a row are a few
 // exchanges between lanes and pairs never leave a lane.  A workgroup takes the rows of a few tokens of one tensor;
-// their sines and cosines are formed once, a pair a thread, from angles reduced in 64 bits, and shared through LDS.
+// their sines and cosines are formed once, a pair a thread, from angles reduced in 64 bits, and shared through LDS:
+// the more tokens a workgroup has, the fewer of them there are to fill the GPU (plan_norm).
+// bf16, 8192 tokens of 32 + 8 heads of 128 columns: 31 us (5.4 TB/s; 41 between passes over different inputs); backward
+// 2 x 4096 tokens of 16 + 4 heads 31 us (4.1 TB/s, since two sums a row come before the first store) and 4.7 us for the
+// weights' sums; a token of 32 sequences into a cache 5.7 us, a launch and one chain of loads.
 
 #include "fa_ops_common.h"
 

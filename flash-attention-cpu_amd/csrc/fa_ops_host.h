@@ -1,5 +1,5 @@
 // fa_ops_host.h -- host side of attention with modified scores, rotary
-// positions and the key / value cache (included by fa_host.cpp, whose device
+// positions, norms and the key / value caches (included by fa_host.cpp, whose device
 // state and stream workspaces it uses).
 //
 // Their kernels are code objects of their own next to fa_kernels.hsaco, each loaded

@@ -1,6 +1,6 @@
 // fa_ops_params.h -- parameter blocks and geometry shared by the host code
-// (fa_ops_host.h) and the kernels of fa_score.hip, fa_cache.hip and
-// fa_rotary.hip.
+// (fa_ops_host.h) and the kernels of fa_score.hip, fa_cache.hip, fa_cache4.hip,
+// fa_rotary.hip and fa_norm.hip.
 #ifndef FA_OPS_PARAMS_H
 #define FA_OPS_PARAMS_H
 

@@ -1,6 +1,10 @@
 // fa_rows.h -- what the kernels for query rows over a cache have in common
 // (fa_cache.hip, fa_cache4.hip): pages, the runs that the keys of all sequences are cut into, and
 // what a row sees.
+//
+// In a window (OPS_WINDOW) only the keys from the first row's window on and the sinks are walked, the sinks last, as if
+// they followed the others (RowsWork::key): bf16, 16 x 32 / 8 heads, one token over 32768 rows in pages, window 4096:
+// 51 us for 269 MB (5.3 TB/s), and 5 us to join the runs.
 #ifndef FA_ROWS_H
 #define FA_ROWS_H
 

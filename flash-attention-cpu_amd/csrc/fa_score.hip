@@ -1,5 +1,6 @@
 // fa_score.hip -- gfx950 kernels of attention with modified scores
-// (fa_score_forward, fa_score_backward).
+// (fa_score_forward, fa_score_backward; with OPS_WINDOW defined those in a
+// window, fa_window_forward and fa_window_backward, as code objects of their own).
 //
 // Scores are computed transposed, so that a lane owns one row of the tile it keeps:
 // forward and dQ kernels keep query rows (S^T = K Q^T, lane: query li, keys 4g + r
@@ -11,7 +12,6 @@
 // Which walked tiles hold a visible pair is decided for 64 tiles at a time: each
 // lane tests one (causal and prefix bounds, document ranges), and two ballots give the
 // tiles to visit and those of them that need the mask element by element.
-
 //
 // Built once a type: OPS_T the element type, OPS_NAME its name in the kernels'.
 
@@ -228,6 +228,9 @@ __device__ __forceinline__ bool window_active(const ScoreParams& p, int lo, int 
 // Bound by the issue of vector instructions (five a score, ten with a cap, transcendental ones counted twice) and of
 // products, which overlap little with two waves a SIMD: bf16, 2 x 16 x 4096^2 all visible, 128 columns 281 us
 // (978 TF/s), capped 339 us (810); causal 140 us (980); 64 columns, 4 x 16 x 4096^2 causal 183 us (750).
+// In a window the walk of a workgroup is short (1024 of 8192 tokens, 128 query rows: 18 tiles of 64 keys), so that its
+// start, the masked tiles at its two ends and the one of the sinks weigh more: bf16, 32 heads of 128 columns, 8192 tokens,
+// window 1024 and 4 sinks 190 us (680 TF/s of visible pairs; matrix units busy 34 % of the time, vector units 45 %).
 template <typename T, int D, int MT, int KG, int MOD, bool VEC>
 __device__ __forceinline__ void score_forward(const ScoreParams& p) {
     using M = Mma<T>;
@@ -982,7 +985,8 @@ struct FarStages {
 // chunks to workgroups of their own (blockIdx >= p.far_first), whose sums score_dkv_sum adds, since the few long
 // blocks would end long after all others.
 // Bound as the forward kernel, with LDS read at half of its rate besides: bf16, 2 x 16 x 4096^2 all visible, 128
-// columns some 615 us (four products, 890 TF/s), dQ 515 us.
+// columns some 615 us (four products, 890 TF/s), dQ 515 us.  Window 512 and 64 sinks, 2 x 16 / 4 heads x 4096^2,
+// 128 columns: dK and dV 131 us, dQ 121 us.
 template <typename T, int D, int MT, int KG, int MOD, bool VEC>
 __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
     using M = Mma<T>;
