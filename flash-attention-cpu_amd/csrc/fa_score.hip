@@ -72,26 +72,28 @@ template <typename Test>
 struct Stages {
     uint64_t vis = 0, part = 0;
     int base, count, lane;
-    // Windows: 64-stage runs that start in here hold no visible pair, and the first `last` stages (of sinks) come
-    // last: their scores may be so far below the others (a bias by distance) that those would lose their low bits
-    // against a reference that starts there.
-    int skip_from = 0, skip_to = 0, last = 0, pass = 0;
+    // Windows: stages before `from` hold no visible pair, but for the first `sinks`, which are walked in pass `when`.
+    // Last where a bias by distance may put their scores so far below the others that those would lose their low bits
+    // against a reference that starts there; else first, since all workgroups start on the same rows then, in cache (32 / 8
+    // heads x 8192^2, window 1024, 4 sinks: 186 us, sinks last 190).
+    int from = 0, sinks = 0, when = 0, pass = 0;
     Test test;
     __device__ __forceinline__ Stages(int n, int lane_, Test t) : base(-64), count(n), lane(lane_), test(t) {}
     // next stage (-1: none); *masked: it needs the mask (an int: uniform flags stay in one scalar register)
     __device__ __forceinline__ int next(int* masked) {
         while (vis == 0) {
             base += 64;
-            if (kWindow && pass == 0 && base >= skip_from && base < skip_to) base = skip_to;
-            if (base >= (kWindow && pass ? last : count)) {
-                if (!kWindow || pass || last == 0) return -1;
+            const bool far = kWindow && sinks && pass == when;
+            if (kWindow && !far && base < from) base = from;
+            if (base >= (far ? sinks : count)) {
+                if (!kWindow || pass || sinks == 0) return -1;
                 pass = 1;
                 base = -64;
                 continue;
             }
             bool p = false, v = false;
             if (base + lane < count) v = test(base + lane, &p);
-            if (kWindow) v = v && (base + lane < last) == (pass != 0);
+            if (kWindow) v = v && (base + lane < sinks) == far;
             vis = __builtin_amdgcn_ballot_w64(v);
             part = __builtin_amdgcn_ballot_w64(v && p);
         }
@@ -168,12 +170,12 @@ __device__ __forceinline__ bool window_meets(const ScoreParams& p, int lo, int h
 // The walked stages that a window leaves: rows before `sinks` (where they are walked for their own sake) and rows
 // [lo, hi], of n stages of ROWS.
 template <int ROWS, typename S>
-__device__ __forceinline__ void window_stages(S* s, int sinks, int lo, int hi, int n) {
+__device__ __forceinline__ void window_stages(S* s, int sinks, bool last, int lo, int hi, int n) {
     const int first = (sinks + ROWS - 1) / ROWS;
-    s->last = first;
+    s->sinks = first;
+    s->when = last ? 1 : 0;
     s->count = min(n, max(first, hi < 0 ? 0 : hi / ROWS + 1));
-    s->skip_from = (first + 63) & ~63;
-    s->skip_to = lo <= 0 ? 0 : lo / ROWS & ~63;
+    s->from = lo <= 0 ? 0 : lo / ROWS;
 }
 
 // One value a lane from global memory into LDS, zero past n.
@@ -206,10 +208,10 @@ __device__ __forceinline__ bool key_stage(const ScoreParams& p, int prefix, int 
 }
 // The stages of keys that the windows of queries [q0, q1) leave.
 template <int SK, typename S>
-__device__ __forceinline__ void window_keys(const ScoreParams& p, S* s, int q0, int q1) {
+__device__ __forceinline__ void window_keys(const ScoreParams& p, S* s, bool last, int q0, int q1) {
     if (!kWindow) return;
     const int up = p.causal && !p.prefix ? 0 : p.window - 1;
-    window_stages<SK>(s, p.sinks, p.q_start + q0 - p.window + 1, p.q_start + q1 - 1 + up, s->count);
+    window_stages<SK>(s, p.sinks, last, p.q_start + q0 - p.window + 1, p.q_start + q1 - 1 + up, s->count);
 }
 // Whether rows of a wave at positions [lo, hi] see a key of [k0, k1), as far as the window tells.
 __device__ __forceinline__ bool window_active(const ScoreParams& p, int lo, int hi, int k0, int k1) {
@@ -230,7 +232,7 @@ __device__ __forceinline__ bool window_active(const ScoreParams& p, int lo, int 
 // (978 TF/s), capped 339 us (810); causal 140 us (980); 64 columns, 4 x 16 x 4096^2 causal 183 us (750).
 // In a window the walk of a workgroup is short (1024 of 8192 tokens, 128 query rows: 18 tiles of 64 keys), so that its
 // start, the masked tiles at its two ends and the one of the sinks weigh more: bf16, 32 heads of 128 columns, 8192 tokens,
-// window 1024 and 4 sinks 190 us (680 TF/s of visible pairs; matrix units busy 34 % of the time, vector units 45 %).
+// window 1024 and 4 sinks 186 us (690 TF/s of visible pairs; matrix units busy 34 % of the time, vector units 45 %).
 template <typename T, int D, int MT, int KG, int MOD, bool VEC>
 __device__ __forceinline__ void score_forward(const ScoreParams& p) {
     using M = Mma<T>;
@@ -289,7 +291,7 @@ __device__ __forceinline__ void score_forward(const ScoreParams& p) {
     }
     auto test = [&](int st, bool* part) -> bool { return key_stage<SK>(p, prefix, st, q0, q1, docs, qr, krng, part); };
     Stages<decltype(test)> stages((p.sk + SK - 1) / SK, lane, test);
-    window_keys<SK>(p, &stages, q0, q1);
+    window_keys<SK>(p, &stages, has_bias<MOD>(p), q0, q1);
     const Fill kfill(p.ks.s, p.d, wave, lane), vfill(p.vs.s, p.d, wave, lane);
     auto fill_k = [&](int st, T* dst, int* ids) {
         kfill(dst, K, st * SK, p.sk);
@@ -744,7 +746,7 @@ __device__ __forceinline__ void score_dq(const ScoreParams& p) {
     }
     auto test = [&](int st, bool* part) -> bool { return key_stage<SK>(p, prefix, st, q0, q1, docs, qr, krng, part); };
     Stages<decltype(test)> stages((p.sk + SK - 1) / SK, lane, test);
-    window_keys<SK>(p, &stages, q0, q1);
+    window_keys<SK>(p, &stages, false, q0, q1);
     const Fill kfill(p.ks.s, p.d, wave, lane), vfill(p.vs.s, p.d, wave, lane);
     auto fill = [&](int st, T* k, T* v, int* ids) {
         kfill(k, K, st * SK, p.sk);
@@ -1081,7 +1083,7 @@ __device__ __forceinline__ void score_dkv(const ScoreParams& p) {
     Stages<decltype(test)> stages(nst, lane, test);
     if constexpr (kWindow) {
         stages.count = far.last;
-        stages.skip_to = far.first & ~63;
+        stages.from = far.first;
     }
     const Fill qfill(p.qs.s, p.d, wave, lane), ofill(p.dos.s, p.d, wave, lane);
     // the next (head, stage): the stages of one head of the group after the other
