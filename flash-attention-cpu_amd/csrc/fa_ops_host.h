@@ -415,15 +415,25 @@ int run_rows(int dev, hipStream_t stream, int dtype, int D, bool vec, RowsParams
     return launch_rows(dev, stream, dtype, module, name, plan, D, vec, p);
 }
 
-// Short query blocks, and few workgroups over many keys, run on the rows kernel, which splits the keys.
-bool score_takes_rows(const fa_score_config& c, size_t keys, int num_cus) {
-    const size_t group = c.heads / c.kv_heads;
+// Short query blocks, and few workgroups over many keys, run on the rows kernel, which splits the keys.  keys: those
+// that any query of the call walks; walk: those that 32 of them do (in a window fewer).
+bool score_takes_rows(const fa_score_config& c, size_t keys, size_t walk, int num_cus) {
+    const size_t group = c.heads / c.kv_heads, cus = static_cast<size_t>(num_cus);
     if (c.seq_len_q * group <= 64) return true;
     // a workgroup of 32 rows takes some 0.6 us per 64 keys: above 2048 keys longer than the split and its merge, at
     // 256 columns above 1024 (1 head, 1900^2 causal: bf16 53 us whole, 35 split, f32 277 and 97; 2 heads of 128
     // columns, 1500^2: bf16 21 and 30, f32 72 and 78)
     const size_t blocks = c.batch * c.heads * ((c.seq_len_q + 31) / 32);
-    return keys >= (c.d_head > 128 ? 1024 : 2048) && 2 * blocks <= static_cast<size_t>(num_cus);
+    if (keys < (c.d_head > 128 ? 1024 : 2048) || 2 * blocks > cus) return false;
+    // The rows kernel takes every block of rows through all of the call's keys, shared out over all CUs, a score kernel's
+    // workgroup only its own through what the window leaves: the split has to save the time of the merge, here in keys of
+    // a walk.  It always does without a window.  With one, 128 blocks, whole and split: 1 head of 128 columns, 4096^2,
+    // window 100 bf16 12 and 44 us, f32 22 and 108; 8 heads of 128, 512 queries at the end of 8192 keys, window 1700
+    // bf16 30 and 36, f32 91 and 71, window 3000 bf16 45 and 41; 1 head of 256, 4000^2, bf16, window 1500 56 and 62,
+    // window 2000 69 and 62.
+    const bool f32 = c.dtype == FA_DTYPE_F32;
+    const size_t merge = f32 ? 256 : c.d_head > 128 ? 576 : 1280, split = keys * blocks / cus;
+    return walk >= merge + (f32 ? split : 2 * split / 3);   // (a key takes 16-bit rows kernels two thirds of that)
 }
 
 int check_score(const fa_score_config* c) {
@@ -598,8 +608,9 @@ int score_forward(void* stream_, const fa_score_config* c, const fa_window* wind
     const bool vec = vec_ok(q, lq, d) && vec_ok(k, lk, d) && vec_ok(v, lv, d) && ovec_ok(out, lo, es) &&
                      cap_ok(c->dtype, c->softcap);
 
-    const size_t keys = window_keys(c->seq_len_k, size, sinks, c->seq_len_q, !c->causal || c->prefix);
-    if (score_takes_rows(*c, keys, g_dev[dev].num_cus)) {
+    const bool both_sides = !c->causal || c->prefix;
+    const size_t keys = window_keys(c->seq_len_k, size, sinks, c->seq_len_q, both_sides);
+    if (score_takes_rows(*c, keys, window_keys(c->seq_len_k, size, sinks, 32, both_sides), g_dev[dev].num_cus)) {
         RowsParams p{};
         p.q = q, p.k = k, p.v = v, p.out = out, p.lse = lse;
         p.slopes = c->slopes, p.q_doc = c->q_doc, p.k_doc = c->k_doc, p.prefix = c->causal ? c->prefix : nullptr;

@@ -89,6 +89,21 @@ def test_long(dtype, heads, d, n, size, sinks):
     Window(dtype, 1, heads, heads // 2, n, n, d, size, sinks, causal=True, seed=n).run_and_check()
 
 
+@pytest.mark.parametrize("causal", (True, False))
+@pytest.mark.parametrize("sinks", (0, 70))
+@pytest.mark.parametrize("dtype,n,d,size", (("f32", 2100, 64, 700), ("bf16", 2100, 64, 1500), ("f16", 2100, 128, 1500),
+                                            ("f32", 1100, 256, 330), ("bf16", 1100, 256, 550)))
+def test_split_keys_of_many_rows(dtype, n, d, size, sinks, causal):
+    """Few heads, keys cut into runs that all blocks of rows walk: whole runs are hidden from some."""
+    Window(dtype, 1, 1, 1, n, n, d, size, sinks, causal=causal, seed=n + sinks).run_and_check(grads=False)
+
+
+@pytest.mark.parametrize("dtype", ("f32", "bf16"))
+@pytest.mark.parametrize("mods", ({"alibi": True, "cap": 9.0}, {"prefix": [1900]}, {"layout": "bshd", "pad": 3}))
+def test_split_keys_of_many_rows_and_other_changes(dtype, mods):
+    Window(dtype, 1, 2, 1, 900, 2600, 64, 2000, 5, q_start=1500, causal=True, seed=14, **mods).run_and_check(grads=False)
+
+
 @pytest.mark.parametrize("dtype", ("f32", "bf16"))
 @pytest.mark.parametrize("sinks", (60, 200, 512, 100000))
 @pytest.mark.parametrize("causal", (True, False))
