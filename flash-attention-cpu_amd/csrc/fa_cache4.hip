@@ -553,7 +553,8 @@ __device__ __forceinline__ void rows4(const RowsParams& p) {
         for (int j = 0; j < NDC; ++j)
 #pragma unroll
             for (int e = 0; e < 8; ++e) q[t][j][e] = _Float16(float(x[j][e]) * up);
-        c[t] = MOD != 0 ? 1.0f : p.scale_log2e * qs[t];
+        // (never 0, which would make NaN of the -inf of keys that a row does not see: scores, below 2^40, are nothing either way)
+        c[t] = MOD != 0 ? 1.0f : fmaxf(p.scale_log2e * qs[t], 0x1p-126f);
 #pragma unroll
         for (int j = 0; j < NO; ++j) o[t][j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
         m[t] = OPS_NEG_INF;

@@ -399,6 +399,17 @@ def test_bf16_queries_of_any_size(big):
     c.check()
 
 
+@pytest.mark.parametrize("dtype,big,scale", (("bf16", 1e-36, 1e-9), ("bf16", 1.0, 1e-44), ("f16", 1.0, 1e-44), ("bf16", 1e-36, 0.1)))
+@pytest.mark.parametrize("length", (0, 40, 3000))
+def test_scales_that_leave_nothing_of_the_scores(dtype, big, scale, length):
+    """Scores of 0, also in f32: the mean of the values, and waves without a key add nothing to it."""
+    c = Attention(dtype, [length], 2, 1, 4, 64, scale=scale, seed=17)
+    c.q *= big
+    c.gq.copy_(c.q)
+    c.run()
+    c.check()
+
+
 def test_queries_of_zeros_and_rows_of_different_size():
     c = Attention("bf16", [100], 2, 1, 4, 64, seed=7)
     c.q[:, :, 1] = 0
