@@ -313,7 +313,22 @@ __device__ __forceinline__ void norm_body(const NormParams& p) {
                 ss += __shfl_xor(ss, m);
                 sg += __shfl_xor(sg, m);
             }
-            const float rs = rsqrtf(__builtin_fmaf(ss, inv_d, p.eps)), mean = sg * rs * rs * inv_d;
+            const float rs = rsqrtf(__builtin_fmaf(ss, inv_d, p.eps));
+            float mean = sg * rs * rs * inv_d;
+            // Squares past f32's range: zeros, though the sum that the mean comes from may have passed it as well; NaN only
+            // where the row itself is not finite.
+            if (__builtin_amdgcn_ballot_w64(rs == 0.0f) != 0) {
+                float zero = 0.0f;
+#pragma unroll
+                for (int k = 0; k < NU; ++k)
+#pragma unroll
+                    for (int e = 0; e < W; ++e) {
+                        zero = __builtin_fmaf(a[k][e], rs, zero);
+                        if (kTwo) zero = __builtin_fmaf(bb[k][e], rs, zero);
+                    }
+                zero = row_sum(zero);
+                if (rs == 0.0f) mean = zero;
+            }
 #pragma unroll
             for (int k = 0; k < NU; ++k)
 #pragma unroll

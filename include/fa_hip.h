@@ -383,7 +383,7 @@ int fa_rotary(void* stream, const fa_rotary_config* cfg, size_t batch, size_t se
  * rotated as fa_rotary does, in one pass:
  *     y = R(position) (x r w),   r = 1 / sqrt(mean over d_head of x^2 + eps)
  * with sums in f32 and one rounding at the end (rows whose sum of squares
- * passes f32's range give zeros).  In place where pointers and strides are the same. */
+ * passes f32's range give zeros, and so are their gradients).  In place where pointers and strides are the same. */
 typedef struct fa_head_norm {
     const void *q_weight, *k_weight;   /* [d_head] of the config's dtype, device memory; NULL: ones */
     float eps;                         /* above 0 */

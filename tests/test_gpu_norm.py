@@ -169,6 +169,40 @@ def test_what_is_not_finite_stays_in_its_row():
         assert rest.all()
 
 
+@pytest.mark.parametrize("dtype", ("f32", "bf16"))
+@pytest.mark.parametrize("d,rot,interleaved", ((64, 64, False), (128, 128, True), (80, 40, False), (50, 18, True), (80, 40, True)))
+@pytest.mark.parametrize("big", (1e20, 3e38))
+def test_rows_whose_squares_pass_the_range(dtype, d, rot, interleaved, big):
+    """Zeros forward and backward, whatever the sums that enter the gradients; other rows as ever."""
+    c = Norm(dtype, 1, 3, 2, 9, d, rot, interleaved, "bshd", seed=8)
+    for x, gx in zip(c.x, c.gx):
+        x[0, 1, 3] = big
+        gx.copy_(x)
+    c.gdy[0][0, 1, 3] = c.gdy[0][0, 1, 3].abs() * 100
+    c.forward()
+    c.backward()
+    torch.cuda.synchronize()
+    for t in c.y + c.dx:
+        assert (t[0, 1, 3] == 0).all() and torch.isfinite(t).all()
+    for i in range(2):
+        c.x[i][0, 1, 3] = 0   # the row's share of the weights' gradients is 0 then too
+        (dx, edx), (dw, edw) = backward_expect(c.x[i], c.dy[i], c.w[i], c.eps, c.pos, c.f, c.gain, interleaved, c.t)
+        dx[0, 1, 3] = 0
+        check("dx", c.dx[i], dx, edx)
+        check("dw", c.dw[i], dw, edw)
+
+
+def test_infinite_rows_are_no_numbers_backward():
+    c = Norm("bf16", 1, 2, 1, 5, 64, 64, seed=9)
+    c.gx[0][0, 1, 2, 7] = math.inf
+    c.backward()
+    torch.cuda.synchronize()
+    assert torch.isnan(c.dx[0][0, 1, 2]).all()
+    keep = torch.ones(1, 2, 5, dtype=torch.bool)
+    keep[0, 1, 2] = False
+    assert torch.isfinite(c.dx[0][keep.cuda()]).all()
+
+
 @pytest.mark.parametrize("dx,dw", ((True, False), (False, True)))
 def test_single_gradients(dx, dw):
     c = Norm("bf16", 2, 4, 2, 50, 64, 64, seed=6)
