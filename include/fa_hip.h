@@ -316,10 +316,11 @@ int fa_score_backward(void* stream, const fa_score_config* cfg, const void* q, c
  * where a query besides sees only keys near it and the first ones (sinks):
  *     |i' - j| < size  or  j < sinks
  * (causal: the last `size` keys, its own among them; not causal: both sides).
- * Keys out of reach are not read.  Results of a window that hides nothing are those
- * of the plain calls, and so are those of window NULL.  Sinks and documents
+ * Keys that no query of the call reaches are not read, but for some next to those that one does.  window NULL is
+ * the plain call, and so is, in score attention, a window that hides nothing: the same bits.  Over a cache only the
+ * device knows whether one does, and results agree as those of sums in another order.  Sinks and documents
  * together are refused (FA_ERR_UNSUPPORTED): the first keys belong to the first document alone;
- * so are, with a window that hides something, distances that may pass 2^30.
+ * so are, in score attention with a window that hides something, distances that may pass 2^30 - 4096.
  *
  * Over a cache the position of filled rows is their row number, that of
  * drafted ones positions[b][t], at least lens[b] (smaller ones count as that), and

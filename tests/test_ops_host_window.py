@@ -39,6 +39,16 @@ def test_far_positions_are_refused():
 
 
 @needs_no_gpu
+def test_how_far_positions_may_be():
+    """The largest distance, here of 5 queries from q_start to key 0, is 2^30 - 4096, as the header says."""
+    last = (1 << 30) - 4096
+    assert set(calls(fa.window(3, 1), q_start=last - 4)) == {NO_DEVICE}
+    assert set(calls(fa.window(3, 1), q_start=last - 3)) == {UNSUPPORTED}
+    assert set(calls(fa.window(last + 1), q_start=last - 3)) == {UNSUPPORTED}   # the query at last + 1
+    assert set(calls(fa.window(last + 2), q_start=last - 3)) == {NO_DEVICE}     # hides nothing
+
+
+@needs_no_gpu
 @pytest.mark.parametrize("size,sinks", ((1, 0), (1, 1 << 62), (1 << 62, 1 << 62), (5, 100)))
 def test_accepted_windows_reach_the_device(size, sinks):
     assert set(calls(fa.window(size, sinks))) == {NO_DEVICE}
