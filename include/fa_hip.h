@@ -515,7 +515,8 @@ typedef struct fa_read_config {
 int fa_cache4_read(void* stream, const fa_kv_cache4* cache, const fa_read_config* cfg, const int32_t* rows, void* k_out,
                    void* v_out);
 /* fa_tree_attention over such a cache, in a sliding window if window != NULL.
- * Values enter the products as f16 (rounded once), and so do probabilities and, by powers of two a row, queries. */
+ * Values enter the products as f16 (rounded once: little beside half a step of a code unless all of a group's values lie
+ * within 1 / 68 of their size), and so do probabilities and, by powers of two a row, queries. */
 int fa_cache4_attention(void* stream, const fa_tree_config* cfg, const fa_window* window, const fa_kv_cache4* cache,
                         const void* q, void* out, float* lse);
 

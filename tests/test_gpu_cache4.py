@@ -359,6 +359,32 @@ def test_masks_and_scores(dtype, mask, mods, page):
     c.check()
 
 
+@pytest.mark.parametrize("dtype", ("bf16", "f16"))
+@pytest.mark.parametrize("page,d,n", ((0, 64, 200), (8, 64, 50), (0, 128, 130)))
+@pytest.mark.parametrize("k_off,v_off", ((5.0, 50.0), (-3.0, 1000.0), (0.0, -200.0)))
+def test_groups_far_from_zero(dtype, page, d, n, k_off, v_off):
+    """Against what codes stand for, unrounded.
+
+    Values of keys off by 2^-11 |k| move scores by at most t = scale sum |q| 2^-11 |k|, and weights by e^(2 t) - 1 of
+    themselves; these changes cancel in the sum, so that they weigh what values differ from v_off.  Values of V are off by
+    2^-11 |v|.
+    """
+    c = Attention(dtype, [0], 4, 2, n, d, page=page, seed=18)
+    g = torch.Generator().manual_seed(19)
+    k, v = ((make(g, c.t, 1, 2, n, d, 1.0).float() + x).to(c.t) for x in (k_off, v_off))
+    c.append(k, v)
+    c.run()
+    torch.cuda.synchronize()
+    k, v = (stands_for(*quantise(x[0])) for x in (k, v))
+    u = unit(torch.float16)
+    for j in range(4):
+        q, kx, vx = c.q[0, j], k[j // 2], v[j // 2]
+        out, e = attend(q, kx, vx, c.see[0], c.scale, dtype=torch.float16)["out"]
+        t = c.scale * u * torch.where(c.see[0], q.double().abs() @ kx.abs().T, 0.0).amax(1, keepdim=True)
+        e = e + torch.expm1(2 * t) * (vx - v_off).abs().amax() + 1.01 * u * vx.abs().amax()
+        check(f"out {j}", c.out[0, j], out, e + unit(c.t) * (out.abs() + e))
+
+
 @pytest.mark.parametrize("d", (64, 128, 256))
 @pytest.mark.parametrize("n,h,page", ((1, 8, 0), (3, 8, 128), (40, 8, 0), (1, 1, 16)))
 def test_long_cache(d, n, h, page):
