@@ -771,12 +771,8 @@ int tree_attention(void* stream, const fa_tree_config* c, const fa_window* windo
                     window_keys(capacity, size, sinks, n, false));
 }
 
-// Norms with rotary positions: one tensor of a launch, checked.
-struct NormCheck {
-    bool wide = true;
-    int heads = 0;   // of all tensors
-};
-int add_norm_tensor(NormParams* p, NormCheck* check, size_t batch, size_t seq, size_t d, size_t es, size_t heads,
+// Norms with rotary positions: one tensor of a launch, checked; *wide: whether 16-byte loads and stores do for all so far.
+int add_norm_tensor(NormParams* p, bool* wide, size_t batch, size_t seq, size_t d, size_t es, size_t heads,
                     const void* x, const fa_strides& xs, const void* dy, const fa_strides* dys, void* out,
                     const OpsLayout& lo, bool norm, const void* w, bool cache) {
     OpsLayout lx, ldy;
@@ -788,8 +784,7 @@ int add_norm_tensor(NormParams* p, NormCheck* check, size_t batch, size_t seq, s
     t.xs = lx.st, t.dys = ldy.st, t.outs = lo.st;
     t.heads = static_cast<int>(heads);
     t.norm = norm ? 1 : 0, t.cache = cache ? 1 : 0;
-    check->wide = check->wide && lx.aligned16 && ldy.aligned16 && lo.aligned16 && aligned16(x) && aligned16(dy) && aligned16(out);
-    check->heads += t.heads;
+    *wide = *wide && lx.aligned16 && ldy.aligned16 && lo.aligned16 && aligned16(x) && aligned16(dy) && aligned16(out);
     return FA_OK;
 }
 bool same_strides(const OpsStrides& a, const OpsStrides& b) { return a.b == b.b && a.s == b.s && a.h == b.h; }
@@ -1047,7 +1042,7 @@ int fa_norm_rotary(void* stream, const fa_rotary_config* cfg, const fa_head_norm
     if (batch > kOpsMaxSeq || seq_len > kOpsMaxSeq || batch * seq_len > kOpsMaxTokens) return FA_ERR_UNSUPPORTED;
     if (!positions) return FA_ERR_INVALID_ARG;
     NormParams p{};
-    NormCheck check;
+    bool wide = true;
     const size_t d = cfg->d_head, es = elem_size(cfg->dtype);
     for (int n = 0; n < (kl ? 2 : 1); ++n) {
         const fa_rotary_tensor* t = n ? kl : ql;
@@ -1058,7 +1053,7 @@ int fa_norm_rotary(void* stream, const fa_rotary_config* cfg, const fa_head_norm
         OpsLayout out;
         if ((rc = resolve_layout(t->out, batch, seq_len, t->heads, d, es, true, &out)) != FA_OK) return rc;
         if (!src || !dst) return FA_ERR_INVALID_ARG;
-        if ((rc = add_norm_tensor(&p, &check, batch, seq_len, d, es, t->heads, src, t->in, nullptr, nullptr, dst, out, true,
+        if ((rc = add_norm_tensor(&p, &wide, batch, seq_len, d, es, t->heads, src, t->in, nullptr, nullptr, dst, out, true,
                                   n ? norm->k_weight : norm->q_weight, false)) != FA_OK)
             return rc;
         // in place the layouts have to agree: a lane reads what it writes
@@ -1068,7 +1063,7 @@ int fa_norm_rotary(void* stream, const fa_rotary_config* cfg, const fa_head_norm
     fill_norm(*cfg, *norm, batch, seq_len, positions, &p);
     int dev;
     if ((rc = ops_begin(&dev, kNormModule)) != FA_OK) return rc;
-    return launch_norm(dev, static_cast<hipStream_t>(stream), cfg->dtype, &p, check.wide);
+    return launch_norm(dev, static_cast<hipStream_t>(stream), cfg->dtype, &p, wide);
 } catch (...) {   // no memory for the tables of modules, kernels and workspaces
     return FA_ERR_ALLOC;
 }
@@ -1085,7 +1080,7 @@ int fa_norm_rotary_backward(void* stream_, const fa_rotary_config* cfg, const fa
     const bool any = batch > 0 && seq_len > 0;
     if (any && !positions) return FA_ERR_INVALID_ARG;
     NormParams p{};
-    NormCheck check;
+    bool wide = true;
     const size_t d = cfg->d_head, es = elem_size(cfg->dtype);
     bool weights = false;
     for (int n = 0; n < (kg ? 2 : 1); ++n) {
@@ -1103,7 +1098,7 @@ int fa_norm_rotary_backward(void* stream_, const fa_rotary_config* cfg, const fa
         OpsLayout out;
         if ((rc = resolve_layout(t->dx, batch, seq_len, t->heads, d, es, true, &out)) != FA_OK) return rc;
         if (!x || !dy) return FA_ERR_INVALID_ARG;
-        if ((rc = add_norm_tensor(&p, &check, batch, seq_len, d, es, t->heads, x, t->x, dy, &t->dout, dx, out, true,
+        if ((rc = add_norm_tensor(&p, &wide, batch, seq_len, d, es, t->heads, x, t->x, dy, &t->dout, dx, out, true,
                                   n ? norm->k_weight : norm->q_weight, false)) != FA_OK)
             return rc;
         NormTensor& added = p.t[p.nt - 1];
@@ -1130,7 +1125,7 @@ int fa_norm_rotary_backward(void* stream_, const fa_rotary_config* cfg, const fa
     if (rows.nt > 0) {
         size_t grid;
         const char* kind;
-        if ((rc = plan_norm(dev, cfg->dtype, check.wide, &rows, &kind, &grid)) != FA_OK) return rc;
+        if ((rc = plan_norm(dev, cfg->dtype, wide, &rows, &kind, &grid)) != FA_OK) return rc;
         if (weights) {
             if ((rc = ws.get(dev, stream, grid * d * sizeof(float))) != FA_OK) return rc;
             float* part = static_cast<float*>(ws.ptr);
@@ -1166,16 +1161,16 @@ int fa_norm_cache_append(void* stream, const fa_kv_cache* cache, const fa_append
     if (n > kOpsMaxSeq || cache->batch * n > kOpsMaxTokens) return FA_ERR_UNSUPPORTED;
     if (!k || !v || !positions) return FA_ERR_INVALID_ARG;
     NormParams p{};
-    NormCheck check;
+    bool wide = true;
     // checked also where there is no room for a row
-    if ((rc = add_norm_tensor(&p, &check, cache->batch, n, d, es, cache->kv_heads, k, cfg->k, nullptr, nullptr, cache->k,
+    if ((rc = add_norm_tensor(&p, &wide, cache->batch, n, d, es, cache->kv_heads, k, cfg->k, nullptr, nullptr, cache->k,
                               ck, true, norm->k_weight, true)) != FA_OK ||
-        (rc = add_norm_tensor(&p, &check, cache->batch, n, d, es, cache->kv_heads, v, cfg->v, nullptr, nullptr, cache->v,
+        (rc = add_norm_tensor(&p, &wide, cache->batch, n, d, es, cache->kv_heads, v, cfg->v, nullptr, nullptr, cache->v,
                               cv, false, nullptr, true)) != FA_OK)
         return rc;
     if (capacity == 0) {
         p.nt = 0;
-        check = NormCheck();
+        wide = true;
     }
     if (cfg->q_layout && cfg->q_layout->heads > 0) {
         const fa_rotary_tensor* t = cfg->q_layout;
@@ -1183,7 +1178,7 @@ int fa_norm_cache_append(void* stream, const fa_kv_cache* cache, const fa_append
         if (t->heads > kOpsMaxSeq) return FA_ERR_UNSUPPORTED;
         if ((rc = resolve_layout(t->out, cache->batch, n, t->heads, d, es, true, &out)) != FA_OK) return rc;
         if (!q || !q_out) return FA_ERR_INVALID_ARG;
-        if ((rc = add_norm_tensor(&p, &check, cache->batch, n, d, es, t->heads, q, t->in, nullptr, nullptr, q_out, out,
+        if ((rc = add_norm_tensor(&p, &wide, cache->batch, n, d, es, t->heads, q, t->in, nullptr, nullptr, q_out, out,
                                   true, norm->q_weight, false)) != FA_OK)
             return rc;
         if (q == q_out && !same_strides(p.t[p.nt - 1].xs, out.st)) return FA_ERR_INVALID_ARG;
@@ -1198,7 +1193,7 @@ int fa_norm_cache_append(void* stream, const fa_kv_cache* cache, const fa_append
     p.pages_per_seq = static_cast<int>(cache->pages_per_seq);
     int dev;
     if ((rc = ops_begin(&dev, kNormModule)) != FA_OK) return rc;
-    return launch_norm(dev, static_cast<hipStream_t>(stream), cache->dtype, &p, check.wide);
+    return launch_norm(dev, static_cast<hipStream_t>(stream), cache->dtype, &p, wide);
 } catch (...) {   // no memory for the tables of modules, kernels and workspaces
     return FA_ERR_ALLOC;
 }
