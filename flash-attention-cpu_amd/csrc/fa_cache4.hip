@@ -55,10 +55,13 @@ __device__ __forceinline__ int small_div(int x, float inv) { return (int)(((floa
 // Append: a workgroup takes a few runs of 8 rows of one head of K or V.  A thread quantises 8 columns of a row, four
 // neighbours a group.  Keys are words then; values meet in LDS, where a thread a column makes a word of
 // 8 rows, with what is there already of rows that are not new.
-// Bound by vector instructions (a quotient by the group's inverse and one correction, which rounds it as a division
-// does: the inverse of an 11-bit number is rounded right by one step from the approximate one, since it lies no nearer than
-// 2^-36 to the middle of two f32 numbers, and from a right inverse the corrected quotient is right).  4 x 2048 rows of
-// K and V, 8 heads of 128 columns, bf16: 18 us (34 MB read, 10 MB written: 2.4 TB/s).
+// Bound by vector instructions, some 220 for 8 columns: 83 make the group's step and its inverse and the codes (24 of them
+// the eight quotients), 54 widen the columns and find the smallest and largest, 51 put words of V together, 44 and a table's
+// look-up move the pieces on their way along and find the place of the next: 12 of the 18 us below.  A quotient is the
+// group's inverse and one correction, which rounds it as a division does: the inverse of an 11-bit number is rounded
+// right by one step from the approximate one, since it lies no nearer than 2^-36 to the middle of two f32 numbers, and from
+// a right inverse the corrected quotient is right.  4 x 2048 rows of K and V, 8 heads of 128 columns, bf16: 18 us (34 MB
+// read, 10 MB written: 2.4 TB/s).
 // ---------------------------------------------------------------------------
 template <typename T>
 __device__ __forceinline__ void cache4_append(const Cache4Params& p) {
