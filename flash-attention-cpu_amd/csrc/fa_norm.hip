@@ -14,7 +14,9 @@
 // the more tokens a workgroup has, the fewer of them there are to fill the GPU (plan_norm).
 // bf16, 8192 tokens of 32 + 8 heads of 128 columns: 31 us (5.4 TB/s; 41 between passes over different inputs); backward
 // 2 x 4096 tokens of 16 + 4 heads 31 us (4.1 TB/s, since two sums a row come before the first store) and 4.7 us for the
-// weights' sums; a token of 32 sequences into a cache 5.7 us, a launch and one chain of loads.
+// weights' sums; a token of 32 sequences into a cache 5.7 us, a launch and one chain of loads.  Where runs of columns are no
+// whole 16 bytes it is bound by loads of single columns: bf16, 8192 tokens of 40 heads of 80 columns, 40 of them rotary in two
+// halves 101 us, interleaved 32.
 
 #include "fa_ops_common.h"
 
