@@ -273,11 +273,11 @@ __device__ __forceinline__ void cache4_read(const Cache4Params& p) {
 // Eight values of a word: codes to the fraction of f16 numbers in [1, 2), times S, plus O.  big(i), off(i): those of
 // pair i.  A value is rounded to f16's 11 bits (from a multiply-add in one step), as the weights of values are.  Half a
 // step of a code is 1 / 30 of its group's range, that rounding 2^-11 of the value: 136 times less or better where a
-// group's values lie around zero, but more than half a step where they lie over 68 ranges from it.  Values in f32 would take the matrix product at a sixteenth of the rate; the codes
-// themselves as an operand, with S and O applied to the sums of every group of columns, would take 8 vector instructions a
-// group of 16 keys and query tile instead of 4, and values and weights in two f16 parts each 15 to 20 % of the time (off by
-// 2.9e-4 then instead of 4.0e-4).  Rows of f16 are off by 4.0e-4 of their size then, of
-// which the rounding of the output alone is 2.1e-4; rows of bf16 by 1.7e-3, all of it the output's.
+// group's values lie around zero, but more than half a step where they lie over 68 ranges from it.  Values in f32 would
+// take the matrix product at a sixteenth of the rate; the codes themselves as an operand, with S and O applied to the sums
+// of every group of columns, would take 8 vector instructions a group of 16 keys and query tile instead of 4, and values and
+// weights in two f16 parts each 15 to 20 % of the time.  Rows of f16 are off by 4.0e-4 of their size (2.9e-4 in two parts),
+// of which the rounding of the output alone is 2.1e-4; rows of bf16 by 1.7e-3, all of it the output's.
 template <typename B, typename O>
 __device__ __forceinline__ h8 dequant(unsigned w, unsigned one, B big, O off) {
     h8 v;
