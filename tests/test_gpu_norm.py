@@ -330,6 +330,35 @@ def test_append(dtype, page, d, rot):
     check("q", qo, *forward_expect(q, w[0], 1e-6, c.pos, f, gain, False, t))
 
 
+@pytest.mark.parametrize("dtype,page,d,rot,n", (("bf16", 16, 128, 128, 700), ("f16", 0, 80, 40, 333), ("f32", 64, 128, 64, 501),
+                                                ("bf16", 0, 64, 64, 1)))
+def test_append_of_prompts(dtype, page, d, rot, n):
+    """Hundreds of tokens of sequences of unequal length, in place of a first or a later part of a prompt."""
+    c = Tree(dtype, [0, 333, -1, 15, 16], 6, 2, n, d, page=page, mask="chain", seed=20)
+    t, code = DT[dtype]
+    g = torch.Generator().manual_seed(21)
+    k, v, q = (torch.randn(5, x, n, d, generator=g).to(t) for x in (2, 2, 6))
+    w = [(1 + 0.3 * torch.randn(d, generator=g)).to(t) for _ in range(2)]
+    gk, gv, gq, gw = k.cuda(), v.cuda(), q.cuda(), [x.cuda() for x in w]
+    cfg = fa.append_config(n, rotary=fa.rotary_config(code, d, rot), q_layout=fa.rotary_tensor(6))
+    fa.cache_append_device(c.cache, cfg, gk.data_ptr(), gv.data_ptr(), c.keep[1].data_ptr(), gq.data_ptr(), gq.data_ptr(),
+                           stream(), norm=fa.head_norm(gw[0].data_ptr(), gw[1].data_ptr(), 1e-5))
+    torch.cuda.synchronize()
+    f, gain = frequencies(rot)
+    rows, values = c.gk.cpu(), c.gv.cpu()
+    for i, x in enumerate(c.lens):
+        if x < 0:
+            continue
+        p, r = c.place(i, torch.arange(x, x + n))
+        check(f"k {i}", rows[p, r].transpose(0, 1)[None],
+              *forward_expect(k[i:i + 1], w[1], 1e-5, c.pos[i:i + 1], f, gain, False, t))
+        assert torch.equal(values[p, r].transpose(0, 1), v[i])
+        if x:   # rows that were there stay
+            p, r = c.place(i, torch.arange(x))
+            assert torch.equal(rows[p, r].transpose(0, 1), c.k[i][:, :x]) and torch.equal(values[p, r].transpose(0, 1), c.v[i][:, :x])
+    check("q", gq, *forward_expect(q, w[0], 1e-5, c.pos, f, gain, False, t))
+
+
 def test_append_stops_at_the_capacity_and_skips_bad_pages():
     c = Tree("bf16", [6, 20], 2, 1, 4, 64, page=8, spare=0, seed=15)
     k = torch.ones(2, 1, 4, 64, dtype=torch.bfloat16, device="cuda")
