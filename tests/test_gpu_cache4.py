@@ -446,6 +446,40 @@ def test_queries_of_zeros_and_rows_of_different_size():
     c.check()
 
 
+def test_pages_far_into_the_pool():
+    """The last pages of a pool whose keys and values each take more than 2^33 bytes: the same bits as in a small pool."""
+    t, code = DT["bf16"]
+    hk, h, d, page, n, per = 2, 8, 128, 64, 1200, 20
+    g = torch.Generator().manual_seed(20)
+    k, v = (torch.randn(2, hk, n, d, generator=g).to(t).cuda() for _ in range(2))
+    q = torch.randn(2, h, 3, d, generator=g).to(t).cuda()
+    rows = torch.arange(n, dtype=torch.int32, device="cuda")[None].repeat(2, 1)
+    results = []
+    for pages in (2 * per, (1 << 27) // (hk * page) + 2 * per):
+        buffers = {x: torch.empty(s, dtype=torch.int32 if x in ("k", "v") else torch.float16, device="cuda")
+                   for x, s in fa.cache4_shapes(pages, hk, page, d).items()}
+        table = (torch.arange(2 * per, dtype=torch.int32).reshape(2, per) + pages - 2 * per).cuda()
+        lens = torch.zeros(2, dtype=torch.int32, device="cuda")
+        cache = fa.kv_cache4(code, 2, hk, d, *(buffers[x].data_ptr() for x in ("k", "k_scale", "v", "v_scale")),
+                             lens.data_ptr(), block_table_ptr=table.data_ptr(), page_size=page, n_pages=pages, pages_per_seq=per)
+        fa.cache4_append_device(cache, fa.append_config(n), k.data_ptr(), v.data_ptr(), stream())
+        lens.fill_(n - 3)
+        got = [torch.full_like(q, 7.0), torch.full((2, h, 3), 7.0, device="cuda"), torch.full_like(q, 7.0),
+               torch.full_like(k, 7.0), torch.full_like(v, 7.0)]
+        cfg = fa.tree_config(h, 3)
+        fa.cache4_attention_device(cfg, cache, q.data_ptr(), got[0].data_ptr(), got[1].data_ptr(), stream())
+        fa.cache4_attention_device(cfg, cache, q.data_ptr(), got[2].data_ptr(), stream=stream(), window=fa.window(300, 5))
+        fa.cache4_read_device(cache, fa.read_config(n), rows.data_ptr(), got[3].data_ptr(), got[4].data_ptr(), stream())
+        torch.cuda.synchronize()
+        results.append(got)
+        del buffers
+        torch.cuda.empty_cache()
+    code_k, big, off = quantise(k.cpu())
+    assert ((results[0][3].double().cpu() - stands_for(code_k, big, off)).abs() <= stands_for(code_k, big, off).abs()
+            * (unit(t) + 2.0 ** -23)).all()
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
 @pytest.mark.parametrize("page", (8, 32))
 def test_bad_pages_hold_no_keys(page):
     c = Attention("bf16", [200, 150], 4, 2, 4, 64, page=page, seed=8)
